@@ -35,6 +35,22 @@ class dcn_problem(ctypes.Structure):
     ]
 
 
+# the structs of include/dcn_seq.h
+class dcn_scan(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32)] + [(n, ctypes.c_int64) for n in (
+        "batch", "steps", "channels", "x_batch", "x_step", "gate_batch", "gate_step", "dy_batch", "dy_step")]
+
+
+class dcn_norm(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("weight_dtype", ctypes.c_int32)] + [(n, ctypes.c_int64) for n in (
+        "rows", "channels", "x_row", "block_row", "gate_row", "dstream_row", "dnormed_row")] + [("eps", ctypes.c_float)]
+
+
+class dcn_logits(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("temperature", ctypes.c_float)]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 # every symbol include/dcn.h declares (checked by the CPU test-suite)
@@ -53,6 +69,12 @@ LEGACY_SYMBOLS = [
     "dcn_deform2d_double_deform_conv_forward_cuda", "dcn_deform2d_double_deform_conv_backward_input_offset_cuda",
     "dcn_deform2d_double_deform_conv_backward_weight_cuda",
     "dcn_conv2d_conv_forward_cuda", "dcn_conv2d_conv_backward_input_cuda", "dcn_conv2d_conv_backward_weight_cuda",
+]
+# those of include/dcn_seq.h
+SEQUENCE_SYMBOLS = [
+    "dcn_scan_checkpoint_bytes", "dcn_scan_forward", "dcn_scan_backward", "dcn_scan_step",
+    "dcn_norm_forward", "dcn_norm_workspace_bytes", "dcn_norm_backward",
+    "dcn_scores_forward", "dcn_scores_backward", "dcn_distill_forward", "dcn_distill_backward",
 ]
 
 
@@ -95,6 +117,19 @@ def lib() -> ctypes.CDLL:
         L.dcn_layer_launch_count.argtypes = [pp, ctypes.c_int]
         L.dcn_layer_forward.argtypes = [pp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
         L.dcn_layer_backward.argtypes = [pp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ctypes.c_size_t, vp]
+        i32, i64, sc, no, lo = (ctypes.c_int32, ctypes.c_int64) + tuple(map(ctypes.POINTER, (dcn_scan, dcn_norm, dcn_logits)))
+        L.dcn_scan_checkpoint_bytes.restype = L.dcn_norm_workspace_bytes.restype = ctypes.c_size_t
+        L.dcn_scan_checkpoint_bytes.argtypes = [sc]
+        L.dcn_scan_forward.argtypes = [sc] + [vp] * 8
+        L.dcn_scan_backward.argtypes = [sc] + [vp] * 10
+        L.dcn_scan_step.argtypes = [i32, i64, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp]
+        L.dcn_norm_workspace_bytes.argtypes = [no]
+        L.dcn_norm_forward.argtypes = [no] + [vp] * 10
+        L.dcn_norm_backward.argtypes = [no] + [vp] * 16 + [ctypes.c_size_t, vp]
+        L.dcn_scores_forward.argtypes = [lo, vp, vp, i64, i32] + [vp] * 6
+        L.dcn_scores_backward.argtypes = [lo, vp, vp, i64, i32] + [vp] * 7
+        L.dcn_distill_forward.argtypes = [lo, vp, i32, vp, i32, vp, i32, vp, vp, vp]
+        L.dcn_distill_backward.argtypes = [lo, vp, i32, vp, i32, vp, i32, vp, vp, vp, vp]
         _lib = L
     return _lib
 

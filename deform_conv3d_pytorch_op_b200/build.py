@@ -14,9 +14,9 @@ import sys
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB = os.path.join(CSRC, "libdcn.so")
 BINDING = os.path.join(os.path.dirname(CSRC), "_dcn_torch.so")
-BINDING_SOURCE = os.path.join(CSRC, "dcn_torch.cpp")
-SOURCES = ["dcn_api.cu", "dcn_simt.cu", "dcn_exact.cu", "dcn_tc.cu"]
-HEADERS = ["dcn_common.cuh", "dcn_internal.h", os.path.join("..", "..", "include", "dcn.h")]
+BINDING_SOURCES = [os.path.join(CSRC, f) for f in ("dcn_torch.cpp", "seq_torch.cpp")]
+SOURCES = ["dcn_api.cu", "dcn_simt.cu", "dcn_exact.cu", "dcn_tc.cu", "seq_scan.cu", "seq_norm.cu", "seq_logits.cu"]
+HEADERS = ["dcn_common.cuh", "dcn_internal.h"] + [os.path.join("..", "..", "include", h) for h in ("dcn.h", "dcn_seq.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"] + os.environ.get("DCN_NVCC_EXTRA", "").split()
 
@@ -48,7 +48,7 @@ def _binding_command() -> list:
              "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
             + [a for p in ext.include_paths() for a in ("-isystem", p)]
             + ["-isystem", os.path.join(cuda, "include"), "-isystem", sysconfig.get_paths()["include"],
-               BINDING_SOURCE, "-o", BINDING, "-L" + CSRC, "-l:libdcn.so", "-L" + lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
+               *BINDING_SOURCES, "-o", BINDING, "-L" + CSRC, "-l:libdcn.so", "-L" + lib, "-lc10", "-lc10_cuda", "-ltorch_cpu",
                "-ltorch", "-ltorch_python", "-L" + os.path.join(cuda, "lib64"), "-lcudart", "-Wl,-rpath,$ORIGIN/csrc"])
 
 

@@ -31,40 +31,17 @@
 #include <string>
 
 #include "../../include/dcn.h"
+#include "dcn_torch.h"
+
+PyObject* dcn_host::g_error = nullptr;
 
 namespace {
 
+using namespace dcn_host;
 using at::Tensor;
 using torch::autograd::Node;
 using torch::autograd::SavedVariable;
 using torch::autograd::variable_list;
-
-PyObject* g_error = nullptr;            // the package's DcnError
-
-struct DcnFailure {
-    std::string text;
-};
-[[noreturn]] void fail(const std::string& text) { throw DcnFailure{text}; }
-
-void check(int status, const char* what) {
-    if (status != DCN_OK)
-        fail(std::string(what) + " failed: " + dcn_status_string(status) + " (status " + std::to_string(status) + ")");
-}
-
-bool env_set(const char* name) {
-    const char* e = getenv(name);
-    return e != nullptr && e[0] != '\0' && strcmp(e, "0") != 0;
-}
-
-struct Range {
-    bool on;
-    explicit Range(const char* name) : on(env_set("DCN_NVTX")) {
-        if (on) nvtxRangePushA(name);
-    }
-    ~Range() {
-        if (on) nvtxRangePop();
-    }
-};
 
 enum Kind { kDeform, kPlain, kLayer };
 
@@ -85,8 +62,6 @@ struct Problem {
     at::MemoryFormat act = at::MemoryFormat::Contiguous;
     int64_t out[3] = {1, 1, 1};          // the last ndim hold the output size
 };
-
-std::string dtype_name(const Tensor& t) { return std::string("torch.") + torch::getTHPDtype(t.scalar_type())->name; }
 
 std::string lower(std::string s) {
     for (char& c : s) c = (char)tolower((unsigned char)c);
@@ -426,24 +401,6 @@ bool transformed(const CallTensors& t) {
 }
 
 // ---- arguments ------------------------------------------------------------------------------------------------
-Tensor tensor_arg(PyObject* o, const char* name, bool optional = false) {
-    if (optional && o == Py_None) return Tensor();
-    if (!THPVariable_Check(o)) {
-        PyErr_Format(PyExc_TypeError, "%s must be a Tensor, not %s", name, Py_TYPE(o)->tp_name);
-        throw python_error();
-    }
-    return THPVariable_Unpack(o);
-}
-
-int64_t int_arg(PyObject* o) {
-    PyObject* i = PyNumber_Index(o);
-    if (i == nullptr) throw python_error();
-    const int64_t v = PyLong_AsLongLong(i);
-    Py_DECREF(i);
-    if (v == -1 && PyErr_Occurred()) throw python_error();
-    return v;
-}
-
 int small_int(int64_t v) {
     if (v < -2147483647ll || v > 2147483647ll) fail("value out of range");
     return (int)v;
@@ -472,12 +429,6 @@ void oob_arg(PyObject* o, Spec& s) {
     if (o == Py_None) return;
     s.oob = PyObject_IsTrue(o);
     if (s.oob < 0) throw python_error();
-}
-
-void count_arg(Py_ssize_t n, Py_ssize_t lo, Py_ssize_t hi) {
-    if (n >= lo && n <= hi) return;
-    PyErr_Format(PyExc_TypeError, "expected %zd to %zd arguments, got %zd", lo, hi, n);
-    throw python_error();
 }
 
 template <typename Parse>
@@ -601,7 +552,6 @@ PyObject* set_error(PyObject*, PyObject* cls) {
     Py_RETURN_NONE;
 }
 
-#define DCN_FAST(fn) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL
 PyMethodDef methods[] = {
     {"conv_offset2d", DCN_FAST(conv_offset<2>), nullptr},
     {"conv_offset3d", DCN_FAST(conv_offset<3>), nullptr},
@@ -616,4 +566,8 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_dcn_torch", nullptr, -1, methods,
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__dcn_torch(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__dcn_torch(void) {
+    PyObject* m = PyModule_Create(&module);
+    if (m != nullptr && PyModule_AddFunctions(m, dcn_host::sequence_methods) != 0) Py_CLEAR(m);
+    return m;
+}
