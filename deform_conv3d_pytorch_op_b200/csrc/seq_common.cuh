@@ -7,6 +7,8 @@
 #include <math_constants.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "../../include/dcn_seq.h"
 #include "dcn_internal.h"
 
@@ -15,11 +17,11 @@ namespace seq {
 
 // N bytes as one load or store moves them
 template <int N>
-struct Raw {
+struct alignas(N) Raw {
     uint32_t u[N / 4];
 };
 template <>
-struct Raw<2> {
+struct alignas(2) Raw<2> {
     uint16_t u;
 };
 
@@ -62,6 +64,24 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { re
 template <>
 __device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
 
+// Pairs of 16-bit elements in a word: one instruction an element in, one a pair out
+template <typename T>
+__device__ __forceinline__ float half_of(uint32_t word, int i) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        return __uint_as_float(i == 0 ? word << 16 : word & 0xffff0000u);
+    } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&word));
+        return i == 0 ? f.x : f.y;
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t word_of(float lo, float hi) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
 // W elements of type T
 template <typename T, int W>
 struct Pack {
@@ -75,8 +95,7 @@ struct Pack {
         } else if constexpr (W == 1) {
             return to_float(*reinterpret_cast<const T*>(&raw.u));
         } else {
-            const uint16_t v = (uint16_t)(raw.u[i / 2] >> (i % 2 * 16));
-            return to_float(*reinterpret_cast<const T*>(&v));
+            return half_of<T>(raw.u[i / 2], i % 2);
         }
     }
     __device__ __forceinline__ void set(const float (&f)[W]) {
@@ -88,22 +107,78 @@ struct Pack {
             raw.u = *reinterpret_cast<const uint16_t*>(&v);
         } else {
 #pragma unroll
-            for (int i = 0; i < W; i += 2) {
-                const T a = from_float<T>(f[i]), b = from_float<T>(f[i + 1]);
-                raw.u[i / 2] = (uint32_t) * reinterpret_cast<const uint16_t*>(&a) |
-                               (uint32_t) * reinterpret_cast<const uint16_t*>(&b) << 16;
-            }
+            for (int i = 0; i < W; i += 2) raw.u[i / 2] = word_of<T>(f[i], f[i + 1]);
         }
     }
 };
 
+__device__ __forceinline__ float ex2(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float rcp(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
 // s(v) = 1 / (1 + exp(-v)) and 1 - s(v), both to a few units in the last place: neither is formed as a difference.
 __device__ __forceinline__ void logistic(float v, float& s, float& rest) {
-    const float t = __expf(-fabsf(v));
-    const float r = __fdividef(1.0f, 1.0f + t), q = t * r;
-    s = v >= 0.0f ? r : q;
-    rest = v >= 0.0f ? q : r;
-    if (v != v) s = rest = v;
+    const float t = ex2(-1.4426950408889634f * fabsf(v));
+    const float r = rcp(1.0f + t), q = t * r;
+    s = v < 0.0f ? q : r;
+    rest = v < 0.0f ? r : q;
+}
+
+// W floats, one or two, as the arithmetic takes them: pairs go through the packed float32 instructions
+template <int W>
+struct Lanes;
+template <>
+struct Lanes<1> {
+    float v;
+    __device__ __forceinline__ float at(int) const { return v; }
+};
+template <>
+struct Lanes<2> {
+    uint64_t v;
+    __device__ __forceinline__ float at(int i) const { return __uint_as_float((uint32_t)(i == 0 ? v : v >> 32)); }
+};
+template <int W>
+__device__ __forceinline__ Lanes<W> lanes(const float (&f)[W]) {
+    Lanes<W> r;
+    if constexpr (W == 1) r.v = f[0];
+    else asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(f[0]), "f"(f[1]));
+    return r;
+}
+template <int W>
+__device__ __forceinline__ Lanes<W> all_lanes(float f) {
+    float a[W];
+#pragma unroll
+    for (int i = 0; i < W; ++i) a[i] = f;
+    return lanes<W>(a);
+}
+__device__ __forceinline__ Lanes<1> fma(Lanes<1> a, Lanes<1> b, Lanes<1> c) { return {fmaf(a.v, b.v, c.v)}; }
+__device__ __forceinline__ Lanes<1> operator*(Lanes<1> a, Lanes<1> b) { return {a.v * b.v}; }
+__device__ __forceinline__ Lanes<1> operator+(Lanes<1> a, Lanes<1> b) { return {a.v + b.v}; }
+__device__ __forceinline__ Lanes<2> fma(Lanes<2> a, Lanes<2> b, Lanes<2> c) {
+    Lanes<2> r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+__device__ __forceinline__ Lanes<2> operator*(Lanes<2> a, Lanes<2> b) {
+    Lanes<2> r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Lanes<2> operator+(Lanes<2> a, Lanes<2> b) {
+    Lanes<2> r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+template <int W>
+__device__ __forceinline__ Lanes<W> operator-(Lanes<W> a, Lanes<W> b) {
+    return fma(b, all_lanes<W>(-1.0f), a);
 }
 
 __device__ __forceinline__ float warp_sum(float v) {
@@ -111,6 +186,22 @@ __device__ __forceinline__ float warp_sum(float v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
+
+// Copies to shared memory that run on while the thread goes on; nothing is read and zeros are written where `in` is false
+__device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+template <int kBytes>
+__device__ __forceinline__ void copy_async(void* to, const void* from, bool in) {
+    if constexpr (kBytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(to)), "l"(from), "r"(in ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(shared_address(to)), "l"(from), "n"(kBytes),
+                     "r"(in ? kBytes : 0)
+                     : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// all of the thread's groups but the `kLast` issued last
+template <int kLast>
+__device__ __forceinline__ void copies_arrived() { asm volatile("cp.async.wait_group %0;" ::"n"(kLast) : "memory"); }
 
 inline bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 inline int elem_bytes(int dtype) { return dtype == DCN_SEQ_F32 ? 4 : 2; }

@@ -33,11 +33,6 @@ enum Kind { kScores, kScoresTop, kDistill };
 // The row's statistics for the backward pass
 enum Stat { kM, kLogS, kEntropy, kRestM = 2, kRestLogS, kRestC, kMass, kNorm };
 
-__device__ __forceinline__ float ex2(float v) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));

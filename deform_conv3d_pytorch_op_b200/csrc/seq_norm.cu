@@ -5,70 +5,124 @@
 //     ds = dstream + q (dsn - sn mean(dsn sn)) = dx;   dyn = ds c s(gate);   dblock = r (dyn - yn mean(dyn yn))
 //     dgate = dyn yn (1 - s(gate));   Z = sum over rows of ds s(gate) yn:  dscale = Z post, dpost = Z scale;   dpre = sum dnormed sn
 //
-// A row lives in the registers of a row of threads, eight elements each, so that every tensor is read or written once: the
-// bound is DRAM.  Up to 256 channels a warp has a row for itself and sums by shuffles alone; above, a CTA has one row at a time.
-// The CTAs of the backward pass walk the rows with Z and dpre in registers and leave one partial sum each; a second kernel
-// adds those in a fixed order.
+// A row lives in the registers of a row of threads, 32 bytes of each tensor a thread, so that every tensor is read or written
+// once: the bound is DRAM.  A row of up to 32 threads (512 channels of 16 bits, 256 of float32) is a warp's, whose sums are shuffles
+// alone; above, a row is that of 64, 128, ... threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of the next row are on their way to its own
+// places in shared memory meanwhile (cp.async), where rows start on 16 bytes; elements of other rows are loaded one by one when
+// they are used.  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the
+// arithmetic goes in pairs through the packed float32 instructions.  The CTAs of the backward pass keep Z and dpre in registers
+// and leave one partial sum each; a second kernel adds those in a fixed order.
 #include "seq_common.cuh"
 
 namespace dcn {
 namespace seq {
 namespace {
 
-constexpr int kPer = 8;                          // elements of a thread
-constexpr int kMostChannels = 1024 * kPer;
+constexpr int64_t kMostChannels = 8192;
 
 struct NormArgs {
     const void *x, *block, *gate, *scale, *post, *pre, *dstream, *dnormed;
     void *stream, *normed, *dx, *dblock, *dgate;
     float *stats, *partial;
     int64_t rows, x_row, block_row, gate_row, dstream_row, dnormed_row;
-    int channels, wide_weights;
+    int channels, threads, wide_weights;         // threads: of a row
     float eps, inv;
 };
 
-// kPer elements of a row, V at a time: the vectors j, j + threads, ...
+// How a row of elements T lies over threads, V at a time: the vectors j, j + threads, ... of thread j
 template <typename T, int V>
-struct Slice {
-    Pack<T, V> v[kPer / V];
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int i = 0; i < kPer / V; ++i) v[i].zero();
-    }
-    __device__ __forceinline__ float at(int e) const { return v[e / V].at(e % V); }
+struct Layout {
+    static constexpr int kPer = 32 / (int)sizeof(T), kVectors = kPer / V, kPairs = kPer / 2;
+    static __device__ __forceinline__ int element(int j, int threads, int e) { return (j + e / V * threads) * V + e % V; }
 };
 
-template <int V>
-__device__ __forceinline__ int element(int j, int threads, int i) { return (j + i * threads) * V; }
-
+// A thread's elements of a row
 template <typename T, int V>
-__device__ __forceinline__ void get(Slice<T, V>& s, const void* base, int64_t offset, int j, int threads, int channels) {
-#pragma unroll
-    for (int i = 0; i < kPer / V; ++i) {
-        const int c = element<V>(j, threads, i);
-        s.v[i].zero();
-        if (base != nullptr && c < channels) s.v[i].get(static_cast<const T*>(base) + offset + c);
+struct Slice {
+    Pack<T, V> v[Layout<T, V>::kVectors];
+    __device__ __forceinline__ float at(int e) const { return v[e / V].at(e % V); }
+    __device__ __forceinline__ Lanes<2> pair(int i) const {
+        const float f[2] = {at(2 * i), at(2 * i + 1)};
+        return lanes<2>(f);
     }
-}
+};
 
 template <typename T, int V>
-__device__ __forceinline__ void put(void* base, int64_t offset, const float (&f)[kPer], int j, int threads, int channels) {
+__device__ __forceinline__ void put(void* base, int64_t offset, const Lanes<2> (&f)[Layout<T, V>::kPairs], int j, int threads,
+                                    int channels) {
     if (base == nullptr) return;
 #pragma unroll
-    for (int i = 0; i < kPer / V; ++i) {
-        const int c = element<V>(j, threads, i);
+    for (int i = 0; i < Layout<T, V>::kVectors; ++i) {
+        const int c = Layout<T, V>::element(j, threads, i * V);
         float part[V];
 #pragma unroll
-        for (int k = 0; k < V; ++k) part[k] = f[i * V + k];
+        for (int k = 0; k < V; ++k) part[k] = f[(i * V + k) / 2].at((i * V + k) % 2);
         Pack<T, V> out;
         out.set(part);
         if (c < channels) out.put(static_cast<T*>(base) + offset + c);
     }
 }
 
+// A thread's elements of one row after the other, of kTensors tensors
+template <typename T, int V, int kTensors, bool kStaged>
+struct Rows {
+    using L = Layout<T, V>;
+    const T* base[kTensors];                     // nullptr: zeros
+    int64_t stride[kTensors];
+    int64_t rows, step;                          // rows in all, and from one of mine to the next
+    int j, threads, channels;                    // my place in the row
+    unsigned char* room;                         // mine of the first vector
+    int width;                                   // bytes from one vector of a thread to its next: of the CTA's threads
+    int stage = 0;
+    static constexpr int kBytes = kStaged ? 2 * kTensors * L::kVectors * 16 : 0;       // of a thread: two rows
+    __device__ __forceinline__ unsigned char* place(int s, int t, int i) const {
+        return room + ((s * kTensors + t) * L::kVectors + i) * width;
+    }
+    __device__ __forceinline__ void fetch(int s, int64_t row) {
+        if (row < rows) {
+#pragma unroll
+            for (int t = 0; t < kTensors; ++t) {
+                const T* from = base[t] + row * stride[t];
+#pragma unroll
+                for (int i = 0; i < L::kVectors; ++i) {
+                    const int c = L::element(j, threads, i * V);
+                    const bool in = base[t] != nullptr && c < channels;
+                    copy_async<16>(place(s, t, i), in ? from + c : base[0], in);
+                }
+            }
+        }
+        copies_issued();
+    }
+    // the row that next() gives first
+    __device__ __forceinline__ void begin(int64_t row) {
+        if constexpr (kStaged) fetch(0, row);
+    }
+    // row `row`, the next one since the last call or begin()
+    __device__ __forceinline__ void next(Slice<T, V> (&to)[kTensors], int64_t row) {
+        if constexpr (kStaged) {
+            fetch(stage ^ 1, row + step);
+            copies_arrived<1>();
+#pragma unroll
+            for (int t = 0; t < kTensors; ++t)
+#pragma unroll
+                for (int i = 0; i < L::kVectors; ++i) to[t].v[i].raw = *reinterpret_cast<const Raw<V * sizeof(T)>*>(place(stage, t, i));
+            stage ^= 1;
+        } else {
+#pragma unroll
+            for (int t = 0; t < kTensors; ++t)
+#pragma unroll
+                for (int i = 0; i < L::kVectors; ++i) {
+                    const int c = L::element(j, threads, i * V);
+                    to[t].v[i].zero();
+                    if (base[t] != nullptr && c < channels) to[t].v[i].get(base[t] + row * stride[t] + c);
+                }
+        }
+    }
+};
+
 // A weight as float32: of its own type, or of the activations'
 template <typename T>
-__device__ __forceinline__ float weight(const void* w, int c, int wide) {
+__device__ __forceinline__ float weight_at(const void* w, int c, int wide) {
     if (w == nullptr) return 1.0f;
     Pack<T, 1> v;
     if (wide) return gload(static_cast<const float*>(w) + c);
@@ -76,158 +130,240 @@ __device__ __forceinline__ float weight(const void* w, int c, int wide) {
     return v.at(0);
 }
 
+// scale post and pre of a row's threads, in shared memory: those of a thread four at a time
 template <typename T, int V>
-__device__ __forceinline__ void get_weights(float (&c)[kPer], float (&pre)[kPer], const NormArgs& p, int j, int threads) {
+struct Weights {
+    using L = Layout<T, V>;
+    static constexpr int kBytes = 2 * L::kPer * 4;          // of a thread
+    float4* at;
+    int width;
+    __device__ __forceinline__ void put(const NormArgs& p, int j, int threads) {
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const int at = element<V>(j, threads, e / V) + e % V;
-        c[e] = pre[e] = 0.0f;
-        if (at < p.channels) {
-            c[e] = weight<T>(p.scale, at, p.wide_weights) * weight<T>(p.post, at, p.wide_weights);
-            pre[e] = weight<T>(p.pre, at, p.wide_weights);
+        for (int i = 0; i < L::kPer / 4; ++i) {
+            float f[2][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const int c = L::element(j, threads, 4 * i + k);
+                const bool in = c < p.channels;
+                f[0][k] = in ? weight_at<T>(p.scale, c, p.wide_weights) * weight_at<T>(p.post, c, p.wide_weights) : 0.0f;
+                f[1][k] = in ? weight_at<T>(p.pre, c, p.wide_weights) : 0.0f;
+            }
+#pragma unroll
+            for (int w = 0; w < 2; ++w) at[(w * (L::kPer / 4) + i) * width] = make_float4(f[w][0], f[w][1], f[w][2], f[w][3]);
         }
     }
-}
+    __device__ __forceinline__ void get(int which, Lanes<2> (&f)[L::kPairs]) const {
+#pragma unroll
+        for (int i = 0; i < L::kPer / 4; ++i) {
+            const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&at[(which * (L::kPer / 4) + i) * width]);
+            f[2 * i].v = v.x;
+            f[2 * i + 1].v = v.y;
+        }
+    }
+};
+
+// The rows of threads of a CTA: 32 (kWarp) or more each
+template <bool kWarp>
+struct Team {
+    int threads, j, group, groups;
+    __device__ __forceinline__ explicit Team(int threads_) : threads(kWarp ? 32 : threads_) {
+        j = threadIdx.x % threads;
+        group = threadIdx.x / threads;
+        groups = blockDim.x / threads;
+    }
+};
 
 // Sums over the threads of a row.  They use two areas in turn, so that one barrier a sum is enough: an area is written again
 // behind the barrier of the sum in between.
 template <bool kWarp>
 struct RowSum {
     float (&room)[2][32];
-    int j, threads, side;
-    __device__ __forceinline__ float operator()(float v) {
-        v = warp_sum(v);
+    const Team<kWarp>& me;
+    int side;
+    __device__ __forceinline__ float operator()(Lanes<2> pair) {
+        float v = warp_sum(pair.at(0) + pair.at(1));
         if constexpr (!kWarp) {
-            float* at = room[side];
+            const int warps = me.threads / 32;
+            float* at = room[side] + me.group * warps;
             side ^= 1;
-            if (j % 32 == 0) at[j / 32] = v;
-            __syncthreads();
-            v = warp_sum(j % 32 < threads / 32 ? at[j % 32] : 0.0f);
+            if (me.j % 32 == 0) at[me.j / 32] = v;
+            asm volatile("bar.sync %0, %1;" ::"r"(me.group + 1), "r"(me.threads) : "memory");
+            v = 0.0f;
+            for (int w = 0; w < warps; w += 2) v += at[w] + at[w + 1];
         }
         return v;
     }
 };
 
-template <typename T, int V, bool kWarp, int kMost>
-__global__ void __launch_bounds__(kMost) norm_forward_kernel(const NormArgs p) {
-    __shared__ float room[2][32];
-    const int threads = kWarp ? 32 : blockDim.x, j = kWarp ? threadIdx.x % 32 : threadIdx.x;
-    const int groups = kWarp ? blockDim.x / 32 : 1, group = kWarp ? threadIdx.x / 32 : 0;
-    RowSum<kWarp> row_sum{room, j, threads, 0};
-    pdl_wait();
-    float c[kPer], pre[kPer];
-    get_weights<T, V>(c, pre, p, j, threads);
-    for (int64_t row = (int64_t)blockIdx.x * groups + group; row < p.rows; row += (int64_t)gridDim.x * groups) {
-        Slice<T, V> x, y, g;
-        get(x, p.x, row * p.x_row, j, threads, p.channels);
-        get(y, p.block, row * p.block_row, j, threads, p.channels);
-        get(g, p.gate, row * p.gate_row, j, threads, p.channels);
-        float s[kPer], sum = 0.0f, r = 0.0f;
-        if (p.block != nullptr) {
+template <typename T, int V>
+__device__ __forceinline__ void gates_of(const Slice<T, V>& g, bool has, Lanes<2> (&on)[Layout<T, V>::kPairs]) {
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) sum = fmaf(y.at(e), y.at(e), sum);
-            r = rsqrtf(row_sum(sum) * p.inv + p.eps);
+    for (int i = 0; i < Layout<T, V>::kPairs; ++i) {
+        float s[2] = {1.0f, 1.0f}, rest;
+        if (has) {
+            logistic(g.at(2 * i), s[0], rest);
+            logistic(g.at(2 * i + 1), s[1], rest);
         }
-        sum = 0.0f;
+        on[i] = lanes<2>(s);
+    }
+}
+
+template <typename T, int V, bool kWarp, int kMost, bool kStaged>
+__global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kernel(const NormArgs p) {
+    using L = Layout<T, V>;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ float room[2][32];
+    const Team<kWarp> me(p.threads);
+    RowSum<kWarp> row_sum{room, me, 0};
+    pdl_wait();
+    Weights<T, V> weights{reinterpret_cast<float4*>(dynamic) + me.j, me.threads};
+    const int64_t first = (int64_t)blockIdx.x * me.groups + me.group, step = (int64_t)gridDim.x * me.groups;
+    Rows<T, V, 3, kStaged> rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate)},
+                                {p.x_row, p.block_row, p.gate_row}, p.rows, step, me.j, me.threads, p.channels,
+                                dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * 16, (int)blockDim.x * 16};
+    rows.begin(first);
+    if (me.group == 0) weights.put(p, me.j, me.threads);
+    __syncthreads();
+    for (int64_t row = first; row < p.rows; row += step) {
+        Slice<T, V> in[3];
+        rows.next(in, row);
+        const Slice<T, V>&x = in[0], &y = in[1], &g = in[2];
+        Lanes<2> s[L::kPairs], w[L::kPairs], sum = all_lanes<2>(0.0f);
+        float r = 0.0f;
+        if (p.block != nullptr) {
+            gates_of<T, V>(g, p.gate != nullptr, s);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            float on = 1.0f, off;
-            if (p.gate != nullptr) logistic(g.at(e), on, off);
-            s[e] = x.at(e);
-            if (p.block != nullptr) s[e] = fmaf(c[e] * on, y.at(e) * r, s[e]);
-            sum = fmaf(s[e], s[e], sum);
+            for (int i = 0; i < L::kPairs; ++i) sum = fma(y.pair(i), y.pair(i), sum);
+            r = rsqrtf(row_sum(sum) * p.inv + p.eps);
+            weights.get(0, w);
+            sum = all_lanes<2>(0.0f);
+#pragma unroll
+            for (int i = 0; i < L::kPairs; ++i) {
+                s[i] = fma(w[i] * s[i], y.pair(i) * all_lanes<2>(r), x.pair(i));
+                sum = fma(s[i], s[i], sum);
+            }
+            put<T, V>(p.stream, row * p.channels, s, me.j, me.threads, p.channels);
+        } else {
+#pragma unroll
+            for (int i = 0; i < L::kPairs; ++i) {
+                s[i] = x.pair(i);
+                sum = fma(s[i], s[i], sum);
+            }
         }
         const float q = rsqrtf(row_sum(sum) * p.inv + p.eps);
-        put<T, V>(p.stream, row * p.channels, s, j, threads, p.channels);
+        weights.get(1, w);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) s[e] = s[e] * q * pre[e];
-        put<T, V>(p.normed, row * p.channels, s, j, threads, p.channels);
-        if (p.stats != nullptr && j == 0) {
+        for (int i = 0; i < L::kPairs; ++i) s[i] = s[i] * all_lanes<2>(q) * w[i];
+        put<T, V>(p.normed, row * p.channels, s, me.j, me.threads, p.channels);
+        if (p.stats != nullptr && me.j == 0) {
             p.stats[2 * row] = r;
             p.stats[2 * row + 1] = q;
         }
     }
+    if constexpr (kStaged) copies_arrived<0>();
 }
 
-template <typename T, int V, bool kWarp, int kMost>
+template <typename T, int V, bool kWarp, int kMost, bool kStaged>
 __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_kernel(const NormArgs p) {
+    using L = Layout<T, V>;
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float room[2][32];
-    const int threads = kWarp ? 32 : blockDim.x, j = kWarp ? threadIdx.x % 32 : threadIdx.x;
-    const int groups = kWarp ? blockDim.x / 32 : 1, group = kWarp ? threadIdx.x / 32 : 0;
-    RowSum<kWarp> row_sum{room, j, threads, 0};
+    const Team<kWarp> me(p.threads);
+    RowSum<kWarp> row_sum{room, me, 0};
     pdl_wait();
-    float c[kPer], pre[kPer], z[kPer], w[kPer];
-    get_weights<T, V>(c, pre, p, j, threads);
+    Weights<T, V> weights{reinterpret_cast<float4*>(dynamic) + me.j, me.threads};
+    const int64_t first = (int64_t)blockIdx.x * me.groups + me.group, step = (int64_t)gridDim.x * me.groups;
+    Rows<T, V, 5, kStaged> rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate),
+                                 static_cast<const T*>(p.dstream), static_cast<const T*>(p.dnormed)},
+                                {p.x_row, p.block_row, p.gate_row, p.dstream_row, p.dnormed_row}, p.rows, step, me.j, me.threads,
+                                p.channels, dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * 16, (int)blockDim.x * 16};
+    rows.begin(first);
+    if (me.group == 0) weights.put(p, me.j, me.threads);
+    __syncthreads();
+    Lanes<2> z[L::kPairs], dpre[L::kPairs];
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) z[e] = w[e] = 0.0f;
-    for (int64_t row = (int64_t)blockIdx.x * groups + group; row < p.rows; row += (int64_t)gridDim.x * groups) {
-        Slice<T, V> x, y, g, ds, dn;
-        get(x, p.x, row * p.x_row, j, threads, p.channels);
-        get(y, p.block, row * p.block_row, j, threads, p.channels);
-        get(g, p.gate, row * p.gate_row, j, threads, p.channels);
-        get(ds, p.dstream, row * p.dstream_row, j, threads, p.channels);
-        get(dn, p.dnormed, row * p.dnormed_row, j, threads, p.channels);
-        const float r = p.block != nullptr ? gload(p.stats + 2 * row) : 0.0f, q = gload(p.stats + 2 * row + 1);
-        float on[kPer], sn[kPer], d[kPer], sum = 0.0f;
+    for (int i = 0; i < L::kPairs; ++i) z[i] = dpre[i] = all_lanes<2>(0.0f);
+    float next_r = 0.0f, next_q = 0.0f;
+    auto fetch_stats = [&](int64_t row) {
+        if (row >= p.rows) return;
+        next_r = gload(p.stats + 2 * row);
+        next_q = gload(p.stats + 2 * row + 1);
+    };
+    fetch_stats(first);
+    for (int64_t row = first; row < p.rows; row += step) {
+        const float r = next_r, q = next_q;
+        fetch_stats(row + step);
+        Slice<T, V> in[5];
+        rows.next(in, row);
+        const Slice<T, V>&x = in[0], &y = in[1], &g = in[2], &ds = in[3], &dn = in[4];
+        const Lanes<2> rr = all_lanes<2>(r), qq = all_lanes<2>(q);
+        Lanes<2> on[L::kPairs], sn[L::kPairs], d[L::kPairs], w[L::kPairs], sum = all_lanes<2>(0.0f);
+        gates_of<T, V>(g, p.gate != nullptr, on);
+        if (p.block != nullptr) {
+            weights.get(0, w);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            float off;
-            on[e] = 1.0f;
-            if (p.gate != nullptr) logistic(g.at(e), on[e], off);
-            sn[e] = (p.block != nullptr ? fmaf(c[e] * on[e], y.at(e) * r, x.at(e)) : x.at(e)) * q;
-            w[e] = fmaf(dn.at(e), sn[e], w[e]);
-            sum = fmaf(dn.at(e) * pre[e], sn[e], sum);
+            for (int i = 0; i < L::kPairs; ++i) sn[i] = fma(w[i] * on[i], y.pair(i) * rr, x.pair(i)) * qq;
+        } else {
+#pragma unroll
+            for (int i = 0; i < L::kPairs; ++i) sn[i] = x.pair(i) * qq;
         }
-        const float m = row_sum(sum) * p.inv;
-        sum = 0.0f;
+        weights.get(1, w);
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            d[e] = fmaf(q, fmaf(-sn[e], m, dn.at(e) * pre[e]), ds.at(e));
-            const float yn = y.at(e) * r;
-            z[e] = fmaf(d[e] * on[e], yn, z[e]);
-            sum = fmaf(d[e] * c[e] * on[e], yn, sum);
+        for (int i = 0; i < L::kPairs; ++i) {
+            dpre[i] = fma(dn.pair(i), sn[i], dpre[i]);
+            d[i] = dn.pair(i) * w[i];
+            sum = fma(d[i], sn[i], sum);
         }
-        put<T, V>(p.dx, row * p.channels, d, j, threads, p.channels);
-        if (p.dblock != nullptr || p.dgate != nullptr) {
-            const float n = row_sum(sum) * p.inv;
-            float out[kPer];
+        const Lanes<2> m = all_lanes<2>(-row_sum(sum) * p.inv);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) out[e] = r * fmaf(-y.at(e) * r, n, d[e] * c[e] * on[e]);
-            put<T, V>(p.dblock, row * p.channels, out, j, threads, p.channels);
-            if (p.dgate != nullptr) {
+        for (int i = 0; i < L::kPairs; ++i) d[i] = fma(qq, fma(sn[i], m, d[i]), ds.pair(i));
+        put<T, V>(p.dx, row * p.channels, d, me.j, me.threads, p.channels);
+        if (p.block == nullptr) continue;
+        weights.get(0, w);
+        sum = all_lanes<2>(0.0f);
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    float s, off;
-                    logistic(g.at(e), s, off);
-                    out[e] = d[e] * c[e] * on[e] * (y.at(e) * r) * off;
-                }
-                put<T, V>(p.dgate, row * p.channels, out, j, threads, p.channels);
+        for (int i = 0; i < L::kPairs; ++i) {
+            const Lanes<2> yn = y.pair(i) * rr, u = d[i] * on[i];
+            z[i] = fma(u, yn, z[i]);
+            sn[i] = u * w[i];                    // the gradient of yn from here on
+            sum = fma(sn[i], yn, sum);
+        }
+        const Lanes<2> n = all_lanes<2>(-row_sum(sum) * p.inv);
+#pragma unroll
+        for (int i = 0; i < L::kPairs; ++i) d[i] = rr * fma(y.pair(i) * rr, n, sn[i]);
+        put<T, V>(p.dblock, row * p.channels, d, me.j, me.threads, p.channels);
+        if (p.dgate != nullptr) {
+#pragma unroll
+            for (int i = 0; i < L::kPairs; ++i) {
+                float off[2], s;
+                logistic(g.at(2 * i), s, off[0]);
+                logistic(g.at(2 * i + 1), s, off[1]);
+                d[i] = sn[i] * (y.pair(i) * rr) * lanes<2>(off);
             }
+            put<T, V>(p.dgate, row * p.channels, d, me.j, me.threads, p.channels);
         }
     }
+    if constexpr (kStaged) copies_arrived<0>();
     if (p.partial == nullptr) return;
-    if constexpr (kWarp) {                       // the warps of a CTA add theirs up, in order
-        __shared__ float all[2][32 * kPer];
-        for (int k = 0; k < groups; ++k) {
-            if (k == group) {
+    // the rows of threads add theirs up, in order (over the weights)
+    Lanes<2>* all = reinterpret_cast<Lanes<2>*>(dynamic) + me.j;
+    for (int k = 0; k < me.groups; ++k) {
+        __syncthreads();
+        if (k == me.group)
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) {
-                    const int at = element<V>(j, threads, e / V) + e % V;
-                    all[0][at] = z[e] = k == 0 ? z[e] : all[0][at] + z[e];
-                    all[1][at] = w[e] = k == 0 ? w[e] : all[1][at] + w[e];
-                }
+            for (int i = 0; i < L::kPairs; ++i) {
+                if (k > 0) z[i] = all[2 * i * me.threads] + z[i], dpre[i] = all[(2 * i + 1) * me.threads] + dpre[i];
+                all[2 * i * me.threads] = z[i], all[(2 * i + 1) * me.threads] = dpre[i];
             }
-            __syncthreads();
-        }
-        if (group != groups - 1) return;
     }
+    if (me.group != me.groups - 1) return;
     float* out = p.partial + (int64_t)blockIdx.x * 2 * p.channels;
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) {
-        const int at = element<V>(j, threads, e / V) + e % V;
+    for (int e = 0; e < L::kPer; ++e) {
+        const int at = L::element(me.j, me.threads, e);
         if (at < p.channels) {
-            out[at] = z[e];
-            out[p.channels + at] = w[e];
+            out[at] = z[e / 2].at(e % 2);
+            out[p.channels + at] = dpre[e / 2].at(e % 2);
         }
     }
 }
@@ -253,55 +389,68 @@ __global__ void __launch_bounds__(1024) norm_weights_kernel(const float* partial
         else static_cast<T*>(out)[at] = from_float<T>(v);
     };
     if (which == 0) {
-        put_weight(dscale, sum * weight<T>(post, at, wide));
-        put_weight(dpost, sum * weight<T>(scale, at, wide));
+        put_weight(dscale, sum * weight_at<T>(post, at, wide));
+        put_weight(dpost, sum * weight_at<T>(scale, at, wide));
     } else {
         put_weight(dpre, sum);
     }
 }
 
-int threads_of(int64_t channels) {
+// Threads of a row, a power of two; 32: a warp's
+int threads_of(int64_t channels, int elem) {
     int t = 32;
-    while ((int64_t)t * kPer < channels) t *= 2;
+    while ((int64_t)t * (32 / elem) < channels) t *= 2;
     return t;
 }
 
-constexpr int kWarpGroups = 4;                   // rows of a CTA whose warps have one each
+// Threads of a CTA: 256, in rows of t, or one row of more
+int cta_of(int t) { return t > 256 ? t : 256; }
 
-// CTAs: enough threads on every SM to have its share of memory traffic in flight, and no more than there are rows
-unsigned grid_of(int64_t rows, int64_t channels, int threads_an_sm) {
-    const int t = threads_of(channels), cta = t == 32 ? 32 * kWarpGroups : t;
-    const int64_t units = t == 32 ? (rows + kWarpGroups - 1) / kWarpGroups : rows;
+// CTAs: as many as the SMs hold at once (so many threads, by registers and shared memory), and no more than there are rows for.
+constexpr int kForwardThreads = 768, kBackwardThreads = 512;
+
+unsigned grid_of(int64_t rows, int64_t channels, int elem, int threads_an_sm) {
+    const int t = threads_of(channels, elem), cta = cta_of(t);
+    const int64_t units = (rows + cta / t - 1) / (cta / t);
     const int64_t most = (int64_t)sm_count() * (threads_an_sm > cta ? threads_an_sm / cta : 1);
     return (unsigned)(units < most ? units : most);
 }
 
-constexpr int kForwardThreads = 1024, kBackwardThreads = 768;
+template <typename K>
+int launch(K kernel, unsigned grid, int cta, size_t smem, const NormArgs& a, cudaStream_t st) {
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return DCN_ERR_CUDA;
+    return launch_dependent(kernel, dim3(grid), dim3(cta), smem, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
+}
 
-template <typename T, int V>
-int run_forward(const NormArgs& a, cudaStream_t st) {
-    const int t = threads_of(a.channels);
-    const dim3 grid(grid_of(a.rows, a.channels, kForwardThreads)), block(t == 32 ? 32 * kWarpGroups : t);
-    const auto kernel = t == 32    ? norm_forward_kernel<T, V, true, 256>
-                        : t <= 256 ? norm_forward_kernel<T, V, false, 256>
-                                   : norm_forward_kernel<T, V, false, 1024>;
-    return launch_dependent(kernel, grid, block, 0, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
+template <typename T, int V, bool kWarp, int kMost>
+int run_as(const NormArgs& a, bool backward, cudaStream_t st) {
+    // two rows of every tensor in shared memory where vectors are read, and an SM has room for as many threads
+    constexpr int kSM = 227 * 1024, kWeights = Weights<T, V>::kBytes;
+    constexpr bool f = V > 1 && kMost * (Rows<T, V, 3, true>::kBytes + kWeights) <= kSM,
+                   b = V > 1 && kMost * (Rows<T, V, 5, true>::kBytes + kWeights) <= kSM;
+    const int cta = cta_of(a.threads);
+    if (backward)
+        return launch(norm_backward_kernel<T, V, kWarp, kMost, b>, grid_of(a.rows, a.channels, sizeof(T), kBackwardThreads), cta,
+                      (size_t)cta * Rows<T, V, 5, b>::kBytes + a.threads * kWeights, a, st);
+    return launch(norm_forward_kernel<T, V, kWarp, kMost, f>, grid_of(a.rows, a.channels, sizeof(T), kForwardThreads), cta,
+                  (size_t)cta * Rows<T, V, 3, f>::kBytes + a.threads * kWeights, a, st);
 }
 
 template <typename T, int V>
-int run_backward(const NormArgs& a, cudaStream_t st) {
-    const int t = threads_of(a.channels);
-    const dim3 grid(grid_of(a.rows, a.channels, kBackwardThreads)), block(t == 32 ? 32 * kWarpGroups : t);
-    const auto kernel = t == 32    ? norm_backward_kernel<T, V, true, 256>
-                        : t <= 256 ? norm_backward_kernel<T, V, false, 256>
-                                   : norm_backward_kernel<T, V, false, 1024>;
-    return launch_dependent(kernel, grid, block, 0, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
+int run(NormArgs a, bool backward, cudaStream_t st) {
+    a.threads = threads_of(a.channels, sizeof(T));
+    if (a.threads == 32) return run_as<T, V, true, 256>(a, backward, st);
+    if (a.threads <= 256) return run_as<T, V, false, 256>(a, backward, st);
+    if constexpr (sizeof(T) == 4)
+        if (a.threads > 512) return run_as<T, V, false, 1024>(a, backward, st);
+    return run_as<T, V, false, 512>(a, backward, st);
 }
 
 template <typename T>
-int run_weights(const NormArgs& a, void* dscale, void* dpost, void* dpre, cudaStream_t st) {
+int run_weights(const NormArgs& a, int elem, void* dscale, void* dpost, void* dpre, cudaStream_t st) {
     const dim3 grid((a.channels + 31) / 32, 2), block(32, 32);
-    const int n = (int)grid_of(a.rows, a.channels, kBackwardThreads);
+    const int n = (int)grid_of(a.rows, a.channels, elem, kBackwardThreads);
     return launch_dependent(norm_weights_kernel<T>, grid, block, 0, st, a.partial, n, a.channels, a.scale, a.post, dscale, dpost,
                             dpre, a.wide_weights) != cudaSuccess
                ? DCN_ERR_CUDA
@@ -326,6 +475,12 @@ NormArgs args_of(const dcn_norm* p) {
     a.eps = p->eps;
     a.inv = 1.0f / (float)p->channels;
     return a;
+}
+
+int run_any(int dtype, bool vec, const NormArgs& a, bool backward, cudaStream_t st) {
+    if (dtype == DCN_SEQ_F32) return vec ? run<float, 4>(a, backward, st) : run<float, 1>(a, backward, st);
+    if (dtype == DCN_SEQ_BF16) return vec ? run<__nv_bfloat16, 8>(a, backward, st) : run<__nv_bfloat16, 1>(a, backward, st);
+    return vec ? run<__half, 8>(a, backward, st) : run<__half, 1>(a, backward, st);
 }
 
 // 16-byte vectors where every row of `v` starts on one
@@ -355,14 +510,12 @@ extern "C" int dcn_norm_forward(const dcn_norm* p, const void* x, const void* bl
     const bool vec = p->channels % per == 0 && wide(x, p->x_row, per) && wide(block, p->block_row, per) &&
                      wide(a.gate, p->gate_row, per) && wide(stream_out, 0, per) && wide(normed, 0, per);
     const cudaStream_t st = (cudaStream_t)stream;
-    if (p->dtype == DCN_SEQ_F32) return vec ? run_forward<float, 4>(a, st) : run_forward<float, 1>(a, st);
-    if (p->dtype == DCN_SEQ_BF16) return vec ? run_forward<__nv_bfloat16, 8>(a, st) : run_forward<__nv_bfloat16, 1>(a, st);
-    return vec ? run_forward<__half, 8>(a, st) : run_forward<__half, 1>(a, st);
+    return run_any(p->dtype, vec, a, false, st);
 }
 
 extern "C" size_t dcn_norm_workspace_bytes(const dcn_norm* p) {
     if (check_norm(p) != DCN_OK) return 0;
-    return (size_t)grid_of(p->rows, p->channels, kBackwardThreads) * 2 * p->channels * sizeof(float);
+    return (size_t)grid_of(p->rows, p->channels, elem_bytes(p->dtype), kBackwardThreads) * 2 * p->channels * sizeof(float);
 }
 
 extern "C" int dcn_norm_backward(const dcn_norm* p, const void* x, const void* block, const void* gate, const void* scale,
@@ -397,12 +550,9 @@ extern "C" int dcn_norm_backward(const dcn_norm* p, const void* x, const void* b
     const bool vec = p->channels % per == 0 && wide(x, p->x_row, per) && wide(block, p->block_row, per) &&
                      wide(a.gate, p->gate_row, per) && wide(dstream, p->dstream_row, per) &&
                      wide(dnormed, p->dnormed_row, per) && wide(dx, 0, per) && wide(dblock, 0, per) && wide(dgate, 0, per);
-    int rc;
-    if (p->dtype == DCN_SEQ_F32) rc = vec ? run_backward<float, 4>(a, st) : run_backward<float, 1>(a, st);
-    else if (p->dtype == DCN_SEQ_BF16) rc = vec ? run_backward<__nv_bfloat16, 8>(a, st) : run_backward<__nv_bfloat16, 1>(a, st);
-    else rc = vec ? run_backward<__half, 8>(a, st) : run_backward<__half, 1>(a, st);
+    const int rc = run_any(p->dtype, vec, a, true, st);
     if (rc != DCN_OK || !weights) return rc;
-    if (p->dtype == DCN_SEQ_F32) return run_weights<float>(a, dscale, dpost, dpre, st);
-    if (p->dtype == DCN_SEQ_BF16) return run_weights<__nv_bfloat16>(a, dscale, dpost, dpre, st);
-    return run_weights<__half>(a, dscale, dpost, dpre, st);
+    if (p->dtype == DCN_SEQ_F32) return run_weights<float>(a, e, dscale, dpost, dpre, st);
+    if (p->dtype == DCN_SEQ_BF16) return run_weights<__nv_bfloat16>(a, e, dscale, dpost, dpre, st);
+    return run_weights<__half>(a, e, dscale, dpost, dpre, st);
 }

@@ -4,15 +4,18 @@
 //     p_t = a_t p_{t+1} + a_t dy_t   (p behind the last step: dlast),   D_t = dy_t + p_{t+1}
 //     dx_t = D_t (1 - a_t),   dgate_t = D_t (h_{t-1} - x_t) a_t (1 - a_t),   dstate = p_0.
 //
-// A gate near one is the common case, and 1 - a is what matters of it: a state that lasts 10^4 steps would lose all of its
-// digits to the rounding of a.  So a step is known by q = min(a, 1 - a) and which of the two it is, as one signed float s (-q for
-// a = 1 - q, q for a = q), and every product with a is a sum with the product with q: a u = fma(s, u, s < 0 ? u : 0).
+// Both directions are scans of affine maps h -> A h + B, whose composition is (A2 A1, A2 B1 + B2).  A lane has a pair of channels,
+// in the packed float32 instructions, and kSteps steps of them: it composes its steps, the warps of a CTA (one behind the other
+// in time) compose theirs through shared memory and the CTAs of a cluster theirs through distributed shared memory; the state
+// that reaches a lane then gives all of its steps.  So x and gate are read once and y is written once, whatever the length: the
+// bound is DRAM.  A cluster walks the time axis in waves of (its CTAs) x 64 steps and carries the state from wave to wave in
+// registers.  Every warp copies its own steps of the next waves to shared memory meanwhile (cp.async, two stages), and sends its
+// results out from there: 16 bytes an instruction where addresses allow it, and no address arithmetic in the recurrence.
 //
-// Both directions are scans of affine maps h -> A h + B, whose composition is (A2 A1, A2 B1 + B2), A kept in the same form.  A thread holds kSteps steps of W
-// channels in registers: it composes its steps, the warps of a CTA (one behind the other in time) compose theirs through shared
-// memory and the CTAs of a cluster theirs through distributed shared memory; then every thread walks its steps once more from
-// the state that reaches it.  So x and gate are read once and y is written once, whatever the length: the bound is DRAM.  A
-// cluster walks the time axis in waves of (its CTAs) x 64 steps and carries the state from wave to wave in registers.
+// A state that lasts 10^4 steps has gates within 10^-4 of one, and what matters of them is 1 - a: the rounding of a alone would cost
+// it three digits.  So the product over a thread's steps is also formed as 1 - A = sum (1 - a_t) a_1 .. a_{t-1}, of which no
+// term is a difference, and A is handed on as a float and the rest that its rounding left.
+//
 // The forward pass leaves the state before every 64th step; the backward pass recomputes the states in between from it, in
 // float32, and reads no y: 4 bytes in 64 steps instead of an activation per step, and no rounded state in a gradient.
 #include <cooperative_groups.h>
@@ -25,9 +28,9 @@ namespace dcn {
 namespace seq {
 namespace {
 
-constexpr int kSteps = 8;                        // of a thread
-constexpr int kWarps = 8;                        // of a CTA, at most
-constexpr int kChunk = kSteps * kWarps;          // steps between checkpoints
+constexpr int kTile = 64;                        // channels of a CTA: two a lane
+constexpr int kChunk = 64;                       // steps of a CTA in a wave, and between checkpoints
+constexpr int kForwardSteps = 16, kBackwardSteps = 8;       // of a thread: what its registers hold
 constexpr int kCluster = 8;                      // CTAs of a cluster, at most
 
 struct ScanArgs {
@@ -38,37 +41,51 @@ struct ScanArgs {
     float *last, *dstate, *checkpoints;
     int64_t steps, channels, chunks;
     int64_t x_batch, x_step, gate_batch, gate_step, dy_batch, dy_step;
-    int tiles;                                   // of 32 W channels
+    int tiles;
 };
 
-__device__ __forceinline__ bool near_one(float s) { return __float_as_int(s) < 0; }
+// h -> A h + B, A = a + more to more digits than a float has
+template <int W>
+struct Map {
+    Lanes<W> a, more, b;
+    __device__ __forceinline__ Lanes<W> operator()(Lanes<W> h) const { return fma(a, h, fma(more, h, b)); }
+};
 
-// s of a gate; -0, a step that keeps the state as it is, outside the sequence
-__device__ __forceinline__ float step_of(float gate, bool in) {
-    const float t = __expf(-fabsf(gate)), q = t * __fdividef(1.0f, 1.0f + t);
-    const uint32_t s = __float_as_uint(q) | (~__float_as_uint(gate) & 0x80000000u);
-    return in ? __uint_as_float(s) : -0.0f;
-}
-// a u, and a h + (1 - a) x
-__device__ __forceinline__ float times(float s, float u) { return fmaf(s, u, near_one(s) ? u : 0.0f); }
-__device__ __forceinline__ float advance(float s, float h, float x) { return fmaf(s, h - x, near_one(s) ? h : x); }
-
-// The product of gates, as A and as 1 - A: each is a sum or product of positive terms, so neither loses digits
+// A product of gates, and one minus it
+template <int W>
 struct Product {
-    float a = 1.0f, rest = 0.0f;
-    __device__ __forceinline__ void by(float s) {
-        rest = fmaf(-s, a, near_one(s) ? rest : 1.0f);
-        a = times(s, a);
+    Lanes<W> a = all_lanes<W>(1.0f), rest = all_lanes<W>(0.0f);
+    __device__ __forceinline__ void by(Lanes<W> gate, Lanes<W> one_minus) {
+        rest = fma(one_minus, a, rest);
+        a = gate * a;
     }
-    __device__ __forceinline__ float signed_form() const { return rest < 0.5f ? -rest : a; }
+    __device__ __forceinline__ void by(const Map<W>& m) { by(m.a, all_lanes<W>(1.0f) - m.a - m.more); }
+    __device__ __forceinline__ Map<W> map(Lanes<W> b) const {
+        float top[W], more[W];
+#pragma unroll
+        for (int i = 0; i < W; ++i) {
+            const float near = 1.0f - rest.at(i);
+            const bool close = rest.at(i) < 0.5f;
+            top[i] = close ? near : a.at(i);
+            more[i] = close ? (1.0f - near) - rest.at(i) : 0.0f;
+        }
+        return {lanes<W>(top), lanes<W>(more), b};
+    }
+};
+
+// Maps in shared memory, by the part of a word that a lane reads
+template <int W>
+struct MapRoom {
+    Lanes<W> v[3][32];
+    __device__ __forceinline__ void put(int lane, const Map<W>& m) { v[0][lane] = m.a, v[1][lane] = m.more, v[2][lane] = m.b; }
+    __device__ __forceinline__ Map<W> get(int lane) const { return {v[0][lane], v[1][lane], v[2][lane]}; }
 };
 
 // Where a thread works
-template <int W>
 struct Place {
     int lane, warp, warps, rank, ranks;
-    int64_t b, c;
-    bool live;
+    int64_t b, c;                                // c: the CTA's first channel
+    int width, mine;                             // channels of the CTA, and of them mine
     __device__ __forceinline__ explicit Place(const ScanArgs& p) {
         const cg::cluster_group cluster = cg::this_cluster();
         lane = threadIdx.x;
@@ -78,8 +95,20 @@ struct Place {
         ranks = (int)cluster.num_blocks();
         const unsigned unit = blockIdx.x / ranks;
         b = unit / p.tiles;
-        c = (int64_t)(unit % p.tiles) * 32 * W + lane * W;
-        live = c < p.channels;
+        c = (int64_t)(unit % p.tiles) * kTile;
+        width = (int)(p.channels - c < kTile ? p.channels - c : kTile);
+        mine = width - 2 * lane < 0 ? 0 : width - 2 * lane > 2 ? 2 : width - 2 * lane;
+    }
+    __device__ __forceinline__ Lanes<2> load(const float* s, int64_t row, int64_t channels) const {
+        float h[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) h[i] = s != nullptr && i < mine ? gload(s + row * channels + c + 2 * lane + i) : 0.0f;
+        return lanes<2>(h);
+    }
+    __device__ __forceinline__ void store(float* s, int64_t row, int64_t channels, Lanes<2> h) const {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (i < mine) s[row * channels + c + 2 * lane + i] = h.at(i);
     }
 };
 
@@ -89,155 +118,197 @@ __device__ __forceinline__ int64_t length_of(const ScanArgs& p, int64_t b) {
     return n < 0 ? 0 : n > p.steps ? p.steps : n;
 }
 
-template <int W>
-__device__ __forceinline__ void load_state(float (&h)[W], const float* s, int64_t at, bool live) {
-#pragma unroll
-    for (int i = 0; i < W; ++i) h[i] = s != nullptr && live ? gload(s + at + i) : 0.0f;
-}
-
-// kSteps packs from step t0 on; zeros where there is none
-template <typename T, int W>
-__device__ __forceinline__ void load_steps(Pack<T, W> (&v)[kSteps], const T* base, int64_t t0, int64_t stride, int64_t len,
-                                           bool live) {
-#pragma unroll
-    for (int k = 0; k < kSteps; ++k) {
-        v[k].zero();
-        if (live && t0 + k < len) v[k].get(base + (t0 + k) * stride);
+// K steps of the CTA's channels in shared memory, a warp's own, moved kBytes at a time
+template <typename T, int kBytes, int K>
+struct Block {
+    T v[K][kTile];
+    static constexpr int kPer = kBytes / (int)sizeof(T), kCols = kTile / kPer, kMoves = K * kCols / 32;
+    static __device__ __forceinline__ int row(int lane, int j) { return kCols <= 32 ? lane / kCols + j * (32 / kCols) : j / 2; }
+    static __device__ __forceinline__ int col(int lane, int j) {
+        return kCols <= 32 ? lane % kCols * kPer : (lane + 32 * (j % 2)) * kPer;
     }
+    // from step t0 on; zeros behind the sequence's end and the last channel
+    __device__ __forceinline__ void fill(const T* base, int64_t t0, int64_t stride, int64_t len, int width, int lane) {
+#pragma unroll
+        for (int j = 0; j < kMoves; ++j) {
+            const int r = row(lane, j), c = col(lane, j);
+            const bool in = t0 + r < len && c < width;
+            const T* from = in ? base + (t0 + r) * stride + c : base;
+            if constexpr (kBytes >= 4) {
+                copy_async<kBytes>(&v[r][c], from, in);
+            } else {
+                Pack<T, 1> one;
+                one.zero();
+                if (in) one.get(from);
+                *reinterpret_cast<uint16_t*>(&v[r][c]) = one.raw.u;
+            }
+        }
+    }
+    // to the steps before `steps`
+    __device__ __forceinline__ void drain(T* base, int64_t t0, int64_t stride, int64_t steps, int width, int lane) const {
+#pragma unroll
+        for (int j = 0; j < kMoves; ++j) {
+            const int r = row(lane, j), c = col(lane, j);
+            const Raw<kBytes> one = *reinterpret_cast<const Raw<kBytes>*>(&v[r][c]);
+            if (t0 + r < steps && c < width) store(base + (t0 + r) * stride + c, one);
+        }
+    }
+    __device__ __forceinline__ Pack<T, 2> get(int k, int lane) const {
+        Pack<T, 2> p;
+        p.raw = *reinterpret_cast<const Raw<2 * sizeof(T)>*>(&v[k][2 * lane]);
+        return p;
+    }
+    __device__ __forceinline__ Lanes<2> at(int k, int lane) const {
+        const Pack<T, 2> p = get(k, lane);
+        const float f[2] = {p.at(0), p.at(1)};
+        return lanes<2>(f);
+    }
+    __device__ __forceinline__ void put(int k, int lane, Lanes<2> x) {
+        const float f[2] = {x.at(0), x.at(1)};
+        Pack<T, 2> p;
+        p.set(f);
+        *reinterpret_cast<Raw<2 * sizeof(T)>*>(&v[k][2 * lane]) = p.raw;
+    }
+};
+
+// Gate and one minus it; one and zero, a step that keeps the state, behind a sequence's end
+template <typename T>
+__device__ __forceinline__ void gates_of(const Pack<T, 2>& g, bool in, Lanes<2>& a, Lanes<2>& keep) {
+    float fa[2], fk[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        logistic(g.at(i), fa[i], fk[i]);
+        if (!in) fa[i] = 1.0f, fk[i] = 0.0f;
+    }
+    a = lanes<2>(fa);
+    keep = lanes<2>(fk);
 }
 
 // Zeros from step `from` on, shared out over the warps of the cluster
-template <typename T, int W>
-__device__ __forceinline__ void zero_rest(const Place<W>& me, T* out, int64_t from, int64_t steps, int64_t channels) {
-    Pack<T, W> z;
-    z.zero();
-    if (me.live)
-        for (int64_t t = from + me.rank * me.warps + me.warp; t < steps; t += me.ranks * me.warps) z.put(out + t * channels);
+template <typename T>
+__device__ __forceinline__ void zero_rest(const Place& me, T* out, int64_t from, int64_t steps, int64_t channels) {
+    for (int64_t t = from + me.rank * me.warps + me.warp; t < steps; t += me.ranks * me.warps)
+        for (int c = me.lane; c < me.width; c += 32) out[t * channels + c] = from_float<T>(0.0f);
 }
 
-template <typename T, int W>
-__global__ void __launch_bounds__(32 * kWarps, 3) scan_forward_kernel(const ScanArgs p) {
-    // maps (A, B) of the warps and of the cluster's CTAs; two of each, so that a wave's are read while the next one's are written
-    __shared__ float2 part[2][kWarps][W][32];
-    __shared__ float2 whole[2][kCluster][W][32];
-    const Place<W> me(p);
+template <typename T, int kBytes>
+struct ForwardRoom {
+    static constexpr int K = kForwardSteps, kWarps = kChunk / K;
+    Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps];
+    // maps of the warps and of the cluster's CTAs; two of each, so that a wave's are read while the next one's are written
+    MapRoom<2> part[2][kWarps], whole[2][kCluster];
+};
+
+template <typename T, int kBytes>
+__global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward_kernel(const ScanArgs p) {
+    constexpr int K = kForwardSteps;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    auto& room = *reinterpret_cast<ForwardRoom<T, kBytes>*>(dynamic);
+    const Place me(p);
     pdl_wait();
     const int64_t len = length_of(p, me.b);
     const T* x = static_cast<const T*>(p.x) + me.b * p.x_batch + me.c;
     const T* gate = static_cast<const T*>(p.gate) + me.b * p.gate_batch + me.c;
     T* y = static_cast<T*>(p.y) + me.b * p.steps * p.channels + me.c;
-    float carry[W];
-    load_state<W>(carry, p.state, me.b * p.channels + me.c, me.live);
+    Lanes<2> carry = me.load(p.state, me.b, p.channels);
 
-    const int chunk = me.warps * kSteps, wave = me.ranks * chunk;
-    int64_t t0 = (int64_t)me.rank * chunk + me.warp * kSteps;      // my first step of this wave
-    Pack<T, W> rx[kSteps], rg[kSteps];
-    load_steps(rx, x, t0, p.x_step, len, me.live);
-    load_steps(rg, gate, t0, p.gate_step, len, me.live);
-    if (me.ranks > 1) cg::this_cluster().sync();                   // every CTA runs before another writes to its memory
-    int side = 0;
+    const int chunk = me.warps * K, wave = me.ranks * chunk;
+    int64_t t0 = (int64_t)me.rank * chunk + me.warp * K;           // my first step of this wave
     int64_t begin = 0;
-    for (; begin < len; begin += wave, t0 += wave, side ^= 1) {
-        float s[kSteps][W], v[kSteps][W], B[W];
-        Product A[W];
+    auto fill = [&](int side, int64_t t) {
+        if (t - me.rank * chunk - me.warp * K < len) {             // (a wave that does not come is not filled)
+            room.x[side][me.warp].fill(x, t, p.x_step, len, me.width, me.lane);
+            room.gate[side][me.warp].fill(gate, t, p.gate_step, len, me.width, me.lane);
+        }
+        copies_issued();
+    };
+    fill(0, t0);
+    fill(1, t0 + wave);
+    if (me.ranks > 1) cg::this_cluster().sync();                   // every CTA runs before another writes to its memory
+    for (int side = 0; begin < len; begin += wave, t0 += wave, side ^= 1) {
+        auto &bx = room.x[side][me.warp], &bg = room.gate[side][me.warp];
+        copies_arrived<1>();
+        __syncwarp();
+        // after each of my steps: y = A h + B of the state h before the first
+        Lanes<2> A[K], B[K], sum = all_lanes<2>(0.0f);
+        Product<2> product;
+        const bool all = begin + wave <= len;
+        auto compose = [&](auto whole) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) B[i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                s[k][i] = step_of(rg[k].at(i), t0 + k < len);
-                v[k][i] = rx[k].at(i);
-                A[i].by(s[k][i]);
-                B[i] = advance(s[k][i], B[i], v[k][i]);
+            for (int k = 0; k < K; ++k) {
+                Lanes<2> a, keep;
+                gates_of<T>(bg.get(k, me.lane), whole.value || t0 + k < len, a, keep);
+                product.by(a, keep);
+                sum = fma(a, sum, keep * bx.at(k, me.lane));
+                A[k] = product.a;
+                B[k] = sum;
             }
-        load_steps(rx, x, t0 + wave, p.x_step, len, me.live);      // the next wave's, in flight during what follows
-        load_steps(rg, gate, t0 + wave, p.gate_step, len, me.live);
-#pragma unroll
-        for (int i = 0; i < W; ++i) part[side][me.warp][i][me.lane] = make_float2(A[i].signed_form(), B[i]);
+        };
+        if (all) compose(std::true_type());
+        else compose(std::false_type());
+        room.part[side][me.warp].put(me.lane, product.map(sum));
         __syncthreads();
-        float h[W];
+        Lanes<2> h = carry;
         if (me.ranks > 1) {
             cg::cluster_group cluster = cg::this_cluster();
             if (me.warp == 0) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    Product a;
-                    float sum = 0.0f;
-                    for (int w = 0; w < me.warps; ++w) {
-                        const float2 n = part[side][w][i][me.lane];
-                        a.by(n.x);
-                        sum = times(n.x, sum) + n.y;
-                    }
-                    const float2 m = make_float2(a.signed_form(), sum);
-                    for (int r = 0; r < me.ranks; ++r) *cluster.map_shared_rank(&whole[side][me.rank][i][me.lane], r) = m;
+                Product<2> all_of;
+                Lanes<2> s = all_lanes<2>(0.0f);
+                for (int w = 0; w < me.warps; ++w) {
+                    const Map<2> m = room.part[side][w].get(me.lane);
+                    all_of.by(m);
+                    s = m(s);
                 }
+                const Map<2> m = all_of.map(s);
+                for (int r = 0; r < me.ranks; ++r) cluster.map_shared_rank(&room.whole[side][me.rank], r)->put(me.lane, m);
             }
             cluster.sync();
-#pragma unroll
-            for (int i = 0; i < W; ++i) h[i] = carry[i];
-            for (int r = 0; r < me.ranks; ++r)
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const float2 m = whole[side][r][i][me.lane];
-                    if (r == me.rank) h[i] = carry[i];
-                    carry[i] = times(m.x, carry[i]) + m.y;
-                }
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) h[i] = carry[i];
-        }
-        if (p.checkpoints != nullptr && me.warp == 0 && me.live && t0 < len) {
-            float* at = p.checkpoints + (me.b * p.chunks + t0 / kChunk) * p.channels + me.c;
-#pragma unroll
-            for (int i = 0; i < W; ++i) at[i] = h[i];
-        }
-        // from the state before the CTA's steps to the one before mine; a cluster of one also finds the state behind them here
-        const int upto = me.ranks > 1 ? me.warp : me.warps;
-        float mine[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) mine[i] = h[i];
-        for (int w = 0; w < upto; ++w)
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float2 m = part[side][w][i][me.lane];
-                if (w == me.warp) mine[i] = h[i];
-                h[i] = times(m.x, h[i]) + m.y;
+            for (int r = 0; r < me.ranks; ++r) {
+                if (r == me.rank) h = carry;
+                carry = room.whole[side][r].get(me.lane)(carry);
             }
-        if (me.ranks > 1) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) mine[i] = h[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) carry[i] = h[i];
         }
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const int64_t t = t0 + k;
-            float out[W];
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                mine[i] = advance(s[k][i], mine[i], v[k][i]);
-                out[i] = t < len ? mine[i] : 0.0f;
+        if (p.checkpoints != nullptr && me.warp == 0 && t0 < len) me.store(p.checkpoints, me.b * p.chunks + t0 / kChunk, p.channels, h);
+        // from the state before the CTA's steps to the one before mine; a CTA by itself also finds the state behind them here
+        Lanes<2> mine = h;
+        for (int w = 0; w < me.warps; ++w) {
+            if (w == me.warp) {
+                mine = h;
+                if (me.ranks > 1) break;
             }
-            Pack<T, W> to;
-            to.set(out);
-            if (me.live && t < p.steps) to.put(y + t * p.channels);
+            h = room.part[side][w].get(me.lane)(h);
         }
+        if (me.ranks == 1) carry = h;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            Lanes<2> v = fma(A[k], mine, B[k]);
+            if (!all && t0 + k >= len) v = all_lanes<2>(0.0f);
+            bx.put(k, me.lane, v);
+        }
+        __syncwarp();
+        bx.drain(y, t0, p.channels, p.steps, me.width, me.lane);
+        __syncwarp();
+        fill(side, t0 + 2 * wave);
     }
+    copies_arrived<0>();
     zero_rest(me, y, begin, p.steps, p.channels);
-    if (me.rank == 0 && me.warp == 0 && me.live) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) p.last[me.b * p.channels + me.c + i] = carry[i];
-    }
+    if (me.rank == 0 && me.warp == 0) me.store(p.last, me.b, p.channels, carry);
 }
 
-template <typename T, int W>
-__global__ void __launch_bounds__(32 * kWarps, 2) scan_backward_kernel(const ScanArgs p) {
-    // of a warp: the product A of its gates (signed), the B of its forward map and the P of its backward map p -> A p + P
-    __shared__ float part[2][kWarps][3][W][32];
-    __shared__ float2 whole[2][kCluster][W][32];                   // (A, P) of the cluster's CTAs
-    const Place<W> me(p);
+template <typename T, int kBytes>
+struct BackwardRoom {
+    static constexpr int K = kBackwardSteps, kWarps = kChunk / K;
+    Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps], dy[2][kWarps];
+    MapRoom<2> part[2][kWarps], whole[2][kCluster];
+    Lanes<2> back[2][kWarps][32];                // the b of the warps' backward maps p -> A p + b, which have the forward ones' A
+};
+
+template <typename T, int kBytes>
+__global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backward_kernel(const ScanArgs p) {
+    constexpr int K = kBackwardSteps;
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    auto& room = *reinterpret_cast<BackwardRoom<T, kBytes>*>(dynamic);
+    const Place me(p);
     pdl_wait();
     const int64_t len = length_of(p, me.b);
     const T* x = static_cast<const T*>(p.x) + me.b * p.x_batch + me.c;
@@ -245,140 +316,107 @@ __global__ void __launch_bounds__(32 * kWarps, 2) scan_backward_kernel(const Sca
     const T* dy = static_cast<const T*>(p.dy) + me.b * p.dy_batch + me.c;
     T* dx = static_cast<T*>(p.dx) + me.b * p.steps * p.channels + me.c;
     T* dgate = static_cast<T*>(p.dgate) + me.b * p.steps * p.channels + me.c;
-    float carry[W];
-    load_state<W>(carry, p.dlast, me.b * p.channels + me.c, me.live);
-    const bool has_dy = p.dy != nullptr && me.live;
+    Lanes<2> carry = me.load(p.dlast, me.b, p.channels);
 
-    const int chunk = me.warps * kSteps, wave = me.ranks * chunk;
+    const int chunk = me.warps * K, wave = me.ranks * chunk;
     const int64_t end = (len + wave - 1) / wave * wave;
-    int64_t t0 = end - wave + (int64_t)me.rank * chunk + me.warp * kSteps;
-    Pack<T, W> rx[kSteps], rg[kSteps], rd[kSteps];
-    if (end > 0) {
-        load_steps(rx, x, t0, p.x_step, len, me.live);
-        load_steps(rg, gate, t0, p.gate_step, len, me.live);
-        load_steps(rd, dy, t0, p.dy_step, len, has_dy);
-    }
+    int64_t begin = end - wave;
+    int64_t t0 = begin + (int64_t)me.rank * chunk + me.warp * K;
+    auto fill = [&](int side, int64_t t) {
+        if (t >= 0) {                                              // (a wave that does not come is not filled)
+            room.x[side][me.warp].fill(x, t, p.x_step, len, me.width, me.lane);
+            room.gate[side][me.warp].fill(gate, t, p.gate_step, len, me.width, me.lane);
+            room.dy[side][me.warp].fill(dy, t, p.dy_step, p.dy == nullptr ? t : len, me.width, me.lane);
+        }
+        copies_issued();
+    };
+    fill(0, t0);
+    fill(1, t0 - wave);
     if (me.ranks > 1) cg::this_cluster().sync();                   // every CTA runs before another writes to its memory
-    int side = 0;
-    for (int64_t begin = end - wave; begin >= 0; begin -= wave, t0 -= wave, side ^= 1) {
-        float before[W];                                           // the state before the CTA's steps
-        load_state<W>(before, p.checkpoints, (me.b * p.chunks + (t0 - me.warp * kSteps) / kChunk) * p.channels + me.c,
-                      me.live && t0 - me.warp * kSteps < len);
-        float s[kSteps][W], d[kSteps][W], h[kSteps][W];
-        Pack<T, W> cx[kSteps];
-        float B[W], P[W];
-        Product A[W];
+    for (int side = 0; begin >= 0; begin -= wave, t0 -= wave, side ^= 1) {
+        auto &bx = room.x[side][me.warp], &bg = room.gate[side][me.warp], &bd = room.dy[side][me.warp];
+        // the state before the CTA's steps
+        const int64_t first = t0 - me.warp * K;
+        Lanes<2> h = me.load(first < len ? p.checkpoints : nullptr, me.b * p.chunks + first / kChunk, p.channels);
+        copies_arrived<1>();
+        __syncwarp();
+        Lanes<2> a[K], keep[K], before[K], sum = all_lanes<2>(0.0f), passed = sum;
+        Product<2> product;
+        const bool all = begin + wave <= len;
+        auto compose = [&](auto whole) {
 #pragma unroll
-        for (int i = 0; i < W; ++i) B[i] = 0.0f, P[i] = 0.0f;
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            cx[k] = rx[k];
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                s[k][i] = step_of(rg[k].at(i), t0 + k < len);
-                d[k][i] = rd[k].at(i);
-                A[i].by(s[k][i]);
-                B[i] = advance(s[k][i], B[i], cx[k].at(i));
+            for (int k = 0; k < K; ++k) {
+                gates_of<T>(bg.get(k, me.lane), whole.value || t0 + k < len, a[k], keep[k]);
+                product.by(a[k], keep[k]);
+                sum = fma(a[k], sum, keep[k] * bx.at(k, me.lane));
             }
-        }
+        };
+        if (all) compose(std::true_type());
+        else compose(std::false_type());
 #pragma unroll
-        for (int k = kSteps - 1; k >= 0; --k)
-#pragma unroll
-            for (int i = 0; i < W; ++i) P[i] = times(s[k][i], d[k][i] + P[i]);
-        if (begin > 0) {
-            load_steps(rx, x, t0 - wave, p.x_step, len, me.live);
-            load_steps(rg, gate, t0 - wave, p.gate_step, len, me.live);
-            load_steps(rd, dy, t0 - wave, p.dy_step, len, has_dy);
-        }
-#pragma unroll
-        for (int i = 0; i < W; ++i) {
-            part[side][me.warp][0][i][me.lane] = A[i].signed_form();
-            part[side][me.warp][1][i][me.lane] = B[i];
-            part[side][me.warp][2][i][me.lane] = P[i];
-        }
+        for (int k = K - 1; k >= 0; --k) passed = a[k] * (bd.at(k, me.lane) + passed);
+        room.part[side][me.warp].put(me.lane, product.map(sum));
+        room.back[side][me.warp][me.lane] = passed;
         __syncthreads();
-        float g[W];                                                // the gradient that reaches the CTA's last step
-#pragma unroll
-        for (int i = 0; i < W; ++i) g[i] = carry[i];
+        auto back_map = [&](int w) {
+            Map<2> m = room.part[side][w].get(me.lane);
+            m.b = room.back[side][w][me.lane];
+            return m;
+        };
+        Lanes<2> g = carry;                                        // the gradient that reaches the CTA's last step
         if (me.ranks > 1) {
             cg::cluster_group cluster = cg::this_cluster();
             if (me.warp == 0) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    Product a;
-                    float sum = 0.0f;
-                    for (int w = me.warps - 1; w >= 0; --w) {
-                        const float n = part[side][w][0][i][me.lane];
-                        a.by(n);
-                        sum = times(n, sum) + part[side][w][2][i][me.lane];
-                    }
-                    const float2 m = make_float2(a.signed_form(), sum);
-                    for (int r = 0; r < me.ranks; ++r) *cluster.map_shared_rank(&whole[side][me.rank][i][me.lane], r) = m;
+                Product<2> all_of;
+                Lanes<2> s = all_lanes<2>(0.0f);
+                for (int w = me.warps - 1; w >= 0; --w) {
+                    const Map<2> m = back_map(w);
+                    all_of.by(m);
+                    s = m(s);
                 }
+                const Map<2> m = all_of.map(s);
+                for (int r = 0; r < me.ranks; ++r) cluster.map_shared_rank(&room.whole[side][me.rank], r)->put(me.lane, m);
             }
             cluster.sync();
-            for (int r = me.ranks - 1; r >= 0; --r)
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const float2 m = whole[side][r][i][me.lane];
-                    if (r == me.rank) g[i] = carry[i];
-                    carry[i] = times(m.x, carry[i]) + m.y;
-                }
-        }
-        for (int w = 0; w < me.warp; ++w)
-#pragma unroll
-            for (int i = 0; i < W; ++i) before[i] = times(part[side][w][0][i][me.lane], before[i]) + part[side][w][1][i][me.lane];
-        const int down = me.ranks > 1 ? me.warp + 1 : 0;
-        float mine[W];
-#pragma unroll
-        for (int i = 0; i < W; ++i) mine[i] = g[i];
-        for (int w = me.warps - 1; w >= down; --w)
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                if (w == me.warp) mine[i] = g[i];
-                g[i] = times(part[side][w][0][i][me.lane], g[i]) + part[side][w][2][i][me.lane];
-            }
-        if (me.ranks > 1) {
-#pragma unroll
-            for (int i = 0; i < W; ++i) mine[i] = g[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) carry[i] = g[i];
-        }
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k)
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                h[k][i] = before[i];
-                before[i] = advance(s[k][i], before[i], cx[k].at(i));
-            }
-#pragma unroll
-        for (int k = kSteps - 1; k >= 0; --k) {
-            const int64_t t = t0 + k;
-            float ox[W], og[W];
-#pragma unroll
-            for (int i = 0; i < W; ++i) {
-                const float D = d[k][i] + mine[i], q = fabsf(s[k][i]);
-                ox[i] = D * (near_one(s[k][i]) ? q : 1.0f - q);
-                og[i] = D * (h[k][i] - cx[k].at(i)) * fmaf(-q, q, q);
-                mine[i] = times(s[k][i], D);
-                if (t >= len) ox[i] = og[i] = 0.0f;
-            }
-            Pack<T, W> vx, vg;
-            vx.set(ox);
-            vg.set(og);
-            if (me.live && t < p.steps) {
-                vx.put(dx + t * p.channels);
-                vg.put(dgate + t * p.channels);
+            for (int r = me.ranks - 1; r >= 0; --r) {
+                if (r == me.rank) g = carry;
+                carry = room.whole[side][r].get(me.lane)(carry);
             }
         }
+        for (int w = 0; w < me.warp; ++w) h = room.part[side][w].get(me.lane)(h);
+        Lanes<2> mine = g;
+        for (int w = me.warps - 1; w >= 0; --w) {
+            if (w == me.warp) {
+                mine = g;
+                if (me.ranks > 1) break;
+            }
+            g = back_map(w)(g);
+        }
+        if (me.ranks == 1) carry = g;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+            before[k] = h;
+            h = fma(a[k], h, keep[k] * bx.at(k, me.lane));
+        }
+#pragma unroll
+        for (int k = K - 1; k >= 0; --k) {
+            const Lanes<2> d = bd.at(k, me.lane) + mine;
+            Lanes<2> ox = d * keep[k], og = ox * a[k] * (before[k] - bx.at(k, me.lane));
+            mine = a[k] * d;
+            if (!all && t0 + k >= len) ox = og = all_lanes<2>(0.0f);
+            bx.put(k, me.lane, ox);
+            bg.put(k, me.lane, og);
+        }
+        __syncwarp();
+        bx.drain(dx, t0, p.channels, p.steps, me.width, me.lane);
+        bg.drain(dgate, t0, p.channels, p.steps, me.width, me.lane);
+        __syncwarp();
+        fill(side, t0 - 2 * wave);
     }
+    copies_arrived<0>();
     zero_rest(me, dx, end, p.steps, p.channels);
     zero_rest(me, dgate, end, p.steps, p.channels);
-    if (p.dstate != nullptr && me.rank == 0 && me.warp == 0 && me.live) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) p.dstate[me.b * p.channels + me.c + i] = carry[i];
-    }
+    if (p.dstate != nullptr && me.rank == 0 && me.warp == 0) me.store(p.dstate, me.b, p.channels, carry);
 }
 
 template <typename T, int W>
@@ -398,7 +436,11 @@ __global__ void __launch_bounds__(128) scan_step_kernel(int64_t rows, int64_t ch
             h.get(state + slot * channels + c);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                out[i] = advance(step_of(vg.at(i), true), h.at(i), vx.at(i));
+                // a h + (1 - a) x as a step from the larger share: no product with a gate near one is rounded
+                float a, keep;
+                logistic(vg.at(i), a, keep);
+                const float from = a < keep ? vx.at(i) : h.at(i), to = a < keep ? h.at(i) : vx.at(i);
+                out[i] = fmaf(a < keep ? a : keep, to - from, from);
             }
             h.set(out);
             h.put(state + slot * channels + c);
@@ -411,31 +453,40 @@ __global__ void __launch_bounds__(128) scan_step_kernel(int64_t rows, int64_t ch
     }
 }
 
-struct Launch {
-    int warps, ranks;
-    unsigned grid;
-};
-
-// CTAs along time: as many warps as the steps fill, and a cluster as long as the GPU has room for more CTAs.
-Launch launch_of(int64_t units, int64_t steps) {
-    Launch l;
-    l.warps = (int)(steps >= kChunk ? kWarps : steps > kSteps ? (steps + kSteps - 1) / kSteps : 1);
-    l.ranks = 1;
-    while (l.ranks < kCluster && (int64_t)l.ranks * kChunk < steps && units * l.ranks < 2 * sm_count()) l.ranks *= 2;
-    l.grid = (unsigned)(units * l.ranks);
-    return l;
+// CTAs of a kernel that an SM holds with its shared memory, asked for once per device (0: it cannot be launched)
+template <typename Room, typename K>
+int resident(K kernel, int threads) {
+    constexpr int kMostDevices = 64;
+    static std::atomic<int> of_device[kMostDevices];
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMostDevices) return 0;
+    int n = of_device[dev];
+    if (n == 0) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Room)) != cudaSuccess ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, sizeof(Room)) != cudaSuccess)
+            return 0;
+        of_device[dev] = n;                      // racing first calls find the same number
+    }
+    return n;
 }
 
+// As many warps as the steps fill, and CTAs along time as long as the GPU holds all of them at once: a cluster walks the whole
+// time axis, and one that had to wait for another would double the time.
 template <typename K>
-int launch_scan(K kernel, const ScanArgs& a, int64_t batch, cudaStream_t st) {
-    const Launch l = launch_of(batch * a.tiles, a.steps);
+int launch_scan(K kernel, int held, size_t smem, int per_thread, const ScanArgs& a, int64_t batch, cudaStream_t st) {
+    if (held == 0) return DCN_ERR_CUDA;
+    const int64_t units = batch * a.tiles;
+    const int warps = (int)(a.steps >= kChunk ? kChunk / per_thread : a.steps > per_thread ? (a.steps + per_thread - 1) / per_thread : 1);
+    int ranks = 1;
+    while (ranks < kCluster && (int64_t)ranks * kChunk < a.steps && 2 * units * ranks <= (int64_t)held * sm_count()) ranks *= 2;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(l.grid);
-    cfg.blockDim = dim3(32, l.warps);
+    cfg.gridDim = dim3((unsigned)(units * ranks));
+    cfg.blockDim = dim3(32, warps);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = l.ranks;
+    attr[0].val.clusterDim.x = ranks;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
@@ -445,19 +496,39 @@ int launch_scan(K kernel, const ScanArgs& a, int64_t batch, cudaStream_t st) {
     return e != cudaSuccess || cudaGetLastError() != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
+template <typename T, int kBytes>
+int run_forward(const ScanArgs& a, int64_t batch, cudaStream_t st) {
+    using Room = ForwardRoom<T, kBytes>;
+    const int held = resident<Room>(scan_forward_kernel<T, kBytes>, 32 * kChunk / kForwardSteps);
+    return launch_scan(scan_forward_kernel<T, kBytes>, held, sizeof(Room), kForwardSteps, a, batch, st);
+}
+
+template <typename T, int kBytes>
+int run_backward(const ScanArgs& a, int64_t batch, cudaStream_t st) {
+    using Room = BackwardRoom<T, kBytes>;
+    const int held = resident<Room>(scan_backward_kernel<T, kBytes>, 32 * kChunk / kBackwardSteps);
+    return launch_scan(scan_backward_kernel<T, kBytes>, held, sizeof(Room), kBackwardSteps, a, batch, st);
+}
+
 int check_scan(const dcn_scan* p) {
     if (p == nullptr) return DCN_ERR_NULL;
     if (!known_type(p->dtype)) return DCN_ERR_UNSUPPORTED;
     if (p->batch < 0 || p->steps < 0 || p->channels < 0) return DCN_ERR_SHAPE;
     constexpr int64_t most = 1ll << 31;
     if (p->batch >= most || p->steps >= most || p->channels >= most) return DCN_ERR_LIMIT;
-    if (p->batch * ((p->channels + 31) / 32) >= 1ll << 27) return DCN_ERR_LIMIT;       // CTAs of a grid, eight to a cluster
+    if (p->batch * ((p->channels + kTile - 1) / kTile) >= 1ll << 27) return DCN_ERR_LIMIT;       // CTAs of a grid, eight to a cluster
     return DCN_OK;
 }
 
-bool even(const void* p, int64_t batch, int64_t step) { return aligned(p, 4) && batch % 2 == 0 && step % 2 == 0; }
+// Bytes that a copy moves at once: 16 or 4 where every row of every tensor starts on as many, an element otherwise
+struct Bytes {
+    int n = 16, e;
+    void by(const void* p, int64_t batch, int64_t step) {
+        while (n > e && (!aligned(p, n) || batch * e % n != 0 || step * e % n != 0)) n = n == 16 ? 4 : e;
+    }
+};
 
-ScanArgs args_of(const dcn_scan* p, int w) {
+ScanArgs args_of(const dcn_scan* p) {
     ScanArgs a = {};
     a.steps = p->steps;
     a.channels = p->channels;
@@ -465,7 +536,7 @@ ScanArgs args_of(const dcn_scan* p, int w) {
     a.x_batch = p->x_batch, a.x_step = p->x_step;
     a.gate_batch = p->gate_batch, a.gate_step = p->gate_step;
     a.dy_batch = p->dy_batch, a.dy_step = p->dy_step;
-    a.tiles = (int)((p->channels + 32 * w - 1) / (32 * w));
+    a.tiles = (int)((p->channels + kTile - 1) / kTile);
     return a;
 }
 
@@ -490,18 +561,22 @@ extern "C" int dcn_scan_forward(const dcn_scan* p, const void* x, const void* ga
     if (!aligned(x, e) || !aligned(gate, e) || !aligned(y, e) || !aligned(state, 4) || !aligned(last, 4) ||
         !aligned(lengths, 8) || !aligned(checkpoints, 4))
         return DCN_ERR_ALIGN;
-    // two channels a thread where pairs of 16-bit elements can be read as one word: lines of 128 bytes a warp
-    const bool two = e == 2 && p->channels % 2 == 0 && even(x, p->x_batch, p->x_step) &&
-                     even(gate, p->gate_batch, p->gate_step) && aligned(y, 4);
-    ScanArgs a = args_of(p, two ? 2 : 1);
+    Bytes bytes{16, e};
+    bytes.by(x, p->x_batch, p->x_step);
+    bytes.by(gate, p->gate_batch, p->gate_step);
+    bytes.by(y, p->channels, p->channels);
+    ScanArgs a = args_of(p);
     a.x = x, a.gate = gate, a.state = state, a.lengths = lengths, a.y = y, a.last = last, a.checkpoints = checkpoints;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (p->dtype == DCN_SEQ_F32) return launch_scan(scan_forward_kernel<float, 1>, a, p->batch, st);
+    if (p->dtype == DCN_SEQ_F32)
+        return bytes.n == 16 ? run_forward<float, 16>(a, p->batch, st) : run_forward<float, 4>(a, p->batch, st);
     if (p->dtype == DCN_SEQ_BF16)
-        return two ? launch_scan(scan_forward_kernel<__nv_bfloat16, 2>, a, p->batch, st)
-                   : launch_scan(scan_forward_kernel<__nv_bfloat16, 1>, a, p->batch, st);
-    return two ? launch_scan(scan_forward_kernel<__half, 2>, a, p->batch, st)
-               : launch_scan(scan_forward_kernel<__half, 1>, a, p->batch, st);
+        return bytes.n == 16  ? run_forward<__nv_bfloat16, 16>(a, p->batch, st)
+               : bytes.n == 4 ? run_forward<__nv_bfloat16, 4>(a, p->batch, st)
+                              : run_forward<__nv_bfloat16, 2>(a, p->batch, st);
+    return bytes.n == 16  ? run_forward<__half, 16>(a, p->batch, st)
+           : bytes.n == 4 ? run_forward<__half, 4>(a, p->batch, st)
+                          : run_forward<__half, 2>(a, p->batch, st);
 }
 
 extern "C" int dcn_scan_backward(const dcn_scan* p, const void* x, const void* gate, const int64_t* lengths,
@@ -516,19 +591,25 @@ extern "C" int dcn_scan_backward(const dcn_scan* p, const void* x, const void* g
     if (!aligned(x, e) || !aligned(gate, e) || !aligned(dy, e) || !aligned(dx, e) || !aligned(dgate, e) ||
         !aligned(dlast, 4) || !aligned(dstate, 4) || !aligned(lengths, 8) || !aligned(checkpoints, 4))
         return DCN_ERR_ALIGN;
-    const bool two = e == 2 && p->channels % 2 == 0 && even(x, p->x_batch, p->x_step) &&
-                     even(gate, p->gate_batch, p->gate_step) && (dy == nullptr || even(dy, p->dy_batch, p->dy_step)) &&
-                     aligned(dx, 4) && aligned(dgate, 4);
-    ScanArgs a = args_of(p, two ? 2 : 1);
+    Bytes bytes{16, e};
+    bytes.by(x, p->x_batch, p->x_step);
+    bytes.by(gate, p->gate_batch, p->gate_step);
+    if (dy != nullptr) bytes.by(dy, p->dy_batch, p->dy_step);
+    bytes.by(dx, p->channels, p->channels);
+    bytes.by(dgate, p->channels, p->channels);
+    ScanArgs a = args_of(p);
     a.x = x, a.gate = gate, a.dy = dy, a.dlast = dlast, a.lengths = lengths, a.dx = dx, a.dgate = dgate, a.dstate = dstate;
     a.checkpoints = const_cast<float*>(checkpoints);
     const cudaStream_t st = (cudaStream_t)stream;
-    if (p->dtype == DCN_SEQ_F32) return launch_scan(scan_backward_kernel<float, 1>, a, p->batch, st);
+    if (p->dtype == DCN_SEQ_F32)
+        return bytes.n == 16 ? run_backward<float, 16>(a, p->batch, st) : run_backward<float, 4>(a, p->batch, st);
     if (p->dtype == DCN_SEQ_BF16)
-        return two ? launch_scan(scan_backward_kernel<__nv_bfloat16, 2>, a, p->batch, st)
-                   : launch_scan(scan_backward_kernel<__nv_bfloat16, 1>, a, p->batch, st);
-    return two ? launch_scan(scan_backward_kernel<__half, 2>, a, p->batch, st)
-               : launch_scan(scan_backward_kernel<__half, 1>, a, p->batch, st);
+        return bytes.n == 16  ? run_backward<__nv_bfloat16, 16>(a, p->batch, st)
+               : bytes.n == 4 ? run_backward<__nv_bfloat16, 4>(a, p->batch, st)
+                              : run_backward<__nv_bfloat16, 2>(a, p->batch, st);
+    return bytes.n == 16  ? run_backward<__half, 16>(a, p->batch, st)
+           : bytes.n == 4 ? run_backward<__half, 4>(a, p->batch, st)
+                          : run_backward<__half, 2>(a, p->batch, st);
 }
 
 namespace {
