@@ -39,6 +39,10 @@ __device__ __forceinline__ void load(Raw<16>& r, const void* p) {
     asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "l"(p));
 }
+// The same where the data is read again soon
+__device__ __forceinline__ void load_kept(Raw<16>& r, const void* p) {
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "l"(p));
+}
 __device__ __forceinline__ void store(void* p, const Raw<2>& r) { *static_cast<uint16_t*>(p) = r.u; }
 __device__ __forceinline__ void store(void* p, const Raw<4>& r) { *static_cast<uint32_t*>(p) = r.u[0]; }
 __device__ __forceinline__ void store(void* p, const Raw<8>& r) { *static_cast<uint2*>(p) = make_uint2(r.u[0], r.u[1]); }

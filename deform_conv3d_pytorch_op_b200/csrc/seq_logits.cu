@@ -21,6 +21,7 @@ namespace seq {
 namespace {
 
 constexpr int kThreads = 256;                    // of a CTA that has a row, or a part of one
+constexpr int kFewThreads = 64;                  // of one that has a short row
 constexpr int kWarpRows = 4;                     // rows of a CTA whose warps have one each
 constexpr int kCluster = 8;
 constexpr int kMostTop = DCN_SCORES_MOST_TOP, kMostK = DCN_DISTILL_MOST_K;
@@ -127,90 +128,169 @@ __device__ __forceinline__ void add_one(Sums& a, float v, float k) {
     if constexpr (kU) a.u = fmaf(e, d, a.u);
 }
 
-// The sums of a thread's elements.  kMarks: without the marked ones.
+template <typename T>
+__device__ __forceinline__ bool marked(const Row<T>& row, const uint8_t* marks, int e) {
+    const int b = mark_of(row, e);
+    return (marks[b >> 3] >> (b & 7) & 1) != 0;
+}
+
+// Elements one by one: those outside vectors, and rows whose logits are as large as the type allows.  Not inlined, so that the
+// usual path stays short.
 template <typename T, bool kU, bool kMarks>
+__device__ __noinline__ Sums add_elements(Sums a, const Row<T>& row, int e0, int e1, int step, float k, const uint8_t* marks) {
+    for (int e = e0; e < e1; e += step) {
+        if constexpr (kMarks)
+            if (marked(row, marks, e)) continue;
+        add_one<kU>(a, row.one(e), k);
+    }
+    return a;
+}
+
+// Words of a vector as the type's own instructions take them
+template <typename T>
+struct Word {
+    static constexpr int kPer = 4 / sizeof(T);
+    static constexpr uint32_t kNothing = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u;
+    static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
+        uint32_t r;
+        if constexpr (sizeof(T) == 4) r = __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+        return r;
+    }
+    static __device__ __forceinline__ float at(uint32_t w, int i) {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+        else return half_of<T>(w, i);
+    }
+    // without the element
+    static __device__ __forceinline__ uint32_t without(uint32_t w, int i) {
+        if constexpr (sizeof(T) == 4) return kNothing;
+        else return i == 0 ? (w & 0xffff0000u) | (kNothing & 0xffffu) : (w & 0xffffu) | (kNothing & 0xffff0000u);
+    }
+};
+
+// Elements 2 i, 2 i + 1 of a vector's words
+template <typename T>
+__device__ __forceinline__ Lanes<2> pair_of(const uint32_t* w, int i) {
+    float f[2];
+    if constexpr (sizeof(T) == 4) f[0] = __uint_as_float(w[2 * i]), f[1] = __uint_as_float(w[2 * i + 1]);
+    else f[0] = half_of<T>(w[i], 0), f[1] = half_of<T>(w[i], 1);
+    return lanes<2>(f);
+}
+
+// The sums of a thread's elements.  kMarks: without the marked ones.  kAgain: the elements are read a second time.
+template <typename T, bool kU, bool kMarks, bool kAgain>
 __device__ __forceinline__ Sums sums_of(const Row<T>& row, int tid, int threads, float k, const uint8_t* marks) {
-    constexpr int kPer = Row<T>::kPer, kBatch = 32 / kPer;
+    using W = Word<T>;
+    constexpr int kPer = Row<T>::kPer, kBatch = 4, kWords = 4 * kBatch;
+    constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     Sums a{kNone, 0.0f, 0.0f};
-    auto marked = [&](int e) {
-        if constexpr (!kMarks) return false;
-        const int b = mark_of(row, e);
-        return (marks[b >> 3] >> (b & 7) & 1) != 0;
-    };
-    for (int e = tid; e < row.head_here; e += threads)
-        if (!marked(e)) add_one<kU>(a, row.one(e), k);
+    const int ends = row.head_here + (row.n - row.tail);          // elements outside vectors: at most one a thread
+    if (tid < ends) {
+        const int e = tid < row.head_here ? tid : row.tail + tid - row.head_here;
+        a = add_elements<T, kU, kMarks>(a, row, e, e + 1, 1, k, marks);
+    }
     for (int v = row.v0 + tid; v < row.v1; v += kBatch * threads) {
-        Pack<T, kPer> raw[kBatch];
-        float f[kBatch * kPer];
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-            if (v + b * threads < row.v1) raw[b].get(row.vec(v + b * threads));
-        float m = a.m;
+        uint32_t w[kWords];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
-            const bool in = v + b * threads < row.v1;
-            uint32_t bits = 0;
-            if constexpr (kMarks) {
-                const int at = 8 + (v + b * threads - row.v0) * kPer;
-                if (in) bits = marks[at >> 3] >> (at & 7);
+            Raw<16> raw = {{W::kNothing, W::kNothing, W::kNothing, W::kNothing}};
+            if (v + b * threads < row.v1) {
+                if constexpr (kAgain) load_kept(raw, row.vec(v + b * threads));
+                else load(raw, row.vec(v + b * threads));
             }
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                f[b * kPer + i] = in && !(kMarks && (bits >> i & 1)) ? raw[b].at(i) : kNone;
-                m = max_nan(m, f[b * kPer + i]);
+            for (int i = 0; i < 4; ++i) w[4 * b + i] = raw.u[i];
+        }
+        if constexpr (kMarks) {
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+                const int at = 8 + (v + b * threads - row.v0) * kPer;
+                if (v + b * threads >= row.v1) break;
+                const uint32_t bits = marks[at >> 3] >> (at & 7) & ((1u << kPer) - 1);
+                if (bits == 0) continue;         // (nearly always)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    if (bits >> i & 1) w[4 * b + i / W::kPer] = W::without(w[4 * b + i / W::kPer], i % W::kPer);
             }
         }
+        uint32_t top = w[0];
+#pragma unroll
+        for (int i = 1; i < kWords; ++i) top = W::max(top, w[i]);
+        float m = max_nan(a.m, W::at(top, 0));
+        if constexpr (W::kPer == 2) m = max_nan(m, W::at(top, 1));
         if (m == kNone) continue;
         if (m != a.m) a.rescale(m, k);
         const Shift shift(m, k);
         if (shift.far) {
-#pragma unroll
-            for (int i = 0; i < kBatch * kPer; ++i) add_one<kU>(a, f[i], k);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kBatch * kPer; ++i) {
-                float d = __fmaf_rn(f[i], k, -shift.mk);
-                if constexpr (kU) d = max_nan(d, -kFar);
-                const float e = ex2(d);
-                a.s += e;
-                if constexpr (kU) a.u = fmaf(e, d, a.u);
+            for (int b = v; b < min(v + kBatch * threads, row.v1); b += threads) {
+                const int e = row.head + b * kPer;
+                a = add_elements<T, kU, kMarks>(a, row, e, e + kPer, 1, k, marks);
             }
+        } else {
+            const Lanes<2> kk = all_lanes<2>(k), shifted = all_lanes<2>(-shift.mk);
+            Lanes<2> s = all_lanes<2>(0.0f), u = s;
+#pragma unroll
+            for (int i = 0; i < kWords * W::kPer / 2; ++i) {
+                // 0 times what is far below is 0, not NaN: logits of -inf are raised to where their d is finite
+                if constexpr (kU && kBf16) w[i] = W::max(w[i], 0xf14af14au);             // -1e30
+                Lanes<2> d = fma(pair_of<T>(w, i), kk, shifted);
+                if constexpr (kU && !kBf16) {
+                    const float f[2] = {max_nan(d.at(0), -kFar), max_nan(d.at(1), -kFar)};
+                    d = lanes<2>(f);
+                }
+                const float e[2] = {ex2(d.at(0)), ex2(d.at(1))};
+                s = s + lanes<2>(e);
+                if constexpr (kU) u = fma(lanes<2>(e), d, u);
+            }
+            a.s += s.at(0) + s.at(1);
+            if constexpr (kU) a.u += u.at(0) + u.at(1);
         }
     }
-    for (int e = row.tail + tid; e < row.n; e += threads)
-        if (!marked(e)) add_one<kU>(a, row.one(e), k);
     return a;
 }
 
-// The threads of a row: a warp, or a CTA.
+// The threads of a row: a warp, or a CTA.  Its sums use two areas in turn, so that one barrier a sum is enough: an area is
+// written again behind the barrier of the sum in between.
 template <bool kWarp>
 struct Team {
-    float* room;                                 // 32 x 2 floats, of a CTA
-    int tid, threads;
+    float2 (&room)[2][32];
+    int tid, threads, side = 0;
     __device__ __forceinline__ void sync() const {
         if constexpr (kWarp) __syncwarp();
         else __syncthreads();
     }
     template <typename F>
-    __device__ __forceinline__ float fold(float v, float none, F&& f) const {
+    __device__ __forceinline__ float2 fold(float2 v, float none, F&& f) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+        for (int o = 16; o > 0; o >>= 1) {
+            v.x = f(v.x, __shfl_xor_sync(0xffffffffu, v.x, o));
+            v.y = f(v.y, __shfl_xor_sync(0xffffffffu, v.y, o));
+        }
         if constexpr (!kWarp) {
+            float2* at = room[side];
+            side ^= 1;
+            if (tid % 32 == 0) at[tid / 32] = v;
             __syncthreads();
-            if (tid % 32 == 0) room[tid / 32] = v;
-            __syncthreads();
-            v = tid % 32 < threads / 32 ? room[tid % 32] : none;
+            v = make_float2(none, none);
 #pragma unroll
-            for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+            for (int w = 0; w < kThreads / 32; ++w)
+                if (w < threads / 32) v = make_float2(f(v.x, at[w].x), f(v.y, at[w].y));
         }
         return v;
     }
-    __device__ __forceinline__ float max(float v) const { return fold(v, kNone, [](float a, float b) { return max_nan(a, b); }); }
-    __device__ __forceinline__ float sum(float v) const { return fold(v, 0.0f, [](float a, float b) { return a + b; }); }
-    __device__ __forceinline__ Sums join(Sums a, float k, bool with_u) const {
+    __device__ __forceinline__ float max(float v) {
+        return fold(make_float2(v, v), kNone, [](float a, float b) { return max_nan(a, b); }).x;
+    }
+    __device__ __forceinline__ float2 sum2(float x, float y) {
+        return fold(make_float2(x, y), 0.0f, [](float a, float b) { return a + b; });
+    }
+    __device__ __forceinline__ float sum(float v) { return sum2(v, 0.0f).x; }
+    __device__ __forceinline__ Sums join(Sums a, float k) {
         a.rescale(max(a.m), k);
-        a.s = sum(a.s);
-        if (with_u) a.u = sum(a.u);
+        const float2 v = sum2(a.s, a.u);
+        a.s = v.x;
+        a.u = v.y;
         return a;
     }
 };
@@ -228,19 +308,21 @@ __device__ __forceinline__ float value_of(uint32_t key) {
     return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key);
 }
 
-constexpr int kRoom = 1024;                      // entries of a list
-
+// What a CTA of kT threads needs for it
+template <int kT>
 struct TopRoom {
-    unsigned long long above[kRoom], equal[kRoom];          // what is over the bound, and what is on it
-    unsigned long long best[kCluster][kMostTop];            // the parts' results, in the first CTA of a cluster
-    uint32_t maxima[kThreads];
+    static constexpr int kWarps = kT / 32, kRoom = 8 * kT, kParts = kT == kThreads ? kCluster : 1;
+    unsigned long long list[kRoom];              // candidates
+    unsigned long long best[kParts][kMostTop];   // the parts' results, where the list is too small; the row's in the end
+    alignas(16) uint32_t keys[kT];               // the largest of the warps' lanes, of all CTAs of the cluster
     uint32_t bound;
-    int n_above, n_equal, count[kThreads / 32];
+    int n, counts[kParts], count[kWarps];
 };
 
 // Entry i of a list goes to the place of its rank
+template <int kT>
 __device__ __forceinline__ void place(const unsigned long long* list, int n, int tid, int top, unsigned long long* out) {
-    for (int i = tid; i < n; i += kThreads) {
+    for (int i = tid; i < n; i += kT) {
         const unsigned long long mine = list[i];
         int rank = 0;
         for (int j = 0; j < n; ++j) rank += list[j] > mine;
@@ -248,126 +330,193 @@ __device__ __forceinline__ void place(const unsigned long long* list, int n, int
     }
 }
 
-__device__ __forceinline__ int block_count(TopRoom& r, int v, int tid) {
+template <int kT>
+__device__ __forceinline__ int block_count(TopRoom<kT>& r, int v, int tid) {
     v = __reduce_add_sync(0xffffffffu, v);
     __syncthreads();
     if (tid % 32 == 0) r.count[tid / 32] = v;
     __syncthreads();
     int sum = 0;
-    for (int w = 0; w < kThreads / 32; ++w) sum += r.count[w];
+    for (int w = 0; w < kT / 32; ++w) sum += r.count[w];
     return sum;
 }
 
-// The `top` largest keys of a CTA's part, in order, into out[0, top) (0 behind the last, where the part has fewer).
-// Bound: the top-th largest of the threads' maxima `mine`, which at least `top` elements reach.  What is over it, rarely much more
-// than `top`, is listed and ranked.  If fewer than `top` are over it, the bound is the value of the last places, which go to the
-// lowest indices that have it.  If more are over it than the list holds (large values all in few threads' hands), the value
-// of the last place is found by bisection.
 template <typename T>
-__device__ __forceinline__ void top_of(const Row<T>& row, float mine, int tid, int top, TopRoom& r, unsigned long long* out) {
-    const bool any = row.v0 + tid < row.v1 || tid < row.head_here || row.tail + tid < row.n;
-    r.maxima[tid] = any ? key_of(mine) : 0;
+__device__ __forceinline__ uint32_t vector_max(const Raw<16>& v) {
+    using W = Word<T>;
+    return W::max(W::max(v.u[0], v.u[1]), W::max(v.u[2], v.u[3]));
+}
+
+// Lists the elements that reach the bound in a room (another CTA's too), whose n counts them, listed or not.  Returns the number
+// of the warp's.
+template <typename T, int kT>
+__device__ __forceinline__ int list_candidates(const Row<T>& row, int tid, uint32_t bound, TopRoom<kT>& r) {
+    using W = Word<T>;
+    constexpr int kPer = Row<T>::kPer, kBatch = 4;
+    const float least = bound == 0 ? kNone : value_of(bound);
+    auto reaches = [&](float v) { return v >= least || v != v; };
+    const int lane = tid % 32;
+    int all = 0;
+    // the lanes of a warp get their places from a prefix sum of their counts, and the warp its own from one addition
+    auto list = [&](uint32_t mask, auto&& element_of) {
+        if (!__any_sync(0xffffffffu, mask != 0)) return;
+        const int n = __popc(mask);
+        int at = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, at, o);
+            if (lane >= o) at += up;
+        }
+        int base = 0;
+        if (lane == 31) base = atomicAdd(&r.n, at);
+        all += __shfl_sync(0xffffffffu, at, 31);
+        at += __shfl_sync(0xffffffffu, base, 31) - n;
+        for (; mask != 0 && at < TopRoom<kT>::kRoom; mask &= mask - 1, ++at) {
+            const int e = element_of(__ffs(mask) - 1);
+            r.list[at] = (unsigned long long)key_of(row.one(e)) << 32 | (uint32_t)~e;
+        }
+    };
+    {
+        const int ends = row.head_here + (row.n - row.tail), e = tid < row.head_here ? tid : row.tail + tid - row.head_here;
+        list(tid < ends && reaches(row.one(e)) ? 1u : 0u, [&](int) { return e; });
+    }
+    for (int first = row.v0 + tid - lane; first < row.v1; first += kBatch * kT) {       // (a warp's first vector)
+        Raw<16> raw[kBatch];
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b)
+            if (first + lane + b * kT < row.v1) load_kept(raw[b], row.vec(first + lane + b * kT));
+        uint32_t mask = 0;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+            if (first + lane + b * kT >= row.v1) break;
+            const uint32_t m = vector_max<T>(raw[b]);
+            float top = W::at(m, 0);
+            if constexpr (W::kPer == 2) top = max_nan(top, W::at(m, 1));
+            if (reaches(top)) {                  // (rarely)
+#pragma unroll
+                for (int i = 0; i < kPer; ++i)
+                    if (reaches(W::at(raw[b].u[i / W::kPer], i % W::kPer))) mask |= 1u << (b * kPer + i);
+            }
+        }
+        list(mask, [&](int bit) { return row.head + (first + lane + bit / kPer * kT) * kPer + bit % kPer; });
+    }
+    return all;
+}
+
+template <typename T, int kT>
+__device__ __noinline__ int count_from(const Row<T>& row, int tid, uint32_t bound, TopRoom<kT>& r) {
+    int n = 0;
+    row.each(tid, kT, [&](int, float v) { n += key_of(v) >= bound; });
+    return block_count(r, n, tid);
+}
+
+// The largest key that `top` elements of the part reach, which is at least `bound`: by bisection
+template <typename T, int kT>
+__device__ __noinline__ uint32_t exact_bound(const Row<T>& row, int tid, int top, uint32_t bound, TopRoom<kT>& r) {
+    uint32_t hi = 0xffffffffu;
+    if (bound < hi && count_from(row, tid, bound + 1, r) < top) return bound;
+    while (bound < hi) {
+        const uint32_t mid = bound + (hi - bound) / 2 + 1;
+        if (count_from(row, tid, mid, r) >= top) bound = mid;
+        else hi = mid - 1;
+    }
+    return bound;
+}
+
+// Entries of the first `need` elements that are on the bound, by index: a vector a thread at a time
+template <typename T, int kT>
+__device__ __noinline__ void first_on_bound(const Row<T>& row, int tid, int need, uint32_t bound, TopRoom<kT>& r, unsigned long long* out) {
+    constexpr int kPer = Row<T>::kPer;
+    int done = 0;
+    // a thread's place from a prefix sum of the counts, threads being in the order of their elements
+    auto place_of = [&](int mine) {
+        int before = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int up = __shfl_up_sync(0xffffffffu, before, o);
+            if (tid % 32 >= o) before += up;
+        }
+        __syncthreads();
+        if (tid % 32 == 31) r.count[tid / 32] = before;
+        __syncthreads();
+        int start = done, all = 0;
+        for (int w = 0; w < kT / 32; ++w) {
+            if (w < tid / 32) start += r.count[w];
+            all += r.count[w];
+        }
+        done += all;
+        return start + before - mine;
+    };
+    auto take = [&](int e0, int n) {             // n elements of mine from e0 on
+        int count = 0;
+        for (int i = 0; i < n; ++i) count += key_of(row.one(e0 + i)) == bound;
+        int at = place_of(count);
+        for (int i = 0; i < n && count > 0; ++i)
+            if (key_of(row.one(e0 + i)) == bound) {
+                if (at < need) out[at] = (unsigned long long)bound << 32 | (uint32_t)~(e0 + i);
+                ++at;
+            }
+    };
+    take(tid, tid < row.head_here ? 1 : 0);
+    for (int v = row.v0; v < row.v1 && done < need; v += kT) take(row.head + (v + tid) * kPer, v + tid < row.v1 ? kPer : 0);
+    if (done < need) take(row.tail + tid, row.tail + tid < row.n ? 1 : 0);
+}
+
+// The largest keys of a warp's lanes, `each` of them, into to[0, each) (0 behind the last element)
+__device__ __forceinline__ void largest_of_warp(float mine, bool any, int each, uint32_t* to) {
+    uint32_t key = any ? key_of(mine) : 0;
+    for (int i = 0; i < each; ++i) {
+        const uint32_t taken = __reduce_max_sync(0xffffffffu, key);
+        const uint32_t who = __ballot_sync(0xffffffffu, key == taken);
+        if (threadIdx.x % 32 == __ffs(who) - 1) {
+            key = 0;
+            to[i] = taken;
+        }
+    }
+}
+
+// The top-th largest of n published keys, each a lane's maximum: at least `top` elements of the row reach it
+template <int kT>
+__device__ __forceinline__ uint32_t bound_of(TopRoom<kT>& r, int n, int tid, int top) {
+    if (tid == 0) r.bound = 0;
+    if (tid >= n) r.keys[tid] = 0;               // (up to a whole number of vectors)
+    __syncthreads();
+    if (tid < n) {
+        const uint32_t mine = r.keys[tid];
+        int rank = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; j += 4) {
+            const uint4 v = *reinterpret_cast<const uint4*>(&r.keys[j]);
+            // equal keys by their place
+            rank += (v.x > mine) + (v.y > mine) + (v.z > mine) + (v.w > mine);
+            rank += (v.x == mine & j < tid) + (v.y == mine & j + 1 < tid) + (v.z == mine & j + 2 < tid) + (v.w == mine & j + 3 < tid);
+        }
+        if (rank == top - 1) r.bound = mine;
+    }
+    __syncthreads();
+    return r.bound;
+}
+
+// Where the list cannot hold what reaches the bound (many equal values, or large ones all in few lanes' hands): the `top` largest of a
+// CTA's part, in order, into out[0, top) (0 behind the last).  If they do not fit either, the value of the part's last place is
+// found by bisection.  Fewer than `top` elements are larger and are listed; the places behind them go to the lowest indices that have
+// the value.
+template <typename T, int kT>
+__device__ __noinline__ void top_of_part(const Row<T>& row, int tid, int top, uint32_t bound, int reach, TopRoom<kT>& r, unsigned long long* out) {
+    __syncthreads();
     if (tid < top) out[tid] = 0;
-    if (tid == 0) r.n_above = r.n_equal = 0;
-    __syncthreads();
-    const uint32_t my_key = r.maxima[tid];
-    int rank = 0;
-    for (int j = 0; j < kThreads; ++j) rank += r.maxima[j] > my_key || (r.maxima[j] == my_key && j < tid);
-    if (rank == top - 1) r.bound = my_key;
-    __syncthreads();
-    uint32_t bound = r.bound;
-    for (int attempt = 0; attempt < 2; ++attempt) {
-        const float least = bound == 0 ? kNone : value_of(bound);
-        row.each(tid, kThreads, [&](int e, float v) {
-            if (v < least) return;
-            const uint32_t key = key_of(v);
-            const unsigned long long entry = (unsigned long long)key << 32 | (uint32_t)~e;
-            if (key > bound) {
-                if (*(volatile int*)&r.n_above <= kRoom) {
-                    const int at = atomicAdd(&r.n_above, 1);
-                    if (at < kRoom) r.above[at] = entry;
-                }
-            } else if (key == bound && *(volatile int*)&r.n_equal <= kRoom) {
-                const int at = atomicAdd(&r.n_equal, 1);
-                if (at < kRoom) r.equal[at] = entry;
-            }
-        });
-        __syncthreads();
-        if (r.n_above <= kRoom) break;
-        uint32_t hi = 0xffffffffu;               // the largest key that `top` elements reach: in [bound, hi]
-        while (bound < hi) {
-            const uint32_t mid = bound + (hi - bound) / 2 + 1;
-            int n = 0;
-            row.each(tid, kThreads, [&](int, float v) { n += key_of(v) >= mid; });
-            if (block_count(r, n, tid) >= top) bound = mid;
-            else hi = mid - 1;
-        }
-        __syncthreads();
-        if (tid == 0) r.n_above = r.n_equal = 0;
-        __syncthreads();
+    if (tid == 0) r.n = 0;
+    int equal = 0;
+    if (reach > TopRoom<kT>::kRoom) {
+        bound = exact_bound(row, tid, top, bound, r);
+        equal = 1;
     }
-    const int above = min(r.n_above, kRoom), equal = r.n_equal;
-    place(r.above, above, tid, top, out);
-    const int need = top - above;
-    if (need > 0 && equal > 0) {
-        if (equal <= kRoom) {
-            place(r.equal, equal, tid, need, out + above);
-        } else {                                 // dense: the first of them by index, a vector a thread at a time
-            constexpr int kPer = Row<T>::kPer;
-            int done = 0;
-            auto take = [&](int e, float v, bool in, int& before) {
-                if (in && key_of(v) == bound) {
-                    if (before < need) out[above + before] = (unsigned long long)bound << 32 | (uint32_t)~e;
-                    ++before;
-                }
-            };
-            // threads in the order of their elements: places from a prefix sum of their counts
-            auto places = [&](int mine_n) {
-                int before = mine_n;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int up = __shfl_up_sync(0xffffffffu, before, o);
-                    if (tid % 32 >= o) before += up;
-                }
-                __syncthreads();
-                if (tid % 32 == 31) r.count[tid / 32] = before;
-                __syncthreads();
-                int start = done, all = 0;
-                for (int w = 0; w < kThreads / 32; ++w) {
-                    if (w < tid / 32) start += r.count[w];
-                    all += r.count[w];
-                }
-                done += all;
-                return start + before - mine_n;
-            };
-            {
-                const bool in = tid < row.head_here;
-                const float v = in ? row.one(tid) : 0.0f;
-                int at = places(in && key_of(v) == bound);
-                take(tid, v, in, at);
-            }
-            for (int v0 = row.v0; v0 < row.v1 && done < need; v0 += kThreads) {
-                const int v = v0 + tid;
-                Pack<T, kPer> a;
-                a.zero();
-                if (v < row.v1) a.get(row.vec(v));
-                int n = 0;
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) n += v < row.v1 && key_of(a.at(i)) == bound;
-                int at = places(n);
-                if (n > 0)
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) take(row.head + v * kPer + i, a.at(i), true, at);
-            }
-            if (done < need) {
-                const int e = row.tail + tid;
-                const bool in = e < row.n;
-                const float v = in ? row.one(e) : 0.0f;
-                int at = places(in && key_of(v) == bound);
-                take(e, v, in, at);
-            }
-        }
-    }
+    __syncthreads();
+    if (bound + equal >= bound) list_candidates(row, tid, bound + equal, r);
+    __syncthreads();
+    const int n = r.n;
+    if (equal) first_on_bound(row, tid, top - n, bound, r, out + n);
+    place<kT>(r.list, n, tid, top, out);
     __syncthreads();
 }
 
@@ -381,7 +530,7 @@ struct LogitsArgs {
     // scores
     const int64_t* tokens;
     int64_t ignore;
-    int top;
+    int top, top_each;                           // top_each: of the largest lanes of a warp, to find a bound from
     float *logprob, *entropy, *top_logprobs;
     int64_t* top_tokens;
     const float *dlogprob, *dentropy, *dtop;
@@ -419,7 +568,7 @@ struct TeacherRoom {
 
 // The teacher's places of a row: tokens and log q (normalised over them where there is no tail)
 template <typename T, bool kWarp>
-__device__ __forceinline__ float teacher_of(const LogitsArgs& p, int64_t row, const Team<kWarp>& team, TeacherRoom& r, int& used) {
+__device__ __forceinline__ float teacher_of(const LogitsArgs& p, int64_t row, Team<kWarp>& team, TeacherRoom& r, int& used) {
     int n = 0;
     float m = kNone;
     for (int i = team.tid; i < p.places; i += team.threads) {
@@ -446,7 +595,7 @@ __device__ __forceinline__ float teacher_of(const LogitsArgs& p, int64_t row, co
 }
 
 template <typename T, bool kWarp>
-__device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, const T* logits, const Team<kWarp>& team,
+__device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, const T* logits, Team<kWarp>& team,
                                             TeacherRoom& r, Sums rest, float norm, int used) {
     // the student's sums over the teacher's tokens, each token once
     Sums best{kNone, 0.0f, 0.0f};
@@ -459,7 +608,7 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, co
         for (int j = 0; j < i; ++j) again |= r.token[j] == t;
         if (!again) add_one<false>(best, r.logit[i], p.k);
     }
-    best = team.join(best, p.k, false);
+    best = team.join(best, p.k);
     mass = team.sum(mass);
     const float m = max_nan(best.m, rest.m);
     Sums all = best, other = rest;
@@ -493,27 +642,37 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, co
     }
 }
 
-template <typename T, int kKind, bool kWarp>
-__global__ void __launch_bounds__(kThreads) logits_forward_kernel(const LogitsArgs p) {
+template <typename T, int kKind, bool kWarp, int kT>
+__global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) {
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ float room[32];
+    __shared__ float2 room[2][32];
     __shared__ Sums parts[kCluster];
     __shared__ TeacherRoom teachers[kKind == kDistill ? (kWarp ? kWarpRows : 1) : 1];
     const cg::cluster_group cluster = cg::this_cluster();
     const int rank = kWarp ? 0 : (int)cluster.block_rank(), ranks = kWarp ? 1 : (int)cluster.num_blocks();
     const int group = kWarp ? threadIdx.x / 32 : 0;
     const int64_t at = kWarp ? (int64_t)blockIdx.x * kWarpRows + group : blockIdx.x / ranks;
-    const Team<kWarp> team{room, kWarp ? (int)threadIdx.x % 32 : (int)threadIdx.x, kWarp ? 32 : kThreads};
-    if (ranks > 1) cluster.sync();               // every CTA runs before another writes to its memory
+    Team<kWarp> team{room, kWarp ? (int)threadIdx.x % 32 : (int)threadIdx.x, kWarp ? 32 : kT};
+    // every CTA of a cluster runs before another writes to its memory
+    if (ranks > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
+    auto arrived = [&] { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); };
     if (at >= p.rows) return;                    // (a warp's row: a CTA's is always there)
     pdl_wait();
     const T* logits = static_cast<const T*>(p.logits) + at * p.stride;
     const Row<T> row(logits, p.vocab, rank, ranks);
-    TopRoom& top = *reinterpret_cast<TopRoom*>(dynamic);
+    TopRoom<kT>& top = *reinterpret_cast<TopRoom<kT>*>(dynamic);
+    constexpr int kWarps = kT / 32;
     TeacherRoom& teacher = teachers[kKind == kDistill ? group : 0];
     uint8_t* marks = dynamic + group * p.marks;
-    float norm = 0.0f;
+    float norm = 0.0f, given = CUDART_NAN_F;
     int used = 0;
+    int64_t token = p.ignore;
+    if constexpr (kKind != kDistill) {           // (on its way while the row is read)
+        if (team.tid == 0 && rank == 0 && p.logprob != nullptr) {
+            token = gload_i64(p.tokens + at);
+            if (token >= 0 && token < p.vocab) given = row.one(token);
+        }
+    }
     if constexpr (kKind == kDistill) {
         for (int i = team.tid; i < p.marks / 4; i += team.threads) reinterpret_cast<uint32_t*>(marks)[i] = 0;
         norm = teacher_of<T, kWarp>(p, at, team, teacher, used);
@@ -528,29 +687,79 @@ __global__ void __launch_bounds__(kThreads) logits_forward_kernel(const LogitsAr
         }
         team.sync();
     }
-    const Sums mine = sums_of<T, kKind != kDistill, kKind == kDistill>(row, team.tid, team.threads, p.k, marks);
-    Sums sums = team.join(mine, p.k, kKind != kDistill);
+    const Sums mine = sums_of<T, kKind != kDistill, kKind == kDistill, kKind == kScoresTop>(row, team.tid, team.threads, p.k, marks);
+    Sums sums = team.join(mine, p.k);
     if constexpr (kKind == kScoresTop) {
-        if (ranks == 1) {
-            top_of(row, mine.m, team.tid, p.top, top, top.best[0]);
-        } else {
-            top_of(row, mine.m, team.tid, p.top, top, top.best[rank]);
-            if (rank > 0 && team.tid < p.top) *cluster.map_shared_rank(&top.best[rank][team.tid], 0) = top.best[rank][team.tid];
+        const int warp = team.tid / 32;
+        const bool any = row.v0 + team.tid < row.v1 || team.tid < row.head_here + (row.n - row.tail);
+        uint32_t* to = top.keys + (rank * kWarps + warp) * p.top_each;
+        largest_of_warp(mine.m, any, p.top_each, to);
+        if (team.tid == 0) top.n = 0;
+        __syncwarp();
+        if (ranks > 1) {
+            const uint32_t key = team.tid % 32 < p.top_each ? to[team.tid % 32] : 0;
+            arrived();
+            for (int r = 0; r < ranks; ++r)
+                if (team.tid % 32 < p.top_each) cluster.map_shared_rank(to, r)[team.tid % 32] = key;
         }
     }
     if (ranks > 1) {
-        if (team.tid == 0) *cluster.map_shared_rank(&parts[rank], 0) = sums;
+        if constexpr (kKind != kScoresTop) arrived();
+        if (team.tid < ranks) *cluster.map_shared_rank(&parts[rank], team.tid) = sums;
         cluster.sync();
-        if (rank > 0) return;
-        float m = parts[0].m;
-        for (int r = 1; r < ranks; ++r) m = max_nan(m, parts[r].m);
-        sums = Sums{m, 0.0f, 0.0f};
-        for (int r = 0; r < ranks; ++r) {
-            Sums other = parts[r];
-            other.rescale(m, p.k);
-            sums.s += other.s;
-            sums.u += other.u;
+        if constexpr (kKind != kScoresTop)
+            if (rank > 0) return;
+    }
+    if constexpr (kKind == kScoresTop) {
+        const uint32_t bound = bound_of<kT>(top, ranks * kWarps * p.top_each, team.tid, p.top);
+        TopRoom<kT>& first = ranks > 1 ? *cluster.map_shared_rank(&top, 0) : top;
+        const int listed = list_candidates(row, team.tid, bound, first);
+        int n = 0;
+        if (ranks > 1) {
+            if (team.tid % 32 == 0) top.count[team.tid / 32] = listed;
+            __syncthreads();
+            if (team.tid < ranks) {
+                for (int w = 0; w < kWarps; ++w) n += top.count[w];
+                cluster.map_shared_rank(&top, team.tid)->counts[rank] = n;
+            }
+            cluster.sync();
+            n = 0;
+            for (int r = 0; r < ranks; ++r) n += top.counts[r];
+        } else {
+            __syncthreads();
+            n = top.n;
         }
+        if (n > TopRoom<kT>::kRoom) {            // (the same for all CTAs of the cluster)
+            top_of_part(row, team.tid, p.top, bound, ranks > 1 ? top.counts[rank] : n, top, top.best[rank]);
+            if (rank > 0)
+                for (int i = team.tid; i < p.top; i += kT)
+                    *cluster.map_shared_rank(&top.best[rank][i], 0) = top.best[rank][i];
+            if (ranks > 1) cluster.sync();
+            if (rank > 0) return;
+            n = ranks * p.top;
+            for (int i = team.tid; i < n; i += kT) top.list[i] = top.best[i / p.top][i % p.top];
+            __syncthreads();
+        }
+        if (rank > 0) return;
+        place<kT>(top.list, n, team.tid, p.top, top.best[0]);
+        __syncthreads();
+    }
+    if (ranks > 1) {                             // the parts' sums, a lane each
+        const int lane = team.tid % 32;
+        Sums part{kNone, 0.0f, 0.0f};
+        if (lane < ranks) part = parts[lane];
+        float m = part.m;
+#pragma unroll
+        for (int o = kCluster / 2; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, o));
+        part.rescale(m, p.k);
+#pragma unroll
+        for (int o = kCluster / 2; o > 0; o >>= 1) {
+            part.s += __shfl_xor_sync(0xffffffffu, part.s, o);
+            part.u += __shfl_xor_sync(0xffffffffu, part.u, o);
+        }
+        sums.m = __shfl_sync(0xffffffffu, part.m, 0);
+        sums.s = __shfl_sync(0xffffffffu, part.s, 0);
+        sums.u = __shfl_sync(0xffffffffu, part.u, 0);
     }
     if constexpr (kKind == kDistill) {
         distill_row<T, kWarp>(p, at, logits, team, teacher, sums, norm, used);
@@ -559,10 +768,9 @@ __global__ void __launch_bounds__(kThreads) logits_forward_kernel(const LogitsAr
         const float entropy = sums.m == kNone ? 0.0f : kLn2 * (log_s - sums.u / sums.s);
         if (team.tid == 0) {
             if (p.logprob != nullptr) {
-                const int64_t t = gload_i64(p.tokens + at);
                 float v = CUDART_NAN_F;
-                if (t == p.ignore) v = 0.0f;
-                else if (t >= 0 && t < p.vocab) v = log_p(row.one(t), sums.m, log_s, p);
+                if (token == p.ignore) v = 0.0f;
+                else if (token >= 0 && token < p.vocab) v = log_p(given, sums.m, log_s, p);
                 p.logprob[at] = v;
             }
             if (p.entropy != nullptr) p.entropy[at] = entropy;
@@ -572,16 +780,8 @@ __global__ void __launch_bounds__(kThreads) logits_forward_kernel(const LogitsAr
             }
         }
         if constexpr (kKind == kScoresTop) {
-            unsigned long long* best = top.best[0];
-            if (ranks > 1) {                     // the parts' best, ranked among one another
-                for (int i = team.tid; i < ranks * p.top; i += kThreads) top.above[i] = top.best[i / p.top][i % p.top];
-                __syncthreads();
-                place(top.above, ranks * p.top, team.tid, p.top, top.equal);
-                __syncthreads();
-                best = top.equal;
-            }
-            for (int i = team.tid; i < p.top; i += kThreads) {
-                const unsigned long long entry = best[i];
+            for (int i = team.tid; i < p.top; i += kT) {
+                const unsigned long long entry = top.best[0][i];
                 p.top_tokens[at * p.top + i] = (int64_t)(uint32_t)~(uint32_t)entry;
                 p.top_logprobs[at * p.top + i] = log_p(value_of((uint32_t)(entry >> 32)), sums.m, log_s, p);
             }
@@ -590,7 +790,8 @@ __global__ void __launch_bounds__(kThreads) logits_forward_kernel(const LogitsAr
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------
-// dz = 2^l (c0 + c1 l), l = log2 p: p from (m, log2 S)
+// dz = 2^l (c0 + c1 l), l = log2 p: p from (m, log2 S).  kLinear: c1 is 0.
+template <bool kLinear>
 struct Slope {
     Shift shift;
     float log_s, c0, c1;
@@ -600,7 +801,25 @@ struct Slope {
     __device__ __forceinline__ float operator()(float v) const {
         if (zero) return 0.0f;
         const float l = max_nan(shift(v) - log_s, -kFar);
-        return ex2(l) * fmaf(c1, l, c0);
+        return ex2(l) * (kLinear ? c0 : fmaf(c1, l, c0));
+    }
+    // a vector's, where the row is neither far nor zero
+    template <typename T>
+    __device__ __forceinline__ void near(const uint32_t* w, float (&f)[16 / sizeof(T)]) const {
+        const Lanes<2> kk = all_lanes<2>(shift.k), shifted = all_lanes<2>(-shift.mk), ss = all_lanes<2>(-log_s);
+#pragma unroll
+        for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
+            Lanes<2> l = fma(pair_of<T>(w, i), kk, shifted) + ss, c = all_lanes<2>(c0);
+            if constexpr (!kLinear) {
+                const float far[2] = {max_nan(l.at(0), -kFar), max_nan(l.at(1), -kFar)};
+                l = lanes<2>(far);
+                c = fma(all_lanes<2>(c1), l, c);
+            }
+            const float e[2] = {ex2(l.at(0)), ex2(l.at(1))};
+            c = lanes<2>(e) * c;
+            f[2 * i] = c.at(0);
+            f[2 * i + 1] = c.at(1);
+        }
     }
 };
 
@@ -609,7 +828,7 @@ __global__ void __launch_bounds__(kThreads) logits_backward_kernel(const LogitsA
     constexpr int kPer = Row<T>::kPer;
     __shared__ int token[kMostTop + 1];
     __shared__ float weight[kMostTop + 1];
-    __shared__ float room[32];
+    __shared__ float2 room[2][32];
     const int tid = threadIdx.x, threads = blockDim.x;
     const int64_t at = blockIdx.x / parts;
     const int part = blockIdx.x % parts;
@@ -618,46 +837,41 @@ __global__ void __launch_bounds__(kThreads) logits_backward_kernel(const LogitsA
     T* out = static_cast<T*>(p.dlogits) + at * p.vocab;
     const float* stat = p.stats + at * DCN_LOGITS_STATS;
     const float m = gload(stat + kM), log_s = gload(stat + kLogS);
-    // the special tokens and what they get beside the slope
-    const Team<false> team{room, tid, threads};
+    // what the row's elements get; the special tokens get a term more
+    Slope<kDistilled> slope(m, p.k, log_s, 0.0f, 0.0f), special = slope;
     int specials;
-    Slope slope(m, p.k, log_s, 0.0f, 0.0f), special = slope;
+    float g = 0.0f;
     if constexpr (kDistilled) {
         specials = p.places;
-        const float g = gload(p.dloss + at) * p.temperature;
-        slope = Slope(gload(stat + kRestM), p.k, gload(stat + kRestLogS), g * gload(stat + kRestC), 0.0f);
+        g = gload(p.dloss + at) * p.temperature;
+        slope = Slope<true>(gload(stat + kRestM), p.k, gload(stat + kRestLogS), g * gload(stat + kRestC), 0.0f);
         special.c0 = g * gload(stat + kMass);
-        const float norm = gload(stat + kNorm);
-        for (int i = tid; i < specials; i += threads) {
-            const int64_t t = gload_i64(p.teacher_tokens + at * p.places + i);
-            const bool in = t >= 0 && t < p.vocab;
-            token[i] = in ? (int)t : -1;
-            weight[i] = in ? -g * expf(teacher_at<T>(p, at * p.places + i) - norm) : 0.0f;
-        }
     } else {
         specials = p.dtop != nullptr ? p.top + 1 : 1;
         const float scale = 1.0f / p.temperature;
         const float gh = p.dentropy != nullptr ? gload(p.dentropy + at) : 0.0f;
-        float all = 0.0f;
-        for (int i = tid; i < specials; i += threads) {
-            float g = 0.0f;
+        auto special_of = [&](int i) {
             int64_t t = -1;
+            float v = 0.0f;
             if (i > 0) {
                 t = gload_i64(p.top_tokens + at * p.top + i - 1);
-                g = gload(p.dtop + at * p.top + i - 1);
+                v = gload(p.dtop + at * p.top + i - 1);
             } else if (p.dlogprob != nullptr) {
                 t = gload_i64(p.tokens + at);
-                g = gload(p.dlogprob + at);
+                v = gload(p.dlogprob + at);
                 if (t == p.ignore) t = -1;
             }
             const bool in = t >= 0 && t < p.vocab;
             token[i] = in ? (int)t : -1;
-            weight[i] = in ? g * scale : 0.0f;
-            all += weight[i];
-        }
+            return weight[i] = in ? v * scale : 0.0f;
+        };
+        float all = 0.0f;
         if (specials > 1) {
+            for (int i = tid; i < specials; i += threads) all += special_of(i);
+            Team<false> team{room, tid, threads};
             all = team.sum(all);
         } else {
+            if (tid == 0) special_of(0);
             __syncthreads();
             all = weight[0];
         }
@@ -667,20 +881,25 @@ __global__ void __launch_bounds__(kThreads) logits_backward_kernel(const LogitsA
     }
     // vectors where the gradient's rows start as the logits' do, elements otherwise
     const bool same = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(row.p) % 16;
+    const bool plain = !slope.zero && !slope.shift.far;
     auto put = [&](int64_t e, float v) { out[e] = from_float<T>(v); };
     for (int e = tid; e < row.head_here; e += threads) put(e, slope(row.one(e)));
     constexpr int kBatch = 4;
     for (int v = row.v0 + tid; v < row.v1; v += kBatch * threads) {
-        Pack<T, kPer> raw[kBatch];
+        Raw<16> raw[kBatch];
 #pragma unroll
         for (int b = 0; b < kBatch; ++b)
-            if (v + b * threads < row.v1) raw[b].get(row.vec(v + b * threads));
+            if (v + b * threads < row.v1) load(raw[b], row.vec(v + b * threads));
 #pragma unroll
         for (int b = 0; b < kBatch; ++b) {
             if (v + b * threads >= row.v1) break;
             float f[kPer];
+            if (plain) {
+                slope.template near<T>(raw[b].u, f);
+            } else {
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) f[i] = slope(raw[b].at(i));
+                for (int i = 0; i < kPer; ++i) f[i] = slope(Word<T>::at(raw[b].u[i / Word<T>::kPer], i % Word<T>::kPer));
+            }
             T* to = out + row.head + (int64_t)(v + b * threads) * kPer;
             if (same) {
                 Pack<T, kPer> o;
@@ -693,6 +912,15 @@ __global__ void __launch_bounds__(kThreads) logits_backward_kernel(const LogitsA
         }
     }
     for (int e = row.tail + tid; e < row.n; e += threads) put(e, slope(row.one(e)));
+    if constexpr (kDistilled) {
+        const float norm = gload(stat + kNorm);
+        for (int i = tid; i < specials; i += threads) {
+            const int64_t t = gload_i64(p.teacher_tokens + at * p.places + i);
+            const bool in = t >= 0 && t < p.vocab;
+            token[i] = in ? (int)t : -1;
+            weight[i] = in ? -g * expf(teacher_at<T>(p, at * p.places + i) - norm) : 0.0f;
+        }
+    }
     __syncthreads();                             // the part's special tokens are written over what stands there
     if (special.zero) return;
     for (int i = tid; i < specials; i += threads) {
@@ -705,7 +933,9 @@ __global__ void __launch_bounds__(kThreads) logits_backward_kernel(const LogitsA
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
-constexpr int kWarpVocab = 2048;                 // rows up to this size: a warp each, where no alternatives are asked for
+constexpr int kWarpVocab = 2048;                 // rows up to this size: a warp each, or two where alternatives are asked for
+
+constexpr int kBackwardPart = 32768;
 
 int parts_of(int64_t rows, int64_t vocab) {
     int parts = 1;
@@ -718,14 +948,26 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
     const bool warp = kKind != kScoresTop && a.vocab <= kWarpVocab;
     const int parts = warp ? 1 : parts_of(a.rows, a.vocab);
     cudaLaunchConfig_t cfg = {};
-    size_t smem = kKind == kScoresTop ? sizeof(TopRoom) : 0;
+    size_t smem = 0;
+    bool few = false;
+    if (kKind == kScoresTop) {
+        few = a.vocab <= kWarpVocab && a.top <= 32;
+        smem = few ? sizeof(TopRoom<kFewThreads>) : sizeof(TopRoom<kThreads>);
+        // of every warp whose lanes all have a vector its share, or one more where that is less than twice `top` in all (the more,
+        // the less is listed that is not among the `top`); of all CTAs together not more than there are keys
+        const int warps = (few ? kFewThreads : kThreads) / 32, vectors = a.vocab / (16 / (int)sizeof(T)) / parts;
+        const int full = vectors / 32 < 1 ? 1 : vectors / 32 < warps ? vectors / 32 : warps;
+        const int share = (a.top + parts * full - 1) / (parts * full), most = 32 / parts;
+        a.top_each = parts * full * share < 2 * a.top ? share + 1 : share;
+        if (a.top_each > most) a.top_each = most;
+    }
     if (kKind == kDistill) {
         const int per = 16 / (int)sizeof(T);
         a.marks = (int)(((a.vocab / per + parts - 1) / parts * per + 8 + 2 * per + 8 + 127) / 128 * 16);
         smem = (size_t)a.marks * (warp ? kWarpRows : 1);
     }
     cfg.gridDim = dim3((unsigned)(warp ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows * parts));
-    cfg.blockDim = dim3(warp ? 32 * kWarpRows : kThreads);
+    cfg.blockDim = dim3(warp ? 32 * kWarpRows : few ? kFewThreads : kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -738,20 +980,22 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
     cudaError_t e = cudaSuccess;
     if constexpr (kKind == kScoresTop) {
-        e = cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, false>, a);
+        e = few ? cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, false, kFewThreads>, a)
+                : cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, false, kThreads>, a);
     } else if (warp) {
-        e = cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, true>, a);
+        e = cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, true, 32 * kWarpRows>, a);
     } else {
-        if (smem > 40 * 1024) e = cudaFuncSetAttribute(logits_forward_kernel<T, kKind, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, false>, a);
+        const auto kernel = logits_forward_kernel<T, kKind, false, kThreads>;
+        if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, a);
     }
     return e != cudaSuccess || cudaGetLastError() != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
 template <typename T, bool kDistilled>
 int run_backward(const LogitsArgs& a, cudaStream_t st) {
-    // parts of at most 16384 elements, of a CTA with a vector or more for each thread
-    const int64_t parts = (a.vocab + 16383) / 16384;
+    // parts of at most kBackwardPart elements, of a CTA with a vector or more for each thread
+    const int64_t parts = (a.vocab + kBackwardPart - 1) / kBackwardPart;
     const int64_t vectors = a.vocab / parts * (int64_t)sizeof(T) / 16;
     const int threads = vectors >= 192 ? 256 : vectors >= 96 ? 128 : 64;
     if (a.rows * parts >= 1ll << 31) return DCN_ERR_LIMIT;
