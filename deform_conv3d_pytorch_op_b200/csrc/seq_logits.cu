@@ -192,21 +192,30 @@ __device__ __forceinline__ Sums sums_of(const Row<T>& row, int tid, int threads,
     }
     for (int v = row.v0 + tid; v < row.v1; v += kBatch * threads) {
         uint32_t w[kWords];
-#pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            Raw<16> raw = {{W::kNothing, W::kNothing, W::kNothing, W::kNothing}};
-            if (v + b * threads < row.v1) {
-                if constexpr (kAgain) load_kept(raw, row.vec(v + b * threads));
-                else load(raw, row.vec(v + b * threads));
-            }
+        const bool whole = v + (kBatch - 1) * threads < row.v1;
+        auto fetch = [&](int b) {
+            Raw<16> raw;
+            if constexpr (kAgain) load_kept(raw, row.vec(v + b * threads));
+            else load(raw, row.vec(v + b * threads));
 #pragma unroll
             for (int i = 0; i < 4; ++i) w[4 * b + i] = raw.u[i];
+        };
+        if (whole) {
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) fetch(b);
+        } else {
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[4 * b + i] = W::kNothing;
+                if (v + b * threads < row.v1) fetch(b);
+            }
         }
         if constexpr (kMarks) {
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 const int at = 8 + (v + b * threads - row.v0) * kPer;
-                if (v + b * threads >= row.v1) break;
+                if (!whole && v + b * threads >= row.v1) break;
                 const uint32_t bits = marks[at >> 3] >> (at & 7) & ((1u << kPer) - 1);
                 if (bits == 0) continue;         // (nearly always)
 #pragma unroll
@@ -567,8 +576,8 @@ struct TeacherRoom {
 };
 
 // The teacher's places of a row: tokens and log q (normalised over them where there is no tail)
-template <typename T, bool kWarp>
-__device__ __forceinline__ float teacher_of(const LogitsArgs& p, int64_t row, Team<kWarp>& team, TeacherRoom& r, int& used) {
+template <typename T, typename Team>
+__device__ __forceinline__ float teacher_of(const LogitsArgs& p, int64_t row, Team& team, TeacherRoom& r, int& used) {
     int n = 0;
     float m = kNone;
     for (int i = team.tid; i < p.places; i += team.threads) {
@@ -594,9 +603,9 @@ __device__ __forceinline__ float teacher_of(const LogitsArgs& p, int64_t row, Te
     return norm;
 }
 
-template <typename T, bool kWarp>
-__device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, const T* logits, Team<kWarp>& team,
-                                            TeacherRoom& r, Sums rest, float norm, int used) {
+// The row's loss and statistics, by a warp, from the student's sums over the other tokens
+__device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, Team<true>& team, const TeacherRoom& r, Sums rest,
+                                            float norm, int used) {
     // the student's sums over the teacher's tokens, each token once
     Sums best{kNone, 0.0f, 0.0f};
     float mass = 0.0f;
@@ -675,7 +684,7 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
     }
     if constexpr (kKind == kDistill) {
         for (int i = team.tid; i < p.marks / 4; i += team.threads) reinterpret_cast<uint32_t*>(marks)[i] = 0;
-        norm = teacher_of<T, kWarp>(p, at, team, teacher, used);
+        norm = teacher_of<T>(p, at, team, teacher, used);
         for (int i = team.tid; i < p.places; i += team.threads) {
             const int t = teacher.token[i];
             if (t < 0) continue;
@@ -762,7 +771,8 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
         sums.u = __shfl_sync(0xffffffffu, part.u, 0);
     }
     if constexpr (kKind == kDistill) {
-        distill_row<T, kWarp>(p, at, logits, team, teacher, sums, norm, used);
+        Team<true> warp{room, (int)threadIdx.x % 32, 32};
+        if (kWarp || team.tid < 32) distill_row(p, at, warp, teacher, sums, norm, used);
     } else {
         const float log_s = log2f(sums.s);
         const float entropy = sums.m == kNone ? 0.0f : kLn2 * (log_s - sums.u / sums.s);
