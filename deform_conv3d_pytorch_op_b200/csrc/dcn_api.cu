@@ -360,7 +360,11 @@ int dcn_debug_expire_wait(int32_t* gave_up, void* stream) {
     return dcn::tc_debug_expire_wait(gave_up, static_cast<cudaStream_t>(stream));
 }
 
-int dcn_check_status(void* stream) { return dcn::tc_check_status(static_cast<cudaStream_t>(stream)); }
+int dcn_check_status(void* stream) {
+    const int tc = dcn::tc_check_status(static_cast<cudaStream_t>(stream));
+    const int scan = dcn::seq::scan_check_status(static_cast<cudaStream_t>(stream));       // (both are read and cleared)
+    return tc != DCN_OK ? tc : scan;
+}
 
 // ------------------------------------------------------------------------------------------------
 // Deformable layer: offset-producing convolution + deformable convolution of the same input

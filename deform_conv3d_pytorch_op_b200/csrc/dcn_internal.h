@@ -121,4 +121,8 @@ int tc_launch_count(const Geom& g, int ndim, int deform, int pass);
 int tc_debug_points(const Geom& g, int ndim, int deform, const float* off, int n, float* coords, int32_t* valid,
                     int32_t* lo, int32_t* hi, void* ws, size_t ws_bytes, cudaStream_t st);
 
+namespace seq {
+int scan_check_status(cudaStream_t st);          // of the sequence operators, seq_scan.cu
+}
+
 }  // namespace dcn

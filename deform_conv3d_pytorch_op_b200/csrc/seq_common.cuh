@@ -202,6 +202,10 @@ __device__ __forceinline__ void copy_async(void* to, const void* from, bool in) 
                      "r"(in ? kBytes : 0)
                      : "memory");
 }
+template <int kBytes>
+__device__ __forceinline__ void copy_async_all(void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], %2;" ::"r"(shared_address(to)), "l"(from), "n"(kBytes) : "memory");
+}
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // all of the thread's groups but the `kLast` issued last
 template <int kLast>

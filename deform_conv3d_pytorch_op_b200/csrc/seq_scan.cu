@@ -6,8 +6,8 @@
 //
 // Both directions are scans of affine maps h -> A h + B, whose composition is (A2 A1, A2 B1 + B2).  A lane has a pair of channels,
 // in the packed float32 instructions, and kSteps steps of them: it composes its steps, the warps of a CTA (one behind the other
-// in time) compose theirs through shared memory and the CTAs of a cluster theirs through distributed shared memory; the state
-// that reaches a lane then gives all of its steps.  So x and gate are read once and y is written once, whatever the length: the
+// in time) compose theirs through shared memory and the CTAs of a cluster theirs through distributed shared memory, a warp for all;
+// the state that reaches a lane then gives all of its steps.  So x and gate are read once and y is written once, whatever the length: the
 // bound is DRAM.  A cluster walks the time axis in waves of (its CTAs) x 64 steps and carries the state from wave to wave in
 // registers.  Every warp copies its own steps of the next waves to shared memory meanwhile (cp.async, two stages), and sends its
 // results out from there: 16 bytes an instruction where addresses allow it, and no address arithmetic in the recurrence.
@@ -73,12 +73,82 @@ struct Product {
     }
 };
 
-// Maps in shared memory, by the part of a word that a lane reads
+// Maps in shared memory, of a lane each
 template <int W>
 struct MapRoom {
-    Lanes<W> v[3][32];
-    __device__ __forceinline__ void put(int lane, const Map<W>& m) { v[0][lane] = m.a, v[1][lane] = m.more, v[2][lane] = m.b; }
-    __device__ __forceinline__ Map<W> get(int lane) const { return {v[0][lane], v[1][lane], v[2][lane]}; }
+    static constexpr uint32_t kBytes = 3 * sizeof(Lanes<W>) * 32;
+    struct alignas(2 * sizeof(Lanes<W>)) Gate {
+        Lanes<W> a, more;
+    };
+    Gate gate[32];
+    Lanes<W> b[32];
+    __device__ __forceinline__ void put(int lane, const Map<W>& m) { gate[lane] = {m.a, m.more}, b[lane] = m.b; }
+    __device__ __forceinline__ Map<W> get(int lane) const {
+        const Gate g = gate[lane];
+        return {g.a, g.more, b[lane]};
+    }
+};
+
+// Set where a wait for a map of another CTA gave up (which nothing but a fault of the GPU brings about)
+__device__ unsigned int g_scan_status;
+constexpr long long kWaitCycles = 1ll << 32;                     // some two seconds
+
+// The exchange of maps in a cluster.  Each CTA sends its own to all (st.async, which counts its bytes on the barrier of the CTA it
+// goes to): a cluster barrier instead would hold every warp until its results of the wave before are in memory.  Two of
+// everything: a CTA sends a wave's map when all maps of the wave before have arrived, so the one it writes over has been read.
+struct Exchange {
+    MapRoom<2> maps[2][kCluster];
+    alignas(8) uint64_t arrived[2];
+    int gave_up;
+
+    __device__ __forceinline__ void begin(int thread) {
+        if (thread == 0) {
+            gave_up = 0;
+            for (int s = 0; s < 2; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&arrived[s])) : "memory");
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+    }
+    // by one thread a wave: so many maps will come
+    __device__ __forceinline__ void expect(int side, int ranks) {
+        asm volatile("{\n .reg .b64 s;\n mbarrier.arrive.expect_tx.shared::cta.b64 s, [%0], %1;\n}" ::"r"(
+                         shared_address(&arrived[side])),
+                     "r"(ranks * MapRoom<2>::kBytes)
+                     : "memory");
+    }
+    // my lane's of the CTA `rank`'s map, to the CTA `to`
+    __device__ __forceinline__ void send(int side, int rank, int to, int lane, const Map<2>& m) {
+        uint32_t gate, b, bar;
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(gate) : "r"(shared_address(&maps[side][rank].gate[lane])), "r"(to));
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(shared_address(&maps[side][rank].b[lane])), "r"(to));
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(shared_address(&arrived[side])), "r"(to));
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(gate), "l"(m.a.v),
+                     "l"(m.more.v), "r"(bar)
+                     : "memory");
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(b), "l"(m.b.v), "r"(bar)
+                     : "memory");
+    }
+    // until all maps of the n-th wave are there.  Bounded: a wait that gives up raises the status word, and the kernel runs to its
+    // end without waiting again.
+    __device__ __forceinline__ void wait(int side, int n) {
+        const uint32_t bar = shared_address(&arrived[side]), parity = n / 2 % 2;
+        long long began = 0;
+        for (;;) {
+            uint32_t ok;
+            asm volatile(
+                "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
+                : "=r"(ok)
+                : "r"(bar), "r"(parity)
+                : "memory");
+            if (ok || *(volatile int*)&gave_up) return;
+            const long long now = clock64();
+            if (began == 0) began = now;
+            if (now - began > kWaitCycles) {
+                *(volatile int*)&gave_up = 1;
+                atomicOr(&g_scan_status, 1u);
+                return;
+            }
+        }
+    }
 };
 
 // Where a thread works
@@ -127,8 +197,17 @@ struct Block {
     static __device__ __forceinline__ int col(int lane, int j) {
         return kCols <= 32 ? lane % kCols * kPer : (lane + 32 * (j % 2)) * kPer;
     }
+    static constexpr int kRows = kCols <= 32 ? 32 / kCols : 1;    // of one move
     // from step t0 on; zeros behind the sequence's end and the last channel
     __device__ __forceinline__ void fill(const T* base, int64_t t0, int64_t stride, int64_t len, int width, int lane) {
+        if (kBytes == 16 && kCols <= 32 && width == kTile && t0 + K <= len) {
+            const T* from = base + (t0 + row(lane, 0)) * stride + col(lane, 0);
+            T* to = &v[row(lane, 0)][col(lane, 0)];
+#pragma unroll
+            for (int j = 0; j < kMoves; ++j, from += kRows * stride)
+                copy_async_all<16>(to + j * kRows * kTile, from);
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < kMoves; ++j) {
             const int r = row(lane, j), c = col(lane, j);
@@ -146,6 +225,14 @@ struct Block {
     }
     // to the steps before `steps`
     __device__ __forceinline__ void drain(T* base, int64_t t0, int64_t stride, int64_t steps, int width, int lane) const {
+        if (kBytes == 16 && kCols <= 32 && width == kTile && t0 + K <= steps) {
+            T* to = base + (t0 + row(lane, 0)) * stride + col(lane, 0);
+            const T* from = &v[row(lane, 0)][col(lane, 0)];
+#pragma unroll
+            for (int j = 0; j < kMoves; ++j, to += kRows * stride)
+                store(to, *reinterpret_cast<const Raw<kBytes>*>(from + j * kRows * kTile));
+            return;
+        }
 #pragma unroll
         for (int j = 0; j < kMoves; ++j) {
             const int r = row(lane, j), c = col(lane, j);
@@ -195,8 +282,9 @@ template <typename T, int kBytes>
 struct ForwardRoom {
     static constexpr int K = kForwardSteps, kWarps = kChunk / K;
     Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps];
-    // maps of the warps and of the cluster's CTAs; two of each, so that a wave's are read while the next one's are written
-    MapRoom<2> part[2][kWarps], whole[2][kCluster];
+    MapRoom<2> part[kWarps];                     // of the warps
+    Lanes<2> start[kWarps][32];                  // the states before their steps
+    Exchange cluster;
 };
 
 template <typename T, int kBytes>
@@ -215,19 +303,19 @@ __global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward
     const int chunk = me.warps * K, wave = me.ranks * chunk;
     int64_t t0 = (int64_t)me.rank * chunk + me.warp * K;           // my first step of this wave
     int64_t begin = 0;
-    auto fill = [&](int side, int64_t t) {
-        if (t - me.rank * chunk - me.warp * K < len) {             // (a wave that does not come is not filled)
-            room.x[side][me.warp].fill(x, t, p.x_step, len, me.width, me.lane);
-            room.gate[side][me.warp].fill(gate, t, p.gate_step, len, me.width, me.lane);
-        }
-        copies_issued();
+    auto fill = [&](auto& block, const T* from, int64_t t, int64_t stride) {
+        if (t - me.rank * chunk - me.warp * K < len) block.fill(from, t, stride, len, me.width, me.lane);
+        copies_issued();                                           // (a wave that does not come is not filled)
     };
-    fill(0, t0);
-    fill(1, t0 + wave);
+    if (me.ranks > 1) room.cluster.begin(me.warp * 32 + me.lane);
+    for (int s = 0; s < 2; ++s) {
+        fill(room.gate[s][me.warp], gate, t0 + s * wave, p.gate_step);
+        fill(room.x[s][me.warp], x, t0 + s * wave, p.x_step);
+    }
     if (me.ranks > 1) cg::this_cluster().sync();                   // every CTA runs before another writes to its memory
-    for (int side = 0; begin < len; begin += wave, t0 += wave, side ^= 1) {
+    for (int side = 0, n = 0; begin < len; begin += wave, t0 += wave, side ^= 1, ++n) {
         auto &bx = room.x[side][me.warp], &bg = room.gate[side][me.warp];
-        copies_arrived<1>();
+        copies_arrived<2>();
         __syncwarp();
         // after each of my steps: y = A h + B of the state h before the first
         Lanes<2> A[K], B[K], sum = all_lanes<2>(0.0f);
@@ -246,39 +334,37 @@ __global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward
         };
         if (all) compose(std::true_type());
         else compose(std::false_type());
-        room.part[side][me.warp].put(me.lane, product.map(sum));
+        room.part[me.warp].put(me.lane, product.map(sum));
         __syncthreads();
-        Lanes<2> h = carry;
-        if (me.ranks > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            if (me.warp == 0) {
-                Product<2> all_of;
+        if (me.warp == 0) {
+            Lanes<2> h = carry;
+            if (me.ranks > 1) {
+                if (me.lane == 0) room.cluster.expect(side, me.ranks);
+                Product<2> product_of;
                 Lanes<2> s = all_lanes<2>(0.0f);
                 for (int w = 0; w < me.warps; ++w) {
-                    const Map<2> m = room.part[side][w].get(me.lane);
-                    all_of.by(m);
+                    const Map<2> m = room.part[w].get(me.lane);
+                    product_of.by(m);
                     s = m(s);
                 }
-                const Map<2> m = all_of.map(s);
-                for (int r = 0; r < me.ranks; ++r) cluster.map_shared_rank(&room.whole[side][me.rank], r)->put(me.lane, m);
+                const Map<2> m = product_of.map(s);
+                for (int r = 0; r < me.ranks; ++r) room.cluster.send(side, me.rank, r, me.lane, m);
+                room.cluster.wait(side, n);
+                for (int r = 0; r < me.ranks; ++r) {
+                    if (r == me.rank) h = carry;
+                    carry = room.cluster.maps[side][r].get(me.lane)(carry);
+                }
             }
-            cluster.sync();
-            for (int r = 0; r < me.ranks; ++r) {
-                if (r == me.rank) h = carry;
-                carry = room.whole[side][r].get(me.lane)(carry);
+            if (p.checkpoints != nullptr && t0 < len) me.store(p.checkpoints, me.b * p.chunks + t0 / kChunk, p.channels, h);
+            for (int w = 0; w < me.warps; ++w) {
+                room.start[w][me.lane] = h;
+                h = room.part[w].get(me.lane)(h);
             }
+            if (me.ranks == 1) carry = h;
         }
-        if (p.checkpoints != nullptr && me.warp == 0 && t0 < len) me.store(p.checkpoints, me.b * p.chunks + t0 / kChunk, p.channels, h);
-        // from the state before the CTA's steps to the one before mine; a CTA by itself also finds the state behind them here
-        Lanes<2> mine = h;
-        for (int w = 0; w < me.warps; ++w) {
-            if (w == me.warp) {
-                mine = h;
-                if (me.ranks > 1) break;
-            }
-            h = room.part[side][w].get(me.lane)(h);
-        }
-        if (me.ranks == 1) carry = h;
+        fill(bg, gate, t0 + 2 * wave, p.gate_step);
+        __syncthreads();
+        const Lanes<2> mine = room.start[me.warp][me.lane];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             Lanes<2> v = fma(A[k], mine, B[k]);
@@ -288,9 +374,10 @@ __global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward
         __syncwarp();
         bx.drain(y, t0, p.channels, p.steps, me.width, me.lane);
         __syncwarp();
-        fill(side, t0 + 2 * wave);
+        fill(bx, x, t0 + 2 * wave, p.x_step);
     }
     copies_arrived<0>();
+    if (me.ranks > 1) cg::this_cluster().sync();                   // (no CTA ends while another could still send to it)
     zero_rest(me, y, begin, p.steps, p.channels);
     if (me.rank == 0 && me.warp == 0) me.store(p.last, me.b, p.channels, carry);
 }
@@ -299,8 +386,10 @@ template <typename T, int kBytes>
 struct BackwardRoom {
     static constexpr int K = kBackwardSteps, kWarps = kChunk / K;
     Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps], dy[2][kWarps];
-    MapRoom<2> part[2][kWarps], whole[2][kCluster];
-    Lanes<2> back[2][kWarps][32];                // the b of the warps' backward maps p -> A p + b, which have the forward ones' A
+    MapRoom<2> part[kWarps];
+    Lanes<2> back[kWarps][32];                   // the b of the warps' backward maps p -> A p + b, which have the forward ones' A
+    Lanes<2> start[kWarps][32], end[kWarps][32]; // the states before their steps, and the gradients behind them
+    Exchange cluster;
 };
 
 template <typename T, int kBytes>
@@ -330,14 +419,12 @@ __global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backwa
         }
         copies_issued();
     };
+    if (me.ranks > 1) room.cluster.begin(me.warp * 32 + me.lane);
     fill(0, t0);
     fill(1, t0 - wave);
     if (me.ranks > 1) cg::this_cluster().sync();                   // every CTA runs before another writes to its memory
-    for (int side = 0; begin >= 0; begin -= wave, t0 -= wave, side ^= 1) {
+    for (int side = 0, n = 0; begin >= 0; begin -= wave, t0 -= wave, side ^= 1, ++n) {
         auto &bx = room.x[side][me.warp], &bg = room.gate[side][me.warp], &bd = room.dy[side][me.warp];
-        // the state before the CTA's steps
-        const int64_t first = t0 - me.warp * K;
-        Lanes<2> h = me.load(first < len ? p.checkpoints : nullptr, me.b * p.chunks + first / kChunk, p.channels);
         copies_arrived<1>();
         __syncwarp();
         Lanes<2> a[K], keep[K], before[K], sum = all_lanes<2>(0.0f), passed = sum;
@@ -355,44 +442,49 @@ __global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backwa
         else compose(std::false_type());
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) passed = a[k] * (bd.at(k, me.lane) + passed);
-        room.part[side][me.warp].put(me.lane, product.map(sum));
-        room.back[side][me.warp][me.lane] = passed;
+        room.part[me.warp].put(me.lane, product.map(sum));
+        room.back[me.warp][me.lane] = passed;
         __syncthreads();
-        auto back_map = [&](int w) {
-            Map<2> m = room.part[side][w].get(me.lane);
-            m.b = room.back[side][w][me.lane];
-            return m;
-        };
-        Lanes<2> g = carry;                                        // the gradient that reaches the CTA's last step
-        if (me.ranks > 1) {
-            cg::cluster_group cluster = cg::this_cluster();
-            if (me.warp == 0) {
-                Product<2> all_of;
+        if (me.warp == (me.warps > 1 ? 1 : 0)) {                   // the states, from the one before the CTA's steps
+            const int64_t first = t0 - me.warp * K;
+            Lanes<2> h = me.load(first < len ? p.checkpoints : nullptr, me.b * p.chunks + first / kChunk, p.channels);
+            for (int w = 0; w < me.warps; ++w) {
+                room.start[w][me.lane] = h;
+                h = room.part[w].get(me.lane)(h);
+            }
+        }
+        if (me.warp == 0) {                                        // the gradients, from the one that reaches the CTA's last step
+            auto back_map = [&](int w) {
+                Map<2> m = room.part[w].get(me.lane);
+                m.b = room.back[w][me.lane];
+                return m;
+            };
+            Lanes<2> g = carry;
+            if (me.ranks > 1) {
+                if (me.lane == 0) room.cluster.expect(side, me.ranks);
+                Product<2> product_of;
                 Lanes<2> s = all_lanes<2>(0.0f);
                 for (int w = me.warps - 1; w >= 0; --w) {
                     const Map<2> m = back_map(w);
-                    all_of.by(m);
+                    product_of.by(m);
                     s = m(s);
                 }
-                const Map<2> m = all_of.map(s);
-                for (int r = 0; r < me.ranks; ++r) cluster.map_shared_rank(&room.whole[side][me.rank], r)->put(me.lane, m);
+                const Map<2> m = product_of.map(s);
+                for (int r = 0; r < me.ranks; ++r) room.cluster.send(side, me.rank, r, me.lane, m);
+                room.cluster.wait(side, n);
+                for (int r = me.ranks - 1; r >= 0; --r) {
+                    if (r == me.rank) g = carry;
+                    carry = room.cluster.maps[side][r].get(me.lane)(carry);
+                }
             }
-            cluster.sync();
-            for (int r = me.ranks - 1; r >= 0; --r) {
-                if (r == me.rank) g = carry;
-                carry = room.whole[side][r].get(me.lane)(carry);
+            for (int w = me.warps - 1; w >= 0; --w) {
+                room.end[w][me.lane] = g;
+                g = back_map(w)(g);
             }
+            if (me.ranks == 1) carry = g;
         }
-        for (int w = 0; w < me.warp; ++w) h = room.part[side][w].get(me.lane)(h);
-        Lanes<2> mine = g;
-        for (int w = me.warps - 1; w >= 0; --w) {
-            if (w == me.warp) {
-                mine = g;
-                if (me.ranks > 1) break;
-            }
-            g = back_map(w)(g);
-        }
-        if (me.ranks == 1) carry = g;
+        __syncthreads();
+        Lanes<2> h = room.start[me.warp][me.lane], mine = room.end[me.warp][me.lane];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             before[k] = h;
@@ -414,6 +506,7 @@ __global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backwa
         fill(side, t0 - 2 * wave);
     }
     copies_arrived<0>();
+    if (me.ranks > 1) cg::this_cluster().sync();                   // (no CTA ends while another could still send to it)
     zero_rest(me, dx, end, p.steps, p.channels);
     zero_rest(me, dgate, end, p.steps, p.channels);
     if (p.dstate != nullptr && me.rank == 0 && me.warp == 0) me.store(p.dstate, me.b, p.channels, carry);
@@ -541,6 +634,16 @@ ScanArgs args_of(const dcn_scan* p) {
 }
 
 }  // namespace
+
+int scan_check_status(cudaStream_t st) {
+    unsigned int v = 0;
+    if (cudaStreamSynchronize(st) != cudaSuccess || cudaMemcpyFromSymbol(&v, g_scan_status, sizeof(v)) != cudaSuccess) return DCN_ERR_CUDA;
+    if (v == 0) return DCN_OK;
+    const unsigned int zero = 0;
+    cudaMemcpyToSymbol(g_scan_status, &zero, sizeof(zero));
+    return DCN_ERR_TIMEOUT;
+}
+
 }  // namespace seq
 }  // namespace dcn
 
