@@ -73,6 +73,9 @@ struct Product {
     }
 };
 
+template <int W>
+__device__ __forceinline__ Map<W> identity() { return {all_lanes<W>(1.0f), all_lanes<W>(0.0f), all_lanes<W>(0.0f)}; }
+
 // Maps in shared memory, of a lane each
 template <int W>
 struct MapRoom {
@@ -101,8 +104,10 @@ struct Exchange {
     alignas(8) uint64_t arrived[2];
     int gave_up;
 
-    __device__ __forceinline__ void begin(int thread) {
-        if (thread == 0) {
+    // by warp 0; the places of CTAs that are not there hold maps that change nothing
+    __device__ __forceinline__ void begin(int lane, int ranks) {
+        for (int r = ranks; r < kCluster; ++r) maps[0][r].put(lane, identity<2>()), maps[1][r].put(lane, identity<2>());
+        if (lane == 0) {
             gave_up = 0;
             for (int s = 0; s < 2; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&arrived[s])) : "memory");
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -115,17 +120,24 @@ struct Exchange {
                      "r"(ranks * MapRoom<2>::kBytes)
                      : "memory");
     }
-    // my lane's of the CTA `rank`'s map, to the CTA `to`
+    // my lane's part of the map of the CTA `rank`, to the CTA `to`
     __device__ __forceinline__ void send(int side, int rank, int to, int lane, const Map<2>& m) {
-        uint32_t gate, b, bar;
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(gate) : "r"(shared_address(&maps[side][rank].gate[lane])), "r"(to));
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(shared_address(&maps[side][rank].b[lane])), "r"(to));
-        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(bar) : "r"(shared_address(&arrived[side])), "r"(to));
+        uint32_t there;                          // this object, in that CTA
+        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(shared_address(this)), "r"(to));
+        const uint32_t here = shared_address(this), bar = there + shared_address(&arrived[side]) - here;
+        const uint32_t gate = there + shared_address(&maps[side][rank].gate[lane]) - here,
+                       b = there + shared_address(&maps[side][rank].b[lane]) - here;
         asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(gate), "l"(m.a.v),
                      "l"(m.more.v), "r"(bar)
                      : "memory");
         asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(b), "l"(m.b.v), "r"(bar)
                      : "memory");
+    }
+    __device__ __forceinline__ void send_all(int side, int rank, int ranks, int lane, const Map<2>& m) {
+        if (lane == 0) expect(side, ranks);
+#pragma unroll
+        for (int r = 0; r < kCluster; ++r)
+            if (r < ranks) send(side, rank, r, lane, m);
     }
     // until all maps of the n-th wave are there.  Bounded: a wait that gives up raises the status word, and the kernel runs to its
     // end without waiting again.
@@ -289,7 +301,7 @@ struct ForwardRoom {
 
 template <typename T, int kBytes>
 __global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward_kernel(const ScanArgs p) {
-    constexpr int K = kForwardSteps;
+    constexpr int K = kForwardSteps, kWarps = kChunk / K;
     extern __shared__ __align__(16) unsigned char dynamic[];
     auto& room = *reinterpret_cast<ForwardRoom<T, kBytes>*>(dynamic);
     const Place me(p);
@@ -307,7 +319,12 @@ __global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward
         if (t - me.rank * chunk - me.warp * K < len) block.fill(from, t, stride, len, me.width, me.lane);
         copies_issued();                                           // (a wave that does not come is not filled)
     };
-    if (me.ranks > 1) room.cluster.begin(me.warp * 32 + me.lane);
+    if (me.warp == 0) {
+        if (me.ranks > 1) room.cluster.begin(me.lane, me.ranks);
+        for (int w = me.warps; w < kWarps; ++w) {                  // (warps that are not there change nothing)
+            room.part[w].put(me.lane, identity<2>());
+        }
+    }
     for (int s = 0; s < 2; ++s) {
         fill(room.gate[s][me.warp], gate, t0 + s * wave, p.gate_step);
         fill(room.x[s][me.warp], x, t0 + s * wave, p.x_step);
@@ -339,24 +356,25 @@ __global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward
         if (me.warp == 0) {
             Lanes<2> h = carry;
             if (me.ranks > 1) {
-                if (me.lane == 0) room.cluster.expect(side, me.ranks);
                 Product<2> product_of;
                 Lanes<2> s = all_lanes<2>(0.0f);
-                for (int w = 0; w < me.warps; ++w) {
+#pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
                     const Map<2> m = room.part[w].get(me.lane);
                     product_of.by(m);
                     s = m(s);
                 }
-                const Map<2> m = product_of.map(s);
-                for (int r = 0; r < me.ranks; ++r) room.cluster.send(side, me.rank, r, me.lane, m);
+                room.cluster.send_all(side, me.rank, me.ranks, me.lane, product_of.map(s));
                 room.cluster.wait(side, n);
-                for (int r = 0; r < me.ranks; ++r) {
+#pragma unroll
+                for (int r = 0; r < kCluster; ++r) {
                     if (r == me.rank) h = carry;
                     carry = room.cluster.maps[side][r].get(me.lane)(carry);
                 }
             }
             if (p.checkpoints != nullptr && t0 < len) me.store(p.checkpoints, me.b * p.chunks + t0 / kChunk, p.channels, h);
-            for (int w = 0; w < me.warps; ++w) {
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
                 room.start[w][me.lane] = h;
                 h = room.part[w].get(me.lane)(h);
             }
@@ -394,7 +412,7 @@ struct BackwardRoom {
 
 template <typename T, int kBytes>
 __global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backward_kernel(const ScanArgs p) {
-    constexpr int K = kBackwardSteps;
+    constexpr int K = kBackwardSteps, kWarps = kChunk / K;
     extern __shared__ __align__(16) unsigned char dynamic[];
     auto& room = *reinterpret_cast<BackwardRoom<T, kBytes>*>(dynamic);
     const Place me(p);
@@ -419,7 +437,13 @@ __global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backwa
         }
         copies_issued();
     };
-    if (me.ranks > 1) room.cluster.begin(me.warp * 32 + me.lane);
+    if (me.warp == 0) {
+        if (me.ranks > 1) room.cluster.begin(me.lane, me.ranks);
+        for (int w = me.warps; w < kWarps; ++w) {                  // (warps that are not there change nothing)
+            room.part[w].put(me.lane, identity<2>());
+            room.back[w][me.lane] = all_lanes<2>(0.0f);
+        }
+    }
     fill(0, t0);
     fill(1, t0 - wave);
     if (me.ranks > 1) cg::this_cluster().sync();                   // every CTA runs before another writes to its memory
@@ -448,7 +472,8 @@ __global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backwa
         if (me.warp == (me.warps > 1 ? 1 : 0)) {                   // the states, from the one before the CTA's steps
             const int64_t first = t0 - me.warp * K;
             Lanes<2> h = me.load(first < len ? p.checkpoints : nullptr, me.b * p.chunks + first / kChunk, p.channels);
-            for (int w = 0; w < me.warps; ++w) {
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
                 room.start[w][me.lane] = h;
                 h = room.part[w].get(me.lane)(h);
             }
@@ -461,23 +486,24 @@ __global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backwa
             };
             Lanes<2> g = carry;
             if (me.ranks > 1) {
-                if (me.lane == 0) room.cluster.expect(side, me.ranks);
                 Product<2> product_of;
                 Lanes<2> s = all_lanes<2>(0.0f);
-                for (int w = me.warps - 1; w >= 0; --w) {
+#pragma unroll
+                for (int w = kWarps - 1; w >= 0; --w) {
                     const Map<2> m = back_map(w);
                     product_of.by(m);
                     s = m(s);
                 }
-                const Map<2> m = product_of.map(s);
-                for (int r = 0; r < me.ranks; ++r) room.cluster.send(side, me.rank, r, me.lane, m);
+                room.cluster.send_all(side, me.rank, me.ranks, me.lane, product_of.map(s));
                 room.cluster.wait(side, n);
-                for (int r = me.ranks - 1; r >= 0; --r) {
+#pragma unroll
+                for (int r = kCluster - 1; r >= 0; --r) {
                     if (r == me.rank) g = carry;
                     carry = room.cluster.maps[side][r].get(me.lane)(carry);
                 }
             }
-            for (int w = me.warps - 1; w >= 0; --w) {
+#pragma unroll
+            for (int w = kWarps - 1; w >= 0; --w) {
                 room.end[w][me.lane] = g;
                 g = back_map(w)(g);
             }
