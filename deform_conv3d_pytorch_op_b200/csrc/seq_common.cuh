@@ -43,6 +43,11 @@ __device__ __forceinline__ void load(Raw<16>& r, const void* p) {
 __device__ __forceinline__ void load_kept(Raw<16>& r, const void* p) {
     asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "l"(p));
 }
+// From shared memory, each time anew
+__device__ __forceinline__ void load_shared(Raw<16>& r, const void* p) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+}
 __device__ __forceinline__ void store(void* p, const Raw<2>& r) { *static_cast<uint16_t*>(p) = r.u; }
 __device__ __forceinline__ void store(void* p, const Raw<4>& r) { *static_cast<uint32_t*>(p) = r.u[0]; }
 __device__ __forceinline__ void store(void* p, const Raw<8>& r) { *static_cast<uint2*>(p) = make_uint2(r.u[0], r.u[1]); }

@@ -74,48 +74,64 @@ struct Rows {
     unsigned char* room;                         // mine of the first vector
     int width;                                   // bytes from one vector of a thread to its next: of the CTA's threads
     int stage = 0;
+    bool first = true;
+    Slice<T, V> here[kStaged ? 1 : kTensors];    // the row's, where it is not in shared memory
     static constexpr int kBytes = kStaged ? 2 * kTensors * L::kVectors * 16 : 0;       // of a thread: two rows
     __device__ __forceinline__ unsigned char* place(int s, int t, int i) const {
         return room + ((s * kTensors + t) * L::kVectors + i) * width;
     }
     __device__ __forceinline__ void fetch(int s, int64_t row) {
         if (row < rows) {
+            const bool whole = channels == threads * L::kPer;
 #pragma unroll
             for (int t = 0; t < kTensors; ++t) {
-                const T* from = base[t] + row * stride[t];
+                if (base[t] == nullptr) continue;
+                const T* from = base[t] + row * stride[t] + L::element(j, threads, 0);
 #pragma unroll
-                for (int i = 0; i < L::kVectors; ++i) {
-                    const int c = L::element(j, threads, i * V);
-                    const bool in = base[t] != nullptr && c < channels;
-                    copy_async<16>(place(s, t, i), in ? from + c : base[0], in);
+                for (int i = 0; i < L::kVectors; ++i, from += threads * V) {
+                    if (whole) copy_async_all<16>(place(s, t, i), from);
+                    else if (L::element(j, threads, i * V) < channels) copy_async<16>(place(s, t, i), from, true);
+                    else copy_async<16>(place(s, t, i), base[t], false);
                 }
             }
         }
         copies_issued();
     }
-    // the row that next() gives first
+    // the row that next() goes to first
     __device__ __forceinline__ void begin(int64_t row) {
         if constexpr (kStaged) fetch(0, row);
     }
-    // row `row`, the next one since the last call or begin()
-    __device__ __forceinline__ void next(Slice<T, V> (&to)[kTensors], int64_t row) {
+    // to row `row`, the next one since the last call or begin()
+    __device__ __forceinline__ void next(int64_t row) {
         if constexpr (kStaged) {
+            stage = first ? 0 : stage ^ 1;
+            first = false;
             fetch(stage ^ 1, row + step);
             copies_arrived<1>();
-#pragma unroll
-            for (int t = 0; t < kTensors; ++t)
-#pragma unroll
-                for (int i = 0; i < L::kVectors; ++i) to[t].v[i].raw = *reinterpret_cast<const Raw<V * sizeof(T)>*>(place(stage, t, i));
-            stage ^= 1;
         } else {
 #pragma unroll
             for (int t = 0; t < kTensors; ++t)
 #pragma unroll
                 for (int i = 0; i < L::kVectors; ++i) {
                     const int c = L::element(j, threads, i * V);
-                    to[t].v[i].zero();
-                    if (base[t] != nullptr && c < channels) to[t].v[i].get(base[t] + row * stride[t] + c);
+                    here[t].v[i].zero();
+                    if (base[t] != nullptr && c < channels) here[t].v[i].get(base[t] + row * stride[t] + c);
                 }
+        }
+    }
+    // the row's elements of a tensor, until the next next(): from shared memory when they are asked for, so that registers hold
+    // no more than what is in use
+    __device__ __forceinline__ Slice<T, V> get(int t) const {
+        if constexpr (!kStaged) {
+            return here[t];
+        } else {
+            Slice<T, V> s;
+#pragma unroll
+            for (int i = 0; i < L::kVectors; ++i) {
+                if (base[t] == nullptr) s.v[i].zero();
+                else load_shared(s.v[i].raw, place(stage, t, i));
+            }
+            return s;
         }
     }
 };
@@ -225,13 +241,13 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
     if (me.group == 0) weights.put(p, me.j, me.threads);
     __syncthreads();
     for (int64_t row = first; row < p.rows; row += step) {
-        Slice<T, V> in[3];
-        rows.next(in, row);
-        const Slice<T, V>&x = in[0], &y = in[1], &g = in[2];
+        rows.next(row);
+        const Slice<T, V> x = rows.get(0);
         Lanes<2> s[L::kPairs], w[L::kPairs], sum = all_lanes<2>(0.0f);
         float r = 0.0f;
         if (p.block != nullptr) {
-            gates_of<T, V>(g, p.gate != nullptr, s);
+            const Slice<T, V> y = rows.get(1);
+            gates_of<T, V>(rows.get(2), p.gate != nullptr, s);
 #pragma unroll
             for (int i = 0; i < L::kPairs; ++i) sum = fma(y.pair(i), y.pair(i), sum);
             r = rsqrtf(row_sum(sum) * p.inv + p.eps);
@@ -293,12 +309,12 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
     for (int64_t row = first; row < p.rows; row += step) {
         const float r = next_r, q = next_q;
         fetch_stats(row + step);
-        Slice<T, V> in[5];
-        rows.next(in, row);
-        const Slice<T, V>&x = in[0], &y = in[1], &g = in[2], &ds = in[3], &dn = in[4];
+        rows.next(row);
+        const Slice<T, V> y = rows.get(1);
         const Lanes<2> rr = all_lanes<2>(r), qq = all_lanes<2>(q);
         Lanes<2> on[L::kPairs], sn[L::kPairs], d[L::kPairs], w[L::kPairs], sum = all_lanes<2>(0.0f);
-        gates_of<T, V>(g, p.gate != nullptr, on);
+        gates_of<T, V>(rows.get(2), p.gate != nullptr, on);
+        const Slice<T, V> x = rows.get(0);
         if (p.block != nullptr) {
             weights.get(0, w);
 #pragma unroll
@@ -307,6 +323,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
 #pragma unroll
             for (int i = 0; i < L::kPairs; ++i) sn[i] = x.pair(i) * qq;
         }
+        const Slice<T, V> dn = rows.get(4);
         weights.get(1, w);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) {
@@ -315,6 +332,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
             sum = fma(d[i], sn[i], sum);
         }
         const Lanes<2> m = all_lanes<2>(-row_sum(sum) * p.inv);
+        const Slice<T, V> ds = rows.get(3);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) d[i] = fma(qq, fma(sn[i], m, d[i]), ds.pair(i));
         put<T, V>(p.dx, row * p.channels, d, me.j, me.threads, p.channels);
@@ -333,6 +351,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
         for (int i = 0; i < L::kPairs; ++i) d[i] = rr * fma(y.pair(i) * rr, n, sn[i]);
         put<T, V>(p.dblock, row * p.channels, d, me.j, me.threads, p.channels);
         if (p.dgate != nullptr) {
+            const Slice<T, V> g = rows.get(2);
 #pragma unroll
             for (int i = 0; i < L::kPairs; ++i) {
                 float off[2], s;
