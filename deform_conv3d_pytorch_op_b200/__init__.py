@@ -4,7 +4,7 @@ Modules ``ConvOffset3d`` / ``ConvOffset2d`` / ``Conv2d`` / ``Conv3d`` (aliases `
 autograd Functions ``ConvOffset3dFunction`` / ``ConvOffset2dFunction`` / ``Conv2dFunction``; the reference's
 FFI call surface is in :mod:`legacy_ops`; all arithmetic runs in ``csrc/libdcn.so`` (C ABI: ``include/dcn.h``).
 What follows a video network's features -- recurrence over time, norms, distillation, scores -- is in :mod:`sequence`
-(C ABI: ``include/dcn_seq.h``).
+(C ABI: ``include/dcn_seq.h``); :mod:`video_sequence` runs them together.
 """
 from ._lib import DcnError, LIB_PATH
 from .functions import (Conv2dFunction, Conv3dFunction, ConvOffset2dFunction, ConvOffset3dFunction,

@@ -94,9 +94,13 @@ class R3D18Deform(nn.Module):
         self.stages = nn.Sequential(*stages)
         self.fc = nn.Linear(8 * w, num_classes)
 
-    def forward(self, x):
+    def features(self, x):
+        """[clips, 8 * width]: what the classifier sees of each clip."""
         x = self.stages(self.stem(x))
-        return self.fc(torch.flatten(F.adaptive_avg_pool3d(x, 1), 1))
+        return torch.flatten(F.adaptive_avg_pool3d(x, 1), 1)
+
+    def forward(self, x):
+        return self.fc(self.features(x))
 
 
 def shard(t: torch.Tensor, rank: int, world: int) -> torch.Tensor:
