@@ -146,6 +146,18 @@ __device__ __forceinline__ float weight_at(const void* w, int c, int wide) {
     return v.at(0);
 }
 
+// A thread's elements of a weight, all on their way before the first is used; ones where there is no weight
+template <typename W, typename T, int V>
+__device__ __forceinline__ void load_weight(Pack<W, 1> (&f)[Layout<T, V>::kPer], const void* w, int j, int threads, int channels) {
+#pragma unroll
+    for (int e = 0; e < Layout<T, V>::kPer; ++e) {
+        const int c = Layout<T, V>::element(j, threads, e);
+        const float one[1] = {1.0f};
+        f[e].set(one);
+        if (w != nullptr && c < channels) f[e].get(static_cast<const W*>(w) + c);
+    }
+}
+
 // scale post and pre of a row's threads, in shared memory: those of a thread four at a time
 template <typename T, int V>
 struct Weights {
@@ -153,20 +165,22 @@ struct Weights {
     static constexpr int kBytes = 2 * L::kPer * 4;          // of a thread
     float4* at;
     int width;
-    __device__ __forceinline__ void put(const NormArgs& p, int j, int threads) {
+    template <typename W>
+    __device__ __forceinline__ void put_as(const NormArgs& p, int j, int threads) {
+        Pack<W, 1> scale[L::kPer], post[L::kPer], pre[L::kPer];
+        load_weight<W, T, V>(scale, p.scale, j, threads, p.channels);
+        load_weight<W, T, V>(post, p.post, j, threads, p.channels);
+        load_weight<W, T, V>(pre, p.pre, j, threads, p.channels);
 #pragma unroll
-        for (int i = 0; i < L::kPer / 4; ++i) {
-            float f[2][4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int c = L::element(j, threads, 4 * i + k);
-                const bool in = c < p.channels;
-                f[0][k] = in ? weight_at<T>(p.scale, c, p.wide_weights) * weight_at<T>(p.post, c, p.wide_weights) : 0.0f;
-                f[1][k] = in ? weight_at<T>(p.pre, c, p.wide_weights) : 0.0f;
-            }
-#pragma unroll
-            for (int w = 0; w < 2; ++w) at[(w * (L::kPer / 4) + i) * width] = make_float4(f[w][0], f[w][1], f[w][2], f[w][3]);
+        for (int i = 0; i < L::kPer; i += 4) {
+            at[i / 4 * width] = make_float4(scale[i].at(0) * post[i].at(0), scale[i + 1].at(0) * post[i + 1].at(0),
+                                            scale[i + 2].at(0) * post[i + 2].at(0), scale[i + 3].at(0) * post[i + 3].at(0));
+            at[(L::kPer + i) / 4 * width] = make_float4(pre[i].at(0), pre[i + 1].at(0), pre[i + 2].at(0), pre[i + 3].at(0));
         }
+    }
+    __device__ __forceinline__ void put(const NormArgs& p, int j, int threads) {
+        if (p.wide_weights) put_as<float>(p, j, threads);
+        else put_as<T>(p, j, threads);
     }
     __device__ __forceinline__ void get(int which, Lanes<2> (&f)[L::kPairs]) const {
 #pragma unroll

@@ -30,7 +30,6 @@ namespace {
 
 constexpr int kTile = 64;                        // channels of a CTA: two a lane
 constexpr int kChunk = 64;                       // steps of a CTA in a wave, and between checkpoints
-constexpr int kForwardSteps = 16, kBackwardSteps = 8;       // of a thread: what its registers hold
 constexpr int kCluster = 8;                      // CTAs of a cluster, at most
 
 struct ScanArgs {
@@ -284,26 +283,31 @@ __device__ __forceinline__ void gates_of(const Pack<T, 2>& g, bool in, Lanes<2>&
 }
 
 // Zeros from step `from` on, shared out over the warps of the cluster
-template <typename T>
+template <typename T, int kBytes>
 __device__ __forceinline__ void zero_rest(const Place& me, T* out, int64_t from, int64_t steps, int64_t channels) {
-    for (int64_t t = from + me.rank * me.warps + me.warp; t < steps; t += me.ranks * me.warps)
-        for (int c = me.lane; c < me.width; c += 32) out[t * channels + c] = from_float<T>(0.0f);
+    using B = Block<T, kBytes, 1>;
+    constexpr int kRows = B::kRows;              // of a warp at a time
+    Raw<kBytes> zero;
+    memset(&zero, 0, sizeof(zero));
+    const int row = B::row(me.lane, 0);
+    for (int64_t t = from + (int64_t)(me.rank * me.warps + me.warp) * kRows + row; t < steps; t += (int64_t)me.ranks * me.warps * kRows)
+        for (int c = B::col(me.lane, 0); c < me.width; c += 32 * B::kPer) store(out + t * channels + c, zero);
 }
 
-template <typename T, int kBytes>
+template <typename T, int kBytes, int K>
 struct ForwardRoom {
-    static constexpr int K = kForwardSteps, kWarps = kChunk / K;
+    static constexpr int kWarps = kChunk / K;
     Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps];
     MapRoom<2> part[kWarps];                     // of the warps
     Lanes<2> start[kWarps][32];                  // the states before their steps
     Exchange cluster;
 };
 
-template <typename T, int kBytes>
-__global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward_kernel(const ScanArgs p) {
-    constexpr int K = kForwardSteps, kWarps = kChunk / K;
+template <typename T, int kBytes, int K>
+__global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(const ScanArgs p) {
+    constexpr int kWarps = kChunk / K;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    auto& room = *reinterpret_cast<ForwardRoom<T, kBytes>*>(dynamic);
+    auto& room = *reinterpret_cast<ForwardRoom<T, kBytes, K>*>(dynamic);
     const Place me(p);
     pdl_wait();
     const int64_t len = length_of(p, me.b);
@@ -396,13 +400,13 @@ __global__ void __launch_bounds__(32 * (kChunk / kForwardSteps), 4) scan_forward
     }
     copies_arrived<0>();
     if (me.ranks > 1) cg::this_cluster().sync();                   // (no CTA ends while another could still send to it)
-    zero_rest(me, y, begin, p.steps, p.channels);
+    zero_rest<T, kBytes>(me, y, begin, p.steps, p.channels);
     if (me.rank == 0 && me.warp == 0) me.store(p.last, me.b, p.channels, carry);
 }
 
-template <typename T, int kBytes>
+template <typename T, int kBytes, int K>
 struct BackwardRoom {
-    static constexpr int K = kBackwardSteps, kWarps = kChunk / K;
+    static constexpr int kWarps = kChunk / K;
     Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps], dy[2][kWarps];
     MapRoom<2> part[kWarps];
     Lanes<2> back[kWarps][32];                   // the b of the warps' backward maps p -> A p + b, which have the forward ones' A
@@ -410,11 +414,11 @@ struct BackwardRoom {
     Exchange cluster;
 };
 
-template <typename T, int kBytes>
-__global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backward_kernel(const ScanArgs p) {
-    constexpr int K = kBackwardSteps, kWarps = kChunk / K;
+template <typename T, int kBytes, int K>
+__global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backward_kernel(const ScanArgs p) {
+    constexpr int kWarps = kChunk / K;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    auto& room = *reinterpret_cast<BackwardRoom<T, kBytes>*>(dynamic);
+    auto& room = *reinterpret_cast<BackwardRoom<T, kBytes, K>*>(dynamic);
     const Place me(p);
     pdl_wait();
     const int64_t len = length_of(p, me.b);
@@ -533,8 +537,8 @@ __global__ void __launch_bounds__(32 * (kChunk / kBackwardSteps), 2) scan_backwa
     }
     copies_arrived<0>();
     if (me.ranks > 1) cg::this_cluster().sync();                   // (no CTA ends while another could still send to it)
-    zero_rest(me, dx, end, p.steps, p.channels);
-    zero_rest(me, dgate, end, p.steps, p.channels);
+    zero_rest<T, kBytes>(me, dx, end, p.steps, p.channels);
+    zero_rest<T, kBytes>(me, dgate, end, p.steps, p.channels);
     if (p.dstate != nullptr && me.rank == 0 && me.warp == 0) me.store(p.dstate, me.b, p.channels, carry);
 }
 
@@ -615,18 +619,32 @@ int launch_scan(K kernel, int held, size_t smem, int per_thread, const ScanArgs&
     return e != cudaSuccess || cudaGetLastError() != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
+template <typename T, int kBytes, int K>
+int forward_as(const ScanArgs& a, int64_t batch, cudaStream_t st) {
+    using Room = ForwardRoom<T, kBytes, K>;
+    const int held = resident<Room>(scan_forward_kernel<T, kBytes, K>, 32 * kChunk / K);
+    return launch_scan(scan_forward_kernel<T, kBytes, K>, held, sizeof(Room), K, a, batch, st);
+}
+
+template <typename T, int kBytes, int K>
+int backward_as(const ScanArgs& a, int64_t batch, cudaStream_t st) {
+    using Room = BackwardRoom<T, kBytes, K>;
+    const int held = resident<Room>(scan_backward_kernel<T, kBytes, K>, 32 * kChunk / K);
+    return launch_scan(scan_backward_kernel<T, kBytes, K>, held, sizeof(Room), K, a, batch, st);
+}
+
+// Steps of a thread, 16 or 8: with 16 the joining of maps costs half as much of a step, with 8 a thread has registers to spare.
+// Measured (us, 16 / 8): forward, bf16, 64x1024x2048 141 / 165, 2x16384x2048 101 / 141; float32, 2x8192x2048 82 / 86.
+// Backward, bf16, 64x1024x2048 265 / 314, 2x16384x2048 188 / 187, 24x777x1024 50 / 66; float32, 2x8192x2048 189 / 183,
+// 46x238x3008 210 / 166.
 template <typename T, int kBytes>
 int run_forward(const ScanArgs& a, int64_t batch, cudaStream_t st) {
-    using Room = ForwardRoom<T, kBytes>;
-    const int held = resident<Room>(scan_forward_kernel<T, kBytes>, 32 * kChunk / kForwardSteps);
-    return launch_scan(scan_forward_kernel<T, kBytes>, held, sizeof(Room), kForwardSteps, a, batch, st);
+    return forward_as<T, kBytes, 16>(a, batch, st);
 }
 
 template <typename T, int kBytes>
 int run_backward(const ScanArgs& a, int64_t batch, cudaStream_t st) {
-    using Room = BackwardRoom<T, kBytes>;
-    const int held = resident<Room>(scan_backward_kernel<T, kBytes>, 32 * kChunk / kBackwardSteps);
-    return launch_scan(scan_backward_kernel<T, kBytes>, held, sizeof(Room), kBackwardSteps, a, batch, st);
+    return backward_as<T, kBytes, sizeof(T) == 2 ? 16 : 8>(a, batch, st);
 }
 
 int check_scan(const dcn_scan* p) {
