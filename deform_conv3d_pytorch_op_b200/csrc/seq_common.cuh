@@ -48,6 +48,9 @@ __device__ __forceinline__ void load_shared(Raw<16>& r, const void* p) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "r"((uint32_t)__cvta_generic_to_shared(p)));
 }
+__device__ __forceinline__ void load_shared(Raw<4>& r, const void* p) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r.u[0]) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+}
 __device__ __forceinline__ void store(void* p, const Raw<2>& r) { *static_cast<uint16_t*>(p) = r.u; }
 __device__ __forceinline__ void store(void* p, const Raw<4>& r) { *static_cast<uint32_t*>(p) = r.u[0]; }
 __device__ __forceinline__ void store(void* p, const Raw<8>& r) { *static_cast<uint2*>(p) = make_uint2(r.u[0], r.u[1]); }
@@ -190,6 +193,10 @@ __device__ __forceinline__ Lanes<W> operator-(Lanes<W> a, Lanes<W> b) {
     return fma(b, all_lanes<W>(-1.0f), a);
 }
 
+__device__ __forceinline__ Lanes<2> shuffle_xor(Lanes<2> a, int o) {
+    return {__shfl_xor_sync(0xffffffffu, (unsigned long long)a.v, o)};
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -209,7 +216,10 @@ __device__ __forceinline__ void copy_async(void* to, const void* from, bool in) 
 }
 template <int kBytes>
 __device__ __forceinline__ void copy_async_all(void* to, const void* from) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], %2;" ::"r"(shared_address(to)), "l"(from), "n"(kBytes) : "memory");
+    if constexpr (kBytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(to)), "l"(from) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(shared_address(to)), "l"(from), "n"(kBytes) : "memory");
 }
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // all of the thread's groups but the `kLast` issued last

@@ -6,10 +6,10 @@
 //     dgate = dyn yn (1 - s(gate));   Z = sum over rows of ds s(gate) yn:  dscale = Z post, dpost = Z scale;   dpre = sum dnormed sn
 //
 // A row lives in the registers of a row of threads, 32 bytes of each tensor a thread, so that every tensor is read or written
-// once: the bound is DRAM.  A row of up to 32 threads (512 channels of 16 bits, 256 of float32) is a warp's, whose sums are shuffles
-// alone; above, a row is that of 64, 128, ... threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of the next row are on their way to its own
-// places in shared memory meanwhile (cp.async), where rows start on 16 bytes; elements of other rows are loaded one by one when
-// they are used.  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the
+// once: the bound is DRAM.  Rows of up to 32 threads (512 channels of 16 bits, 256 of float32) share a warp, and their sums are
+// shuffles alone; above, a row is that of 64, 128, ... threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of the next row are on their way to its own
+// places in shared memory meanwhile (cp.async, 16 or 4 bytes at a time, as rows start on them); rows of an odd number of 16-bit
+// elements are loaded one by one when they are used.  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the
 // arithmetic goes in pairs through the packed float32 instructions.  The CTAs of the backward pass keep Z and dpre in registers
 // and leave one partial sum each; a second kernel adds those in a fixed order.
 #include "seq_common.cuh"
@@ -74,9 +74,10 @@ struct Rows {
     unsigned char* room;                         // mine of the first vector
     int width;                                   // bytes from one vector of a thread to its next: of the CTA's threads
     int stage = 0;
-    bool first = true;
+    bool first = true, live = true;              // live: the row is there (rows of a warp end together)
     Slice<T, V> here[kStaged ? 1 : kTensors];    // the row's, where it is not in shared memory
-    static constexpr int kBytes = kStaged ? 2 * kTensors * L::kVectors * 16 : 0;       // of a thread: two rows
+    static constexpr int kMove = V * (int)sizeof(T);
+    static constexpr int kBytes = kStaged ? 2 * kTensors * L::kVectors * kMove : 0;    // of a thread: two rows
     __device__ __forceinline__ unsigned char* place(int s, int t, int i) const {
         return room + ((s * kTensors + t) * L::kVectors + i) * width;
     }
@@ -89,9 +90,9 @@ struct Rows {
                 const T* from = base[t] + row * stride[t] + L::element(j, threads, 0);
 #pragma unroll
                 for (int i = 0; i < L::kVectors; ++i, from += threads * V) {
-                    if (whole) copy_async_all<16>(place(s, t, i), from);
-                    else if (L::element(j, threads, i * V) < channels) copy_async<16>(place(s, t, i), from, true);
-                    else copy_async<16>(place(s, t, i), base[t], false);
+                    if (whole) copy_async_all<kMove>(place(s, t, i), from);
+                    else if (L::element(j, threads, i * V) < channels) copy_async<kMove>(place(s, t, i), from, true);
+                    else copy_async<kMove>(place(s, t, i), base[t], false);
                 }
             }
         }
@@ -103,6 +104,7 @@ struct Rows {
     }
     // to row `row`, the next one since the last call or begin()
     __device__ __forceinline__ void next(int64_t row) {
+        live = row < rows;
         if constexpr (kStaged) {
             stage = first ? 0 : stage ^ 1;
             first = false;
@@ -115,7 +117,7 @@ struct Rows {
                 for (int i = 0; i < L::kVectors; ++i) {
                     const int c = L::element(j, threads, i * V);
                     here[t].v[i].zero();
-                    if (base[t] != nullptr && c < channels) here[t].v[i].get(base[t] + row * stride[t] + c);
+                    if (live && base[t] != nullptr && c < channels) here[t].v[i].get(base[t] + row * stride[t] + c);
                 }
         }
     }
@@ -128,7 +130,7 @@ struct Rows {
             Slice<T, V> s;
 #pragma unroll
             for (int i = 0; i < L::kVectors; ++i) {
-                if (base[t] == nullptr) s.v[i].zero();
+                if (base[t] == nullptr || !live) s.v[i].zero();
                 else load_shared(s.v[i].raw, place(stage, t, i));
             }
             return s;
@@ -192,14 +194,18 @@ struct Weights {
     }
 };
 
-// The rows of threads of a CTA: 32 (kWarp) or more each
+// The rows of threads of a CTA: within warps (kWarp: up to 32 each), or of 64 and more.  The rows of a warp are walked together.
 template <bool kWarp>
 struct Team {
     int threads, j, group, groups;
-    __device__ __forceinline__ explicit Team(int threads_) : threads(kWarp ? 32 : threads_) {
+    __device__ __forceinline__ explicit Team(int threads_) : threads(threads_) {
         j = threadIdx.x % threads;
         group = threadIdx.x / threads;
         groups = blockDim.x / threads;
+    }
+    // the first row that a thread of the warp walks: the loop goes on as long as it is there
+    __device__ __forceinline__ int64_t warp_row(int64_t row) const {
+        return kWarp ? row - (threadIdx.x % 32) / threads : row;
     }
 };
 
@@ -211,8 +217,13 @@ struct RowSum {
     const Team<kWarp>& me;
     int side;
     __device__ __forceinline__ float operator()(Lanes<2> pair) {
-        float v = warp_sum(pair.at(0) + pair.at(1));
-        if constexpr (!kWarp) {
+        float v = pair.at(0) + pair.at(1);
+        if constexpr (kWarp) {
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1)
+                if (o < me.threads) v += __shfl_xor_sync(0xffffffffu, v, o);
+        } else {
+            v = warp_sum(v);
             const int warps = me.threads / 32;
             float* at = room[side] + me.group * warps;
             side ^= 1;
@@ -250,11 +261,11 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
     const int64_t first = (int64_t)blockIdx.x * me.groups + me.group, step = (int64_t)gridDim.x * me.groups;
     Rows<T, V, 3, kStaged> rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate)},
                                 {p.x_row, p.block_row, p.gate_row}, p.rows, step, me.j, me.threads, p.channels,
-                                dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * 16, (int)blockDim.x * 16};
+                                dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * V * sizeof(T), (int)(blockDim.x * V * sizeof(T))};
     rows.begin(first);
     if (me.group == 0) weights.put(p, me.j, me.threads);
     __syncthreads();
-    for (int64_t row = first; row < p.rows; row += step) {
+    for (int64_t row = first; me.warp_row(row) < p.rows; row += step) {
         rows.next(row);
         const Slice<T, V> x = rows.get(0);
         Lanes<2> s[L::kPairs], w[L::kPairs], sum = all_lanes<2>(0.0f);
@@ -272,7 +283,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
                 s[i] = fma(w[i] * s[i], y.pair(i) * all_lanes<2>(r), x.pair(i));
                 sum = fma(s[i], s[i], sum);
             }
-            put<T, V>(p.stream, row * p.channels, s, me.j, me.threads, p.channels);
+            put<T, V>(p.stream, row * p.channels, s, me.j, me.threads, rows.live ? p.channels : 0);
         } else {
 #pragma unroll
             for (int i = 0; i < L::kPairs; ++i) {
@@ -284,8 +295,8 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
         weights.get(1, w);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) s[i] = s[i] * all_lanes<2>(q) * w[i];
-        put<T, V>(p.normed, row * p.channels, s, me.j, me.threads, p.channels);
-        if (p.stats != nullptr && me.j == 0) {
+        put<T, V>(p.normed, row * p.channels, s, me.j, me.threads, rows.live ? p.channels : 0);
+        if (p.stats != nullptr && me.j == 0 && rows.live) {
             p.stats[2 * row] = r;
             p.stats[2 * row + 1] = q;
         }
@@ -306,7 +317,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
     Rows<T, V, 5, kStaged> rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate),
                                  static_cast<const T*>(p.dstream), static_cast<const T*>(p.dnormed)},
                                 {p.x_row, p.block_row, p.gate_row, p.dstream_row, p.dnormed_row}, p.rows, step, me.j, me.threads,
-                                p.channels, dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * 16, (int)blockDim.x * 16};
+                                p.channels, dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * V * sizeof(T), (int)(blockDim.x * V * sizeof(T))};
     rows.begin(first);
     if (me.group == 0) weights.put(p, me.j, me.threads);
     __syncthreads();
@@ -320,7 +331,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
         next_q = gload(p.stats + 2 * row + 1);
     };
     fetch_stats(first);
-    for (int64_t row = first; row < p.rows; row += step) {
+    for (int64_t row = first; me.warp_row(row) < p.rows; row += step) {
         const float r = next_r, q = next_q;
         fetch_stats(row + step);
         rows.next(row);
@@ -349,7 +360,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
         const Slice<T, V> ds = rows.get(3);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) d[i] = fma(qq, fma(sn[i], m, d[i]), ds.pair(i));
-        put<T, V>(p.dx, row * p.channels, d, me.j, me.threads, p.channels);
+        put<T, V>(p.dx, row * p.channels, d, me.j, me.threads, rows.live ? p.channels : 0);
         if (p.block == nullptr) continue;
         weights.get(0, w);
         sum = all_lanes<2>(0.0f);
@@ -363,7 +374,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
         const Lanes<2> n = all_lanes<2>(-row_sum(sum) * p.inv);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) d[i] = rr * fma(y.pair(i) * rr, n, sn[i]);
-        put<T, V>(p.dblock, row * p.channels, d, me.j, me.threads, p.channels);
+        put<T, V>(p.dblock, row * p.channels, d, me.j, me.threads, rows.live ? p.channels : 0);
         if (p.dgate != nullptr) {
             const Slice<T, V> g = rows.get(2);
 #pragma unroll
@@ -373,23 +384,33 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
                 logistic(g.at(2 * i + 1), s, off[1]);
                 d[i] = sn[i] * (y.pair(i) * rr) * lanes<2>(off);
             }
-            put<T, V>(p.dgate, row * p.channels, d, me.j, me.threads, p.channels);
+            put<T, V>(p.dgate, row * p.channels, d, me.j, me.threads, rows.live ? p.channels : 0);
         }
     }
     if constexpr (kStaged) copies_arrived<0>();
     if (p.partial == nullptr) return;
-    // the rows of threads add theirs up, in order (over the weights)
+    // the rows of threads add theirs up: those of a warp as a tree, the others in order (over the weights)
+    int rows_left = me.groups, mine = me.group;
+    if constexpr (kWarp) {
+#pragma unroll
+        for (int o = 16; o >= 4; o >>= 1) {
+            if (o < me.threads) break;
+#pragma unroll
+            for (int i = 0; i < L::kPairs; ++i) z[i] = z[i] + shuffle_xor(z[i], o), dpre[i] = dpre[i] + shuffle_xor(dpre[i], o);
+        }
+        rows_left = blockDim.x / 32, mine = threadIdx.x % 32 < me.threads ? threadIdx.x / 32 : -1;
+    }
     Lanes<2>* all = reinterpret_cast<Lanes<2>*>(dynamic) + me.j;
-    for (int k = 0; k < me.groups; ++k) {
+    for (int k = 0; k < rows_left; ++k) {
         __syncthreads();
-        if (k == me.group)
+        if (k == mine)
 #pragma unroll
             for (int i = 0; i < L::kPairs; ++i) {
                 if (k > 0) z[i] = all[2 * i * me.threads] + z[i], dpre[i] = all[(2 * i + 1) * me.threads] + dpre[i];
                 all[2 * i * me.threads] = z[i], all[(2 * i + 1) * me.threads] = dpre[i];
             }
     }
-    if (me.group != me.groups - 1) return;
+    if (mine != rows_left - 1) return;
     float* out = p.partial + (int64_t)blockIdx.x * 2 * p.channels;
 #pragma unroll
     for (int e = 0; e < L::kPer; ++e) {
@@ -429,9 +450,9 @@ __global__ void __launch_bounds__(1024) norm_weights_kernel(const float* partial
     }
 }
 
-// Threads of a row, a power of two; 32: a warp's
+// Threads of a row, a power of two
 int threads_of(int64_t channels, int elem) {
-    int t = 32;
+    int t = 4;
     while ((int64_t)t * (32 / elem) < channels) t *= 2;
     return t;
 }
@@ -460,8 +481,8 @@ template <typename T, int V, bool kWarp, int kMost>
 int run_as(const NormArgs& a, bool backward, cudaStream_t st) {
     // two rows of every tensor in shared memory where vectors are read, and an SM has room for as many threads
     constexpr int kSM = 227 * 1024, kWeights = Weights<T, V>::kBytes;
-    constexpr bool f = V > 1 && kMost * (Rows<T, V, 3, true>::kBytes + kWeights) <= kSM,
-                   b = V > 1 && kMost * (Rows<T, V, 5, true>::kBytes + kWeights) <= kSM;
+    constexpr bool f = V * sizeof(T) >= 4 && kMost * (Rows<T, V, 3, true>::kBytes + kWeights) <= kSM,
+                   b = V * sizeof(T) >= 4 && kMost * (Rows<T, V, 5, true>::kBytes + kWeights) <= kSM;
     const int cta = cta_of(a.threads);
     if (backward)
         return launch(norm_backward_kernel<T, V, kWarp, kMost, b>, grid_of(a.rows, a.channels, sizeof(T), kBackwardThreads), cta,
@@ -473,7 +494,7 @@ int run_as(const NormArgs& a, bool backward, cudaStream_t st) {
 template <typename T, int V>
 int run(NormArgs a, bool backward, cudaStream_t st) {
     a.threads = threads_of(a.channels, sizeof(T));
-    if (a.threads == 32) return run_as<T, V, true, 256>(a, backward, st);
+    if (a.threads <= 32) return run_as<T, V, true, 256>(a, backward, st);
     if (a.threads <= 256) return run_as<T, V, false, 256>(a, backward, st);
     if constexpr (sizeof(T) == 4)
         if (a.threads > 512) return run_as<T, V, false, 1024>(a, backward, st);
@@ -510,14 +531,24 @@ NormArgs args_of(const dcn_norm* p) {
     return a;
 }
 
-int run_any(int dtype, bool vec, const NormArgs& a, bool backward, cudaStream_t st) {
-    if (dtype == DCN_SEQ_F32) return vec ? run<float, 4>(a, backward, st) : run<float, 1>(a, backward, st);
-    if (dtype == DCN_SEQ_BF16) return vec ? run<__nv_bfloat16, 8>(a, backward, st) : run<__nv_bfloat16, 1>(a, backward, st);
-    return vec ? run<__half, 8>(a, backward, st) : run<__half, 1>(a, backward, st);
-}
+// Elements moved at once: 16 bytes where every row of every tensor starts on one, pairs of 16-bit elements where they start on
+// 4, one otherwise.
+struct Vector {
+    int n, elem;
+    explicit Vector(const dcn_norm* p) : n(16 / elem_bytes(p->dtype)), elem(elem_bytes(p->dtype)) {}
+    void by(const void* v, int64_t row) {
+        while (v != nullptr && n > 1 && (!aligned(v, n * elem) || row % n != 0)) n = n == 8 ? 2 : 1;
+    }
+};
 
-// 16-byte vectors where every row of `v` starts on one
-bool wide(const void* v, int64_t row, int per) { return v == nullptr || (aligned(v, 16) && row % per == 0); }
+int run_any(int dtype, int n, const NormArgs& a, bool backward, cudaStream_t st) {
+    if (dtype == DCN_SEQ_F32) return n == 4 ? run<float, 4>(a, backward, st) : run<float, 1>(a, backward, st);
+    if (dtype == DCN_SEQ_BF16)
+        return n == 8   ? run<__nv_bfloat16, 8>(a, backward, st)
+               : n == 2 ? run<__nv_bfloat16, 2>(a, backward, st)
+                        : run<__nv_bfloat16, 1>(a, backward, st);
+    return n == 8 ? run<__half, 8>(a, backward, st) : n == 2 ? run<__half, 2>(a, backward, st) : run<__half, 1>(a, backward, st);
+}
 
 }  // namespace
 }  // namespace seq
@@ -531,7 +562,7 @@ extern "C" int dcn_norm_forward(const dcn_norm* p, const void* x, const void* bl
     if (bad != DCN_OK) return bad;
     if (p->rows == 0) return DCN_OK;
     if (x == nullptr || normed == nullptr || (block != nullptr) != (stream_out != nullptr)) return DCN_ERR_NULL;
-    const int e = elem_bytes(p->dtype), we = elem_bytes(p->weight_dtype), per = 16 / e;
+    const int e = elem_bytes(p->dtype), we = elem_bytes(p->weight_dtype);
     for (const void* v : {x, block, gate, (const void*)stream_out, (const void*)normed})
         if (!aligned(v, e)) return DCN_ERR_ALIGN;
     for (const void* v : {scale, post, pre})
@@ -540,10 +571,11 @@ extern "C" int dcn_norm_forward(const dcn_norm* p, const void* x, const void* bl
     NormArgs a = args_of(p);
     a.x = x, a.block = block, a.gate = block != nullptr ? gate : nullptr, a.scale = scale, a.post = post, a.pre = pre;
     a.stream = stream_out, a.normed = normed, a.stats = stats;
-    const bool vec = p->channels % per == 0 && wide(x, p->x_row, per) && wide(block, p->block_row, per) &&
-                     wide(a.gate, p->gate_row, per) && wide(stream_out, 0, per) && wide(normed, 0, per);
+    Vector vec(p);
+    vec.by(x, p->x_row), vec.by(block, p->block_row), vec.by(a.gate, p->gate_row);
+    vec.by(stream_out, p->channels), vec.by(normed, p->channels);          // (so the channels are whole vectors too)
     const cudaStream_t st = (cudaStream_t)stream;
-    return run_any(p->dtype, vec, a, false, st);
+    return run_any(p->dtype, vec.n, a, false, st);
 }
 
 extern "C" size_t dcn_norm_workspace_bytes(const dcn_norm* p) {
@@ -559,7 +591,7 @@ extern "C" int dcn_norm_backward(const dcn_norm* p, const void* x, const void* b
     if (bad != DCN_OK) return bad;
     const bool weights = dscale != nullptr || dpost != nullptr || dpre != nullptr;
     const cudaStream_t st = (cudaStream_t)stream;
-    const int e = elem_bytes(p->dtype), we = elem_bytes(p->weight_dtype), per = 16 / e;
+    const int e = elem_bytes(p->dtype), we = elem_bytes(p->weight_dtype);
     for (const void* v : {scale, post, pre, (const void*)dscale, (const void*)dpost, (const void*)dpre})
         if (!aligned(v, we)) return DCN_ERR_ALIGN;
     if (p->rows == 0) {
@@ -580,10 +612,12 @@ extern "C" int dcn_norm_backward(const dcn_norm* p, const void* x, const void* b
     a.stats = const_cast<float*>(stats), a.dstream = dstream, a.dnormed = dnormed;
     a.dx = dx, a.dblock = dblock, a.dgate = dgate;
     a.partial = weights ? static_cast<float*>(workspace) : nullptr;
-    const bool vec = p->channels % per == 0 && wide(x, p->x_row, per) && wide(block, p->block_row, per) &&
-                     wide(a.gate, p->gate_row, per) && wide(dstream, p->dstream_row, per) &&
-                     wide(dnormed, p->dnormed_row, per) && wide(dx, 0, per) && wide(dblock, 0, per) && wide(dgate, 0, per);
-    const int rc = run_any(p->dtype, vec, a, true, st);
+    Vector vec(p);
+    vec.by(x, p->x_row), vec.by(block, p->block_row), vec.by(a.gate, p->gate_row);
+    vec.by(dstream, p->dstream_row), vec.by(dnormed, p->dnormed_row);
+    vec.by(x, p->channels);                      // (channels are whole vectors)
+    vec.by(dx, p->channels), vec.by(dblock, p->channels), vec.by(dgate, p->channels);
+    const int rc = run_any(p->dtype, vec.n, a, true, st);
     if (rc != DCN_OK || !weights) return rc;
     if (p->dtype == DCN_SEQ_F32) return run_weights<float>(a, e, dscale, dpost, dpre, st);
     if (p->dtype == DCN_SEQ_BF16) return run_weights<__nv_bfloat16>(a, e, dscale, dpost, dpre, st);
