@@ -58,6 +58,11 @@ __device__ __forceinline__ void store(void* p, const Raw<16>& r) {
     *static_cast<uint4*>(p) = make_uint4(r.u[0], r.u[1], r.u[2], r.u[3]);
 }
 
+// A result that is not read again soon: it does not push out of L2 what is
+__device__ __forceinline__ void store_streaming(void* p, const Raw<16>& r) {
+    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(r.u[0]), "r"(r.u[1]), "r"(r.u[2]), "r"(r.u[3]) : "memory");
+}
+
 __device__ __forceinline__ int64_t gload_i64(const int64_t* p) {
     long long r;
     asm volatile("ld.global.s64 %0, [%1];" : "=l"(r) : "l"(p));

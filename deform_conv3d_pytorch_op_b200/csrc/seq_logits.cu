@@ -833,14 +833,17 @@ struct Slope {
     }
 };
 
-template <typename T, bool kDistilled>
-__global__ void __launch_bounds__(kThreads) logits_backward_kernel(const LogitsArgs p, int parts) {
+// kStream: the gradient's rows are whole 32-byte sectors, which then need not be kept in L2 (of others the rest comes from another
+// warp, and sending them off early costs a second write)
+template <typename T, bool kDistilled, bool kStream>
+__global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const LogitsArgs p, int parts) {
     constexpr int kPer = Row<T>::kPer;
     __shared__ int token[kMostTop + 1];
     __shared__ float weight[kMostTop + 1];
     __shared__ float2 room[2][32];
     const int tid = threadIdx.x, threads = blockDim.x;
-    const int64_t at = blockIdx.x / parts;
+    // the rows that were read last come first: in a loss, whose backward pass follows its forward pass, they are still in L2
+    const int64_t at = p.rows - 1 - blockIdx.x / parts;
     const int part = blockIdx.x % parts;
     pdl_wait();
     const Row<T> row(static_cast<const T*>(p.logits) + at * p.stride, p.vocab, part, parts);
@@ -889,39 +892,49 @@ __global__ void __launch_bounds__(kThreads) logits_backward_kernel(const LogitsA
         slope.c1 = -scale * kLn2 * gh;
         special = slope;
     }
-    // vectors where the gradient's rows start as the logits' do, elements otherwise
-    const bool same = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(row.p) % 16;
-    const bool plain = !slope.zero && !slope.shift.far;
     auto put = [&](int64_t e, float v) { out[e] = from_float<T>(v); };
-    for (int e = tid; e < row.head_here; e += threads) put(e, slope(row.one(e)));
+    const int ends = row.head_here + (row.n - row.tail);          // elements outside vectors: at most one a thread
+    if (tid < ends) {
+        const int e = tid < row.head_here ? tid : row.tail + tid - row.head_here;
+        put(e, slope(row.one(e)));
+    }
+    // vectors where the gradient's rows start as the logits' do, elements otherwise and in rows that are far or zero
     constexpr int kBatch = 4;
+    const bool vectors = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(row.p) % 16 && !slope.zero && !slope.shift.far;
+    T* to = out + row.head;
     for (int v = row.v0 + tid; v < row.v1; v += kBatch * threads) {
-        Raw<16> raw[kBatch];
+        if (vectors && v + (kBatch - 1) * threads < row.v1) {
+            Raw<16> raw[kBatch];
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b)
-            if (v + b * threads < row.v1) load(raw[b], row.vec(v + b * threads));
+            for (int b = 0; b < kBatch; ++b) load(raw[b], row.vec(v + b * threads));
 #pragma unroll
-        for (int b = 0; b < kBatch; ++b) {
-            if (v + b * threads >= row.v1) break;
-            float f[kPer];
-            if (plain) {
+            for (int b = 0; b < kBatch; ++b) {
+                float f[kPer];
                 slope.template near<T>(raw[b].u, f);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kPer; ++i) f[i] = slope(Word<T>::at(raw[b].u[i / Word<T>::kPer], i % Word<T>::kPer));
-            }
-            T* to = out + row.head + (int64_t)(v + b * threads) * kPer;
-            if (same) {
                 Pack<T, kPer> o;
                 o.set(f);
-                o.put(to);
-            } else {
+                if constexpr (kStream) store_streaming(to + (int64_t)(v + b * threads) * kPer, o.raw);
+                else o.put(to + (int64_t)(v + b * threads) * kPer);
+            }
+        } else {
+#pragma unroll 1
+            for (int u = v; u < min(v + kBatch * threads, row.v1); u += threads) {
+                Raw<16> raw;
+                load(raw, row.vec(u));
+                float f[kPer];
+                if (vectors) {
+                    slope.template near<T>(raw.u, f);
+                    Pack<T, kPer> o;
+                    o.set(f);
+                    o.put(to + (int64_t)u * kPer);
+                } else {
 #pragma unroll
-                for (int i = 0; i < kPer; ++i) to[i] = from_float<T>(f[i]);
+                    for (int i = 0; i < kPer; ++i)
+                        put(row.head + (int64_t)u * kPer + i, slope(Word<T>::at(raw.u[i / Word<T>::kPer], i % Word<T>::kPer)));
+                }
             }
         }
     }
-    for (int e = row.tail + tid; e < row.n; e += threads) put(e, slope(row.one(e)));
     if constexpr (kDistilled) {
         const float norm = gload(stat + kNorm);
         for (int i = tid; i < specials; i += threads) {
@@ -1009,8 +1022,9 @@ int run_backward(const LogitsArgs& a, cudaStream_t st) {
     const int64_t vectors = a.vocab / parts * (int64_t)sizeof(T) / 16;
     const int threads = vectors >= 192 ? 256 : vectors >= 96 ? 128 : 64;
     if (a.rows * parts >= 1ll << 31) return DCN_ERR_LIMIT;
-    return launch_dependent(logits_backward_kernel<T, kDistilled>, dim3((unsigned)(a.rows * parts)), dim3(threads), 0, st, a,
-                            (int)parts) != cudaSuccess
+    const bool stream = a.vocab * sizeof(T) % 32 == 0 && aligned(a.dlogits, 32);
+    const auto kernel = stream ? logits_backward_kernel<T, kDistilled, true> : logits_backward_kernel<T, kDistilled, false>;
+    return launch_dependent(kernel, dim3((unsigned)(a.rows * parts)), dim3(threads), 0, st, a, (int)parts) != cudaSuccess
                ? DCN_ERR_CUDA
                : DCN_OK;
 }
