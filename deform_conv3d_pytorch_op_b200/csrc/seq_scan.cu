@@ -601,7 +601,7 @@ int launch_scan(K kernel, int held, size_t smem, int per_thread, const ScanArgs&
     const int64_t units = batch * a.tiles;
     const int warps = (int)(a.steps >= kChunk ? kChunk / per_thread : a.steps > per_thread ? (a.steps + per_thread - 1) / per_thread : 1);
     int ranks = 1;
-    while (ranks < kCluster && (int64_t)ranks * kChunk < a.steps && 2 * units * ranks <= (int64_t)held * sm_count()) ranks *= 2;
+    while (ranks < kCluster && (int64_t)ranks * kChunk < a.steps && units * (ranks + 1) <= (int64_t)held * sm_count()) ++ranks;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(units * ranks));
     cfg.blockDim = dim3(32, warps);
