@@ -75,19 +75,22 @@ struct Product {
 template <int W>
 __device__ __forceinline__ Map<W> identity() { return {all_lanes<W>(1.0f), all_lanes<W>(0.0f), all_lanes<W>(0.0f)}; }
 
-// Maps in shared memory, of a lane each
-template <int W>
+// Maps of two channels in shared memory, a lane each.  `more` is below the last digit of a: eight digits of it are plenty, and
+// what they save lets an SM hold another CTA.
 struct MapRoom {
-    static constexpr uint32_t kBytes = 3 * sizeof(Lanes<W>) * 32;
-    struct alignas(2 * sizeof(Lanes<W>)) Gate {
-        Lanes<W> a, more;
+    static constexpr uint32_t kBytes = (2 * sizeof(Lanes<2>) + 4) * 32;
+    struct alignas(16) Pair {
+        Lanes<2> a, b;
     };
-    Gate gate[32];
-    Lanes<W> b[32];
-    __device__ __forceinline__ void put(int lane, const Map<W>& m) { gate[lane] = {m.a, m.more}, b[lane] = m.b; }
-    __device__ __forceinline__ Map<W> get(int lane) const {
-        const Gate g = gate[lane];
-        return {g.a, g.more, b[lane]};
+    Pair ab[32];
+    uint32_t more[32];
+    static __device__ __forceinline__ uint32_t packed(Lanes<2> more) { return word_of<__nv_bfloat16>(more.at(0), more.at(1)); }
+    __device__ __forceinline__ void put(int lane, const Map<2>& m) { ab[lane] = {m.a, m.b}, more[lane] = packed(m.more); }
+    __device__ __forceinline__ Map<2> get(int lane) const {
+        const Pair p = ab[lane];
+        const uint32_t w = more[lane];
+        const float f[2] = {half_of<__nv_bfloat16>(w, 0), half_of<__nv_bfloat16>(w, 1)};
+        return {p.a, lanes<2>(f), p.b};
     }
 };
 
@@ -99,7 +102,7 @@ constexpr long long kWaitCycles = 1ll << 32;                     // some two sec
 // goes to): a cluster barrier instead would hold every warp until its results of the wave before are in memory.  Two of
 // everything: a CTA sends a wave's map when all maps of the wave before have arrived, so the one it writes over has been read.
 struct Exchange {
-    MapRoom<2> maps[2][kCluster];
+    MapRoom maps[2][kCluster];
     alignas(8) uint64_t arrived[2];
     int gave_up;
 
@@ -116,7 +119,7 @@ struct Exchange {
     __device__ __forceinline__ void expect(int side, int ranks) {
         asm volatile("{\n .reg .b64 s;\n mbarrier.arrive.expect_tx.shared::cta.b64 s, [%0], %1;\n}" ::"r"(
                          shared_address(&arrived[side])),
-                     "r"(ranks * MapRoom<2>::kBytes)
+                     "r"(ranks * MapRoom::kBytes)
                      : "memory");
     }
     // my lane's part of the map of the CTA `rank`, to the CTA `to`
@@ -124,12 +127,13 @@ struct Exchange {
         uint32_t there;                          // this object, in that CTA
         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(shared_address(this)), "r"(to));
         const uint32_t here = shared_address(this), bar = there + shared_address(&arrived[side]) - here;
-        const uint32_t gate = there + shared_address(&maps[side][rank].gate[lane]) - here,
-                       b = there + shared_address(&maps[side][rank].b[lane]) - here;
-        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(gate), "l"(m.a.v),
-                     "l"(m.more.v), "r"(bar)
+        const uint32_t ab = there + shared_address(&maps[side][rank].ab[lane]) - here,
+                       more = there + shared_address(&maps[side][rank].more[lane]) - here;
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.b64 [%0], {%1, %2}, [%3];" ::"r"(ab), "l"(m.a.v),
+                     "l"(m.b.v), "r"(bar)
                      : "memory");
-        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b64 [%0], %1, [%2];" ::"r"(b), "l"(m.b.v), "r"(bar)
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(more),
+                     "r"(MapRoom::packed(m.more)), "r"(bar)
                      : "memory");
     }
     __device__ __forceinline__ void send_all(int side, int rank, int ranks, int lane, const Map<2>& m) {
@@ -298,7 +302,7 @@ template <typename T, int kBytes, int K>
 struct ForwardRoom {
     static constexpr int kWarps = kChunk / K;
     Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps];
-    MapRoom<2> part[kWarps];                     // of the warps
+    MapRoom part[kWarps];                     // of the warps
     Lanes<2> start[kWarps][32];                  // the states before their steps
     Exchange cluster;
 };
@@ -407,10 +411,10 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
 template <typename T, int kBytes, int K>
 struct BackwardRoom {
     static constexpr int kWarps = kChunk / K;
-    Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps], dy[2][kWarps];
-    MapRoom<2> part[kWarps];
-    Lanes<2> back[kWarps][32];                   // the b of the warps' backward maps p -> A p + b, which have the forward ones' A
-    Lanes<2> start[kWarps][32], end[kWarps][32]; // the states before their steps, and the gradients behind them
+    Block<T, kBytes, K> x[2][kWarps], dy[2][kWarps], gate[kWarps];
+    MapRoom part[kWarps];                        // of the warps; b gives way to the states before their steps
+    // the b of the warps' backward maps p -> A p + b, which have the forward ones' A; then the gradients behind their steps
+    Lanes<2> back[kWarps][32];
     Exchange cluster;
 };
 
@@ -433,12 +437,16 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
     const int64_t end = (len + wave - 1) / wave * wave;
     int64_t begin = end - wave;
     int64_t t0 = begin + (int64_t)me.rank * chunk + me.warp * K;
+    // (a wave that does not come is not filled)
     auto fill = [&](int side, int64_t t) {
-        if (t >= 0) {                                              // (a wave that does not come is not filled)
+        if (t >= 0) {
             room.x[side][me.warp].fill(x, t, p.x_step, len, me.width, me.lane);
-            room.gate[side][me.warp].fill(gate, t, p.gate_step, len, me.width, me.lane);
             room.dy[side][me.warp].fill(dy, t, p.dy_step, p.dy == nullptr ? t : len, me.width, me.lane);
         }
+        copies_issued();
+    };
+    auto fill_gate = [&](int64_t t) {
+        if (t >= 0) room.gate[me.warp].fill(gate, t, p.gate_step, len, me.width, me.lane);
         copies_issued();
     };
     if (me.warp == 0) {
@@ -449,10 +457,11 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
         }
     }
     fill(0, t0);
+    fill_gate(t0);
     fill(1, t0 - wave);
     if (me.ranks > 1) cg::this_cluster().sync();                   // every CTA runs before another writes to its memory
     for (int side = 0, n = 0; begin >= 0; begin -= wave, t0 -= wave, side ^= 1, ++n) {
-        auto &bx = room.x[side][me.warp], &bg = room.gate[side][me.warp], &bd = room.dy[side][me.warp];
+        auto &bx = room.x[side][me.warp], &bg = room.gate[me.warp], &bd = room.dy[side][me.warp];
         copies_arrived<1>();
         __syncwarp();
         Lanes<2> a[K], keep[K], before[K], sum = all_lanes<2>(0.0f), passed = sum;
@@ -473,18 +482,20 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
         room.part[me.warp].put(me.lane, product.map(sum));
         room.back[me.warp][me.lane] = passed;
         __syncthreads();
+        fill_gate(t0 - wave);
         if (me.warp == (me.warps > 1 ? 1 : 0)) {                   // the states, from the one before the CTA's steps
             const int64_t first = t0 - me.warp * K;
             Lanes<2> h = me.load(first < len ? p.checkpoints : nullptr, me.b * p.chunks + first / kChunk, p.channels);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                room.start[w][me.lane] = h;
-                h = room.part[w].get(me.lane)(h);
+                const Map<2> m = room.part[w].get(me.lane);
+                room.part[w].ab[me.lane].b = h;
+                h = m(h);
             }
         }
         if (me.warp == 0) {                                        // the gradients, from the one that reaches the CTA's last step
             auto back_map = [&](int w) {
-                Map<2> m = room.part[w].get(me.lane);
+                Map<2> m = room.part[w].get(me.lane);              // (its b may be gone)
                 m.b = room.back[w][me.lane];
                 return m;
             };
@@ -508,13 +519,14 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
             }
 #pragma unroll
             for (int w = kWarps - 1; w >= 0; --w) {
-                room.end[w][me.lane] = g;
-                g = back_map(w)(g);
+                const Map<2> m = back_map(w);
+                room.back[w][me.lane] = g;
+                g = m(g);
             }
             if (me.ranks == 1) carry = g;
         }
         __syncthreads();
-        Lanes<2> h = room.start[me.warp][me.lane], mine = room.end[me.warp][me.lane];
+        Lanes<2> h = room.part[me.warp].ab[me.lane].b, mine = room.back[me.warp][me.lane];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             before[k] = h;
@@ -527,11 +539,11 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
             mine = a[k] * d;
             if (!all && t0 + k >= len) ox = og = all_lanes<2>(0.0f);
             bx.put(k, me.lane, ox);
-            bg.put(k, me.lane, og);
+            bd.put(k, me.lane, og);
         }
         __syncwarp();
         bx.drain(dx, t0, p.channels, p.steps, me.width, me.lane);
-        bg.drain(dgate, t0, p.channels, p.steps, me.width, me.lane);
+        bd.drain(dgate, t0, p.channels, p.steps, me.width, me.lane);
         __syncwarp();
         fill(side, t0 - 2 * wave);
     }
@@ -633,10 +645,10 @@ int backward_as(const ScanArgs& a, int64_t batch, cudaStream_t st) {
     return launch_scan(scan_backward_kernel<T, kBytes, K>, held, sizeof(Room), K, a, batch, st);
 }
 
-// Steps of a thread, 16 or 8: with 16 the joining of maps costs half as much of a step, with 8 a thread has registers to spare.
-// Measured (us, 16 / 8): forward, bf16, 64x1024x2048 141 / 165, 2x16384x2048 101 / 141; float32, 2x8192x2048 82 / 86.
-// Backward, bf16, 64x1024x2048 265 / 314, 2x16384x2048 188 / 187, 24x777x1024 50 / 66; float32, 2x8192x2048 189 / 183,
-// 46x238x3008 210 / 166.
+// Steps of a thread, 16 or 8: with 16 the joining of maps costs half as much of a step, with 8 a thread has registers to spare, and
+// float32 data holds the SM's shared memory anyhow.  Measured (us, 16 / 8): forward, bf16, 64x1024x2048 141 / 165, 2x16384x2048
+// 101 / 141; float32, 2x8192x2048 82 / 86.  Backward, bf16, 64x1024x2048 252 / 326, 2x16384x2048 151 / 187; float32,
+// 2x8192x2048 132 / 127, 46x238x3008 113 / 102.
 template <typename T, int kBytes>
 int run_forward(const ScanArgs& a, int64_t batch, cudaStream_t st) {
     return forward_as<T, kBytes, 16>(a, batch, st);
