@@ -148,57 +148,38 @@ __device__ __forceinline__ void logistic(float v, float& s, float& rest) {
     rest = v < 0.0f ? r : q;
 }
 
-// W floats, one or two, as the arithmetic takes them: pairs go through the packed float32 instructions
-template <int W>
-struct Lanes;
-template <>
-struct Lanes<1> {
-    float v;
-    __device__ __forceinline__ float at(int) const { return v; }
-};
-template <>
-struct Lanes<2> {
+// Two floats as the packed float32 instructions take them
+struct Lanes {
     uint64_t v;
     __device__ __forceinline__ float at(int i) const { return __uint_as_float((uint32_t)(i == 0 ? v : v >> 32)); }
 };
-template <int W>
-__device__ __forceinline__ Lanes<W> lanes(const float (&f)[W]) {
-    Lanes<W> r;
-    if constexpr (W == 1) r.v = f[0];
-    else asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(f[0]), "f"(f[1]));
+__device__ __forceinline__ Lanes lanes(const float (&f)[2]) {
+    Lanes r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(f[0]), "f"(f[1]));
     return r;
 }
-template <int W>
-__device__ __forceinline__ Lanes<W> all_lanes(float f) {
-    float a[W];
-#pragma unroll
-    for (int i = 0; i < W; ++i) a[i] = f;
-    return lanes<W>(a);
+__device__ __forceinline__ Lanes all_lanes(float f) {
+    const float a[2] = {f, f};
+    return lanes(a);
 }
-__device__ __forceinline__ Lanes<1> fma(Lanes<1> a, Lanes<1> b, Lanes<1> c) { return {fmaf(a.v, b.v, c.v)}; }
-__device__ __forceinline__ Lanes<1> operator*(Lanes<1> a, Lanes<1> b) { return {a.v * b.v}; }
-__device__ __forceinline__ Lanes<1> operator+(Lanes<1> a, Lanes<1> b) { return {a.v + b.v}; }
-__device__ __forceinline__ Lanes<2> fma(Lanes<2> a, Lanes<2> b, Lanes<2> c) {
-    Lanes<2> r;
+__device__ __forceinline__ Lanes fma(Lanes a, Lanes b, Lanes c) {
+    Lanes r;
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
     return r;
 }
-__device__ __forceinline__ Lanes<2> operator*(Lanes<2> a, Lanes<2> b) {
-    Lanes<2> r;
+__device__ __forceinline__ Lanes operator*(Lanes a, Lanes b) {
+    Lanes r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
 }
-__device__ __forceinline__ Lanes<2> operator+(Lanes<2> a, Lanes<2> b) {
-    Lanes<2> r;
+__device__ __forceinline__ Lanes operator+(Lanes a, Lanes b) {
+    Lanes r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
     return r;
 }
-template <int W>
-__device__ __forceinline__ Lanes<W> operator-(Lanes<W> a, Lanes<W> b) {
-    return fma(b, all_lanes<W>(-1.0f), a);
-}
+__device__ __forceinline__ Lanes operator-(Lanes a, Lanes b) { return fma(b, all_lanes(-1.0f), a); }
 
-__device__ __forceinline__ Lanes<2> shuffle_xor(Lanes<2> a, int o) {
+__device__ __forceinline__ Lanes shuffle_xor(Lanes a, int o) {
     return {__shfl_xor_sync(0xffffffffu, (unsigned long long)a.v, o)};
 }
 

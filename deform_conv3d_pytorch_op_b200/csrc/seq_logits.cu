@@ -171,11 +171,11 @@ struct Word {
 
 // Elements 2 i, 2 i + 1 of a vector's words
 template <typename T>
-__device__ __forceinline__ Lanes<2> pair_of(const uint32_t* w, int i) {
+__device__ __forceinline__ Lanes pair_of(const uint32_t* w, int i) {
     float f[2];
     if constexpr (sizeof(T) == 4) f[0] = __uint_as_float(w[2 * i]), f[1] = __uint_as_float(w[2 * i + 1]);
     else f[0] = half_of<T>(w[i], 0), f[1] = half_of<T>(w[i], 1);
-    return lanes<2>(f);
+    return lanes(f);
 }
 
 // The sums of a thread's elements.  kMarks: without the marked ones.  kAgain: the elements are read a second time.
@@ -237,20 +237,20 @@ __device__ __forceinline__ Sums sums_of(const Row<T>& row, int tid, int threads,
                 a = add_elements<T, kU, kMarks>(a, row, e, e + kPer, 1, k, marks);
             }
         } else {
-            const Lanes<2> kk = all_lanes<2>(k), shifted = all_lanes<2>(-shift.mk);
-            Lanes<2> s = all_lanes<2>(0.0f), u = s;
+            const Lanes kk = all_lanes(k), shifted = all_lanes(-shift.mk);
+            Lanes s = all_lanes(0.0f), u = s;
 #pragma unroll
             for (int i = 0; i < kWords * W::kPer / 2; ++i) {
                 // 0 times what is far below is 0, not NaN: logits of -inf are raised to where their d is finite
                 if constexpr (kU && kBf16) w[i] = W::max(w[i], 0xf14af14au);             // -1e30
-                Lanes<2> d = fma(pair_of<T>(w, i), kk, shifted);
+                Lanes d = fma(pair_of<T>(w, i), kk, shifted);
                 if constexpr (kU && !kBf16) {
                     const float f[2] = {max_nan(d.at(0), -kFar), max_nan(d.at(1), -kFar)};
-                    d = lanes<2>(f);
+                    d = lanes(f);
                 }
                 const float e[2] = {ex2(d.at(0)), ex2(d.at(1))};
-                s = s + lanes<2>(e);
-                if constexpr (kU) u = fma(lanes<2>(e), d, u);
+                s = s + lanes(e);
+                if constexpr (kU) u = fma(lanes(e), d, u);
             }
             a.s += s.at(0) + s.at(1);
             if constexpr (kU) a.u += u.at(0) + u.at(1);
@@ -816,17 +816,17 @@ struct Slope {
     // a vector's, where the row is neither far nor zero
     template <typename T>
     __device__ __forceinline__ void near(const uint32_t* w, float (&f)[16 / sizeof(T)]) const {
-        const Lanes<2> kk = all_lanes<2>(shift.k), shifted = all_lanes<2>(-shift.mk), ss = all_lanes<2>(-log_s);
+        const Lanes kk = all_lanes(shift.k), shifted = all_lanes(-shift.mk), ss = all_lanes(-log_s);
 #pragma unroll
         for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
-            Lanes<2> l = fma(pair_of<T>(w, i), kk, shifted) + ss, c = all_lanes<2>(c0);
+            Lanes l = fma(pair_of<T>(w, i), kk, shifted) + ss, c = all_lanes(c0);
             if constexpr (!kLinear) {
                 const float far[2] = {max_nan(l.at(0), -kFar), max_nan(l.at(1), -kFar)};
-                l = lanes<2>(far);
-                c = fma(all_lanes<2>(c1), l, c);
+                l = lanes(far);
+                c = fma(all_lanes(c1), l, c);
             }
             const float e[2] = {ex2(l.at(0)), ex2(l.at(1))};
-            c = lanes<2>(e) * c;
+            c = lanes(e) * c;
             f[2 * i] = c.at(0);
             f[2 * i + 1] = c.at(1);
         }

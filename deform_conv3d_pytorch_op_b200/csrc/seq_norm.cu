@@ -41,14 +41,14 @@ template <typename T, int V>
 struct Slice {
     Pack<T, V> v[Layout<T, V>::kVectors];
     __device__ __forceinline__ float at(int e) const { return v[e / V].at(e % V); }
-    __device__ __forceinline__ Lanes<2> pair(int i) const {
+    __device__ __forceinline__ Lanes pair(int i) const {
         const float f[2] = {at(2 * i), at(2 * i + 1)};
-        return lanes<2>(f);
+        return lanes(f);
     }
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void put(void* base, int64_t offset, const Lanes<2> (&f)[Layout<T, V>::kPairs], int j, int threads,
+__device__ __forceinline__ void put(void* base, int64_t offset, const Lanes (&f)[Layout<T, V>::kPairs], int j, int threads,
                                     int channels) {
     if (base == nullptr) return;
 #pragma unroll
@@ -184,7 +184,7 @@ struct Weights {
         if (p.wide_weights) put_as<float>(p, j, threads);
         else put_as<T>(p, j, threads);
     }
-    __device__ __forceinline__ void get(int which, Lanes<2> (&f)[L::kPairs]) const {
+    __device__ __forceinline__ void get(int which, Lanes (&f)[L::kPairs]) const {
 #pragma unroll
         for (int i = 0; i < L::kPer / 4; ++i) {
             const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&at[(which * (L::kPer / 4) + i) * width]);
@@ -216,7 +216,7 @@ struct RowSum {
     float (&room)[2][32];
     const Team<kWarp>& me;
     int side;
-    __device__ __forceinline__ float operator()(Lanes<2> pair) {
+    __device__ __forceinline__ float operator()(Lanes pair) {
         float v = pair.at(0) + pair.at(1);
         if constexpr (kWarp) {
 #pragma unroll
@@ -237,7 +237,7 @@ struct RowSum {
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void gates_of(const Slice<T, V>& g, bool has, Lanes<2> (&on)[Layout<T, V>::kPairs]) {
+__device__ __forceinline__ void gates_of(const Slice<T, V>& g, bool has, Lanes (&on)[Layout<T, V>::kPairs]) {
 #pragma unroll
     for (int i = 0; i < Layout<T, V>::kPairs; ++i) {
         float s[2] = {1.0f, 1.0f}, rest;
@@ -245,7 +245,7 @@ __device__ __forceinline__ void gates_of(const Slice<T, V>& g, bool has, Lanes<2
             logistic(g.at(2 * i), s[0], rest);
             logistic(g.at(2 * i + 1), s[1], rest);
         }
-        on[i] = lanes<2>(s);
+        on[i] = lanes(s);
     }
 }
 
@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
     for (int64_t row = first; me.warp_row(row) < p.rows; row += step) {
         rows.next(row);
         const Slice<T, V> x = rows.get(0);
-        Lanes<2> s[L::kPairs], w[L::kPairs], sum = all_lanes<2>(0.0f);
+        Lanes s[L::kPairs], w[L::kPairs], sum = all_lanes(0.0f);
         float r = 0.0f;
         if (p.block != nullptr) {
             const Slice<T, V> y = rows.get(1);
@@ -277,10 +277,10 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
             for (int i = 0; i < L::kPairs; ++i) sum = fma(y.pair(i), y.pair(i), sum);
             r = rsqrtf(row_sum(sum) * p.inv + p.eps);
             weights.get(0, w);
-            sum = all_lanes<2>(0.0f);
+            sum = all_lanes(0.0f);
 #pragma unroll
             for (int i = 0; i < L::kPairs; ++i) {
-                s[i] = fma(w[i] * s[i], y.pair(i) * all_lanes<2>(r), x.pair(i));
+                s[i] = fma(w[i] * s[i], y.pair(i) * all_lanes(r), x.pair(i));
                 sum = fma(s[i], s[i], sum);
             }
             put<T, V>(p.stream, row * p.channels, s, me.j, me.threads, rows.live ? p.channels : 0);
@@ -294,7 +294,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
         const float q = rsqrtf(row_sum(sum) * p.inv + p.eps);
         weights.get(1, w);
 #pragma unroll
-        for (int i = 0; i < L::kPairs; ++i) s[i] = s[i] * all_lanes<2>(q) * w[i];
+        for (int i = 0; i < L::kPairs; ++i) s[i] = s[i] * all_lanes(q) * w[i];
         put<T, V>(p.normed, row * p.channels, s, me.j, me.threads, rows.live ? p.channels : 0);
         if (p.stats != nullptr && me.j == 0 && rows.live) {
             p.stats[2 * row] = r;
@@ -321,9 +321,9 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
     rows.begin(first);
     if (me.group == 0) weights.put(p, me.j, me.threads);
     __syncthreads();
-    Lanes<2> z[L::kPairs], dpre[L::kPairs];
+    Lanes z[L::kPairs], dpre[L::kPairs];
 #pragma unroll
-    for (int i = 0; i < L::kPairs; ++i) z[i] = dpre[i] = all_lanes<2>(0.0f);
+    for (int i = 0; i < L::kPairs; ++i) z[i] = dpre[i] = all_lanes(0.0f);
     float next_r = 0.0f, next_q = 0.0f;
     auto fetch_stats = [&](int64_t row) {
         if (row >= p.rows) return;
@@ -336,8 +336,8 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
         fetch_stats(row + step);
         rows.next(row);
         const Slice<T, V> y = rows.get(1);
-        const Lanes<2> rr = all_lanes<2>(r), qq = all_lanes<2>(q);
-        Lanes<2> on[L::kPairs], sn[L::kPairs], d[L::kPairs], w[L::kPairs], sum = all_lanes<2>(0.0f);
+        const Lanes rr = all_lanes(r), qq = all_lanes(q);
+        Lanes on[L::kPairs], sn[L::kPairs], d[L::kPairs], w[L::kPairs], sum = all_lanes(0.0f);
         gates_of<T, V>(rows.get(2), p.gate != nullptr, on);
         const Slice<T, V> x = rows.get(0);
         if (p.block != nullptr) {
@@ -356,22 +356,22 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
             d[i] = dn.pair(i) * w[i];
             sum = fma(d[i], sn[i], sum);
         }
-        const Lanes<2> m = all_lanes<2>(-row_sum(sum) * p.inv);
+        const Lanes m = all_lanes(-row_sum(sum) * p.inv);
         const Slice<T, V> ds = rows.get(3);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) d[i] = fma(qq, fma(sn[i], m, d[i]), ds.pair(i));
         put<T, V>(p.dx, row * p.channels, d, me.j, me.threads, rows.live ? p.channels : 0);
         if (p.block == nullptr) continue;
         weights.get(0, w);
-        sum = all_lanes<2>(0.0f);
+        sum = all_lanes(0.0f);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) {
-            const Lanes<2> yn = y.pair(i) * rr, u = d[i] * on[i];
+            const Lanes yn = y.pair(i) * rr, u = d[i] * on[i];
             z[i] = fma(u, yn, z[i]);
             sn[i] = u * w[i];                    // the gradient of yn from here on
             sum = fma(sn[i], yn, sum);
         }
-        const Lanes<2> n = all_lanes<2>(-row_sum(sum) * p.inv);
+        const Lanes n = all_lanes(-row_sum(sum) * p.inv);
 #pragma unroll
         for (int i = 0; i < L::kPairs; ++i) d[i] = rr * fma(y.pair(i) * rr, n, sn[i]);
         put<T, V>(p.dblock, row * p.channels, d, me.j, me.threads, rows.live ? p.channels : 0);
@@ -382,7 +382,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
                 float off[2], s;
                 logistic(g.at(2 * i), s, off[0]);
                 logistic(g.at(2 * i + 1), s, off[1]);
-                d[i] = sn[i] * (y.pair(i) * rr) * lanes<2>(off);
+                d[i] = sn[i] * (y.pair(i) * rr) * lanes(off);
             }
             put<T, V>(p.dgate, row * p.channels, d, me.j, me.threads, rows.live ? p.channels : 0);
         }
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
         }
         rows_left = blockDim.x / 32, mine = threadIdx.x % 32 < me.threads ? threadIdx.x / 32 : -1;
     }
-    Lanes<2>* all = reinterpret_cast<Lanes<2>*>(dynamic) + me.j;
+    Lanes* all = reinterpret_cast<Lanes*>(dynamic) + me.j;
     for (int k = 0; k < rows_left; ++k) {
         __syncthreads();
         if (k == mine)

@@ -5,10 +5,10 @@
 //     dx_t = D_t (1 - a_t),   dgate_t = D_t (h_{t-1} - x_t) a_t (1 - a_t),   dstate = p_0.
 //
 // Both directions are scans of affine maps h -> A h + B, whose composition is (A2 A1, A2 B1 + B2).  A lane has a pair of channels,
-// in the packed float32 instructions, and kSteps steps of them: it composes its steps, the warps of a CTA (one behind the other
-// in time) compose theirs through shared memory and the CTAs of a cluster theirs through distributed shared memory, a warp for all;
-// the state that reaches a lane then gives all of its steps.  So x and gate are read once and y is written once, whatever the length: the
-// bound is DRAM.  A cluster walks the time axis in waves of (its CTAs) x 64 steps and carries the state from wave to wave in
+// in the packed float32 instructions, and K steps of them: it composes its steps, the warps of a CTA (one behind the other in time)
+// compose theirs through shared memory and the CTAs of a cluster theirs through distributed shared memory, a warp for all; the
+// state that reaches a lane then gives all of its steps.  So x and gate are read once and y is written once, whatever the length:
+// the bound is DRAM.  A cluster walks the time axis in waves of (its CTAs) x 64 steps and carries the state from wave to wave in
 // registers.  Every warp copies its own steps of the next waves to shared memory meanwhile (cp.async, two stages), and sends its
 // results out from there: 16 bytes an instruction where addresses allow it, and no address arithmetic in the recurrence.
 //
@@ -44,53 +44,50 @@ struct ScanArgs {
 };
 
 // h -> A h + B, A = a + more to more digits than a float has
-template <int W>
 struct Map {
-    Lanes<W> a, more, b;
-    __device__ __forceinline__ Lanes<W> operator()(Lanes<W> h) const { return fma(a, h, fma(more, h, b)); }
+    Lanes a, more, b;
+    __device__ __forceinline__ Lanes operator()(Lanes h) const { return fma(a, h, fma(more, h, b)); }
 };
 
 // A product of gates, and one minus it
-template <int W>
 struct Product {
-    Lanes<W> a = all_lanes<W>(1.0f), rest = all_lanes<W>(0.0f);
-    __device__ __forceinline__ void by(Lanes<W> gate, Lanes<W> one_minus) {
+    Lanes a = all_lanes(1.0f), rest = all_lanes(0.0f);
+    __device__ __forceinline__ void by(Lanes gate, Lanes one_minus) {
         rest = fma(one_minus, a, rest);
         a = gate * a;
     }
-    __device__ __forceinline__ void by(const Map<W>& m) { by(m.a, all_lanes<W>(1.0f) - m.a - m.more); }
-    __device__ __forceinline__ Map<W> map(Lanes<W> b) const {
-        float top[W], more[W];
+    __device__ __forceinline__ void by(const Map& m) { by(m.a, all_lanes(1.0f) - m.a - m.more); }
+    __device__ __forceinline__ Map map(Lanes b) const {
+        float top[2], more[2];
 #pragma unroll
-        for (int i = 0; i < W; ++i) {
+        for (int i = 0; i < 2; ++i) {
             const float near = 1.0f - rest.at(i);
             const bool close = rest.at(i) < 0.5f;
             top[i] = close ? near : a.at(i);
             more[i] = close ? (1.0f - near) - rest.at(i) : 0.0f;
         }
-        return {lanes<W>(top), lanes<W>(more), b};
+        return {lanes(top), lanes(more), b};
     }
 };
 
-template <int W>
-__device__ __forceinline__ Map<W> identity() { return {all_lanes<W>(1.0f), all_lanes<W>(0.0f), all_lanes<W>(0.0f)}; }
+__device__ __forceinline__ Map identity() { return {all_lanes(1.0f), all_lanes(0.0f), all_lanes(0.0f)}; }
 
 // Maps of two channels in shared memory, a lane each.  `more` is below the last digit of a: eight digits of it are plenty, and
 // what they save lets an SM hold another CTA.
 struct MapRoom {
-    static constexpr uint32_t kBytes = (2 * sizeof(Lanes<2>) + 4) * 32;
+    static constexpr uint32_t kBytes = (2 * sizeof(Lanes) + 4) * 32;
     struct alignas(16) Pair {
-        Lanes<2> a, b;
+        Lanes a, b;
     };
     Pair ab[32];
     uint32_t more[32];
-    static __device__ __forceinline__ uint32_t packed(Lanes<2> more) { return word_of<__nv_bfloat16>(more.at(0), more.at(1)); }
-    __device__ __forceinline__ void put(int lane, const Map<2>& m) { ab[lane] = {m.a, m.b}, more[lane] = packed(m.more); }
-    __device__ __forceinline__ Map<2> get(int lane) const {
+    static __device__ __forceinline__ uint32_t packed(Lanes more) { return word_of<__nv_bfloat16>(more.at(0), more.at(1)); }
+    __device__ __forceinline__ void put(int lane, const Map& m) { ab[lane] = {m.a, m.b}, more[lane] = packed(m.more); }
+    __device__ __forceinline__ Map get(int lane) const {
         const Pair p = ab[lane];
         const uint32_t w = more[lane];
         const float f[2] = {half_of<__nv_bfloat16>(w, 0), half_of<__nv_bfloat16>(w, 1)};
-        return {p.a, lanes<2>(f), p.b};
+        return {p.a, lanes(f), p.b};
     }
 };
 
@@ -108,7 +105,7 @@ struct Exchange {
 
     // by warp 0; the places of CTAs that are not there hold maps that change nothing
     __device__ __forceinline__ void begin(int lane, int ranks) {
-        for (int r = ranks; r < kCluster; ++r) maps[0][r].put(lane, identity<2>()), maps[1][r].put(lane, identity<2>());
+        for (int r = ranks; r < kCluster; ++r) maps[0][r].put(lane, identity()), maps[1][r].put(lane, identity());
         if (lane == 0) {
             gave_up = 0;
             for (int s = 0; s < 2; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&arrived[s])) : "memory");
@@ -123,7 +120,7 @@ struct Exchange {
                      : "memory");
     }
     // my lane's part of the map of the CTA `rank`, to the CTA `to`
-    __device__ __forceinline__ void send(int side, int rank, int to, int lane, const Map<2>& m) {
+    __device__ __forceinline__ void send(int side, int rank, int to, int lane, const Map& m) {
         uint32_t there;                          // this object, in that CTA
         asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(shared_address(this)), "r"(to));
         const uint32_t here = shared_address(this), bar = there + shared_address(&arrived[side]) - here;
@@ -136,7 +133,7 @@ struct Exchange {
                      "r"(MapRoom::packed(m.more)), "r"(bar)
                      : "memory");
     }
-    __device__ __forceinline__ void send_all(int side, int rank, int ranks, int lane, const Map<2>& m) {
+    __device__ __forceinline__ void send_all(int side, int rank, int ranks, int lane, const Map& m) {
         if (lane == 0) expect(side, ranks);
 #pragma unroll
         for (int r = 0; r < kCluster; ++r)
@@ -184,13 +181,13 @@ struct Place {
         width = (int)(p.channels - c < kTile ? p.channels - c : kTile);
         mine = width - 2 * lane < 0 ? 0 : width - 2 * lane > 2 ? 2 : width - 2 * lane;
     }
-    __device__ __forceinline__ Lanes<2> load(const float* s, int64_t row, int64_t channels) const {
+    __device__ __forceinline__ Lanes load(const float* s, int64_t row, int64_t channels) const {
         float h[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) h[i] = s != nullptr && i < mine ? gload(s + row * channels + c + 2 * lane + i) : 0.0f;
-        return lanes<2>(h);
+        return lanes(h);
     }
-    __device__ __forceinline__ void store(float* s, int64_t row, int64_t channels, Lanes<2> h) const {
+    __device__ __forceinline__ void store(float* s, int64_t row, int64_t channels, Lanes h) const {
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             if (i < mine) s[row * channels + c + 2 * lane + i] = h.at(i);
@@ -260,12 +257,12 @@ struct Block {
         p.raw = *reinterpret_cast<const Raw<2 * sizeof(T)>*>(&v[k][2 * lane]);
         return p;
     }
-    __device__ __forceinline__ Lanes<2> at(int k, int lane) const {
+    __device__ __forceinline__ Lanes at(int k, int lane) const {
         const Pack<T, 2> p = get(k, lane);
         const float f[2] = {p.at(0), p.at(1)};
-        return lanes<2>(f);
+        return lanes(f);
     }
-    __device__ __forceinline__ void put(int k, int lane, Lanes<2> x) {
+    __device__ __forceinline__ void put(int k, int lane, Lanes x) {
         const float f[2] = {x.at(0), x.at(1)};
         Pack<T, 2> p;
         p.set(f);
@@ -275,15 +272,15 @@ struct Block {
 
 // Gate and one minus it; one and zero, a step that keeps the state, behind a sequence's end
 template <typename T>
-__device__ __forceinline__ void gates_of(const Pack<T, 2>& g, bool in, Lanes<2>& a, Lanes<2>& keep) {
+__device__ __forceinline__ void gates_of(const Pack<T, 2>& g, bool in, Lanes& a, Lanes& keep) {
     float fa[2], fk[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         logistic(g.at(i), fa[i], fk[i]);
         if (!in) fa[i] = 1.0f, fk[i] = 0.0f;
     }
-    a = lanes<2>(fa);
-    keep = lanes<2>(fk);
+    a = lanes(fa);
+    keep = lanes(fk);
 }
 
 // Zeros from step `from` on, shared out over the warps of the cluster
@@ -303,7 +300,7 @@ struct ForwardRoom {
     static constexpr int kWarps = kChunk / K;
     Block<T, kBytes, K> x[2][kWarps], gate[2][kWarps];
     MapRoom part[kWarps];                     // of the warps
-    Lanes<2> start[kWarps][32];                  // the states before their steps
+    Lanes start[kWarps][32];                  // the states before their steps
     Exchange cluster;
 };
 
@@ -318,7 +315,7 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
     const T* x = static_cast<const T*>(p.x) + me.b * p.x_batch + me.c;
     const T* gate = static_cast<const T*>(p.gate) + me.b * p.gate_batch + me.c;
     T* y = static_cast<T*>(p.y) + me.b * p.steps * p.channels + me.c;
-    Lanes<2> carry = me.load(p.state, me.b, p.channels);
+    Lanes carry = me.load(p.state, me.b, p.channels);
 
     const int chunk = me.warps * K, wave = me.ranks * chunk;
     int64_t t0 = (int64_t)me.rank * chunk + me.warp * K;           // my first step of this wave
@@ -330,7 +327,7 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
     if (me.warp == 0) {
         if (me.ranks > 1) room.cluster.begin(me.lane, me.ranks);
         for (int w = me.warps; w < kWarps; ++w) {                  // (warps that are not there change nothing)
-            room.part[w].put(me.lane, identity<2>());
+            room.part[w].put(me.lane, identity());
         }
     }
     for (int s = 0; s < 2; ++s) {
@@ -343,13 +340,13 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
         copies_arrived<2>();
         __syncwarp();
         // after each of my steps: y = A h + B of the state h before the first
-        Lanes<2> A[K], B[K], sum = all_lanes<2>(0.0f);
-        Product<2> product;
+        Lanes A[K], B[K], sum = all_lanes(0.0f);
+        Product product;
         const bool all = begin + wave <= len;
         auto compose = [&](auto whole) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                Lanes<2> a, keep;
+                Lanes a, keep;
                 gates_of<T>(bg.get(k, me.lane), whole.value || t0 + k < len, a, keep);
                 product.by(a, keep);
                 sum = fma(a, sum, keep * bx.at(k, me.lane));
@@ -362,13 +359,13 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
         room.part[me.warp].put(me.lane, product.map(sum));
         __syncthreads();
         if (me.warp == 0) {
-            Lanes<2> h = carry;
+            Lanes h = carry;
             if (me.ranks > 1) {
-                Product<2> product_of;
-                Lanes<2> s = all_lanes<2>(0.0f);
+                Product product_of;
+                Lanes s = all_lanes(0.0f);
 #pragma unroll
                 for (int w = 0; w < kWarps; ++w) {
-                    const Map<2> m = room.part[w].get(me.lane);
+                    const Map m = room.part[w].get(me.lane);
                     product_of.by(m);
                     s = m(s);
                 }
@@ -390,11 +387,11 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
         }
         fill(bg, gate, t0 + 2 * wave, p.gate_step);
         __syncthreads();
-        const Lanes<2> mine = room.start[me.warp][me.lane];
+        const Lanes mine = room.start[me.warp][me.lane];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            Lanes<2> v = fma(A[k], mine, B[k]);
-            if (!all && t0 + k >= len) v = all_lanes<2>(0.0f);
+            Lanes v = fma(A[k], mine, B[k]);
+            if (!all && t0 + k >= len) v = all_lanes(0.0f);
             bx.put(k, me.lane, v);
         }
         __syncwarp();
@@ -414,7 +411,7 @@ struct BackwardRoom {
     Block<T, kBytes, K> x[2][kWarps], dy[2][kWarps], gate[kWarps];
     MapRoom part[kWarps];                        // of the warps; b gives way to the states before their steps
     // the b of the warps' backward maps p -> A p + b, which have the forward ones' A; then the gradients behind their steps
-    Lanes<2> back[kWarps][32];
+    Lanes back[kWarps][32];
     Exchange cluster;
 };
 
@@ -431,7 +428,7 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
     const T* dy = static_cast<const T*>(p.dy) + me.b * p.dy_batch + me.c;
     T* dx = static_cast<T*>(p.dx) + me.b * p.steps * p.channels + me.c;
     T* dgate = static_cast<T*>(p.dgate) + me.b * p.steps * p.channels + me.c;
-    Lanes<2> carry = me.load(p.dlast, me.b, p.channels);
+    Lanes carry = me.load(p.dlast, me.b, p.channels);
 
     const int chunk = me.warps * K, wave = me.ranks * chunk;
     const int64_t end = (len + wave - 1) / wave * wave;
@@ -452,8 +449,8 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
     if (me.warp == 0) {
         if (me.ranks > 1) room.cluster.begin(me.lane, me.ranks);
         for (int w = me.warps; w < kWarps; ++w) {                  // (warps that are not there change nothing)
-            room.part[w].put(me.lane, identity<2>());
-            room.back[w][me.lane] = all_lanes<2>(0.0f);
+            room.part[w].put(me.lane, identity());
+            room.back[w][me.lane] = all_lanes(0.0f);
         }
     }
     fill(0, t0);
@@ -464,8 +461,8 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
         auto &bx = room.x[side][me.warp], &bg = room.gate[me.warp], &bd = room.dy[side][me.warp];
         copies_arrived<1>();
         __syncwarp();
-        Lanes<2> a[K], keep[K], before[K], sum = all_lanes<2>(0.0f), passed = sum;
-        Product<2> product;
+        Lanes a[K], keep[K], before[K], sum = all_lanes(0.0f), passed = sum;
+        Product product;
         const bool all = begin + wave <= len;
         auto compose = [&](auto whole) {
 #pragma unroll
@@ -485,27 +482,27 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
         fill_gate(t0 - wave);
         if (me.warp == (me.warps > 1 ? 1 : 0)) {                   // the states, from the one before the CTA's steps
             const int64_t first = t0 - me.warp * K;
-            Lanes<2> h = me.load(first < len ? p.checkpoints : nullptr, me.b * p.chunks + first / kChunk, p.channels);
+            Lanes h = me.load(first < len ? p.checkpoints : nullptr, me.b * p.chunks + first / kChunk, p.channels);
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) {
-                const Map<2> m = room.part[w].get(me.lane);
+                const Map m = room.part[w].get(me.lane);
                 room.part[w].ab[me.lane].b = h;
                 h = m(h);
             }
         }
         if (me.warp == 0) {                                        // the gradients, from the one that reaches the CTA's last step
             auto back_map = [&](int w) {
-                Map<2> m = room.part[w].get(me.lane);              // (its b may be gone)
+                Map m = room.part[w].get(me.lane);              // (its b may be gone)
                 m.b = room.back[w][me.lane];
                 return m;
             };
-            Lanes<2> g = carry;
+            Lanes g = carry;
             if (me.ranks > 1) {
-                Product<2> product_of;
-                Lanes<2> s = all_lanes<2>(0.0f);
+                Product product_of;
+                Lanes s = all_lanes(0.0f);
 #pragma unroll
                 for (int w = kWarps - 1; w >= 0; --w) {
-                    const Map<2> m = back_map(w);
+                    const Map m = back_map(w);
                     product_of.by(m);
                     s = m(s);
                 }
@@ -519,14 +516,14 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
             }
 #pragma unroll
             for (int w = kWarps - 1; w >= 0; --w) {
-                const Map<2> m = back_map(w);
+                const Map m = back_map(w);
                 room.back[w][me.lane] = g;
                 g = m(g);
             }
             if (me.ranks == 1) carry = g;
         }
         __syncthreads();
-        Lanes<2> h = room.part[me.warp].ab[me.lane].b, mine = room.back[me.warp][me.lane];
+        Lanes h = room.part[me.warp].ab[me.lane].b, mine = room.back[me.warp][me.lane];
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             before[k] = h;
@@ -534,10 +531,10 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
         }
 #pragma unroll
         for (int k = K - 1; k >= 0; --k) {
-            const Lanes<2> d = bd.at(k, me.lane) + mine;
-            Lanes<2> ox = d * keep[k], og = ox * a[k] * (before[k] - bx.at(k, me.lane));
+            const Lanes d = bd.at(k, me.lane) + mine;
+            Lanes ox = d * keep[k], og = ox * a[k] * (before[k] - bx.at(k, me.lane));
             mine = a[k] * d;
-            if (!all && t0 + k >= len) ox = og = all_lanes<2>(0.0f);
+            if (!all && t0 + k >= len) ox = og = all_lanes(0.0f);
             bx.put(k, me.lane, ox);
             bd.put(k, me.lane, og);
         }

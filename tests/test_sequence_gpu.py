@@ -35,7 +35,7 @@ def grads(outs, ins, gouts):
 
 # ---- gated scan -----------------------------------------------------------------------------------------------------------
 SCANS = [(1, 1, 1), (2, 3, 5), (3, 8, 32), (1, 9, 64), (2, 63, 33), (2, 64, 66), (2, 65, 34), (1, 129, 100), (3, 513, 96),
-         (1, 1200, 34), (2, 2050, 130), (150, 70, 64), (5, 300, 2048)]
+         (1, 1200, 34), (2, 2050, 130), (150, 70, 64), (5, 300, 2048), (1, 700, 5000), (3, 1000, 1601)]
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
@@ -157,7 +157,8 @@ def test_steps_are_the_scan(kind, channels):
 
 
 # ---- gated residual norm --------------------------------------------------------------------------------------------------
-NORMS = [(1, 1), (3, 7), (5, 32), (17, 256), (4, 257), (9, 512), (33, 1000), (6, 2048), (3, 4099), (5, 8192), (3000, 64), (700, 520)]
+NORMS = [(1, 1), (3, 7), (5, 32), (17, 256), (4, 257), (9, 512), (33, 1000), (6, 2048), (3, 4099), (5, 8192), (3000, 64), (700, 520),
+         (40, 1022), (9, 4098), (71, 34), (1025, 16), (33, 130), (2001, 100), (2, 6002)]
 
 
 @pytest.mark.parametrize("kind,weights", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f16", "f32"), ("f16", "f16")])
