@@ -6,12 +6,21 @@
 //     dgate = dyn yn (1 - s(gate));   Z = sum over rows of ds s(gate) yn:  dscale = Z post, dpost = Z scale;   dpre = sum dnormed sn
 //
 // A row lives in the registers of a row of threads, 32 bytes of each tensor a thread, so that every tensor is read or written
-// once: the bound is DRAM.  Rows of up to 32 threads (512 channels of 16 bits, 256 of float32) share a warp, and their sums are
-// shuffles alone; above, a row is that of 64, 128, ... threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of the next row are on their way to its own
-// places in shared memory meanwhile (cp.async, 16 or 4 bytes at a time, as rows start on them); rows of an odd number of 16-bit
-// elements are loaded one by one when they are used.  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the
-// arithmetic goes in pairs through the packed float32 instructions.  The CTAs of the backward pass keep Z and dpre in registers
-// and leave one partial sum each; a second kernel adds those in a fixed order.
+// once.  Rows of up to 32 threads (512 channels of 16 bits, 256 of float32) share a warp, and their sums are shuffles alone; above,
+// a row is that of 64, 128, ... threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of
+// the next row are on their way to its own places in shared memory meanwhile (cp.async, 16 or 4 bytes at a time, as rows start on
+// them); rows of an odd number of 16-bit elements are loaded one by one when they are used.  Weights are in shared memory too, once
+// a CTA (registers for them would cost a third of the threads), and the arithmetic goes in pairs through the packed float32
+// instructions.  The CTAs of the backward pass keep Z and dpre in registers and leave one partial sum each; a second kernel adds
+// those in a fixed order.
+//
+// The bound is DRAM, and the arithmetic, which leaves a third of the issue slots, stands close behind.  Measured, forward and
+// backward with the sums of the weights' gradients, against a copy of the same bytes at 6.5 TB/s:
+//     32768 x 2048 bf16    117 us (5.7 TB/s, 88 %)   209 us (5.1 TB/s, 79 %)
+//     32768 x 2046 bf16    190 us                    348 us      pairs: four times the loads and stores of a row
+//     32768 x 2047 bf16    388 us                    925 us      element by element, nothing ahead
+//     4096 x 8192 float32  141 us (4.8 TB/s, 73 %)   350 us (3.1 TB/s, 47 %)     rows too long to be held twice: nothing ahead
+//     65536 x 64 bf16       10 us (4.0 TB/s)          22 us (3.1 TB/s)           in L2; eight rows to a warp
 #include "seq_common.cuh"
 
 namespace dcn {
@@ -261,7 +270,8 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
     const int64_t first = (int64_t)blockIdx.x * me.groups + me.group, step = (int64_t)gridDim.x * me.groups;
     Rows<T, V, 3, kStaged> rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate)},
                                 {p.x_row, p.block_row, p.gate_row}, p.rows, step, me.j, me.threads, p.channels,
-                                dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * V * sizeof(T), (int)(blockDim.x * V * sizeof(T))};
+                                dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * V * sizeof(T),
+                                (int)(blockDim.x * V * sizeof(T))};
     rows.begin(first);
     if (me.group == 0) weights.put(p, me.j, me.threads);
     __syncthreads();
@@ -317,7 +327,8 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
     Rows<T, V, 5, kStaged> rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate),
                                  static_cast<const T*>(p.dstream), static_cast<const T*>(p.dnormed)},
                                 {p.x_row, p.block_row, p.gate_row, p.dstream_row, p.dnormed_row}, p.rows, step, me.j, me.threads,
-                                p.channels, dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * V * sizeof(T), (int)(blockDim.x * V * sizeof(T))};
+                                p.channels, dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * V * sizeof(T),
+                                (int)(blockDim.x * V * sizeof(T))};
     rows.begin(first);
     if (me.group == 0) weights.put(p, me.j, me.threads);
     __syncthreads();
@@ -470,9 +481,11 @@ unsigned grid_of(int64_t rows, int64_t channels, int elem, int threads_an_sm) {
     return (unsigned)(units < most ? units : most);
 }
 
+// `most`: the shared memory of the kernel's largest CTA.  It is what is asked for at every launch, so that calls of several host
+// threads do not take it from one another.
 template <typename K>
-int launch(K kernel, unsigned grid, int cta, size_t smem, const NormArgs& a, cudaStream_t st) {
-    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+int launch(K kernel, unsigned grid, int cta, size_t smem, int most, const NormArgs& a, cudaStream_t st) {
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess)
         return DCN_ERR_CUDA;
     return launch_dependent(kernel, dim3(grid), dim3(cta), smem, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
@@ -486,9 +499,11 @@ int run_as(const NormArgs& a, bool backward, cudaStream_t st) {
     const int cta = cta_of(a.threads);
     if (backward)
         return launch(norm_backward_kernel<T, V, kWarp, kMost, b>, grid_of(a.rows, a.channels, sizeof(T), kBackwardThreads), cta,
-                      (size_t)cta * Rows<T, V, 5, b>::kBytes + a.threads * kWeights, a, st);
+                      (size_t)cta * Rows<T, V, 5, b>::kBytes + a.threads * kWeights,
+                      kMost * (Rows<T, V, 5, b>::kBytes + kWeights), a, st);
     return launch(norm_forward_kernel<T, V, kWarp, kMost, f>, grid_of(a.rows, a.channels, sizeof(T), kForwardThreads), cta,
-                  (size_t)cta * Rows<T, V, 3, f>::kBytes + a.threads * kWeights, a, st);
+                  (size_t)cta * Rows<T, V, 3, f>::kBytes + a.threads * kWeights,
+                  kMost * (Rows<T, V, 3, f>::kBytes + kWeights), a, st);
 }
 
 template <typename T, int V>

@@ -4,16 +4,23 @@
 //     p_t = a_t p_{t+1} + a_t dy_t   (p behind the last step: dlast),   D_t = dy_t + p_{t+1}
 //     dx_t = D_t (1 - a_t),   dgate_t = D_t (h_{t-1} - x_t) a_t (1 - a_t),   dstate = p_0.
 //
-// Both directions are scans of affine maps h -> A h + B, whose composition is (A2 A1, A2 B1 + B2).  A lane has a pair of channels,
-// in the packed float32 instructions, and K steps of them: it composes its steps, the warps of a CTA (one behind the other in time)
-// compose theirs through shared memory and the CTAs of a cluster theirs through distributed shared memory, a warp for all; the
-// state that reaches a lane then gives all of its steps.  So x and gate are read once and y is written once, whatever the length:
-// the bound is DRAM.  A cluster walks the time axis in waves of (its CTAs) x 64 steps and carries the state from wave to wave in
-// registers.  Every warp copies its own steps of the next waves to shared memory meanwhile (cp.async, two stages), and sends its
-// results out from there: 16 bytes an instruction where addresses allow it, and no address arithmetic in the recurrence.
+// Both directions are scans of affine maps h -> A h + B, whose composition is (A2 A1, A2 B1 + B2).  A lane has a pair of
+// channels, in the packed float32 instructions, and K steps of them: it composes its steps, the warps of a CTA (one behind the
+// other in time) compose theirs through shared memory and the CTAs of a cluster theirs through distributed shared memory, a warp
+// for all; the state that reaches a lane then gives all of its steps.  So x and gate are read once and y is written once, whatever
+// the length.  A cluster walks the time axis in waves of (its CTAs) x 64 steps and carries the state from wave to wave in
+// registers.  Every warp copies its own steps of the next waves to shared memory meanwhile (cp.async, two waves ahead; the gates
+// of the backward pass one, which lets an SM hold four CTAs), and sends its results out from there: 16 bytes an instruction where
+// addresses allow it, and no address arithmetic in the recurrence.
 //
-// A state that lasts 10^4 steps has gates within 10^-4 of one, and what matters of them is 1 - a: the rounding of a alone would cost
-// it three digits.  So the product over a thread's steps is also formed as 1 - A = sum (1 - a_t) a_1 .. a_{t-1}, of which no
+// What bounds it depends on how many sequences there are.  Measured, bf16, against a copy of the same bytes at 6.5 TB/s:
+//     64 x 1024 x 2048 (2048 units, one CTA each)   forward 140 us (5.8 TB/s, 88 %)   backward 252 us (5.3 TB/s, 82 %): DRAM
+//     2 x 16384 x 2048 (64 units in clusters)       forward  98 us (4.2 TB/s, 64 %)   backward 148 us (4.6 TB/s, 70 %)
+// Few long sequences walk few clusters through many waves, and in each wave's exchange of maps its warps have nothing but copies
+// under way: latency, with DRAM 44 % busy and 53 % of the issue slots taken in the forward pass.
+//
+// A state that lasts 10^4 steps has gates within 10^-4 of one, and what matters of them is 1 - a: the rounding of a alone would
+// cost it three digits.  So the product over a thread's steps is also formed as 1 - A = sum (1 - a_t) a_1 .. a_{t-1}, of which no
 // term is a difference, and A is handed on as a float and the rest that its rounding left.
 //
 // The forward pass leaves the state before every 64th step; the backward pass recomputes the states in between from it, in
@@ -83,12 +90,12 @@ struct MapRoom {
     uint32_t more[32];
     static __device__ __forceinline__ uint32_t packed(Lanes more) { return word_of<__nv_bfloat16>(more.at(0), more.at(1)); }
     __device__ __forceinline__ void put(int lane, const Map& m) { ab[lane] = {m.a, m.b}, more[lane] = packed(m.more); }
-    __device__ __forceinline__ Map get(int lane) const {
-        const Pair p = ab[lane];
+    __device__ __forceinline__ Map get(int lane, Lanes b) const {                  // with another b: its own is not read
         const uint32_t w = more[lane];
         const float f[2] = {half_of<__nv_bfloat16>(w, 0), half_of<__nv_bfloat16>(w, 1)};
-        return {p.a, lanes(f), p.b};
+        return {ab[lane].a, lanes(f), b};
     }
+    __device__ __forceinline__ Map get(int lane) const { return get(lane, ab[lane].b); }
 };
 
 // Set where a wait for a map of another CTA gave up (which nothing but a fault of the GPU brings about)
@@ -96,8 +103,9 @@ __device__ unsigned int g_scan_status;
 constexpr long long kWaitCycles = 1ll << 32;                     // some two seconds
 
 // The exchange of maps in a cluster.  Each CTA sends its own to all (st.async, which counts its bytes on the barrier of the CTA it
-// goes to): a cluster barrier instead would hold every warp until its results of the wave before are in memory.  Two of
-// everything: a CTA sends a wave's map when all maps of the wave before have arrived, so the one it writes over has been read.
+// goes to): a cluster barrier instead holds every warp until its results of the wave before are in memory (2x16384x2048 bf16,
+// forward: 120 us with it, 101 us without).  Two of everything: a CTA sends a wave's map when all maps of the wave before have
+// arrived, so the one it writes over has been read.
 struct Exchange {
     MapRoom maps[2][kCluster];
     alignas(8) uint64_t arrived[2];
@@ -108,7 +116,8 @@ struct Exchange {
         for (int r = ranks; r < kCluster; ++r) maps[0][r].put(lane, identity()), maps[1][r].put(lane, identity());
         if (lane == 0) {
             gave_up = 0;
-            for (int s = 0; s < 2; ++s) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&arrived[s])) : "memory");
+            for (int s = 0; s < 2; ++s)
+                asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&arrived[s])) : "memory");
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         }
     }
@@ -147,7 +156,8 @@ struct Exchange {
         for (;;) {
             uint32_t ok;
             asm volatile(
-                "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
+                "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+                " selp.b32 %0, 1, 0, p;\n}"
                 : "=r"(ok)
                 : "r"(bar), "r"(parity)
                 : "memory");
@@ -291,7 +301,8 @@ __device__ __forceinline__ void zero_rest(const Place& me, T* out, int64_t from,
     Raw<kBytes> zero;
     memset(&zero, 0, sizeof(zero));
     const int row = B::row(me.lane, 0);
-    for (int64_t t = from + (int64_t)(me.rank * me.warps + me.warp) * kRows + row; t < steps; t += (int64_t)me.ranks * me.warps * kRows)
+    const int64_t all = (int64_t)me.ranks * me.warps * kRows;
+    for (int64_t t = from + (int64_t)(me.rank * me.warps + me.warp) * kRows + row; t < steps; t += all)
         for (int c = B::col(me.lane, 0); c < me.width; c += 32 * B::kPer) store(out + t * channels + c, zero);
 }
 
@@ -491,11 +502,7 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
             }
         }
         if (me.warp == 0) {                                        // the gradients, from the one that reaches the CTA's last step
-            auto back_map = [&](int w) {
-                Map m = room.part[w].get(me.lane);              // (its b may be gone)
-                m.b = room.back[w][me.lane];
-                return m;
-            };
+            auto back_map = [&](int w) { return room.part[w].get(me.lane, room.back[w][me.lane]); };
             Lanes g = carry;
             if (me.ranks > 1) {
                 Product product_of;
@@ -551,9 +558,13 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
     if (p.dstate != nullptr && me.rank == 0 && me.warp == 0) me.store(p.dstate, me.b, p.channels, carry);
 }
 
+// One step of each row's state, in place: W channels a thread, and as many threads as there are channels, for the fewest dependent
+// loads: gate and x, the slot, the state.  A call of 16 x 512 float32 takes 1.8 us on the GPU, most of it launch and two trips to
+// memory, and 4.6 us from call to call, which is the host's share.
 template <typename T, int W>
-__global__ void __launch_bounds__(128) scan_step_kernel(int64_t rows, int64_t channels, const T* x, int64_t x_row, const T* gate,
-                                                        int64_t gate_row, float* state, int64_t pool, const int64_t* slots, T* y) {
+__global__ void __launch_bounds__(128)
+    scan_step_kernel(int64_t rows, int64_t channels, const T* x, int64_t x_row, const T* gate, int64_t gate_row, float* state,
+                     int64_t pool, const int64_t* slots, T* y) {
     pdl_wait();
     const int64_t c = ((int64_t)blockIdx.x * 128 + threadIdx.x) * W;
     if (c >= channels) return;
@@ -603,12 +614,14 @@ int resident(K kernel, int threads) {
 }
 
 // As many warps as the steps fill, and CTAs along time as long as the GPU holds all of them at once: a cluster walks the whole
-// time axis, and one that had to wait for another would double the time.
+// time axis, and one that had to wait for another would double the time.  (Any number of them, and not powers of two alone: where
+// an SM held three CTAs, the backward pass of 2x16384x2048 bf16 took 156 us in clusters of six, 185 us in clusters of four.)
 template <typename K>
 int launch_scan(K kernel, int held, size_t smem, int per_thread, const ScanArgs& a, int64_t batch, cudaStream_t st) {
     if (held == 0) return DCN_ERR_CUDA;
     const int64_t units = batch * a.tiles;
-    const int warps = (int)(a.steps >= kChunk ? kChunk / per_thread : a.steps > per_thread ? (a.steps + per_thread - 1) / per_thread : 1);
+    const int64_t filled = (a.steps + per_thread - 1) / per_thread;
+    const int warps = (int)(a.steps >= kChunk ? kChunk / per_thread : filled > 1 ? filled : 1);
     int ranks = 1;
     while (ranks < kCluster && (int64_t)ranks * kChunk < a.steps && units * (ranks + 1) <= (int64_t)held * sm_count()) ++ranks;
     cudaLaunchConfig_t cfg = {};
@@ -662,7 +675,8 @@ int check_scan(const dcn_scan* p) {
     if (p->batch < 0 || p->steps < 0 || p->channels < 0) return DCN_ERR_SHAPE;
     constexpr int64_t most = 1ll << 31;
     if (p->batch >= most || p->steps >= most || p->channels >= most) return DCN_ERR_LIMIT;
-    if (p->batch * ((p->channels + kTile - 1) / kTile) >= 1ll << 27) return DCN_ERR_LIMIT;       // CTAs of a grid, eight to a cluster
+    // (CTAs of a grid, eight to a cluster)
+    if (p->batch * ((p->channels + kTile - 1) / kTile) >= 1ll << 27) return DCN_ERR_LIMIT;
     return DCN_OK;
 }
 
@@ -690,7 +704,8 @@ ScanArgs args_of(const dcn_scan* p) {
 
 int scan_check_status(cudaStream_t st) {
     unsigned int v = 0;
-    if (cudaStreamSynchronize(st) != cudaSuccess || cudaMemcpyFromSymbol(&v, g_scan_status, sizeof(v)) != cudaSuccess) return DCN_ERR_CUDA;
+    if (cudaStreamSynchronize(st) != cudaSuccess || cudaMemcpyFromSymbol(&v, g_scan_status, sizeof(v)) != cudaSuccess)
+        return DCN_ERR_CUDA;
     if (v == 0) return DCN_OK;
     const unsigned int zero = 0;
     cudaMemcpyToSymbol(g_scan_status, &zero, sizeof(zero));

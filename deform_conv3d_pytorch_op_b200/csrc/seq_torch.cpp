@@ -84,7 +84,8 @@ void shaped(const Tensor& t, const char* name, at::IntArrayRef want) {
 
 Tensor whole_numbers(const Tensor& t, const char* name) {
     if (!t.defined()) return t;
-    if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt) fail(std::string(name) + " must be int64 or int32, got " + dtype_name(t));
+    if (t.scalar_type() != at::kLong && t.scalar_type() != at::kInt)
+        fail(std::string(name) + " must be int64 or int32, got " + dtype_name(t));
     return t.to(at::kLong).contiguous();
 }
 
@@ -268,7 +269,8 @@ dcn_logits logits_of(const Numbers& n, const Tensor& logits, int64_t rows) {
 void check_logits(const Numbers& n, const Tensor& logits) {
     on_gpu(logits, "logits");
     type_of(logits, "logits");
-    if (logits.dim() < 1 || logits.size(-1) < 1) fail("logits have shape " + shape_text(logits.sizes()) + ", expected (..., vocabulary)");
+    if (logits.dim() < 1 || logits.size(-1) < 1)
+        fail("logits have shape " + shape_text(logits.sizes()) + ", expected (..., vocabulary)");
     if (!((float)n.temperature >= 1e-3f && (float)n.temperature <= 1e3f)) fail("temperature must lie between 1e-3 and 1e3");
 }
 
@@ -280,8 +282,8 @@ variable_list scores_forward(const Numbers& n, const variable_list& in, bool kee
     shaped(in[1], "tokens", lead);
     const Tensor tokens = whole_numbers(in[1], "tokens");
     if (n.top < 0 || n.top > DCN_SCORES_MOST_TOP || n.top > in[0].size(-1))
-        fail("top is " + std::to_string(n.top) + ": 0 to " + std::to_string((int)DCN_SCORES_MOST_TOP) + ", and at most the vocabulary's " +
-             std::to_string(in[0].size(-1)) + ", are supported");
+        fail("top is " + std::to_string(n.top) + ": 0 to " + std::to_string((int)DCN_SCORES_MOST_TOP) +
+             ", and at most the vocabulary's " + std::to_string(in[0].size(-1)) + ", are supported");
     const int64_t rows = product(lead);
     const Tensor logits = rows_of(in[0], rows, in[0].size(-1));
     const dcn_logits p = logits_of(n, logits, rows);
@@ -319,7 +321,8 @@ variable_list scores_backward(const Numbers& n, const variable_list& kept, const
 // logits, teacher_logprobs, teacher_tokens -> loss
 variable_list distill_forward(const Numbers& n, const variable_list& in, bool keep, variable_list& kept) {
     check_logits(n, in[0]);
-    if (in[0].size(-1) > DCN_DISTILL_MOST_VOCAB) fail("the vocabulary is limited to " + std::to_string((int)DCN_DISTILL_MOST_VOCAB) + " tokens");
+    if (in[0].size(-1) > DCN_DISTILL_MOST_VOCAB)
+        fail("the vocabulary is limited to " + std::to_string((int)DCN_DISTILL_MOST_VOCAB) + " tokens");
     const std::vector<int64_t> lead = without_last(in[0]);
     beside(in[1], "teacher_logprobs", in[0], "logits");
     beside(in[2], "teacher_tokens", in[0], "logits");
@@ -425,7 +428,8 @@ variable_list call(const Operator& op, const Numbers& n, const variable_list& in
     need = need && at::GradMode::is_enabled();
     for (size_t i = op.differentiable; i < in.size(); ++i)
         if (in[i].defined() && in[i].requires_grad() && at::GradMode::is_enabled())
-            fail(std::string("there is no gradient with respect to ") + (&op == &kDistill ? "the teacher" : "this input") + ": detach it");
+            fail(std::string("there is no gradient with respect to ") + (&op == &kDistill ? "the teacher" : "this input") +
+                 ": detach it");
     variable_list kept;
     if (!need) {
         at::NoGradGuard no_grad;
