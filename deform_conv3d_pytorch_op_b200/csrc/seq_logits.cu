@@ -113,7 +113,8 @@ template <typename T>
 __device__ __forceinline__ int mark_of(const Row<T>& row, int e) { return e - row.head - row.v0 * Row<T>::kPer + 8; }
 template <typename T>
 __device__ __forceinline__ bool in_part(const Row<T>& row, int e) {
-    return e < row.head ? e < row.head_here : e >= row.tail || (e >= row.head + row.v0 * Row<T>::kPer && e < row.head + row.v1 * Row<T>::kPer);
+    return e < row.head ? e < row.head_here
+                        : e >= row.tail || (e >= row.head + row.v0 * Row<T>::kPer && e < row.head + row.v1 * Row<T>::kPer);
 }
 
 template <bool kU>
@@ -150,7 +151,9 @@ __device__ __noinline__ Sums add_elements(Sums a, const Row<T>& row, int e0, int
 template <typename T>
 struct Word {
     static constexpr int kPer = 4 / sizeof(T);
-    static constexpr uint32_t kNothing = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u : 0xfc00fc00u;
+    static constexpr uint32_t kNothing = sizeof(T) == 4                            ? 0xff800000u
+                                         : std::is_same<T, __nv_bfloat16>::value ? 0xff80ff80u
+                                                                                 : 0xfc00fc00u;
     static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) {
         uint32_t r;
         if constexpr (sizeof(T) == 4) r = __float_as_uint(max_nan(__uint_as_float(a), __uint_as_float(b)));
@@ -434,7 +437,8 @@ __device__ __noinline__ uint32_t exact_bound(const Row<T>& row, int tid, int top
 
 // Entries of the first `need` elements that are on the bound, by index: a vector a thread at a time
 template <typename T, int kT>
-__device__ __noinline__ void first_on_bound(const Row<T>& row, int tid, int need, uint32_t bound, TopRoom<kT>& r, unsigned long long* out) {
+__device__ __noinline__ void first_on_bound(const Row<T>& row, int tid, int need, uint32_t bound, TopRoom<kT>& r,
+                                            unsigned long long* out) {
     constexpr int kPer = Row<T>::kPer;
     int done = 0;
     // a thread's place from a prefix sum of the counts, threads being in the order of their elements
@@ -506,12 +510,13 @@ __device__ __forceinline__ uint32_t bound_of(TopRoom<kT>& r, int n, int tid, int
     return r.bound;
 }
 
-// Where the list cannot hold what reaches the bound (many equal values, or large ones all in few lanes' hands): the `top` largest of a
-// CTA's part, in order, into out[0, top) (0 behind the last).  If they do not fit either, the value of the part's last place is
-// found by bisection.  Fewer than `top` elements are larger and are listed; the places behind them go to the lowest indices that have
-// the value.
+// Where the list cannot hold what reaches the bound (many equal values, or large ones all in few lanes' hands): the `top` largest
+// of a CTA's part, in order, into out[0, top) (0 behind the last).  If they do not fit either, the value of the part's last place is
+// found by bisection.  Fewer than `top` elements are larger and are listed; the places behind them go to the lowest indices that
+// have the value.
 template <typename T, int kT>
-__device__ __noinline__ void top_of_part(const Row<T>& row, int tid, int top, uint32_t bound, int reach, TopRoom<kT>& r, unsigned long long* out) {
+__device__ __noinline__ void top_of_part(const Row<T>& row, int tid, int top, uint32_t bound, int reach, TopRoom<kT>& r,
+                                         unsigned long long* out) {
     __syncthreads();
     if (tid < top) out[tid] = 0;
     if (tid == 0) r.n = 0;
@@ -573,52 +578,51 @@ __device__ __forceinline__ float product_or_zero(float p, float v) { return p > 
 struct TeacherRoom {
     int token[kMostK];                           // -1: not used
     float log_q[kMostK], logit[kMostK];
+    int repeats;                                 // not 0: a token may be there twice
 };
 
-// The teacher's places of a row: tokens and log q (normalised over them where there is no tail)
-template <typename T, typename Team>
-__device__ __forceinline__ float teacher_of(const LogitsArgs& p, int64_t row, Team& team, TeacherRoom& r, int& used) {
-    int n = 0;
-    float m = kNone;
-    for (int i = team.tid; i < p.places; i += team.threads) {
-        const int64_t t = gload_i64(p.teacher_tokens + row * p.places + i);
-        const bool in = t >= 0 && t < p.vocab;
-        const float lq = in ? teacher_at<T>(p, row * p.places + i) : kNone;
-        r.token[i] = in ? (int)t : -1;
-        r.log_q[i] = lq;
-        n += in;
-        m = max_nan(m, lq);
+// The row's loss and statistics, by a warp, from the teacher's places and the student's sums over the other tokens
+__device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, int lane, TeacherRoom& r, Sums rest) {
+    const auto largest = [](float v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    };
+    const auto total = [](float v) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    float top = kNone, norm = 0.0f;
+    bool used = false;
+    for (int i = lane; i < p.places; i += 32) {
+        used |= r.token[i] >= 0;
+        top = max_nan(top, r.log_q[i]);
     }
-    used = (int)team.sum((float)n);
-    float norm = 0.0f;
-    if (!p.tail) {
-        m = team.max(m);
+    used = __any_sync(0xffffffffu, used);
+    if (!p.tail) {                               // log q normalised over the places
+        top = largest(top);
         float s = 0.0f;
-        for (int i = team.tid; i < p.places; i += team.threads) s += m == kNone ? 0.0f : expf(r.log_q[i] - m);
-        norm = m == kNone ? 0.0f : m + logf(team.sum(s));
-        if (m == kNone) used = 0;                // no probability anywhere: as if no place were used
-        for (int i = team.tid; i < p.places; i += team.threads) r.log_q[i] -= norm;
+        for (int i = lane; i < p.places; i += 32) s += top == kNone ? 0.0f : expf(r.log_q[i] - top);
+        if (top != kNone) norm = top + logf(total(s));
+        else used = false;                       // no probability anywhere: as if no place were used
+        for (int i = lane; i < p.places; i += 32) r.log_q[i] -= norm;
     }
-    team.sync();
-    return norm;
-}
-
-// The row's loss and statistics, by a warp, from the student's sums over the other tokens
-__device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, Team<true>& team, const TeacherRoom& r, Sums rest,
-                                            float norm, int used) {
     // the student's sums over the teacher's tokens, each token once
     Sums best{kNone, 0.0f, 0.0f};
     float mass = 0.0f;
-    for (int i = team.tid; i < p.places; i += team.threads) {
+    for (int i = lane; i < p.places; i += 32) {
         const int t = r.token[i];
         if (t < 0) continue;
         mass += expf(r.log_q[i]);
         bool again = false;
-        for (int j = 0; j < i; ++j) again |= r.token[j] == t;
+        if (r.repeats != 0)
+            for (int j = 0; j < i; ++j) again |= r.token[j] == t;
         if (!again) add_one<false>(best, r.logit[i], p.k);
     }
-    best = team.join(best, p.k);
-    mass = team.sum(mass);
+    best.rescale(largest(best.m), p.k);
+    best.s = total(best.s);
+    mass = total(mass);
     const float m = max_nan(best.m, rest.m);
     Sums all = best, other = rest;
     if (m != kNone) {
@@ -627,13 +631,13 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, Te
     }
     const float log_s = log2f(all.s + other.s), rest_log_s = log2f(rest.s);
     float loss = 0.0f;
-    for (int i = team.tid; i < p.places; i += team.threads) {
+    for (int i = lane; i < p.places; i += 32) {
         if (r.token[i] < 0) continue;
         const float lq = r.log_q[i];
         loss += product_or_zero(expf(lq), lq - log_p(r.logit[i], m, log_s, p));
     }
-    loss = team.sum(loss);
-    if (team.tid != 0) return;
+    loss = total(loss);
+    if (lane != 0) return;
     float q_rest = 0.0f, c = 0.0f;
     if (p.tail && rest.m != kNone) q_rest = fmaxf(1.0f - mass, 0.0f);
     if (mass != mass) q_rest = mass;
@@ -642,7 +646,7 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, Te
         loss += product_or_zero(q_rest, logf(q_rest) - log_rest);
         c = fmaf(mass + q_rest, expf(log_rest), -q_rest);
     }
-    if (used == 0) loss = c = mass = q_rest = 0.0f;
+    if (!used) loss = c = mass = q_rest = 0.0f;
     p.loss[row] = loss * p.temperature * p.temperature;
     if (p.stats != nullptr) {
         float* s = p.stats + row * DCN_LOGITS_STATS;
@@ -673,8 +677,7 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
     constexpr int kWarps = kT / 32;
     TeacherRoom& teacher = teachers[kKind == kDistill ? group : 0];
     uint8_t* marks = dynamic + group * p.marks;
-    float norm = 0.0f, given = CUDART_NAN_F;
-    int used = 0;
+    float given = CUDART_NAN_F;
     int64_t token = p.ignore;
     if constexpr (kKind != kDistill) {           // (on its way while the row is read)
         if (team.tid == 0 && rank == 0 && p.logprob != nullptr) {
@@ -682,21 +685,55 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
             if (token >= 0 && token < p.vocab) given = row.one(token);
         }
     }
+    // The teacher's places, one or (in a warp's row) up to four a thread.  What the sums need of them are the marks; the student's
+    // logits there are on their way while the row is read.
+    constexpr int kPlaces = kKind != kDistill ? 1 : kWarp ? kMostK / 32 : 1;
+    float at_place[kPlaces];
+    if constexpr (kKind == kDistill && !kWarp) {  // (the row's beginning is on its way to L2 while the marks are made: 1 to 3 %)
+        if (team.tid == 0 && row.v1 > row.v0)
+            asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(row.vec(row.v0)),
+                         "r"(min(row.v1 - row.v0, 2048) * 16)
+                         : "memory");
+    }
     if constexpr (kKind == kDistill) {
-        for (int i = team.tid; i < p.marks / 4; i += team.threads) reinterpret_cast<uint32_t*>(marks)[i] = 0;
-        norm = teacher_of<T>(p, at, team, teacher, used);
-        for (int i = team.tid; i < p.places; i += team.threads) {
-            const int t = teacher.token[i];
-            if (t < 0) continue;
-            if (rank == 0) teacher.logit[i] = row.one(t);
-            if (in_part(row, t)) {
-                const int b = mark_of(row, t);
-                atomicOr(reinterpret_cast<uint32_t*>(marks) + (b >> 5), 1u << (b & 31));
+        int64_t t[kPlaces];
+        float lq[kPlaces];
+#pragma unroll
+        for (int q = 0; q < kPlaces; ++q) {
+            const int i = team.tid + q * team.threads;
+            t[q] = i < p.places ? gload_i64(p.teacher_tokens + at * p.places + i) : -1;
+            lq[q] = i < p.places ? teacher_at<T>(p, at * p.places + i) : kNone;
+        }
+        for (int i = team.tid; i < p.marks / 16; i += team.threads) reinterpret_cast<uint4*>(marks)[i] = make_uint4(0, 0, 0, 0);
+        if (team.tid == 0) teacher.repeats = ranks > 1;          // (no CTA of a cluster sees all places)
+        team.sync();
+#pragma unroll
+        for (int q = 0; q < kPlaces; ++q) {
+            const int i = team.tid + q * team.threads;
+            const bool in = t[q] >= 0 && t[q] < p.vocab;
+            at_place[q] = in && rank == 0 ? row.one(t[q]) : kNone;
+            if (i < p.places) {
+                teacher.token[i] = in ? (int)t[q] : -1;
+                teacher.log_q[i] = in ? lq[q] : kNone;
+            }
+            if (in && in_part(row, (int)t[q])) {
+                const int b = mark_of(row, (int)t[q]);
+                const uint32_t bit = 1u << (b & 31);
+                if (atomicOr(reinterpret_cast<uint32_t*>(marks) + (b >> 5), bit) & bit) teacher.repeats = 1;
             }
         }
         team.sync();
     }
-    const Sums mine = sums_of<T, kKind != kDistill, kKind == kDistill, kKind == kScoresTop>(row, team.tid, team.threads, p.k, marks);
+    const Sums mine =
+        sums_of<T, kKind != kDistill, kKind == kDistill, kKind == kScoresTop>(row, team.tid, team.threads, p.k, marks);
+    if constexpr (kKind == kDistill) {
+#pragma unroll
+        for (int q = 0; q < kPlaces; ++q) {
+            const int i = team.tid + q * team.threads;
+            if (i < p.places) teacher.logit[i] = at_place[q];
+        }
+        __syncwarp();                            // (a CTA's row: the barriers of the join)
+    }
     Sums sums = team.join(mine, p.k);
     if constexpr (kKind == kScoresTop) {
         const int warp = team.tid / 32;
@@ -771,8 +808,7 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
         sums.u = __shfl_sync(0xffffffffu, part.u, 0);
     }
     if constexpr (kKind == kDistill) {
-        Team<true> warp{room, (int)threadIdx.x % 32, 32};
-        if (kWarp || team.tid < 32) distill_row(p, at, warp, teacher, sums, norm, used);
+        if (kWarp || team.tid < 32) distill_row(p, at, team.tid, teacher, sums);
     } else {
         const float log_s = log2f(sums.s);
         const float entropy = sums.m == kNone ? 0.0f : kLn2 * (log_s - sums.u / sums.s);
@@ -900,7 +936,8 @@ __global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const Logi
     }
     // vectors where the gradient's rows start as the logits' do, elements otherwise and in rows that are far or zero
     constexpr int kBatch = 4;
-    const bool vectors = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(row.p) % 16 && !slope.zero && !slope.shift.far;
+    const bool alike = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(row.p) % 16;
+    const bool vectors = alike && !slope.zero && !slope.shift.far;
     T* to = out + row.head;
     for (int v = row.v0 + tid; v < row.v1; v += kBatch * threads) {
         if (vectors && v + (kBatch - 1) * threads < row.v1) {
@@ -1009,7 +1046,9 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
         e = cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, true, 32 * kWarpRows>, a);
     } else {
         const auto kernel = logits_forward_kernel<T, kKind, false, kThreads>;
-        if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        // (the same for every call, so that calls of several host threads do not take it from one another)
+        constexpr int most = (DCN_DISTILL_MOST_VOCAB / 8 + 1024) / 16 * 16;
+        if (smem > 40 * 1024) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
         if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, kernel, a);
     }
     return e != cudaSuccess || cudaGetLastError() != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;

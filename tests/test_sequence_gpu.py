@@ -595,3 +595,36 @@ def test_refusals():
     for shape in ((2, 0), (0,)):
         with pytest.raises(E):
             scores(torch.zeros(shape, device="cuda"))
+
+
+def test_sizes_of_several_host_threads():
+    """Calls of one kernel with different amounts of shared memory at the same time"""
+    import threading
+    g = gen(91)
+    norms = [randn(g, 8, c) for c in (300, 700, 1300, 2000)]
+    wants = [dcn.ResidualNormFunction.apply(x, x) for x in norms]
+    rows = [(randn(g, 300, v, dtype=torch.bfloat16), torch.randint(0, v, (300, 2), generator=g, device="cuda")) for v in (340000, 400000)]
+    q = torch.full((300, 2), math.log(0.25), device="cuda")
+    losses = [dcn.DistillTopkFunction.apply(x, q, t) for x, t in rows]
+    torch.cuda.synchronize()
+    start, bad = threading.Barrier(4), []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait(30)
+                for _ in range(400):
+                    got = dcn.ResidualNormFunction.apply(norms[i], norms[i])
+                for _ in range(20):
+                    loss = dcn.DistillTopkFunction.apply(rows[i % 2][0], q, rows[i % 2][1])
+                torch.cuda.current_stream().synchronize()
+                assert all(torch.equal(a, b) for a, b in zip(got, wants[i])) and torch.equal(loss, losses[i % 2])
+        except Exception as e:                   # reported by the test's own thread
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
