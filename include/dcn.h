@@ -236,8 +236,8 @@ int dcn_debug_tc_points(const dcn_problem* p, const void* offset, int32_t n, voi
  * dcn_check_status reports DCN_ERR_TIMEOUT.  No counterpart in the reference (its kernels have no error path). */
 int dcn_debug_expire_wait(int32_t* gave_up, void* stream);
 
-/* Reads and clears the sticky device-side status word of the tensor-core kernels (bounded waits that
- * gave up).  Synchronises `stream`.  DCN_OK or DCN_ERR_TIMEOUT. */
+/* Reads and clears the sticky device-side status word of the tensor-core kernels and of the gated scan of
+ * dcn_seq.h (bounded waits that gave up).  Synchronises `stream`.  DCN_OK or DCN_ERR_TIMEOUT. */
 int dcn_check_status(void* stream);
 
 /* ---------------------------------------------------------------------------------------------
