@@ -60,7 +60,8 @@ __device__ __forceinline__ void store(void* p, const Raw<16>& r) {
 
 // A result that is not read again soon: it does not push out of L2 what is
 __device__ __forceinline__ void store_streaming(void* p, const Raw<16>& r) {
-    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(r.u[0]), "r"(r.u[1]), "r"(r.u[2]), "r"(r.u[3]) : "memory");
+    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(r.u[0]), "r"(r.u[1]), "r"(r.u[2]), "r"(r.u[3])
+                 : "memory");
 }
 
 __device__ __forceinline__ int64_t gload_i64(const int64_t* p) {
@@ -194,7 +195,8 @@ __device__ __forceinline__ uint32_t shared_address(const void* p) { return (uint
 template <int kBytes>
 __device__ __forceinline__ void copy_async(void* to, const void* from, bool in) {
     if constexpr (kBytes == 16)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(to)), "l"(from), "r"(in ? 16 : 0) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(to)), "l"(from), "r"(in ? 16 : 0)
+                     : "memory");
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(shared_address(to)), "l"(from), "n"(kBytes),
                      "r"(in ? kBytes : 0)
@@ -206,6 +208,15 @@ __device__ __forceinline__ void copy_async_all(void* to, const void* from) {
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_address(to)), "l"(from) : "memory");
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(shared_address(to)), "l"(from), "n"(kBytes) : "memory");
+}
+// the first `bytes` of kBytes, zeros behind them
+template <int kBytes>
+__device__ __forceinline__ void copy_async_some(void* to, const void* from, int bytes) {
+    if constexpr (kBytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(to)), "l"(from), "r"(bytes) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(shared_address(to)), "l"(from), "n"(kBytes), "r"(bytes)
+                     : "memory");
 }
 __device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 // all of the thread's groups but the `kLast` issued last

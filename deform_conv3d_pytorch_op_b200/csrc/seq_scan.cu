@@ -210,56 +210,149 @@ __device__ __forceinline__ int64_t length_of(const ScanArgs& p, int64_t b) {
     return n < 0 ? 0 : n > p.steps ? p.steps : n;
 }
 
-// K steps of the CTA's channels in shared memory, a warp's own, moved kBytes at a time
+// Where rows start on 4 bytes or in the middle of them (kBytes 2): 0 or 1 element, for the even and the odd ones behind step t0
+template <typename T, int kBytes>
+struct Skew {
+    int even = 0, odd = 0;
+    __device__ __forceinline__ Skew(const T* base, int64_t t0, int64_t stride) {
+        if constexpr (kBytes == 2) {
+            even = (int)(((unsigned)(reinterpret_cast<uintptr_t>(base) / 2) + (unsigned)t0 * (unsigned)stride) & 1);
+            odd = (even + (int)stride) & 1;
+        }
+    }
+    __device__ __forceinline__ int at(int t) const { return kBytes == 2 ? (t % 2 == 0 ? even : odd) : 0; }
+};
+
+// K steps of the CTA's channels in shared memory, a warp's own.  They come and go 16 bytes at a time, or 4 where that is what all
+// rows start on.  16-bit rows that start in the middle of 4 bytes (kBytes 2) move 4 bytes at a time too: they arrive in shared memory
+// with their skew, which align() takes out, and the elements at their ends that share 4 bytes with others leave on their own.
+// Measured, bf16, forward and backward: 64x1024x2046 183 and 416 us, 64x1024x2047 248 and 500 us (378 and 682 us element by element),
+// against 143 and 255 us at 2048 channels: four times the copies, in a kernel whose issue slots are two thirds taken.
 template <typename T, int kBytes, int K>
 struct Block {
-    T v[K][kTile];
-    static constexpr int kPer = kBytes / (int)sizeof(T), kCols = kTile / kPer, kMoves = K * kCols / 32;
-    static __device__ __forceinline__ int row(int lane, int j) { return kCols <= 32 ? lane / kCols + j * (32 / kCols) : j / 2; }
-    static __device__ __forceinline__ int col(int lane, int j) {
-        return kCols <= 32 ? lane % kCols * kPer : (lane + 32 * (j % 2)) * kPer;
-    }
-    static constexpr int kRows = kCols <= 32 ? 32 / kCols : 1;    // of one move
-    // from step t0 on; zeros behind the sequence's end and the last channel
-    __device__ __forceinline__ void fill(const T* base, int64_t t0, int64_t stride, int64_t len, int width, int lane) {
-        if (kBytes == 16 && kCols <= 32 && width == kTile && t0 + K <= len) {
-            const T* from = base + (t0 + row(lane, 0)) * stride + col(lane, 0);
-            T* to = &v[row(lane, 0)][col(lane, 0)];
+    static constexpr int kMove = kBytes == 2 ? 4 : kBytes, kPer = kMove / (int)sizeof(T), kSlots = kTile / kPer;
+    static constexpr int kRows = kSlots <= 32 ? 32 / kSlots : 1;  // rows of a move
+    static constexpr int kMoves = K * kSlots / 32, kHalves = kSlots <= 32 ? 1 : kSlots / 32;       // kHalves: moves of a row
+    T v[K][kTile + (kBytes == 2 ? 2 : 0)];
+    static __device__ __forceinline__ int row(int lane, int j) { return kSlots <= 32 ? lane / kSlots + j * kRows : j / kHalves; }
+    static __device__ __forceinline__ int slot(int lane, int j) { return kSlots <= 32 ? lane % kSlots : lane + 32 * (j % kHalves); }
+    // from step t0 on; zeros behind the sequence's end.  left: channels to the tensor's end; what lies behind them is left as it is.
+    __device__ __forceinline__ void fill(const T* tensor, const T* base, int64_t t0, int64_t stride, int64_t len, int left,
+                                         int lane) {
+        const Skew<T, kBytes> skew(base, t0, stride);
+        const T* q = base + t0 * stride;
+        const bool all = t0 + K <= len;
+        if (kBytes == 2 && all && q - 1 >= tensor) {
 #pragma unroll
-            for (int j = 0; j < kMoves; ++j, from += kRows * stride)
-                copy_async_all<16>(to + j * kRows * kTile, from);
+            for (int p = 0; p < 2; ++p) {
+                const int bytes = min(2 * (left + skew.at(p) - 2 * lane), 4);
+                const T* from = q + p * stride - skew.at(p) + 2 * lane;
+                if (bytes > 0)
+#pragma unroll
+                    for (int i = 0; i < K / 2; ++i, from += 2 * stride) copy_async_some<4>(&v[2 * i + p][2 * lane], from, bytes);
+            }
+            if (lane < K && skew.at(lane) != 0 && left >= kTile)
+                copy_async_some<4>(&v[lane][kTile], q + lane * stride - 1 + kTile, left > kTile ? 4 : 2);
             return;
         }
+        if (kBytes != 2 && all) {
 #pragma unroll
-        for (int j = 0; j < kMoves; ++j) {
-            const int r = row(lane, j), c = col(lane, j);
-            const bool in = t0 + r < len && c < width;
-            const T* from = in ? base + (t0 + r) * stride + c : base;
-            if constexpr (kBytes >= 4) {
-                copy_async<kBytes>(&v[r][c], from, in);
-            } else {
+            for (int h = 0; h < kHalves; ++h) {
+                const T* from = q + row(lane, 0) * stride + slot(lane, h) * kPer;
+                if (slot(lane, h) * kPer < left)
+#pragma unroll
+                    for (int j = h; j < kMoves; j += kHalves, from += kRows * stride)
+                        copy_async_all<kMove>(&v[row(lane, j)][slot(lane, j) * kPer], from);
+            }
+            return;
+        }
+#pragma unroll 1
+        for (int j = lane; j < K * (kSlots + (kBytes == 2)); j += 32) {
+            const int r = kBytes == 2 ? j / (kSlots + 1) : j / kSlots, i = kBytes == 2 ? j % (kSlots + 1) : j % kSlots;
+            const int sk = skew.at(r);
+            const T* from = q + r * stride - sk + i * kPer;
+            const int there = t0 + r < len ? left + sk - i * kPer : 0;
+            if (kBytes != 2 || from >= tensor || there <= 0) {
+                const T* any = reinterpret_cast<const T*>(reinterpret_cast<uintptr_t>(tensor) / kMove * kMove);
+                copy_async_some<kMove>(&v[r][i * kPer], there > 0 ? from : any,
+                                       there <= 0 ? 0 : there >= kPer ? kMove : there * (int)sizeof(T));
+            } else {                             // nothing is read that lies before the tensor
                 Pack<T, 1> one;
-                one.zero();
-                if (in) one.get(from);
-                *reinterpret_cast<uint16_t*>(&v[r][c]) = one.raw.u;
+                one.get(tensor);
+                *reinterpret_cast<Raw<sizeof(T)>*>(&v[r][1]) = one.raw;
+            }
+        }
+    }
+    // Rows t0, ..., t0 + K - 1 of a tensor's `steps`, from word(row, move, skew) and one(row, channel)
+    template <typename F, typename G>
+    static __device__ __forceinline__ void send(T* base, int64_t t0, int64_t stride, int64_t steps, int width, int lane, F&& word,
+                                                G&& one) {
+        const Skew<T, kBytes> skew(base, t0, stride);
+        T* q = base + t0 * stride;
+        const bool all = t0 + K <= steps;
+        if constexpr (kBytes == 2) {
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {        // (behind a skew, a lane's word has its second element and the next lane's first)
+                const int sk = skew.at(p);
+                T* to = q + p * stride + sk + 2 * lane;
+                if (2 * lane + sk + 1 >= width) continue;
+                if (all) {
+#pragma unroll
+                    for (int i = 0; i < K / 2; ++i, to += 2 * stride) store(to, word(2 * i + p, lane, sk));
+                } else {
+#pragma unroll 1
+                    for (int r = p; r < K && t0 + r < steps; r += 2, to += 2 * stride) store(to, word(r, lane, sk));
+                }
+            }
+            // the first element behind a skew, and the last where words end before it
+            const int r = lane / 2, sk = skew.at(r);
+            if (r < K && t0 + r < steps && (lane % 2 == 0 ? sk : (width + sk) % 2) != 0) {
+                const int c = lane % 2 == 0 ? 0 : width - 1;
+                store(q + r * stride + c, one(r, c));
+            }
+        } else {
+#pragma unroll
+            for (int h = 0; h < kHalves; ++h) {
+                T* to = q + row(lane, 0) * stride + slot(lane, h) * kPer;
+                if (slot(lane, h) * kPer >= width) continue;
+                if (all) {
+#pragma unroll
+                    for (int j = h; j < kMoves; j += kHalves, to += kRows * stride) store(to, word(row(lane, j), slot(lane, j), 0));
+                } else {
+#pragma unroll 1
+                    for (int j = h; j < kMoves; j += kHalves, to += kRows * stride)
+                        if (t0 + row(lane, j) < steps) store(to, word(row(lane, j), slot(lane, j), 0));
+                }
             }
         }
     }
     // to the steps before `steps`
     __device__ __forceinline__ void drain(T* base, int64_t t0, int64_t stride, int64_t steps, int width, int lane) const {
-        if (kBytes == 16 && kCols <= 32 && width == kTile && t0 + K <= steps) {
-            T* to = base + (t0 + row(lane, 0)) * stride + col(lane, 0);
-            const T* from = &v[row(lane, 0)][col(lane, 0)];
+        send(base, t0, stride, steps, width, lane,
+             [&](int r, int i, int skew) {
+                 Raw<kMove> w = *reinterpret_cast<const Raw<kMove>*>(&v[r][i * kPer]);
+                 if (kBytes == 2 && skew != 0) w.u[0] = __funnelshift_r(w.u[0], word(r, i + 1), 16);
+                 return w;
+             },
+             [&](int r, int c) { return *reinterpret_cast<const Raw<sizeof(T)>*>(&v[r][c]); });
+    }
+    __device__ __forceinline__ uint32_t& word(int r, int i) { return reinterpret_cast<uint32_t*>(&v[r][0])[i]; }
+    __device__ __forceinline__ const uint32_t& word(int r, int i) const { return reinterpret_cast<const uint32_t*>(&v[r][0])[i]; }
+    // takes the rows' skew out, once they have arrived
+    __device__ __forceinline__ void align(const T* base, int64_t t0, int64_t stride, int lane) {
+        if constexpr (kBytes == 2) {
+            const Skew<T, kBytes> skew(base, t0, stride);
 #pragma unroll
-            for (int j = 0; j < kMoves; ++j, to += kRows * stride)
-                store(to, *reinterpret_cast<const Raw<kBytes>*>(from + j * kRows * kTile));
-            return;
-        }
+            for (int p = 0; p < 2; ++p) {
+                if (skew.at(p) == 0) continue;
+                uint32_t w[K / 2];
 #pragma unroll
-        for (int j = 0; j < kMoves; ++j) {
-            const int r = row(lane, j), c = col(lane, j);
-            const Raw<kBytes> one = *reinterpret_cast<const Raw<kBytes>*>(&v[r][c]);
-            if (t0 + r < steps && c < width) store(base + (t0 + r) * stride + c, one);
+                for (int i = 0; i < K / 2; ++i) w[i] = __funnelshift_r(word(2 * i + p, lane), word(2 * i + p, lane + 1), 16);
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < K / 2; ++i) word(2 * i + p, lane) = w[i];
+            }
+            __syncwarp();
         }
     }
     __device__ __forceinline__ Pack<T, 2> get(int k, int lane) const {
@@ -296,14 +389,12 @@ __device__ __forceinline__ void gates_of(const Pack<T, 2>& g, bool in, Lanes& a,
 // Zeros from step `from` on, shared out over the warps of the cluster
 template <typename T, int kBytes>
 __device__ __forceinline__ void zero_rest(const Place& me, T* out, int64_t from, int64_t steps, int64_t channels) {
-    using B = Block<T, kBytes, 1>;
-    constexpr int kRows = B::kRows;              // of a warp at a time
-    Raw<kBytes> zero;
-    memset(&zero, 0, sizeof(zero));
-    const int row = B::row(me.lane, 0);
+    using B = Block<T, kBytes, 4>;
+    constexpr int kRows = 4;                     // of a warp at a time
     const int64_t all = (int64_t)me.ranks * me.warps * kRows;
-    for (int64_t t = from + (int64_t)(me.rank * me.warps + me.warp) * kRows + row; t < steps; t += all)
-        for (int c = B::col(me.lane, 0); c < me.width; c += 32 * B::kPer) store(out + t * channels + c, zero);
+    for (int64_t t = from + (int64_t)(me.rank * me.warps + me.warp) * kRows; t < steps; t += all)
+        B::send(out, t, channels, steps, me.width, me.lane, [](int, int, int) { return Raw<B::kMove>{}; },
+                [](int, int) { return Raw<sizeof(T)>{}; });
 }
 
 template <typename T, int kBytes, int K>
@@ -331,9 +422,11 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
     const int chunk = me.warps * K, wave = me.ranks * chunk;
     int64_t t0 = (int64_t)me.rank * chunk + me.warp * K;           // my first step of this wave
     int64_t begin = 0;
-    auto fill = [&](auto& block, const T* from, int64_t t, int64_t stride) {
-        if (t - me.rank * chunk - me.warp * K < len) block.fill(from, t, stride, len, me.width, me.lane);
-        copies_issued();                                           // (a wave that does not come is not filled)
+    const int left = (int)(p.channels - me.c < 2 * kTile ? p.channels - me.c : 2 * kTile);
+    auto fill = [&](auto& block, const void* tensor, const T* from, int64_t t, int64_t stride) {
+        if (t - me.rank * chunk - me.warp * K < len)               // (a wave that does not come is not filled)
+            block.fill(static_cast<const T*>(tensor), from, t, stride, len, left, me.lane);
+        copies_issued();
     };
     if (me.warp == 0) {
         if (me.ranks > 1) room.cluster.begin(me.lane, me.ranks);
@@ -342,14 +435,16 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
         }
     }
     for (int s = 0; s < 2; ++s) {
-        fill(room.gate[s][me.warp], gate, t0 + s * wave, p.gate_step);
-        fill(room.x[s][me.warp], x, t0 + s * wave, p.x_step);
+        fill(room.gate[s][me.warp], p.gate, gate, t0 + s * wave, p.gate_step);
+        fill(room.x[s][me.warp], p.x, x, t0 + s * wave, p.x_step);
     }
     if (me.ranks > 1) cg::this_cluster().sync();                   // every CTA runs before another writes to its memory
     for (int side = 0, n = 0; begin < len; begin += wave, t0 += wave, side ^= 1, ++n) {
         auto &bx = room.x[side][me.warp], &bg = room.gate[side][me.warp];
         copies_arrived<2>();
         __syncwarp();
+        bg.align(gate, t0, p.gate_step, me.lane);
+        bx.align(x, t0, p.x_step, me.lane);
         // after each of my steps: y = A h + B of the state h before the first
         Lanes A[K], B[K], sum = all_lanes(0.0f);
         Product product;
@@ -396,7 +491,7 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
             }
             if (me.ranks == 1) carry = h;
         }
-        fill(bg, gate, t0 + 2 * wave, p.gate_step);
+        fill(bg, p.gate, gate, t0 + 2 * wave, p.gate_step);
         __syncthreads();
         const Lanes mine = room.start[me.warp][me.lane];
 #pragma unroll
@@ -408,7 +503,7 @@ __global__ void __launch_bounds__(32 * (kChunk / K), 4) scan_forward_kernel(cons
         __syncwarp();
         bx.drain(y, t0, p.channels, p.steps, me.width, me.lane);
         __syncwarp();
-        fill(bx, x, t0 + 2 * wave, p.x_step);
+        fill(bx, p.x, x, t0 + 2 * wave, p.x_step);
     }
     copies_arrived<0>();
     if (me.ranks > 1) cg::this_cluster().sync();                   // (no CTA ends while another could still send to it)
@@ -445,16 +540,17 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
     const int64_t end = (len + wave - 1) / wave * wave;
     int64_t begin = end - wave;
     int64_t t0 = begin + (int64_t)me.rank * chunk + me.warp * K;
+    const int left = (int)(p.channels - me.c < 2 * kTile ? p.channels - me.c : 2 * kTile);
     // (a wave that does not come is not filled)
     auto fill = [&](int side, int64_t t) {
         if (t >= 0) {
-            room.x[side][me.warp].fill(x, t, p.x_step, len, me.width, me.lane);
-            room.dy[side][me.warp].fill(dy, t, p.dy_step, p.dy == nullptr ? t : len, me.width, me.lane);
+            room.x[side][me.warp].fill(static_cast<const T*>(p.x), x, t, p.x_step, len, left, me.lane);
+            room.dy[side][me.warp].fill(static_cast<const T*>(p.dy), dy, t, p.dy_step, p.dy == nullptr ? t : len, left, me.lane);
         }
         copies_issued();
     };
     auto fill_gate = [&](int64_t t) {
-        if (t >= 0) room.gate[me.warp].fill(gate, t, p.gate_step, len, me.width, me.lane);
+        if (t >= 0) room.gate[me.warp].fill(static_cast<const T*>(p.gate), gate, t, p.gate_step, len, left, me.lane);
         copies_issued();
     };
     if (me.warp == 0) {
@@ -472,6 +568,9 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
         auto &bx = room.x[side][me.warp], &bg = room.gate[me.warp], &bd = room.dy[side][me.warp];
         copies_arrived<1>();
         __syncwarp();
+        bg.align(gate, t0, p.gate_step, me.lane);
+        bx.align(x, t0, p.x_step, me.lane);
+        if (p.dy != nullptr) bd.align(dy, t0, p.dy_step, me.lane);
         Lanes a[K], keep[K], before[K], sum = all_lanes(0.0f), passed = sum;
         Product product;
         const bool all = begin + wave <= len;
@@ -680,9 +779,9 @@ int check_scan(const dcn_scan* p) {
     return DCN_OK;
 }
 
-// Bytes that a copy moves at once: 16 or 4 where every row of every tensor starts on as many, an element otherwise
+// Bytes that every row of every tensor starts on: 16, 4 or an element's
 struct Bytes {
-    int n = 16, e;
+    int n, e;
     void by(const void* p, int64_t batch, int64_t step) {
         while (n > e && (!aligned(p, n) || batch * e % n != 0 || step * e % n != 0)) n = n == 16 ? 4 : e;
     }
@@ -732,22 +831,22 @@ extern "C" int dcn_scan_forward(const dcn_scan* p, const void* x, const void* ga
     if (!aligned(x, e) || !aligned(gate, e) || !aligned(y, e) || !aligned(state, 4) || !aligned(last, 4) ||
         !aligned(lengths, 8) || !aligned(checkpoints, 4))
         return DCN_ERR_ALIGN;
-    Bytes bytes{16, e};
-    bytes.by(x, p->x_batch, p->x_step);
-    bytes.by(gate, p->gate_batch, p->gate_step);
-    bytes.by(y, p->channels, p->channels);
+    Bytes rows{16, e};
+    rows.by(x, p->x_batch, p->x_step);
+    rows.by(gate, p->gate_batch, p->gate_step);
+    rows.by(y, p->channels, p->channels);
     ScanArgs a = args_of(p);
     a.x = x, a.gate = gate, a.state = state, a.lengths = lengths, a.y = y, a.last = last, a.checkpoints = checkpoints;
     const cudaStream_t st = (cudaStream_t)stream;
     if (p->dtype == DCN_SEQ_F32)
-        return bytes.n == 16 ? run_forward<float, 16>(a, p->batch, st) : run_forward<float, 4>(a, p->batch, st);
+        return rows.n == 16 ? run_forward<float, 16>(a, p->batch, st) : run_forward<float, 4>(a, p->batch, st);
     if (p->dtype == DCN_SEQ_BF16)
-        return bytes.n == 16  ? run_forward<__nv_bfloat16, 16>(a, p->batch, st)
-               : bytes.n == 4 ? run_forward<__nv_bfloat16, 4>(a, p->batch, st)
-                              : run_forward<__nv_bfloat16, 2>(a, p->batch, st);
-    return bytes.n == 16  ? run_forward<__half, 16>(a, p->batch, st)
-           : bytes.n == 4 ? run_forward<__half, 4>(a, p->batch, st)
-                          : run_forward<__half, 2>(a, p->batch, st);
+        return rows.n == 16  ? run_forward<__nv_bfloat16, 16>(a, p->batch, st)
+               : rows.n == 4 ? run_forward<__nv_bfloat16, 4>(a, p->batch, st)
+                             : run_forward<__nv_bfloat16, 2>(a, p->batch, st);
+    return rows.n == 16  ? run_forward<__half, 16>(a, p->batch, st)
+           : rows.n == 4 ? run_forward<__half, 4>(a, p->batch, st)
+                         : run_forward<__half, 2>(a, p->batch, st);
 }
 
 extern "C" int dcn_scan_backward(const dcn_scan* p, const void* x, const void* gate, const int64_t* lengths,
@@ -762,25 +861,25 @@ extern "C" int dcn_scan_backward(const dcn_scan* p, const void* x, const void* g
     if (!aligned(x, e) || !aligned(gate, e) || !aligned(dy, e) || !aligned(dx, e) || !aligned(dgate, e) ||
         !aligned(dlast, 4) || !aligned(dstate, 4) || !aligned(lengths, 8) || !aligned(checkpoints, 4))
         return DCN_ERR_ALIGN;
-    Bytes bytes{16, e};
-    bytes.by(x, p->x_batch, p->x_step);
-    bytes.by(gate, p->gate_batch, p->gate_step);
-    if (dy != nullptr) bytes.by(dy, p->dy_batch, p->dy_step);
-    bytes.by(dx, p->channels, p->channels);
-    bytes.by(dgate, p->channels, p->channels);
+    Bytes rows{16, e};
+    rows.by(x, p->x_batch, p->x_step);
+    rows.by(gate, p->gate_batch, p->gate_step);
+    if (dy != nullptr) rows.by(dy, p->dy_batch, p->dy_step);
+    rows.by(dx, p->channels, p->channels);
+    rows.by(dgate, p->channels, p->channels);
     ScanArgs a = args_of(p);
     a.x = x, a.gate = gate, a.dy = dy, a.dlast = dlast, a.lengths = lengths, a.dx = dx, a.dgate = dgate, a.dstate = dstate;
     a.checkpoints = const_cast<float*>(checkpoints);
     const cudaStream_t st = (cudaStream_t)stream;
     if (p->dtype == DCN_SEQ_F32)
-        return bytes.n == 16 ? run_backward<float, 16>(a, p->batch, st) : run_backward<float, 4>(a, p->batch, st);
+        return rows.n == 16 ? run_backward<float, 16>(a, p->batch, st) : run_backward<float, 4>(a, p->batch, st);
     if (p->dtype == DCN_SEQ_BF16)
-        return bytes.n == 16  ? run_backward<__nv_bfloat16, 16>(a, p->batch, st)
-               : bytes.n == 4 ? run_backward<__nv_bfloat16, 4>(a, p->batch, st)
-                              : run_backward<__nv_bfloat16, 2>(a, p->batch, st);
-    return bytes.n == 16  ? run_backward<__half, 16>(a, p->batch, st)
-           : bytes.n == 4 ? run_backward<__half, 4>(a, p->batch, st)
-                          : run_backward<__half, 2>(a, p->batch, st);
+        return rows.n == 16  ? run_backward<__nv_bfloat16, 16>(a, p->batch, st)
+               : rows.n == 4 ? run_backward<__nv_bfloat16, 4>(a, p->batch, st)
+                             : run_backward<__nv_bfloat16, 2>(a, p->batch, st);
+    return rows.n == 16  ? run_backward<__half, 16>(a, p->batch, st)
+           : rows.n == 4 ? run_backward<__half, 4>(a, p->batch, st)
+                         : run_backward<__half, 2>(a, p->batch, st);
 }
 
 namespace {

@@ -628,3 +628,38 @@ def test_sizes_of_several_host_threads():
     for t in threads:
         t.join()
     assert not bad, bad
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("channels", [1, 2, 7, 63, 64, 65, 127, 130])
+def test_scan_rows_that_start_anywhere(kind, channels):
+    """The C calls on tensors that start in the middle of 16 bytes, between guards: the same bits, and nothing written beside"""
+    import ctypes
+    from deform_conv3d_pytorch_op_b200 import _lib
+    L, t, b, n = _lib.lib(), TYPES[kind], 2, 150
+    g = gen(92)
+    x, gate, dy = (randn(g, b, n, channels, dtype=t) for _ in range(3))
+    lengths = torch.tensor([n, 70], device="cuda")
+    xr, gr = x.clone().requires_grad_(), gate.clone().requires_grad_()
+    y, last = dcn.GatedScanFunction.apply(xr, gr, None, lengths)
+    wants = (y.detach(),) + torch.autograd.grad(y, (xr, gr), dy)
+    ptr = lambda a: ctypes.c_void_p(a.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for off in (0, 1, 2, 3, 4, 7):
+        def shifted(a=None):
+            big = torch.full((b * n * channels + 32,), 77.0, dtype=t, device="cuda")
+            part = big[8 + off:8 + off + b * n * channels].view(b, n, channels)
+            if a is not None:
+                part.copy_(a)
+            return big, part
+
+        (_, sx), (_, sg), (_, sd) = shifted(x), shifted(gate), shifted(dy)
+        outs = [shifted() for _ in range(3)]
+        p = _lib.dcn_scan({"f32": 0, "bf16": 1, "f16": 2}[kind], b, n, channels, *(n * channels, channels) * 3)
+        end, ckpt = torch.empty(b, channels, device="cuda"), torch.empty(b, 3, channels, device="cuda")
+        assert L.dcn_scan_forward(ctypes.byref(p), ptr(sx), ptr(sg), None, ptr(lengths), ptr(outs[0][1]), ptr(end), ptr(ckpt), stream) == 0
+        assert L.dcn_scan_backward(ctypes.byref(p), ptr(sx), ptr(sg), ptr(lengths), ptr(ckpt), ptr(sd), None, ptr(outs[1][1]),
+                                   ptr(outs[2][1]), None, stream) == 0
+        for (big, part), want in zip(outs, wants):
+            assert torch.equal(part, want)
+            assert bool((big[:8 + off] == 77).all()) and bool((big[8 + off + b * n * channels:] == 77).all())
