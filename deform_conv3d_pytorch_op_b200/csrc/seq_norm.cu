@@ -9,16 +9,16 @@
 // once.  Rows of up to 32 threads (512 channels of 16 bits, 256 of float32) share a warp, and their sums are shuffles alone; above,
 // a row is that of 64, 128, ... threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of
 // the next row are on their way to its own places in shared memory meanwhile (cp.async, 16 or 4 bytes at a time, as rows start on
-// them); rows of an odd number of 16-bit elements are loaded one by one when they are used.  Weights are in shared memory too, once
-// a CTA (registers for them would cost a third of the threads), and the arithmetic goes in pairs through the packed float32
-// instructions.  The CTAs of the backward pass keep Z and dpre in registers and leave one partial sum each; a second kernel adds
-// those in a fixed order.
+// them).  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the arithmetic
+// goes in pairs through the packed float32 instructions.  The CTAs of the backward pass keep Z and dpre in registers and leave one
+// partial sum each; a second kernel adds those in a fixed order.
 //
 // The bound is DRAM, and the arithmetic, which leaves a third of the issue slots, stands close behind.  Measured, forward and
 // backward with the sums of the weights' gradients, against a copy of the same bytes at 6.5 TB/s:
 //     32768 x 2048 bf16    117 us (5.7 TB/s, 88 %)   209 us (5.1 TB/s, 79 %)
 //     32768 x 2046 bf16    190 us                    348 us      pairs: four times the loads and stores of a row
-//     32768 x 2047 bf16    388 us                    925 us      element by element, nothing ahead
+//     32768 x 2047 bf16    248 us                    574 us      pairs that lie across the tensor's 4 bytes (392 and 887 us
+//                                                                when elements were loaded and stored one by one)
 //     4096 x 8192 float32  141 us (4.8 TB/s, 73 %)   350 us (3.1 TB/s, 47 %)     rows too long to be held twice: nothing ahead
 //     65536 x 64 bf16       10 us (4.0 TB/s)          22 us (3.1 TB/s)           in L2; eight rows to a warp
 #include "seq_common.cuh"
@@ -38,18 +38,31 @@ struct NormArgs {
     float eps, inv;
 };
 
-// How a row of elements T lies over threads, V at a time: the vectors j, j + threads, ... of thread j
+// How a row of elements T lies over threads, V at a time: the vectors j, j + threads, ... of thread j.  16-bit rows that start in
+// the middle of 4 bytes (V 1) lie in pairs as well (kSkew): they move 4 bytes at a time, as these lie in the tensor, and a thread
+// has its pair from two neighbouring ones.  Neighbours are those of a segment, the threads that a row and a warp share: its pairs
+// are next to one another, whichever vectors they are, and its last thread fetches the 4 bytes behind them too.
 template <typename T, int V>
 struct Layout {
-    static constexpr int kPer = 32 / (int)sizeof(T), kVectors = kPer / V, kPairs = kPer / 2;
-    static __device__ __forceinline__ int element(int j, int threads, int e) { return (j + e / V * threads) * V + e % V; }
+    static constexpr bool kSkew = V * sizeof(T) == 2;
+    static constexpr int kV = kSkew ? 2 : V, kPer = 32 / (int)sizeof(T), kVectors = kPer / kV, kPairs = kPer / 2;
+    static __device__ __forceinline__ int element(int j, int threads, int e) {
+        if constexpr (kSkew) {
+            const int s = segment(threads);
+            return (j / s * s * kVectors + e / kV * s + j % s) * kV + e % kV;
+        }
+        return (j + e / kV * threads) * kV + e % kV;
+    }
+    static __host__ __device__ __forceinline__ int segment(int threads) { return threads < 32 ? threads : 32; }
+    static __device__ __forceinline__ int at_segment(int threads) { return (int)threadIdx.x % segment(threads); }
 };
 
 // A thread's elements of a row
 template <typename T, int V>
 struct Slice {
-    Pack<T, V> v[Layout<T, V>::kVectors];
-    __device__ __forceinline__ float at(int e) const { return v[e / V].at(e % V); }
+    static constexpr int kV = Layout<T, V>::kV;
+    Pack<T, kV> v[Layout<T, V>::kVectors];
+    __device__ __forceinline__ float at(int e) const { return v[e / kV].at(e % kV); }
     __device__ __forceinline__ Lanes pair(int i) const {
         const float f[2] = {at(2 * i), at(2 * i + 1)};
         return lanes(f);
@@ -59,16 +72,49 @@ struct Slice {
 template <typename T, int V>
 __device__ __forceinline__ void put(void* base, int64_t offset, const Lanes (&f)[Layout<T, V>::kPairs], int j, int threads,
                                     int channels) {
+    using L = Layout<T, V>;
     if (base == nullptr) return;
+    T* out = static_cast<T*>(base) + offset;
+    const bool skew = L::kSkew && reinterpret_cast<uintptr_t>(out) % 4 != 0;
+    uint32_t words[L::kSkew ? L::kVectors : 1];
 #pragma unroll
-    for (int i = 0; i < Layout<T, V>::kVectors; ++i) {
-        const int c = Layout<T, V>::element(j, threads, i * V);
-        float part[V];
+    for (int i = 0; i < L::kVectors; ++i) {
+        const int c = L::element(j, threads, i * L::kV);
+        float part[L::kV];
 #pragma unroll
-        for (int k = 0; k < V; ++k) part[k] = f[(i * V + k) / 2].at((i * V + k) % 2);
-        Pack<T, V> out;
-        out.set(part);
-        if (c < channels) out.put(static_cast<T*>(base) + offset + c);
+        for (int k = 0; k < L::kV; ++k) part[k] = f[(i * L::kV + k) / 2].at((i * L::kV + k) % 2);
+        Pack<T, L::kV> mine;
+        mine.set(part);
+        if constexpr (L::kSkew) {
+            words[i] = mine.raw.u[0];
+        } else {
+            if (c < channels) mine.put(out + c);
+        }
+    }
+    if constexpr (L::kSkew) {
+        // (every lane takes part in the shuffles, whatever its row's skew: a warp's rows may differ in it)
+        const int s = L::segment(threads), l = L::at_segment(threads), next_lane = (int)threadIdx.x % 32 - l + (l + 1) % s;
+        uint32_t nexts[L::kVectors];
+#pragma unroll
+        for (int i = 0; i < L::kVectors; ++i)
+            nexts[i] = __shfl_sync(0xffffffffu, l == 0 && i + 1 < L::kVectors ? words[i + 1] : words[i], next_lane);
+        if (skew) {                              // 4 bytes are a pair's second element and the next pair's first
+#pragma unroll
+            for (int i = 0; i < L::kVectors; ++i) {
+                const int c = L::element(j, threads, i * L::kV);
+                const bool both = c + 2 < channels && (i + 1 < L::kVectors || l + 1 < s);
+                if (i == 0 && l == 0 && c < channels) store(out + c, Raw<2>{(uint16_t)words[i]});
+                if (both) store(out + c + 1, Raw<4>{{__funnelshift_r(words[i], nexts[i], 16)}});
+                if (!both && c + 1 < channels) store(out + c + 1, Raw<2>{(uint16_t)(words[i] >> 16)});
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < L::kVectors; ++i) {
+                const int c = L::element(j, threads, i * L::kV);
+                if (c + 1 < channels) store(out + c, Raw<4>{{words[i]}});
+                if (c + 1 == channels) store(out + c, Raw<2>{(uint16_t)words[i]});
+            }
+        }
     }
 }
 
@@ -83,12 +129,27 @@ struct Rows {
     unsigned char* room;                         // mine of the first vector
     int width;                                   // bytes from one vector of a thread to its next: of the CTA's threads
     int stage = 0;
+    int64_t now = 0;
     bool first = true, live = true;              // live: the row is there (rows of a warp end together)
     Slice<T, V> here[kStaged ? 1 : kTensors];    // the row's, where it is not in shared memory
-    static constexpr int kMove = V * (int)sizeof(T);
+    static constexpr int kMove = L::kV * (int)sizeof(T);
     static constexpr int kBytes = kStaged ? 2 * kTensors * L::kVectors * kMove : 0;    // of a thread: two rows
+    static constexpr int kExtra = kStaged && L::kSkew ? 2 * kTensors * kMove : 0;      // of a segment: what its last thread fetches
+    // where thread n of a CTA's has its first vector, in rows of `threads`; and `width` for n threads
+    static __device__ __forceinline__ int offset_of(int n, int threads) {
+        const int s = L::segment(threads);
+        return (L::kSkew ? n / s * (s * L::kVectors + 1) + n % s : n) * kMove;
+    }
+    static __device__ __forceinline__ int width_of(int n, int threads) {
+        return (L::kSkew ? n * L::kVectors + n / L::segment(threads) : n) * kMove;
+    }
     __device__ __forceinline__ unsigned char* place(int s, int t, int i) const {
+        if constexpr (L::kSkew) return room + (s * kTensors + t) * width + i * L::segment(threads) * kMove;
         return room + ((s * kTensors + t) * L::kVectors + i) * width;
+    }
+    __device__ __forceinline__ bool skewed(int t, int64_t row) const {
+        return L::kSkew &&
+               (((unsigned)(reinterpret_cast<uintptr_t>(base[t]) / 2) + (unsigned)row * (unsigned)stride[t]) & 1) != 0;
     }
     __device__ __forceinline__ void fetch(int s, int64_t row) {
         if (row < rows) {
@@ -97,6 +158,26 @@ struct Rows {
             for (int t = 0; t < kTensors; ++t) {
                 if (base[t] == nullptr) continue;
                 const T* from = base[t] + row * stride[t] + L::element(j, threads, 0);
+                if constexpr (L::kSkew) {        // zeros from the row's end on; nothing is read that lies before the tensor
+                    const int skew = skewed(t, row), apart = L::kV * L::segment(threads);
+                    from -= skew;
+                    int left = channels - L::element(j, threads, 0) + skew;
+                    if (from < base[t]) {
+                        Pack<T, 1> one;
+                        one.get(base[t]);
+                        *reinterpret_cast<Raw<2>*>(place(s, t, 0) + 2) = one.raw;
+                    } else if (left >= 0) {
+                        copy_async_some<4>(place(s, t, 0), from, min(2 * left, 4));
+                    }
+#pragma unroll
+                    for (int i = 1; i < L::kVectors; ++i) {
+                        from += apart, left -= apart;
+                        if (left >= 0) copy_async_some<4>(place(s, t, i), from, min(2 * left, 4));
+                    }
+                    if (L::at_segment(threads) + 1 == L::segment(threads) && left >= 2)
+                        copy_async_some<4>(place(s, t, L::kVectors - 1) + 4, from + 2, min(2 * left - 4, 4));
+                    continue;
+                }
 #pragma unroll
                 for (int i = 0; i < L::kVectors; ++i, from += threads * V) {
                     if (whole) copy_async_all<kMove>(place(s, t, i), from);
@@ -109,24 +190,45 @@ struct Rows {
     }
     // the row that next() goes to first
     __device__ __forceinline__ void begin(int64_t row) {
+        if constexpr (kStaged && L::kSkew) {     // (what lies far behind the rows' ends is not fetched)
+            for (int t = 0; t < 2 * kTensors; ++t)
+                for (int i = 0; i < L::kVectors; ++i) {
+                    *reinterpret_cast<uint32_t*>(place(0, t, i)) = 0;
+                    if (i + 1 == L::kVectors && L::at_segment(threads) + 1 == L::segment(threads))
+                        *reinterpret_cast<uint32_t*>(place(0, t, i) + 4) = 0;
+                }
+            __syncwarp();
+        }
         if constexpr (kStaged) fetch(0, row);
     }
     // to row `row`, the next one since the last call or begin()
     __device__ __forceinline__ void next(int64_t row) {
         live = row < rows;
+        now = row;
         if constexpr (kStaged) {
             stage = first ? 0 : stage ^ 1;
             first = false;
+            if (L::kSkew) __syncwarp();          // (neighbours have read what is fetched over)
             fetch(stage ^ 1, row + step);
             copies_arrived<1>();
+            if (L::kSkew) __syncwarp();
         } else {
 #pragma unroll
             for (int t = 0; t < kTensors; ++t)
 #pragma unroll
                 for (int i = 0; i < L::kVectors; ++i) {
-                    const int c = L::element(j, threads, i * V);
+                    const int c = L::element(j, threads, i * L::kV);
                     here[t].v[i].zero();
-                    if (live && base[t] != nullptr && c < channels) here[t].v[i].get(base[t] + row * stride[t] + c);
+                    if (!live || base[t] == nullptr || c >= channels) continue;
+                    const T* from = base[t] + row * stride[t] + c;
+                    if constexpr (L::kSkew) {
+                        Raw<2> lo, hi{0};
+                        load(lo, from);
+                        if (c + 1 < channels) load(hi, from + 1);
+                        here[t].v[i].raw.u[0] = lo.u | (uint32_t)hi.u << 16;
+                    } else {
+                        here[t].v[i].get(from);
+                    }
                 }
         }
     }
@@ -139,8 +241,16 @@ struct Rows {
             Slice<T, V> s;
 #pragma unroll
             for (int i = 0; i < L::kVectors; ++i) {
-                if (base[t] == nullptr || !live) s.v[i].zero();
-                else load_shared(s.v[i].raw, place(stage, t, i));
+                if (base[t] == nullptr || !live) {
+                    s.v[i].zero();
+                    continue;
+                }
+                load_shared(s.v[i].raw, place(stage, t, i));
+                if constexpr (L::kSkew) {
+                    Raw<4> next;
+                    load_shared(next, place(stage, t, i) + 4);
+                    s.v[i].raw.u[0] = __funnelshift_r(s.v[i].raw.u[0], next.u[0], skewed(t, now) ? 16 : 0);
+                }
             }
             return s;
         }
@@ -268,10 +378,12 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kern
     pdl_wait();
     Weights<T, V> weights{reinterpret_cast<float4*>(dynamic) + me.j, me.threads};
     const int64_t first = (int64_t)blockIdx.x * me.groups + me.group, step = (int64_t)gridDim.x * me.groups;
-    Rows<T, V, 3, kStaged> rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate)},
-                                {p.x_row, p.block_row, p.gate_row}, p.rows, step, me.j, me.threads, p.channels,
-                                dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * V * sizeof(T),
-                                (int)(blockDim.x * V * sizeof(T))};
+    using R = Rows<T, V, 3, kStaged>;
+    R rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate)},
+           {p.x_row, p.block_row, p.gate_row},
+           p.rows, step, me.j, me.threads, p.channels,
+           dynamic + me.threads * Weights<T, V>::kBytes + R::offset_of(threadIdx.x, me.threads),
+           R::width_of(blockDim.x, me.threads)};
     rows.begin(first);
     if (me.group == 0) weights.put(p, me.j, me.threads);
     __syncthreads();
@@ -324,11 +436,13 @@ __global__ void __launch_bounds__(kMost, kMost == 256 ? 2 : 1) norm_backward_ker
     pdl_wait();
     Weights<T, V> weights{reinterpret_cast<float4*>(dynamic) + me.j, me.threads};
     const int64_t first = (int64_t)blockIdx.x * me.groups + me.group, step = (int64_t)gridDim.x * me.groups;
-    Rows<T, V, 5, kStaged> rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate),
-                                 static_cast<const T*>(p.dstream), static_cast<const T*>(p.dnormed)},
-                                {p.x_row, p.block_row, p.gate_row, p.dstream_row, p.dnormed_row}, p.rows, step, me.j, me.threads,
-                                p.channels, dynamic + me.threads * Weights<T, V>::kBytes + threadIdx.x * V * sizeof(T),
-                                (int)(blockDim.x * V * sizeof(T))};
+    using R = Rows<T, V, 5, kStaged>;
+    R rows{{static_cast<const T*>(p.x), static_cast<const T*>(p.block), static_cast<const T*>(p.gate),
+            static_cast<const T*>(p.dstream), static_cast<const T*>(p.dnormed)},
+           {p.x_row, p.block_row, p.gate_row, p.dstream_row, p.dnormed_row},
+           p.rows, step, me.j, me.threads, p.channels,
+           dynamic + me.threads * Weights<T, V>::kBytes + R::offset_of(threadIdx.x, me.threads),
+           R::width_of(blockDim.x, me.threads)};
     rows.begin(first);
     if (me.group == 0) weights.put(p, me.j, me.threads);
     __syncthreads();
@@ -492,18 +606,19 @@ int launch(K kernel, unsigned grid, int cta, size_t smem, int most, const NormAr
 
 template <typename T, int V, bool kWarp, int kMost>
 int run_as(const NormArgs& a, bool backward, cudaStream_t st) {
-    // two rows of every tensor in shared memory where vectors are read, and an SM has room for as many threads
-    constexpr int kSM = 227 * 1024, kWeights = Weights<T, V>::kBytes;
-    constexpr bool f = V * sizeof(T) >= 4 && kMost * (Rows<T, V, 3, true>::kBytes + kWeights) <= kSM,
-                   b = V * sizeof(T) >= 4 && kMost * (Rows<T, V, 5, true>::kBytes + kWeights) <= kSM;
-    const int cta = cta_of(a.threads);
+    // two rows of every tensor in shared memory where an SM has room for as many threads
+    constexpr int kSM = 226 * 1024, kWeights = kMost * Weights<T, V>::kBytes, kSegments = kMost / (kWarp ? 4 : 32);
+    using F = Rows<T, V, 3, true>;
+    using B = Rows<T, V, 5, true>;
+    constexpr int kForward = kMost * F::kBytes + kSegments * F::kExtra, kBackward = kMost * B::kBytes + kSegments * B::kExtra;
+    constexpr bool f = kForward + kWeights <= kSM, b = kBackward + kWeights <= kSM;
+    const int cta = cta_of(a.threads), segments = cta / (a.threads < 32 ? a.threads : 32);
+    const size_t weights = (size_t)a.threads * Weights<T, V>::kBytes;
     if (backward)
         return launch(norm_backward_kernel<T, V, kWarp, kMost, b>, grid_of(a.rows, a.channels, sizeof(T), kBackwardThreads), cta,
-                      (size_t)cta * Rows<T, V, 5, b>::kBytes + a.threads * kWeights,
-                      kMost * (Rows<T, V, 5, b>::kBytes + kWeights), a, st);
+                      weights + (b ? cta * B::kBytes + segments * B::kExtra : 0), kWeights + (b ? kBackward : 0), a, st);
     return launch(norm_forward_kernel<T, V, kWarp, kMost, f>, grid_of(a.rows, a.channels, sizeof(T), kForwardThreads), cta,
-                  (size_t)cta * Rows<T, V, 3, f>::kBytes + a.threads * kWeights,
-                  kMost * (Rows<T, V, 3, f>::kBytes + kWeights), a, st);
+                  weights + (f ? cta * F::kBytes + segments * F::kExtra : 0), kWeights + (f ? kForward : 0), a, st);
 }
 
 template <typename T, int V>

@@ -663,3 +663,39 @@ def test_scan_rows_that_start_anywhere(kind, channels):
         for (big, part), want in zip(outs, wants):
             assert torch.equal(part, want)
             assert bool((big[:8 + off] == 77).all()) and bool((big[8 + off + b * n * channels:] == 77).all())
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("channels", [1, 3, 33, 63, 65, 129, 511, 513, 1025, 2047, 4097, 8191])
+def test_norm_rows_that_start_anywhere(kind, channels):
+    """The C calls on odd rows that start in the middle of 16 bytes, between guards: the same bits, and nothing written beside"""
+    import ctypes
+    from deform_conv3d_pytorch_op_b200 import _lib
+    L, t, n = _lib.lib(), TYPES[kind], 37
+    g = gen(93)
+    ins = [randn(g, n, channels, dtype=t) for _ in range(5)]           # x, block, gate and the gradients of the two results
+    w = [randn(g, channels) for _ in range(3)]
+    leaves = [a.clone().requires_grad_() for a in ins[:3]]
+    outs = dcn.ResidualNormFunction.apply(*leaves, *w)
+    wants = [o.detach() for o in outs] + list(torch.autograd.grad(outs, leaves, ins[3:]))
+    ptr = lambda a: ctypes.c_void_p(a.data_ptr())
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for off in (0, 1, 2, 3, 4, 7):
+        def shifted(a=None):
+            big = torch.full((n * channels + 32,), 77.0, dtype=t, device="cuda")
+            part = big[8 + off:8 + off + n * channels].view(n, channels)
+            if a is not None:
+                part.copy_(a)
+            return big, part
+
+        s = [shifted(a)[1] for a in ins]
+        got = [shifted() for _ in wants]
+        stats = torch.empty(n, 2, device="cuda")
+        p = _lib.dcn_norm(dtype={"f32": 0, "bf16": 1, "f16": 2}[kind], weight_dtype=0, rows=n, channels=channels, x_row=channels,
+                          block_row=channels, gate_row=channels, dstream_row=channels, dnormed_row=channels, eps=1e-6)
+        assert L.dcn_norm_forward(ctypes.byref(p), *map(ptr, s[:3]), *map(ptr, w), ptr(got[0][1]), ptr(got[1][1]), ptr(stats), stream) == 0
+        assert L.dcn_norm_backward(ctypes.byref(p), *map(ptr, s[:3]), *map(ptr, w), ptr(stats), ptr(s[3]), ptr(s[4]),
+                                   *(ptr(a[1]) for a in got[2:]), None, None, None, None, 0, stream) == 0
+        for (big, part), want in zip(got, wants):
+            assert torch.equal(part, want)
+            assert bool((big[:8 + off] == 77).all()) and bool((big[8 + off + n * channels:] == 77).all())
