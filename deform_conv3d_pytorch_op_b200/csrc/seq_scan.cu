@@ -14,7 +14,7 @@
 // addresses allow it, and no address arithmetic in the recurrence.
 //
 // What bounds it depends on how many sequences there are.  Measured, bf16, against a copy of the same bytes at 6.5 TB/s:
-//     64 x 1024 x 2048 (2048 units, one CTA each)   forward 140 us (5.8 TB/s, 88 %)   backward 252 us (5.3 TB/s, 82 %): DRAM
+//     64 x 1024 x 2048 (2048 units, one CTA each)   forward 138 us (5.8 TB/s, 90 %)   backward 253 us (5.3 TB/s, 81 %): DRAM
 //     2 x 16384 x 2048 (64 units in clusters)       forward  98 us (4.2 TB/s, 64 %)   backward 148 us (4.6 TB/s, 70 %)
 // Few long sequences walk few clusters through many waves, and in each wave's exchange of maps its warps have nothing but copies
 // under way: latency, with DRAM 44 % busy and 53 % of the issue slots taken in the forward pass.
