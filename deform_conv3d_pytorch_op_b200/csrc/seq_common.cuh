@@ -48,6 +48,9 @@ __device__ __forceinline__ void load_shared(Raw<16>& r, const void* p) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r.u[0]), "=r"(r.u[1]), "=r"(r.u[2]), "=r"(r.u[3]) : "r"((uint32_t)__cvta_generic_to_shared(p)));
 }
+__device__ __forceinline__ void load_shared(Raw<8>& r, const void* p) {
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.u[0]), "=r"(r.u[1]) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+}
 __device__ __forceinline__ void load_shared(Raw<4>& r, const void* p) {
     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r.u[0]) : "r"((uint32_t)__cvta_generic_to_shared(p)));
 }

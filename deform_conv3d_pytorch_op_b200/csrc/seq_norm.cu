@@ -8,17 +8,19 @@
 // A row lives in the registers of a row of threads, 32 bytes of each tensor a thread, so that every tensor is read or written
 // once.  Rows of up to 32 threads (512 channels of 16 bits, 256 of float32) share a warp, and their sums are shuffles alone; above,
 // a row is that of 64, 128, ... threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of
-// the next row are on their way to its own places in shared memory meanwhile (cp.async, 16 or 4 bytes at a time, as rows start on
-// them).  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the arithmetic
+// the next row are on their way to its own places in shared memory meanwhile (cp.async, 16, 8 or 4 bytes at a time, as rows start
+// on them).  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the arithmetic
 // goes in pairs through the packed float32 instructions.  The CTAs of the backward pass keep Z and dpre in registers and leave one
 // partial sum each; a second kernel adds those in a fixed order.
 //
 // The bound is DRAM, and the arithmetic, which leaves a third of the issue slots, stands close behind.  Measured, forward and
 // backward with the sums of the weights' gradients, against a copy of the same bytes at 6.5 TB/s:
 //     32768 x 2048 bf16    117 us (5.7 TB/s, 88 %)   209 us (5.1 TB/s, 79 %)
-//     32768 x 2046 bf16    190 us                    348 us      pairs: four times the loads and stores of a row
+//     32768 x 2044 bf16    143 us                    261 us      rows on 8 bytes: twice the loads and stores
+//     32768 x 2046 bf16    192 us                    347 us      on 4 bytes: four times as many
 //     32768 x 2047 bf16    248 us                    574 us      pairs that lie across the tensor's 4 bytes (392 and 887 us
 //                                                                when elements were loaded and stored one by one)
+//     16384 x 2046 float32 125 us                    205 us      on 8 bytes (by 4, at 2047: 174 and 286 us)
 //     4096 x 8192 float32  141 us (4.8 TB/s, 73 %)   350 us (3.1 TB/s, 47 %)     rows too long to be held twice: nothing ahead
 //     65536 x 64 bf16       10 us (4.0 TB/s)          22 us (3.1 TB/s)           in L2; eight rows to a warp
 #include "seq_common.cuh"
@@ -661,23 +663,31 @@ NormArgs args_of(const dcn_norm* p) {
     return a;
 }
 
-// Elements moved at once: 16 bytes where every row of every tensor starts on one, pairs of 16-bit elements where they start on
-// 4, one otherwise.
+// Elements of a vector: 16 bytes, 8 or 4 where every row of every tensor starts on as many, one element otherwise (of which 16-bit
+// ones move two at a time all the same).
 struct Vector {
     int n, elem;
     explicit Vector(const dcn_norm* p) : n(16 / elem_bytes(p->dtype)), elem(elem_bytes(p->dtype)) {}
     void by(const void* v, int64_t row) {
-        while (v != nullptr && n > 1 && (!aligned(v, n * elem) || row % n != 0)) n = n == 8 ? 2 : 1;
+        while (v != nullptr && n > 1 && (!aligned(v, n * elem) || row % n != 0)) n /= 2;
     }
 };
 
+template <typename T>
+int run_16(int n, const NormArgs& a, bool backward, cudaStream_t st) {
+    return n == 8   ? run<T, 8>(a, backward, st)
+           : n == 4 ? run<T, 4>(a, backward, st)
+           : n == 2 ? run<T, 2>(a, backward, st)
+                    : run<T, 1>(a, backward, st);
+}
+
 int run_any(int dtype, int n, const NormArgs& a, bool backward, cudaStream_t st) {
-    if (dtype == DCN_SEQ_F32) return n == 4 ? run<float, 4>(a, backward, st) : run<float, 1>(a, backward, st);
-    if (dtype == DCN_SEQ_BF16)
-        return n == 8   ? run<__nv_bfloat16, 8>(a, backward, st)
-               : n == 2 ? run<__nv_bfloat16, 2>(a, backward, st)
-                        : run<__nv_bfloat16, 1>(a, backward, st);
-    return n == 8 ? run<__half, 8>(a, backward, st) : n == 2 ? run<__half, 2>(a, backward, st) : run<__half, 1>(a, backward, st);
+    if (dtype == DCN_SEQ_F32)
+        return n == 4   ? run<float, 4>(a, backward, st)
+               : n == 2 ? run<float, 2>(a, backward, st)
+                        : run<float, 1>(a, backward, st);
+    if (dtype == DCN_SEQ_BF16) return run_16<__nv_bfloat16>(n, a, backward, st);
+    return run_16<__half>(n, a, backward, st);
 }
 
 }  // namespace
