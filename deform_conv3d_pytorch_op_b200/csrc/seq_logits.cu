@@ -12,6 +12,8 @@
 // element by element.
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "seq_common.cuh"
 
 namespace cg = cooperative_groups;
@@ -73,15 +75,16 @@ struct Sums {
     }
 };
 
-// A row, or a part of one: vectors [v0, v1), the elements before the first vector (head) and behind the last (from tail on)
+// A row, or a part of one: vectors [v0, v1), the elements before the first vector (head) and behind the last (from tail on).
+// single: without vectors, all elements one by one.
 template <typename T>
 struct Row {
     static constexpr int kPer = 16 / sizeof(T);
     const T* p;
     int n, head, head_here, v0, v1, tail;
-    __device__ __forceinline__ Row(const T* p_, int n_, int part, int parts) : p(p_), n(n_) {
+    __device__ __forceinline__ Row(const T* p_, int n_, int part, int parts, bool single = false) : p(p_), n(n_) {
         const int off = (int)(reinterpret_cast<uintptr_t>(p) % 16) / (int)sizeof(T);
-        head = min(n, (kPer - off) % kPer);
+        head = single ? n : min(n, (kPer - off) % kPer);
         const int vectors = (n - head) / kPer;
         v0 = (int)((int64_t)vectors * part / parts);
         v1 = (int)((int64_t)vectors * (part + 1) / parts);
@@ -188,10 +191,11 @@ __device__ __forceinline__ Sums sums_of(const Row<T>& row, int tid, int threads,
     constexpr int kPer = Row<T>::kPer, kBatch = 4, kWords = 4 * kBatch;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     Sums a{kNone, 0.0f, 0.0f};
-    const int ends = row.head_here + (row.n - row.tail);          // elements outside vectors: at most one a thread
+    const int ends = row.head_here + (row.n - row.tail);          // elements outside vectors: at most one a thread, beside vectors
     if (tid < ends) {
-        const int e = tid < row.head_here ? tid : row.tail + tid - row.head_here;
-        a = add_elements<T, kU, kMarks>(a, row, e, e + 1, 1, k, marks);
+        const bool head = tid < row.head_here;
+        const int e = head ? tid : row.tail + tid - row.head_here;
+        a = add_elements<T, kU, kMarks>(a, row, e, head ? row.head_here : e + 1, threads, k, marks);
     }
     for (int v = row.v0 + tid; v < row.v1; v += kBatch * threads) {
         uint32_t w[kWords];
@@ -388,9 +392,10 @@ __device__ __forceinline__ int list_candidates(const Row<T>& row, int tid, uint3
             r.list[at] = (unsigned long long)key_of(row.one(e)) << 32 | (uint32_t)~e;
         }
     };
-    {
-        const int ends = row.head_here + (row.n - row.tail), e = tid < row.head_here ? tid : row.tail + tid - row.head_here;
-        list(tid < ends && reaches(row.one(e)) ? 1u : 0u, [&](int) { return e; });
+    const int ends = row.head_here + (row.n - row.tail);
+    for (int i = tid; i - tid < ends; i += kT) {
+        const int e = i < row.head_here ? i : row.tail + i - row.head_here;
+        list(i < ends && reaches(row.one(e)) ? 1u : 0u, [&](int) { return e; });
     }
     for (int first = row.v0 + tid - lane; first < row.v1; first += kBatch * kT) {       // (a warp's first vector)
         Raw<16> raw[kBatch];
@@ -545,6 +550,7 @@ struct LogitsArgs {
     const int64_t* tokens;
     int64_t ignore;
     int top, top_each;                           // top_each: of the largest lanes of a warp, to find a bound from
+    int single;                                  // rows are read element by element
     float *logprob, *entropy, *top_logprobs;
     int64_t* top_tokens;
     const float *dlogprob, *dentropy, *dtop;
@@ -672,7 +678,7 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
     if (at >= p.rows) return;                    // (a warp's row: a CTA's is always there)
     pdl_wait();
     const T* logits = static_cast<const T*>(p.logits) + at * p.stride;
-    const Row<T> row(logits, p.vocab, rank, ranks);
+    const Row<T> row(logits, p.vocab, rank, ranks, kKind == kScoresTop && p.single != 0);
     TopRoom<kT>& top = *reinterpret_cast<TopRoom<kT>*>(dynamic);
     constexpr int kWarps = kT / 32;
     TeacherRoom& teacher = teachers[kKind == kDistill ? group : 0];
@@ -1016,7 +1022,14 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
         // of every warp whose lanes all have a vector its share, or one more where that is less than twice `top` in all (the more,
         // the less is listed that is not among the `top`); of all CTAs together not more than there are keys
         const int warps = (few ? kFewThreads : kThreads) / 32, vectors = a.vocab / (16 / (int)sizeof(T)) / parts;
-        const int full = vectors / 32 < 1 ? 1 : vectors / 32 < warps ? vectors / 32 : warps;
+        // Short rows of which many are asked for are read element by element: where not many more lanes than `top` have a vector,
+        // the largest of the lanes bound little and most elements would be ranked.  Such rows are shorter than the list, so that
+        // nothing but the usual path reads them.  (Element by element / in vectors, us: 12332x320 bf16, 50 best 128 / 558; 4096
+        // rows of bf16, 1000 with 128 best 100 / 777, with 70 66 / 99; 2000 with 128 122 / 100; by 64 threads, 256 with 20 31 / 26,
+        // with 28 the same, 128 with 32 27 / 40.)
+        a.single = parts == 1 && 8 * std::min(vectors, 32 * warps) < (few ? 10 : 15) * a.top;
+        const int lanes = a.single ? a.vocab : vectors;
+        const int full = lanes / 32 < 1 ? 1 : lanes / 32 < warps ? lanes / 32 : warps;
         const int share = (a.top + parts * full - 1) / (parts * full), most = 32 / parts;
         a.top_each = parts * full * share < 2 * a.top ? share + 1 : share;
         if (a.top_each > most) a.top_each = most;
