@@ -7,7 +7,7 @@
 //
 // A row lives in the registers of a row of threads, 32 bytes of each tensor a thread, so that every tensor is read or written
 // once.  Rows of up to 32 threads (512 channels of 16 bits, 256 of float32) share a warp, and their sums are shuffles alone; above,
-// a row is that of 64, 128, ... threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of
+// a row is that of 64 to 512 (float32: 1024) threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of
 // the next row are on their way to its own places in shared memory meanwhile (cp.async, 16, 8 or 4 bytes at a time, as rows start
 // on them).  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the arithmetic
 // goes in pairs through the packed float32 instructions.  The CTAs of the backward pass keep Z and dpre in registers and leave one
@@ -23,6 +23,8 @@
 //     16384 x 2046 float32 125 us                    205 us      on 8 bytes (by 4, at 2047: 174 and 286 us)
 //     4096 x 8192 float32  141 us (4.8 TB/s, 73 %)   350 us (3.1 TB/s, 47 %)     rows too long to be held twice: nothing ahead
 //     65536 x 64 bf16       10 us (4.0 TB/s)          22 us (3.1 TB/s)           in L2; eight rows to a warp
+#include <algorithm>
+
 #include "seq_common.cuh"
 
 namespace dcn {
@@ -371,7 +373,7 @@ __device__ __forceinline__ void gates_of(const Slice<T, V>& g, bool has, Lanes (
 }
 
 template <typename T, int V, bool kWarp, int kMost, bool kStaged>
-__global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : 1) norm_forward_kernel(const NormArgs p) {
+__global__ void __launch_bounds__(kMost, kMost == 256 ? 3 : kMost == 384 ? 2 : 1) norm_forward_kernel(const NormArgs p) {
     using L = Layout<T, V>;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float room[2][32];
@@ -577,23 +579,28 @@ __global__ void __launch_bounds__(1024) norm_weights_kernel(const float* partial
     }
 }
 
-// Threads of a row, a power of two
+// Threads of a row: a power of two up to 256, which share a CTA of 256, then a multiple of 64, so that few are idle and an SM holds
+// two rows up to 384 (16384x4480 bf16, forward and backward: 169 and 354 us; 280 and 453 us with 512 threads a row)
 int threads_of(int64_t channels, int elem) {
+    const int64_t wanted = (channels * elem + 31) / 32;
+    if (wanted > 256) return (int)((wanted + 63) / 64 * 64);
     int t = 4;
-    while ((int64_t)t * (32 / elem) < channels) t *= 2;
+    while (t < wanted) t *= 2;
     return t;
 }
 
 // Threads of a CTA: 256, in rows of t, or one row of more
 int cta_of(int t) { return t > 256 ? t : 256; }
 
-// CTAs: as many as the SMs hold at once (so many threads, by registers and shared memory), and no more than there are rows for.
+// CTAs: as many as the SMs hold at once (so many threads by registers, and `smem` a CTA), and no more than there are rows for: one
+// more would start when others end, and walk its rows alone (16384x4096 bf16, forward: 137 us, 156 us with a third CTA an SM).
 constexpr int kForwardThreads = 768, kBackwardThreads = 512;
 
-unsigned grid_of(int64_t rows, int64_t channels, int elem, int threads_an_sm) {
+unsigned grid_of(int64_t rows, int64_t channels, int elem, int threads_an_sm, size_t smem = 0) {
     const int t = threads_of(channels, elem), cta = cta_of(t);
     const int64_t units = (rows + cta / t - 1) / (cta / t);
-    const int64_t most = (int64_t)sm_count() * (threads_an_sm > cta ? threads_an_sm / cta : 1);
+    const int held = std::max(1, std::min(threads_an_sm / cta, (int)(228 * 1024 / (smem + 1024))));
+    const int64_t most = (int64_t)sm_count() * held;
     return (unsigned)(units < most ? units : most);
 }
 
@@ -619,8 +626,9 @@ int run_as(const NormArgs& a, bool backward, cudaStream_t st) {
     if (backward)
         return launch(norm_backward_kernel<T, V, kWarp, kMost, b>, grid_of(a.rows, a.channels, sizeof(T), kBackwardThreads), cta,
                       weights + (b ? cta * B::kBytes + segments * B::kExtra : 0), kWeights + (b ? kBackward : 0), a, st);
-    return launch(norm_forward_kernel<T, V, kWarp, kMost, f>, grid_of(a.rows, a.channels, sizeof(T), kForwardThreads), cta,
-                  weights + (f ? cta * F::kBytes + segments * F::kExtra : 0), kWeights + (f ? kForward : 0), a, st);
+    const size_t smem = weights + (f ? cta * F::kBytes + segments * F::kExtra : 0);
+    return launch(norm_forward_kernel<T, V, kWarp, kMost, f>, grid_of(a.rows, a.channels, sizeof(T), kForwardThreads, smem), cta,
+                  smem, kWeights + (f ? kForward : 0), a, st);
 }
 
 template <typename T, int V>
@@ -628,6 +636,7 @@ int run(NormArgs a, bool backward, cudaStream_t st) {
     a.threads = threads_of(a.channels, sizeof(T));
     if (a.threads <= 32) return run_as<T, V, true, 256>(a, backward, st);
     if (a.threads <= 256) return run_as<T, V, false, 256>(a, backward, st);
+    if (a.threads <= 384) return run_as<T, V, false, 384>(a, backward, st);
     if constexpr (sizeof(T) == 4)
         if (a.threads > 512) return run_as<T, V, false, 1024>(a, backward, st);
     return run_as<T, V, false, 512>(a, backward, st);
