@@ -23,7 +23,8 @@ namespace seq {
 namespace {
 
 constexpr int kThreads = 256;                    // of a CTA that has a row, or a part of one
-constexpr int kFewThreads = 64;                  // of one that has a short row
+// of one that has a short row and up to 32 alternatives of it; up to 64: twice as many (4096x1000 bf16, 50 best 36 us, by 256 70 us)
+constexpr int kFewThreads = 64;
 constexpr int kWarpRows = 4;                     // rows of a CTA whose warps have one each
 constexpr int kCluster = 8;
 constexpr int kMostTop = DCN_SCORES_MOST_TOP, kMostK = DCN_DISTILL_MOST_K;
@@ -1015,19 +1016,21 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
     const int parts = warp ? 1 : parts_of(a.rows, a.vocab);
     cudaLaunchConfig_t cfg = {};
     size_t smem = 0;
-    bool few = false;
+    int threads = kThreads;
     if (kKind == kScoresTop) {
-        few = a.vocab <= kWarpVocab && a.top <= 32;
-        smem = few ? sizeof(TopRoom<kFewThreads>) : sizeof(TopRoom<kThreads>);
+        if (a.vocab <= kWarpVocab && a.top <= 64) threads = a.top <= 32 ? kFewThreads : 2 * kFewThreads;
+        smem = threads == kThreads      ? sizeof(TopRoom<kThreads>)
+               : threads == kFewThreads ? sizeof(TopRoom<kFewThreads>)
+                                        : sizeof(TopRoom<2 * kFewThreads>);
         // of every warp whose lanes all have a vector its share, or one more where that is less than twice `top` in all (the more,
         // the less is listed that is not among the `top`); of all CTAs together not more than there are keys
-        const int warps = (few ? kFewThreads : kThreads) / 32, vectors = a.vocab / (16 / (int)sizeof(T)) / parts;
+        const int warps = threads / 32, vectors = a.vocab / (16 / (int)sizeof(T)) / parts;
         // Short rows of which many are asked for are read element by element: where not many more lanes than `top` have a vector,
         // the largest of the lanes bound little and most elements would be ranked.  Such rows are shorter than the list, so that
-        // nothing but the usual path reads them.  (Element by element / in vectors, us: 12332x320 bf16, 50 best 128 / 558; 4096
-        // rows of bf16, 1000 with 128 best 100 / 777, with 70 66 / 99; 2000 with 128 122 / 100; by 64 threads, 256 with 20 31 / 26,
-        // with 28 the same, 128 with 32 27 / 40.)
-        a.single = parts == 1 && 8 * std::min(vectors, 32 * warps) < (few ? 10 : 15) * a.top;
+        // nothing but the usual path reads them.  (Element by element / in vectors, us, by 256 threads: 12332x320 bf16, 50 best 128 /
+        // 558; 4096 rows of bf16, 1000 with 128 best 100 / 777, with 70 66 / 99; 2000 with 128 122 / 100; by 64 threads, 256 with
+        // 20 31 / 26, with 28 the same, 128 with 32 27 / 40.)
+        a.single = parts == 1 && 8 * std::min(vectors, 32 * warps) < (threads == kFewThreads ? 10 : 15) * a.top;
         const int lanes = a.single ? a.vocab : vectors;
         const int full = lanes / 32 < 1 ? 1 : lanes / 32 < warps ? lanes / 32 : warps;
         const int share = (a.top + parts * full - 1) / (parts * full), most = 32 / parts;
@@ -1040,7 +1043,7 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
         smem = (size_t)a.marks * (warp ? kWarpRows : 1);
     }
     cfg.gridDim = dim3((unsigned)(warp ? (a.rows + kWarpRows - 1) / kWarpRows : a.rows * parts));
-    cfg.blockDim = dim3(warp ? 32 * kWarpRows : few ? kFewThreads : kThreads);
+    cfg.blockDim = dim3(warp ? 32 * kWarpRows : threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
@@ -1053,8 +1056,10 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
     cudaError_t e = cudaSuccess;
     if constexpr (kKind == kScoresTop) {
-        e = few ? cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, false, kFewThreads>, a)
-                : cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, false, kThreads>, a);
+        const auto kernel = threads == kThreads      ? logits_forward_kernel<T, kKind, false, kThreads>
+                            : threads == kFewThreads ? logits_forward_kernel<T, kKind, false, kFewThreads>
+                                                     : logits_forward_kernel<T, kKind, false, 2 * kFewThreads>;
+        e = cudaLaunchKernelEx(&cfg, kernel, a);
     } else if (warp) {
         e = cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, true, 32 * kWarpRows>, a);
     } else {

@@ -7,11 +7,11 @@
 //
 // A row lives in the registers of a row of threads, 32 bytes of each tensor a thread, so that every tensor is read or written
 // once.  Rows of up to 32 threads (512 channels of 16 bits, 256 of float32) share a warp, and their sums are shuffles alone; above,
-// a row is that of 64 to 512 (float32: 1024) threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a thread's elements of
-// the next row are on their way to its own places in shared memory meanwhile (cp.async, 16, 8 or 4 bytes at a time, as rows start
-// on them).  Weights are in shared memory too, once a CTA (registers for them would cost a third of the threads), and the arithmetic
-// goes in pairs through the packed float32 instructions.  The CTAs of the backward pass keep Z and dpre in registers and leave one
-// partial sum each; a second kernel adds those in a fixed order.
+// a row is that of 64 to 512 (float32: 1024) threads of a CTA, which meet at a barrier of their own.  CTAs walk the rows; a
+// thread's elements of the next row are on their way to its own places in shared memory meanwhile (cp.async, 16, 8 or 4 bytes at a
+// time, as rows start on them).  Weights are in shared memory too, once a CTA (registers for them would cost a third of the
+// threads), and the arithmetic goes in pairs through the packed float32 instructions.  The CTAs of the backward pass keep Z and
+// dpre in registers and leave one partial sum each; a second kernel adds those in a fixed order.
 //
 // The bound is DRAM, and the arithmetic, which leaves a third of the issue slots, stands close behind.  Measured, forward and
 // backward with the sums of the weights' gradients, against a copy of the same bytes at 6.5 TB/s:
