@@ -186,18 +186,18 @@ __device__ __forceinline__ Lanes pair_of(const uint32_t* w, int i) {
 }
 
 // The sums of a thread's elements.  kMarks: without the marked ones.  kAgain: the elements are read a second time.
-template <typename T, bool kU, bool kMarks, bool kAgain>
+template <typename T, bool kU, bool kMarks, bool kAgain, bool kSingle>
 __device__ __forceinline__ Sums sums_of(const Row<T>& row, int tid, int threads, float k, const uint8_t* marks) {
     using W = Word<T>;
     constexpr int kPer = Row<T>::kPer, kBatch = 4, kWords = 4 * kBatch;
     constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
     Sums a{kNone, 0.0f, 0.0f};
-    const int ends = row.head_here + (row.n - row.tail);          // elements outside vectors: at most one a thread, beside vectors
+    const int ends = row.head_here + (row.n - row.tail);          // elements outside vectors: at most one a thread, or all (kSingle)
     if (tid < ends) {
-        const bool head = tid < row.head_here;
-        const int e = head ? tid : row.tail + tid - row.head_here;
-        a = add_elements<T, kU, kMarks>(a, row, e, head ? row.head_here : e + 1, threads, k, marks);
+        const int e = tid < row.head_here ? tid : row.tail + tid - row.head_here;
+        a = add_elements<T, kU, kMarks>(a, row, e, kSingle ? ends : e + 1, kSingle ? threads : 1, k, marks);
     }
+    if constexpr (kSingle) return a;
     for (int v = row.v0 + tid; v < row.v1; v += kBatch * threads) {
         uint32_t w[kWords];
         const bool whole = v + (kBatch - 1) * threads < row.v1;
@@ -366,7 +366,7 @@ __device__ __forceinline__ uint32_t vector_max(const Raw<16>& v) {
 
 // Lists the elements that reach the bound in a room (another CTA's too), whose n counts them, listed or not.  Returns the number
 // of the warp's.
-template <typename T, int kT>
+template <bool kSingle, typename T, int kT>
 __device__ __forceinline__ int list_candidates(const Row<T>& row, int tid, uint32_t bound, TopRoom<kT>& r) {
     using W = Word<T>;
     constexpr int kPer = Row<T>::kPer, kBatch = 4;
@@ -394,10 +394,11 @@ __device__ __forceinline__ int list_candidates(const Row<T>& row, int tid, uint3
         }
     };
     const int ends = row.head_here + (row.n - row.tail);
-    for (int i = tid; i - tid < ends; i += kT) {
+    for (int i = tid; i - tid < (kSingle ? ends : kT); i += kT) {
         const int e = i < row.head_here ? i : row.tail + i - row.head_here;
         list(i < ends && reaches(row.one(e)) ? 1u : 0u, [&](int) { return e; });
     }
+    if constexpr (kSingle) return all;
     for (int first = row.v0 + tid - lane; first < row.v1; first += kBatch * kT) {       // (a warp's first vector)
         Raw<16> raw[kBatch];
 #pragma unroll
@@ -532,7 +533,7 @@ __device__ __noinline__ void top_of_part(const Row<T>& row, int tid, int top, ui
         equal = 1;
     }
     __syncthreads();
-    if (bound + equal >= bound) list_candidates(row, tid, bound + equal, r);
+    if (bound + equal >= bound) list_candidates<false>(row, tid, bound + equal, r);
     __syncthreads();
     const int n = r.n;
     if (equal) first_on_bound(row, tid, top - n, bound, r, out + n);
@@ -551,7 +552,6 @@ struct LogitsArgs {
     const int64_t* tokens;
     int64_t ignore;
     int top, top_each;                           // top_each: of the largest lanes of a warp, to find a bound from
-    int single;                                  // rows are read element by element
     float *logprob, *entropy, *top_logprobs;
     int64_t* top_tokens;
     const float *dlogprob, *dentropy, *dtop;
@@ -662,7 +662,7 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, in
     }
 }
 
-template <typename T, int kKind, bool kWarp, int kT>
+template <typename T, int kKind, bool kWarp, int kT, bool kSingle = false>
 __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float2 room[2][32];
@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
     if (at >= p.rows) return;                    // (a warp's row: a CTA's is always there)
     pdl_wait();
     const T* logits = static_cast<const T*>(p.logits) + at * p.stride;
-    const Row<T> row(logits, p.vocab, rank, ranks, kKind == kScoresTop && p.single != 0);
+    const Row<T> row(logits, p.vocab, rank, ranks, kSingle);
     TopRoom<kT>& top = *reinterpret_cast<TopRoom<kT>*>(dynamic);
     constexpr int kWarps = kT / 32;
     TeacherRoom& teacher = teachers[kKind == kDistill ? group : 0];
@@ -732,7 +732,7 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
         team.sync();
     }
     const Sums mine =
-        sums_of<T, kKind != kDistill, kKind == kDistill, kKind == kScoresTop>(row, team.tid, team.threads, p.k, marks);
+        sums_of<T, kKind != kDistill, kKind == kDistill, kKind == kScoresTop, kSingle>(row, team.tid, team.threads, p.k, marks);
     if constexpr (kKind == kDistill) {
 #pragma unroll
         for (int q = 0; q < kPlaces; ++q) {
@@ -766,7 +766,7 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
     if constexpr (kKind == kScoresTop) {
         const uint32_t bound = bound_of<kT>(top, ranks * kWarps * p.top_each, team.tid, p.top);
         TopRoom<kT>& first = ranks > 1 ? *cluster.map_shared_rank(&top, 0) : top;
-        const int listed = list_candidates(row, team.tid, bound, first);
+        const int listed = list_candidates<kSingle>(row, team.tid, bound, first);
         int n = 0;
         if (ranks > 1) {
             if (team.tid % 32 == 0) top.count[team.tid / 32] = listed;
@@ -1017,6 +1017,7 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
     cudaLaunchConfig_t cfg = {};
     size_t smem = 0;
     int threads = kThreads;
+    bool single = false;
     if (kKind == kScoresTop) {
         if (a.vocab <= kWarpVocab && a.top <= 64) threads = a.top <= 32 ? kFewThreads : 2 * kFewThreads;
         smem = threads == kThreads      ? sizeof(TopRoom<kThreads>)
@@ -1030,8 +1031,8 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
         // nothing but the usual path reads them.  (Element by element / in vectors, us, by 256 threads: 12332x320 bf16, 50 best 128 /
         // 558; 4096 rows of bf16, 1000 with 128 best 100 / 777, with 70 66 / 99; 2000 with 128 122 / 100; by 64 threads, 256 with
         // 20 31 / 26, with 28 the same, 128 with 32 27 / 40.)
-        a.single = parts == 1 && 8 * std::min(vectors, 32 * warps) < (threads == kFewThreads ? 10 : 15) * a.top;
-        const int lanes = a.single ? a.vocab : vectors;
+        single = parts == 1 && 8 * std::min(vectors, 32 * warps) < (threads == kFewThreads ? 10 : 15) * a.top;
+        const int lanes = single ? a.vocab : vectors;
         const int full = lanes / 32 < 1 ? 1 : lanes / 32 < warps ? lanes / 32 : warps;
         const int share = (a.top + parts * full - 1) / (parts * full), most = 32 / parts;
         a.top_each = parts * full * share < 2 * a.top ? share + 1 : share;
@@ -1056,10 +1057,14 @@ int run_forward(LogitsArgs a, cudaStream_t st) {
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
     cudaError_t e = cudaSuccess;
     if constexpr (kKind == kScoresTop) {
-        const auto kernel = threads == kThreads      ? logits_forward_kernel<T, kKind, false, kThreads>
-                            : threads == kFewThreads ? logits_forward_kernel<T, kKind, false, kFewThreads>
-                                                     : logits_forward_kernel<T, kKind, false, 2 * kFewThreads>;
-        e = cudaLaunchKernelEx(&cfg, kernel, a);
+        const auto launch = [&](auto one_by_one) {
+            constexpr bool kSingle = one_by_one.value;
+            const auto kernel = threads == kThreads      ? logits_forward_kernel<T, kKind, false, kThreads, kSingle>
+                                : threads == kFewThreads ? logits_forward_kernel<T, kKind, false, kFewThreads, kSingle>
+                                                         : logits_forward_kernel<T, kKind, false, 2 * kFewThreads, kSingle>;
+            return cudaLaunchKernelEx(&cfg, kernel, a);
+        };
+        e = single ? launch(std::true_type()) : launch(std::false_type());
     } else if (warp) {
         e = cudaLaunchKernelEx(&cfg, logits_forward_kernel<T, kKind, true, 32 * kWarpRows>, a);
     } else {
