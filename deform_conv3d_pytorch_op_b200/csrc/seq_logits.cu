@@ -29,7 +29,8 @@ constexpr int kWarpRows = 4;                     // rows of a CTA whose warps ha
 constexpr int kCluster = 8;
 constexpr int kMostTop = DCN_SCORES_MOST_TOP, kMostK = DCN_DISTILL_MOST_K;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr float kFar = 1e30f;                    // logits beyond it are shifted before they are scaled
+constexpr float kFar = 1e30f;                    // d is not below minus it: 0 times it is 0
+constexpr float kNear = 4194304.0f;              // 2^22: up to here a rounded m k is off by an eighth at most
 constexpr float kNone = -__builtin_huge_valf();
 
 enum Kind { kScores, kScoresTop, kDistill };
@@ -43,21 +44,23 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// d = (v - m) k.  As one product and one sum, unless that could overflow where v - m does not (masks of a type's lowest value);
-// the rounded m k is the same wherever a row's m is used, so it drops out of d - log2 S.
+// d = (v - m) k.  As one product and one sum, v k - c with c = m k, where m k is small: the rounded m k is the same wherever a row's
+// m is used, so what it is off by drops out of d - log2 S.  Larger ones (masks of any finite value, and what is summed before
+// anything else is seen) are off by more than 2^d has room for, or overflow where v - m does not: there the difference comes first,
+// (v - b) k with b = m.
 struct Shift {
-    float m, k, mk;
+    float k, b, c;
     bool far;
-    __device__ __forceinline__ Shift(float m_, float k_) : m(m_), k(k_) {
-        mk = __fmul_rn(m, k);
-        far = !(fabsf(m) < kFar);
+    __device__ __forceinline__ Shift(float m, float k_) : k(k_) {
+        const float mk = __fmul_rn(m, k);
+        far = !(fabsf(mk) < kNear);
+        b = far ? m : 0.0f;
+        c = far ? 0.0f : mk;
     }
-    __device__ __forceinline__ float operator()(float v) const {
-        return far ? __fmul_rn(__fsub_rn(v, m), k) : __fmaf_rn(v, k, -mk);
-    }
-    // from sums at this m to sums at another
+    __device__ __forceinline__ float operator()(float v) const { return __fmaf_rn(__fsub_rn(v, b), k, -c); }
+    // from sums at this m to sums at another, each as its d are formed
     __device__ __forceinline__ float to(const Shift& o) const {
-        return max_nan(far || o.far ? __fmul_rn(__fsub_rn(m, o.m), k) : __fsub_rn(mk, o.mk), -kFar);
+        return max_nan(__fmaf_rn(__fsub_rn(b, o.b), k, __fsub_rn(c, o.c)), -kFar);
     }
 };
 
@@ -139,8 +142,7 @@ __device__ __forceinline__ bool marked(const Row<T>& row, const uint8_t* marks, 
     return (marks[b >> 3] >> (b & 7) & 1) != 0;
 }
 
-// Elements one by one: those outside vectors, and rows whose logits are as large as the type allows.  Not inlined, so that the
-// usual path stays short.
+// Elements one by one, those outside vectors.  Not inlined, so that the usual path stays short.
 template <typename T, bool kU, bool kMarks>
 __device__ __noinline__ Sums add_elements(Sums a, const Row<T>& row, int e0, int e1, int step, float k, const uint8_t* marks) {
     for (int e = e0; e < e1; e += step) {
@@ -239,20 +241,15 @@ __device__ __forceinline__ Sums sums_of(const Row<T>& row, int tid, int threads,
         if (m == kNone) continue;
         if (m != a.m) a.rescale(m, k);
         const Shift shift(m, k);
-        if (shift.far) {
-            for (int b = v; b < min(v + kBatch * threads, row.v1); b += threads) {
-                const int e = row.head + b * kPer;
-                a = add_elements<T, kU, kMarks>(a, row, e, e + kPer, 1, k, marks);
-            }
-        } else {
-            const Lanes kk = all_lanes(k), shifted = all_lanes(-shift.mk);
+        auto add = [&](auto far) {
+            const Lanes kk = all_lanes(k), shifted = all_lanes(far.value ? -shift.b : -shift.c);
             Lanes s = all_lanes(0.0f), u = s;
 #pragma unroll
             for (int i = 0; i < kWords * W::kPer / 2; ++i) {
                 // 0 times what is far below is 0, not NaN: logits of -inf are raised to where their d is finite
-                if constexpr (kU && kBf16) w[i] = W::max(w[i], 0xf14af14au);             // -1e30
-                Lanes d = fma(pair_of<T>(w, i), kk, shifted);
-                if constexpr (kU && !kBf16) {
+                if constexpr (kU && kBf16 && !far.value) w[i] = W::max(w[i], 0xf14af14au);            // -1e30
+                Lanes d = far.value ? (pair_of<T>(w, i) + shifted) * kk : fma(pair_of<T>(w, i), kk, shifted);
+                if constexpr (kU && (!kBf16 || far.value)) {
                     const float f[2] = {max_nan(d.at(0), -kFar), max_nan(d.at(1), -kFar)};
                     d = lanes(f);
                 }
@@ -262,7 +259,9 @@ __device__ __forceinline__ Sums sums_of(const Row<T>& row, int tid, int threads,
             }
             a.s += s.at(0) + s.at(1);
             if constexpr (kU) a.u += u.at(0) + u.at(1);
-        }
+        };
+        if (shift.far) add(std::true_type());
+        else add(std::false_type());
     }
     return a;
 }
@@ -662,8 +661,14 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, in
     }
 }
 
+// 48 registers a thread where a fifth CTA of 256 threads is worth more (4096x8192 float32, 20 best: 56 us, 59 us with 58)
+template <typename T, int kKind, int kT, bool kSingle>
+constexpr int kHeld = kKind == kScoresTop && !kSingle && (std::is_same<T, __half>::value || (sizeof(T) == 4 && kT == kThreads))
+                          ? 5 * kThreads / kT
+                          : 0;
+
 template <typename T, int kKind, bool kWarp, int kT, bool kSingle = false>
-__global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) {
+__global__ void __launch_bounds__(kT, (kHeld<T, kKind, kT, kSingle>)) logits_forward_kernel(const LogitsArgs p) {
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ float2 room[2][32];
     __shared__ Sums parts[kCluster];
@@ -843,26 +848,29 @@ __global__ void __launch_bounds__(kT) logits_forward_kernel(const LogitsArgs p) 
 }
 
 // ---- backward -------------------------------------------------------------------------------------------------------------
-// dz = 2^l (c0 + c1 l), l = log2 p: p from (m, log2 S).  kLinear: c1 is 0.
+// dz = 2^l (c0 + c1 l), l = log2 p = (v - m) k - log2 S.  kLinear: c1 is 0.
 template <bool kLinear>
 struct Slope {
-    Shift shift;
-    float log_s, c0, c1;
-    bool zero;
-    __device__ __forceinline__ Slope(float m, float k, float log_s_, float c0_, float c1_)
-        : shift(m, k), log_s(log_s_), c0(c0_), c1(c1_), zero(m == kNone) {}
+    float minus_m, k, minus_log_s, c0, c1;
+    // (log_s of the sums as they were formed; here without what their m k is off by)
+    __device__ __forceinline__ Slope(float m, float k_, float log_s, float c0_, float c1_)
+        : minus_m(-m), k(k_), minus_log_s(-log_s), c0(c0_), c1(c1_) {
+        const Shift shift(m, k);
+        if (!shift.far) minus_log_s += __fmaf_rn(m, k, -shift.c);
+    }
+    __device__ __forceinline__ bool zero() const { return minus_m == -kNone; }
     __device__ __forceinline__ float operator()(float v) const {
-        if (zero) return 0.0f;
-        const float l = max_nan(shift(v) - log_s, -kFar);
+        if (zero()) return 0.0f;
+        const float l = max_nan(__fmaf_rn(__fadd_rn(v, minus_m), k, minus_log_s), -kFar);
         return ex2(l) * (kLinear ? c0 : fmaf(c1, l, c0));
     }
-    // a vector's, where the row is neither far nor zero
+    // a vector's, where the row is not zero
     template <typename T>
-    __device__ __forceinline__ void near(const uint32_t* w, float (&f)[16 / sizeof(T)]) const {
-        const Lanes kk = all_lanes(shift.k), shifted = all_lanes(-shift.mk), ss = all_lanes(-log_s);
+    __device__ __forceinline__ void vector(const uint32_t* w, float (&f)[16 / sizeof(T)]) const {
+        const Lanes kk = all_lanes(k), shifted = all_lanes(minus_m), ss = all_lanes(minus_log_s);
 #pragma unroll
         for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
-            Lanes l = fma(pair_of<T>(w, i), kk, shifted) + ss, c = all_lanes(c0);
+            Lanes l = fma(pair_of<T>(w, i) + shifted, kk, ss), c = all_lanes(c0);
             if constexpr (!kLinear) {
                 const float far[2] = {max_nan(l.at(0), -kFar), max_nan(l.at(1), -kFar)};
                 l = lanes(far);
@@ -892,16 +900,12 @@ __global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const Logi
     const Row<T> row(static_cast<const T*>(p.logits) + at * p.stride, p.vocab, part, parts);
     T* out = static_cast<T*>(p.dlogits) + at * p.vocab;
     const float* stat = p.stats + at * DCN_LOGITS_STATS;
-    const float m = gload(stat + kM), log_s = gload(stat + kLogS);
     // what the row's elements get; the special tokens get a term more
-    Slope<kDistilled> slope(m, p.k, log_s, 0.0f, 0.0f), special = slope;
+    Slope<kDistilled> slope(gload(stat + (kDistilled ? kRestM : kM)), p.k, gload(stat + (kDistilled ? kRestLogS : kLogS)), 0.0f, 0.0f);
     int specials;
-    float g = 0.0f;
     if constexpr (kDistilled) {
         specials = p.places;
-        g = gload(p.dloss + at) * p.temperature;
-        slope = Slope<true>(gload(stat + kRestM), p.k, gload(stat + kRestLogS), g * gload(stat + kRestC), 0.0f);
-        special.c0 = g * gload(stat + kMass);
+        slope.c0 = gload(p.dloss + at) * p.temperature * gload(stat + kRestC);
     } else {
         specials = p.dtop != nullptr ? p.top + 1 : 1;
         const float scale = 1.0f / p.temperature;
@@ -933,7 +937,6 @@ __global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const Logi
         }
         slope.c0 = -fmaf(gh * scale, gload(stat + kEntropy), all);
         slope.c1 = -scale * kLn2 * gh;
-        special = slope;
     }
     auto put = [&](int64_t e, float v) { out[e] = from_float<T>(v); };
     const int ends = row.head_here + (row.n - row.tail);          // elements outside vectors: at most one a thread
@@ -941,10 +944,10 @@ __global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const Logi
         const int e = tid < row.head_here ? tid : row.tail + tid - row.head_here;
         put(e, slope(row.one(e)));
     }
-    // vectors where the gradient's rows start as the logits' do, elements otherwise and in rows that are far or zero
+    // vectors where the gradient's rows start as the logits' do, elements otherwise and in rows that are zero
     constexpr int kBatch = 4;
     const bool alike = reinterpret_cast<uintptr_t>(out) % 16 == reinterpret_cast<uintptr_t>(row.p) % 16;
-    const bool vectors = alike && !slope.zero && !slope.shift.far;
+    const bool vectors = alike && !slope.zero();
     T* to = out + row.head;
     for (int v = row.v0 + tid; v < row.v1; v += kBatch * threads) {
         if (vectors && v + (kBatch - 1) * threads < row.v1) {
@@ -954,7 +957,7 @@ __global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const Logi
 #pragma unroll
             for (int b = 0; b < kBatch; ++b) {
                 float f[kPer];
-                slope.template near<T>(raw[b].u, f);
+                slope.template vector<T>(raw[b].u, f);
                 Pack<T, kPer> o;
                 o.set(f);
                 if constexpr (kStream) store_streaming(to + (int64_t)(v + b * threads) * kPer, o.raw);
@@ -967,7 +970,7 @@ __global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const Logi
                 load(raw, row.vec(u));
                 float f[kPer];
                 if (vectors) {
-                    slope.template near<T>(raw.u, f);
+                    slope.template vector<T>(raw.u, f);
                     Pack<T, kPer> o;
                     o.set(f);
                     o.put(to + (int64_t)u * kPer);
@@ -979,8 +982,9 @@ __global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const Logi
             }
         }
     }
-    if constexpr (kDistilled) {
-        const float norm = gload(stat + kNorm);
+    if constexpr (kDistilled) {                  // (read here: the registers were the row's)
+        const float g = gload(p.dloss + at) * p.temperature, norm = gload(stat + kNorm);
+        slope = Slope<true>(gload(stat + kM), p.k, gload(stat + kLogS), g * gload(stat + kMass), 0.0f);
         for (int i = tid; i < specials; i += threads) {
             const int64_t t = gload_i64(p.teacher_tokens + at * p.places + i);
             const bool in = t >= 0 && t < p.vocab;
@@ -989,13 +993,13 @@ __global__ void __launch_bounds__(kThreads, 6) logits_backward_kernel(const Logi
         }
     }
     __syncthreads();                             // the part's special tokens are written over what stands there
-    if (special.zero) return;
+    if (slope.zero()) return;
     for (int i = tid; i < specials; i += threads) {
         const int t = token[i];
         if (t < 0 || !in_part(row, t)) continue;
         float w = 0.0f;
         for (int j = 0; j < specials; ++j) w += token[j] == t ? weight[j] : 0.0f;
-        put(t, special(row.one(t)) + w);
+        put(t, slope(row.one(t)) + w);
     }
 }
 

@@ -1,0 +1,113 @@
+"""The sequence operators at the edges of their values, and of how they are called."""
+import math
+
+import pytest
+import torch
+
+from tests import sequence_reference as ref
+from tests.sequence_reference import TYPES, close
+
+pytestmark = pytest.mark.gpu
+dcn = pytest.importorskip("deform_conv3d_pytorch_op_b200")
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(g, *shape, std=1.0, mean=0.0, dtype=torch.float32):
+    return (torch.randn(shape, generator=g, device="cuda") * std + mean).to(dtype)
+
+
+def wide(t):
+    return t.detach().double().requires_grad_()
+
+
+# ---- logits of any finite size ----------------------------------------------------------------------------------------------
+def _masked_rows(g, v, value, t):
+    """Rows of which a finite value masks everything, contiguous parts, the ends alone, all but a token, and rows near it"""
+    rows = randn(g, 9, v, std=2.0, dtype=t)
+    rows[0] = value
+    rows[1, : v // 2] = value
+    rows[2, v // 3:] = value
+    rows[3, :3] = rows[3, -3:] = value
+    rows[4, 3:-3] = value
+    rows[5] = value
+    rows[5, v // 2] = 1.0
+    rows[6, ::2] = value
+    rows[7] = value * (1 + randn(g, v).abs() / 16)            # nothing but values of this size, and all different
+    rows[8] = value
+    rows[8, 1] = -value                                       # both signs
+    return rows
+
+
+# Results are compared row by row at the bound of every other row: a difference to the largest logit is rounded once, relative
+# to itself, whatever the size of the two.
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [-1e6, -1e9, -1e10, -1e12, -1e20, -3e38, 1e10, 1e20])
+def test_scores_of_rows_with_large_finite_values(kind, value):
+    for v in (301, 1500, 5003, 70001):
+        g, t = gen(v), TYPES[kind]
+        logits = _masked_rows(g, v, value, t).requires_grad_()
+        w = wide(logits)
+        for temperature, top in ((1.0, 0), (0.1, 3), (1.0, min(v, 100))):
+            if abs(value) > 1e38 and temperature < 1:
+                continue                                      # (their log p is beyond float32)
+            tokens = torch.tensor([0, v - 1, v // 2] * 3, device="cuda")
+            outs = dcn.TokenScoresFunction.apply(logits, tokens, top, temperature)
+            wants = ref.token_scores(w, tokens, top, temperature)
+            gouts = [randn(g, *o.shape) for o in outs[:3] if o is not None]
+            (got,) = torch.autograd.grad([o for o in outs[:3] if o is not None], logits, gouts)
+            (want,) = torch.autograd.grad(wants[:3 if top else 2], w, [a.double() for a in gouts])
+            for r in range(9):
+                what = (v, temperature, top, r)
+                for a, b in zip(outs[:3], wants):
+                    if a is not None:
+                        b = b[r].float().double() if abs(value) > 1e38 else b[r]
+                        close(a[r], b, what, scale=1.0)
+                if top:
+                    assert torch.equal(outs[3][r], wants[3][r]), what
+                close(got[r], want[r], what, scale=1e-3)
+
+
+def _distill_by_formula(z, lq, tokens, dloss, temperature, tail):
+    """Loss and gradient in 64 bits, from differences to the largest logit of each part: log p itself, of a size of 1e20, would
+    not hold what the tokens of the rest are to one another."""
+    z, lq, dloss = z.detach().double() / temperature, lq.double(), dloss.double()
+    teachers = torch.zeros_like(z, dtype=torch.bool).scatter_(1, tokens, True)
+    m, rest = z.amax(1, keepdim=True), z.masked_fill(teachers, -math.inf)
+    top = rest.amax(1, keepdim=True)
+    s = torch.exp(z - m).sum(1, keepdim=True)
+    e = torch.exp(rest - top)
+    if not tail:
+        lq = torch.log_softmax(lq, 1)
+    q = torch.exp(lq)
+    left = (1 - q.sum(1, keepdim=True)).clamp(min=0) if tail else torch.zeros_like(m)
+    loss = (q * (lq - (z.gather(1, tokens) - m - torch.log(s)))).sum(1, keepdim=True)
+    loss = loss + torch.where(left > 0, left * (torch.log(left) - (top - m + torch.log(e.sum(1, keepdim=True)) - torch.log(s))), 0.0)
+    dz = torch.exp(z - m) / s * (q.sum(1, keepdim=True) + left) - left * e / e.sum(1, keepdim=True)
+    dz.scatter_add_(1, tokens, -q)
+    return loss[:, 0] * temperature ** 2, dz * temperature * dloss[:, None]
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [-1e6, -1e9, -1e10, -1e12, -1e20, 1e10])
+@pytest.mark.parametrize("tail", [True, False])
+def test_distill_of_rows_with_large_finite_values(kind, value, tail):
+    for v, k in ((301, 5), (2500, 20), (70001, 64)):
+        g, t = gen(v + k), TYPES[kind]
+        logits = _masked_rows(g, v, value, t)
+        teacher = randn(g, 9, v, std=2.0)
+        best, tokens = teacher.topk(k)
+        lq = best - teacher.logsumexp(-1, keepdim=True)
+        keep = logits[2].gather(0, tokens[2])
+        logits[2] = value                                     # all that the teacher does not name
+        logits[2].scatter_(0, tokens[2], torch.where(keep == value, torch.ones_like(keep), keep))
+        logits.requires_grad_()
+        for temperature in (1.0, 0.1):
+            loss, go = dcn.DistillTopkFunction.apply(logits, lq, tokens, temperature, tail), randn(g, 9)
+            (got,) = torch.autograd.grad(loss, logits, go)
+            want, grad = _distill_by_formula(logits, lq, tokens, go, temperature, tail)
+            for r in range(9):
+                close(loss[r], want[r], (v, temperature, r), scale=1.0)
+                close(got[r], grad[r], (v, temperature, r), scale=1e-3)
