@@ -111,3 +111,22 @@ def test_distill_of_rows_with_large_finite_values(kind, value, tail):
             for r in range(9):
                 close(loss[r], want[r], (v, temperature, r), scale=1.0)
                 close(got[r], grad[r], (v, temperature, r), scale=1e-3)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("value", [-1e29, -1e30, -1e36, -3e38])
+@pytest.mark.parametrize("v", [301, 70001])
+def test_distill_with_all_other_tokens_masked_by_the_lowest_values(kind, value, v):
+    """The rest of the teacher's probability meets a log p of the mask's size: a loss that float32 holds, and the right one."""
+    g, t, k = gen(v), TYPES[kind], 7
+    teacher = randn(g, 4, v, std=2.0)
+    best, tokens = teacher.topk(k)
+    lq = best - teacher.logsumexp(-1, keepdim=True)
+    logits = torch.full((4, v), value, device="cuda", dtype=t)
+    logits.scatter_(1, tokens, randn(g, 4, k, dtype=t))
+    logits.requires_grad_()
+    loss = dcn.DistillTopkFunction.apply(logits, lq, tokens)
+    (a,) = torch.autograd.grad(loss.sum(), logits)
+    want, b = _distill_by_formula(logits, lq, tokens, torch.ones(4, device="cuda"), 1.0, True)
+    close(loss, want)
+    close(a, b, scale=1e-3)
