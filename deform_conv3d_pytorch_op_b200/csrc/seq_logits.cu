@@ -30,6 +30,7 @@ constexpr int kCluster = 8;
 constexpr int kMostTop = DCN_SCORES_MOST_TOP, kMostK = DCN_DISTILL_MOST_K;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kFar = 1e30f;                    // d is not below minus it: 0 times it is 0
+constexpr float kGone = 1e4f;                    // 2^-kGone is 0, and what kGone is multiplied with stays finite
 constexpr float kNear = 4194304.0f;              // 2^22: up to here a rounded m k is off by an eighth at most
 constexpr float kNone = -__builtin_huge_valf();
 
@@ -863,7 +864,7 @@ struct Slope {
     __device__ __forceinline__ bool zero() const { return minus_m == -kNone; }
     __device__ __forceinline__ float operator()(float v) const {
         if (zero()) return 0.0f;
-        const float l = max_nan(__fmaf_rn(__fadd_rn(v, minus_m), k, minus_log_s), -kFar);
+        const float l = max_nan(__fmaf_rn(__fadd_rn(v, minus_m), k, minus_log_s), -kGone);
         return ex2(l) * (kLinear ? c0 : fmaf(c1, l, c0));
     }
     // a vector's, where the row is not zero
@@ -874,7 +875,7 @@ struct Slope {
         for (int i = 0; i < 8 / (int)sizeof(T); ++i) {
             Lanes l = fma(pair_of<T>(w, i) + shifted, kk, ss), c = all_lanes(c0);
             if constexpr (!kLinear) {
-                const float far[2] = {max_nan(l.at(0), -kFar), max_nan(l.at(1), -kFar)};
+                const float far[2] = {max_nan(l.at(0), -kGone), max_nan(l.at(1), -kGone)};
                 l = lanes(far);
                 c = fma(all_lanes(c1), l, c);
             }

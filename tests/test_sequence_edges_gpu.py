@@ -130,3 +130,21 @@ def test_distill_with_all_other_tokens_masked_by_the_lowest_values(kind, value, 
     want, b = _distill_by_formula(logits, lq, tokens, torch.ones(4, device="cuda"), 1.0, True)
     close(loss, want)
     close(a, b, scale=1e-3)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dentropy,temperature", [(1.0, 1.0), (1e9, 1.0), (3e6, 1e-3), (-1e20, 2.0)])
+def test_entropy_gradients_of_any_size_beside_masked_tokens(kind, dentropy, temperature):
+    """p log p of a token that cannot come is 0 whatever it is multiplied with (loss scaling, low temperatures)."""
+    g, t = gen(5), TYPES[kind]
+    for v in (300, 5003):
+        logits = randn(g, 5, v, std=0.01 if temperature < 1 else 1.0, dtype=torch.float32)
+        logits[0, ::3], logits[1, v // 2:], logits[2, :5] = -math.inf, -math.inf, -1e4
+        logits = logits.to(t).requires_grad_()
+        w = wide(logits)
+        entropy = dcn.TokenScoresFunction.apply(logits, None, 0, temperature)[1]
+        want = ref.token_scores(w, torch.zeros(5, dtype=torch.long, device="cuda"), 0, temperature)[1]
+        go = torch.full((5,), dentropy, device="cuda")
+        (a,), (b,) = torch.autograd.grad(entropy, logits, go), torch.autograd.grad(want, w, go.double())
+        for r in range(5):
+            close(a[r], b[r], (v, r))
