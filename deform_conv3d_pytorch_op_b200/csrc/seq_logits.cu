@@ -107,7 +107,7 @@ struct Row {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) f(head + v * kPer + i, a.at(i));
         }
-        for (int e = tail + tid; e < n; e += threads) f(e, one(e));
+        for (int i = tid; i < n - tail; i += threads) f(tail + i, one(tail + i));     // (tail + tid may be past 31 bits)
     }
     __device__ __forceinline__ float one(int64_t e) const {
         Pack<T, 1> a;
@@ -479,7 +479,7 @@ __device__ __noinline__ void first_on_bound(const Row<T>& row, int tid, int need
     };
     take(tid, tid < row.head_here ? 1 : 0);
     for (int v = row.v0; v < row.v1 && done < need; v += kT) take(row.head + (v + tid) * kPer, v + tid < row.v1 ? kPer : 0);
-    if (done < need) take(row.tail + tid, row.tail + tid < row.n ? 1 : 0);
+    if (done < need) take(row.tail + tid, tid < row.n - row.tail ? 1 : 0);
 }
 
 // The largest keys of a warp's lanes, `each` of them, into to[0, each) (0 behind the last element)

@@ -148,3 +148,25 @@ def test_entropy_gradients_of_any_size_beside_masked_tokens(kind, dentropy, temp
         (a,), (b,) = torch.autograd.grad(entropy, logits, go), torch.autograd.grad(want, w, go.double())
         for r in range(5):
             close(a[r], b[r], (v, r))
+
+
+@pytest.mark.parametrize("start", [0, 3])
+def test_scores_of_a_row_of_nearly_2_to_the_31_tokens(start):
+    """Alternatives among equal values, whose last elements are counted behind the row's last vector"""
+    v = 2 ** 31 - 1
+    row = torch.zeros(v + start, device="cuda", dtype=torch.bfloat16)[start:][None]
+    high = {v - 1: 3.0, v - 4: 2.0, 17: 2.5, 2 ** 30: 1.0}
+    for at, value in high.items():
+        row[0, at] = value
+    logprob, entropy, best, best_tokens = dcn.TokenScoresFunction.apply(row, torch.tensor([v - 1], device="cuda"), 128)
+    first = sorted(high, key=lambda at: -high[at])
+    assert best_tokens[0].tolist() == first + [i for i in range(126) if i != 17][:124]
+    total = v - len(high) + sum(math.exp(x) for x in high.values())
+    wants = [x - math.log(total) for x in [high[at] for at in first] + [0.0] * 124]
+    # a thread adds some 2^15 batches of its 2^20 elements to one float, each at half a unit of the sum's last place: 2^-10 of S, and
+    # of U, at most
+    log = 22 * ref.CHAIN + 2.0 ** -10
+    assert float((best[0].double() - torch.tensor(wants, device="cuda", dtype=torch.float64)).abs().max()) <= log
+    assert abs(float(logprob) - wants[0]) <= log
+    mean = sum(x * math.exp(x) for x in high.values()) / total
+    assert abs(float(entropy) - (math.log(total) - mean)) <= 2 * log + 4.4 * 2.0 ** -10      # (U / S is 3 / ln 2)
