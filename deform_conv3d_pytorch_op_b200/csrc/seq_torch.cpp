@@ -611,15 +611,19 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
-// (x, gate, state, slots): one step, the state in place
+// (x, gate, state, slots): one step, the state in place.  kInner: for the Function of sequence.py
+template <bool kInner>
 PyObject* scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         count_arg(n, 3, 4);
         const Tensor x0 = tensor_arg(a[0], "x"), gate0 = tensor_arg(a[1], "gate"), state = tensor_arg(a[2], "state");
         const Tensor slots0 = n > 3 ? tensor_arg(a[3], "slots", true) : Tensor();
-        pybind11::gil_scoped_release no_gil;
         if (at::GradMode::is_enabled() && (x0.requires_grad() || gate0.requires_grad() || state.requires_grad()))
             fail("step has no gradient: call it under torch.no_grad(), or take apply");
+        for (const Tensor& t : {x0, gate0, state})               // (before the state advances)
+            if (torch::autograd::isFwGradDefined(t)) fail("step has no derivative: take apply");
+        if (!kInner && transformed({x0, gate0, state, slots0})) Py_RETURN_NOTIMPLEMENTED;
+        pybind11::gil_scoped_release no_gil;
         at::NoGradGuard no_grad;
         on_gpu(x0, "x");
         const int32_t type = type_of(x0, "x");
@@ -655,7 +659,8 @@ PyMethodDef dcn_host::sequence_methods[] = {
     {"gated_scan", DCN_FAST(apply<&kScan>), nullptr},
     {"gated_scan_forward", DCN_FAST(forward<&kScan>), nullptr},
     {"gated_scan_backward", DCN_FAST(backward<&kScan>), nullptr},
-    {"gated_scan_step", DCN_FAST(scan_step), nullptr},
+    {"gated_scan_step", DCN_FAST(scan_step<false>), nullptr},
+    {"gated_scan_step_forward", DCN_FAST(scan_step<true>), nullptr},
     {"residual_norm", DCN_FAST(apply<&kNorm>), nullptr},
     {"residual_norm_forward", DCN_FAST(forward<&kNorm>), nullptr},
     {"residual_norm_backward", DCN_FAST(backward<&kNorm>), nullptr},

@@ -60,6 +60,19 @@ _TokenScoresFunction = _function("token_scores", 1)
 _DistillTopkFunction = _function("distill_topk", 1)
 
 
+class _GatedScanStepFunction(Function):
+    """A step that traces record; it has no derivative of any kind (and no transform: there is no setup_context)."""
+
+    @staticmethod
+    def forward(ctx, x, gate, state, slots):
+        return _lib.native().gated_scan_step_forward(x, gate, state, slots)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        raise RuntimeError("step has no gradient: take apply")
+
+
 class GatedScanFunction:
     """Per-channel recurrence over time: ``h_t = a_t h_{t-1} + (1 - a_t) x_t``, ``a_t = sigmoid(gate_t)``."""
 
@@ -78,7 +91,8 @@ class GatedScanFunction:
         """One step of running sequences, without gradients: ``x``, ``gate`` [rows, channels]; ``state`` [pool, channels]
         float32, contiguous, advanced in place at the rows ``slots`` [rows] (0, 1, ... if None), each of which occurs once; a
         slot outside the pool is skipped, and its row is zero.  Returns the new states [rows, channels] in x's type."""
-        return _lib.native().gated_scan_step(x, gate, state, slots)
+        out = _lib.native().gated_scan_step(x, gate, state, slots)
+        return _GatedScanStepFunction.apply(x, gate, state, slots) if out is NotImplemented else out
 
 
 class ResidualNormFunction:

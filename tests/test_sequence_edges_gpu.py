@@ -170,3 +170,52 @@ def test_scores_of_a_row_of_nearly_2_to_the_31_tokens(start):
     assert abs(float(logprob) - wants[0]) <= log
     mean = sum(x * math.exp(x) for x in high.values()) / total
     assert abs(float(entropy) - (math.log(total) - mean)) <= 2 * log + 4.4 * 2.0 ** -10      # (U / S is 3 / ln 2)
+
+
+# ---- single steps -----------------------------------------------------------------------------------------------------------
+def test_traced_steps_advance_the_pool():
+    from deform_conv3d_pytorch_op_b200.video_sequence import SequenceHead
+    torch.manual_seed(6)
+    g = gen(6)
+    slots = torch.tensor([3, 0, 5], device="cuda")
+    step = lambda x, gate, state, slots: dcn.GatedScanFunction.step(x, gate, state, slots)  # noqa: E731
+    example = [randn(g, 3, 20), randn(g, 3, 20), randn(g, 6, 20)]
+    traced = torch.jit.trace(step, (*example, slots), check_trace=False)
+    x, gate, pool = randn(g, 3, 20), randn(g, 3, 20), randn(g, 6, 20)
+    for _ in range(3):
+        want_pool = pool.clone()
+        want = dcn.GatedScanFunction.step(x, gate, want_pool, slots)
+        assert torch.equal(traced(x, gate, pool, slots), want) and torch.equal(pool, want_pool)
+    head = SequenceHead(12, 24, 9, device="cuda")
+
+    class Live(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.head = head
+
+        def forward(self, f, a, b, s):
+            return self.head.step(f, [a, b], s)
+
+    live = torch.jit.trace(Live(), (randn(g, 3, 12), *head.new_pool(6), slots), check_trace=False)
+    here, there = head.new_pool(6), head.new_pool(6)
+    for _ in range(4):
+        f = randn(g, 3, 12)
+        assert torch.equal(live(f, *here, slots), head.step(f, there, slots))
+        assert all(torch.equal(a, b) for a, b in zip(here, there))
+    assert all(bool(a[slots].any()) for a in here)
+
+
+def test_steps_refuse_derivatives_and_transforms():
+    import torch.autograd.forward_ad as fwad
+    g = gen(7)
+    x, gate, pool = randn(g, 3, 20), randn(g, 3, 20), randn(g, 3, 20)
+    before = pool.clone()
+    with fwad.dual_level():
+        for i in range(3):
+            args = [x, gate, pool]
+            args[i] = fwad.make_dual(args[i], torch.ones_like(args[i]))
+            with pytest.raises(RuntimeError), torch.no_grad():
+                dcn.GatedScanFunction.step(*args)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda a, b, c: dcn.GatedScanFunction.step(a[None], b[None], c[None]))(x, gate, pool)
+    assert torch.equal(pool, before)
