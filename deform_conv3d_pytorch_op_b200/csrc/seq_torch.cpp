@@ -641,13 +641,13 @@ PyObject* scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Tensor x = dense_last(x0), gate = dense_last(gate0), slots = whole_numbers(slots0, "slots");
         const c10::cuda::CUDAGuard guard(x.device());
         Tensor y = at::empty(x.sizes(), x.options());
+        state.unsafeGetTensorImpl()->bump_version();             // (refuses an inference tensor outside inference mode: nothing ran)
         {
             Range range("dcn_scan_step");
             check(dcn_scan_step(type, x.size(0), x.size(1), ptr(x), x.stride(0), ptr(gate), gate.stride(0), fptr(state),
                                 state.size(0), iptr(slots), wptr(y), current_stream(x)),
                   "dcn_scan_step");
         }
-        state.unsafeGetTensorImpl()->bump_version();
         pybind11::gil_scoped_acquire gil;
         return THPVariable_Wrap(std::move(y));
     });

@@ -219,3 +219,18 @@ def test_steps_refuse_derivatives_and_transforms():
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda a, b, c: dcn.GatedScanFunction.step(a[None], b[None], c[None]))(x, gate, pool)
     assert torch.equal(pool, before)
+
+
+def test_steps_leave_an_inference_pool_alone_outside_inference_mode():
+    g = gen(8)
+    x, gate = randn(g, 3, 20), randn(g, 3, 20)
+    with torch.inference_mode():
+        pool = randn(g, 3, 20)
+        before = pool.clone()
+    with torch.no_grad(), pytest.raises(RuntimeError, match="nference"):
+        dcn.GatedScanFunction.step(x, gate, pool)
+    torch.cuda.synchronize()
+    assert torch.equal(pool, before)
+    with torch.inference_mode():
+        y = dcn.GatedScanFunction.step(x, gate, pool)
+        assert torch.equal(y, pool) and not torch.equal(pool, before)
