@@ -42,7 +42,7 @@ size_t dcn_scan_checkpoint_bytes(const dcn_scan* p);
 /* y [batch, steps, channels] (dense) and last [batch, channels] (float32): the states after each step and after the last one.
  * `state` [batch, channels] float32, or NULL for zeros.  `lengths` [batch] int64, or NULL: sequence b has lengths[b] steps (taken
  * into [0, steps]); behind them y is zero, and x and gate are not used, whatever they hold.  `checkpoints` NULL where no
- * gradient is wanted. */
+ * gradient is wanted.  An infinite state (or x) stays infinite while gates are above zero in float32 (those above -87). */
 int dcn_scan_forward(const dcn_scan* p, const void* x, const void* gate, const float* state, const int64_t* lengths, void* y,
                      float* last, float* checkpoints, void* stream);
 

@@ -234,3 +234,50 @@ def test_steps_leave_an_inference_pool_alone_outside_inference_mode():
     with torch.inference_mode():
         y = dcn.GatedScanFunction.step(x, gate, pool)
         assert torch.equal(y, pool) and not torch.equal(pool, before)
+
+
+# ---- infinite states --------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("gates", ["mixed", "slow", "fast"])
+@pytest.mark.parametrize("shape", [(1, 5, 3), (2, 40, 70), (1, 64, 5), (2, 130, 33), (1, 1500, 40), (160, 200, 64)])
+def test_scan_keeps_infinite_states(shape, gates, kind):
+    """They stay what they are while gates are above zero, wherever a thread's, a warp's or a CTA's steps end.  Gates of -8 give a
+    product that float32 does not hold after a few of a thread's steps."""
+    b, n, c = shape
+    g, t = gen(n + c), TYPES[kind]
+    mean, std = {"mixed": (1.0, 1.5), "slow": (12.0, 0.5), "fast": (-8.0, 0.5)}[gates]
+    x, gate, state = randn(g, b, n, c, dtype=t), randn(g, b, n, c, mean=mean, std=std, dtype=t), randn(g, b, c)
+    lengths = torch.randint(1, n + 1, (b,), generator=g, device="cuda")
+    lengths[0] = n
+    state[0, 0], state[-1, 1] = math.inf, -math.inf
+    x[0, n // 2, 2] = math.inf                                # from a step on
+    if b > 1:
+        lengths[1], state[1, 0] = 0, -math.inf
+    dy, dlast = randn(g, b, n, c, dtype=t), randn(g, b, c)
+    ins = [v.requires_grad_() for v in (x, gate, state)]
+    for le in (None, lengths):
+        y, last = dcn.GatedScanFunction.apply(*ins, le)
+        w = [wide(v) for v in ins]
+        wy, wl = ref.scan(*w, le)
+        close(y, wy, "y")
+        close(last, wl, "last")
+        got = torch.autograd.grad((y, last), ins, (dy, dlast))
+        want = torch.autograd.grad((wy, wl), w, (dy.double(), dlast.double()))
+        for name, a, v in zip(("dx", "dgate", "dstate"), got, want):
+            if name != "dgate":
+                close(a, v, name)
+            else:                                             # (no number where the state, or x, is infinite)
+                there = torch.isfinite(v) & torch.isfinite(a)
+                assert bool((there | ~torch.isfinite(v)).all())
+                close(torch.where(there, a, 0.0), torch.where(there, v, 0.0), name)
+
+
+def test_scan_with_an_infinite_state_in_odd_channels_only():
+    """Channels beside an infinite one, of its pair and its vectors, are not touched."""
+    g = gen(11)
+    x, gate, state = randn(g, 2, 300, 64), randn(g, 2, 300, 64, mean=2.0), randn(g, 2, 64)
+    y, last = dcn.GatedScanFunction.apply(x, gate, state)
+    state[:, 1::2] = math.inf
+    z, end = dcn.GatedScanFunction.apply(x, gate, state)
+    assert torch.equal(z[..., ::2], y[..., ::2]) and torch.equal(end[:, ::2], last[:, ::2])
+    assert bool((z[..., 1::2] == math.inf).all()) and bool((end[:, 1::2] == math.inf).all())
