@@ -683,11 +683,12 @@ __global__ void __launch_bounds__(128)
             h.get(state + slot * channels + c);
 #pragma unroll
             for (int i = 0; i < W; ++i) {
-                // a h + (1 - a) x as a step from the larger share: no product with a gate near one is rounded
+                // a h + (1 - a) x as a step from the larger share: no product with a gate near one is rounded.  As it stands where
+                // the two are further apart than float32 holds.
                 float a, keep;
                 logistic(vg.at(i), a, keep);
-                const float from = a < keep ? vx.at(i) : h.at(i), to = a < keep ? h.at(i) : vx.at(i);
-                out[i] = fmaf(a < keep ? a : keep, to - from, from);
+                const float from = a < keep ? vx.at(i) : h.at(i), to = a < keep ? h.at(i) : vx.at(i), way = to - from;
+                out[i] = fabsf(way) < CUDART_INF_F ? fmaf(a < keep ? a : keep, way, from) : fmaf(a, h.at(i), keep * vx.at(i));
             }
             h.set(out);
             h.put(state + slot * channels + c);

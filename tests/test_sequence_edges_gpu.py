@@ -281,3 +281,22 @@ def test_scan_with_an_infinite_state_in_odd_channels_only():
     z, end = dcn.GatedScanFunction.apply(x, gate, state)
     assert torch.equal(z[..., ::2], y[..., ::2]) and torch.equal(end[:, ::2], last[:, ::2])
     assert bool((z[..., 1::2] == math.inf).all()) and bool((end[:, 1::2] == math.inf).all())
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("channels", [64, 7])
+def test_steps_between_values_of_any_size(kind, channels):
+    """An infinite state stays infinite, and finite ones of opposite signs meet in between, however far apart."""
+    t = TYPES[kind]
+    big = 3e38
+    h = torch.tensor([math.inf, -math.inf, math.inf, 1.0, big, -big, big, math.inf, math.nan, 1e30, 2.0], device="cuda")
+    x = torch.tensor([1.0, -2.0, math.inf, -math.inf, -big, big, big, -math.inf, 1.0, -1e30, math.nan], device="cuda").to(t)
+    for gate in (-3.0, 0.0, 0.25, 9.0):
+        pool = h[:, None].repeat(1, channels)
+        xs, gs = x[:, None].repeat(1, channels), torch.full((len(x), channels), gate, device="cuda", dtype=t)
+        want = ref.scan(xs[:, None].double(), gs[:, None].double(), pool.double())[1]
+        y = dcn.GatedScanFunction.step(xs, gs, pool)
+        for r in range(len(x)):                               # (a difference of two large values: their rounding)
+            close(pool[r], want[r], r, scale=min(float(h[r].abs().nan_to_num(0, 0)), 3e38))
+            close(y[r], torch.where(want[r].abs() > torch.finfo(t).max, want[r].sign() * math.inf, want[r]), r,
+                  scale=min(float(h[r].abs().nan_to_num(0, 0)), 3e38))
