@@ -192,7 +192,8 @@ class ResidualNorm(nn.Module):
 
 
 class TopkDistillLoss(nn.Module):
-    """Mean of :class:`DistillTopkFunction` over the rows.  :meth:`teacher` makes its targets from a teacher's logits."""
+    """Mean of :class:`DistillTopkFunction` over all rows, those without a used place among them (whose loss is 0).
+    :meth:`teacher` makes its targets from a teacher's logits."""
 
     def __init__(self, k, temperature=1.0, tail=True):
         super().__init__()

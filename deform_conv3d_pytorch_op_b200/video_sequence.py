@@ -80,13 +80,16 @@ class SequenceHead(nn.Module):
 
 
 def train_step(head, loss, opt, features, teacher, lengths=None):
-    """One step from the teacher's best classes (``loss.teacher(logits)``); padding behind a sequence's clips is left out."""
+    """One step from the teacher's best classes (``loss.teacher(logits)``).  Padding behind a sequence's clips is left out: the
+    loss is the mean over the clips, however long the batch's longest sequence is (0 without any)."""
     logits, _ = head(features, lengths=lengths)
     logprobs, classes = teacher
     if lengths is not None:
         behind = torch.arange(features.size(1), device=features.device)[None, :] >= lengths[:, None]
         classes = torch.where(behind[..., None], -1, classes)
     value = loss(logits, logprobs, classes)
+    if lengths is not None:                        # (the mean over all rows, of which those behind a sequence's end have 0)
+        value = value * (behind.numel() / (~behind).sum().clamp(min=1))
     opt.zero_grad(set_to_none=True)
     value.backward()
     opt.step()

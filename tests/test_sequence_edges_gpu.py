@@ -300,3 +300,36 @@ def test_steps_between_values_of_any_size(kind, channels):
             close(pool[r], want[r], r, scale=min(float(h[r].abs().nan_to_num(0, 0)), 3e38))
             close(y[r], torch.where(want[r].abs() > torch.finfo(t).max, want[r].sign() * math.inf, want[r]), r,
                   scale=min(float(h[r].abs().nan_to_num(0, 0)), 3e38))
+
+
+# ---- the head ---------------------------------------------------------------------------------------------------------------
+def test_padding_does_not_change_a_training_step():
+    from deform_conv3d_pytorch_op_b200.video_sequence import SequenceHead, train_step
+    g = gen(13)
+    loss = dcn.TopkDistillLoss(4, temperature=1.5)
+    x, judged = randn(g, 4, 9, 16), randn(g, 4, 9, 20, std=2.0)
+    lengths = torch.tensor([9, 0, 3, 7], device="cuda")
+    results = []
+    tf32 = torch.backends.cuda.matmul.allow_tf32
+    torch.backends.cuda.matmul.allow_tf32 = False
+    try:
+        for clips in (9, 10, 40):
+            torch.manual_seed(14)
+            head = SequenceHead(16, 32, 20, device="cuda")
+            opt = torch.optim.SGD(head.parameters(), lr=0.0)
+            features, teacher = randn(g, 4, clips, 16), randn(g, 4, clips, 20)
+            features[:, :9], teacher[:, :9] = x, judged
+            value = train_step(head, loss, opt, features, loss.teacher(teacher), lengths)
+            results.append([value] + [p.grad for p in head.parameters()])
+        real = torch.arange(9, device="cuda")[None] < lengths[:, None]
+        logits = head(x, lengths=lengths)[0]
+        lq, classes = loss.teacher(judged)
+        alone = dcn.DistillTopkFunction.apply(logits[real], lq[real], classes[real], 1.5)
+        none = train_step(head, loss, opt, x, loss.teacher(judged), torch.zeros_like(lengths))
+    finally:
+        torch.backends.cuda.matmul.allow_tf32 = tf32
+    close(results[0][0], alone.mean().double(), chain=8 * ref.CHAIN)
+    for other in results[1:]:                                 # products and sums of another number of rows: another order
+        for a, b in zip(other, results[0]):
+            close(a, b.double(), chain=8 * ref.CHAIN)
+    assert float(none) == 0.0
