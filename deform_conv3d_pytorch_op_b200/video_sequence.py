@@ -74,8 +74,8 @@ class SequenceHead(nn.Module):
 
     @torch.no_grad()
     def answer(self, logits, top=5):
-        """(classes [..., top], their probabilities, entropy) of logits."""
-        _, entropy, best, classes = TokenScoresFunction.apply(logits, None, top)
+        """(classes [..., top], their probabilities, entropy) of logits; all classes where there are fewer."""
+        _, entropy, best, classes = TokenScoresFunction.apply(logits, None, min(top, logits.size(-1)))
         return classes, best.exp(), entropy
 
 

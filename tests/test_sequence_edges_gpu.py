@@ -333,3 +333,13 @@ def test_padding_does_not_change_a_training_step():
         for a, b in zip(other, results[0]):
             close(a, b.double(), chain=8 * ref.CHAIN)
     assert float(none) == 0.0
+
+
+def test_answers_of_few_classes():
+    from deform_conv3d_pytorch_op_b200.video_sequence import SequenceHead
+    head = SequenceHead(8, 16, 3, device="cuda")
+    logits = randn(gen(15), 2, 4, 3)
+    classes, p, entropy = head.answer(logits)
+    assert classes.shape == p.shape == (2, 4, 3) and entropy.shape == (2, 4)
+    assert torch.equal(classes, logits.sort(-1, descending=True, stable=True).indices)
+    assert head.answer(logits, top=2)[0].shape == (2, 4, 2)
