@@ -341,5 +341,5 @@ def test_answers_of_few_classes():
     logits = randn(gen(15), 2, 4, 3)
     classes, p, entropy = head.answer(logits)
     assert classes.shape == p.shape == (2, 4, 3) and entropy.shape == (2, 4)
-    assert torch.equal(classes, logits.sort(-1, descending=True, stable=True).indices)
+    assert torch.equal(classes, logits.sort(dim=-1, descending=True, stable=True).indices)
     assert head.answer(logits, top=2)[0].shape == (2, 4, 2)
