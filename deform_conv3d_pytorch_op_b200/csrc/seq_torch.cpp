@@ -89,6 +89,15 @@ Tensor whole_numbers(const Tensor& t, const char* name) {
     return t.to(at::kLong).contiguous();
 }
 
+// Its own values in memory, not those of which it is the negative (the imaginary part of a conjugate)
+Tensor in_memory(Tensor t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+
+variable_list in_memory(const variable_list& v) {
+    variable_list r;
+    for (const Tensor& t : v) r.push_back(in_memory(t));
+    return r;
+}
+
 // The last axis dense; any strides over the others
 Tensor dense_last(const Tensor& t) {
     return !t.defined() || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
@@ -394,7 +403,7 @@ struct SequenceBackward : public Node {
             variable_list kept;
             for (auto& v : saved) kept.push_back(v.unpack(self));
             at::NoGradGuard no_grad;
-            by_slot = op->backward(numbers, kept, grads, want);
+            by_slot = op->backward(numbers, kept, in_memory(grads), want);
         } catch (const DcnFailure& e) {
             pybind11::gil_scoped_acquire gil;
             PyErr_SetString(g_error, e.text.c_str());
@@ -514,7 +523,7 @@ Numbers numbers_of(const Operator& op, PyObject* const* a, Py_ssize_t n, variabl
     auto tensors = [&](std::initializer_list<const char*> names, int required) {
         int i = 0;
         for (const char* name : names) {
-            in.push_back(i < n ? tensor_arg(a[i], name, i >= required) : Tensor());
+            in.push_back(i < n ? in_memory(tensor_arg(a[i], name, i >= required)) : Tensor());
             ++i;
         }
     };
@@ -605,7 +614,7 @@ PyObject* backward(PyObject*, PyObject* const* a, Py_ssize_t n) {
         {
             pybind11::gil_scoped_release no_gil;
             at::NoGradGuard no_grad;
-            out = op->backward(m, kept, grads, want);
+            out = op->backward(m, kept, in_memory(grads), want);
         }
         return wrap(std::move(out), false);
     });
@@ -616,8 +625,8 @@ template <bool kInner>
 PyObject* scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         count_arg(n, 3, 4);
-        const Tensor x0 = tensor_arg(a[0], "x"), gate0 = tensor_arg(a[1], "gate"), state = tensor_arg(a[2], "state");
-        const Tensor slots0 = n > 3 ? tensor_arg(a[3], "slots", true) : Tensor();
+        const Tensor x0 = in_memory(tensor_arg(a[0], "x")), gate0 = in_memory(tensor_arg(a[1], "gate"));
+        const Tensor state = tensor_arg(a[2], "state"), slots0 = n > 3 ? in_memory(tensor_arg(a[3], "slots", true)) : Tensor();
         if (at::GradMode::is_enabled() && (x0.requires_grad() || gate0.requires_grad() || state.requires_grad()))
             fail("step has no gradient: call it under torch.no_grad(), or take apply");
         for (const Tensor& t : {x0, gate0, state})               // (before the state advances)
@@ -634,7 +643,7 @@ PyObject* scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         typed(gate0, "gate", x0.scalar_type(), "x");
         shaped(gate0, "gate", x0.sizes());
         typed(state, "state", at::kFloat);
-        if (state.dim() != 2 || state.size(1) != x0.size(1) || !state.is_contiguous())
+        if (state.dim() != 2 || state.size(1) != x0.size(1) || !state.is_contiguous() || state.is_neg())
             fail("state has shape " + shape_text(state.sizes()) + ", expected a contiguous (pool, " + std::to_string(x0.size(1)) + ")");
         shaped(slots0, "slots", {x0.size(0)});
         if (!slots0.defined() && state.size(0) < x0.size(0)) fail("state has fewer rows than x, and no slots are given");

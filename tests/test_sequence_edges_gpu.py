@@ -343,3 +343,40 @@ def test_answers_of_few_classes():
     assert classes.shape == p.shape == (2, 4, 3) and entropy.shape == (2, 4)
     assert torch.equal(classes, logits.sort(dim=-1, descending=True, stable=True).indices)
     assert head.answer(logits, top=2)[0].shape == (2, 4, 2)
+
+
+# ---- views and callers --------------------------------------------------------------------------------------------------------
+def _negated(t):
+    """-t as a view whose memory holds t, as the imaginary part of a conjugate is"""
+    v = torch._neg_view(t)
+    assert v.is_neg() and v.stride(-1) == 1 and torch.equal(v, -t)
+    return v
+
+
+def test_negated_views():
+    g = gen(16)
+    x, gate, state = randn(g, 2, 30, 24), randn(g, 2, 30, 24), randn(g, 2, 24)
+    logits, tokens = randn(g, 3, 700), torch.tensor([1, 2, 3], device="cuda")
+    teacher = randn(g, 3, 700)
+    best, places = teacher.topk(5)
+    lq = best - teacher.logsumexp(-1, keepdim=True)
+    weight = randn(g, 24)
+    for fn, args in ((lambda a, b, c: dcn.GatedScanFunction.apply(a, b, c), (x, gate, state)),
+                     (lambda a, b, c: dcn.ResidualNormFunction.apply(a, b, None, None, None, c), (x, gate, weight)),
+                     (lambda a: dcn.TokenScoresFunction.apply(a, tokens, 3)[:3], (logits,)),
+                     (lambda a: (dcn.DistillTopkFunction.apply(a, lq, places),), (logits,)),
+                     (lambda a: (dcn.DistillTopkFunction.apply(logits, a, places),), (lq,))):
+        wanted = [(-a).requires_grad_(a is not lq) for a in args]
+        given = [_negated(a).detach().requires_grad_(a is not lq) for a in args]
+        want, got = fn(*wanted), fn(*given)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        if args[0] is lq:
+            continue
+        gouts = [randn(g, *o.shape) for o in want]
+        for a, b in zip(torch.autograd.grad(got, given, [_negated(v) for v in gouts]), torch.autograd.grad(want, wanted, [-v for v in gouts])):
+            assert torch.equal(a, b)
+    pool, same = state.clone(), state.clone()
+    assert torch.equal(dcn.GatedScanFunction.step(_negated(x[:, 0]), _negated(gate[:, 0]), pool),
+                       dcn.GatedScanFunction.step(-x[:, 0], -gate[:, 0], same)) and torch.equal(pool, same)
+    with pytest.raises(dcn.DcnError, match="state"):
+        dcn.GatedScanFunction.step(x[:, 0], gate[:, 0], _negated(state))
