@@ -380,3 +380,24 @@ def test_negated_views():
                        dcn.GatedScanFunction.step(-x[:, 0], -gate[:, 0], same)) and torch.equal(pool, same)
     with pytest.raises(dcn.DcnError, match="state"):
         dcn.GatedScanFunction.step(x[:, 0], gate[:, 0], _negated(state))
+
+
+def test_compiled_callers_keep_the_operators():
+    g = gen(17)
+    x, gate, state = randn(g, 2, 30, 24), randn(g, 2, 30, 24), randn(g, 2, 24)
+    logits, tokens = randn(g, 3, 700), torch.tensor([1, 2, 3], device="cuda")
+    lq, places = torch.full((3, 4), -2.0, device="cuda"), torch.arange(4, device="cuda").expand(3, 4).contiguous()
+    for fn, args in ((lambda a, b, c: dcn.GatedScanFunction.apply(a * 2, b, c)[0].relu(), (x, gate, state)),
+                     (lambda a, b: dcn.ResidualNormFunction.apply(a * 2, b)[1].relu(), (x, gate)),
+                     (lambda a: sum(o.sum() for o in dcn.TokenScoresFunction.apply(a * 2, tokens, 3)[:3]), (logits,)),
+                     (lambda a: dcn.DistillTopkFunction.apply(a * 2, lq, places).relu(), (logits,))):
+        args = [a.clone().requires_grad_() for a in args]
+        y, want = torch.compile(fn, backend="aot_eager")(*args), fn(*args)
+        assert torch.allclose(y, want, rtol=1e-6, atol=1e-6)
+        for a, b in zip(torch.autograd.grad(y.sum(), args), torch.autograd.grad(want.sum(), args)):
+            assert torch.allclose(a, b, rtol=1e-5, atol=1e-6)
+    pool, same = state.clone(), state.clone()
+    stepped = torch.compile(lambda a, b, p: dcn.GatedScanFunction.step(a * 2, b, p) + 1, backend="aot_eager")
+    for i in range(3):
+        want = dcn.GatedScanFunction.step(x[:, i] * 2, gate[:, i], same) + 1
+        assert torch.equal(stepped(x[:, i], gate[:, i], pool), want) and torch.equal(pool, same)
