@@ -90,7 +90,10 @@ Tensor whole_numbers(const Tensor& t, const char* name) {
 }
 
 // Its own values in memory, not those of which it is the negative (the imaginary part of a conjugate)
-Tensor in_memory(Tensor t) { return t.defined() && t.is_neg() ? t.resolve_neg() : t; }
+Tensor in_memory(Tensor t) {
+    if (t.defined() && t.is_neg()) return t.resolve_neg();
+    return t;
+}
 
 variable_list in_memory(const variable_list& v) {
     variable_list r;
@@ -468,12 +471,17 @@ variable_list call(const Operator& op, const Numbers& n, const variable_list& in
     return out;
 }
 
+bool inside_transform() {
+    return torch::jit::tracer::isTracing() ||
+           c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode);
+}
+
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+
 bool transformed(const variable_list& in) {
-    if (torch::jit::tracer::isTracing() ||
-        c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode))
-        return true;
+    if (inside_transform()) return true;
     for (const Tensor& v : in)
-        if (v.defined() && torch::autograd::isFwGradDefined(v)) return true;
+        if (has_tangent(v)) return true;
     return false;
 }
 
@@ -629,9 +637,9 @@ PyObject* scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
         const Tensor state = tensor_arg(a[2], "state"), slots0 = n > 3 ? in_memory(tensor_arg(a[3], "slots", true)) : Tensor();
         if (at::GradMode::is_enabled() && (x0.requires_grad() || gate0.requires_grad() || state.requires_grad()))
             fail("step has no gradient: call it under torch.no_grad(), or take apply");
-        for (const Tensor& t : {x0, gate0, state})               // (before the state advances)
-            if (torch::autograd::isFwGradDefined(t)) fail("step has no derivative: take apply");
-        if (!kInner && transformed({x0, gate0, state, slots0})) Py_RETURN_NOTIMPLEMENTED;
+        if (has_tangent(x0) || has_tangent(gate0) || has_tangent(state))         // (before the state advances)
+            fail("step has no derivative: take apply");
+        if (!kInner && inside_transform()) Py_RETURN_NOTIMPLEMENTED;
         pybind11::gil_scoped_release no_gil;
         at::NoGradGuard no_grad;
         on_gpu(x0, "x");
