@@ -113,6 +113,24 @@ def test_distill_of_rows_with_large_finite_values(kind, value, tail):
                 close(got[r], grad[r], (v, temperature, r), scale=1e-3)
 
 
+@pytest.mark.parametrize("temperature", [1.0, 1e-3])
+def test_scores_of_float16_rows_at_the_ends_of_their_range(temperature):
+    for v in (301, 1500, 70001):
+        g = gen(v)
+        logits = _masked_rows(g, v, -6e4, torch.float16).requires_grad_()
+        w, tokens = wide(logits), torch.tensor([0, v - 1, v // 2] * 3, device="cuda")
+        outs = dcn.TokenScoresFunction.apply(logits, tokens, 5, temperature)
+        wants = ref.token_scores(w, tokens, 5, temperature)
+        gouts = [randn(g, 9), randn(g, 9), randn(g, 9, 5)]
+        (got,) = torch.autograd.grad(outs[:3], logits, [a * temperature for a in gouts])
+        (want,) = torch.autograd.grad(wants[:3], w, [a.double() * temperature for a in gouts])
+        for r in range(9):
+            for a, b in zip(outs[:3], wants):
+                close(a[r], b[r], (v, r), scale=1.0)
+            assert torch.equal(outs[3][r], wants[3][r])
+            close(got[r], want[r], (v, r), scale=1e-3)
+
+
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("value", [-1e29, -1e30, -1e36, -3e38])
 @pytest.mark.parametrize("v", [301, 70001])
