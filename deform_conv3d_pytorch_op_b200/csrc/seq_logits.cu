@@ -649,9 +649,10 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, in
     if (p.tail && rest.m != kNone) q_rest = fmaxf(1.0f - mass, 0.0f);
     if (mass != mass) q_rest = mass;
     if (rest.m != kNone) {
-        const float plain = (rest.m - m) / p.temperature;      // as in log_p, and where `to` would be cut off
-        const float log_rest =
-            (fabsf(plain) > 0.5f * kFar ? plain : kLn2 * Shift(rest.m, p.k).to(Shift(m, p.k))) + kLn2 * (rest_log_s - log_s);
+        const float apart = Shift(rest.m, p.k).to(Shift(m, p.k));
+        float log_rest = kLn2 * apart;
+        if (!(apart > -0.5f * kFar)) log_rest = (rest.m - m) / p.temperature;    // (rarely: as in log_p, where `to` is cut off)
+        log_rest += kLn2 * (rest_log_s - log_s);
         loss += product_or_zero(q_rest, logf(q_rest) - log_rest);
         c = fmaf(mass + q_rest, expf(log_rest), -q_rest);
     }
