@@ -23,7 +23,7 @@ namespace seq {
 namespace {
 
 constexpr int kThreads = 256;                    // of a CTA that has a row, or a part of one
-// of one that has a short row and up to 32 alternatives of it; up to 64: twice as many (4096x1000 bf16, 50 best 36 us, by 256 70 us)
+// of one that has a short row and up to 32 alternatives of it; up to 64: twice as many (4096x1000 bf16, 50 best 37 us, by 256 70 us)
 constexpr int kFewThreads = 64;
 constexpr int kWarpRows = 4;                     // rows of a CTA whose warps have one each
 constexpr int kCluster = 8;

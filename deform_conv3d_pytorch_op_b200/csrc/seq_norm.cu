@@ -21,7 +21,10 @@
 //     32768 x 2047 bf16    248 us                    574 us      pairs that lie across the tensor's 4 bytes (392 and 887 us
 //                                                                when elements were loaded and stored one by one)
 //     16384 x 2046 float32 125 us                    205 us      on 8 bytes (by 4, at 2047: 174 and 286 us)
-//     4096 x 8192 float32  141 us (4.8 TB/s, 73 %)   350 us (3.1 TB/s, 47 %)     rows too long to be held twice: nothing ahead
+//     10080 x 2112 bf16     84 us (33 of a copy)     141 us (52)  132 of a row's 256 threads have elements, all issue
+//     21289 x 2145 bf16    346 us (70)               780 us (112) the same, and odd rows
+//     4096 x 8192 float32  140 us (4.8 TB/s, 74 %)   334 us (3.2 TB/s, 49 %)     above 4096 channels rows are too long to be held
+//                                                                twice, nothing is ahead, and the backward pass spills registers
 //     65536 x 64 bf16       10 us (4.0 TB/s)          22 us (3.1 TB/s)           in L2; eight rows to a warp
 #include <algorithm>
 

@@ -14,10 +14,13 @@
 // addresses allow it, and no address arithmetic in the recurrence.
 //
 // What bounds it depends on how many sequences there are.  Measured, bf16, against a copy of the same bytes at 6.5 TB/s:
-//     64 x 1024 x 2048 (2048 units, one CTA each)   forward 138 us (5.8 TB/s, 90 %)   backward 253 us (5.3 TB/s, 81 %): DRAM
-//     2 x 16384 x 2048 (64 units in clusters)       forward  98 us (4.2 TB/s, 64 %)   backward 148 us (4.6 TB/s, 70 %)
+//     64 x 1024 x 2048 (2048 units, one CTA each)   forward 140 us (5.8 TB/s, 88 %)   backward 254 us (5.3 TB/s, 81 %): DRAM
+//     2 x 16384 x 2048 (64 units in clusters)       forward 101 us (4.0 TB/s, 61 %)   backward 150 us (4.5 TB/s, 69 %)
 // Few long sequences walk few clusters through many waves, and in each wave's exchange of maps its warps have nothing but copies
-// under way: latency, with DRAM 44 % busy and 53 % of the issue slots taken in the forward pass.
+// under way: latency, with DRAM 43 % busy and 53 % of the issue slots taken in the forward pass.  Sequences of fewer than 64 steps
+// are far from a copy (56 x 9 x 3776 fp16: 18 and 26 us, 2 and 3 at a copy's rate): a CTA takes the shared memory of 64 steps however
+// many it has, and a last wave that is not whole is copied with its guards.  A tile of 64 channels that a width does not fill costs
+// what a full one does (38 x 6862 x 257 fp16: 234 and 416 us, 62 and 103 at a copy's rate; the narrow rows' 4-byte copies are in it).
 //
 // A state that lasts 10^4 steps has gates within 10^-4 of one, and what matters of them is 1 - a: the rounding of a alone would
 // cost it three digits.  So the product over a thread's steps is also formed as 1 - A = sum (1 - a_t) a_1 .. a_{t-1}, of which no
@@ -664,7 +667,8 @@ __global__ void __launch_bounds__(32 * (kChunk / K), K == 16 ? 4 : 2) scan_backw
 
 // One step of each row's state, in place: W channels a thread, and as many threads as there are channels, for the fewest dependent
 // loads: gate and x, the slot, the state.  A call of 16 x 512 float32 takes 1.8 us on the GPU, most of it launch and two trips to
-// memory, and 4.6 us from call to call, which is the host's share.
+// memory, and 4.9 us from call to call, which is the host's share.  Widths that four do not divide take one channel a thread: 1555 x
+// 1286 bf16 12.3 us, 4.3 at a copy's rate.
 template <typename T, int W>
 __global__ void __launch_bounds__(128)
     scan_step_kernel(int64_t rows, int64_t channels, const T* x, int64_t x_row, const T* gate, int64_t gate_row, float* state,

@@ -115,7 +115,8 @@ class ResidualNormFunction:
 
 
 class TokenScoresFunction:
-    """Scores of rows of logits [..., vocabulary], ``log p = log_softmax(logits / temperature)``."""
+    """Scores of rows of logits [..., vocabulary], ``log p = log_softmax(logits / temperature)``.  Logits may be any finite values
+    (masks of -1e9 or of the type's lowest value among them) and -inf."""
 
     @staticmethod
     def apply(logits, tokens=None, top=0, temperature=1.0, ignore_index=-100):
@@ -138,8 +139,9 @@ class DistillTopkFunction:
 
         ``teacher_logprobs``, ``teacher_tokens`` [..., k], k up to 128: log-probabilities at this temperature and their tokens, as
         :class:`TokenScoresFunction` gives them for a teacher's logits.  ``tail``: all other tokens together are one more
-        outcome, with the teacher's remaining probability; otherwise the teacher's are renormalised over the k tokens.  A token
-        outside the vocabulary (-1) marks an unused place; a row without any has loss 0.  Gradient: logits."""
+        outcome, with the teacher's remaining probability; it is left out where the student has masked all of them (-inf).  Without
+        ``tail`` the teacher's are renormalised over the k tokens.  A token outside the vocabulary (-1) marks an unused place; a row
+        without any has loss 0.  Gradient: logits."""
         args = (logits, teacher_logprobs, teacher_tokens, temperature, tail)
         out = _lib.native().distill_topk(*args)
         return _DistillTopkFunction.apply(*args) if out is NotImplemented else out

@@ -30,7 +30,7 @@ enum { DCN_SEQ_F32 = 0, DCN_SEQ_BF16 = 1, DCN_SEQ_F16 = 2 };
  * ------------------------------------------------------------------------------------------- */
 typedef struct dcn_scan {
     int32_t dtype;                              /* x, gate, y, dy, dx, dgate */
-    int64_t batch, steps, channels;             /* any may be 0; batch * ceil(channels / 32) < 2^27 */
+    int64_t batch, steps, channels;             /* any may be 0; batch * ceil(channels / 64) < 2^27 */
     int64_t x_batch, x_step;                    /* strides of x over batch and steps */
     int64_t gate_batch, gate_step;
     int64_t dy_batch, dy_step;                  /* backward only */
@@ -116,7 +116,8 @@ int dcn_scores_backward(const dcn_logits* p, const void* logits, const int64_t* 
 
 /* loss [rows] = temperature^2 KL(teacher || student), the student's p against the teacher's q over its k best tokens:
  * tail = 1: q = exp(teacher_logprobs), and all other tokens together are one more outcome, of q_rest = max(0, 1 - sum q); it is
- *           left out where the student has no mass there;
+ *           left out where the student has no mass there (all its other logits are -inf), however much the teacher has: 1 - sum q
+ *           is not 0 but of the size of its roundings where the teacher's tokens are all there are;
  * tail = 0: q = softmax(teacher_logprobs), over the k tokens alone.
  * teacher_logprobs are those of teacher logits / temperature, [rows, k] dense, of type teacher_dtype (float32 or dtype);
  * teacher_tokens int64 [rows, k].  A token outside [0, vocab) marks a place that is not used; a row without any has loss 0 and
