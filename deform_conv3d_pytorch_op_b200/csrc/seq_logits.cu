@@ -580,6 +580,13 @@ __device__ __forceinline__ float log_p(float v, float m, float log_s, const Logi
     return fabsf(plain) > kFar ? plain - kLn2 * log_s : kLn2 * (Shift(m, p.k)(v) - log_s);
 }
 
+// temperature times it, which float32 holds where log p is too low for it
+__device__ __forceinline__ float scaled_log_p(float v, float m, float log_s, const LogitsArgs& p) {
+    if (m == kNone) return kNone;
+    const float apart = v - m;
+    return fabsf(apart) > kFar ? fmaf(-kLn2 * p.temperature, log_s, apart) : kLn2 * p.temperature * (Shift(m, p.k)(v) - log_s);
+}
+
 __device__ __forceinline__ float product_or_zero(float p, float v) { return p > 0.0f || p != p ? p * v : 0.0f; }
 
 struct TeacherRoom {
@@ -641,7 +648,7 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, in
     for (int i = lane; i < p.places; i += 32) {
         if (r.token[i] < 0) continue;
         const float lq = r.log_q[i];
-        loss += product_or_zero(expf(lq), lq - log_p(r.logit[i], m, log_s, p));
+        loss += product_or_zero(expf(lq), fmaf(p.temperature, lq, -scaled_log_p(r.logit[i], m, log_s, p)));
     }
     loss = total(loss);
     if (lane != 0) return;
@@ -649,15 +656,15 @@ __device__ __forceinline__ void distill_row(const LogitsArgs& p, int64_t row, in
     if (p.tail && rest.m != kNone) q_rest = fmaxf(1.0f - mass, 0.0f);
     if (mass != mass) q_rest = mass;
     if (rest.m != kNone) {
-        const float apart = Shift(rest.m, p.k).to(Shift(m, p.k));
-        float log_rest = kLn2 * apart;
-        if (!(apart > -0.5f * kFar)) log_rest = (rest.m - m) / p.temperature;    // (rarely: as in log_p, where `to` is cut off)
-        log_rest += kLn2 * (rest_log_s - log_s);
-        loss += product_or_zero(q_rest, logf(q_rest) - log_rest);
-        c = fmaf(mass + q_rest, expf(log_rest), -q_rest);
+        const float apart = Shift(rest.m, p.k).to(Shift(m, p.k)), unit = kLn2 * p.temperature;
+        float log_rest = unit * apart;           // times the temperature, as the others'
+        if (!(apart > -0.5f * kFar)) log_rest = rest.m - m;                      // (rarely: where `to` is cut off)
+        log_rest = fmaf(unit, rest_log_s - log_s, log_rest);
+        loss += product_or_zero(q_rest, fmaf(p.temperature, logf(q_rest), -log_rest));
+        c = fmaf(mass + q_rest, expf(kLn2 * (apart + (rest_log_s - log_s))), -q_rest);
     }
     if (!used) loss = c = mass = q_rest = 0.0f;
-    p.loss[row] = loss * p.temperature * p.temperature;
+    p.loss[row] = loss * p.temperature;
     if (p.stats != nullptr) {
         float* s = p.stats + row * DCN_LOGITS_STATS;
         s[kM] = m, s[kLogS] = log_s, s[kRestM] = rest.m, s[kRestLogS] = rest_log_s;

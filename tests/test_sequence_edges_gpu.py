@@ -151,6 +151,30 @@ def test_distill_with_all_other_tokens_masked_by_the_lowest_values(kind, value, 
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("tail", [True, False])
+@pytest.mark.parametrize("temperature", [0.5, 0.05])
+def test_distill_at_low_temperatures_beside_the_lowest_values(kind, tail, temperature):
+    """temperature^2 KL is a number where log p itself, the lowest value over the temperature, is beyond float32."""
+    for v, k in ((301, 7), (5003, 40)):
+        g, t = gen(v), TYPES[kind]
+        teacher = randn(g, 3, v, std=2.0)
+        best, tokens = teacher.topk(k)
+        lq = best - teacher.logsumexp(-1, keepdim=True)
+        logits = randn(g, 3, v, dtype=t)
+        logits[0, tokens[0, k // 2]] = torch.finfo(t).min     # one of the teacher's, all of the others, half of everything
+        logits[1] = torch.full_like(logits[1], torch.finfo(t).min).scatter_(0, tokens[1], logits[1, tokens[1]])
+        logits[2, v // 2:] = torch.finfo(t).min
+        logits.requires_grad_()
+        loss = dcn.DistillTopkFunction.apply(logits, lq, tokens, temperature, tail)
+        go = randn(g, 3)
+        (a,) = torch.autograd.grad(loss, logits, go)
+        want, b = _distill_by_formula(logits, lq, tokens, go, temperature, tail)
+        for r in range(3):
+            close(loss[r], want[r], (v, r), scale=1.0)
+            close(a[r], b[r], (v, r), scale=1e-3)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("dentropy,temperature", [(1.0, 1.0), (1e9, 1.0), (3e6, 1e-3), (-1e20, 2.0)])
 def test_entropy_gradients_of_any_size_beside_masked_tokens(kind, dentropy, temperature):
     """p log p of a token that cannot come is 0 whatever it is multiplied with (loss scaling, low temperatures)."""
