@@ -13,14 +13,15 @@ from .modules import (Conv2d, Conv3d, ConvOffset2d, ConvOffset3d, DeformConv2d, 
                       DeformLayer3d, LegacyConvOffset2d)
 from .legacy_ops import conv2d_op, deform_conv2d_double_op, deform_conv2d_op, deform_conv3d_op
 from .ops import Op, check_status
-from .sequence import (DistillTopkFunction, GatedScan, GatedScanFunction, ResidualNorm, ResidualNormFunction,
-                       TokenScoresFunction, TopkDistillLoss)
+from .sequence import (DecayAttentionFunction, DistillTopkFunction, GatedScan, GatedScanFunction, GroupNormActFunction, ResidualNorm,
+                       ResidualNormFunction, TokenSampleFunction, TokenScoresFunction, TopkDistillLoss)
 
 __all__ = [
     "DcnError", "LIB_PATH", "Op", "check_status",
     "ConvOffset3dFunction", "ConvOffset2dFunction", "Conv2dFunction", "Conv3dFunction", "DeformLayerFunction", "LegacyConvOffset2dFunction",
     "ConvOffset3d", "ConvOffset2d", "Conv2d", "Conv3d", "DeformConv3d", "DeformConv2d", "DeformLayer3d", "DeformLayer2d", "LegacyConvOffset2d",
     "GatedScanFunction", "ResidualNormFunction", "TokenScoresFunction", "DistillTopkFunction",
+    "DecayAttentionFunction", "GroupNormActFunction", "TokenSampleFunction",
     "GatedScan", "ResidualNorm", "TopkDistillLoss",
     "deform_conv3d_op", "deform_conv2d_op", "deform_conv2d_double_op", "conv2d_op",
 ]

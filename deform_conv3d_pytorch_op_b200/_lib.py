@@ -51,6 +51,24 @@ class dcn_logits(ctypes.Structure):
                 ("temperature", ctypes.c_float)]
 
 
+class dcn_attn(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32)] + [(n, ctypes.c_int64) for n in (
+        "batch", "steps", "heads", "kv_heads", "dk", "dv", "q_batch", "q_step", "q_head", "k_batch", "k_step", "k_head",
+        "v_batch", "v_step", "v_head", "dout_batch", "dout_step", "dout_head")] + [("scale", ctypes.c_float)]
+
+
+class dcn_gnorm(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "weight_dtype", "act")] + [(n, ctypes.c_int64) for n in (
+        "samples", "positions", "channels", "groups")] + [("eps", ctypes.c_float)]
+
+
+class dcn_sample(ctypes.Structure):
+    _fields_ = [("dtype", ctypes.c_int32), ("rows", ctypes.c_int64), ("vocab", ctypes.c_int64), ("row_stride", ctypes.c_int64),
+                ("temperature", ctypes.c_float), ("top_p", ctypes.c_float), ("min_p", ctypes.c_float), ("top_k", ctypes.c_int64),
+                ("temperatures", ctypes.c_void_p), ("top_ps", ctypes.c_void_p), ("min_ps", ctypes.c_void_p),
+                ("top_ks", ctypes.c_void_p)]
+
+
 _lib: Optional[ctypes.CDLL] = None
 
 # every symbol include/dcn.h declares (checked by the CPU test-suite)
@@ -75,6 +93,9 @@ SEQUENCE_SYMBOLS = [
     "dcn_scan_checkpoint_bytes", "dcn_scan_forward", "dcn_scan_backward", "dcn_scan_step",
     "dcn_norm_forward", "dcn_norm_workspace_bytes", "dcn_norm_backward",
     "dcn_scores_forward", "dcn_scores_backward", "dcn_distill_forward", "dcn_distill_backward",
+    "dcn_attn_workspace_bytes", "dcn_attn_forward", "dcn_attn_backward", "dcn_attn_step",
+    "dcn_gnorm_workspace_bytes", "dcn_gnorm_forward", "dcn_gnorm_backward",
+    "dcn_sample_workspace_bytes", "dcn_sample_tokens",
 ]
 
 
@@ -130,6 +151,18 @@ def lib() -> ctypes.CDLL:
         L.dcn_scores_backward.argtypes = [lo, vp, vp, i64, i32] + [vp] * 7
         L.dcn_distill_forward.argtypes = [lo, vp, i32, vp, i32, vp, i32, vp, vp, vp]
         L.dcn_distill_backward.argtypes = [lo, vp, i32, vp, i32, vp, i32, vp, vp, vp, vp]
+        at, gn, sa = map(ctypes.POINTER, (dcn_attn, dcn_gnorm, dcn_sample))
+        for f in (L.dcn_attn_workspace_bytes, L.dcn_gnorm_workspace_bytes, L.dcn_sample_workspace_bytes):
+            f.restype = ctypes.c_size_t
+        L.dcn_attn_workspace_bytes.argtypes = [at, i32]
+        L.dcn_attn_forward.argtypes = [at] + [vp] * 9 + [ctypes.c_size_t, vp]
+        L.dcn_attn_backward.argtypes = [at] + [vp] * 13 + [ctypes.c_size_t, vp]
+        L.dcn_attn_step.argtypes = [at] + [vp] * 5 + [i64] + [vp] * 3
+        L.dcn_gnorm_workspace_bytes.argtypes = [gn, i32]
+        L.dcn_gnorm_forward.argtypes = [gn] + [vp] * 7 + [ctypes.c_size_t, vp]
+        L.dcn_gnorm_backward.argtypes = [gn] + [vp] * 11 + [ctypes.c_size_t, vp]
+        L.dcn_sample_workspace_bytes.argtypes = [sa]
+        L.dcn_sample_tokens.argtypes = [sa] + [vp] * 5 + [ctypes.c_size_t, vp]
         _lib = L
     return _lib
 

@@ -15,7 +15,8 @@ CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB = os.path.join(CSRC, "libdcn.so")
 BINDING = os.path.join(os.path.dirname(CSRC), "_dcn_torch.so")
 BINDING_SOURCES = [os.path.join(CSRC, f) for f in ("dcn_torch.cpp", "seq_torch.cpp")]
-SOURCES = ["dcn_api.cu", "dcn_simt.cu", "dcn_exact.cu", "dcn_tc.cu", "seq_scan.cu", "seq_norm.cu", "seq_logits.cu"]
+SOURCES = ["dcn_api.cu", "dcn_simt.cu", "dcn_exact.cu", "dcn_tc.cu", "seq_scan.cu", "seq_norm.cu", "seq_logits.cu", "seq_attn.cu", "seq_gnorm.cu",
+           "seq_sample.cu"]
 HEADERS = ["dcn_common.cuh", "dcn_internal.h"] + [os.path.join("..", "..", "include", h) for h in ("dcn.h", "dcn_seq.h")]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"] + os.environ.get("DCN_NVCC_EXTRA", "").split()

@@ -1,0 +1,873 @@
+// Decayed linear attention over time, for each head with its decay g:
+//     S_t = g S_{t-1} + k_t v_t^T,    out_t = scale S_t^T q_t
+// In chunks of 64 steps, with X the state before a chunk and i, j steps of it,
+//     out_i = scale (sum_{j <= i} g^(i-j) (q_i . k_j) v_j  +  g^(i+1) X^T q_i),     X' = g^64 X + sum_j g^(63-j) k_j v_j^T
+// One kernel runs through (a, b, c) = (q, k, v) in this way.  The gradients are the same sums over other operands:
+//     dq: (dout, v, k) with the states S^T;   back in time, with R_t = g R_{t+1} + scale q_t dout_t^T the gradient of S_t,
+//     dk: (v, dout, q) with R^T;   dv: (k, q, dout) with R;   R starts as dlast with one power of g less: g^i X and g^(64-j).
+//
+// A CTA of four warps walks one sequence's chunks for one head and 64 columns of c, the state in the accumulators of its warps (a
+// quarter of a's columns each).  A warp has 16 steps of the chunk: their scores become the operand of the product with c in
+// registers; the state meets a as a rounded copy in shared memory.  The next chunk's tiles are on their way (cp.async) meanwhile.
+// Where there are fewer heads than the GPU holds CTAs, the time axis is split: a first launch sums each part's k_t v_t^T, and
+// a CTA of the second folds what lies before its own part.
+#include <algorithm>
+#include <cmath>
+
+#include "seq_common.cuh"
+
+namespace dcn {
+namespace seq {
+namespace {
+
+constexpr int kChunk = 64, kCols = 64, kThreads = 128, kMostWidth = 128, kMostParts = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Strides {
+    int64_t batch, step, head;
+};
+
+struct Operand {
+    const void* p;
+    Strides s;
+    int share;                                   // heads that read the same one
+    int width, bytes;                            // elements of a row; bytes that are copied at once
+};
+
+struct Job {
+    Operand a, b, c;
+    void* out;                                   // [batch, steps, heads, c.width], dense; float32 where wide
+    const float* init;                           // [batch, heads, ...]: element (i, j) at i * init_i + j * init_j; NULL: zeros
+    float* end;                                  // [batch, heads, a.width, c.width] dense, or NULL
+    int init_i, init_j;
+    int reverse, wide;
+    float init_scale, end_scale;
+    int pairs;                                   // out's rows start on two elements
+};
+
+struct AttnArgs {
+    Job job[3];
+    const float* log_decay;
+    const int64_t* lengths;
+    float* parts;                                // [job][batch * heads][part][a.width][c.width]
+    int64_t steps, part_steps;
+    int batch, heads, jobs, tiles, n_parts;      // tiles: of 64 columns, the most that a job has
+    int tile_of[3];
+    float scale;
+};
+
+__device__ __forceinline__ float log2_decay(const float* log_decay, int h) {
+    float g;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(g) : "l"(log_decay + h));
+    g = g > 0.0f ? 0.0f : g;
+    return fmaxf(g * kLog2e, -1e4f) + (g != g ? g : 0.0f);     // (finite, so that 0 steps are a factor of 1)
+}
+__device__ __forceinline__ float power(float lg, int n) { return ex2(lg * (float)n); }
+
+// ---- products: D[16 x 8] += A[16 x k] B[k x 8], k = 16 for 16-bit types and 8 for float32 -----------------------------------------
+// Operands come from tiles in shared memory, rows of `a` columns.  16-bit tiles are swizzled by 16 bytes (the row's low three bits);
+// float32 tiles have 8 columns more than they need, and the elements 2t and 2t + 1 of k stand for the instruction's t and t + 4.
+template <typename T>
+struct Tile {
+    static constexpr int kK = 16;
+    static constexpr int row_elems(int cols) { return cols; }
+    // address of 16 bytes
+    static __device__ __forceinline__ uint32_t at(uint32_t base, int row, int col, int cols) {
+        return base + row * cols * 2 + (((col >> 3) ^ (row & 7)) << 4) + (col & 7) * 2;
+    }
+};
+template <>
+struct Tile<float> {
+    static constexpr int kK = 8;
+    static constexpr int row_elems(int cols) { return cols + 8; }
+    static __device__ __forceinline__ uint32_t at(uint32_t base, int row, int col, int cols) {
+        return base + (row * (cols + 8) + col) * 4;
+    }
+};
+
+template <typename T>
+struct FragA {
+    uint32_t v[4];
+};
+template <typename T>
+struct FragB {
+    uint32_t v[2];
+};
+// float32: each element as the sum of two of TF32 (11 bits each), which leaves 2^-22 of it
+template <>
+struct FragA<float> {
+    uint32_t v[4], low[4];
+};
+template <>
+struct FragB<float> {
+    uint32_t v[2], low[2];
+};
+
+__device__ __forceinline__ void split(float f, uint32_t& big, uint32_t& low) {
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(big) : "f"(f));
+    const float rest = f - __uint_as_float(big);
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(low) : "f"(rest));
+}
+
+template <typename T>
+__device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+template <typename T>
+__device__ __forceinline__ void mma(float (&d)[4], const FragA<T>& a, const FragB<T>& b) {
+    if constexpr (std::is_same<T, float>::value) {
+        mma8(d, a.low, b.v);
+        mma8(d, a.v, b.low);
+        mma8(d, a.v, b.v);
+    } else {
+        mma16<T>(d, a.v, b.v);
+    }
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ float lds_float(uint32_t a) {
+    float f;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(a) : "memory");
+    return f;
+}
+__device__ __forceinline__ float2 lds_float2(uint32_t a) {
+    float2 f;
+    asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(a) : "memory");
+    return f;
+}
+
+// A[m][k] = tile[m0 + m][k0 + k]
+template <typename T>
+__device__ __forceinline__ void load_a(FragA<T>& f, uint32_t base, int m0, int k0, int cols, int lane) {
+    if constexpr (std::is_same<T, float>::value) {
+        const int g = lane >> 2, t = lane & 3;
+        const float2 x = lds_float2(Tile<T>::at(base, m0 + g, k0 + 2 * t, cols));
+        const float2 y = lds_float2(Tile<T>::at(base, m0 + g + 8, k0 + 2 * t, cols));
+        split(x.x, f.v[0], f.low[0]), split(y.x, f.v[1], f.low[1]), split(x.y, f.v[2], f.low[2]), split(y.y, f.v[3], f.low[3]);
+    } else {
+        ldsm4(f.v, Tile<T>::at(base, m0 + (lane & 15), k0 + (lane >> 4) * 8, cols));
+    }
+}
+// two of B[k][n] = tile[n0 + n][k0 + k], for n0 and n0 + 8
+template <typename T>
+__device__ __forceinline__ void load_b(FragB<T> (&f)[2], uint32_t base, int n0, int k0, int cols, int lane) {
+    if constexpr (std::is_same<T, float>::value) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float2 x = lds_float2(Tile<T>::at(base, n0 + 8 * i + g, k0 + 2 * t, cols));
+            split(x.x, f[i].v[0], f[i].low[0]), split(x.y, f[i].v[1], f[i].low[1]);
+        }
+    } else {
+        uint32_t r[4];
+        ldsm4(r, Tile<T>::at(base, n0 + (lane >> 4) * 8 + (lane & 7), k0 + ((lane >> 3) & 1) * 8, cols));
+        f[0].v[0] = r[0], f[0].v[1] = r[1], f[1].v[0] = r[2], f[1].v[1] = r[3];
+    }
+}
+// two of B[k][n] = tile[k0 + k][n0 + n], for n0 and n0 + 8
+template <typename T>
+__device__ __forceinline__ void load_bt(FragB<T> (&f)[2], uint32_t base, int k0, int n0, int cols, int lane) {
+    if constexpr (std::is_same<T, float>::value) {
+        const int g = lane >> 2, t = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+                split(lds_float(Tile<T>::at(base, k0 + 2 * t + e, n0 + 8 * i + g, cols)), f[i].v[e], f[i].low[e]);
+    } else {
+        uint32_t r[4];
+        ldsm4t(r, Tile<T>::at(base, k0 + (lane & 15), n0 + (lane >> 4) * 8, cols));
+        f[0].v[0] = r[0], f[0].v[1] = r[1], f[1].v[0] = r[2], f[1].v[1] = r[3];
+    }
+}
+// A[m][k] = tile[k0 + k][m0 + m] * weight of row k0 + k.  16-bit: rounded, and (low) what the rounding left
+template <typename T>
+__device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, uint32_t base, int k0, int m0, int cols, int lane, float lg,
+                                        int last_power, int rows) {
+    const int g = lane >> 2, t = lane & 3;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int j = k0 + 2 * t + e;
+            const float w = j < rows ? power(lg, last_power - j) : 0.0f;
+            split(w * lds_float(Tile<T>::at(base, j, m0 + g, cols)), f.v[2 * e], f.low[2 * e]);
+            split(w * lds_float(Tile<T>::at(base, j, m0 + g + 8, cols)), f.v[2 * e + 1], f.low[2 * e + 1]);
+        }
+    } else {
+        uint32_t r[4];
+        // matrices: (k 0-7, m 0-7), (k 0-7, m 8-15), (k 8-15, m 0-7), (k 8-15, m 8-15), each transposed
+        ldsm4t(r, Tile<T>::at(base, k0 + (lane >> 4) * 8 + (lane & 7), m0 + ((lane >> 3) & 1) * 8, cols));
+        float w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int j = k0 + 2 * t + (e & 1) + (e >> 1) * 8;
+            w[e] = j < rows ? power(lg, last_power - j) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {            // 0: (g, k 2t), 1: (g + 8, k 2t), 2: (g, k 2t + 8), 3: (g + 8, k 2t + 8)
+            const float x = half_of<T>(r[i], 0) * w[(i >> 1) * 2], y = half_of<T>(r[i], 1) * w[(i >> 1) * 2 + 1];
+            f.v[i] = word_of<T>(x, y);
+            low.v[i] = word_of<T>(x - half_of<T>(f.v[i], 0), y - half_of<T>(f.v[i], 1));
+        }
+    }
+}
+// the scores of 16 steps as the left operand of the product over k0, k0 + 1, ...
+template <typename T, int N>
+__device__ __forceinline__ void scores_as_a(FragA<T>& f, const float (&s)[N][4], int step) {
+    if constexpr (std::is_same<T, float>::value) {
+        split(s[step][0], f.v[0], f.low[0]), split(s[step][2], f.v[1], f.low[1]);
+        split(s[step][1], f.v[2], f.low[2]), split(s[step][3], f.v[3], f.low[3]);
+    } else {
+        f.v[0] = word_of<T>(s[2 * step][0], s[2 * step][1]), f.v[1] = word_of<T>(s[2 * step][2], s[2 * step][3]);
+        f.v[2] = word_of<T>(s[2 * step + 1][0], s[2 * step + 1][1]), f.v[3] = word_of<T>(s[2 * step + 1][2], s[2 * step + 1][3]);
+    }
+}
+
+// ---- tiles ----------------------------------------------------------------------------------------------------------------
+// Rows first, first + 1, ... of a sequence (back in time from `length` where reverse) into a tile of kCols_ columns; zeros beyond the
+// length and the operand's width.
+template <typename T, int kCols_>
+__device__ __forceinline__ void load_tile(uint32_t base, const Operand& o, const char* from, int64_t first, int64_t length, int col0,
+                                          bool reverse) {
+    constexpr int kElem = sizeof(T), kVec = 16 / kElem, kPerRow = kCols_ / kVec;
+    const int width = o.width - col0;            // (may be above kCols_)
+    for (int i = threadIdx.x; i < kChunk * kPerRow; i += kThreads) {
+        const int row = i / kPerRow, col = (i % kPerRow) * kVec;
+        const int64_t pos = first + row;
+        const bool in = pos < length && col < width;
+        const int64_t t = reverse ? length - 1 - pos : pos;
+        const char* src = from + (in ? (t * o.s.step + col0 + col) * kElem : 0);
+        const uint32_t dst = Tile<T>::at(base, row, col, kCols_);
+        const int bytes = in ? min(16, (width - col) * kElem) : 0;
+        if (o.bytes == 16) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+        } else if (o.bytes == 8) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst + e), "l"(bytes > e ? src + e : from),
+                             "r"(max(0, min(8, bytes - e))) : "memory");
+        } else if (o.bytes == 4) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst + e), "l"(bytes > e ? src + e : from),
+                             "r"(max(0, min(4, bytes - e))) : "memory");
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                Raw<2> r;
+                r.u = 0;
+                if (bytes > e) load(r, src + e);
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + e), "h"(r.u) : "memory");
+            }
+        }
+    }
+}
+
+template <typename T, int KA>
+struct Shape {
+    static constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
+    static constexpr int kTileA = kChunk * Tile<T>::row_elems(KA) * (int)sizeof(T);
+    static constexpr int kTileC = kChunk * Tile<T>::row_elems(kCols) * (int)sizeof(T);
+    static constexpr int kState = KA * Tile<T>::row_elems(kCols) * (int)sizeof(T);
+    static constexpr int kStage = 2 * kTileA + kTileC;
+    static constexpr int kBytes = kStages * kStage + kState + 32;
+};
+
+// The maximum of a CTA's states, for the power of two that keeps a float16 copy of them in range
+__device__ __forceinline__ float cta_max(float v, float* slots) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(slots[0], slots[1]), fmaxf(slots[2], slots[3]));
+}
+
+// kEnds: the sums of each part's b_j c_j^T alone
+template <typename T, int KA, bool kEnds>
+__global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
+    using S = Shape<T, KA>;
+    using L = Tile<T>;
+    constexpr int kM = KA / 64;                  // 16-row tiles of the state that a warp has
+    constexpr int kN = kCols / 8;
+    constexpr int kSteps = kChunk / L::kK;
+    extern __shared__ __align__(128) char smem[];
+    const uint32_t tiles = shared_address(smem), copy = tiles + S::kStages * S::kStage;
+    float* const slots = reinterpret_cast<float*>(smem + S::kStages * S::kStage + S::kState);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+    int u = blockIdx.x;
+    const int tile = u % args.tiles;
+    u /= args.tiles;
+    const int which = u % args.jobs;
+    const int unit = u / args.jobs, h = unit % args.heads, b = unit / args.heads;
+    const Job& job = args.job[which];
+    if (tile >= args.tile_of[which]) return;
+    const int col0 = tile * kCols, part = blockIdx.y;
+    pdl_wait();
+
+    const int64_t steps = args.steps;
+    int64_t length = steps;
+    if (args.lengths != nullptr) length = min(max(gload_i64(args.lengths + b), (int64_t)0), steps);
+    const int64_t begin = (int64_t)part * args.part_steps, stop = min(begin + args.part_steps, steps);
+    const int64_t finish = min(stop, length);    // of the steps there are
+    const bool reverse = job.reverse != 0;
+    const float lg = log2_decay(args.log_decay, h);
+    const int extra = reverse ? 0 : 1;           // powers of g on the state before a chunk, at its first step
+    const int wa = job.a.width, wc = job.c.width;
+    const char* const from_a = static_cast<const char*>(job.a.p) + (b * job.a.s.batch + h / job.a.share * job.a.s.head) * (int64_t)sizeof(T);
+    const char* const from_b = static_cast<const char*>(job.b.p) + (b * job.b.s.batch + h / job.b.share * job.b.s.head) * (int64_t)sizeof(T);
+    const char* const from_c = static_cast<const char*>(job.c.p) + (b * job.c.s.batch + h / job.c.share * job.c.s.head) * (int64_t)sizeof(T);
+    auto fetch = [&](int stage, int64_t first) {
+        const uint32_t base = tiles + stage * S::kStage;
+        if constexpr (!kEnds) load_tile<T, KA>(base, job.a, from_a, first, length, 0, reverse);
+        load_tile<T, KA>(base + S::kTileA, job.b, from_b, first, length, 0, reverse);
+        load_tile<T, kCols>(base + 2 * S::kTileA, job.c, from_c, first, length, col0, reverse);
+        copies_issued();
+    };
+    if (S::kStages == 2 && begin < finish) fetch(0, begin);
+
+    // the state before this part
+    float x[kM][kN][4];
+    const int64_t parts_of = ((int64_t)which * args.batch * args.heads + unit) * args.n_parts;
+#pragma unroll
+    for (int m = 0; m < kM; ++m)
+#pragma unroll
+        for (int n = 0; n < kN; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[m][n][e] = 0.0f;
+                if constexpr (!kEnds) {
+                    const int i = (warp * kM + m) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                    if (job.init != nullptr && i < wa && j < wc)
+                        x[m][n][e] = job.init_scale * gload(job.init + (int64_t)unit * wa * wc + (int64_t)i * job.init_i + (int64_t)j * job.init_j);
+                }
+            }
+    if constexpr (!kEnds) {
+        const float whole = ex2(lg * (float)args.part_steps);
+        for (int s = 0; s < part; ++s) {
+            const float* const sums = args.parts + (parts_of + s) * wa * wc;
+            // (a part that the sequence ends in is the last one that anything reads)
+#pragma unroll
+            for (int m = 0; m < kM; ++m)
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int i = (warp * kM + m) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                        if (i < wa && j < wc && begin < length) x[m][n][e] = fmaf(x[m][n][e], whole, gload(sums + (int64_t)i * wc + j));
+                    }
+        }
+    }
+
+    float down = 1.0f, up = 1.0f;                // float16: the copy is the state times `down`
+    auto put_copy = [&]() {
+        if constexpr (std::is_same<T, __half>::value) {
+            float most = 0.0f;
+#pragma unroll
+            for (int m = 0; m < kM; ++m)
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[m][n][e]));
+            most = cta_max(most, slots);
+            const int over = max((int)(__float_as_uint(most) >> 23) - 127 - 14, 0);
+            down = __uint_as_float((uint32_t)(127 - min(over, 126)) << 23);
+            up = __uint_as_float((uint32_t)(127 + min(over, 126)) << 23);
+        }
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t at = L::at(copy, (warp * kM + m) * 16 + g + half * 8, n * 8 + 2 * t, kCols);
+                    const float p = x[m][n][2 * half], q = x[m][n][2 * half + 1];
+                    if constexpr (std::is_same<T, float>::value)
+                        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(p), "f"(q) : "memory");
+                    else
+                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(word_of<T>(p * down, q * down)) : "memory");
+                }
+    };
+    if constexpr (!kEnds) put_copy();
+
+    int stage = 0;
+    for (int64_t first = begin; first < finish; first += kChunk) {
+        const int rows = (int)min((int64_t)kChunk, finish - first);
+        if constexpr (S::kStages == 1) fetch(0, first);
+        copies_arrived<0>();
+        __syncthreads();                         // this chunk's tiles and the copy of the state are there
+        if (S::kStages == 2 && first + kChunk < finish) fetch(stage ^ 1, first + kChunk);
+        const uint32_t at = tiles + (S::kStages == 2 ? stage : 0) * S::kStage, bt = at + S::kTileA, ct = at + 2 * S::kTileA;
+        if constexpr (!kEnds) {
+            // which 16 steps a warp has goes round, so that the long rows of the triangle do not always meet the same scheduler
+            const int m0 = ((warp + blockIdx.x + (int)(first / kChunk)) & 3) * 16;
+            if (m0 < rows) {
+                float o[kN][4] = {};
+#pragma unroll 2
+                for (int k = 0; k < KA; k += L::kK) {
+                    FragA<T> fa;
+                    load_a<T>(fa, at, m0, k, KA, lane);
+#pragma unroll
+                    for (int n = 0; n < kN; n += 2) {
+                        FragB<T> fb[2];
+                        load_bt<T>(fb, copy, k, n * 8, kCols, lane);
+                        mma<T>(o[n], fa, fb[0]);
+                        mma<T>(o[n + 1], fa, fb[1]);
+                    }
+                }
+                const float w0 = power(lg, m0 + g + extra) * up, w1 = power(lg, m0 + g + 8 + extra) * up;
+#pragma unroll
+                for (int n = 0; n < kN; ++n) o[n][0] *= w0, o[n][1] *= w0, o[n][2] *= w1, o[n][3] *= w1;
+                float s[kN][4] = {};
+#pragma unroll 2
+                for (int k = 0; k < KA; k += L::kK) {
+                    FragA<T> fa;
+                    load_a<T>(fa, at, m0, k, KA, lane);
+#pragma unroll
+                    for (int n = 0; n < kN; n += 2) {
+                        if (n * 8 > m0) continue;
+                        FragB<T> fb[2];
+                        load_b<T>(fb, bt, n * 8, k, KA, lane);
+                        mma<T>(s[n], fa, fb[0]);
+                        mma<T>(s[n + 1], fa, fb[1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = m0 + g + (e >> 1) * 8 - (n * 8 + 2 * t + (e & 1));
+                        s[n][e] = d >= 0 ? s[n][e] * power(lg, d) : 0.0f;
+                    }
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    if (k * L::kK > m0 + 15) continue;
+                    FragA<T> fa;
+                    scores_as_a<T>(fa, s, k);
+#pragma unroll
+                    for (int n = 0; n < kN; n += 2) {
+                        FragB<T> fb[2];
+                        load_bt<T>(fb, ct, k * L::kK, n * 8, kCols, lane);
+                        mma<T>(o[n], fa, fb[0]);
+                        mma<T>(o[n + 1], fa, fb[1]);
+                    }
+                }
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int row = m0 + g + half * 8;
+                    if (row >= rows) continue;
+                    const int64_t pos = first + row, step = reverse ? length - 1 - pos : pos;
+                    const int64_t to = (((int64_t)b * steps + step) * args.heads + h) * wc + col0;
+#pragma unroll
+                    for (int n = 0; n < kN; ++n) {
+                        const int c = n * 8 + 2 * t;
+                        const float p = o[n][2 * half] * args.scale, q = o[n][2 * half + 1] * args.scale;
+                        const bool both = c + 1 < wc - col0, pairs = job.pairs != 0;
+                        if (c >= wc - col0) continue;
+                        if (std::is_same<T, float>::value || job.wide) {
+                            float* const d = static_cast<float*>(job.out) + to + c;
+                            if (both && pairs) *reinterpret_cast<float2*>(d) = make_float2(p, q);
+                            else {
+                                d[0] = p;
+                                if (both) d[1] = q;
+                            }
+                        } else {
+                            T* const d = static_cast<T*>(job.out) + to + c;
+                            if constexpr (!std::is_same<T, float>::value) {
+                                if (both && pairs) store(d, Raw<4>{{word_of<T>(p, q)}});
+                                else {
+                                    d[0] = from_float<T>(p);
+                                    if (both) d[1] = from_float<T>(q);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+        }
+        // the state behind this chunk
+        const float whole = power(lg, rows);
+        const int last_power = rows - extra;
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[m][n][e] *= whole;
+#pragma unroll 1
+        for (int k = 0; k < kChunk; k += L::kK) {
+            FragB<T> fb[kN / 2][2];
+#pragma unroll
+            for (int n = 0; n < kN; n += 2) load_bt<T>(fb[n / 2], ct, k, n * 8, kCols, lane);
+#pragma unroll
+            for (int m = 0; m < kM; ++m) {
+                FragA<T> fa, low;
+                load_at<T>(fa, low, bt, k, (warp * kM + m) * 16, KA, lane, lg, last_power, rows);
+#pragma unroll
+                for (int n = 0; n < kN; n += 2) {
+                    mma<T>(x[m][n], fa, fb[n / 2][0]);
+                    mma<T>(x[m][n + 1], fa, fb[n / 2][1]);
+                    if constexpr (!std::is_same<T, float>::value) {
+                        mma<T>(x[m][n], low, fb[n / 2][0]);
+                        mma<T>(x[m][n + 1], low, fb[n / 2][1]);
+                    }
+                }
+            }
+        }
+        __syncthreads();                         // every warp is done with the tiles and the copy
+        if constexpr (!kEnds) put_copy();
+        stage ^= 1;
+    }
+
+    // (the first part ends a sequence of no steps)
+    const bool ends_here = kEnds || (length > begin && length <= begin + args.part_steps) || (length == 0 && part == 0);
+    float* const to = kEnds ? args.parts + (parts_of + part) * wa * wc : job.end != nullptr ? job.end + (int64_t)unit * wa * wc : nullptr;
+    if (ends_here && to != nullptr) {
+        const float by = kEnds ? 1.0f : job.end_scale;
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int n = 0; n < kN; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int i = (warp * kM + m) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                    if (i < wa && j < wc) to[(int64_t)i * wc + j] = by * x[m][n][e];
+                }
+    }
+    if constexpr (!kEnds) {
+        // zeros behind the length
+        const int64_t from = max(begin, length);
+        const int n = min(kCols, wc - col0);
+        const int64_t count = (stop - from) * n;
+        for (int64_t i = threadIdx.x; i < count; i += kThreads) {
+            const int64_t step = from + i / n, to_ = (((int64_t)b * steps + step) * args.heads + h) * wc + col0 + i % n;
+            if (std::is_same<T, float>::value || job.wide) static_cast<float*>(job.out)[to_] = 0.0f;
+            else static_cast<T*>(job.out)[to_] = from_float<T>(0.0f);
+        }
+    }
+}
+
+// Sum of the gradients of the heads that share a key or a value
+template <typename T>
+__global__ void __launch_bounds__(256) shared_kernel(const float* from, T* to, int64_t count, int share, int width) {
+    pdl_wait();
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+        const int64_t row = i / width;
+        const float* p = from + row * share * width + i % width;
+        float sum = 0.0f;
+        for (int s = 0; s < share; ++s) sum += gload(p + (int64_t)s * width);
+        to[i] = from_float<T>(sum);
+    }
+}
+
+// ---- a single step --------------------------------------------------------------------------------------------------------
+// A CTA advances a head's state of one sequence, kW columns of dv a thread, rows of dk over the rest; it is read and written once.
+struct StepArgs {
+    const void *q, *k, *v;
+    Strides qs, ks, vs;
+    const float* log_decay;
+    float* state;
+    const int64_t* slots;
+    void* out;
+    int64_t pool;
+    int heads, share, dk, dv;
+    float scale;
+};
+
+template <typename T, int kW>
+__global__ void __launch_bounds__(kThreads) attn_step_kernel(const StepArgs a) {
+    __shared__ float key[kMostWidth], query[kMostWidth], sums[kThreads * kW];
+    pdl_wait();
+    const int h = blockIdx.x % a.heads;
+    const int64_t r = blockIdx.x / a.heads;
+    const int64_t slot = a.slots != nullptr ? gload_i64(a.slots + r) : r;
+    T* const out = static_cast<T*>(a.out) + (r * a.heads + h) * a.dv;
+    if (slot < 0 || slot >= a.pool) {
+        for (int j = threadIdx.x; j < a.dv; j += kThreads) out[j] = from_float<T>(0.0f);
+        return;
+    }
+    const int groups = (a.dv + kW - 1) / kW, sets = kThreads / groups, set = threadIdx.x / groups, j = threadIdx.x % groups * kW;
+    const T* const q = static_cast<const T*>(a.q) + r * a.qs.batch + h * a.qs.head;
+    const T* const k = static_cast<const T*>(a.k) + r * a.ks.batch + h / a.share * a.ks.head;
+    const T* const v = static_cast<const T*>(a.v) + r * a.vs.batch + h / a.share * a.vs.head;
+    const float decay = ex2(log2_decay(a.log_decay, h));
+    for (int i = threadIdx.x; i < a.dk; i += kThreads) {
+        Pack<T, 1> p;
+        p.get(k + i), key[i] = p.at(0);
+        p.get(q + i), query[i] = p.at(0) * a.scale;
+    }
+    float value[kW], sum[kW];
+#pragma unroll
+    for (int e = 0; e < kW; ++e) {
+        Pack<T, 1> p;
+        p.zero();
+        if (set < sets && j + e < a.dv) p.get(v + j + e);
+        value[e] = p.at(0), sum[e] = 0.0f;
+    }
+    __syncthreads();
+    float* const state = a.state + (slot * a.heads + h) * (int64_t)a.dk * a.dv;
+    if (set < sets) {
+#pragma unroll 8
+        for (int i = set; i < a.dk; i += sets) {
+            Pack<float, kW> s;
+            float f[kW];
+            s.get(state + (int64_t)i * a.dv + j);
+#pragma unroll
+            for (int e = 0; e < kW; ++e) {
+                f[e] = fmaf(s.at(e), decay, key[i] * value[e]);
+                sum[e] = fmaf(f[e], query[i], sum[e]);
+            }
+            s.set(f);
+            s.put(state + (int64_t)i * a.dv + j);
+        }
+#pragma unroll
+        for (int e = 0; e < kW; ++e) sums[(set * groups + threadIdx.x % groups) * kW + e] = sum[e];
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < a.dv; c += kThreads) {
+        float s = 0.0f;
+        for (int p = 0; p < sets; ++p) s += sums[p * groups * kW + c];
+        out[c] = from_float<T>(s);
+    }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------------
+int check_attn(const dcn_attn* p) {
+    if (p == nullptr) return DCN_ERR_NULL;
+    if (!known_type(p->dtype)) return DCN_ERR_UNSUPPORTED;
+    if (p->batch < 0 || p->steps < 0 || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads != 0 || p->dk < 1 || p->dv < 1)
+        return DCN_ERR_SHAPE;
+    if (!std::isfinite(p->scale) || p->scale == 0.0f || !std::isfinite(1.0f / p->scale)) return DCN_ERR_SHAPE;
+    if (p->dk > kMostWidth || p->dv > kMostWidth || p->heads > 65535 || p->steps >= 1ll << 31) return DCN_ERR_LIMIT;
+    if (p->batch >= (1ll << 27) / p->heads) return DCN_ERR_LIMIT;
+    return DCN_OK;
+}
+
+int wide_of(const dcn_attn* p, bool backward) { return (int)(backward ? std::max(p->dk, p->dv) : p->dk) > 64 ? 128 : 64; }
+
+// How many parts the time axis is split into.  Time goes in chunks of a CTA; a GPU holds `held` of them at once.  More parts fill the
+// GPU, and cost a pass over b and c for their sums (a third of a chunk's time) and the folding (about a chunk's for each part before).
+int parts_for(const dcn_attn* p, bool backward) {
+    const int64_t ct = (backward ? std::max(p->dk, p->dv) : p->dv) > 64 ? 2 : 1;
+    const int64_t units = p->batch * p->heads * ct * (backward ? 3 : 1), chunks = (p->steps + kChunk - 1) / kChunk;
+    const int64_t held = (int64_t)sm_count() * (wide_of(p, backward) == 128 || p->dtype == DCN_SEQ_F32 ? 2 : 3);
+    int best = 1;
+    double least = 1e300;
+    for (int n = 1; n <= kMostParts && n <= chunks; ++n) {
+        const int64_t each = (chunks + n - 1) / n;
+        if (n > 1 && each < 4) break;
+        if ((chunks + each - 1) / each != n) continue;
+        const double waves = (double)((units * n + held - 1) / held), sums = n > 1 ? (double)((units * (n - 1) + held - 1) / held) : 0;
+        const double time = waves * (each + 1 + 0.5 * (n - 1)) + sums * (0.4 * each + 1) + (n > 1 ? 4 : 0);
+        if (time < least * 0.97) least = time, best = n;
+    }
+    return best;
+}
+
+template <typename T, int KA, bool kEnds>
+int launch_attn(const AttnArgs& a, int parts, cudaStream_t st) {
+    constexpr int kBytes = Shape<T, KA>::kBytes;
+    if (cudaFuncSetAttribute(attn_kernel<T, KA, kEnds>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess)
+        return DCN_ERR_CUDA;
+    const dim3 grid((unsigned)((int64_t)a.batch * a.heads * a.jobs * a.tiles), (unsigned)parts);
+    return launch_dependent(attn_kernel<T, KA, kEnds>, grid, dim3(kThreads), kBytes, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
+}
+
+template <typename T, int KA>
+int run_parts(const AttnArgs& a, cudaStream_t st) {
+    if (a.n_parts > 1) {
+        const int rc = launch_attn<T, KA, true>(a, a.n_parts - 1, st);
+        if (rc != DCN_OK) return rc;
+    }
+    return launch_attn<T, KA, false>(a, a.n_parts, st);
+}
+
+template <typename T>
+int run_attn(const AttnArgs& a, int wide, cudaStream_t st) {
+    return wide == 128 ? run_parts<T, 128>(a, st) : run_parts<T, 64>(a, st);
+}
+
+int run_attn_any(const dcn_attn* p, const AttnArgs& a, bool backward, cudaStream_t st) {
+    const int wide = wide_of(p, backward);
+    return p->dtype == DCN_SEQ_F32    ? run_attn<float>(a, wide, st)
+           : p->dtype == DCN_SEQ_BF16 ? run_attn<__nv_bfloat16>(a, wide, st)
+                                      : run_attn<__half>(a, wide, st);
+}
+
+// Bytes that every row of an operand starts on, as cp.async takes them (2: element by element)
+Operand operand(const dcn_attn* p, const void* at, int64_t batch, int64_t step, int64_t head, int64_t width, int share) {
+    const int e = elem_bytes(p->dtype);
+    Operand o = {at, {p->batch > 1 ? batch : 0, p->steps > 1 ? step : 0, head}, share, (int)width, 16};
+    while (o.bytes > 2 && (!aligned(at, o.bytes) || o.s.batch * e % o.bytes != 0 || o.s.step * e % o.bytes != 0 || head * e % o.bytes != 0))
+        o.bytes /= 2;
+    return o;
+}
+
+struct Operands {
+    Operand q, k, v, d;
+};
+Operands operands(const dcn_attn* p, const void* q, const void* k, const void* v, const void* dout) {
+    const int share = (int)(p->heads / p->kv_heads);
+    return {operand(p, q, p->q_batch, p->q_step, p->heads > 1 ? p->q_head : 0, p->dk, 1),
+            operand(p, k, p->k_batch, p->k_step, p->kv_heads > 1 ? p->k_head : 0, p->dk, share),
+            operand(p, v, p->v_batch, p->v_step, p->kv_heads > 1 ? p->v_head : 0, p->dv, share),
+            operand(p, dout, p->dout_batch, p->dout_step, p->heads > 1 ? p->dout_head : 0, p->dv, 1)};
+}
+
+AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* lengths, bool backward) {
+    AttnArgs a = {};
+    a.log_decay = log_decay, a.lengths = lengths;
+    a.steps = p->steps;
+    a.batch = (int)p->batch, a.heads = (int)p->heads;
+    a.n_parts = parts_for(p, backward);
+    const int64_t chunks = (p->steps + kChunk - 1) / kChunk;
+    a.part_steps = std::max<int64_t>(1, (chunks + a.n_parts - 1) / a.n_parts) * kChunk;
+    a.scale = p->scale;
+    return a;
+}
+
+void add(AttnArgs& a, const Job& j, int elem) {
+    a.tile_of[a.jobs] = (j.c.width + kCols - 1) / kCols;
+    a.tiles = std::max(a.tiles, a.tile_of[a.jobs]);
+    a.job[a.jobs] = j;
+    a.job[a.jobs++].pairs = j.c.width % 2 == 0 && aligned(j.out, 2 * (j.wide ? 4 : elem));
+}
+
+size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
+size_t state_elems(const dcn_attn* p) { return (size_t)p->batch * p->heads * p->dk * p->dv; }
+size_t parts_bytes(const dcn_attn* p, bool backward) {
+    const int n = parts_for(p, backward);
+    if (n <= 1) return 0;
+    if (!backward) return rounded((size_t)n * state_elems(p) * 4);
+    const size_t dk = p->dk, dv = p->dv, most = std::max(dk, dv) * dv;         // the jobs' states are dv x dk, dv x dk and dk x dv
+    return rounded(3 * (size_t)n * p->batch * p->heads * std::max(most, dk * dv) * 4);
+}
+
+bool attn_aligned(const dcn_attn* p, std::initializer_list<const void*> elems, std::initializer_list<const void*> floats) {
+    for (const void* v : elems)
+        if (!aligned(v, elem_bytes(p->dtype))) return false;
+    for (const void* v : floats)
+        if (!aligned(v, 4)) return false;
+    return true;
+}
+
+}  // namespace
+}  // namespace seq
+}  // namespace dcn
+
+using namespace dcn::seq;
+using dcn::launch_dependent;
+
+extern "C" size_t dcn_attn_workspace_bytes(const dcn_attn* p, int32_t backward) {
+    if (check_attn(p) != DCN_OK || p->batch == 0) return 0;
+    size_t n = parts_bytes(p, backward != 0);
+    if (backward && p->heads != p->kv_heads) n += rounded((size_t)p->batch * p->steps * p->heads * p->dk * 4) + rounded((size_t)p->batch * p->steps * p->heads * p->dv * 4);
+    return n;
+}
+
+extern "C" int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay,
+                                const float* state, const int64_t* lengths, void* out, float* last, void* workspace,
+                                size_t workspace_bytes, void* stream) {
+    const int bad = check_attn(p);
+    if (bad != DCN_OK) return bad;
+    if (p->batch == 0) return DCN_OK;
+    if (log_decay == nullptr || last == nullptr || (p->steps > 0 && (q == nullptr || k == nullptr || v == nullptr || out == nullptr)))
+        return DCN_ERR_NULL;
+    if (!attn_aligned(p, {q, k, v, out}, {log_decay, state, last}) || !aligned(lengths, 8)) return DCN_ERR_ALIGN;
+    const size_t need = dcn_attn_workspace_bytes(p, 0);
+    if (need > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
+    AttnArgs a = attn_args(p, log_decay, lengths, false);
+    const Operands o = operands(p, q, k, v, nullptr);
+    a.parts = static_cast<float*>(workspace);
+    add(a, {o.q, o.k, o.v, out, state, last, (int)p->dv, 1, 0, 0, 1.0f, 1.0f}, elem_bytes(p->dtype));
+    return run_attn_any(p, a, false, (cudaStream_t)stream);
+}
+
+extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay,
+                                 const float* state, const int64_t* lengths, const void* dout, const float* dlast, void* dq, void* dk,
+                                 void* dv, float* dstate, void* workspace, size_t workspace_bytes, void* stream) {
+    const int bad = check_attn(p);
+    if (bad != DCN_OK) return bad;
+    if (p->batch == 0) return DCN_OK;
+    if (log_decay == nullptr || (p->steps > 0 && (q == nullptr || k == nullptr || v == nullptr))) return DCN_ERR_NULL;
+    if (!attn_aligned(p, {q, k, v, dout, dq, dk, dv}, {log_decay, state, dlast, dstate}) || !aligned(lengths, 8)) return DCN_ERR_ALIGN;
+    const size_t need = dcn_attn_workspace_bytes(p, 1);
+    if (need > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (dout == nullptr && p->steps > 0) return DCN_ERR_NULL;
+    AttnArgs a = attn_args(p, log_decay, lengths, true);
+    const Operands o = operands(p, q, k, v, dout);
+    a.parts = static_cast<float*>(workspace);
+    const bool shared = p->heads != p->kv_heads;
+    char* const wide_k = static_cast<char*>(workspace) + parts_bytes(p, true);
+    char* const wide_v = wide_k + rounded((size_t)p->batch * p->steps * p->heads * p->dk * 4);
+    const int across = (int)p->dv, elem = elem_bytes(p->dtype);
+    const float s = p->scale;
+    if (dq != nullptr) add(a, {o.d, o.v, o.k, dq, state, nullptr, 1, across, 0, 0, 1.0f, 1.0f}, elem);
+    if (dk != nullptr) add(a, {o.v, o.d, o.q, shared ? wide_k : dk, dlast, nullptr, 1, across, 1, shared, 1.0f / s, 1.0f}, elem);
+    if (dv != nullptr || dstate != nullptr) {
+        if (dv == nullptr && p->steps > 0) return DCN_ERR_NULL;
+        add(a, {o.k, o.q, o.d, shared ? wide_v : dv, dlast, dstate, across, 1, 1, shared, 1.0f / s, s}, elem);
+    }
+    if (a.jobs == 0) return DCN_OK;
+    int rc = run_attn_any(p, a, true, st);
+    if (rc != DCN_OK || !shared || p->steps == 0) return rc;
+    const int share = (int)(p->heads / p->kv_heads);
+    auto sum = [&](const char* from, void* to, int64_t width) {
+        const int64_t count = p->batch * p->steps * p->kv_heads * width;
+        const dim3 grid((unsigned)std::min<int64_t>((count + 255) / 256, 148 * 16));
+        cudaError_t e;
+        const float* f = reinterpret_cast<const float*>(from);
+        if (p->dtype == DCN_SEQ_F32) e = launch_dependent(shared_kernel<float>, grid, dim3(256), 0, st, f, static_cast<float*>(to), count, share, (int)width);
+        else if (p->dtype == DCN_SEQ_BF16) e = launch_dependent(shared_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, f, static_cast<__nv_bfloat16*>(to), count, share, (int)width);
+        else e = launch_dependent(shared_kernel<__half>, grid, dim3(256), 0, st, f, static_cast<__half*>(to), count, share, (int)width);
+        return e == cudaSuccess ? DCN_OK : DCN_ERR_CUDA;
+    };
+    if (dk != nullptr) rc = sum(wide_k, dk, p->dk);
+    if (rc == DCN_OK && dv != nullptr) rc = sum(wide_v, dv, p->dv);
+    return rc;
+}
+
+extern "C" int dcn_attn_step(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay,
+                             float* pool_state, int64_t pool, const int64_t* slots, void* out, void* stream) {
+    const int bad = check_attn(p);
+    if (bad != DCN_OK) return bad;
+    if (p->steps != 1 || pool < 0 || (slots == nullptr && pool < p->batch)) return DCN_ERR_SHAPE;
+    if (p->batch == 0) return DCN_OK;
+    if (q == nullptr || k == nullptr || v == nullptr || log_decay == nullptr || out == nullptr || (pool_state == nullptr && pool > 0))
+        return DCN_ERR_NULL;
+    if (!attn_aligned(p, {q, k, v, out}, {log_decay, pool_state}) || !aligned(slots, 8)) return DCN_ERR_ALIGN;
+    StepArgs a = {q, k, v, {p->q_batch, 0, p->q_head}, {p->k_batch, 0, p->k_head}, {p->v_batch, 0, p->v_head}, log_decay, pool_state,
+                  slots, out, pool, (int)p->heads, (int)(p->heads / p->kv_heads), (int)p->dk, (int)p->dv, p->scale};
+    const dim3 grid((unsigned)(p->batch * p->heads));
+    const cudaStream_t st = (cudaStream_t)stream;
+    const bool wide = p->dv % 4 == 0 && aligned(pool_state, 16);
+    auto go = [&](auto* type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        return wide ? launch_dependent(attn_step_kernel<T, 4>, grid, dim3(kThreads), 0, st, a)
+                    : launch_dependent(attn_step_kernel<T, 1>, grid, dim3(kThreads), 0, st, a);
+    };
+    const cudaError_t e = p->dtype == DCN_SEQ_F32    ? go((float*)nullptr)
+                          : p->dtype == DCN_SEQ_BF16 ? go((__nv_bfloat16*)nullptr)
+                                                     : go((__half*)nullptr);
+    return e == cudaSuccess ? DCN_OK : DCN_ERR_CUDA;
+}

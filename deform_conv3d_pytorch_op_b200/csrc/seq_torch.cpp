@@ -14,6 +14,7 @@
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
+#include <cmath>
 #include <mutex>
 #include <vector>
 
@@ -31,6 +32,9 @@ struct Numbers {                         // what a call says beside its tensors
     int32_t top = 0;
     double temperature = 1.0, eps = 1e-6;
     bool tail = true;
+    double scale = 0.0;                  // 0: the default
+    int64_t groups = 1;
+    int32_t act = 0;
 };
 
 struct Operator {
@@ -371,10 +375,166 @@ variable_list distill_backward(const Numbers& n, const variable_list& kept, cons
     return {dlogits};
 }
 
+// ---- decayed attention: q, k, v, log_decay, state, lengths -> out, last -------------------------------------------------------
+void check_heads(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, int64_t dims, const char* expected) {
+    on_gpu(q, "q");
+    type_of(q, "q");
+    if (q.dim() != dims) fail("q has shape " + shape_text(q.sizes()) + ", expected " + expected);
+    beside(k, "k", q, "q");
+    beside(v, "v", q, "q");
+    beside(log_decay, "log_decay", q, "q");
+    typed(k, "k", q.scalar_type(), "q");
+    typed(v, "v", q.scalar_type(), "q");
+    const int64_t heads = q.size(dims - 2), dk = q.size(dims - 1);
+    if (k.dim() != dims || v.dim() != dims) fail(std::string("k and v have the dimensions of q: ") + expected);
+    const int64_t kv = k.size(dims - 2);
+    if (heads < 1 || kv < 1 || heads % kv != 0)
+        fail("k has " + std::to_string(kv) + " heads, which do not divide q's " + std::to_string(heads));
+    std::vector<int64_t> ks = q.sizes().vec(), vs = q.sizes().vec();
+    ks[dims - 2] = vs[dims - 2] = kv;
+    vs[dims - 1] = v.size(dims - 1);
+    shaped(k, "k", ks);
+    shaped(v, "v", vs);
+    for (int64_t w : {dk, v.size(dims - 1)})
+        if (w < 1 || w > 128) fail("heads have 1 to 128 elements, got " + std::to_string(w));
+    typed(log_decay, "log_decay", at::kFloat);
+    shaped(log_decay, "log_decay", {heads});
+}
+
+dcn_attn attn_of(const Numbers& n, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& dout) {
+    dcn_attn p = {};
+    const bool step = q.dim() == 3;
+    const int h = step ? 1 : 2;
+    p.dtype = type_of(q, "q");
+    p.batch = q.size(0), p.steps = step ? 1 : q.size(1), p.heads = q.size(h), p.kv_heads = k.size(h);
+    p.dk = q.size(h + 1), p.dv = v.size(h + 1);
+    p.q_batch = q.stride(0), p.q_step = step ? 0 : q.stride(1), p.q_head = q.stride(h);
+    p.k_batch = k.stride(0), p.k_step = step ? 0 : k.stride(1), p.k_head = k.stride(h);
+    p.v_batch = v.stride(0), p.v_step = step ? 0 : v.stride(1), p.v_head = v.stride(h);
+    if (dout.defined()) p.dout_batch = dout.stride(0), p.dout_step = dout.stride(1), p.dout_head = dout.stride(2);
+    p.scale = n.scale != 0.0 ? (float)n.scale : (float)(1.0 / std::sqrt((double)p.dk));
+    return p;
+}
+
+Tensor workspace(size_t bytes, const Tensor& x) {
+    return bytes > 0 ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
+}
+
+variable_list attn_forward(const Numbers& n, const variable_list& in, bool keep, variable_list& kept) {
+    check_heads(in[0], in[1], in[2], in[3], 4, "(batch, steps, heads, elements)");
+    const int64_t batch = in[0].size(0), heads = in[0].size(2), dk = in[0].size(3), dv = in[2].size(3);
+    beside(in[4], "state", in[0], "q");
+    beside(in[5], "lengths", in[0], "q");
+    typed(in[4], "state", at::kFloat);
+    shaped(in[4], "state", {batch, heads, dk, dv});
+    shaped(in[5], "lengths", {batch});
+    const Tensor lengths = whole_numbers(in[5], "lengths"), decay = in[3].contiguous();
+    const Tensor q = dense_last(in[0]), k = dense_last(in[1]), v = dense_last(in[2]);
+    const Tensor state = in[4].defined() ? in[4].contiguous() : in[4];
+    const dcn_attn p = attn_of(n, q, k, v, Tensor());
+    const c10::cuda::CUDAGuard guard(q.device());
+    const Tensor out = at::empty({batch, in[0].size(1), heads, dv}, q.options()), last = floats({batch, heads, dk, dv}, q);
+    const size_t bytes = dcn_attn_workspace_bytes(&p, 0);
+    const Tensor ws = workspace(bytes, q);
+    Range range("dcn_attn_forward");
+    check(dcn_attn_forward(&p, ptr(q), ptr(k), ptr(v), fptr(decay), fptr(state), iptr(lengths), wptr(out), fptr(last), wptr(ws), bytes,
+                           current_stream(q)),
+          "dcn_attn_forward");
+    if (keep) kept = {in[0], in[1], in[2], in[3].detach(), in[4], lengths};
+    return {out, last};
+}
+
+variable_list attn_backward(const Numbers& n, const variable_list& kept, const variable_list& grads, const std::vector<bool>& want) {
+    const Tensor q = dense_last(kept[0]), k = dense_last(kept[1]), v = dense_last(kept[2]), decay = kept[3].contiguous();
+    const Tensor state = kept[4].defined() ? kept[4].contiguous() : kept[4];
+    Tensor dout = grads[0];
+    const c10::cuda::CUDAGuard guard(q.device());
+    // (a gradient of the last state alone)
+    if (!dout.defined()) dout = at::zeros({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
+    dout = dense_last(dout);
+    const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : grads[1];
+    const dcn_attn p = attn_of(n, q, k, v, dout);
+    const Tensor dq = maybe(want[0], q), dk = maybe(want[1], k), dv = maybe(want[2] || want[4], v);
+    const Tensor dstate = want[4] ? floats({p.batch, p.heads, p.dk, p.dv}, q) : Tensor();
+    const size_t bytes = dcn_attn_workspace_bytes(&p, 1);
+    const Tensor ws = workspace(bytes, q);
+    Range range("dcn_attn_backward");
+    check(dcn_attn_backward(&p, ptr(q), ptr(k), ptr(v), fptr(decay), fptr(state), iptr(kept[5]), ptr(dout), fptr(dlast), wptr(dq),
+                            wptr(dk), wptr(dv), fptr(dstate), wptr(ws), bytes, current_stream(q)),
+          "dcn_attn_backward");
+    return {dq, dk, want[2] ? dv : Tensor(), Tensor(), dstate};
+}
+
+// ---- group norm with an activation: x, weight, bias, residual -> y ------------------------------------------------------------
+dcn_gnorm gnorm_of(const Numbers& n, const Tensor& x, const Tensor& weight, const Tensor& bias) {
+    dcn_gnorm p = {};
+    p.dtype = type_of(x, "x");
+    p.weight_dtype = weight.defined() ? type_of(weight, "weight") : bias.defined() ? type_of(bias, "bias") : p.dtype;
+    p.act = n.act;
+    p.samples = x.size(0), p.channels = x.size(-1);
+    p.positions = 1;
+    for (int64_t i = 1; i + 1 < x.dim(); ++i) p.positions *= x.size(i);
+    p.groups = n.groups;
+    p.eps = (float)n.eps;
+    return p;
+}
+
+variable_list gnorm_forward(const Numbers& n, const variable_list& in, bool keep, variable_list& kept) {
+    on_gpu(in[0], "x");
+    type_of(in[0], "x");
+    if (in[0].dim() < 2 || in[0].size(-1) < 1 || in[0].size(-1) > 8192)
+        fail("x has shape " + shape_text(in[0].sizes()) + ", expected (samples, ..., channels) of 1 to 8192 channels");
+    if (n.groups < 1 || in[0].size(-1) % n.groups != 0)
+        fail(std::to_string(n.groups) + " groups do not divide the " + std::to_string(in[0].size(-1)) + " channels");
+    if (!(n.eps >= 0.0)) fail("eps must not be negative");
+    if (n.act < DCN_ACT_NONE || n.act > DCN_ACT_SILU) fail("the activation is none, relu or silu");
+    beside(in[1], "weight", in[0], "x");
+    beside(in[2], "bias", in[0], "x");
+    beside(in[3], "residual", in[0], "x");
+    shaped(in[1], "weight", {in[0].size(-1)});
+    shaped(in[2], "bias", {in[0].size(-1)});
+    if (in[1].defined() && in[1].scalar_type() != at::kFloat) typed(in[1], "weight", in[0].scalar_type(), "x (or torch.float32)");
+    if (in[2].defined() && in[2].scalar_type() != at::kFloat) typed(in[2], "bias", in[0].scalar_type(), "x (or torch.float32)");
+    if (in[1].defined()) typed(in[2], "bias", in[1].scalar_type(), "weight");
+    typed(in[3], "residual", in[0].scalar_type(), "x");
+    shaped(in[3], "residual", in[0].sizes());
+    const Tensor x = in[0].contiguous(), weight = in[1].defined() ? in[1].contiguous() : in[1],
+                 bias = in[2].defined() ? in[2].contiguous() : in[2], residual = in[3].defined() ? in[3].contiguous() : in[3];
+    const dcn_gnorm p = gnorm_of(n, x, weight, bias);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor y = at::empty(x.sizes(), x.options()), stats = keep ? floats({p.samples, p.groups, 2}, x) : Tensor();
+    const size_t bytes = dcn_gnorm_workspace_bytes(&p, 0);
+    const Tensor ws = workspace(bytes, x);
+    Range range("dcn_gnorm_forward");
+    check(dcn_gnorm_forward(&p, ptr(x), ptr(weight), ptr(bias), ptr(residual), wptr(y), fptr(stats), wptr(ws), bytes, current_stream(x)),
+          "dcn_gnorm_forward");
+    if (keep) kept = {in[0], in[1], in[2], in[3], stats};
+    return {y};
+}
+
+variable_list gnorm_backward(const Numbers& n, const variable_list& kept, const variable_list& grads, const std::vector<bool>& want) {
+    const Tensor x = kept[0].contiguous(), weight = kept[1].defined() ? kept[1].contiguous() : kept[1],
+                 bias = kept[2].defined() ? kept[2].contiguous() : kept[2], residual = kept[3].defined() ? kept[3].contiguous() : kept[3];
+    const Tensor dy = grads[0].contiguous();
+    const dcn_gnorm p = gnorm_of(n, x, weight, bias);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor dx = maybe(want[0], x), dw = want[1] ? at::empty(weight.sizes(), weight.options()) : Tensor(),
+                 db = want[2] ? at::empty(bias.sizes(), bias.options()) : Tensor(), dres = maybe(want[3], x);
+    const size_t bytes = dcn_gnorm_workspace_bytes(&p, 1);
+    const Tensor ws = workspace(bytes, x);
+    Range range("dcn_gnorm_backward");
+    check(dcn_gnorm_backward(&p, ptr(x), ptr(weight), ptr(bias), ptr(residual), fptr(kept[4]), ptr(dy), wptr(dx), wptr(dw), wptr(db),
+                             wptr(dres), wptr(ws), bytes, current_stream(x)),
+          "dcn_gnorm_backward");
+    return {dx, dw, db, dres};
+}
+
 const Operator kScan = {"gated_scan", "GatedScanFunctionBackward", 4, 3, scan_forward, scan_backward};
 const Operator kNorm = {"residual_norm", "ResidualNormFunctionBackward", 6, 6, norm_forward, norm_backward};
 const Operator kScores = {"token_scores", "TokenScoresFunctionBackward", 2, 1, scores_forward, scores_backward};
 const Operator kDistill = {"distill_topk", "DistillTopkFunctionBackward", 3, 1, distill_forward, distill_backward};
+const Operator kAttn = {"decay_attention", "DecayAttentionFunctionBackward", 6, 5, attn_forward, attn_backward};
+const Operator kGnorm = {"group_norm_act", "GroupNormActFunctionBackward", 4, 4, gnorm_forward, gnorm_backward};
 
 // ---- the graph node -------------------------------------------------------------------------------------------------------
 struct SequenceBackward : public Node {
@@ -498,6 +658,14 @@ int32_t small_arg(PyObject* o) {
     return (int32_t)v;
 }
 
+// The scale of decayed attention: None for the default
+double scale_arg(PyObject* o) {
+    if (o == Py_None) return 0.0;
+    const double v = float_arg(o);
+    if (!std::isfinite((float)v) || (float)v == 0.0f || !std::isfinite(1.0f / (float)v)) fail("scale must be a finite number other than 0");
+    return v;
+}
+
 PyObject* wrap(variable_list&& v, bool single) {
     if (single) return THPVariable_Wrap(std::move(v[0]));
     PyObject* t = PyTuple_New((Py_ssize_t)v.size());
@@ -548,6 +716,17 @@ Numbers numbers_of(const Operator& op, PyObject* const* a, Py_ssize_t n, variabl
         if (n > 2) m.top = small_arg(a[2]);
         if (n > 3) m.temperature = float_arg(a[3]);
         if (n > 4) m.ignore = int_arg(a[4]);
+    } else if (&op == &kAttn) {
+        count_arg(n, 4, 7);
+        tensors({"q", "k", "v", "log_decay", "state", "lengths"}, 4);
+        if (n > 6) m.scale = scale_arg(a[6]);
+        if (at::GradMode::is_enabled() && in[3].requires_grad()) fail("log_decay has no gradient: detach it");
+    } else if (&op == &kGnorm) {
+        count_arg(n, 7, 7);
+        tensors({"x", "weight", "bias", "residual"}, 1);
+        m.groups = int_arg(a[4]);
+        m.act = small_arg(a[5]);
+        m.eps = float_arg(a[6]);
     } else {
         count_arg(n, 3, 5);
         tensors({"logits", "teacher_logprobs", "teacher_tokens"}, 3);
@@ -572,7 +751,7 @@ PyObject* apply(PyObject*, PyObject* const* a, Py_ssize_t n) {
             pybind11::gil_scoped_release no_gil;
             out = call(*op, m, in);
         }
-        return wrap(std::move(out), op == &kDistill);
+        return wrap(std::move(out), op == &kDistill || op == &kGnorm);
     });
 }
 
@@ -670,9 +849,130 @@ PyObject* scan_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     });
 }
 
+
+// (q, k, v, log_decay, state, slots, scale): one step, the states in place.  kInner: for the Function of sequence.py
+template <bool kInner>
+PyObject* attn_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        count_arg(n, 5, 7);
+        const Tensor q0 = in_memory(tensor_arg(a[0], "q")), k0 = in_memory(tensor_arg(a[1], "k")), v0 = in_memory(tensor_arg(a[2], "v"));
+        const Tensor decay0 = in_memory(tensor_arg(a[3], "log_decay")), state = tensor_arg(a[4], "state");
+        const Tensor slots0 = n > 5 ? in_memory(tensor_arg(a[5], "slots", true)) : Tensor();
+        Numbers m;
+        if (n > 6) m.scale = scale_arg(a[6]);
+        for (const Tensor* t : {&q0, &k0, &v0, &decay0, &state}) {
+            if (at::GradMode::is_enabled() && t->requires_grad())
+                fail("step has no gradient: call it under torch.no_grad(), or take apply");
+            if (has_tangent(*t)) fail("step has no derivative: take apply");
+        }
+        if (!kInner && inside_transform()) Py_RETURN_NOTIMPLEMENTED;
+        pybind11::gil_scoped_release no_gil;
+        at::NoGradGuard no_grad;
+        check_heads(q0, k0, v0, decay0, 3, "(rows, heads, elements)");
+        beside(state, "state", q0, "q");
+        beside(slots0, "slots", q0, "q");
+        typed(state, "state", at::kFloat);
+        const std::vector<int64_t> of = {q0.size(1), q0.size(2), v0.size(2)};
+        if (state.dim() != 4 || state.sizes().slice(1) != at::IntArrayRef(of) || !state.is_contiguous() || state.is_neg())
+            fail("state has shape " + shape_text(state.sizes()) + ", expected a contiguous (pool, " + shape_text(of).substr(1));
+        shaped(slots0, "slots", {q0.size(0)});
+        if (!slots0.defined() && state.size(0) < q0.size(0)) fail("state has fewer rows than q, and no slots are given");
+        const Tensor q = dense_last(q0), k = dense_last(k0), v = dense_last(v0), decay = decay0.contiguous();
+        const Tensor slots = whole_numbers(slots0, "slots");
+        const dcn_attn p = attn_of(m, q, k, v, Tensor());
+        const c10::cuda::CUDAGuard guard(q.device());
+        Tensor out = at::empty({q.size(0), q.size(1), v.size(2)}, q.options());
+        state.unsafeGetTensorImpl()->bump_version();             // (refuses an inference tensor outside inference mode: nothing ran)
+        {
+            Range range("dcn_attn_step");
+            check(dcn_attn_step(&p, ptr(q), ptr(k), ptr(v), fptr(decay), fptr(state), state.size(0), iptr(slots), wptr(out),
+                                current_stream(q)),
+                  "dcn_attn_step");
+        }
+        pybind11::gil_scoped_acquire gil;
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// (logits, uniform, temperature, top_k, top_p, min_p) -> (tokens, logprob); a setting is a number or a tensor with one for each row
+template <bool kInner>
+PyObject* token_sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        count_arg(n, 2, 6);
+        const Tensor logits0 = in_memory(tensor_arg(a[0], "logits")), uniform0 = in_memory(tensor_arg(a[1], "uniform"));
+        if (at::GradMode::is_enabled() && logits0.requires_grad())
+            fail("sampling has no gradient: call it under torch.no_grad() (TokenScoresFunction gives a token's log p with its own)");
+        if (has_tangent(logits0)) fail("sampling has no derivative");
+        static const char* const names[] = {"temperature", "top_k", "top_p", "min_p"};
+        double numbers[4] = {1.0, 0.0, 1.0, 0.0};
+        int64_t top_k = 0;
+        Tensor rows_own[4];
+        for (int i = 0; i < 4 && i + 2 < n; ++i) {
+            if (THPVariable_Check(a[i + 2])) rows_own[i] = in_memory(THPVariable_Unpack(a[i + 2]));
+            else if (i == 1) top_k = int_arg(a[i + 2]);
+            else numbers[i] = float_arg(a[i + 2]);
+        }
+        if (!kInner && inside_transform()) Py_RETURN_NOTIMPLEMENTED;
+        Tensor tokens, logprob;
+        {
+            pybind11::gil_scoped_release no_gil;
+            at::NoGradGuard no_grad;
+            on_gpu(logits0, "logits");
+            type_of(logits0, "logits");
+            if (logits0.dim() < 1 || logits0.size(-1) < 1 || logits0.size(-1) > 1 << 20)
+                fail("logits have shape " + shape_text(logits0.sizes()) + ", expected (..., vocabulary) of 1 to 2^20 tokens");
+            const std::vector<int64_t> lead = without_last(logits0);
+            beside(uniform0, "uniform", logits0, "logits");
+            typed(uniform0, "uniform", at::kFloat);
+            shaped(uniform0, "uniform", lead);
+            for (int i = 0; i < 4; ++i) {
+                if (!rows_own[i].defined()) continue;
+                beside(rows_own[i], names[i], logits0, "logits");
+                shaped(rows_own[i], names[i], lead);
+                if (i == 1) {
+                    rows_own[i] = whole_numbers(rows_own[i], names[i]);
+                } else {
+                    if (!rows_own[i].is_floating_point()) fail(std::string(names[i]) + " must be a number or floating-point numbers");
+                    rows_own[i] = rows_own[i].to(at::kFloat).contiguous();
+                }
+            }
+            if (!rows_own[0].defined() && !(numbers[0] == 0.0 || ((float)numbers[0] >= 1e-3f && (float)numbers[0] <= 1e3f)))
+                fail("temperature must be 0 or lie between 1e-3 and 1e3");
+            for (int i = 2; i < 4; ++i)
+                if (!rows_own[i].defined() && !(numbers[i] >= 0.0 && numbers[i] <= 1.0)) fail(std::string(names[i]) + " must lie between 0 and 1");
+            const int64_t rows = product(lead);
+            const Tensor logits = rows_of(logits0, rows, logits0.size(-1)), uniform = uniform0.contiguous();
+            dcn_sample p = {};
+            p.dtype = type_of(logits, "logits");
+            p.rows = rows, p.vocab = logits.size(-1), p.row_stride = row_stride(logits);
+            p.temperature = (float)numbers[0], p.top_p = (float)numbers[2], p.min_p = (float)numbers[3];
+            p.top_k = top_k;
+            p.temperatures = fptr(rows_own[0]), p.top_ks = iptr(rows_own[1]), p.top_ps = fptr(rows_own[2]), p.min_ps = fptr(rows_own[3]);
+            const c10::cuda::CUDAGuard guard(logits.device());
+            tokens = at::empty(lead, logits.options().dtype(at::kLong)), logprob = floats(lead, logits);
+            const size_t bytes = dcn_sample_workspace_bytes(&p);
+            const Tensor ws = workspace(bytes, logits);
+            Range range("dcn_sample_tokens");
+            check(dcn_sample_tokens(&p, ptr(logits), fptr(uniform), iptr(tokens), fptr(logprob), wptr(ws), bytes, current_stream(logits)),
+                  "dcn_sample_tokens");
+        }
+        return wrap({tokens, logprob}, false);
+    });
+}
+
 }  // namespace
 
 PyMethodDef dcn_host::sequence_methods[] = {
+    {"decay_attention", DCN_FAST(apply<&kAttn>), nullptr},
+    {"decay_attention_forward", DCN_FAST(forward<&kAttn>), nullptr},
+    {"decay_attention_backward", DCN_FAST(backward<&kAttn>), nullptr},
+    {"decay_attention_step", DCN_FAST(attn_step<false>), nullptr},
+    {"decay_attention_step_forward", DCN_FAST(attn_step<true>), nullptr},
+    {"group_norm_act", DCN_FAST(apply<&kGnorm>), nullptr},
+    {"group_norm_act_forward", DCN_FAST(forward<&kGnorm>), nullptr},
+    {"group_norm_act_backward", DCN_FAST(backward<&kGnorm>), nullptr},
+    {"token_sample", DCN_FAST(token_sample<false>), nullptr},
+    {"token_sample_forward", DCN_FAST(token_sample<true>), nullptr},
     {"gated_scan", DCN_FAST(apply<&kScan>), nullptr},
     {"gated_scan_forward", DCN_FAST(forward<&kScan>), nullptr},
     {"gated_scan_backward", DCN_FAST(backward<&kScan>), nullptr},

@@ -5,8 +5,12 @@ the loss against a larger teacher and the scores that it answers with.  (The ref
 * :class:`ResidualNormFunction`  -- norm behind a block, gate, scaled residual and the norm before the next block in one pass
 * :class:`TokenScoresFunction`   -- log-probabilities of given tokens (or classes), entropy and the best alternatives
 * :class:`DistillTopkFunction`   -- KL divergence from a teacher's best tokens
+* :class:`DecayAttentionFunction` -- linear attention whose states decay, head by head, its gradient, and its form for one step
+* :class:`GroupNormActFunction`  -- group norm of channels-last features with a residual and an activation
+* :class:`TokenSampleFunction`   -- tokens (or classes) drawn by given random numbers after temperature, top-k, top-p and min-p
 
-and the modules :class:`GatedScan`, :class:`ResidualNorm` and :class:`TopkDistillLoss` over them.
+and the modules :class:`GatedScan`, :class:`ResidualNorm`, :class:`TopkDistillLoss`, :class:`DecayAttention` and :class:`GroupNormAct`
+over them.
 
 Tensors are float32, bfloat16 or float16 on a CUDA device; the last axis should be dense (it is copied otherwise), the others may
 have any strides, so the parts of one projection's output are taken as they are.  Sums, statistics and states are float32.  Calls
@@ -58,6 +62,37 @@ _GatedScanFunction = _function("gated_scan", 3)
 _ResidualNormFunction = _function("residual_norm", 6)
 _TokenScoresFunction = _function("token_scores", 1)
 _DistillTopkFunction = _function("distill_topk", 1)
+
+
+_DecayAttentionFunction = _function("decay_attention", 5)
+_GroupNormActFunction = _function("group_norm_act", 4)
+
+
+class _DecayAttentionStepFunction(Function):
+    """As _GatedScanStepFunction."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _lib.native().decay_attention_step_forward(*args)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        raise RuntimeError("step has no gradient: take apply")
+
+
+class _TokenSampleFunction(Function):
+    """As _GatedScanStepFunction."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        out = _lib.native().token_sample_forward(*args)
+        ctx.mark_non_differentiable(*out)
+        return out
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError("sampling has no gradient")
 
 
 class _GatedScanStepFunction(Function):
@@ -145,6 +180,75 @@ class DistillTopkFunction:
         args = (logits, teacher_logprobs, teacher_tokens, temperature, tail)
         out = _lib.native().distill_topk(*args)
         return _DistillTopkFunction.apply(*args) if out is NotImplemented else out
+
+
+class DecayAttentionFunction:
+    """Linear attention over time whose states decay, for each head: ``S_t = exp(log_decay) S_{t-1} + k_t v_t^T``,
+    ``out_t = scale S_t^T q_t``."""
+
+    @staticmethod
+    def apply(q, k, v, log_decay, state=None, lengths=None, scale=None):
+        """``(out, last)``: [batch, steps, heads, dv] in q's type, and the last states [batch, heads, dk, dv] in float32.
+
+        ``q`` [batch, steps, heads, dk], ``k`` and ``v`` [batch, steps, kv_heads, dk or dv] (1 to 128 each), where kv_heads divides
+        heads: neighbouring heads share a key and a value.  ``log_decay`` [heads] float32, taken as 0 where it is above: no gradient.
+        ``state`` [batch, heads, dk, dv] float32: the states before the first step (zeros); ``lengths`` [batch] int64 or int32: steps
+        of each sequence.  Behind them out is zero, q, k and v are not read, and last is the state after the sequence's own steps.
+        ``scale``: 1 / sqrt(dk) if None.  Gradients: q, k, v, state.
+
+        In 16-bit types a step's weight on each of the steps of its block of 64, and the state that it meets from before, are rounded
+        to the type (the states themselves are float32); NaN or infinity at a step may reach steps of its block before it."""
+        args = (q, k, v, log_decay, state, lengths, scale)
+        out = _lib.native().decay_attention(*args)
+        return _DecayAttentionFunction.apply(*args) if out is NotImplemented else out
+
+    @staticmethod
+    def step(q, k, v, log_decay, state, slots=None, scale=None):
+        """One step of running sequences, without gradients: ``q`` [rows, heads, dk], ``k``, ``v`` [rows, kv_heads, dk or dv];
+        ``state`` [pool, heads, dk, dv] float32, contiguous, advanced in place at the rows ``slots`` [rows] (0, 1, ... if None),
+        each of which occurs once; a slot outside the pool is skipped, and its row is zero.  Returns [rows, heads, dv]."""
+        args = (q, k, v, log_decay, state, slots, scale)
+        out = _lib.native().decay_attention_step(*args)
+        return _DecayAttentionStepFunction.apply(*args) if out is NotImplemented else out
+
+
+_ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "silu": 2}
+
+
+class GroupNormActFunction:
+    """``act((x - mean) / sqrt(var + eps) * weight + bias + residual)``, mean and variance over the positions and channels of each
+    sample's groups."""
+
+    @staticmethod
+    def apply(x, groups, weight=None, bias=None, residual=None, activation=None, eps=1e-5):
+        """``y`` in x's type and shape [samples, ..., channels] (1 to 8192 channels, copied where it is not contiguous).
+
+        ``weight``, ``bias`` [channels], both float32 or both of x's type; ``residual`` as x; ``activation``: None, "relu" or "silu".
+        Gradients: x, weight, bias, residual; sums over samples are made in a fixed order."""
+        act = _ACTIVATIONS.get(activation)
+        if act is None:
+            raise _lib.DcnError("activation is %r: None, 'relu' and 'silu' are supported" % (activation,))
+        args = (x, weight, bias, residual, groups, act, eps)
+        out = _lib.native().group_norm_act(*args)
+        return _GroupNormActFunction.apply(*args) if out is NotImplemented else out
+
+
+class TokenSampleFunction:
+    """Tokens drawn from rows of logits [..., vocabulary] (up to 2^20) by given random numbers."""
+
+    @staticmethod
+    def apply(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """``(tokens, logprob)``, int64 and float32 [...], from ``uniform`` [...] float32 in [0, 1).
+
+        A row keeps its ``top_k`` largest logits (all for 0), equal ones by index; of these the fewest that have ``top_p`` of the
+        probability; of these the ones with ``min_p`` of the largest probability.  The token is where the kept probabilities,
+        added by index, pass ``uniform`` of their sum, and logprob its logarithm among them.  Each setting is a number or a tensor
+        [...] with one for each row.  ``temperature`` lies between 1e-3 and 1e3 (a tensor's is taken into it), or is 0 for the best token.
+        Probabilities are whole numbers of 2^-40 of the largest, so that a draw does not depend on how sums are split.  Logits of -inf
+        stand for tokens that cannot come; rows of nothing else, with NaN or with +inf give token -1 and NaN.  No gradient."""
+        args = (logits, uniform, temperature, top_k, top_p, min_p)
+        out = _lib.native().token_sample(*args)
+        return _TokenSampleFunction.apply(*args) if out is NotImplemented else out
 
 
 class GatedScan(nn.Module):

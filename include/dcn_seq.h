@@ -5,6 +5,9 @@
  *   gated residual norm  stream = x + scale * s(gate) * rms(block) * post,  normed = rms(stream) * pre
  *   token scores         log-probabilities of given tokens, entropy and the best alternatives of rows of logits
  *   distillation         KL divergence from a teacher's top tokens, with the gradient of the student's logits
+ *   decayed attention    S_t = g S_{t-1} + k_t v_t^T, out_t = scale S_t^T q_t, per head over time
+ *   group norm           y = act(norm(x) w + b + residual) over a sample's groups of channels, channels last
+ *   token sampling       one token of each row, drawn by a given random number after top-k, top-p and min-p
  *
  * The reference (lshiwjx/deform_conv3d_pytorch_op) has no counterpart of these.  Conventions as in dcn.h: device pointers on
  * the current device, `stream` a cudaStream_t passed as void*, nothing is allocated and nothing synchronises, no state is kept
@@ -129,6 +132,94 @@ int dcn_distill_forward(const dcn_logits* p, const void* logits, int32_t k, cons
 int dcn_distill_backward(const dcn_logits* p, const void* logits, int32_t k, const void* teacher_logprobs, int32_t teacher_dtype,
                          const int64_t* teacher_tokens, int32_t tail, const float* stats, const float* dloss, void* dlogits,
                          void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Decayed linear attention: for each head with its decay g = exp(log_decay), a state S [dk, dv],
+ *   S_t = g S_{t-1} + k_t v_t^T,   out_t = scale S_t^T q_t
+ * ------------------------------------------------------------------------------------------- */
+typedef struct dcn_attn {
+    int32_t dtype;                              /* q, k, v, out and their gradients */
+    int64_t batch, steps, heads, kv_heads;      /* kv_heads divides heads: head h has the key and value h / (heads / kv_heads) */
+    int64_t dk, dv;                             /* 1 to 128 each */
+    int64_t q_batch, q_step, q_head;            /* strides */
+    int64_t k_batch, k_step, k_head;
+    int64_t v_batch, v_step, v_head;
+    int64_t dout_batch, dout_step, dout_head;   /* backward only */
+    float scale;                                /* finite, not 0 */
+} dcn_attn;
+
+/* Scratch bytes of dcn_attn_forward (backward = 0) and dcn_attn_backward (backward = 1) on the current device; may be 0. */
+size_t dcn_attn_workspace_bytes(const dcn_attn* p, int32_t backward);
+
+/* out [batch, steps, heads, dv] (dense) and last [batch, heads, dk, dv] (float32): the state after the last step.  log_decay float32
+ * [heads], taken as 0 where it is above; `state` [batch, heads, dk, dv] float32, or NULL for zeros.  `lengths` [batch] int64, or
+ * NULL: sequence b has lengths[b] steps (taken into [0, steps]); behind them out is zero, and q, k and v are not read.
+ * In 16-bit types the state that meets q, and the weights that meet v within 64 steps, are rounded to the type; `last` is not. */
+int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay, const float* state,
+                     const int64_t* lengths, void* out, float* last, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dq, dk, dv (dense, zero behind a sequence's length) and dstate (float32) -- any may be NULL = not wanted, dv only where dstate is
+ * -- from dout and dlast (float32, may be NULL for zeros). */
+int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay, const float* state,
+                      const int64_t* lengths, const void* dout, const float* dlast, void* dq, void* dk, void* dv, float* dstate,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* One step of `p->batch` sequences (p->steps is 1, strides over steps are not used) whose states are rows of a pool:
+ * pool_state [pool, heads, dk, dv] float32, dense; state[slots[r]] advances in place, out [batch, heads, dv] dense.  slots int64
+ * [batch] or NULL for 0, 1, ...; a slot outside [0, pool) leaves the pool alone and gives zeros.  No slot may occur twice. */
+int dcn_attn_step(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay, float* pool_state,
+                  int64_t pool, const int64_t* slots, void* out, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Group norm with an activation, channels last: the statistics of a sample's group are over all its positions and its channels,
+ *   y = act((x - mean) / sqrt(var + eps) * weight + bias + residual)      (weight 1, bias and residual 0 where NULL)
+ * ------------------------------------------------------------------------------------------- */
+enum { DCN_ACT_NONE = 0, DCN_ACT_RELU = 1, DCN_ACT_SILU = 2 };
+
+typedef struct dcn_gnorm {
+    int32_t dtype;                              /* x, residual, y, dy, dx, dresidual: [samples, positions, channels], dense */
+    int32_t weight_dtype;                       /* weight, bias [channels] and their gradients: float32 or dtype */
+    int32_t act;
+    int64_t samples, positions, channels, groups;   /* groups divides channels, channels <= 8192 */
+    float eps;
+} dcn_gnorm;
+
+/* Scratch bytes of dcn_gnorm_forward (backward = 0) and dcn_gnorm_backward (backward = 1) on the current device; may be 0. */
+size_t dcn_gnorm_workspace_bytes(const dcn_gnorm* p, int32_t backward);
+
+/* stats float32 [samples, groups, 2]: mean and 1 / sqrt(var + eps), for the backward pass, or NULL. */
+int dcn_gnorm_forward(const dcn_gnorm* p, const void* x, const void* weight, const void* bias, const void* residual, void* y,
+                      float* stats, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dx, dresidual, dweight and dbias (any may be NULL = not wanted) from dy.  Sums over samples are made in a fixed order. */
+int dcn_gnorm_backward(const dcn_gnorm* p, const void* x, const void* weight, const void* bias, const void* residual,
+                       const float* stats, const void* dy, void* dx, void* dweight, void* dbias, void* dresidual, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Token sampling.  The weights of a row are whole numbers, w = floor(2^40 exp((logit - largest) / temperature)) with the exponential
+ * in float32, so that sums are exact and a draw does not depend on how a row is split.  Kept are, one behind the other,
+ *   the top_k largest logits, equal ones by their index (all where top_k <= 0),
+ *   of these the fewest largest whose weights reach top_p of their sum (all where top_p >= 1),
+ *   of these the ones whose exponential is at least min_p; the largest logit always stays.
+ * The token is the first by index up to which the kept weights exceed floor(uniform * their sum); logprob is log(w / sum).
+ * temperature 0: the largest logit.  A row of NaN, +inf or -inf alone, or with a NaN setting, gives token -1 and logprob NaN.
+ * ------------------------------------------------------------------------------------------- */
+typedef struct dcn_sample {
+    int32_t dtype;                              /* logits */
+    int64_t rows, vocab;                        /* rows < 2^27, 1 <= vocab <= 2^20 */
+    int64_t row_stride;
+    float temperature, top_p, min_p;            /* 0 or 1e-3 to 1e3 (rows' own are taken into it); 0 to 1; 0 to 1 */
+    int64_t top_k;
+    const float *temperatures, *top_ps, *min_ps;    /* [rows] each, or NULL: the number above for all rows */
+    const int64_t* top_ks;
+} dcn_sample;
+
+size_t dcn_sample_workspace_bytes(const dcn_sample* p);
+
+/* tokens int64 and logprobs float32 [rows] from uniforms float32 [rows] in [0, 1) (others are taken into it). */
+int dcn_sample_tokens(const dcn_sample* p, const void* logits, const float* uniforms, int64_t* tokens, float* logprobs,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }
