@@ -18,14 +18,16 @@ namespace seq {
 namespace {
 
 constexpr int64_t kMostChannels = 8192;
+constexpr int kThreads = 256;                    // of a CTA of the two passes, at most
 constexpr int kHeldBytes = 96 * 1024;            // of a sample's tensors, so that two CTAs share an SM
 
 struct GnormArgs {
     const void *x, *weight, *bias, *residual, *dy;
     void *y, *dx, *dresidual;
     float *stats;                                // [samples][groups][2]
-    float *partial;                              // forward [samples][splits][groups][2], backward [samples][splits][channels][2]
-    float *sums;                                 // backward [samples][groups][2]
+    float *partial;                              // [samples][splits][groups][2]
+    float *channel_sums;                         // backward [CTAs][channels][2]
+    void *dweight, *dbias;
     int64_t samples, positions, split_positions;
     int channels, groups, per_group, vectors, act, wide_weights, splits;
     float eps, inv;                              // 1 / elements of a group
@@ -44,23 +46,94 @@ __device__ __forceinline__ float weight_at(const void* w, int c, int wide, float
     return p.at(0);
 }
 
-__device__ __forceinline__ float activate(float z, int act) {
-    if (act == DCN_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if (act == DCN_ACT_SILU) {
-        float s, rest;
-        logistic(z, s, rest);
-        return z * s;
+// The weights of V channels, all on their way at once
+template <typename T, int V>
+__device__ __forceinline__ void weights_at(const void* w, int c0, int wide, float none, float (&out)[V]) {
+    if (w == nullptr) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[e] = none;
+    } else if (wide) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[e] = gload(static_cast<const float*>(w) + c0 + e);
+    } else {
+        Pack<T, 1> p[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) p[e].get(static_cast<const T*>(w) + c0 + e);
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[e] = p[e].at(0);
+    }
+}
+
+// The elements of a vector in pairs, as the packed instructions take them (one alone beside a zero)
+template <int V>
+struct Pairs {
+    static constexpr int kN = (V + 1) / 2;
+    Lanes v[kN];
+    template <typename T>
+    __device__ __forceinline__ void from(const Pack<T, V>& p) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const float f[2] = {p.at(2 * i), 2 * i + 1 < V ? p.at(2 * i + 1 < V ? 2 * i + 1 : 0) : 0.0f};
+            v[i] = lanes(f);
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ Pack<T, V> pack() const {
+        float f[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) f[e] = v[e / 2].at(e % 2);
+        Pack<T, V> p;
+        p.set(f);
+        return p;
+    }
+    __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] = all_lanes(f);
+    }
+    __device__ __forceinline__ float at(int e) const { return v[e / 2].at(e % 2); }
+    // each element of two vectors
+    template <typename F>
+    __device__ __forceinline__ void map(F&& f) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            const float r[2] = {f(v[i].at(0), 2 * i), 2 * i + 1 < V ? f(v[i].at(1), 2 * i + 1) : 0.0f};
+            v[i] = lanes(r);
+        }
+    }
+};
+
+// y = act(z)
+template <int V>
+__device__ __forceinline__ void activate(Pairs<V>& z, int act) {
+    if (act == DCN_ACT_RELU) {
+        z.map([](float v, int) {
+            float r;
+            asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+            return r;
+        });
+    } else if (act == DCN_ACT_SILU) {
+        z.map([](float v, int) {
+            float s, rest;
+            logistic(v, s, rest);
+            return v * s;
+        });
+    }
+}
+// dy act'(z)
+template <int V>
+__device__ __forceinline__ Pairs<V> activate_gradient(Pairs<V> z, const Pairs<V>& dy, int act) {
+    if (act == DCN_ACT_RELU) {
+        z.map([&](float v, int e) { return v <= 0.0f ? 0.0f : dy.at(e); });
+    } else if (act == DCN_ACT_SILU) {
+        z.map([&](float v, int e) {
+            float s, rest;
+            logistic(v, s, rest);
+            return dy.at(e) * (s * fmaf(v, rest, 1.0f));
+        });
+    } else {
+        z = dy;
     }
     return z;
-}
-__device__ __forceinline__ float activate_gradient(float z, float dy, int act) {
-    if (act == DCN_ACT_RELU) return z > 0.0f ? dy : (z != z ? z : 0.0f);
-    if (act == DCN_ACT_SILU) {
-        float s, rest;
-        logistic(z, s, rest);
-        return dy * (s * fmaf(z, rest, 1.0f));
-    }
-    return dy;
 }
 
 // How the vectors of a row of channels lie over the threads: rows of threads where a row of vectors is shorter than the CTA, blocks of
@@ -78,87 +151,206 @@ struct Grid {
     }
 };
 
-// Mean and sum of squares about it from `n` entries (count, mean, sum) of which a warp reads e, e + 32, ...
-template <typename F>
-__device__ __forceinline__ void join(int n, F&& entry, float& mean, float& sq, float& count) {
-    const int lane = threadIdx.x & 31;
-    float c = 0.0f, s = 0.0f;
-    for (int i = lane; i < n; i += 32) {
-        float ci, mi, qi;
-        entry(i, ci, mi, qi);
-        c += ci, s = fmaf(ci, mi, s);
+// Sums over the rows of threads of entries [row][channel][2] in shared memory: the channels' to entries [channel][2] (and `out`, added
+// to what is there where `add`), and the groups' of them times w to `sums` [group][2] (may be null).  In a fixed order.
+template <typename W>
+__device__ __forceinline__ void join_channels(const GnormArgs& a, int rows, float2* entries, float* out, bool add, float* sums, W&& weight) {
+    const int n = blockDim.x, c = a.channels, parts = max(1, min(n / c, rows));
+    __syncthreads();
+    for (int c0 = 0; c0 < c; c0 += n) {
+        const int ch = parts > 1 ? threadIdx.x % c : c0 + threadIdx.x, part = parts > 1 ? threadIdx.x / c : 0;
+        const bool in = ch < c && part < parts;
+        float2 s = {0.0f, 0.0f};
+        if (in)
+            for (int r = part; r < rows; r += parts) s.x += entries[r * c + ch].x, s.y += entries[r * c + ch].y;
+        if (parts > 1) {
+            __syncthreads();
+            if (in) entries[part * c + ch] = s;
+            __syncthreads();
+            if (part == 0)
+                for (int k = 1; k < parts; ++k) s.x += entries[k * c + ch].x, s.y += entries[k * c + ch].y;
+        }
+        if (in && part == 0) {
+            entries[ch] = s;
+            if (out != nullptr) {
+                float2 o = add ? *reinterpret_cast<float2*>(out + 2 * ch) : make_float2(0.0f, 0.0f);
+                o.x += s.x, o.y += s.y;
+                *reinterpret_cast<float2*>(out + 2 * ch) = o;
+            }
+        }
     }
-    count = warp_sum(c);
-    mean = count > 0.0f ? warp_sum(s) / count : 0.0f;
-    float q = 0.0f;
-    for (int i = lane; i < n; i += 32) {
-        float ci, mi, qi;
-        entry(i, ci, mi, qi);
-        const float d = mi - mean;
-        q += ci > 0.0f ? fmaf(ci * d, d, qi) : 0.0f;
+    if (sums == nullptr) return;
+    __syncthreads();
+    const bool few = a.per_group > 16 && a.groups < n;           // a warp has a group, or a thread
+    const int step = few ? 32 : 1, lane = few ? threadIdx.x & 31 : 0;
+    for (int g = threadIdx.x / step; g < a.groups; g += n / step) {
+        float2 s = {0.0f, 0.0f};
+        for (int i = lane; i < a.per_group; i += step) {
+            const int ch = g * a.per_group + i;
+            const float w = weight(ch);
+            s.x = fmaf(entries[ch].x, w, s.x), s.y = fmaf(entries[ch].y, w, s.y);
+        }
+        if (few) s.x = warp_sum(s.x), s.y = warp_sum(s.y);
+        if (lane == 0) *reinterpret_cast<float2*>(sums + 2 * g) = s;
     }
-    sq = warp_sum(q);
 }
 
 // Sums of one thread's column over its positions, from its first element on
 template <int V>
 struct Moments {
-    float first[V], s[V], q[V];
+    Pairs<V> less, s, q;                         // less: the first element, negative
     int n = 0;
     template <typename T>
     __device__ __forceinline__ void add(const Pack<T, V>& p) {
+        Pairs<V> x;
+        x.from(p);
+        if (n == 0) {
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-            const float v = p.at(e);
-            if (n == 0) first[e] = v, s[e] = 0.0f, q[e] = 0.0f;
-            const float d = v - first[e];
-            s[e] += d, q[e] = fmaf(d, d, q[e]);
+            for (int i = 0; i < Pairs<V>::kN; ++i) less.v[i] = x.v[i] * all_lanes(-1.0f);
+            s.fill(0.0f), q.fill(0.0f);
         }
         ++n;
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) {
+            const Lanes d = x.v[i] + less.v[i];
+            s.v[i] = s.v[i] + d, q.v[i] = fma(d, d, q.v[i]);
+        }
     }
-    __device__ __forceinline__ void put(float* mean, float* sq, float& count) const {
-        count = (float)n;
+    __device__ __forceinline__ void put(float* mean, float* sq) const {
+        const float by = n > 0 ? 1.0f / (float)n : 0.0f;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            const float m = n > 0 ? s[e] / (float)n : 0.0f;
-            mean[e] = n > 0 ? first[e] + m : 0.0f;
-            sq[e] = n > 0 ? fmaxf(q[e] - s[e] * m, 0.0f) : 0.0f;
+            const float m = n > 0 ? s.at(e) * by : 0.0f;
+            mean[e] = n > 0 ? m - less.at(e) : 0.0f;
+            sq[e] = n > 0 ? fmaxf(fmaf(-s.at(e), m, q.at(e)), 0.0f) : 0.0f;
         }
     }
 };
 
-// Means and sums of every group from the threads' own ones in shared memory: entries [row][channel]
-__device__ __forceinline__ void join_groups(const GnormArgs& a, int rows, const float* counts, const float* means, const float* sqs,
-                                            float* out, bool finish) {
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-    for (int g = warp; g < a.groups; g += warps) {
-        float mean, sq, count;
-        join(rows * a.per_group, [&](int i, float& c, float& m, float& q) {
-            const int r = i / a.per_group, ch = g * a.per_group + i % a.per_group;
-            c = counts[r], m = means[r * a.channels + ch], q = sqs[r * a.channels + ch];
-        }, mean, sq, count);
-        if ((threadIdx.x & 31) == 0) {
-            out[2 * g] = mean;
-            out[2 * g + 1] = finish ? rsqrtf(fmaf(sq, a.inv, a.eps)) : sq;
-        }
+// The groups of a thread's channels, one behind the other
+struct GroupOf {
+    int g, left, per;
+    __device__ __forceinline__ GroupOf(const GnormArgs& a, int c0) : g(c0 / a.per_group), left((c0 / a.per_group + 1) * a.per_group - c0), per(a.per_group) {}
+    __device__ __forceinline__ int next() {
+        const int now = g;
+        if (--left == 0) ++g, left = per;
+        return now;
     }
-}
+};
 
-template <typename T, int V>
-__device__ __forceinline__ void apply_vector(const GnormArgs& a, const Pack<T, V>& x, int64_t at, int c0, const float* stats) {
-    Pack<T, V> res, y;
-    if (a.residual != nullptr) res.get(static_cast<const T*>(a.residual) + at);
-    float f[V];
+// The threads' moments as entries of join_channels: counts times means, and squares, about one number of each group, which adds up
+// (the mean of the group's first channel in the first row of threads)
+template <int V>
+__device__ __forceinline__ void put_first(const GnormArgs& a, const Moments<V>& m, int c0, float* about) {
+    float mean[V], sq[V];
+    m.put(mean, sq);
+    GroupOf group(a, c0);
 #pragma unroll
     for (int e = 0; e < V; ++e) {
-        const int c = c0 + e, g = c / a.per_group;
-        const float h = (x.at(e) - stats[2 * g]) * stats[2 * g + 1];
-        float z = fmaf(h, weight_at<T>(a.weight, c, a.wide_weights, 1.0f), weight_at<T>(a.bias, c, a.wide_weights, 0.0f));
-        if (a.residual != nullptr) z += res.at(e);
-        f[e] = activate(z, a.act);
+        const bool first = group.left == a.per_group;
+        const int g = group.next();
+        if (first) about[g] = mean[e];
     }
-    y.set(f);
-    y.put(static_cast<T*>(a.y) + at);
+}
+template <int V>
+__device__ __forceinline__ void put_entries(const GnormArgs& a, const Moments<V>& m, int c0, const float* about, float2* entries) {
+    float mean[V], sq[V];
+    m.put(mean, sq);
+    GroupOf group(a, c0);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        const float d = mean[e] - about[group.next()], n = (float)m.n;
+        entries[e] = make_float2(n * d, fmaf(n * d, d, sq[e]));
+    }
+}
+// Another such number: the middle one of a channel's first, middle and last element, so that one that is far off does no harm
+template <typename T>
+__device__ __forceinline__ float typical(const GnormArgs& a, const T* x, int64_t positions) {
+    Pack<T, 1> p, q, r;
+    p.get(x), q.get(x + positions / 2 * a.channels), r.get(x + (positions - 1) * a.channels);
+    return fmaxf(fminf(p.at(0), q.at(0)), fminf(fmaxf(p.at(0), q.at(0)), r.at(0)));
+}
+// A group's mean and 1 / sqrt(var + eps) from such sums
+__device__ __forceinline__ float2 finish(const GnormArgs& a, float about, float2 s) {
+    const float d = s.x * a.inv;
+    return make_float2(about + d, rsqrtf(fmaf(fmaxf(fmaf(-s.x, d, s.y), 0.0f), a.inv, a.eps)));
+}
+
+// What a thread needs of its channels: z = (x - mean) (r w) + b
+template <typename T, int V>
+struct Channels {
+    Pairs<V> less, rw, b;                        // less: the mean, negative
+    __device__ __forceinline__ void get(const GnormArgs& a, int c0, const float* stats) {
+        GroupOf group(a, c0);
+        float m[V], r[V], w[V];
+        weights_at<T, V>(a.weight, c0, a.wide_weights, 1.0f, r);
+        weights_at<T, V>(a.bias, c0, a.wide_weights, 0.0f, w);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int g = group.next();
+            m[e] = -stats[2 * g];
+            r[e] *= stats[2 * g + 1];
+        }
+        less.map([&](float, int e) { return m[e]; });
+        rw.map([&](float, int e) { return r[e]; });
+        b.map([&](float, int e) { return w[e]; });
+    }
+    __device__ __forceinline__ Pairs<V> z(const Pairs<V>& x, const Pack<T, V>& res, bool residual) const {
+        Pairs<V> out, more;
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) out.v[i] = fma(x.v[i] + less.v[i], rw.v[i], b.v[i]);
+        if (residual) {
+            more.from(res);
+#pragma unroll
+            for (int i = 0; i < Pairs<V>::kN; ++i) out.v[i] = out.v[i] + more.v[i];
+        }
+        return out;
+    }
+};
+
+// A thread's vectors of the next positions, on their way to its own places in shared memory while it works: no barrier, no registers.
+constexpr int kDepth = 8;
+template <typename T, int V>
+struct Ring {
+    static constexpr int kBytes = sizeof(T) * V, kKind = kDepth * kThreads * kBytes;         // kKind: of a tensor
+    char* at;
+    __device__ __forceinline__ Ring(char* smem) : at(smem + threadIdx.x * kBytes) {}
+    __device__ __forceinline__ void issue(int slot, int kind, const T* from) const {
+        char* const to = at + kind * kKind + slot * (kThreads * kBytes);
+        if constexpr (kBytes >= 4) {
+            copy_async_all<kBytes>(to, from);
+        } else {
+            Pack<T, V> p;
+            p.get(from);
+            *reinterpret_cast<Raw<kBytes>*>(to) = p.raw;
+        }
+    }
+    __device__ __forceinline__ void get(Pack<T, V>& p, int slot, int kind) const {
+        const char* const from = at + kind * kKind + slot * (kThreads * kBytes);
+        if constexpr (kBytes >= 4) load_shared(p.raw, from);
+        else p.raw = *reinterpret_cast<const Raw<kBytes>*>(from);
+    }
+};
+// n positions: issue(slot) asks for the next one's vectors, use(slot, ahead) has the oldest one's and calls ahead() when it has read them
+template <typename I>
+__device__ __forceinline__ void stream_begin(int n, I&& issue) {
+#pragma unroll
+    for (int j = 0; j < kDepth - 1; ++j) {
+        if (j < n) issue(j);
+        copies_issued();
+    }
+}
+template <typename I, typename U>
+__device__ __forceinline__ void stream(int n, I&& issue, U&& use) {
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        copies_arrived<kDepth - 2>();
+        use(i % kDepth, [&] {
+            if (i + kDepth - 1 < n) issue((i + kDepth - 1) % kDepth);
+            copies_issued();
+        });
+    }
+    copies_arrived<0>();
 }
 
 // ---- samples that a CTA holds ---------------------------------------------------------------------------------------------
@@ -168,35 +360,54 @@ __global__ void __launch_bounds__(512) gnorm_held_kernel(const GnormArgs a) {
     const Grid grid(a.vectors);
     const int mine = (int)((a.positions + grid.rows - 1) / grid.rows) * grid.blocks;     // vectors of a thread
     Raw<sizeof(T) * V>* const held = reinterpret_cast<Raw<sizeof(T) * V>*>(smem);
-    float* const means = reinterpret_cast<float*>(smem + ((size_t)mine * blockDim.x * sizeof(T) * V + 15) / 16 * 16);
-    float* const sqs = means + grid.rows * a.channels;
-    float* const stats = sqs + grid.rows * a.channels;
-    float* const counts = stats + 2 * a.groups;
+    float2* const entries = reinterpret_cast<float2*>(smem + ((size_t)mine * blockDim.x * sizeof(T) * V + 15) / 16 * 16);
+    float* const stats = reinterpret_cast<float*>(entries + grid.rows * a.channels);
+    float* const about = stats + 2 * a.groups;
     pdl_wait();
     for (int64_t sample = blockIdx.x; sample < a.samples; sample += gridDim.x) {
         const int64_t base = sample * a.positions * a.channels;
-        int k = 0;
-        for (int b = 0; b < grid.blocks; ++b) {
+        auto load = [&](int b, int& k, Moments<V>& m) {
             const int col = grid.col + b * blockDim.x;
-            if (grid.row < 0 || col >= a.vectors) continue;
-            Moments<V> m;
-            for (int64_t p = grid.row; p < a.positions; p += grid.rows, ++k) {
-                Pack<T, V> x;
-                x.get(static_cast<const T*>(a.x) + base + p * a.channels + col * V);
-                m.add(x);
-                held[(size_t)k * blockDim.x + threadIdx.x] = x.raw;
+            const T* const x = static_cast<const T*>(a.x) + base + col * V;
+            int i = 0;
+            for (int64_t p = grid.row; p < a.positions; p += grid.rows, ++i) {
+                if constexpr (sizeof(T) * V >= 4) copy_async_all<sizeof(T) * V>(&held[(size_t)(k + i) * blockDim.x + threadIdx.x], x + p * a.channels);
+                else seq::load(held[(size_t)(k + i) * blockDim.x + threadIdx.x], x + p * a.channels);
             }
-            float mean[V], sq[V], count;
-            m.put(mean, sq, count);
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                means[grid.row * a.channels + col * V + e] = mean[e];
-                sqs[grid.row * a.channels + col * V + e] = sq[e];
+            copies_issued();
+            copies_arrived<0>();
+            for (int j = 0; j < i; ++j, ++k) {
+                Pack<T, V> v;
+                v.raw = held[(size_t)k * blockDim.x + threadIdx.x];
+                m.add(v);
             }
-            if (col == 0) counts[grid.row] = count;
+        };
+        int k = 0;
+        Moments<V> m;
+        auto in = [&](int b) { return grid.row >= 0 && grid.col + b * (int)blockDim.x < a.vectors; };
+        auto own = [&](int b) { return entries + grid.row * a.channels + (grid.col + b * blockDim.x) * V; };
+        if (grid.blocks == 1) {
+            if (in(0)) load(0, k, m);
+            if (grid.row == 0) put_first(a, m, grid.col * V, about);
+            __syncthreads();
+            if (in(0)) put_entries(a, m, grid.col * V, about, own(0));
+        } else {
+            for (int g = threadIdx.x; g < a.groups; g += blockDim.x)
+                about[g] = typical(a, static_cast<const T*>(a.x) + base + g * a.per_group, a.positions);
+            __syncthreads();
+            for (int b = 0; b < grid.blocks; ++b) {
+                if (!in(b)) continue;
+                Moments<V> mb;
+                load(b, k, mb);
+                put_entries(a, mb, (grid.col + b * blockDim.x) * V, about, own(b));
+            }
         }
+        join_channels(a, grid.rows, entries, nullptr, false, stats, [](int) { return 1.0f; });
         __syncthreads();
-        join_groups(a, grid.rows, counts, means, sqs, stats, true);
+        for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
+            const float2 f = finish(a, about[g], make_float2(stats[2 * g], stats[2 * g + 1]));
+            stats[2 * g] = f.x, stats[2 * g + 1] = f.y;
+        }
         __syncthreads();
         if (a.stats != nullptr)
             for (int i = threadIdx.x; i < 2 * a.groups; i += blockDim.x) a.stats[sample * 2 * a.groups + i] = stats[i];
@@ -204,11 +415,50 @@ __global__ void __launch_bounds__(512) gnorm_held_kernel(const GnormArgs a) {
         for (int b = 0; b < grid.blocks; ++b) {
             const int col = grid.col + b * blockDim.x;
             if (grid.row < 0 || col >= a.vectors) continue;
+            Channels<T, V> ch;
+            ch.get(a, col * V, stats);
             for (int64_t p = grid.row; p < a.positions; p += grid.rows, ++k) {
-                Pack<T, V> x;
+                const int64_t at = base + p * a.channels + col * V;
+                Pack<T, V> x, res;
                 x.raw = held[(size_t)k * blockDim.x + threadIdx.x];
-                apply_vector<T, V>(a, x, base + p * a.channels + col * V, col * V, stats);
+                if (a.residual != nullptr) res.get(static_cast<const T*>(a.residual) + at);
+                Pairs<V> v;
+                v.from(x);
+                v = ch.z(v, res, a.residual != nullptr);
+                activate(v, a.act);
+                v.template pack<T>().put(static_cast<T*>(a.y) + at);
             }
+        }
+        __syncthreads();
+    }
+}
+
+// Sums over a sample's splits of f(split, first number, second, first number of split 0) by group, finished by g(group, sums, that
+// number).  Threads share out (group, split); `room` holds two floats of each thread.
+template <typename F, typename G>
+__device__ __forceinline__ void gather_splits(const GnormArgs& a, int64_t sample, float* room, F&& f, G&& finish) {
+    const float* const partial = a.partial + sample * a.splits * 2 * a.groups;
+    const int n = blockDim.x, per = n / a.groups;               // threads of a group (0: each thread has several groups)
+    for (int g0 = 0; g0 < a.groups; g0 += n) {
+        const int g = per > 0 ? threadIdx.x % a.groups : g0 + threadIdx.x, part = per > 0 ? threadIdx.x / a.groups : 0;
+        const bool in = per > 0 ? part < per : g < a.groups;
+        float x = 0.0f, y = 0.0f, m0 = 0.0f;
+        if (in) {
+            m0 = gload(partial + 2 * g);
+#pragma unroll 4
+            for (int i = part; i < a.splits; i += max(per, 1)) {
+                Pack<float, 2> p;
+                p.get(partial + ((int64_t)i * a.groups + g) * 2);
+                float xi, yi;
+                f(i, p.at(0), p.at(1), m0, xi, yi);
+                x += xi, y += yi;
+            }
+        }
+        room[2 * threadIdx.x] = x, room[2 * threadIdx.x + 1] = y;
+        __syncthreads();
+        if (in && part == 0) {
+            for (int k = 1; k < per; ++k) x += room[2 * (threadIdx.x + k * a.groups)], y += room[2 * (threadIdx.x + k * a.groups) + 1];
+            finish(g, x, y, m0);
         }
         __syncthreads();
     }
@@ -216,147 +466,193 @@ __global__ void __launch_bounds__(512) gnorm_held_kernel(const GnormArgs a) {
 
 // ---- two passes -----------------------------------------------------------------------------------------------------------
 template <typename T, int V>
-__global__ void __launch_bounds__(512) gnorm_sums_kernel(const GnormArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) gnorm_sums_kernel(const GnormArgs a) {
     extern __shared__ __align__(16) char smem[];
     const Grid grid(a.vectors);
-    float* const means = reinterpret_cast<float*>(smem);
-    float* const sqs = means + grid.rows * a.channels;
-    float* const counts = sqs + grid.rows * a.channels;
+    const Ring<T, V> ring(smem);
+    // (in the ring's place, once nothing more comes into it)
+    float2* const entries = reinterpret_cast<float2*>(smem + (grid.blocks == 1 ? 0 : ring.kKind));
+    float* const about = reinterpret_cast<float*>(smem + (grid.blocks == 1 ? max((int)ring.kKind, grid.rows * 8 * a.channels) : ring.kKind + 8 * a.channels));
+    float* const sums = about + a.groups + (a.groups & 1);
     pdl_wait();
     const int64_t sample = blockIdx.x / a.splits;
     const int split = blockIdx.x % a.splits;
     const int64_t begin = split * a.split_positions, end = min(begin + a.split_positions, a.positions);
-    const T* const x = static_cast<const T*>(a.x) + sample * a.positions * a.channels;
+    const T* const x = static_cast<const T*>(a.x) + (sample * a.positions + begin) * a.channels;
+    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) about[g] = typical(a, x + g * a.per_group, end - begin);
+    const int n = grid.row < 0 ? 0 : (int)((end - begin - grid.row + grid.rows - 1) / grid.rows);
+    const int64_t step = (int64_t)grid.rows * a.channels;
     for (int b = 0; b < grid.blocks; ++b) {
-        const int col = grid.col + b * blockDim.x;
-        if (grid.row < 0 || col >= a.vectors) continue;
+        const int col = grid.col + b * blockDim.x, mine = col < a.vectors ? n : 0;
         Moments<V> m;
-        int64_t p = begin + grid.row;
-        for (; p + 3 * grid.rows < end; p += 4 * grid.rows) {
-            Pack<T, V> v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i].get(x + (p + i * grid.rows) * a.channels + col * V);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m.add(v[i]);
-        }
-        for (; p < end; p += grid.rows) {
+        const T* next = x + grid.row * a.channels + col * V;
+        auto issue = [&](int slot) {
+            ring.issue(slot, 0, next);
+            next += step;
+        };
+        stream_begin(mine, issue);
+        stream(mine, issue, [&](int slot, auto&& ahead) {
             Pack<T, V> v;
-            v.get(x + p * a.channels + col * V);
+            ring.get(v, slot, 0);
+            ahead();
             m.add(v);
-        }
-        float mean[V], sq[V], count;
-        m.put(mean, sq, count);
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            means[grid.row * a.channels + col * V + e] = mean[e];
-            sqs[grid.row * a.channels + col * V + e] = sq[e];
-        }
-        if (col == 0) counts[grid.row] = count;
+        });
+        if (grid.blocks == 1 || b == 0) __syncthreads();
+        if (grid.row >= 0 && col < a.vectors) put_entries(a, m, col * V, about, entries + grid.row * a.channels + col * V);
     }
+    join_channels(a, grid.rows, entries, nullptr, false, sums, [](int) { return 1.0f; });
     __syncthreads();
-    join_groups(a, grid.rows, counts, means, sqs, a.partial + (int64_t)blockIdx.x * 2 * a.groups, false);
+    // of a split: its mean, and its squares about that
+    float* const out = a.partial + (int64_t)blockIdx.x * 2 * a.groups;
+    const float by = 1.0f / ((float)(end - begin) * (float)a.per_group);
+    for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
+        const float d = sums[2 * g] * by;
+        out[2 * g] = about[g] + d, out[2 * g + 1] = fmaxf(fmaf(-sums[2 * g], d, sums[2 * g + 1]), 0.0f);
+    }
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(512) gnorm_apply_kernel(const GnormArgs a) {
+__global__ void __launch_bounds__(kThreads, 3) gnorm_apply_kernel(const GnormArgs a) {
     extern __shared__ __align__(16) char smem[];
-    float* const stats = reinterpret_cast<float*>(smem);
+    const int kinds = a.residual != nullptr ? 2 : 1;
+    const Ring<T, V> ring(smem);
+    float* const stats = reinterpret_cast<float*>(smem + kinds * ring.kKind);
     const Grid grid(a.vectors);
     const int64_t block = gridDim.x - 1 - blockIdx.x, sample = block / a.splits;
     const int split = (int)(block % a.splits);
     const int64_t begin = split * a.split_positions, end = min(begin + a.split_positions, a.positions);
+    const int n = grid.row < 0 ? 0 : (int)((end - begin - grid.row + grid.rows - 1) / grid.rows);
+    const int64_t first = (sample * a.positions + begin + grid.row) * a.channels, step = (int64_t)grid.rows * a.channels;
+    const T *x, *res;
+    auto issue = [&](int slot) {
+        ring.issue(slot, 0, x);
+        x += step;
+        if (kinds == 2) ring.issue(slot, 1, res), res += step;
+    };
+    auto start = [&](int b) {
+        const int col = grid.col + b * blockDim.x;
+        x = static_cast<const T*>(a.x) + first + col * V, res = static_cast<const T*>(a.residual) + first + col * V;
+        stream_begin(col < a.vectors ? n : 0, issue);
+    };
     pdl_wait();
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-    const float* const partial = a.partial + sample * a.splits * 2 * a.groups;
-    for (int g = warp; g < a.groups; g += warps) {
-        float mean, sq, count;
-        join(a.splits, [&](int i, float& c, float& m, float& q) {
-            const int64_t from = i * a.split_positions;
-            c = (float)((min(from + a.split_positions, a.positions) - from) * a.per_group);
-            m = gload(partial + (int64_t)i * 2 * a.groups + 2 * g), q = gload(partial + (int64_t)i * 2 * a.groups + 2 * g + 1);
-        }, mean, sq, count);
-        if ((threadIdx.x & 31) == 0) stats[2 * g] = mean, stats[2 * g + 1] = rsqrtf(fmaf(sq, a.inv, a.eps));
-    }
-    __syncthreads();
+    start(0);
+    // the splits' statistics, about the first one's mean: their means differ by little
+    gather_splits(a, sample, stats + 2 * a.groups, [&](int i, float m, float q, float m0, float& sx, float& sy) {
+        const int64_t from = i * a.split_positions;
+        const float c = (float)((min(from + a.split_positions, a.positions) - from) * a.per_group), d = m - m0;
+        sx = c * d, sy = fmaf(c * d, d, q);
+    }, [&](int g, float sx, float sy, float m0) {
+        const float2 f = finish(a, m0, make_float2(sx, sy));
+        stats[2 * g] = f.x, stats[2 * g + 1] = f.y;
+    });
     if (a.stats != nullptr && split == 0)
         for (int i = threadIdx.x; i < 2 * a.groups; i += blockDim.x) a.stats[sample * 2 * a.groups + i] = stats[i];
-    const int64_t base = sample * a.positions * a.channels;
     for (int b = 0; b < grid.blocks; ++b) {
+        if (b > 0) start(b);
         const int col = grid.col + b * blockDim.x;
         if (grid.row < 0 || col >= a.vectors) continue;
-        for (int64_t p = begin + grid.row; p < end; p += grid.rows) {
-            Pack<T, V> x;
-            x.get(static_cast<const T*>(a.x) + base + p * a.channels + col * V);
-            apply_vector<T, V>(a, x, base + p * a.channels + col * V, col * V, stats);
-        }
+        Channels<T, V> ch;
+        ch.get(a, col * V, stats);
+        T* y = static_cast<T*>(a.y) + first + col * V;
+        stream(n, issue, [&](int slot, auto&& ahead) {
+            Pack<T, V> v, r;
+            ring.get(v, slot, 0);
+            if (kinds == 2) ring.get(r, slot, 1);
+            ahead();
+            Pairs<V> z;
+            z.from(v);
+            z = ch.z(z, r, kinds == 2);
+            activate(z, a.act);
+            z.template pack<T>().put(y);
+            y += step;
+        });
     }
 }
 
 // ---- gradients ------------------------------------------------------------------------------------------------------------
-// dz and h of a vector
-template <typename T, int V>
-__device__ __forceinline__ void gradients_of(const GnormArgs& a, const Pack<T, V>& x, const Pack<T, V>& dy, const Pack<T, V>& res, int c0,
-                                             const float* stats, float (&dz)[V], float (&h)[V]) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int c = c0 + e, g = c / a.per_group;
-        h[e] = (x.at(e) - stats[2 * g]) * stats[2 * g + 1];
-        float z = fmaf(h[e], weight_at<T>(a.weight, c, a.wide_weights, 1.0f), weight_at<T>(a.bias, c, a.wide_weights, 0.0f));
-        if (a.residual != nullptr) z += res.at(e);
-        dz[e] = activate_gradient(z, dy.at(e), a.act);
-    }
-}
-
+// With d = x - mean: sums of dz and of dz d (h is d r);   dx = dz (r w) - (s1 + d s2), s1 = r mean(dz w), s2 = r^2 mean(dz w h)
 template <typename T, int V>
 struct Loads {
     Pack<T, V> x, dy, res;
+    __device__ __forceinline__ void get(const GnormArgs& a, const Ring<T, V>& ring, int slot) {
+        ring.get(x, slot, 0), ring.get(dy, slot, 1);
+        if (a.residual != nullptr) ring.get(res, slot, 2);
+    }
     __device__ __forceinline__ void get(const GnormArgs& a, int64_t at) {
         x.get(static_cast<const T*>(a.x) + at);
         dy.get(static_cast<const T*>(a.dy) + at);
         if (a.residual != nullptr) res.get(static_cast<const T*>(a.residual) + at);
     }
+    // dz, and x - mean
+    __device__ __forceinline__ Pairs<V> gradient(const GnormArgs& a, const Channels<T, V>& ch, Pairs<V>& d) const {
+        Pairs<V> g, z;
+        d.from(x), g.from(dy);
+        if (a.act != DCN_ACT_NONE) z = ch.z(d, res, a.residual != nullptr);
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) d.v[i] = d.v[i] + ch.less.v[i];
+        return activate_gradient(z, g, a.act);
+    }
+};
+
+// The next position's vectors of x, dy and the residual
+template <typename T, int V>
+struct Sources {
+    const T *x, *dy, *res;
+    int64_t step;
+    __device__ __forceinline__ Sources(const GnormArgs& a, int64_t at, int64_t step_)
+        : x(static_cast<const T*>(a.x) + at), dy(static_cast<const T*>(a.dy) + at),
+          res(a.residual != nullptr ? static_cast<const T*>(a.residual) + at : nullptr), step(step_) {}
+    __device__ __forceinline__ void issue(const Ring<T, V>& ring, int slot) {
+        ring.issue(slot, 0, x), ring.issue(slot, 1, dy);
+        x += step, dy += step;
+        if (res != nullptr) ring.issue(slot, 2, res), res += step;
+    }
 };
 
 template <typename T, int V>
-__device__ __forceinline__ void put_gradients(const GnormArgs& a, const Loads<T, V>& v, int64_t at, int c0, const float* stats,
-                                              const float* sums) {
-    float dz[V], h[V], dx[V];
-    gradients_of<T, V>(a, v.x, v.dy, v.res, c0, stats, dz, h);
+struct Sums {
+    Pairs<V> s, q;
+    __device__ __forceinline__ Sums() { s.fill(0.0f), q.fill(0.0f); }
+    __device__ __forceinline__ void add(const GnormArgs& a, const Channels<T, V>& ch, const Loads<T, V>& v) {
+        Pairs<V> d;
+        const Pairs<V> dz = v.gradient(a, ch, d);
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-        const int c = c0 + e, g = c / a.per_group;
-        const float dh = dz[e] * weight_at<T>(a.weight, c, a.wide_weights, 1.0f);
-        dx[e] = stats[2 * g + 1] * (dh - sums[2 * g] * a.inv - h[e] * (sums[2 * g + 1] * a.inv));
+        for (int i = 0; i < Pairs<V>::kN; ++i) s.v[i] = s.v[i] + dz.v[i], q.v[i] = fma(dz.v[i], d.v[i], q.v[i]);
     }
-    Pack<T, V> o;
-    if (a.dx != nullptr) o.set(dx), o.put(static_cast<T*>(a.dx) + at);
-    if (a.dresidual != nullptr) o.set(dz), o.put(static_cast<T*>(a.dresidual) + at);
-}
+    // to [channel][2] as sums of dz and dz h
+    __device__ __forceinline__ void put(const GnormArgs& a, int c0, const float* stats, float2* out) const {
+        GroupOf group(a, c0);
+#pragma unroll
+        for (int e = 0; e < V; ++e) out[e] = make_float2(s.at(e), q.at(e) * stats[2 * group.next() + 1]);
+    }
+};
 
-// Channels' sums of dz and dz h over the rows of threads, from shared memory [row][channel][2], to `out` [channel][2], and the groups'
-// sums of them times w to `sums` [group][2] (may be null)
-template <typename T>
-__device__ __forceinline__ void join_channels(const GnormArgs& a, int rows, float* entries, float* out, bool add, float* sums) {
-    for (int i = threadIdx.x; i < 2 * a.channels; i += blockDim.x) {
-        float s = 0.0f;
-        for (int r = 0; r < rows; ++r) s += entries[r * 2 * a.channels + i];
-        entries[i] = s;
-        if (out != nullptr) out[i] = add ? out[i] + s : s;
-    }
-    if (sums == nullptr) return;
-    __syncthreads();
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-    for (int g = warp; g < a.groups; g += warps) {
-        float s = 0.0f, q = 0.0f;
-        for (int i = threadIdx.x & 31; i < a.per_group; i += 32) {
-            const int c = g * a.per_group + i;
-            const float w = weight_at<T>(a.weight, c, a.wide_weights, 1.0f);
-            s = fmaf(entries[2 * c], w, s), q = fmaf(entries[2 * c + 1], w, q);
+template <typename T, int V>
+struct Gradient {
+    Channels<T, V> ch;
+    Pairs<V> s1, s2;                             // negative
+    __device__ __forceinline__ void get(const GnormArgs& a, int c0, const float* stats, const float* sums) {
+        ch.get(a, c0, stats);
+        GroupOf group(a, c0);
+        float p[V], q[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            const int g = group.next();
+            const float r = stats[2 * g + 1];
+            p[e] = -r * (sums[2 * g] * a.inv), q[e] = -r * r * (sums[2 * g + 1] * a.inv);
         }
-        s = warp_sum(s), q = warp_sum(q);
-        if ((threadIdx.x & 31) == 0) sums[2 * g] = s, sums[2 * g + 1] = q;
+        s1.map([&](float, int e) { return p[e]; });
+        s2.map([&](float, int e) { return q[e]; });
     }
-}
+    __device__ __forceinline__ void put(const GnormArgs& a, const Loads<T, V>& v, int64_t at) const {
+        Pairs<V> d, dx;
+        const Pairs<V> dz = v.gradient(a, ch, d);
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) dx.v[i] = fma(dz.v[i], ch.rw.v[i], fma(d.v[i], s2.v[i], s1.v[i]));
+        if (a.dx != nullptr) dx.template pack<T>().put(static_cast<T*>(a.dx) + at);
+        if (a.dresidual != nullptr) dz.template pack<T>().put(static_cast<T*>(a.dresidual) + at);
+    }
+};
 
 template <typename T, int V>
 __global__ void __launch_bounds__(512) gnorm_held_backward_kernel(const GnormArgs a) {
@@ -365,8 +661,8 @@ __global__ void __launch_bounds__(512) gnorm_held_backward_kernel(const GnormArg
     const int mine = (int)((a.positions + grid.rows - 1) / grid.rows) * grid.blocks;
     const int kinds = a.residual != nullptr ? 3 : 2;
     Raw<sizeof(T) * V>* const held = reinterpret_cast<Raw<sizeof(T) * V>*>(smem);
-    float* const entries = reinterpret_cast<float*>(smem + ((size_t)mine * kinds * blockDim.x * sizeof(T) * V + 15) / 16 * 16);
-    float* const stats = entries + grid.rows * 2 * a.channels;
+    float2* const entries = reinterpret_cast<float2*>(smem + ((size_t)mine * kinds * blockDim.x * sizeof(T) * V + 15) / 16 * 16);
+    float* const stats = reinterpret_cast<float*>(entries + grid.rows * a.channels);
     float* const sums = stats + 2 * a.groups;
     float* const total = sums + 2 * a.groups;    // [channels][2] of all the CTA's samples
     for (int i = threadIdx.x; i < 2 * a.channels; i += blockDim.x) total[i] = 0.0f;
@@ -379,152 +675,158 @@ __global__ void __launch_bounds__(512) gnorm_held_backward_kernel(const GnormArg
         for (int b = 0; b < grid.blocks; ++b) {
             const int col = grid.col + b * blockDim.x;
             if (grid.row < 0 || col >= a.vectors) continue;
-            float s[V] = {}, q[V] = {};
+            Channels<T, V> ch;
+            ch.get(a, col * V, stats);
+            Sums<T, V> sum;
             for (int64_t p = grid.row; p < a.positions; p += grid.rows, ++k) {
                 Loads<T, V> v;
                 v.get(a, base + p * a.channels + col * V);
-                float dz[V], h[V];
-                gradients_of<T, V>(a, v.x, v.dy, v.res, col * V, stats, dz, h);
-#pragma unroll
-                for (int e = 0; e < V; ++e) s[e] += dz[e], q[e] = fmaf(dz[e], h[e], q[e]);
+                sum.add(a, ch, v);
                 held[(size_t)(kinds * k) * blockDim.x + threadIdx.x] = v.x.raw;
                 held[(size_t)(kinds * k + 1) * blockDim.x + threadIdx.x] = v.dy.raw;
                 if (kinds == 3) held[(size_t)(kinds * k + 2) * blockDim.x + threadIdx.x] = v.res.raw;
             }
-#pragma unroll
-            for (int e = 0; e < V; ++e) {
-                entries[(grid.row * a.channels + col * V + e) * 2] = s[e];
-                entries[(grid.row * a.channels + col * V + e) * 2 + 1] = q[e];
-            }
+            sum.put(a, col * V, stats, entries + grid.row * a.channels + col * V);
         }
-        __syncthreads();
-        join_channels<T>(a, grid.rows, entries, total, true, sums);
+        join_channels(a, grid.rows, entries, total, true, sums, [&](int c) { return weight_at<T>(a.weight, c, a.wide_weights, 1.0f); });
         __syncthreads();
         k = 0;
         if (a.dx != nullptr || a.dresidual != nullptr)
             for (int b = 0; b < grid.blocks; ++b) {
                 const int col = grid.col + b * blockDim.x;
                 if (grid.row < 0 || col >= a.vectors) continue;
+                Gradient<T, V> gr;
+                gr.get(a, col * V, stats, sums);
                 for (int64_t p = grid.row; p < a.positions; p += grid.rows, ++k) {
                     Loads<T, V> v;
                     v.x.raw = held[(size_t)(kinds * k) * blockDim.x + threadIdx.x];
                     v.dy.raw = held[(size_t)(kinds * k + 1) * blockDim.x + threadIdx.x];
                     if (kinds == 3) v.res.raw = held[(size_t)(kinds * k + 2) * blockDim.x + threadIdx.x];
-                    put_gradients<T, V>(a, v, base + p * a.channels + col * V, col * V, stats, sums);
+                    gr.put(a, v, base + p * a.channels + col * V);
                 }
             }
         __syncthreads();
     }
-    if (a.partial != nullptr)
-        for (int i = threadIdx.x; i < 2 * a.channels; i += blockDim.x) a.partial[(int64_t)blockIdx.x * 2 * a.channels + i] = total[i];
+    for (int i = threadIdx.x; i < 2 * a.channels; i += blockDim.x) a.channel_sums[(int64_t)blockIdx.x * 2 * a.channels + i] = total[i];
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(512) gnorm_sums_backward_kernel(const GnormArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) gnorm_sums_backward_kernel(const GnormArgs a) {
     extern __shared__ __align__(16) char smem[];
     const Grid grid(a.vectors);
-    float* const entries = reinterpret_cast<float*>(smem);
-    float* const stats = entries + grid.rows * 2 * a.channels;
+    const Ring<T, V> ring(smem);
+    const int room = (a.residual != nullptr ? 3 : 2) * ring.kKind;
+    float2* const entries = reinterpret_cast<float2*>(smem + (grid.blocks == 1 ? 0 : room));       // (as in the forward pass)
+    float* const stats = reinterpret_cast<float*>(smem + (grid.blocks == 1 ? max(room, grid.rows * 8 * a.channels) : room + 8 * a.channels));
     pdl_wait();
     const int64_t sample = blockIdx.x / a.splits;
     const int split = blockIdx.x % a.splits;
     const int64_t begin = split * a.split_positions, end = min(begin + a.split_positions, a.positions);
-    const int64_t base = sample * a.positions * a.channels;
-    for (int i = threadIdx.x; i < 2 * a.groups; i += blockDim.x) stats[i] = gload(a.stats + sample * 2 * a.groups + i);
-    __syncthreads();
+    const int n = grid.row < 0 ? 0 : (int)((end - begin - grid.row + grid.rows - 1) / grid.rows);
+    const int64_t first = (sample * a.positions + begin + grid.row) * a.channels;
     for (int b = 0; b < grid.blocks; ++b) {
-        const int col = grid.col + b * blockDim.x;
-        if (grid.row < 0 || col >= a.vectors) continue;
-        float s[V] = {}, q[V] = {};
-        for (int64_t p = begin + grid.row; p < end; p += grid.rows) {
-            Loads<T, V> v;
-            v.get(a, base + p * a.channels + col * V);
-            float dz[V], h[V];
-            gradients_of<T, V>(a, v.x, v.dy, v.res, col * V, stats, dz, h);
-#pragma unroll
-            for (int e = 0; e < V; ++e) s[e] += dz[e], q[e] = fmaf(dz[e], h[e], q[e]);
+        const int col = grid.col + b * blockDim.x, mine = col < a.vectors ? n : 0;
+        Sources<T, V> from(a, first + col * V, (int64_t)grid.rows * a.channels);
+        auto issue = [&](int slot) { from.issue(ring, slot); };
+        stream_begin(mine, issue);
+        if (b == 0) {
+            for (int i = threadIdx.x; i < 2 * a.groups; i += blockDim.x) stats[i] = gload(a.stats + sample * 2 * a.groups + i);
+            __syncthreads();
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-            entries[(grid.row * a.channels + col * V + e) * 2] = s[e];
-            entries[(grid.row * a.channels + col * V + e) * 2 + 1] = q[e];
+        Sums<T, V> sum;
+        if (mine > 0) {
+            Channels<T, V> ch;
+            ch.get(a, col * V, stats);
+            stream(mine, issue, [&](int slot, auto&& ahead) {
+                Loads<T, V> v;
+                v.get(a, ring, slot);
+                ahead();
+                sum.add(a, ch, v);
+            });
         }
+        if (grid.blocks == 1) __syncthreads();
+        if (grid.row >= 0 && col < a.vectors) sum.put(a, col * V, stats, entries + grid.row * a.channels + col * V);
     }
-    __syncthreads();
-    join_channels<T>(a, grid.rows, entries, a.partial + (int64_t)blockIdx.x * 2 * a.channels, false, nullptr);
+    join_channels(a, grid.rows, entries, a.channel_sums + (int64_t)blockIdx.x * 2 * a.channels, false,
+                  a.partial + (int64_t)blockIdx.x * 2 * a.groups, [&](int c) { return weight_at<T>(a.weight, c, a.wide_weights, 1.0f); });
 }
 
-// A sample's group sums from its splits' channel sums
+// dw and db of 32 channels: sums of n partial ones [n][channels][2], in a fixed order
 template <typename T>
-__global__ void __launch_bounds__(256) gnorm_join_kernel(const GnormArgs a) {
-    pdl_wait();
-    const int64_t sample = blockIdx.x;
-    const float* const partial = a.partial + sample * a.splits * 2 * a.channels;
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5;
-    for (int g = blockIdx.y * warps + warp; g < a.groups; g += gridDim.y * warps) {
-        float s = 0.0f, q = 0.0f;
-        for (int i = threadIdx.x & 31; i < a.per_group * a.splits; i += 32) {
-            const int c = g * a.per_group + i % a.per_group, split = i / a.per_group;
-            const float w = weight_at<T>(a.weight, c, a.wide_weights, 1.0f);
-            const float* const p = partial + ((int64_t)split * a.channels + c) * 2;
-            s = fmaf(gload(p), w, s), q = fmaf(gload(p + 1), w, q);
+__device__ __forceinline__ void weight_gradients(const GnormArgs& a, int block, int64_t n, float* room) {
+    const int rows = blockDim.x / 32, lane = threadIdx.x % 32, row = threadIdx.x / 32, c = block * 32 + lane;
+    Lanes sum = all_lanes(0.0f);
+    if (c < a.channels && row < rows) {
+#pragma unroll 8
+        for (int64_t i = row; i < n; i += rows) {
+            Pack<float, 2> p;
+            p.get(a.channel_sums + (i * a.channels + c) * 2);
+            const float f[2] = {p.at(0), p.at(1)};
+            sum = sum + lanes(f);
         }
-        s = warp_sum(s), q = warp_sum(q);
-        if ((threadIdx.x & 31) == 0) a.sums[(sample * a.groups + g) * 2] = s, a.sums[(sample * a.groups + g) * 2 + 1] = q;
     }
+    room[2 * threadIdx.x] = sum.at(0), room[2 * threadIdx.x + 1] = sum.at(1);
+    __syncthreads();
+    if (row != 0 || c >= a.channels) return;
+    float s = 0.0f, q = 0.0f;
+    for (int k = 0; k < rows; ++k) s += room[2 * (k * 32 + lane)], q += room[2 * (k * 32 + lane) + 1];
+    auto put = [&](void* p, float v) {
+        if (p == nullptr) return;
+        if (a.wide_weights) static_cast<float*>(p)[c] = v;
+        else static_cast<T*>(p)[c] = from_float<T>(v);
+    };
+    put(a.dweight, q), put(a.dbias, s);
 }
 
 template <typename T, int V>
-__global__ void __launch_bounds__(512) gnorm_apply_backward_kernel(const GnormArgs a) {
+__global__ void __launch_bounds__(kThreads, 2) gnorm_apply_backward_kernel(const GnormArgs a) {
     extern __shared__ __align__(16) char smem[];
-    float* const stats = reinterpret_cast<float*>(smem);
+    const Ring<T, V> ring(smem);
+    float* const stats = reinterpret_cast<float*>(smem + (a.residual != nullptr ? 3 : 2) * ring.kKind);
     float* const sums = stats + 2 * a.groups;
     const Grid grid(a.vectors);
+    const int first = a.dweight != nullptr || a.dbias != nullptr ? (a.channels + 31) / 32 : 0;      // blocks for these
+    pdl_wait();
+    if ((int)blockIdx.x < first) {
+        weight_gradients<T>(a, blockIdx.x, a.samples * a.splits, stats);
+        return;
+    }
     const int64_t block = gridDim.x - 1 - blockIdx.x, sample = block / a.splits;
     const int split = (int)(block % a.splits);
     const int64_t begin = split * a.split_positions, end = min(begin + a.split_positions, a.positions);
-    pdl_wait();
-    for (int i = threadIdx.x; i < 2 * a.groups; i += blockDim.x) {
-        stats[i] = gload(a.stats + sample * 2 * a.groups + i);
-        sums[i] = gload(a.sums + sample * 2 * a.groups + i);
-    }
-    __syncthreads();
-    const int64_t base = sample * a.positions * a.channels;
+    const int n = grid.row < 0 ? 0 : (int)((end - begin - grid.row + grid.rows - 1) / grid.rows);
+    const int64_t at = (sample * a.positions + begin + grid.row) * a.channels, step = (int64_t)grid.rows * a.channels;
+    Sources<T, V> from(a, at + grid.col * V, step);
+    auto issue = [&](int slot) { from.issue(ring, slot); };
+    stream_begin(grid.col < a.vectors ? n : 0, issue);
+    for (int i = threadIdx.x; i < 2 * a.groups; i += blockDim.x) stats[i] = gload(a.stats + sample * 2 * a.groups + i);
+    gather_splits(a, sample, sums + 2 * a.groups, [&](int, float p, float q, float, float& x, float& y) { x = p, y = q; },
+                  [&](int g, float x, float y, float) { sums[2 * g] = x, sums[2 * g + 1] = y; });
     for (int b = 0; b < grid.blocks; ++b) {
         const int col = grid.col + b * blockDim.x;
-        if (grid.row < 0 || col >= a.vectors) continue;
-        for (int64_t p = begin + grid.row; p < end; p += grid.rows) {
-            const int64_t at = base + p * a.channels + col * V;
-            Loads<T, V> v;
-            v.get(a, at);
-            put_gradients<T, V>(a, v, at, col * V, stats, sums);
+        if (b > 0) {
+            from = Sources<T, V>(a, at + col * V, step);
+            stream_begin(col < a.vectors ? n : 0, issue);
         }
+        if (grid.row < 0 || col >= a.vectors) continue;
+        Gradient<T, V> gr;
+        gr.get(a, col * V, stats, sums);
+        int64_t to = at + col * V;
+        stream(n, issue, [&](int slot, auto&& ahead) {
+            Loads<T, V> v;
+            v.get(a, ring, slot);
+            ahead();
+            gr.put(a, v, to);
+            to += step;
+        });
     }
 }
 
-// dw and db: sums of n partial ones [n][channels][2], in a fixed order
 template <typename T>
-__global__ void __launch_bounds__(1024) gnorm_weights_kernel(const float* partial, int64_t n, int channels, void* dw, void* db, int wide) {
-    __shared__ float s[32][33], q[32][33];
-    const int c = blockIdx.x * 32 + threadIdx.x;
+__global__ void __launch_bounds__(512) gnorm_weights_kernel(const GnormArgs a, int64_t n) {
+    extern __shared__ __align__(16) char smem[];
     pdl_wait();
-    float a = 0.0f, b = 0.0f;
-    if (c < channels)
-        for (int64_t i = threadIdx.y; i < n; i += 32) a += gload(partial + (i * channels + c) * 2), b += gload(partial + (i * channels + c) * 2 + 1);
-    s[threadIdx.x][threadIdx.y] = a, q[threadIdx.x][threadIdx.y] = b;
-    __syncthreads();
-    a = warp_sum(s[threadIdx.y][threadIdx.x]), b = warp_sum(q[threadIdx.y][threadIdx.x]);
-    const int mine = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && mine < channels) {
-        if (db != nullptr) {
-            if (wide) static_cast<float*>(db)[mine] = a;
-            else static_cast<T*>(db)[mine] = from_float<T>(a);
-        }
-        if (dw != nullptr) {
-            if (wide) static_cast<float*>(dw)[mine] = b;
-            else static_cast<T*>(dw)[mine] = from_float<T>(b);
-        }
-    }
+    weight_gradients<T>(a, blockIdx.x, n, reinterpret_cast<float*>(smem));
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------------
@@ -545,7 +847,7 @@ struct Plan {
     int threads, rows, blocks, splits;
     int64_t split_positions, ctas;
     bool held;
-    size_t smem;
+    size_t smem, ring;                           // ring: of one tensor
 };
 
 Plan plan_of(const dcn_gnorm* p, int v, bool backward, bool residual) {
@@ -567,23 +869,30 @@ Plan plan_of(const dcn_gnorm* p, int v, bool backward, bool residual) {
     lay(threads);
     const int64_t mine = (p->positions + r.rows - 1) / r.rows * r.blocks;
     const size_t data = ((size_t)mine * kinds * r.threads * e * v + 15) / 16 * 16;
-    const size_t more = ((size_t)r.rows * 2 * c + 4 * p->groups + (backward ? 2 * c : r.rows)) * 4;
-    if (mine < (1 << 20) && data <= kHeldBytes && data + more <= 200 * 1024) {
+    const size_t held_sums = ((size_t)r.rows * 2 * c + 4 * p->groups + (backward ? 2 * c : 0)) * 4;
+    if (mine < (1 << 20) && data <= kHeldBytes && data + held_sums <= 200 * 1024) {
         r.held = true;
-        r.smem = data + more;
+        r.smem = data + held_sums;
         const int64_t per_sm = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(2048 / r.threads, 16), 220 * 1024 / (r.smem + 1024)));
         r.ctas = std::max<int64_t>(1, std::min<int64_t>(p->samples, per_sm * sm_count()));
         r.splits = 1;
         return r;
     }
-    lay(vectors > 256 && vectors <= 512 ? (vectors + 31) / 32 * 32 : 256);
-    const int64_t target = (int64_t)sm_count() * 8;
-    const int64_t most = std::max<int64_t>(1, p->positions / (8 * r.rows));
-    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, (target + p->samples - 1) / std::max<int64_t>(1, p->samples)));
+    // One wave of CTAs, each with eight positions a thread or more, and so much of x that the splits' statistics, which each CTA of
+    // the second pass reads, are an eighth of it: splits * groups * 8 bytes <= positions / splits * channels * e / 8
+    const int blocks = (vectors + kThreads - 1) / kThreads, width = (vectors + blocks - 1) / blocks;
+    lay((kThreads / width * width + 31) / 32 * 32);
+    const int64_t target = (int64_t)sm_count() * ((backward ? 2 : 3) * kThreads / r.threads);
+    int64_t most = std::max<int64_t>(1, p->positions / (8 * r.rows));
+    while (most > 1 && most * most > p->positions * c * e / (64 * p->groups)) most = most * 7 / 8;
+    r.splits = (int)std::max<int64_t>(1, std::min<int64_t>(most, target / std::max<int64_t>(1, p->samples)));
     r.split_positions = (p->positions + r.splits - 1) / r.splits;
     r.splits = (int)((p->positions + r.split_positions - 1) / r.split_positions);
     r.ctas = p->samples * r.splits;
-    r.smem = ((size_t)r.rows * 2 * c + (backward ? 2 * p->groups : r.rows)) * 4;
+    r.ring = (size_t)kDepth * kThreads * e * v;
+    const size_t sums = (size_t)r.rows * 2 * c * 4, more = (size_t)(backward ? 2 : 4) * p->groups * 4 + 8;
+    if (backward) r.smem = r.blocks == 1 ? std::max(kinds * r.ring, sums) + more : kinds * r.ring + sums + more;
+    else r.smem = (r.blocks == 1 ? std::max(r.ring, sums) : r.ring + sums) + more;
     return r;
 }
 
@@ -618,25 +927,22 @@ template <typename T, int V>
 int forward_as(const GnormArgs& a, const Plan& r, cudaStream_t st) {
     if (r.held) return launch_gnorm(gnorm_held_kernel<T, V>, r.ctas, r, r.smem, a, st);
     const int rc = launch_gnorm(gnorm_sums_kernel<T, V>, r.ctas, r, r.smem, a, st);
-    return rc != DCN_OK ? rc : launch_gnorm(gnorm_apply_kernel<T, V>, r.ctas, r, 2 * a.groups * 4, a, st);
+    return rc != DCN_OK ? rc : launch_gnorm(gnorm_apply_kernel<T, V>, r.ctas, r, (a.residual != nullptr ? 2 : 1) * r.ring + (2 * a.groups + 2 * r.threads) * 4, a, st);
 }
 
 template <typename T, int V>
-int backward_as(const GnormArgs& a, const Plan& r, void* dw, void* db, cudaStream_t st) {
-    int rc;
-    if (r.held) {
-        rc = launch_gnorm(gnorm_held_backward_kernel<T, V>, r.ctas, r, r.smem, a, st);
-    } else {
-        rc = launch_gnorm(gnorm_sums_backward_kernel<T, V>, r.ctas, r, r.smem, a, st);
-        if (rc == DCN_OK && (a.dx != nullptr || a.dresidual != nullptr)) {
-            const dim3 grid((unsigned)a.samples, (unsigned)std::min(8, (a.groups + 7) / 8));
-            if (launch_dependent(gnorm_join_kernel<T>, grid, dim3(256), 0, st, a) != cudaSuccess) return DCN_ERR_CUDA;
-            rc = launch_gnorm(gnorm_apply_backward_kernel<T, V>, r.ctas, r, 4 * a.groups * 4, a, st);
-        }
-    }
-    if (rc != DCN_OK || (dw == nullptr && db == nullptr)) return rc;
-    return launch_dependent(gnorm_weights_kernel<T>, dim3((a.channels + 31) / 32), dim3(32, 32), 0, st, (const float*)a.partial,
-                            r.held ? r.ctas : a.samples * a.splits, a.channels, dw, db, a.wide_weights) != cudaSuccess
+int backward_as(const GnormArgs& a, const Plan& r, cudaStream_t st) {
+    const bool weights = a.dweight != nullptr || a.dbias != nullptr, data = a.dx != nullptr || a.dresidual != nullptr;
+    const int blocks = weights ? (a.channels + 31) / 32 : 0;
+    const size_t room = (a.residual != nullptr ? 3 : 2) * r.ring + 2 * r.threads * 4;
+    const int rc = r.held ? launch_gnorm(gnorm_held_backward_kernel<T, V>, r.ctas, r, r.smem, a, st)
+                          : launch_gnorm(gnorm_sums_backward_kernel<T, V>, r.ctas, r, r.smem, a, st);
+    if (rc != DCN_OK || (!weights && r.held)) return rc;
+    if (!r.held && data)
+        return launch_gnorm(gnorm_apply_backward_kernel<T, V>, blocks + r.ctas, r, 4 * a.groups * 4 + room, a, st);
+    if (!weights) return DCN_OK;
+    return launch_dependent(gnorm_weights_kernel<T>, dim3(blocks), dim3(512), 2 * 512 * 4, st, a, r.held ? r.ctas : a.samples * a.splits) !=
+                   cudaSuccess
                ? DCN_ERR_CUDA
                : DCN_OK;
 }
@@ -665,8 +971,8 @@ size_t gnorm_bytes(const dcn_gnorm* p, bool backward) {
         for (int residual = 0; residual < (backward ? 2 : 1); ++residual) {
             const Plan r = plan_of(p, v, backward, residual != 0);
             size_t n = 0;
-            if (backward) n = up256((size_t)r.ctas * 2 * p->channels * 4) + (r.held ? 0 : up256((size_t)p->samples * p->groups * 8));
-            else if (!r.held) n = up256((size_t)r.ctas * 2 * p->groups * 4);
+            if (!r.held) n = up256((size_t)r.ctas * 2 * p->groups * 4);
+            if (backward) n += up256((size_t)r.ctas * 2 * p->channels * 4);
             most = std::max(most, n);
         }
     return most;
@@ -698,7 +1004,7 @@ extern "C" int dcn_gnorm_forward(const dcn_gnorm* p, const void* x, const void* 
     if (x == nullptr || y == nullptr) return DCN_ERR_NULL;
     if (!gnorm_aligned(p, {x, residual, y}, {weight, bias}) || !aligned(stats, 4)) return DCN_ERR_ALIGN;
     const size_t need = gnorm_bytes(p, false);
-    if (need > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
+    if (need > 0 && (workspace == nullptr || !aligned(workspace, 8) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
     Vec vec(p);
     vec.by(x), vec.by(residual), vec.by(y);
     const Plan r = plan_of(p, vec.n, false, false);
@@ -726,17 +1032,17 @@ extern "C" int dcn_gnorm_backward(const dcn_gnorm* p, const void* x, const void*
     }
     if (x == nullptr || dy == nullptr || stats == nullptr) return DCN_ERR_NULL;
     const size_t need = gnorm_bytes(p, true);
-    if (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need) return DCN_ERR_WORKSPACE;
+    if (workspace == nullptr || !aligned(workspace, 8) || workspace_bytes < need) return DCN_ERR_WORKSPACE;
     Vec vec(p);
     vec.by(x), vec.by(residual), vec.by(dy), vec.by(dx), vec.by(dresidual);
     const Plan r = plan_of(p, vec.n, true, residual != nullptr);
     if (r.ctas >= 1ll << 31) return DCN_ERR_LIMIT;
     GnormArgs a = gnorm_args(p, r);
     a.x = x, a.weight = weight, a.bias = bias, a.residual = residual, a.dy = dy, a.stats = const_cast<float*>(stats);
-    a.dx = dx, a.dresidual = dresidual;
-    a.partial = static_cast<float*>(workspace);
-    a.sums = reinterpret_cast<float*>(static_cast<char*>(workspace) + up256((size_t)r.ctas * 2 * p->channels * 4));
+    a.dx = dx, a.dresidual = dresidual, a.dweight = dweight, a.dbias = dbias;
+    a.channel_sums = static_cast<float*>(workspace);
+    a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + up256((size_t)r.ctas * 2 * p->channels * 4));
     return by_type(p->dtype, vec.n, [&](auto* t, auto v) {
-        return backward_as<std::remove_pointer_t<decltype(t)>, decltype(v)::value>(a, r, dweight, dbias, st);
+        return backward_as<std::remove_pointer_t<decltype(t)>, decltype(v)::value>(a, r, st);
     });
 }

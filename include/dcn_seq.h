@@ -184,7 +184,8 @@ typedef struct dcn_gnorm {
     float eps;
 } dcn_gnorm;
 
-/* Scratch bytes of dcn_gnorm_forward (backward = 0) and dcn_gnorm_backward (backward = 1) on the current device; may be 0. */
+/* Scratch bytes (aligned to 8) of dcn_gnorm_forward (backward = 0) and dcn_gnorm_backward (backward = 1) on the current device; may be
+ * 0. */
 size_t dcn_gnorm_workspace_bytes(const dcn_gnorm* p, int32_t backward);
 
 /* stats float32 [samples, groups, 2]: mean and 1 / sqrt(var + eps), for the backward pass, or NULL. */
