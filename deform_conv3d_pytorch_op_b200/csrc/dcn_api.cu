@@ -362,8 +362,9 @@ int dcn_debug_expire_wait(int32_t* gave_up, void* stream) {
 
 int dcn_check_status(void* stream) {
     const int tc = dcn::tc_check_status(static_cast<cudaStream_t>(stream));
-    const int scan = dcn::seq::scan_check_status(static_cast<cudaStream_t>(stream));       // (both are read and cleared)
-    return tc != DCN_OK ? tc : scan;
+    const int scan = dcn::seq::scan_check_status(static_cast<cudaStream_t>(stream));       // (all are read and cleared)
+    const int attn = dcn::seq::attn_check_status(static_cast<cudaStream_t>(stream));
+    return tc != DCN_OK ? tc : scan != DCN_OK ? scan : attn;
 }
 
 // ------------------------------------------------------------------------------------------------

@@ -123,6 +123,7 @@ int tc_debug_points(const Geom& g, int ndim, int deform, const float* off, int n
 
 namespace seq {
 int scan_check_status(cudaStream_t st);          // of the sequence operators, seq_scan.cu
+int attn_check_status(cudaStream_t st);          // and seq_attn.cu
 }
 
 }  // namespace dcn

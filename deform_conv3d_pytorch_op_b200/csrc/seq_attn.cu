@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "dcn_tc_common.cuh"
 #include "seq_common.cuh"
 
 namespace dcn {
@@ -63,6 +64,8 @@ __device__ __forceinline__ float log2_decay(const float* log_decay, int h) {
     return fmaxf(g * kLog2e, -1e4f) + (g != g ? g : 0.0f);     // (finite, so that 0 steps are a factor of 1)
 }
 __device__ __forceinline__ float power(float lg, int n) { return ex2(lg * (float)n); }
+
+#include "seq_attn_tc.cuh"
 
 // ---- products: D[16 x 8] += A[16 x k] B[k x 8], k = 16 for 16-bit types and 8 for float32 -----------------------------------------
 // Operands come from tiles in shared memory, rows of `a` columns.  16-bit tiles are swizzled by 16 bytes (the row's low three bits);
@@ -665,11 +668,11 @@ int check_attn(const dcn_attn* p) {
 int wide_of(const dcn_attn* p, bool backward) { return (int)(backward ? std::max(p->dk, p->dv) : p->dk) > 64 ? 128 : 64; }
 
 // How many parts the time axis is split into.  Time goes in chunks of a CTA; a GPU holds `held` of them at once.  More parts fill the
-// GPU, and cost a pass over b and c for their sums (a third of a chunk's time) and the folding (about a chunk's for each part before).
-int parts_for(const dcn_attn* p, bool backward) {
-    const int64_t ct = (backward ? std::max(p->dk, p->dv) : p->dv) > 64 ? 2 : 1;
-    const int64_t units = p->batch * p->heads * ct * (backward ? 3 : 1), chunks = (p->steps + kChunk - 1) / kChunk;
-    const int64_t held = (int64_t)sm_count() * (wide_of(p, backward) == 128 || p->dtype == DCN_SEQ_F32 ? 2 : 3);
+// GPU, and cost a pass over b and c for their sums (half of a chunk's time) and the folding (half a chunk's for each part before).
+int parts_for(const dcn_attn* p, bool backward, bool tensor) {
+    const int64_t ct = (backward ? std::max(p->dk, p->dv) : p->dv) > 64 ? 2 : 1, chunk = tensor ? tcgen::kSteps : kChunk;
+    const int64_t units = p->batch * p->heads * ct * (backward ? 3 : 1), chunks = (p->steps + chunk - 1) / chunk;
+    const int64_t held = (int64_t)sm_count() * (tensor ? 1 : wide_of(p, backward) == 128 || p->dtype == DCN_SEQ_F32 ? 2 : 3);
     int best = 1;
     double least = 1e300;
     for (int n = 1; n <= kMostParts && n <= chunks; ++n) {
@@ -677,7 +680,7 @@ int parts_for(const dcn_attn* p, bool backward) {
         if (n > 1 && each < 4) break;
         if ((chunks + each - 1) / each != n) continue;
         const double waves = (double)((units * n + held - 1) / held), sums = n > 1 ? (double)((units * (n - 1) + held - 1) / held) : 0;
-        const double time = waves * (each + 1 + 0.5 * (n - 1)) + sums * (0.4 * each + 1) + (n > 1 ? 4 : 0);
+        const double time = waves * (each + 2 + 0.25 * (n - 1)) + sums * (0.5 * each + 2) + (n > 1 ? 2 : 0);
         if (time < least * 0.97) least = time, best = n;
     }
     return best;
@@ -692,25 +695,36 @@ int launch_attn(const AttnArgs& a, int parts, cudaStream_t st) {
     return launch_dependent(attn_kernel<T, KA, kEnds>, grid, dim3(kThreads), kBytes, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
+template <typename T, int KA, bool kEnds>
+int launch_attn_tc(const AttnArgs& a, int parts, cudaStream_t st) {
+    constexpr int kBytes = tcgen::Room<T, KA>::kBytes;
+    const auto kernel = tcgen::attn_tc_kernel<T, KA, kEnds>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess) return DCN_ERR_CUDA;
+    const dim3 grid((unsigned)((int64_t)a.batch * a.heads * a.jobs * a.tiles), (unsigned)parts);
+    return launch_dependent(kernel, grid, dim3(tcgen::kThreads), kBytes, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
+}
+
 template <typename T, int KA>
-int run_parts(const AttnArgs& a, cudaStream_t st) {
-    if (a.n_parts > 1) {
-        const int rc = launch_attn<T, KA, true>(a, a.n_parts - 1, st);
-        if (rc != DCN_OK) return rc;
-    }
-    return launch_attn<T, KA, false>(a, a.n_parts, st);
+int run_parts(const AttnArgs& a, bool tensor, cudaStream_t st) {
+    if constexpr (!std::is_same<T, float>::value)
+        if (tensor) {
+            const int rc = a.n_parts > 1 ? launch_attn_tc<T, KA, true>(a, a.n_parts - 1, st) : DCN_OK;
+            return rc != DCN_OK ? rc : launch_attn_tc<T, KA, false>(a, a.n_parts, st);
+        }
+    const int rc = a.n_parts > 1 ? launch_attn<T, KA, true>(a, a.n_parts - 1, st) : DCN_OK;
+    return rc != DCN_OK ? rc : launch_attn<T, KA, false>(a, a.n_parts, st);
 }
 
 template <typename T>
-int run_attn(const AttnArgs& a, int wide, cudaStream_t st) {
-    return wide == 128 ? run_parts<T, 128>(a, st) : run_parts<T, 64>(a, st);
+int run_attn(const AttnArgs& a, int wide, bool tensor, cudaStream_t st) {
+    return wide == 128 ? run_parts<T, 128>(a, tensor, st) : run_parts<T, 64>(a, tensor, st);
 }
 
-int run_attn_any(const dcn_attn* p, const AttnArgs& a, bool backward, cudaStream_t st) {
+int run_attn_any(const dcn_attn* p, const AttnArgs& a, bool backward, bool tensor, cudaStream_t st) {
     const int wide = wide_of(p, backward);
-    return p->dtype == DCN_SEQ_F32    ? run_attn<float>(a, wide, st)
-           : p->dtype == DCN_SEQ_BF16 ? run_attn<__nv_bfloat16>(a, wide, st)
-                                      : run_attn<__half>(a, wide, st);
+    return p->dtype == DCN_SEQ_F32    ? run_attn<float>(a, wide, false, st)
+           : p->dtype == DCN_SEQ_BF16 ? run_attn<__nv_bfloat16>(a, wide, tensor, st)
+                                      : run_attn<__half>(a, wide, tensor, st);
 }
 
 // Bytes that every row of an operand starts on, as cp.async takes them (2: element by element)
@@ -733,14 +747,24 @@ Operands operands(const dcn_attn* p, const void* q, const void* k, const void* v
             operand(p, dout, p->dout_batch, p->dout_step, p->heads > 1 ? p->dout_head : 0, p->dv, 1)};
 }
 
-AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* lengths, bool backward) {
+// The fifth-generation tensor cores take 16-bit rows of whole 16 bytes
+bool takes_tensor(const dcn_attn* p, const Operands& o, std::initializer_list<const void*> results) {
+    if (p->dtype == DCN_SEQ_F32 || p->dk % 8 != 0 || p->dv % 8 != 0) return false;
+    for (const Operand* x : {&o.q, &o.k, &o.v, &o.d})
+        if (x->bytes != 16) return false;
+    for (const void* r : results)
+        if (!aligned(r, 16)) return false;
+    return true;
+}
+
+AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* lengths, bool backward, bool tensor) {
     AttnArgs a = {};
     a.log_decay = log_decay, a.lengths = lengths;
     a.steps = p->steps;
     a.batch = (int)p->batch, a.heads = (int)p->heads;
-    a.n_parts = parts_for(p, backward);
-    const int64_t chunks = (p->steps + kChunk - 1) / kChunk;
-    a.part_steps = std::max<int64_t>(1, (chunks + a.n_parts - 1) / a.n_parts) * kChunk;
+    a.n_parts = parts_for(p, backward, tensor);
+    const int64_t chunk = tensor ? tcgen::kSteps : kChunk, chunks = (p->steps + chunk - 1) / chunk;
+    a.part_steps = std::max<int64_t>(1, (chunks + a.n_parts - 1) / a.n_parts) * chunk;
     a.scale = p->scale;
     return a;
 }
@@ -755,7 +779,7 @@ void add(AttnArgs& a, const Job& j, int elem) {
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 size_t state_elems(const dcn_attn* p) { return (size_t)p->batch * p->heads * p->dk * p->dv; }
 size_t parts_bytes(const dcn_attn* p, bool backward) {
-    const int n = parts_for(p, backward);
+    const int n = std::max(parts_for(p, backward, false), parts_for(p, backward, true));         // (whichever a call's pointers allow)
     if (n <= 1) return 0;
     if (!backward) return rounded((size_t)n * state_elems(p) * 4);
     const size_t dk = p->dk, dv = p->dv, most = std::max(dk, dv) * dv;         // the jobs' states are dv x dk, dv x dk and dk x dv
@@ -771,6 +795,16 @@ bool attn_aligned(const dcn_attn* p, std::initializer_list<const void*> elems, s
 }
 
 }  // namespace
+
+int attn_check_status(cudaStream_t st) {
+    unsigned int v = 0;
+    if (cudaStreamSynchronize(st) != cudaSuccess || cudaMemcpyFromSymbol(&v, tc::g_tc_status, sizeof(v)) != cudaSuccess) return DCN_ERR_CUDA;
+    if (v == 0) return DCN_OK;
+    const unsigned int zero = 0;
+    cudaMemcpyToSymbol(tc::g_tc_status, &zero, sizeof(zero));
+    return DCN_ERR_TIMEOUT;
+}
+
 }  // namespace seq
 }  // namespace dcn
 
@@ -795,11 +829,12 @@ extern "C" int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k,
     if (!attn_aligned(p, {q, k, v, out}, {log_decay, state, last}) || !aligned(lengths, 8)) return DCN_ERR_ALIGN;
     const size_t need = dcn_attn_workspace_bytes(p, 0);
     if (need > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
-    AttnArgs a = attn_args(p, log_decay, lengths, false);
     const Operands o = operands(p, q, k, v, nullptr);
+    const bool tensor = takes_tensor(p, o, {out, last, workspace});
+    AttnArgs a = attn_args(p, log_decay, lengths, false, tensor);
     a.parts = static_cast<float*>(workspace);
     add(a, {o.q, o.k, o.v, out, state, last, (int)p->dv, 1, 0, 0, 1.0f, 1.0f}, elem_bytes(p->dtype));
-    return run_attn_any(p, a, false, (cudaStream_t)stream);
+    return run_attn_any(p, a, false, tensor, (cudaStream_t)stream);
 }
 
 extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay,
@@ -814,8 +849,9 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
     if (need > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;
     if (dout == nullptr && p->steps > 0) return DCN_ERR_NULL;
-    AttnArgs a = attn_args(p, log_decay, lengths, true);
     const Operands o = operands(p, q, k, v, dout);
+    const bool tensor = takes_tensor(p, o, {dq, dk, dv, dstate, workspace});
+    AttnArgs a = attn_args(p, log_decay, lengths, true, tensor);
     a.parts = static_cast<float*>(workspace);
     const bool shared = p->heads != p->kv_heads;
     char* const wide_k = static_cast<char*>(workspace) + parts_bytes(p, true);
@@ -829,7 +865,7 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
         add(a, {o.k, o.q, o.d, shared ? wide_v : dv, dlast, dstate, across, 1, 1, shared, 1.0f / s, s}, elem);
     }
     if (a.jobs == 0) return DCN_OK;
-    int rc = run_attn_any(p, a, true, st);
+    int rc = run_attn_any(p, a, true, tensor, st);
     if (rc != DCN_OK || !shared || p->steps == 0) return rc;
     const int share = (int)(p->heads / p->kv_heads);
     auto sum = [&](const char* from, void* to, int64_t width) {
