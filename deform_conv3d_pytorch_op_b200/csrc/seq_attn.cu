@@ -14,6 +14,8 @@
 #include <algorithm>
 #include <cmath>
 
+#include <cuda.h>
+
 #include "dcn_tc_common.cuh"
 #include "seq_common.cuh"
 
@@ -33,6 +35,7 @@ struct Operand {
     Strides s;
     int share;                                   // heads that read the same one
     int width, bytes;                            // elements of a row; bytes that are copied at once
+    int map;                                     // of the call's tensor maps
 };
 
 struct Job {
@@ -696,41 +699,42 @@ int launch_attn(const AttnArgs& a, int parts, cudaStream_t st) {
 }
 
 template <typename T, int KA, bool kEnds>
-int launch_attn_tc(const AttnArgs& a, int parts, cudaStream_t st) {
+int launch_attn_tc(const AttnArgs& a, const tcgen::Maps& maps, int parts, cudaStream_t st) {
     constexpr int kBytes = tcgen::Room<T, KA>::kBytes;
     const auto kernel = tcgen::attn_tc_kernel<T, KA, kEnds>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess) return DCN_ERR_CUDA;
     const dim3 grid((unsigned)((int64_t)a.batch * a.heads * a.jobs * a.tiles), (unsigned)parts);
-    return launch_dependent(kernel, grid, dim3(tcgen::kThreads), kBytes, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
+    return launch_dependent(kernel, grid, dim3(tcgen::kThreads), kBytes, st, a, maps) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
 template <typename T, int KA>
-int run_parts(const AttnArgs& a, bool tensor, cudaStream_t st) {
+int run_parts(const AttnArgs& a, const tcgen::Maps* maps, cudaStream_t st) {
     if constexpr (!std::is_same<T, float>::value)
-        if (tensor) {
-            const int rc = a.n_parts > 1 ? launch_attn_tc<T, KA, true>(a, a.n_parts - 1, st) : DCN_OK;
-            return rc != DCN_OK ? rc : launch_attn_tc<T, KA, false>(a, a.n_parts, st);
+        if (maps != nullptr) {
+            const int rc = a.n_parts > 1 ? launch_attn_tc<T, KA, true>(a, *maps, a.n_parts - 1, st) : DCN_OK;
+            return rc != DCN_OK ? rc : launch_attn_tc<T, KA, false>(a, *maps, a.n_parts, st);
         }
     const int rc = a.n_parts > 1 ? launch_attn<T, KA, true>(a, a.n_parts - 1, st) : DCN_OK;
     return rc != DCN_OK ? rc : launch_attn<T, KA, false>(a, a.n_parts, st);
 }
 
 template <typename T>
-int run_attn(const AttnArgs& a, int wide, bool tensor, cudaStream_t st) {
-    return wide == 128 ? run_parts<T, 128>(a, tensor, st) : run_parts<T, 64>(a, tensor, st);
+int run_attn(const AttnArgs& a, int wide, const tcgen::Maps* maps, cudaStream_t st) {
+    return wide == 128 ? run_parts<T, 128>(a, maps, st) : run_parts<T, 64>(a, maps, st);
 }
 
-int run_attn_any(const dcn_attn* p, const AttnArgs& a, bool backward, bool tensor, cudaStream_t st) {
+// maps: those of the call's operands, or null where the tensor cores' kernel does not take them
+int run_attn_any(const dcn_attn* p, const AttnArgs& a, bool backward, const tcgen::Maps* maps, cudaStream_t st) {
     const int wide = wide_of(p, backward);
-    return p->dtype == DCN_SEQ_F32    ? run_attn<float>(a, wide, false, st)
-           : p->dtype == DCN_SEQ_BF16 ? run_attn<__nv_bfloat16>(a, wide, tensor, st)
-                                      : run_attn<__half>(a, wide, tensor, st);
+    return p->dtype == DCN_SEQ_F32    ? run_attn<float>(a, wide, nullptr, st)
+           : p->dtype == DCN_SEQ_BF16 ? run_attn<__nv_bfloat16>(a, wide, maps, st)
+                                      : run_attn<__half>(a, wide, maps, st);
 }
 
 // Bytes that every row of an operand starts on, as cp.async takes them (2: element by element)
-Operand operand(const dcn_attn* p, const void* at, int64_t batch, int64_t step, int64_t head, int64_t width, int share) {
+Operand operand(const dcn_attn* p, int map, const void* at, int64_t batch, int64_t step, int64_t head, int64_t width, int share) {
     const int e = elem_bytes(p->dtype);
-    Operand o = {at, {p->batch > 1 ? batch : 0, p->steps > 1 ? step : 0, head}, share, (int)width, 16};
+    Operand o = {at, {p->batch > 1 ? batch : 0, p->steps > 1 ? step : 0, head}, share, (int)width, 16, map};
     while (o.bytes > 2 && (!aligned(at, o.bytes) || o.s.batch * e % o.bytes != 0 || o.s.step * e % o.bytes != 0 || head * e % o.bytes != 0))
         o.bytes /= 2;
     return o;
@@ -741,19 +745,56 @@ struct Operands {
 };
 Operands operands(const dcn_attn* p, const void* q, const void* k, const void* v, const void* dout) {
     const int share = (int)(p->heads / p->kv_heads);
-    return {operand(p, q, p->q_batch, p->q_step, p->heads > 1 ? p->q_head : 0, p->dk, 1),
-            operand(p, k, p->k_batch, p->k_step, p->kv_heads > 1 ? p->k_head : 0, p->dk, share),
-            operand(p, v, p->v_batch, p->v_step, p->kv_heads > 1 ? p->v_head : 0, p->dv, share),
-            operand(p, dout, p->dout_batch, p->dout_step, p->heads > 1 ? p->dout_head : 0, p->dv, 1)};
+    return {operand(p, 0, q, p->q_batch, p->q_step, p->heads > 1 ? p->q_head : 0, p->dk, 1),
+            operand(p, 1, k, p->k_batch, p->k_step, p->kv_heads > 1 ? p->k_head : 0, p->dk, share),
+            operand(p, 2, v, p->v_batch, p->v_step, p->kv_heads > 1 ? p->v_head : 0, p->dv, share),
+            operand(p, 3, dout, p->dout_batch, p->dout_step, p->heads > 1 ? p->dout_head : 0, p->dv, 1)};
 }
 
-// The fifth-generation tensor cores take 16-bit rows of whole 16 bytes
+// The tensor cores' kernel takes 16-bit rows of whole 16 bytes that do not lie on top of one another
 bool takes_tensor(const dcn_attn* p, const Operands& o, std::initializer_list<const void*> results) {
-    if (p->dtype == DCN_SEQ_F32 || p->dk % 8 != 0 || p->dv % 8 != 0) return false;
-    for (const Operand* x : {&o.q, &o.k, &o.v, &o.d})
+    if (p->dtype == DCN_SEQ_F32 || p->dk % 8 != 0 || p->dv % 8 != 0 || p->steps == 0) return false;
+    for (const Operand* x : {&o.q, &o.k, &o.v, &o.d}) {
         if (x->bytes != 16) return false;
+        if (x->p == nullptr) continue;
+        const int64_t heads = p->heads / x->share;
+        if ((p->batch > 1 && x->s.batch <= 0) || (p->steps > 1 && x->s.step <= 0) || (heads > 1 && x->s.head <= 0)) return false;
+        if (x->s.batch >= 1ll << 38 || x->s.step >= 1ll << 38 || x->s.head >= 1ll << 38) return false;
+    }
     for (const void* r : results)
         if (!aligned(r, 16)) return false;
+    return true;
+}
+
+// The driver's function, found at run time: the library is not linked with the driver's
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                 const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+    static const EncodeTiled found = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess || r != cudaDriverEntryPointSuccess)
+            f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return found;
+}
+
+bool make_maps(const dcn_attn* p, const Operands& o, tcgen::Maps& maps) {
+    const EncodeTiled encode = encode_tiled();
+    if (encode == nullptr) return false;
+    for (const Operand* x : {&o.q, &o.k, &o.v, &o.d}) {
+        if (x->p == nullptr) continue;
+        const cuuint64_t heads = (cuuint64_t)(p->heads / x->share), row = ((cuuint64_t)x->width * 2 + 15) / 16 * 16;
+        const cuuint64_t dims[4] = {(cuuint64_t)x->width, heads, (cuuint64_t)p->steps, (cuuint64_t)p->batch};
+        const cuuint64_t strides[3] = {heads > 1 ? (cuuint64_t)x->s.head * 2 : row, p->steps > 1 ? (cuuint64_t)x->s.step * 2 : row,
+                                       p->batch > 1 ? (cuuint64_t)x->s.batch * 2 : row};
+        const cuuint32_t box[4] = {64, 1, tcgen::kSteps, 1}, ones[4] = {1, 1, 1, 1};
+        const CUtensorMapDataType type = p->dtype == DCN_SEQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+        if (encode(&maps.of[x->map], type, 4, const_cast<void*>(x->p), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return false;
+    }
     return true;
 }
 
@@ -830,11 +871,12 @@ extern "C" int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k,
     const size_t need = dcn_attn_workspace_bytes(p, 0);
     if (need > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
     const Operands o = operands(p, q, k, v, nullptr);
-    const bool tensor = takes_tensor(p, o, {out, last, workspace});
+    tcgen::Maps maps = {};
+    const bool tensor = takes_tensor(p, o, {out, last, workspace}) && make_maps(p, o, maps);
     AttnArgs a = attn_args(p, log_decay, lengths, false, tensor);
     a.parts = static_cast<float*>(workspace);
     add(a, {o.q, o.k, o.v, out, state, last, (int)p->dv, 1, 0, 0, 1.0f, 1.0f}, elem_bytes(p->dtype));
-    return run_attn_any(p, a, false, tensor, (cudaStream_t)stream);
+    return run_attn_any(p, a, false, tensor ? &maps : nullptr, (cudaStream_t)stream);
 }
 
 extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay,
@@ -850,7 +892,8 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
     const cudaStream_t st = (cudaStream_t)stream;
     if (dout == nullptr && p->steps > 0) return DCN_ERR_NULL;
     const Operands o = operands(p, q, k, v, dout);
-    const bool tensor = takes_tensor(p, o, {dq, dk, dv, dstate, workspace});
+    tcgen::Maps maps = {};
+    const bool tensor = takes_tensor(p, o, {dq, dk, dv, dstate, workspace}) && make_maps(p, o, maps);
     AttnArgs a = attn_args(p, log_decay, lengths, true, tensor);
     a.parts = static_cast<float*>(workspace);
     const bool shared = p->heads != p->kv_heads;
@@ -865,7 +908,7 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
         add(a, {o.k, o.q, o.d, shared ? wide_v : dv, dlast, dstate, across, 1, 1, shared, 1.0f / s, s}, elem);
     }
     if (a.jobs == 0) return DCN_OK;
-    int rc = run_attn_any(p, a, true, tensor, st);
+    int rc = run_attn_any(p, a, true, tensor ? &maps : nullptr, st);
     if (rc != DCN_OK || !shared || p->steps == 0) return rc;
     const int share = (int)(p->heads / p->kv_heads);
     auto sum = [&](const char* from, void* to, int64_t width) {

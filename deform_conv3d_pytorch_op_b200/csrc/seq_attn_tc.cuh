@@ -4,15 +4,18 @@
 //     P      = scores, weighted by g^(i-j) and cut above the diagonal, as 16-bit operand in tensor memory
 //     O1     = A X,  O2 = P C         128 x 64                     out = scale (g^(i+1) O1 + O2)
 //     U      = B^T C', C'_j = g^(127-j) c_j                        X'  = g^128 X + U
-// C' is the sum of three bfloat16 (two float16) tiles, so that the products of the state are those of float32; X is in the registers of
-// four warps in float32, and meets A as a rounded copy in shared memory.
+// C' is a sum of 16-bit tiles, so many that what the state is made of is exact to 2^-17 (two of bfloat16) where it only meets A, and to
+// float32's own 2^-24 (three) where it is a result; two of float16 are exact to 2^-22.  X is in the registers of four warps in float32, and
+// meets A as a rounded copy in shared memory.
 //
-// A CTA has one job's head (or a part of its time axis) and 64 columns of c: two such tiles of a chunk and a copy ahead fill shared
-// memory.  Four warps load (cp.async, two chunks), four make P and the output, four make C' and the state, one thread issues the products.
-// The loop that bounds the chain is C' -> U -> X -> O1; everything else runs beside it.
+// A CTA has one job's head (or a part of its time axis) and 64 columns of c: two chunks' tiles, C' and X fill shared memory.  One
+// thread loads (TMA, a chunk ahead), four warps make P and the output, four make C' (half a chunk ahead of its product), four keep the
+// state, and two threads issue the products, one those with A, one U, so that neither chain waits for the other's operands.
+//
+// Rows of a tile are steps in the order of time.  Back in time, position i of a chunk is row 127 - i, and triangle and weights are mirrored.
 namespace tcgen {
 
-constexpr int kSteps = 128, kDv = 64, kThreads = 13 * 32;
+constexpr int kSteps = 128, kDv = 64, kThreads = 16 * 32;
 constexpr uint32_t kTmScores = 0, kTmO1 = 128, kTmO2 = 192, kTmU = 256, kTmP = 320;      // columns of tensor memory
 
 template <typename T, int KA>
@@ -25,12 +28,31 @@ struct Room {
 };
 
 struct Control {
-    uint64_t full[2], empty[2], scores_full, scores_empty, p_full, out_full, out_empty, c_full, u_full, x_full;
+    uint64_t full[2], empty[2], zeroed, scores_full, scores_empty, p_full, out_full, out_empty, c_full[2], c_empty[2], u_full, u_empty, x_full, x_empty;
     uint32_t tmem;
     float up[2], most[4];
-    float power[kSteps + 1];                     // g^n
-    alignas(16) float back[32];                  // g^(31-n)
+    float none[32], power[kSteps + 1];           // g^n behind 32 zeros for what is not before a step
 };
+
+// Bounded wait.  It polls: a chunk's chain has a dozen of them one behind the other, and a parked thread wakes late (with
+// tc::mbar_wait a chunk of the 2x16384x16x128 case took 6.8 us).
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
+    const uint32_t at = tc::smem_u32(bar);
+    const long long t0 = clock64();
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 64; ++i) {
+            uint32_t done;
+            asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
+                         : "=r"(done) : "r"(at), "r"(parity) : "memory");
+            if (done) return true;
+        }
+        if (clock64() - t0 > tc::kWaitCycles) {
+            atomicOr(&tc::g_tc_status, 1u);
+            return false;
+        }
+    }
+}
 
 template <typename T>
 __host__ __device__ constexpr uint32_t idesc(int m, int n, int a_mn_major, int b_mn_major) {
@@ -54,27 +76,21 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// A tile's rows first, first + 1, ... of an operand, 64 columns to a half; zeros beyond the length and the width.  128 threads
-template <int kCols_>
-__device__ __forceinline__ void load_rows(uint32_t to, const Operand& o, const char* from, int64_t first, int64_t length, int col0, bool reverse,
-                                          int tid) {
-    constexpr int kChunks = kCols_ / 8, kRows = 128 / kChunks;   // of 16 bytes in a row; rows at a time (a multiple of 8)
-    const int c = tid % kChunks, r0 = tid / kChunks, left = (o.width - col0 - c * 8) * 2, bytes = left <= 0 ? 0 : left >= 16 ? 16 : left;
-    const int64_t t0 = reverse ? length - 1 - first - r0 : first + r0, step = (reverse ? -kRows : kRows) * o.s.step * 2;
-    const char* src = from + (t0 * o.s.step + col0 + c * 8) * 2;
-    uint32_t dst = to + (c >> 3) * (kSteps * 128) + tc::swz_offset(r0, c & 7);
-    const int rows = (int)min((int64_t)kSteps, length - first) - r0;             // row r0 + p * kRows is there while p * kRows < rows
-#pragma unroll
-    for (int p = 0; p < kSteps / kRows; ++p) {
-        const bool in = p * kRows < rows && bytes > 0;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? src : from), "r"(in ? bytes : 0) : "memory");
-        src += step, dst += kRows * 128;
-    }
+// The operands as [batch][steps][heads][width], boxes of 64 elements of 128 steps
+struct alignas(64) Maps {
+    CUtensorMap of[4];
+};
+
+// 128 rows of 64 elements from `col`, row 0 at time t (zeros outside of the tensor, before time 0 too)
+__device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap& map, int col, int head, int t, int batch, uint64_t* bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(to),
+                 "l"(reinterpret_cast<uint64_t>(&map)), "r"(col), "r"(head), "r"(t), "r"(batch), "r"(tc::smem_u32(bar))
+                 : "memory");
 }
 
 // kEnds: the sums of each part's b_j c_j^T alone
 template <typename T, int KA, bool kEnds>
-__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs args) {
+__global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs args, const __grid_constant__ Maps maps) {
     using R = Room<T, KA>;
     extern __shared__ char raw[];
     char* const smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
@@ -91,15 +107,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     if (tile >= args.tile_of[which]) return;
     const int col0 = tile * kDv, part = blockIdx.y;
 
-    if (warp == 12) {
+    if (warp == 3) {
         tc::tmem_alloc(&ctl.tmem, 512);
         tc::tmem_relinquish();
     }
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 2; ++s) tc::mbar_init(&ctl.full[s], 4), tc::mbar_init(&ctl.empty[s], 1 + 4);
+        for (int s = 0; s < 2; ++s) {
+            tc::mbar_init(&ctl.full[s], 1), tc::mbar_init(&ctl.empty[s], (kEnds ? 1 : 2) + 4);
+            tc::mbar_init(&ctl.c_full[s], 4), tc::mbar_init(&ctl.c_empty[s], 1);
+        }
+        tc::mbar_init(&ctl.zeroed, 4);
         tc::mbar_init(&ctl.scores_full, 1), tc::mbar_init(&ctl.scores_empty, 4), tc::mbar_init(&ctl.p_full, 4);
         tc::mbar_init(&ctl.out_full, 1), tc::mbar_init(&ctl.out_empty, 4);
-        tc::mbar_init(&ctl.c_full, 4), tc::mbar_init(&ctl.u_full, 1), tc::mbar_init(&ctl.x_full, 4);
+        tc::mbar_init(&ctl.u_full, 1), tc::mbar_init(&ctl.u_empty, 4), tc::mbar_init(&ctl.x_full, 4), tc::mbar_init(&ctl.x_empty, 1);
         tc::fence_barrier_init();
     }
     pdl_wait();
@@ -110,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         const int n = threadIdx.x;
         const float w = n == 0 ? (g != g ? g : 1.0f) : (float)exp((double)n * (double)g);
         ctl.power[n] = w;
-        if (n < 32) ctl.back[31 - n] = w;
+        if (n < 32) ctl.none[n] = 0.0f;
     }
     const int64_t steps = args.steps;
     int64_t length = steps;
@@ -125,85 +145,72 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     tc::tc_fence_after();
     const uint32_t tmem = ctl.tmem;
     const int64_t parts_of = ((int64_t)which * args.batch * args.heads + unit) * args.n_parts;
+    // tiles that C' is the sum of
+    const int parts = job.end != nullptr ? R::kParts : 2;
 
-    if (warp < 4) {
+    // Behind a sequence's end, but inside the tensor, rows hold what they may: b's and c's of the last chunk are made zeros
+    const int ragged = !reverse && length < steps && chunks > 0 && length < begin + (int64_t)chunks * kSteps ? chunks - 1 : -1;
+
+    if (warp == 0) {
         // ---- loads
-        const char* const from_a = static_cast<const char*>(job.a.p) + (b * job.a.s.batch + h / job.a.share * job.a.s.head) * 2;
-        const char* const from_b = static_cast<const char*>(job.b.p) + (b * job.b.s.batch + h / job.b.share * job.b.s.head) * 2;
-        const char* const from_c = static_cast<const char*>(job.c.p) + (b * job.c.s.batch + h / job.c.share * job.c.s.head) * 2;
-        auto issue = [&](int n) {
-            const uint32_t to = base + (n & 1) * R::kStage;
-            const int64_t first = begin + (int64_t)n * kSteps;
-            if constexpr (!kEnds) load_rows<KA>(to, job.a, from_a, first, length, 0, reverse, threadIdx.x);
-            load_rows<KA>(to + R::kA, job.b, from_b, first, length, 0, reverse, threadIdx.x);
-            load_rows<kDv>(to + 2 * R::kA, job.c, from_c, first, length, col0, reverse, threadIdx.x);
-            copies_issued();
-        };
-        auto arrived = [&](int n) {
-            tc::fence_proxy_async_smem();
-            tc::mbar_arrive_warp(&ctl.full[n & 1]);
-        };
-        for (int n = 0; n < chunks; ++n) {
-            if (n >= 2 && !tc::mbar_wait(&ctl.empty[n & 1], ((n >> 1) & 1) ^ 1)) break;
-            issue(n);
-            if (n == 0 && chunks > 1) continue;
-            if (n == 1) {
-                copies_arrived<1>();
-                arrived(0);
+        if (lane == 0) {
+            int n = 0;
+            for (; n < chunks; ++n) {
+                uint64_t* const bar = &ctl.full[n & 1];
+                if (n >= 2 && !wait(&ctl.empty[n & 1], ((n >> 1) & 1) ^ 1)) break;
+                const uint32_t to = base + (n & 1) * R::kStage;
+                const int64_t first = begin + (int64_t)n * kSteps;
+                const int t = (int)(reverse ? length - kSteps - first : first);
+                tc::mbar_arrive_expect_tx(bar, (kEnds ? R::kA : 2 * R::kA) + R::kHalf);
+#pragma unroll
+                for (int k = 0; k < KA / 64; ++k) {
+                    if constexpr (!kEnds) load_box(to + k * R::kHalf, maps.of[job.a.map], 64 * k, h / job.a.share, t, b, bar);
+                    load_box(to + R::kA + k * R::kHalf, maps.of[job.b.map], 64 * k, h / job.b.share, t, b, bar);
+                }
+                load_box(to + 2 * R::kA, maps.of[job.c.map], col0, h / job.c.share, t, b, bar);
             }
-            copies_arrived<0>();
-            arrived(n);
+            for (int k = max(n - 2, 0); k < n; ++k) wait(&ctl.full[k & 1], (k >> 1) & 1);       // (nothing is under way at the end)
         }
-    } else if (warp < 8) {
+    } else if (warp >= 4 && warp < 8) {
         // ---- scores to weights, and the output
         if constexpr (!kEnds) {
-            const int w = warp & 3, i = w * 32 + lane;
+            const int w = warp & 3, i = reverse ? kSteps - 1 - (w * 32 + lane) : w * 32 + lane;        // the position
             const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16);
             bool ok = true;
-            const float near = ctl.power[lane + 1];
             for (int n = 0; n < chunks; ++n) {
-                ok = tc::mbar_wait(&ctl.scores_full, n & 1);
+                ok = wait(&ctl.scores_full, n & 1);
                 if (!ok) break;
                 __syncwarp();
                 tc::tc_fence_after();
+                // (short code in loops: the roles' instructions together would not stay in the caches that feed the schedulers)
 #pragma unroll 1
                 for (int cb = 0; cb < 4; ++cb) {
-                    uint32_t packed[16];
-                    if (cb > w) {
-#pragma unroll
-                        for (int k = 0; k < 16; ++k) packed[k] = 0;
-                    } else {
-                        uint32_t v[32];
+                    const int back = reverse ? cb - w : w - cb;  // blocks of 32 steps back
+                    uint32_t v[32];
+                    if (back >= 0) {
                         tc::tmem_ld32(rows_at + kTmScores + cb * 32, v);
                         tc::tmem_ld_wait();
-                        if (cb == w) {
+                        const float* const f = ctl.power + 32 * back + (reverse ? -lane : lane);
+                        if (reverse) {
 #pragma unroll
-                            for (int k = 0; k < 16; ++k) {
-                                const int d = lane - 2 * k;      // steps back
-                                const float x = d >= 0 ? __uint_as_float(v[2 * k]) * ctl.power[max(d, 0)] : 0.0f;
-                                const float y = d >= 1 ? __uint_as_float(v[2 * k + 1]) * ctl.power[max(d - 1, 0)] : 0.0f;
-                                packed[k] = word_of<T>(x, y);
-                            }
+                            for (int k = 0; k < 16; ++k)
+                                v[k] = word_of<T>(__uint_as_float(v[2 * k]) * f[2 * k], __uint_as_float(v[2 * k + 1]) * f[2 * k + 1]);
                         } else {
-                            const Lanes f = all_lanes(near * ctl.power[32 * (w - cb - 1)]);
 #pragma unroll
-                            for (int k = 0; k < 16; k += 2) {
-                                const float4 c = *reinterpret_cast<const float4*>(&ctl.back[2 * k]);
-                                const float c0[2] = {c.x, c.y}, c1[2] = {c.z, c.w};
-                                const float x0[2] = {__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])};
-                                const float x1[2] = {__uint_as_float(v[2 * k + 2]), __uint_as_float(v[2 * k + 3])};
-                                const Lanes p = lanes(x0) * (f * lanes(c0)), q = lanes(x1) * (f * lanes(c1));
-                                packed[k] = word_of<T>(p.at(0), p.at(1)), packed[k + 1] = word_of<T>(q.at(0), q.at(1));
-                            }
+                            for (int k = 0; k < 16; ++k)
+                                v[k] = word_of<T>(__uint_as_float(v[2 * k]) * f[-2 * k], __uint_as_float(v[2 * k + 1]) * f[-2 * k - 1]);
                         }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[k] = 0;
                     }
-                    tmem_st16(rows_at + kTmP + cb * 16, packed);
+                    tmem_st16(rows_at + kTmP + cb * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
                 }
                 tmem_st_wait();
                 tc::tc_fence_before();
                 tc::mbar_arrive_warp(&ctl.scores_empty);
                 tc::mbar_arrive_warp(&ctl.p_full);
-                ok = tc::mbar_wait(&ctl.out_full, n & 1);
+                ok = wait(&ctl.out_full, n & 1);
                 if (!ok) break;
                 __syncwarp();
                 tc::tc_fence_after();
@@ -258,9 +265,58 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
             }
         }
-    } else if (warp < 12) {
-        // ---- the weighted c, and the state
-        const int tid = threadIdx.x - 256, w = warp & 3, i = w * 32 + lane;
+    } else if (warp >= 8 && warp < 12) {
+        // ---- the weighted c, half a chunk at a time
+        const int tid = threadIdx.x - 256, c = tid & 7, r0 = tid >> 3;           // 16 bytes of rows r0, r0 + 16, ...
+        const uint32_t place = tc::swz_offset(r0, c);
+        bool ok = true;
+        for (int n = 0; n < chunks && ok; ++n) {
+            ok = wait(&ctl.full[n & 1], (n >> 1) & 1);
+            const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps), top = rows - extra;
+            if (ok && n == ragged) {
+                const uint32_t tile = base + (n & 1) * R::kStage + R::kA;        // b's halves, and c's behind them
+                for (int k = tid; k < (KA / 64 + 1) * (kSteps - rows) * 8; k += 128)
+                    tc::st_shared_v4(tile + k / ((kSteps - rows) * 8) * R::kHalf + tc::swz_offset(rows + k / 8 % (kSteps - rows), k % 8), 0, 0, 0, 0);
+                tc::fence_proxy_async_smem();
+                tc::mbar_arrive_warp(&ctl.zeroed);
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+            }
+            for (int half = 0; half < 2 && ok; ++half) {
+                ok = n == 0 || wait(&ctl.c_empty[half], (n - 1) & 1);
+                if (!ok) break;
+                const uint32_t from = base + (n & 1) * R::kStage + 2 * R::kA + place + half * 8192, to = base + R::kWeighted + place + half * 8192;
+#pragma unroll 1
+                for (int p = 0; p < 4; ++p) {
+                    const int row = r0 + 16 * p + 64 * half, j = reverse ? kSteps - 1 - row : row;
+                    const Lanes f = all_lanes(j < rows ? ctl.power[max(top - j, 0)] : 0.0f);
+                    const uint4 v = tc::lds128(from + p * 2048);
+                    const uint32_t in[4] = {v.x, v.y, v.z, v.w};
+                    uint32_t out[R::kParts][4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float e[2] = {half_of<T>(in[k], 0), half_of<T>(in[k], 1)};
+                        Lanes r = lanes(e) * f;
+#pragma unroll
+                        for (int q = 0; q < R::kParts; ++q) {
+                            out[q][k] = word_of<T>(r.at(0), r.at(1));
+                            if (q + 1 < R::kParts) {
+                                const float t[2] = {half_of<T>(out[q][k], 0), half_of<T>(out[q][k], 1)};
+                                r = r - lanes(t);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int q = 0; q < R::kParts; ++q)
+                        if (q < 2 || parts > 2) tc::st_shared_v4(to + q * R::kHalf + p * 2048, out[q][0], out[q][1], out[q][2], out[q][3]);
+                }
+                tc::fence_proxy_async_smem();
+                tc::mbar_arrive_warp(&ctl.c_full[half]);
+            }
+            if (ok) tc::mbar_arrive_warp(&ctl.empty[n & 1]);
+        }
+    } else if (warp >= 12) {
+        // ---- the state
+        const int tid = threadIdx.x - 384, w = warp & 3, i = w * 32 + lane;
         const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16) + kTmU;
         const bool mine = i < KA;                // (the products have 128 rows: behind a's 64 columns they find those of c)
         float x[kDv];
@@ -306,70 +362,47 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 if (tid == 0) ctl.up[n & 1] = 1.0f;
             }
             if (mine) {
-                const uint32_t row = base + R::kState;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const float* const v = x + 8 * c;
-                    tc::st_shared_v4(row + tc::swz_offset(i, c), word_of<T>(v[0] * down, v[1] * down), word_of<T>(v[2] * down, v[3] * down),
+                    tc::st_shared_v4(base + R::kState + tc::swz_offset(i, c), word_of<T>(v[0] * down, v[1] * down), word_of<T>(v[2] * down, v[3] * down),
                                      word_of<T>(v[4] * down, v[5] * down), word_of<T>(v[6] * down, v[7] * down));
                 }
             }
             tc::fence_proxy_async_smem();
             tc::mbar_arrive_warp(&ctl.x_full);
         };
-        const int c = tid & 7, r0 = tid >> 3;    // of the tile of c: 16 bytes of rows r0, r0 + 16, ...
-        const uint32_t place = tc::swz_offset(r0, c);
         bool ok = true;
+        if constexpr (!kEnds) put_copy(0);
         for (int n = 0; n < chunks; ++n) {
-            if constexpr (!kEnds) put_copy(n);
-            ok = tc::mbar_wait(&ctl.full[n & 1], (n >> 1) & 1);
-            if (!ok) break;
-            const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps), top = rows - extra;
-            const uint32_t from = base + (n & 1) * R::kStage + 2 * R::kA + place, to = base + R::kWeighted + place;
-#pragma unroll 2
-            for (int p = 0; p < 8; ++p) {
-                const int j = r0 + 16 * p;
-                const float weight = j < rows ? ctl.power[top - j] : 0.0f;
-                const Lanes f = all_lanes(weight);
-                const uint4 v = tc::lds128(from + p * 2048);
-                const uint32_t in[4] = {v.x, v.y, v.z, v.w};
-                uint32_t out[R::kParts][4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float e[2] = {half_of<T>(in[k], 0), half_of<T>(in[k], 1)};
-                    Lanes r = lanes(e) * f;
-#pragma unroll
-                    for (int q = 0; q < R::kParts; ++q) {
-                        out[q][k] = word_of<T>(r.at(0), r.at(1));
-                        if (q + 1 < R::kParts) {
-                            const float t[2] = {half_of<T>(out[q][k], 0), half_of<T>(out[q][k], 1)};
-                            r = r - lanes(t);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int q = 0; q < R::kParts; ++q)
-                    tc::st_shared_v4(to + q * R::kHalf + p * 2048, out[q][0], out[q][1], out[q][2], out[q][3]);
-            }
-            tc::fence_proxy_async_smem();
-            tc::tc_fence_before();               // (U of the chunk before has been read)
-            tc::mbar_arrive_warp(&ctl.c_full);
-            tc::mbar_arrive_warp(&ctl.empty[n & 1]);
-            ok = tc::mbar_wait(&ctl.u_full, n & 1);
+            const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps);
+            const Lanes whole = all_lanes(ctl.power[rows]);
+            ok = wait(&ctl.u_full, n & 1);
             if (!ok) break;
             __syncwarp();
             tc::tc_fence_after();
-            const Lanes whole = all_lanes(ctl.power[rows]);
 #pragma unroll
             for (int cb = 0; cb < 2; ++cb) {
                 uint32_t v[32];
                 tc::tmem_ld32(rows_at + cb * 32, v);
                 tc::tmem_ld_wait();
+                if (cb == 1) {
+                    tc::tc_fence_before();
+                    tc::mbar_arrive_warp(&ctl.u_empty);
+                }
 #pragma unroll
                 for (int k = 0; k < 32; k += 2) {
                     const float a[2] = {x[cb * 32 + k], x[cb * 32 + k + 1]}, e[2] = {__uint_as_float(v[k]), __uint_as_float(v[k + 1])};
                     const Lanes r = fma(lanes(a), whole, lanes(e));
                     x[cb * 32 + k] = r.at(0), x[cb * 32 + k + 1] = r.at(1);
+                }
+            }
+            if constexpr (!kEnds) {
+                if (n + 1 < chunks) {
+                    ok = wait(&ctl.x_empty, n & 1);     // A has met the copy before
+                    if (!ok) break;
+                    __syncwarp();
+                    put_copy(n + 1);
                 }
             }
         }
@@ -382,16 +415,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 if (col0 + k < wc)
                     *reinterpret_cast<float4*>(to + (int64_t)i * wc + col0 + k) = make_float4(by * x[k], by * x[k + 1], by * x[k + 2], by * x[k + 3]);
         }
-    } else if (lane == 0) {
-        // ---- products
-        bool ok = true;
-        for (int n = 0; n < chunks && ok; ++n) {
-            const int s = n & 1;
-            const uint32_t a = base + s * R::kStage, bt = a + R::kA, ct = a + 2 * R::kA;
-            ok = tc::mbar_wait(&ctl.full[s], (n >> 1) & 1);
-            if (!ok) break;
-            if constexpr (!kEnds) {
-                ok = n == 0 || tc::mbar_wait(&ctl.scores_empty, (n - 1) & 1);
+    } else if (warp == 2) {
+        // ---- the products with A
+        if (!kEnds && lane == 0) {
+            bool ok = true;
+            for (int n = 0; n < chunks && ok; ++n) {
+                const int s = n & 1;
+                const uint32_t a = base + s * R::kStage, bt = a + R::kA, ct = a + 2 * R::kA;
+                ok = wait(&ctl.full[s], (n >> 1) & 1) && (n != ragged || wait(&ctl.zeroed, 0)) &&
+                     (n == 0 || wait(&ctl.scores_empty, (n - 1) & 1));
                 if (!ok) break;
                 tc::tc_fence_after();
 #pragma unroll
@@ -400,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     tc::umma_bf16(tmem + kTmScores, tc::make_desc(a + off, 16, 1024), tc::make_desc(bt + off, 16, 1024), idesc<T>(128, 128, 0, 0), k > 0);
                 }
                 tc::umma_commit(&ctl.scores_full);
-                ok = tc::mbar_wait(&ctl.x_full, n & 1) && (n == 0 || tc::mbar_wait(&ctl.out_empty, (n - 1) & 1));
+                ok = wait(&ctl.x_full, n & 1) && (n == 0 || wait(&ctl.out_empty, (n - 1) & 1));
                 if (!ok) break;
                 tc::tc_fence_after();
 #pragma unroll
@@ -409,35 +441,52 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     tc::umma_bf16(tmem + kTmO1, tc::make_desc(a + off, 16, 1024), tc::make_desc(base + R::kState + k * 2048, R::kHalf, 1024),
                                   idesc<T>(128, kDv, 0, 1), k > 0);
                 }
-            }
-            ok = tc::mbar_wait(&ctl.c_full, n & 1);
-            if (!ok) break;
-            tc::tc_fence_after();
-#pragma unroll 1
-            for (int q = 0; q < R::kParts; ++q)
-#pragma unroll
-                for (int k = 0; k < kSteps / 16; ++k)
-                    tc::umma_bf16(tmem + kTmU, tc::make_desc(bt + k * 2048, R::kHalf, 1024),
-                                  tc::make_desc(base + R::kWeighted + q * R::kHalf + k * 2048, R::kHalf, 1024), idesc<T>(128, kDv, 1, 1), q + k > 0);
-            tc::umma_commit(&ctl.u_full);
-            if constexpr (!kEnds) {
-                ok = tc::mbar_wait(&ctl.p_full, n & 1);
+                tc::umma_commit(&ctl.x_empty);
+                ok = wait(&ctl.p_full, n & 1);
                 if (!ok) break;
                 tc::tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < kSteps / 16; ++k)
                     umma_ts(tmem + kTmO2, tmem + kTmP + k * 8, tc::make_desc(ct + k * 2048, R::kHalf, 1024), idesc<T>(128, kDv, 0, 1), k > 0);
                 tc::umma_commit(&ctl.out_full);
+                tc::umma_commit(&ctl.empty[s]);
             }
+            if (ok && chunks > 0) wait(&ctl.empty[(chunks - 1) & 1], ((chunks - 1) >> 1) & 1);       // nothing is under way at the end
+        }
+    } else if (warp == 3 && lane == 0) {
+        // ---- U
+        bool ok = true;
+        for (int n = 0; n < chunks && ok; ++n) {
+            const int s = n & 1;
+            const uint32_t bt = base + s * R::kStage + R::kA;
+            ok = wait(&ctl.full[s], (n >> 1) & 1) && (n != ragged || wait(&ctl.zeroed, 0)) &&
+                 (n == 0 || wait(&ctl.u_empty, (n - 1) & 1));
+            for (int half = 0; half < 2 && ok; ++half) {
+                ok = wait(&ctl.c_full[half], n & 1);
+                if (!ok) break;
+                tc::tc_fence_after();
+#pragma unroll 1
+                for (int q = 0; q < parts; ++q)
+#pragma unroll
+                    for (int k = 0; k < kSteps / 32; ++k) {
+                        const uint32_t rows = (half * 4 + k) * 2048;
+                        tc::umma_bf16(tmem + kTmU, tc::make_desc(bt + rows, R::kHalf, 1024),
+                                      tc::make_desc(base + R::kWeighted + q * R::kHalf + rows, R::kHalf, 1024), idesc<T>(128, kDv, 1, 1),
+                                      half + q + k > 0);
+                    }
+                tc::umma_commit(&ctl.c_empty[half]);
+            }
+            if (!ok) break;
+            tc::umma_commit(&ctl.u_full);
             tc::umma_commit(&ctl.empty[s]);
         }
-        if (ok && chunks > 0) tc::mbar_wait(&ctl.empty[(chunks - 1) & 1], ((chunks - 1) >> 1) & 1);       // nothing is under way at the end
+        if (ok && chunks > 0) wait(&ctl.empty[(chunks - 1) & 1], ((chunks - 1) >> 1) & 1);
     }
 
     pdl_trigger();
     tc::tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 3) {
         tc::tc_fence_after();
         tc::tmem_dealloc(tmem, 512);
     }
