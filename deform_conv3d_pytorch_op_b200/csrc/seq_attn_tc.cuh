@@ -43,7 +43,7 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
 #pragma unroll 1
         for (int i = 0; i < 64; ++i) {
             uint32_t done;
-            asm volatile("{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
+            asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
                          : "=r"(done) : "r"(at), "r"(parity) : "memory");
             if (done) return true;
         }
@@ -54,6 +54,14 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
     }
 }
 
+// From a table in shared memory that does not change any more, by its shared address (through a generic one the 32 loads of a block
+// of scores took 600 cycles)
+__device__ __forceinline__ float table(uint32_t at) {
+    float f;
+    asm("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(at));
+    return f;
+}
+
 template <typename T>
 __host__ __device__ constexpr uint32_t idesc(int m, int n, int a_mn_major, int b_mn_major) {
     const uint32_t fmt = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
@@ -61,11 +69,31 @@ __host__ __device__ constexpr uint32_t idesc(int m, int n, int a_mn_major, int b
            ((uint32_t)(m >> 4) << 24);
 }
 
-// D (+)= A B with A in tensor memory
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t id, uint32_t accumulate) {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
-                 "l"(b_desc), "r"(id), "r"(accumulate)
-                 : "memory");
+// Products and their commits are issued by one lane of a warp that runs as one, so that descriptors are in uniform registers
+__device__ __forceinline__ uint32_t elected() {
+    uint32_t yes;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(yes));
+    return yes;
+}
+// D (+)= A B of tiles in shared memory
+__device__ __forceinline__ void umma(uint32_t yes, uint32_t d, uint64_t a_desc, uint64_t b_desc, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a_desc), "l"(b_desc), "r"(id), "r"(accumulate), "r"(yes)
+        : "memory");
+}
+// ... with A in tensor memory
+__device__ __forceinline__ void umma_ts(uint32_t yes, uint32_t d, uint32_t a, uint64_t b_desc, uint32_t id, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n setp.ne.b32 q, %5, 0;\n @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b_desc), "r"(id), "r"(accumulate), "r"(yes)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t yes, uint64_t* bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(tc::smem_u32(bar)),
+        "r"(yes)
+        : "memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
     asm volatile(
@@ -143,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    const uint32_t tmem = ctl.tmem;
+    const uint32_t tmem = ctl.tmem, power = tc::smem_u32(ctl.power);
     const int64_t parts_of = ((int64_t)which * args.batch * args.heads + unit) * args.n_parts;
     // tiles that C' is the sum of
     const int parts = job.end != nullptr ? R::kParts : 2;
@@ -174,6 +202,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     } else if (warp >= 4 && warp < 8) {
         // ---- scores to weights, and the output
         if constexpr (!kEnds) {
+            const bool wide = job.wide != 0;
+            char* const out = static_cast<char*>(job.out);
             const int w = warp & 3, i = reverse ? kSteps - 1 - (w * 32 + lane) : w * 32 + lane;        // the position
             const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16);
             bool ok = true;
@@ -190,15 +220,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     if (back >= 0) {
                         tc::tmem_ld32(rows_at + kTmScores + cb * 32, v);
                         tc::tmem_ld_wait();
-                        const float* const f = ctl.power + 32 * back + (reverse ? -lane : lane);
+                        const uint32_t f = power + 4 * (32 * back + (reverse ? -lane : lane));
                         if (reverse) {
 #pragma unroll
                             for (int k = 0; k < 16; ++k)
-                                v[k] = word_of<T>(__uint_as_float(v[2 * k]) * f[2 * k], __uint_as_float(v[2 * k + 1]) * f[2 * k + 1]);
+                                v[k] = word_of<T>(__uint_as_float(v[2 * k]) * table(f + 8 * k), __uint_as_float(v[2 * k + 1]) * table(f + 8 * k + 4));
                         } else {
 #pragma unroll
                             for (int k = 0; k < 16; ++k)
-                                v[k] = word_of<T>(__uint_as_float(v[2 * k]) * f[-2 * k], __uint_as_float(v[2 * k + 1]) * f[-2 * k - 1]);
+                                v[k] = word_of<T>(__uint_as_float(v[2 * k]) * table(f - 8 * k), __uint_as_float(v[2 * k + 1]) * table(f - 8 * k - 4));
                         }
                     } else {
 #pragma unroll
@@ -215,8 +245,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 __syncwarp();
                 tc::tc_fence_after();
                 const int64_t pos = begin + (int64_t)n * kSteps + i;
-                const float w1 = ctl.power[i + extra] * ctl.up[n & 1];
-                const Lanes f1 = all_lanes(w1 * args.scale), f2 = all_lanes(args.scale);
+                const float scale = args.scale, w1 = table(power + 4 * (i + extra)) * ctl.up[n & 1] * scale;
                 const int64_t step = reverse ? length - 1 - pos : pos, at = (((int64_t)b * steps + step) * args.heads + h) * wc + col0;
 #pragma unroll 1
                 for (int cb = 0; cb < 2; ++cb) {
@@ -231,19 +260,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     if (pos < finish) {
                     float o[32];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        const float a[2] = {__uint_as_float(p[k]), __uint_as_float(p[k + 1])}, c[2] = {__uint_as_float(q[k]), __uint_as_float(q[k + 1])};
-                        const Lanes r = fma(lanes(a), f1, lanes(c) * f2);
-                        o[k] = r.at(0), o[k + 1] = r.at(1);
-                    }
+                    for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(p[k]), w1, __uint_as_float(q[k]) * scale);
 #pragma unroll
                     for (int k = 0; k < 32; k += 8) {            // (widths are multiples of 8)
                         if (col0 + cb * 32 + k >= wc) continue;
-                        if (job.wide) {
-                            float4* const d = reinterpret_cast<float4*>(static_cast<float*>(job.out) + at + cb * 32 + k);
+                        if (wide) {
+                            float4* const d = reinterpret_cast<float4*>(out + (at + cb * 32 + k) * 4);
                             d[0] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]), d[1] = make_float4(o[k + 4], o[k + 5], o[k + 6], o[k + 7]);
                         } else {
-                            store(static_cast<T*>(job.out) + at + cb * 32 + k,
+                            store(out + (at + cb * 32 + k) * 2,
                                   Raw<16>{{word_of<T>(o[k], o[k + 1]), word_of<T>(o[k + 2], o[k + 3]), word_of<T>(o[k + 4], o[k + 5]),
                                            word_of<T>(o[k + 6], o[k + 7])}});
                         }
@@ -288,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
 #pragma unroll 1
                 for (int p = 0; p < 4; ++p) {
                     const int row = r0 + 16 * p + 64 * half, j = reverse ? kSteps - 1 - row : row;
-                    const Lanes f = all_lanes(j < rows ? ctl.power[max(top - j, 0)] : 0.0f);
+                    const Lanes f = all_lanes(j < rows ? table(power + 4 * max(top - j, 0)) : 0.0f);
                     const uint4 v = tc::lds128(from + p * 2048);
                     const uint32_t in[4] = {v.x, v.y, v.z, v.w};
                     uint32_t out[R::kParts][4];
@@ -298,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                         Lanes r = lanes(e) * f;
 #pragma unroll
                         for (int q = 0; q < R::kParts; ++q) {
+                            if (q == 2 && parts <= 2) break;
                             out[q][k] = word_of<T>(r.at(0), r.at(1));
                             if (q + 1 < R::kParts) {
                                 const float t[2] = {half_of<T>(out[q][k], 0), half_of<T>(out[q][k], 1)};
@@ -376,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         if constexpr (!kEnds) put_copy(0);
         for (int n = 0; n < chunks; ++n) {
             const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps);
-            const Lanes whole = all_lanes(ctl.power[rows]);
+            const Lanes whole = all_lanes(table(power + 4 * rows));
             ok = wait(&ctl.u_full, n & 1);
             if (!ok) break;
             __syncwarp();
@@ -417,68 +443,74 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         }
     } else if (warp == 2) {
         // ---- the products with A
-        if (!kEnds && lane == 0) {
+        if (!kEnds) {
             bool ok = true;
+            const uint32_t yes = elected();
+            const uint64_t a_desc = tc::make_desc(base, 16, 1024), b_desc = tc::make_desc(base + R::kA, 16, 1024);
+            const uint64_t c_desc = tc::make_desc(base + 2 * R::kA, R::kHalf, 1024), x_desc = tc::make_desc(base + R::kState, R::kHalf, 1024);
             for (int n = 0; n < chunks && ok; ++n) {
                 const int s = n & 1;
-                const uint32_t a = base + s * R::kStage, bt = a + R::kA, ct = a + 2 * R::kA;
+                const uint64_t stage = (uint64_t)(s * R::kStage >> 4);
                 ok = wait(&ctl.full[s], (n >> 1) & 1) && (n != ragged || wait(&ctl.zeroed, 0)) &&
                      (n == 0 || wait(&ctl.scores_empty, (n - 1) & 1));
                 if (!ok) break;
+                __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < KA / 16; ++k) {
-                    const uint32_t off = (k >> 2) * R::kHalf + (k & 3) * 32;
-                    tc::umma_bf16(tmem + kTmScores, tc::make_desc(a + off, 16, 1024), tc::make_desc(bt + off, 16, 1024), idesc<T>(128, 128, 0, 0), k > 0);
+                    const uint64_t off = stage + ((k >> 2) * R::kHalf + (k & 3) * 32 >> 4);
+                    umma(yes, tmem + kTmScores, a_desc + off, b_desc + off, idesc<T>(128, 128, 0, 0), k > 0);
                 }
-                tc::umma_commit(&ctl.scores_full);
+                commit(yes, &ctl.scores_full);
                 ok = wait(&ctl.x_full, n & 1) && (n == 0 || wait(&ctl.out_empty, (n - 1) & 1));
                 if (!ok) break;
+                __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll
-                for (int k = 0; k < KA / 16; ++k) {
-                    const uint32_t off = (k >> 2) * R::kHalf + (k & 3) * 32;
-                    tc::umma_bf16(tmem + kTmO1, tc::make_desc(a + off, 16, 1024), tc::make_desc(base + R::kState + k * 2048, R::kHalf, 1024),
+                for (int k = 0; k < KA / 16; ++k)
+                    umma(yes, tmem + kTmO1, a_desc + stage + ((k >> 2) * R::kHalf + (k & 3) * 32 >> 4), x_desc + (k * 2048 >> 4),
                                   idesc<T>(128, kDv, 0, 1), k > 0);
-                }
-                tc::umma_commit(&ctl.x_empty);
+                commit(yes, &ctl.x_empty);
                 ok = wait(&ctl.p_full, n & 1);
                 if (!ok) break;
+                __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < kSteps / 16; ++k)
-                    umma_ts(tmem + kTmO2, tmem + kTmP + k * 8, tc::make_desc(ct + k * 2048, R::kHalf, 1024), idesc<T>(128, kDv, 0, 1), k > 0);
-                tc::umma_commit(&ctl.out_full);
-                tc::umma_commit(&ctl.empty[s]);
+                    umma_ts(yes, tmem + kTmO2, tmem + kTmP + k * 8, c_desc + stage + (k * 2048 >> 4), idesc<T>(128, kDv, 0, 1), k > 0);
+                commit(yes, &ctl.out_full);
+                commit(yes, &ctl.empty[s]);
             }
             if (ok && chunks > 0) wait(&ctl.empty[(chunks - 1) & 1], ((chunks - 1) >> 1) & 1);       // nothing is under way at the end
         }
-    } else if (warp == 3 && lane == 0) {
+    } else if (warp == 3) {
         // ---- U
         bool ok = true;
+        const uint32_t yes = elected();
+        const uint64_t b_desc = tc::make_desc(base + R::kA, R::kHalf, 1024), w_desc = tc::make_desc(base + R::kWeighted, R::kHalf, 1024);
         for (int n = 0; n < chunks && ok; ++n) {
             const int s = n & 1;
-            const uint32_t bt = base + s * R::kStage + R::kA;
+            const uint64_t stage = (uint64_t)(s * R::kStage >> 4);
             ok = wait(&ctl.full[s], (n >> 1) & 1) && (n != ragged || wait(&ctl.zeroed, 0)) &&
                  (n == 0 || wait(&ctl.u_empty, (n - 1) & 1));
             for (int half = 0; half < 2 && ok; ++half) {
                 ok = wait(&ctl.c_full[half], n & 1);
                 if (!ok) break;
+                __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll 1
                 for (int q = 0; q < parts; ++q)
 #pragma unroll
                     for (int k = 0; k < kSteps / 32; ++k) {
-                        const uint32_t rows = (half * 4 + k) * 2048;
-                        tc::umma_bf16(tmem + kTmU, tc::make_desc(bt + rows, R::kHalf, 1024),
-                                      tc::make_desc(base + R::kWeighted + q * R::kHalf + rows, R::kHalf, 1024), idesc<T>(128, kDv, 1, 1),
+                        const uint64_t rows = (uint64_t)(half * 4 + k) * (2048 >> 4);
+                        umma(yes, tmem + kTmU, b_desc + stage + rows, w_desc + (uint64_t)q * (R::kHalf >> 4) + rows, idesc<T>(128, kDv, 1, 1),
                                       half + q + k > 0);
                     }
-                tc::umma_commit(&ctl.c_empty[half]);
+                commit(yes, &ctl.c_empty[half]);
             }
             if (!ok) break;
-            tc::umma_commit(&ctl.u_full);
-            tc::umma_commit(&ctl.empty[s]);
+            commit(yes, &ctl.u_full);
+            commit(yes, &ctl.empty[s]);
         }
         if (ok && chunks > 0) wait(&ctl.empty[(chunks - 1) & 1], ((chunks - 1) >> 1) & 1);
     }
