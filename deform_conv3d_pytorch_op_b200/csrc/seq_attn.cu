@@ -47,6 +47,7 @@ struct Job {
     int reverse, wide;
     float init_scale, end_scale;
     int pairs;                                   // out's rows start on two elements
+    int sectors;                                 // ... and on 32 bytes, which all columns fill
 };
 
 struct AttnArgs {
@@ -814,6 +815,7 @@ void add(AttnArgs& a, const Job& j, int elem) {
     a.tile_of[a.jobs] = (j.c.width + kCols - 1) / kCols;
     a.tiles = std::max(a.tiles, a.tile_of[a.jobs]);
     a.job[a.jobs] = j;
+    a.job[a.jobs].sectors = j.c.width % 16 == 0 && aligned(j.out, 32);
     a.job[a.jobs++].pairs = j.c.width % 2 == 0 && aligned(j.out, 2 * (j.wide ? 4 : elem));
 }
 

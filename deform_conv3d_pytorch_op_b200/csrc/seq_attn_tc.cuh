@@ -8,27 +8,28 @@
 // float32's own 2^-24 (three) where it is a result; two of float16 are exact to 2^-22.  X is in the registers of four warps in float32, and
 // meets A as a rounded copy in shared memory.
 //
-// A CTA has one job's head (or a part of its time axis) and 64 columns of c: two chunks' tiles, C' and X fill shared memory.  One
-// thread loads (TMA, a chunk ahead), four warps make P and the output, four make C' (half a chunk ahead of its product), four keep the
-// state, and two threads issue the products, one those with A, one U, so that neither chain waits for the other's operands.
+// A CTA has one job's head (or a part of its time axis) and 64 columns of c: two chunks' tiles (three of up to 64 columns), C' and X fill
+// shared memory.  One warp loads (TMA), three issue products (scores and O1, O2, U), each as soon as its own operands are there, four
+// make P, four the output, four C' (half a chunk ahead of its product), four keep the state.
 //
 // Rows of a tile are steps in the order of time.  Back in time, position i of a chunk is row 127 - i, and triangle and weights are mirrored.
 namespace tcgen {
 
-constexpr int kSteps = 128, kDv = 64, kThreads = 16 * 32;
-constexpr uint32_t kTmScores = 0, kTmO1 = 128, kTmO2 = 192, kTmU = 256, kTmP = 320;      // columns of tensor memory
+constexpr int kSteps = 128, kDv = 64, kThreads = 20 * 32;
+constexpr uint32_t kTmScores = 0, kTmO1 = 128, kTmO2 = 192, kTmU = 256, kTmP = 320;      // columns of tensor memory; two of P
 
 template <typename T, int KA>
 struct Room {
     static constexpr int kParts = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;
     static constexpr int kHalf = kSteps * 128;                   // bytes of a tile of 64 columns
-    static constexpr int kA = KA / 64 * kHalf, kStage = 2 * kA + kHalf;
-    static constexpr int kWeighted = 2 * kStage, kState = kWeighted + kParts * kHalf, kControl = kState + KA * 128;
+    static constexpr int kA = KA / 64 * kHalf, kStage = 2 * kA + kHalf, kStages = KA == 64 ? 3 : 2;
+    static constexpr int kWeighted = kStages * kStage, kState = kWeighted + kParts * kHalf, kControl = kState + KA * 128;
     static constexpr int kBytes = kControl + 2048 + 1024;        // (and what aligns it to 1024)
 };
 
 struct Control {
-    uint64_t full[2], empty[2], zeroed, scores_full, scores_empty, p_full, out_full, out_empty, c_full[2], c_empty[2], u_full, u_empty, x_full, x_empty;
+    uint64_t full[3], full_c[3], empty[3], zeroed, scores_full, scores_empty, p_full, p_empty[2], out_full, out_empty, c_full[2], c_empty[2], u_full, u_empty,
+        x_full, x_empty;
     uint32_t tmem;
     float up[2], most[4];
     float none[32], power[kSteps + 1];           // g^n behind 32 zeros for what is not before a step
@@ -140,10 +141,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         tc::tmem_relinquish();
     }
     if (threadIdx.x == 0) {
-        for (int s = 0; s < 2; ++s) {
-            tc::mbar_init(&ctl.full[s], 1), tc::mbar_init(&ctl.empty[s], (kEnds ? 1 : 2) + 4);
-            tc::mbar_init(&ctl.c_full[s], 4), tc::mbar_init(&ctl.c_empty[s], 1);
-        }
+        for (int s = 0; s < R::kStages; ++s) tc::mbar_init(&ctl.full[s], 1), tc::mbar_init(&ctl.full_c[s], 1), tc::mbar_init(&ctl.empty[s], 1 + 4 + (kEnds ? 0 : 2));
+        for (int s = 0; s < 2; ++s) tc::mbar_init(&ctl.c_full[s], 4), tc::mbar_init(&ctl.c_empty[s], 1), tc::mbar_init(&ctl.p_empty[s], 1);
         tc::mbar_init(&ctl.zeroed, 4);
         tc::mbar_init(&ctl.scores_full, 1), tc::mbar_init(&ctl.scores_empty, 4), tc::mbar_init(&ctl.p_full, 4);
         tc::mbar_init(&ctl.out_full, 1), tc::mbar_init(&ctl.out_empty, 4);
@@ -183,33 +182,33 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         // ---- loads
         if (lane == 0) {
             int n = 0;
-            for (; n < chunks; ++n) {
-                uint64_t* const bar = &ctl.full[n & 1];
-                if (n >= 2 && !wait(&ctl.empty[n & 1], ((n >> 1) & 1) ^ 1)) break;
-                const uint32_t to = base + (n & 1) * R::kStage;
+            tc::Ring ring;
+            for (; n < chunks; ++n, ring.next(R::kStages)) {
+                uint64_t* const bar = &ctl.full[ring.i];
+                if (n >= R::kStages && !wait(&ctl.empty[ring.i], ring.ph ^ 1)) break;
+                const uint32_t to = base + ring.i * R::kStage;
                 const int64_t first = begin + (int64_t)n * kSteps;
                 const int t = (int)(reverse ? length - kSteps - first : first);
-                tc::mbar_arrive_expect_tx(bar, (kEnds ? R::kA : 2 * R::kA) + R::kHalf);
+                tc::mbar_arrive_expect_tx(bar, kEnds ? R::kA : 2 * R::kA);
 #pragma unroll
                 for (int k = 0; k < KA / 64; ++k) {
-                    if constexpr (!kEnds) load_box(to + k * R::kHalf, maps.of[job.a.map], 64 * k, h / job.a.share, t, b, bar);
                     load_box(to + R::kA + k * R::kHalf, maps.of[job.b.map], 64 * k, h / job.b.share, t, b, bar);
+                    if constexpr (!kEnds) load_box(to + k * R::kHalf, maps.of[job.a.map], 64 * k, h / job.a.share, t, b, bar);
                 }
-                load_box(to + 2 * R::kA, maps.of[job.c.map], col0, h / job.c.share, t, b, bar);
+                tc::mbar_arrive_expect_tx(&ctl.full_c[ring.i], R::kHalf);
+                load_box(to + 2 * R::kA, maps.of[job.c.map], col0, h / job.c.share, t, b, &ctl.full_c[ring.i]);
             }
-            for (int k = max(n - 2, 0); k < n; ++k) wait(&ctl.full[k & 1], (k >> 1) & 1);       // (nothing is under way at the end)
+            for (int k = max(n - R::kStages, 0); k < n; ++k)     // (nothing is under way at the end)
+                wait(&ctl.full[k % R::kStages], k / R::kStages & 1), wait(&ctl.full_c[k % R::kStages], k / R::kStages & 1);
         }
     } else if (warp >= 4 && warp < 8) {
-        // ---- scores to weights, and the output
+        // ---- scores to weights
         if constexpr (!kEnds) {
-            const bool wide = job.wide != 0;
-            char* const out = static_cast<char*>(job.out);
-            const int w = warp & 3, i = reverse ? kSteps - 1 - (w * 32 + lane) : w * 32 + lane;        // the position
+            const int w = warp & 3;
             const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16);
-            bool ok = true;
             for (int n = 0; n < chunks; ++n) {
-                ok = wait(&ctl.scores_full, n & 1);
-                if (!ok) break;
+                if (n >= 2 && !wait(&ctl.p_empty[n & 1], ((n >> 1) & 1) ^ 1)) break;
+                if (!wait(&ctl.scores_full, n & 1)) break;
                 __syncwarp();
                 tc::tc_fence_after();
                 // (short code in loops: the roles' instructions together would not stay in the caches that feed the schedulers)
@@ -234,53 +233,73 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
 #pragma unroll
                         for (int k = 0; k < 16; ++k) v[k] = 0;
                     }
-                    tmem_st16(rows_at + kTmP + cb * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
+                    tmem_st16(rows_at + kTmP + (n & 1) * 64 + cb * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
                 }
                 tmem_st_wait();
                 tc::tc_fence_before();
                 tc::mbar_arrive_warp(&ctl.scores_empty);
                 tc::mbar_arrive_warp(&ctl.p_full);
-                ok = wait(&ctl.out_full, n & 1);
-                if (!ok) break;
+            }
+        }
+    } else if (warp >= 8 && warp < 12) {
+        // ---- the output
+        if constexpr (!kEnds) {
+            const bool wide = job.wide != 0;
+            char* const out = static_cast<char*>(job.out);
+            const int w = warp & 3, r = w * 32 + lane, i = reverse ? kSteps - 1 - r : r;     // the row, and its position
+            const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16);
+            const float scale = args.scale, weight = table(power + 4 * (i + extra)) * scale;
+            const int64_t row_bytes = (int64_t)args.heads * wc * (wide ? 4 : 2);
+            char* const first_row = out + (((int64_t)b * steps * args.heads + h) * wc + col0) * (wide ? 4 : 2);
+            for (int n = 0; n < chunks; ++n) {
+                if (!wait(&ctl.x_empty, n & 1) || !wait(&ctl.out_full, n & 1)) break;       // O1 and O2
                 __syncwarp();
                 tc::tc_fence_after();
-                const int64_t pos = begin + (int64_t)n * kSteps + i;
-                const float scale = args.scale, w1 = table(power + 4 * (i + extra)) * ctl.up[n & 1] * scale;
-                const int64_t step = reverse ? length - 1 - pos : pos, at = (((int64_t)b * steps + step) * args.heads + h) * wc + col0;
+                const float w1 = weight * ctl.up[n & 1];
+                const bool in = i < (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps);
+                const int64_t t = reverse ? length - kSteps - begin - (int64_t)n * kSteps + r : begin + (int64_t)n * kSteps + r;
+                char* to = first_row + t * row_bytes;
 #pragma unroll 1
-                for (int cb = 0; cb < 2; ++cb) {
-                    uint32_t p[32], q[32];
-                    tc::tmem_ld32(rows_at + kTmO1 + cb * 32, p);
-                    tc::tmem_ld32(rows_at + kTmO2 + cb * 32, q);
+                for (int cb = 0; cb < 4; ++cb) {
+                    uint32_t p[16], q[16];
+                    tc::tmem_ld16(rows_at + kTmO1 + cb * 16, p);
+                    tc::tmem_ld16(rows_at + kTmO2 + cb * 16, q);
                     tc::tmem_ld_wait();
-                    if (cb == 1) {
+                    if (cb == 3) {
                         tc::tc_fence_before();
                         tc::mbar_arrive_warp(&ctl.out_empty);
                     }
-                    if (pos < finish) {
-                    float o[32];
+                    float o[16];
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) o[k] = fmaf(__uint_as_float(p[k]), w1, __uint_as_float(q[k]) * scale);
-#pragma unroll
-                    for (int k = 0; k < 32; k += 8) {            // (widths are multiples of 8)
-                        if (col0 + cb * 32 + k >= wc) continue;
+                    for (int k = 0; k < 16; ++k) o[k] = fmaf(__uint_as_float(p[k]), w1, __uint_as_float(q[k]) * scale);
+                    if (in && col0 + cb * 16 < wc) {             // (widths are multiples of 8)
+                        const bool both = col0 + cb * 16 + 8 < wc;
                         if (wide) {
-                            float4* const d = reinterpret_cast<float4*>(out + (at + cb * 32 + k) * 4);
-                            d[0] = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]), d[1] = make_float4(o[k + 4], o[k + 5], o[k + 6], o[k + 7]);
+#pragma unroll
+                            for (int k = 0; k < 16; k += 4)
+                                if (k < 8 || both) *reinterpret_cast<float4*>(to + k * 4) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                         } else {
-                            store(out + (at + cb * 32 + k) * 2,
-                                  Raw<16>{{word_of<T>(o[k], o[k + 1]), word_of<T>(o[k + 2], o[k + 3]), word_of<T>(o[k + 4], o[k + 5]),
-                                           word_of<T>(o[k + 6], o[k + 7])}});
+                            uint32_t v[8];
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) v[k] = word_of<T>(o[2 * k], o[2 * k + 1]);
+                            if (job.sectors) {                   // whole sectors of 32 bytes
+                                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+                                             "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                                             : "memory");
+                            } else {
+                                store(to, Raw<16>{{v[0], v[1], v[2], v[3]}});
+                                if (both) store(to + 16, Raw<16>{{v[4], v[5], v[6], v[7]}});
+                            }
                         }
                     }
-                    }
+                    to += wide ? 64 : 32;
                     __syncwarp();
                 }
             }
             // zeros behind the length
             const int64_t from = max(begin, length);
             const int cols = min(kDv, wc - col0) / 8;
-            for (int64_t k = threadIdx.x - 128; k < (stop - from) * cols; k += 128) {
+            for (int64_t k = threadIdx.x - 256; k < (stop - from) * cols; k += 128) {
                 const int64_t at = (((int64_t)b * steps + from + k / cols) * args.heads + h) * wc + col0 + k % cols * 8;
                 if (job.wide) {
                     float4* const d = reinterpret_cast<float4*>(static_cast<float*>(job.out) + at);
@@ -290,16 +309,17 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
             }
         }
-    } else if (warp >= 8 && warp < 12) {
+    } else if (warp >= 12 && warp < 16) {
         // ---- the weighted c, half a chunk at a time
-        const int tid = threadIdx.x - 256, c = tid & 7, r0 = tid >> 3;           // 16 bytes of rows r0, r0 + 16, ...
+        const int tid = threadIdx.x - 384, c = tid & 7, r0 = tid >> 3;           // 16 bytes of rows r0, r0 + 16, ...
         const uint32_t place = tc::swz_offset(r0, c);
         bool ok = true;
-        for (int n = 0; n < chunks && ok; ++n) {
-            ok = wait(&ctl.full[n & 1], (n >> 1) & 1);
+        tc::Ring ring;
+        for (int n = 0; n < chunks && ok; ++n, ring.next(R::kStages)) {
+            ok = wait(&ctl.full_c[ring.i], ring.ph);
             const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps), top = rows - extra;
-            if (ok && n == ragged) {
-                const uint32_t tile = base + (n & 1) * R::kStage + R::kA;        // b's halves, and c's behind them
+            if (ok && n == ragged && wait(&ctl.full[ring.i], ring.ph)) {
+                const uint32_t tile = base + ring.i * R::kStage + R::kA;        // b's halves, and c's behind them
                 for (int k = tid; k < (KA / 64 + 1) * (kSteps - rows) * 8; k += 128)
                     tc::st_shared_v4(tile + k / ((kSteps - rows) * 8) * R::kHalf + tc::swz_offset(rows + k / 8 % (kSteps - rows), k % 8), 0, 0, 0, 0);
                 tc::fence_proxy_async_smem();
@@ -309,7 +329,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             for (int half = 0; half < 2 && ok; ++half) {
                 ok = n == 0 || wait(&ctl.c_empty[half], (n - 1) & 1);
                 if (!ok) break;
-                const uint32_t from = base + (n & 1) * R::kStage + 2 * R::kA + place + half * 8192, to = base + R::kWeighted + place + half * 8192;
+                const uint32_t from = base + ring.i * R::kStage + 2 * R::kA + place + half * 8192, to = base + R::kWeighted + place + half * 8192;
 #pragma unroll 1
                 for (int p = 0; p < 4; ++p) {
                     const int row = r0 + 16 * p + 64 * half, j = reverse ? kSteps - 1 - row : row;
@@ -338,11 +358,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 tc::fence_proxy_async_smem();
                 tc::mbar_arrive_warp(&ctl.c_full[half]);
             }
-            if (ok) tc::mbar_arrive_warp(&ctl.empty[n & 1]);
+            if (ok) tc::mbar_arrive_warp(&ctl.empty[ring.i]);
         }
-    } else if (warp >= 12) {
+    } else if (warp >= 16) {
         // ---- the state
-        const int tid = threadIdx.x - 384, w = warp & 3, i = w * 32 + lane;
+        const int tid = threadIdx.x - 512, w = warp & 3, i = w * 32 + lane;
         const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16) + kTmU;
         const bool mine = i < KA;                // (the products have 128 rows: behind a's 64 columns they find those of c)
         float x[kDv];
@@ -408,19 +428,19 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             __syncwarp();
             tc::tc_fence_after();
 #pragma unroll
-            for (int cb = 0; cb < 2; ++cb) {
-                uint32_t v[32];
-                tc::tmem_ld32(rows_at + cb * 32, v);
+            for (int cb = 0; cb < 4; ++cb) {
+                uint32_t v[16];
+                tc::tmem_ld16(rows_at + cb * 16, v);
                 tc::tmem_ld_wait();
-                if (cb == 1) {
+                if (cb == 3) {
                     tc::tc_fence_before();
                     tc::mbar_arrive_warp(&ctl.u_empty);
                 }
 #pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                    const float a[2] = {x[cb * 32 + k], x[cb * 32 + k + 1]}, e[2] = {__uint_as_float(v[k]), __uint_as_float(v[k + 1])};
+                for (int k = 0; k < 16; k += 2) {
+                    const float a[2] = {x[cb * 16 + k], x[cb * 16 + k + 1]}, e[2] = {__uint_as_float(v[k]), __uint_as_float(v[k + 1])};
                     const Lanes r = fma(lanes(a), whole, lanes(e));
-                    x[cb * 32 + k] = r.at(0), x[cb * 32 + k + 1] = r.at(1);
+                    x[cb * 16 + k] = r.at(0), x[cb * 16 + k + 1] = r.at(1);
                 }
             }
             if constexpr (!kEnds) {
@@ -441,19 +461,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 if (col0 + k < wc)
                     *reinterpret_cast<float4*>(to + (int64_t)i * wc + col0 + k) = make_float4(by * x[k], by * x[k + 1], by * x[k + 2], by * x[k + 3]);
         }
-    } else if (warp == 2) {
-        // ---- the products with A
-        if (!kEnds) {
-            bool ok = true;
+    } else if (warp == 1) {
+        // ---- scores and O1
+        if constexpr (!kEnds) {
             const uint32_t yes = elected();
             const uint64_t a_desc = tc::make_desc(base, 16, 1024), b_desc = tc::make_desc(base + R::kA, 16, 1024);
-            const uint64_t c_desc = tc::make_desc(base + 2 * R::kA, R::kHalf, 1024), x_desc = tc::make_desc(base + R::kState, R::kHalf, 1024);
-            for (int n = 0; n < chunks && ok; ++n) {
-                const int s = n & 1;
-                const uint64_t stage = (uint64_t)(s * R::kStage >> 4);
-                ok = wait(&ctl.full[s], (n >> 1) & 1) && (n != ragged || wait(&ctl.zeroed, 0)) &&
-                     (n == 0 || wait(&ctl.scores_empty, (n - 1) & 1));
-                if (!ok) break;
+            const uint64_t x_desc = tc::make_desc(base + R::kState, R::kHalf, 1024);
+            tc::Ring ring;
+            for (int n = 0; n < chunks; ++n, ring.next(R::kStages)) {
+                const uint64_t stage = (uint64_t)(ring.i * R::kStage >> 4);
+                if (!wait(&ctl.full[ring.i], ring.ph) || (n == ragged && !wait(&ctl.zeroed, 0)) || (n > 0 && !wait(&ctl.scores_empty, (n - 1) & 1))) break;
                 __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll
@@ -462,37 +479,47 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     umma(yes, tmem + kTmScores, a_desc + off, b_desc + off, idesc<T>(128, 128, 0, 0), k > 0);
                 }
                 commit(yes, &ctl.scores_full);
-                ok = wait(&ctl.x_full, n & 1) && (n == 0 || wait(&ctl.out_empty, (n - 1) & 1));
-                if (!ok) break;
+                if (!wait(&ctl.x_full, n & 1) || (n > 0 && !wait(&ctl.out_empty, (n - 1) & 1))) break;
                 __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < KA / 16; ++k)
                     umma(yes, tmem + kTmO1, a_desc + stage + ((k >> 2) * R::kHalf + (k & 3) * 32 >> 4), x_desc + (k * 2048 >> 4),
-                                  idesc<T>(128, kDv, 0, 1), k > 0);
+                         idesc<T>(128, kDv, 0, 1), k > 0);
                 commit(yes, &ctl.x_empty);
-                ok = wait(&ctl.p_full, n & 1);
-                if (!ok) break;
+                commit(yes, &ctl.empty[ring.i]);
+            }
+        }
+    } else if (warp == 2) {
+        // ---- O2
+        if constexpr (!kEnds) {
+            const uint32_t yes = elected();
+            const uint64_t c_desc = tc::make_desc(base + 2 * R::kA, R::kHalf, 1024);
+            tc::Ring ring;
+            for (int n = 0; n < chunks; ++n, ring.next(R::kStages)) {
+                const uint64_t stage = (uint64_t)(ring.i * R::kStage >> 4);
+                if (!wait(&ctl.full_c[ring.i], ring.ph) || (n == ragged && !wait(&ctl.zeroed, 0)) || !wait(&ctl.p_full, n & 1) ||
+                    (n > 0 && !wait(&ctl.out_empty, (n - 1) & 1)))
+                    break;
                 __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < kSteps / 16; ++k)
-                    umma_ts(yes, tmem + kTmO2, tmem + kTmP + k * 8, c_desc + stage + (k * 2048 >> 4), idesc<T>(128, kDv, 0, 1), k > 0);
+                    umma_ts(yes, tmem + kTmO2, tmem + kTmP + (n & 1) * 64 + k * 8, c_desc + stage + (k * 2048 >> 4), idesc<T>(128, kDv, 0, 1), k > 0);
+                commit(yes, &ctl.p_empty[n & 1]);
                 commit(yes, &ctl.out_full);
-                commit(yes, &ctl.empty[s]);
+                commit(yes, &ctl.empty[ring.i]);
             }
-            if (ok && chunks > 0) wait(&ctl.empty[(chunks - 1) & 1], ((chunks - 1) >> 1) & 1);       // nothing is under way at the end
         }
     } else if (warp == 3) {
         // ---- U
-        bool ok = true;
         const uint32_t yes = elected();
         const uint64_t b_desc = tc::make_desc(base + R::kA, R::kHalf, 1024), w_desc = tc::make_desc(base + R::kWeighted, R::kHalf, 1024);
-        for (int n = 0; n < chunks && ok; ++n) {
-            const int s = n & 1;
-            const uint64_t stage = (uint64_t)(s * R::kStage >> 4);
-            ok = wait(&ctl.full[s], (n >> 1) & 1) && (n != ragged || wait(&ctl.zeroed, 0)) &&
-                 (n == 0 || wait(&ctl.u_empty, (n - 1) & 1));
+        bool ok = true;
+        tc::Ring ring;
+        for (int n = 0; n < chunks && ok; ++n, ring.next(R::kStages)) {
+            const uint64_t stage = (uint64_t)(ring.i * R::kStage >> 4);
+            ok = wait(&ctl.full[ring.i], ring.ph) && (n != ragged || wait(&ctl.zeroed, 0)) && (n == 0 || wait(&ctl.u_empty, (n - 1) & 1));
             for (int half = 0; half < 2 && ok; ++half) {
                 ok = wait(&ctl.c_full[half], n & 1);
                 if (!ok) break;
@@ -504,16 +531,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     for (int k = 0; k < kSteps / 32; ++k) {
                         const uint64_t rows = (uint64_t)(half * 4 + k) * (2048 >> 4);
                         umma(yes, tmem + kTmU, b_desc + stage + rows, w_desc + (uint64_t)q * (R::kHalf >> 4) + rows, idesc<T>(128, kDv, 1, 1),
-                                      half + q + k > 0);
+                             half + q + k > 0);
                     }
                 commit(yes, &ctl.c_empty[half]);
             }
             if (!ok) break;
             commit(yes, &ctl.u_full);
-            commit(yes, &ctl.empty[s]);
+            commit(yes, &ctl.empty[ring.i]);
         }
-        if (ok && chunks > 0) wait(&ctl.empty[(chunks - 1) & 1], ((chunks - 1) >> 1) & 1);
     }
+    // nothing is under way at the end: the last chunks' places have been given back by all who read them
+    if (warp == 3)
+        for (int k = max(chunks - R::kStages, 0); k < chunks; ++k) wait(&ctl.empty[k % R::kStages], k / R::kStages & 1);
 
     pdl_trigger();
     tc::tc_fence_before();
