@@ -16,7 +16,7 @@
 namespace tcgen {
 
 constexpr int kSteps = 128, kDv = 64, kThreads = 20 * 32;
-constexpr uint32_t kTmScores = 0, kTmO1 = 128, kTmO2 = 192, kTmU = 256, kTmP = 320;      // columns of tensor memory; two of P
+constexpr uint32_t kTmScores = 0, kTmU = 128, kTmP = 192, kTmO1 = 256, kTmO2 = 320, kTmTurn = 128;  // columns of tensor memory; O1 and O2 twice
 
 template <typename T, int KA>
 struct Room {
@@ -28,10 +28,10 @@ struct Room {
 };
 
 struct Control {
-    uint64_t full[3], full_c[3], empty[3], zeroed, scores_full, scores_empty, p_full, p_empty[2], out_full, out_empty, c_full[2], c_empty[2], u_full, u_empty,
+    uint64_t full[3], full_c[3], empty[3], zeroed, scores_full, scores_empty, p_full, p_empty, out_full[2], out_empty[2], c_full[2], c_empty[2], u_full, u_empty,
         x_full, x_empty;
     uint32_t tmem;
-    float up[2], most[4];
+    float up[4], most[4];
     float none[32], power[kSteps + 1];           // g^n behind 32 zeros for what is not before a step
 };
 
@@ -142,10 +142,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < R::kStages; ++s) tc::mbar_init(&ctl.full[s], 1), tc::mbar_init(&ctl.full_c[s], 1), tc::mbar_init(&ctl.empty[s], 1 + 4 + (kEnds ? 0 : 2));
-        for (int s = 0; s < 2; ++s) tc::mbar_init(&ctl.c_full[s], 4), tc::mbar_init(&ctl.c_empty[s], 1), tc::mbar_init(&ctl.p_empty[s], 1);
+        for (int s = 0; s < 2; ++s) tc::mbar_init(&ctl.c_full[s], 4), tc::mbar_init(&ctl.c_empty[s], 1), tc::mbar_init(&ctl.out_full[s], 1), tc::mbar_init(&ctl.out_empty[s], 4);
         tc::mbar_init(&ctl.zeroed, 4);
         tc::mbar_init(&ctl.scores_full, 1), tc::mbar_init(&ctl.scores_empty, 4), tc::mbar_init(&ctl.p_full, 4);
-        tc::mbar_init(&ctl.out_full, 1), tc::mbar_init(&ctl.out_empty, 4);
+        tc::mbar_init(&ctl.p_empty, 1);
         tc::mbar_init(&ctl.u_full, 1), tc::mbar_init(&ctl.u_empty, 4), tc::mbar_init(&ctl.x_full, 4), tc::mbar_init(&ctl.x_empty, 1);
         tc::fence_barrier_init();
     }
@@ -207,8 +207,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             const int w = warp & 3;
             const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16);
             for (int n = 0; n < chunks; ++n) {
-                if (n >= 2 && !wait(&ctl.p_empty[n & 1], ((n >> 1) & 1) ^ 1)) break;
-                if (!wait(&ctl.scores_full, n & 1)) break;
+                if (!wait(&ctl.scores_full, n & 1) || (n > 0 && !wait(&ctl.p_empty, (n - 1) & 1))) break;
                 __syncwarp();
                 tc::tc_fence_after();
                 // (short code in loops: the roles' instructions together would not stay in the caches that feed the schedulers)
@@ -233,7 +232,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
 #pragma unroll
                         for (int k = 0; k < 16; ++k) v[k] = 0;
                     }
-                    tmem_st16(rows_at + kTmP + (n & 1) * 64 + cb * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
+                    tmem_st16(rows_at + kTmP + cb * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
                 }
                 tmem_st_wait();
                 tc::tc_fence_before();
@@ -252,22 +251,22 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             const int64_t row_bytes = (int64_t)args.heads * wc * (wide ? 4 : 2);
             char* const first_row = out + (((int64_t)b * steps * args.heads + h) * wc + col0) * (wide ? 4 : 2);
             for (int n = 0; n < chunks; ++n) {
-                if (!wait(&ctl.x_empty, n & 1) || !wait(&ctl.out_full, n & 1)) break;       // O1 and O2
+                if (!wait(&ctl.out_full[n & 1], (n >> 1) & 1)) break;
                 __syncwarp();
                 tc::tc_fence_after();
-                const float w1 = weight * ctl.up[n & 1];
+                const float w1 = weight * ctl.up[n & 3];
                 const bool in = i < (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps);
                 const int64_t t = reverse ? length - kSteps - begin - (int64_t)n * kSteps + r : begin + (int64_t)n * kSteps + r;
                 char* to = first_row + t * row_bytes;
 #pragma unroll 1
                 for (int cb = 0; cb < 4; ++cb) {
                     uint32_t p[16], q[16];
-                    tc::tmem_ld16(rows_at + kTmO1 + cb * 16, p);
-                    tc::tmem_ld16(rows_at + kTmO2 + cb * 16, q);
+                    tc::tmem_ld16(rows_at + kTmO1 + (n & 1) * kTmTurn + cb * 16, p);
+                    tc::tmem_ld16(rows_at + kTmO2 + (n & 1) * kTmTurn + cb * 16, q);
                     tc::tmem_ld_wait();
                     if (cb == 3) {
                         tc::tc_fence_before();
-                        tc::mbar_arrive_warp(&ctl.out_empty);
+                        tc::mbar_arrive_warp(&ctl.out_empty[n & 1]);
                     }
                     float o[16];
 #pragma unroll
@@ -403,9 +402,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 const int over = min(max((int)(__float_as_uint(most) >> 23) - 127 - 14, 0), 126);
                 down = __uint_as_float((uint32_t)(127 - over) << 23);
-                if (tid == 0) ctl.up[n & 1] = __uint_as_float((uint32_t)(127 + over) << 23);
+                if (tid == 0) ctl.up[n & 3] = __uint_as_float((uint32_t)(127 + over) << 23);
             } else {
-                if (tid == 0) ctl.up[n & 1] = 1.0f;
+                if (tid == 0) ctl.up[n & 3] = 1.0f;
             }
             if (mine) {
 #pragma unroll
@@ -462,11 +461,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     *reinterpret_cast<float4*>(to + (int64_t)i * wc + col0 + k) = make_float4(by * x[k], by * x[k + 1], by * x[k + 2], by * x[k + 3]);
         }
     } else if (warp == 1) {
-        // ---- scores and O1
+        // ---- scores
         if constexpr (!kEnds) {
             const uint32_t yes = elected();
             const uint64_t a_desc = tc::make_desc(base, 16, 1024), b_desc = tc::make_desc(base + R::kA, 16, 1024);
-            const uint64_t x_desc = tc::make_desc(base + R::kState, R::kHalf, 1024);
             tc::Ring ring;
             for (int n = 0; n < chunks; ++n, ring.next(R::kStages)) {
                 const uint64_t stage = (uint64_t)(ring.i * R::kStage >> 4);
@@ -479,35 +477,35 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     umma(yes, tmem + kTmScores, a_desc + off, b_desc + off, idesc<T>(128, 128, 0, 0), k > 0);
                 }
                 commit(yes, &ctl.scores_full);
-                if (!wait(&ctl.x_full, n & 1) || (n > 0 && !wait(&ctl.out_empty, (n - 1) & 1))) break;
-                __syncwarp();
-                tc::tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < KA / 16; ++k)
-                    umma(yes, tmem + kTmO1, a_desc + stage + ((k >> 2) * R::kHalf + (k & 3) * 32 >> 4), x_desc + (k * 2048 >> 4),
-                         idesc<T>(128, kDv, 0, 1), k > 0);
-                commit(yes, &ctl.x_empty);
                 commit(yes, &ctl.empty[ring.i]);
             }
         }
     } else if (warp == 2) {
-        // ---- O2
+        // ---- O1 and O2
         if constexpr (!kEnds) {
             const uint32_t yes = elected();
-            const uint64_t c_desc = tc::make_desc(base + 2 * R::kA, R::kHalf, 1024);
+            const uint64_t a_desc = tc::make_desc(base, 16, 1024), c_desc = tc::make_desc(base + 2 * R::kA, R::kHalf, 1024);
+            const uint64_t x_desc = tc::make_desc(base + R::kState, R::kHalf, 1024);
             tc::Ring ring;
             for (int n = 0; n < chunks; ++n, ring.next(R::kStages)) {
                 const uint64_t stage = (uint64_t)(ring.i * R::kStage >> 4);
-                if (!wait(&ctl.full_c[ring.i], ring.ph) || (n == ragged && !wait(&ctl.zeroed, 0)) || !wait(&ctl.p_full, n & 1) ||
-                    (n > 0 && !wait(&ctl.out_empty, (n - 1) & 1)))
-                    break;
+                const uint32_t turn = tmem + (n & 1) * kTmTurn;
+                if (!wait(&ctl.full[ring.i], ring.ph) || !wait(&ctl.x_full, n & 1) || (n >= 2 && !wait(&ctl.out_empty[n & 1], ((n >> 1) & 1) ^ 1))) break;
+                __syncwarp();
+                tc::tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < KA / 16; ++k)
+                    umma(yes, turn + kTmO1, a_desc + stage + ((k >> 2) * R::kHalf + (k & 3) * 32 >> 4), x_desc + (k * 2048 >> 4),
+                         idesc<T>(128, kDv, 0, 1), k > 0);
+                commit(yes, &ctl.x_empty);
+                if (!wait(&ctl.full_c[ring.i], ring.ph) || (n == ragged && !wait(&ctl.zeroed, 0)) || !wait(&ctl.p_full, n & 1)) break;
                 __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll
                 for (int k = 0; k < kSteps / 16; ++k)
-                    umma_ts(yes, tmem + kTmO2, tmem + kTmP + (n & 1) * 64 + k * 8, c_desc + stage + (k * 2048 >> 4), idesc<T>(128, kDv, 0, 1), k > 0);
-                commit(yes, &ctl.p_empty[n & 1]);
-                commit(yes, &ctl.out_full);
+                    umma_ts(yes, turn + kTmO2, tmem + kTmP + k * 8, c_desc + stage + (k * 2048 >> 4), idesc<T>(128, kDv, 0, 1), k > 0);
+                commit(yes, &ctl.p_empty);
+                commit(yes, &ctl.out_full[n & 1]);
                 commit(yes, &ctl.empty[ring.i]);
             }
         }
