@@ -32,7 +32,9 @@ struct Control {
         x_full, x_empty;
     uint32_t tmem;
     float up[4], most[4];
-    float none[32], power[kSteps + 1];           // g^n behind 32 zeros for what is not before a step
+    float power[kSteps + 1];                     // g^n
+    float diagonal[64];                          // [32 + row - column]: weights of 32 x 32 scores on the diagonal, 0 behind it
+    alignas(16) float across[32];                // [column]: those of a row in front of such a block, from its last column but one on
 };
 
 // Bounded wait.  It polls: a chunk's chain has a dozen of them one behind the other, and a parked thread wakes late (with
@@ -150,14 +152,18 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         tc::fence_barrier_init();
     }
     pdl_wait();
+    float log_decay;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(log_decay) : "l"(args.log_decay + h));
+    log_decay = log_decay > 0.0f ? 0.0f : log_decay;
     if (threadIdx.x <= kSteps) {
-        float g;
-        asm volatile("ld.global.f32 %0, [%1];" : "=f"(g) : "l"(args.log_decay + h));
-        g = g > 0.0f ? 0.0f : g;
         const int n = threadIdx.x;
-        const float w = n == 0 ? (g != g ? g : 1.0f) : (float)exp((double)n * (double)g);
+        const float w = n == 0 ? (log_decay != log_decay ? log_decay : 1.0f) : (float)exp((double)n * (double)log_decay);
         ctl.power[n] = w;
-        if (n < 32) ctl.none[n] = 0.0f;
+        if (n < 32) {
+            ctl.across[job.reverse ? n : 31 - n] = w;
+            ctl.diagonal[job.reverse ? 32 - n : 32 + n] = w;
+            if (n > 0) ctl.diagonal[job.reverse ? 32 + n : 32 - n] = 0.0f;
+        }
     }
     const int64_t steps = args.steps;
     int64_t length = steps;
@@ -172,8 +178,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     tc::tc_fence_after();
     const uint32_t tmem = ctl.tmem, power = tc::smem_u32(ctl.power);
     const int64_t parts_of = ((int64_t)which * args.batch * args.heads + unit) * args.n_parts;
-    // tiles that C' is the sum of
-    const int parts = job.end != nullptr ? R::kParts : 2;
+    // Tiles that C' is the sum of: all where the state is a result and the chunk so near its end that two would be seen in it (those
+    // before it count e^-1.5 and less), else two
+    const auto parts_of_chunk = [&](int n) {
+        const float after = (float)(length - begin - (int64_t)(n + 1) * kSteps);
+        return job.end != nullptr && after * -log_decay < 1.5f ? R::kParts : 2;
+    };
 
     // Behind a sequence's end, but inside the tensor, rows hold what they may: b's and c's of the last chunk are made zeros
     const int ragged = !reverse && length < steps && chunks > 0 && length < begin + (int64_t)chunks * kSteps ? chunks - 1 : -1;
@@ -205,7 +215,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         // ---- scores to weights
         if constexpr (!kEnds) {
             const int w = warp & 3;
-            const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16);
+            const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16), diagonal = tc::smem_u32(ctl.diagonal + 32 + lane);
+            const float near = table(power + 4 * (reverse ? 32 - lane : lane + 1));
             for (int n = 0; n < chunks; ++n) {
                 if (!wait(&ctl.scores_full, n & 1) || (n > 0 && !wait(&ctl.p_empty, (n - 1) & 1))) break;
                 __syncwarp();
@@ -214,20 +225,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
 #pragma unroll 1
                 for (int cb = 0; cb < 4; ++cb) {
                     const int back = reverse ? cb - w : w - cb;  // blocks of 32 steps back
+                    if (back < 0 && n > 0) continue;             // (zeros already)
                     uint32_t v[32];
                     if (back >= 0) {
                         tc::tmem_ld32(rows_at + kTmScores + cb * 32, v);
                         tc::tmem_ld_wait();
-                        const uint32_t f = power + 4 * (32 * back + (reverse ? -lane : lane));
-                        if (reverse) {
+                    }
+                    if (back > 0) {
+                        const Lanes f = all_lanes(near * table(power + 128 * (back - 1)));
 #pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                v[k] = word_of<T>(__uint_as_float(v[2 * k]) * table(f + 8 * k), __uint_as_float(v[2 * k + 1]) * table(f + 8 * k + 4));
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                v[k] = word_of<T>(__uint_as_float(v[2 * k]) * table(f - 8 * k), __uint_as_float(v[2 * k + 1]) * table(f - 8 * k - 4));
+                        for (int k = 0; k < 16; k += 2) {
+                            Raw<16> c;
+                            load_shared(c, ctl.across + 2 * k);
+                            const float c0[2] = {__uint_as_float(c.u[0]), __uint_as_float(c.u[1])}, c1[2] = {__uint_as_float(c.u[2]), __uint_as_float(c.u[3])};
+                            const float x0[2] = {__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])};
+                            const float x1[2] = {__uint_as_float(v[2 * k + 2]), __uint_as_float(v[2 * k + 3])};
+                            const Lanes y0 = lanes(x0) * (f * lanes(c0)), y1 = lanes(x1) * (f * lanes(c1));
+                            v[k] = word_of<T>(y0.at(0), y0.at(1)), v[k + 1] = word_of<T>(y1.at(0), y1.at(1));
                         }
+                    } else if (back == 0) {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            v[k] = word_of<T>(__uint_as_float(v[2 * k]) * table(diagonal - 8 * k), __uint_as_float(v[2 * k + 1]) * table(diagonal - 8 * k - 4));
                     } else {
 #pragma unroll
                         for (int k = 0; k < 16; ++k) v[k] = 0;
@@ -316,7 +335,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         tc::Ring ring;
         for (int n = 0; n < chunks && ok; ++n, ring.next(R::kStages)) {
             ok = wait(&ctl.full_c[ring.i], ring.ph);
-            const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps), top = rows - extra;
+            const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps), top = rows - extra, parts = parts_of_chunk(n);
             if (ok && n == ragged && wait(&ctl.full[ring.i], ring.ph)) {
                 const uint32_t tile = base + ring.i * R::kStage + R::kA;        // b's halves, and c's behind them
                 for (int k = tid; k < (KA / 64 + 1) * (kSteps - rows) * 8; k += 128)
@@ -372,9 +391,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         }
         if constexpr (!kEnds) {
             if (part > 0 && begin < length && i < wa) {
-                float g;
-                asm volatile("ld.global.f32 %0, [%1];" : "=f"(g) : "l"(args.log_decay + h));
-                const float whole = (float)exp((double)args.part_steps * (double)(g > 0.0f ? 0.0f : g));
+                const float whole = (float)exp((double)args.part_steps * (double)log_decay);
                 for (int s = 0; s < part; ++s) {
                     const float* const sums = args.parts + (parts_of + s) * wa * wc + (int64_t)i * wc + col0;
 #pragma unroll
@@ -524,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 __syncwarp();
                 tc::tc_fence_after();
 #pragma unroll 1
-                for (int q = 0; q < parts; ++q)
+                for (int q = 0, parts = parts_of_chunk(n); q < parts; ++q)
 #pragma unroll
                     for (int k = 0; k < kSteps / 32; ++k) {
                         const uint64_t rows = (uint64_t)(half * 4 + k) * (2048 >> 4);
