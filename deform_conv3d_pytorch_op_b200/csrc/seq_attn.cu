@@ -24,7 +24,6 @@ namespace seq {
 namespace {
 
 constexpr int kChunk = 64, kCols = 64, kThreads = 128, kMostWidth = 128, kMostParts = 32;
-constexpr float kLog2e = 1.4426950408889634f;
 
 struct Strides {
     int64_t batch, step, head;
@@ -61,13 +60,20 @@ struct AttnArgs {
     float scale;
 };
 
-__device__ __forceinline__ float log2_decay(const float* log_decay, int h) {
-    float g;
-    asm volatile("ld.global.f32 %0, [%1];" : "=f"(g) : "l"(log_decay + h));
-    g = g > 0.0f ? 0.0f : g;
-    return fmaxf(g * kLog2e, -1e4f) + (g != g ? g : 0.0f);     // (finite, so that 0 steps are a factor of 1)
+__device__ __forceinline__ double log_decay_of(const float* log_decay, int h) {
+    const float g = gload(log_decay + h);
+    return g > 0.0f ? 0.0 : (double)g;
 }
-__device__ __forceinline__ float power(float lg, int n) { return ex2(lg * (float)n); }
+// g^n, rounded once (1 for no steps, whatever the decay)
+__device__ __forceinline__ float power_of(double log_decay, int64_t n) {
+    return n == 0 && log_decay == log_decay ? 1.0f : (float)exp((double)n * log_decay);
+}
+// from a table of them in shared memory
+__device__ __forceinline__ float power(uint32_t table, int n) {
+    float f;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(table + 4 * n));
+    return f;
+}
 
 #include "seq_attn_tc.cuh"
 
@@ -208,14 +214,14 @@ __device__ __forceinline__ void load_bt(FragB<T> (&f)[2], uint32_t base, int k0,
 }
 // A[m][k] = tile[k0 + k][m0 + m] * weight of row k0 + k.  16-bit: rounded, and (low) what the rounding left
 template <typename T>
-__device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, uint32_t base, int k0, int m0, int cols, int lane, float lg,
+__device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, uint32_t base, int k0, int m0, int cols, int lane, uint32_t table,
                                         int last_power, int rows) {
     const int g = lane >> 2, t = lane & 3;
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             const int j = k0 + 2 * t + e;
-            const float w = j < rows ? power(lg, last_power - j) : 0.0f;
+            const float w = j < rows ? power(table, max(last_power - j, 0)) : 0.0f;
             split(w * lds_float(Tile<T>::at(base, j, m0 + g, cols)), f.v[2 * e], f.low[2 * e]);
             split(w * lds_float(Tile<T>::at(base, j, m0 + g + 8, cols)), f.v[2 * e + 1], f.low[2 * e + 1]);
         }
@@ -227,7 +233,7 @@ __device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, uint32_t bas
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int j = k0 + 2 * t + (e & 1) + (e >> 1) * 8;
-            w[e] = j < rows ? power(lg, last_power - j) : 0.0f;
+            w[e] = j < rows ? power(table, max(last_power - j, 0)) : 0.0f;
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {            // 0: (g, k 2t), 1: (g + 8, k 2t), 2: (g, k 2t + 8), 3: (g + 8, k 2t + 8)
@@ -296,7 +302,8 @@ struct Shape {
     static constexpr int kTileC = kChunk * Tile<T>::row_elems(kCols) * (int)sizeof(T);
     static constexpr int kState = KA * Tile<T>::row_elems(kCols) * (int)sizeof(T);
     static constexpr int kStage = 2 * kTileA + kTileC;
-    static constexpr int kBytes = kStages * kStage + kState + 32;
+    static constexpr int kTable = kStages * kStage + kState;             // g^n, 0 to 64
+    static constexpr int kBytes = kTable + (kChunk + 1) * 4 + 32;
 };
 
 // The maximum of a CTA's states, for the power of two that keeps a float16 copy of them in range
@@ -318,7 +325,9 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
     constexpr int kSteps = kChunk / L::kK;
     extern __shared__ __align__(128) char smem[];
     const uint32_t tiles = shared_address(smem), copy = tiles + S::kStages * S::kStage;
-    float* const slots = reinterpret_cast<float*>(smem + S::kStages * S::kStage + S::kState);
+    float* const powers = reinterpret_cast<float*>(smem + S::kTable);
+    float* const slots = powers + kChunk + 1;
+    const uint32_t table = shared_address(powers);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
     int u = blockIdx.x;
@@ -337,9 +346,11 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
     const int64_t begin = (int64_t)part * args.part_steps, stop = min(begin + args.part_steps, steps);
     const int64_t finish = min(stop, length);    // of the steps there are
     const bool reverse = job.reverse != 0;
-    const float lg = log2_decay(args.log_decay, h);
+    const double log_decay = log_decay_of(args.log_decay, h);
+    if (threadIdx.x <= kChunk) powers[threadIdx.x] = power_of(log_decay, threadIdx.x);
     const int extra = reverse ? 0 : 1;           // powers of g on the state before a chunk, at its first step
     const int wa = job.a.width, wc = job.c.width;
+    const int k_end = (wa + L::kK - 1) / L::kK * L::kK, n_end = min(kN, (wc - col0 + 15) / 16 * 2);        // of a's width, of c's columns
     const char* const from_a = static_cast<const char*>(job.a.p) + (b * job.a.s.batch + h / job.a.share * job.a.s.head) * (int64_t)sizeof(T);
     const char* const from_b = static_cast<const char*>(job.b.p) + (b * job.b.s.batch + h / job.b.share * job.b.s.head) * (int64_t)sizeof(T);
     const char* const from_c = static_cast<const char*>(job.c.p) + (b * job.c.s.batch + h / job.c.share * job.c.s.head) * (int64_t)sizeof(T);
@@ -363,13 +374,13 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
             for (int e = 0; e < 4; ++e) {
                 x[m][n][e] = 0.0f;
                 if constexpr (!kEnds) {
-                    const int i = (warp * kM + m) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                    const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
                     if (job.init != nullptr && i < wa && j < wc)
                         x[m][n][e] = job.init_scale * gload(job.init + (int64_t)unit * wa * wc + (int64_t)i * job.init_i + (int64_t)j * job.init_j);
                 }
             }
     if constexpr (!kEnds) {
-        const float whole = ex2(lg * (float)args.part_steps);
+        const float whole = power_of(log_decay, args.part_steps);
         for (int s = 0; s < part; ++s) {
             const float* const sums = args.parts + (parts_of + s) * wa * wc;
             // (a part that the sequence ends in is the last one that anything reads)
@@ -379,7 +390,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
                 for (int n = 0; n < kN; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int i = (warp * kM + m) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                        const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
                         if (i < wa && j < wc && begin < length) x[m][n][e] = fmaf(x[m][n][e], whole, gload(sums + (int64_t)i * wc + j));
                     }
         }
@@ -406,7 +417,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
             for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint32_t at = L::at(copy, (warp * kM + m) * 16 + g + half * 8, n * 8 + 2 * t, kCols);
+                    const uint32_t at = L::at(copy, (m * 4 + warp) * 16 + g + half * 8, n * 8 + 2 * t, kCols);
                     const float p = x[m][n][2 * half], q = x[m][n][2 * half + 1];
                     if constexpr (std::is_same<T, float>::value)
                         asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(p), "f"(q) : "memory");
@@ -430,23 +441,24 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
             if (m0 < rows) {
                 float o[kN][4] = {};
 #pragma unroll 2
-                for (int k = 0; k < KA; k += L::kK) {
+                for (int k = 0; k < k_end; k += L::kK) {
                     FragA<T> fa;
                     load_a<T>(fa, at, m0, k, KA, lane);
 #pragma unroll
                     for (int n = 0; n < kN; n += 2) {
+                        if (n >= n_end) continue;
                         FragB<T> fb[2];
                         load_bt<T>(fb, copy, k, n * 8, kCols, lane);
                         mma<T>(o[n], fa, fb[0]);
                         mma<T>(o[n + 1], fa, fb[1]);
                     }
                 }
-                const float w0 = power(lg, m0 + g + extra) * up, w1 = power(lg, m0 + g + 8 + extra) * up;
+                const float w0 = power(table, m0 + g + extra) * up, w1 = power(table, m0 + g + 8 + extra) * up;
 #pragma unroll
                 for (int n = 0; n < kN; ++n) o[n][0] *= w0, o[n][1] *= w0, o[n][2] *= w1, o[n][3] *= w1;
                 float s[kN][4] = {};
 #pragma unroll 2
-                for (int k = 0; k < KA; k += L::kK) {
+                for (int k = 0; k < k_end; k += L::kK) {
                     FragA<T> fa;
                     load_a<T>(fa, at, m0, k, KA, lane);
 #pragma unroll
@@ -463,15 +475,16 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int d = m0 + g + (e >> 1) * 8 - (n * 8 + 2 * t + (e & 1));
-                        s[n][e] = d >= 0 ? s[n][e] * power(lg, d) : 0.0f;
+                        s[n][e] = d >= 0 ? s[n][e] * power(table, max(d, 0)) : 0.0f;
                     }
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
-                    if (k * L::kK > m0 + 15) continue;
+                    if (k * L::kK > m0 + 15 || k * L::kK >= rows) continue;
                     FragA<T> fa;
                     scores_as_a<T>(fa, s, k);
 #pragma unroll
                     for (int n = 0; n < kN; n += 2) {
+                        if (n >= n_end) continue;
                         FragB<T> fb[2];
                         load_bt<T>(fb, ct, k * L::kK, n * 8, kCols, lane);
                         mma<T>(o[n], fa, fb[0]);
@@ -512,7 +525,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
             }
         }
         // the state behind this chunk
-        const float whole = power(lg, rows);
+        const float whole = power(table, rows);
         const int last_power = rows - extra;
 #pragma unroll
         for (int m = 0; m < kM; ++m)
@@ -521,16 +534,19 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x[m][n][e] *= whole;
 #pragma unroll 1
-        for (int k = 0; k < kChunk; k += L::kK) {
+        for (int k = 0; k < rows; k += L::kK) {
             FragB<T> fb[kN / 2][2];
 #pragma unroll
-            for (int n = 0; n < kN; n += 2) load_bt<T>(fb[n / 2], ct, k, n * 8, kCols, lane);
+            for (int n = 0; n < kN; n += 2)
+                if (n < n_end) load_bt<T>(fb[n / 2], ct, k, n * 8, kCols, lane);
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
+                if ((m * 4 + warp) * 16 >= wa) continue;
                 FragA<T> fa, low;
-                load_at<T>(fa, low, bt, k, (warp * kM + m) * 16, KA, lane, lg, last_power, rows);
+                load_at<T>(fa, low, bt, k, (m * 4 + warp) * 16, KA, lane, table, last_power, rows);
 #pragma unroll
                 for (int n = 0; n < kN; n += 2) {
+                    if (n >= n_end) continue;
                     mma<T>(x[m][n], fa, fb[n / 2][0]);
                     mma<T>(x[m][n + 1], fa, fb[n / 2][1]);
                     if constexpr (!std::is_same<T, float>::value) {
@@ -556,7 +572,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
             for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = (warp * kM + m) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                    const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
                     if (i < wa && j < wc) to[(int64_t)i * wc + j] = by * x[m][n][e];
                 }
     }
@@ -616,7 +632,7 @@ __global__ void __launch_bounds__(kThreads) attn_step_kernel(const StepArgs a) {
     const T* const q = static_cast<const T*>(a.q) + r * a.qs.batch + h * a.qs.head;
     const T* const k = static_cast<const T*>(a.k) + r * a.ks.batch + h / a.share * a.ks.head;
     const T* const v = static_cast<const T*>(a.v) + r * a.vs.batch + h / a.share * a.vs.head;
-    const float decay = ex2(log2_decay(a.log_decay, h));
+    const float decay = power_of(log_decay_of(a.log_decay, h), 1);
     for (int i = threadIdx.x; i < a.dk; i += kThreads) {
         Pack<T, 1> p;
         p.get(k + i), key[i] = p.at(0);
@@ -672,7 +688,8 @@ int check_attn(const dcn_attn* p) {
 int wide_of(const dcn_attn* p, bool backward) { return (int)(backward ? std::max(p->dk, p->dv) : p->dk) > 64 ? 128 : 64; }
 
 // How many parts the time axis is split into.  Time goes in chunks of a CTA; a GPU holds `held` of them at once.  More parts fill the
-// GPU, and cost a pass over b and c for their sums (half of a chunk's time) and the folding (half a chunk's for each part before).
+// GPU, and cost a pass over b and c for their sums (half of a chunk's time) and the folding (a quarter of a chunk's for each part
+// before), and each CTA what it costs to begin and to end.  (5x331x6x(40, 72) float32, 30 heads: three parts instead of one.)
 int parts_for(const dcn_attn* p, bool backward, bool tensor) {
     const int64_t ct = (backward ? std::max(p->dk, p->dv) : p->dv) > 64 ? 2 : 1, chunk = tensor ? tcgen::kSteps : kChunk;
     const int64_t units = p->batch * p->heads * ct * (backward ? 3 : 1), chunks = (p->steps + chunk - 1) / chunk;
@@ -681,10 +698,9 @@ int parts_for(const dcn_attn* p, bool backward, bool tensor) {
     double least = 1e300;
     for (int n = 1; n <= kMostParts && n <= chunks; ++n) {
         const int64_t each = (chunks + n - 1) / n;
-        if (n > 1 && each < 4) break;
         if ((chunks + each - 1) / each != n) continue;
         const double waves = (double)((units * n + held - 1) / held), sums = n > 1 ? (double)((units * (n - 1) + held - 1) / held) : 0;
-        const double time = waves * (each + 2 + 0.25 * (n - 1)) + sums * (0.5 * each + 2) + (n > 1 ? 2 : 0);
+        const double fixed = tensor ? 2 : 0.7, time = waves * (each + fixed + 0.25 * (n - 1)) + sums * (0.5 * each + fixed) + (n > 1 ? 0.5 * fixed : 0);
         if (time < least * 0.97) least = time, best = n;
     }
     return best;
