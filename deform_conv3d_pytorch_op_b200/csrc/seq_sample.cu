@@ -268,18 +268,33 @@ __device__ __forceinline__ unsigned long long scan64(Shared& s, unsigned long lo
     return before;
 }
 
-// This CTA's logits of at least `least` in bins up to `last` into its list (as many as it holds; all are counted)
-template <typename T>
-__device__ __forceinline__ void collect(const Row<T>& row, Shared& s, int last, float least) {
+// This CTA's logits of at least `least` in bins first to last into its list (as many as it holds; all are counted).  kBefore: and how many
+// lie in front of these bins, and their mass, for each thread's
+template <bool kBefore, typename T>
+__device__ __forceinline__ void collect(const Row<T>& row, Shared& s, int first, int last, float least, unsigned long long& count, unsigned long long& mass) {
     if (threadIdx.x == 0) s.listed = 0;
     __syncthreads();
-    const float to = last == kBins - 1 ? kBins + 32.0f : (float)(last + 1);
+    const float from = (float)first, to = last == kBins - 1 ? kBins + 32.0f : (float)(last + 1);
+    Halves before;
+    uint32_t n = 0;
     row.each([&](float v, int index) {
-        if (!(-row.argument(v) * kBinsPerArgument < to) || v < least) return;
+        const float x = row.argument(v), t = -x * kBinsPerArgument;
+        if (!(t < to) || v < least) return;
+        if (kBefore && t < from) {
+            before.add(expf(x));
+            ++n;
+            return;
+        }
         const uint32_t at = atomicAdd(&s.listed, 1u);
         if (at < kList) s.list[at] = candidate(v, index);
     });
     __syncthreads();
+    count = n, mass = before.sum();
+}
+template <typename T>
+__device__ __forceinline__ void collect(const Row<T>& row, Shared& s, int last, float least) {
+    unsigned long long count, mass;
+    collect<false>(row, s, 0, last, least, count, mass);
 }
 // The CTAs' lists in the first one's; how many there are in all
 __device__ __forceinline__ uint32_t join_lists(Shared& s, Team& team) {
@@ -485,8 +500,9 @@ __device__ Cut cut_at(const Row<T>& row, Shared& s, cg::cluster_group& cluster, 
 // A CTA's candidates, each thread with its own
 struct Listed {
     static constexpr int kEach = kList / kThreads;
-    unsigned long long weight[kEach];            // 0 for what is not kept
+    unsigned long long weight[kEach];
     int bin[kEach];
+    unsigned long long front_count = 0, front_mass = 0;          // what the thread has seen of bins before all of these
     template <typename T>
     __device__ __forceinline__ void get(const Row<T>& row, const Shared& s) {
 #pragma unroll
@@ -501,7 +517,7 @@ struct Listed {
     }
     // over the cluster: how many lie in front of a bin, and their mass
     __device__ __forceinline__ void before(Shared& s, Team& team, int b, unsigned long long& count, unsigned long long& mass) const {
-        count = mass = 0;
+        count = front_count, mass = front_mass;
 #pragma unroll
         for (int j = 0; j < kEach; ++j)
             if (bin[j] < b) ++count, mass += weight[j];
@@ -741,14 +757,26 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
             }
             return;
         }
-        // More: the lists stay with their CTAs, each with what its warps have of the row
-        unsigned long long kept = 0, longest = threadIdx.x == 0 && s.listed > kList ? 1 : 0;
-        team.exchange(s, longest, none);
-        listed = longest == 0;
+        // More: the lists stay with their CTAs, each with what its warps have of the row.  Where they are too long, they are made anew, of
+        // the bins alone that the limit can lie in, and the token is looked for in the row itself.
+        const auto fits = [&] {
+            unsigned long long longest = threadIdx.x == 0 && s.listed > kList ? 1 : 0;
+            team.exchange(s, longest, none);
+            return longest == 0;
+        };
+        unsigned long long kept = 0;
+        bool narrow = false, usable = fits();
+        if (!usable) {
+            narrow = true;
+            row.only_up_to(last, temperature);
+            collect<true>(row, s, first, last, -CUDART_INF_F, mine.front_count, mine.front_mass);
+            row.floor = -CUDART_INF_F;
+            usable = fits();
+        }
         mine.get(row, s);
         if (by_count) {
-            listed = listed && cut_in(row, s, team, mine, first, last, of_count, cut, kept);
-            if (!listed) {
+            usable = usable && cut_in(row, s, team, mine, first, last, of_count, cut, kept);
+            if (!usable) {
                 histogram(row, s, cluster);
                 cut = cut_at(row, s, cluster, of_count, kept);
             }
@@ -757,14 +785,15 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
         if (by_mass) {
             const auto below = of_share(fmax((double)top_p * (double)total, 1e-300));
             Cut other;
-            // (behind a count's cut the share has been reached)
-            listed = listed && cut_in(row, s, team, mine, by_count ? 0 : first, last, below, other, kept);
-            if (!listed) {
+            // (the share of a count lies in front of its limit: a list of that one's bin alone does not have it)
+            usable = usable && !(by_count && narrow) && cut_in(row, s, team, mine, by_count ? 0 : first, last, below, other, kept);
+            if (!usable) {
                 histogram(row, s, cluster);
                 other = cut_at(row, s, cluster, below, kept);
             }
             cut = other;
         }
+        listed = usable && !narrow;
         // nothing below the cut is looked at again
         if (cut.bin == kBins) row.floor = logit_of((unsigned long long)cut.key << 20);
         else row.only_up_to(cut.bin, temperature);
@@ -793,7 +822,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < Listed::kEach; ++j) {
             const int i = threadIdx.x + j * kThreads;
-            index[j] = 0x7fffffff;
+            index[j] = 0x7fffffff;       // (not kept)
             if (i < s.listed) {
                 const unsigned long long c = s.list[i];
                 if (c >= least && expf(row.argument(logit_of(c))) >= min_p) index[j] = index_of(c), of_warp += mine.weight[j];
@@ -804,23 +833,47 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
         const unsigned long long target = min((unsigned long long)floor(u * (double)total), total - 1), before = team.before_a;
         own = s.shared_a[team.turn ^ 1][rank];
         if (target < before || target >= before + own) return;
-        // the first index up to which there is more
-        int lo = 0, hi = a.vocab - 1;
-        while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            unsigned long long sum = 0;
-#pragma unroll
-            for (int j = 0; j < Listed::kEach; ++j) sum += index[j] <= mid ? mine.weight[j] : 0;
-            cta_sums(s, sum, none);
-            if (sum > target - before) hi = mid;
-            else lo = mid + 1;
-        }
+        // The token among this CTA's: by buckets of indices, then inside of one
+        const int base = max(rank * kWarps * each * Row<T>::kV - row.skew, 0), span = kWarps * each * Row<T>::kV;
+        int shift = 0;
+        while (span >> shift >= kBins) ++shift;
+        clear(s);
 #pragma unroll
         for (int j = 0; j < Listed::kEach; ++j)
-            if (index[j] == lo) {
-                a.tokens[r] = lo;
-                a.logprobs[r] = (float)(log((double)mine.weight[j]) - log((double)total));
+            if (index[j] != 0x7fffffff && mine.weight[j] != 0) atomicAdd(&s.mass[(index[j] - base) >> shift], mine.weight[j]);
+        if (threadIdx.x == 0) s.narrowed = 0;
+        __syncthreads();
+        constexpr int kPer = kBins / kThreads;
+        unsigned long long sum = 0, all;
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) sum += s.mass[threadIdx.x * kPer + k];
+        unsigned long long up = before + scan64(s, sum, all);
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) {
+            const unsigned long long m = s.mass[threadIdx.x * kPer + k];
+            if (target >= up && target < up + m) s.found = threadIdx.x * kPer + k, s.found_mass = up;
+            up += m;
+        }
+        __syncthreads();
+        const int bucket = s.found;
+        up = s.found_mass;
+#pragma unroll
+        for (int j = 0; j < Listed::kEach; ++j)
+            if (index[j] != 0x7fffffff && mine.weight[j] != 0 && (index[j] - base) >> shift == bucket) {
+                const uint32_t at = atomicAdd(&s.narrowed, 1u);          // (a bucket has at most 2^20 / 2048 indices)
+                s.narrow[at] = (unsigned long long)(index[j] - base) << 41 | mine.weight[j];
             }
+        __syncthreads();
+        constexpr unsigned long long kWeight = (1ull << 41) - 1;
+        const int n = s.narrowed;
+        if (threadIdx.x < n) {
+            const unsigned long long c = s.narrow[threadIdx.x], w = c & kWeight;
+            for (int k = 0; k < n; ++k) up += s.narrow[k] < c ? s.narrow[k] & kWeight : 0;
+            if (target >= up && target < up + w) {
+                a.tokens[r] = base + (int)(c >> 41);
+                a.logprobs[r] = (float)(log((double)w) - log((double)total));
+            }
+        }
         return;
     }
     row.each([&](float v, int index) { of_warp += weight(v, index); });
