@@ -15,10 +15,12 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+import math
 import os
 
 from .functions import DeformLayerFunction
 from .modules import ConvOffset3d
+from .sequence import GroupNormAct
 
 
 class DeformUnit(nn.Module):
@@ -58,19 +60,29 @@ def _conv3(cin, cout, stride, deformable, precision, deform):
     return nn.Conv3d(cin, cout, 3, stride=stride, padding=1, bias=False)
 
 
+def _group_norm(channels, activation=None):
+    return GroupNormAct(math.gcd(32, channels), channels, activation)
+
+
 class BasicBlock(nn.Module):
-    def __init__(self, cin, cout, stride, deformable, precision, deform):
+    """``norm``: "batch", or "group" (the norms bring activation and shortcut with them)"""
+
+    def __init__(self, cin, cout, stride, deformable, precision, deform, norm="batch"):
         super().__init__()
+        self.norm = norm
         self.conv1 = _conv3(cin, cout, stride, deformable, precision, deform)
-        self.bn1 = nn.BatchNorm3d(cout)
+        self.bn1 = nn.BatchNorm3d(cout) if norm == "batch" else _group_norm(cout, "relu")
         self.conv2 = _conv3(cout, cout, 1, deformable, precision, deform)
-        self.bn2 = nn.BatchNorm3d(cout)
+        self.bn2 = nn.BatchNorm3d(cout) if norm == "batch" else _group_norm(cout, "relu")
         self.down = None
         if stride != 1 or cin != cout:
-            self.down = nn.Sequential(nn.Conv3d(cin, cout, 1, stride=stride, bias=False), nn.BatchNorm3d(cout))
+            self.down = nn.Sequential(nn.Conv3d(cin, cout, 1, stride=stride, bias=False),
+                                      nn.BatchNorm3d(cout) if norm == "batch" else _group_norm(cout))
 
     def forward(self, x):
         idt = x if self.down is None else self.down(x)
+        if self.norm == "group":
+            return self.bn2(self.conv2(self.bn1(self.conv1(x))), idt)
         y = F.relu(self.bn1(self.conv1(x)), inplace=True)
         y = self.bn2(self.conv2(y))
         return F.relu(y + idt, inplace=True)
@@ -78,19 +90,22 @@ class BasicBlock(nn.Module):
 
 class R3D18Deform(nn.Module):
     """Stem 3->64 (3,7,7)/(1,2,2) + BN + ReLU + maxpool 3/2; stages 64/128/256/512 x 2 blocks, strides 1/2/2/2;
-    stages 3-4 deformable; global average pool; linear 512 -> num_classes."""
+    stages 3-4 deformable; global average pool; linear 512 -> num_classes.  ``norm="group"``: group norms of up to 32 groups in the
+    place of batch norms, for training on few clips a GPU (channels_last_3d storage of clips and weights spares their copies)."""
 
-    def __init__(self, num_classes=400, width=64, precision="auto", deform=True):
+    def __init__(self, num_classes=400, width=64, precision="auto", deform=True, norm="batch"):
         super().__init__()
+        if norm not in ("batch", "group"):
+            raise ValueError("norm is %r: 'batch' or 'group'" % (norm,))
         w = width
         self.stem = nn.Sequential(nn.Conv3d(3, w, (3, 7, 7), stride=(1, 2, 2), padding=(1, 3, 3), bias=False),
-                                  nn.BatchNorm3d(w), nn.ReLU(inplace=True),
+                                  *([nn.BatchNorm3d(w), nn.ReLU(inplace=True)] if norm == "batch" else [_group_norm(w, "relu")]),
                                   nn.MaxPool3d(3, stride=2, padding=1))
         cfg = [(w, w, 1, False), (w, 2 * w, 2, False), (2 * w, 4 * w, 2, True), (4 * w, 8 * w, 2, True)]
         stages = []
         for cin, cout, stride, deformable in cfg:
-            stages.append(nn.Sequential(BasicBlock(cin, cout, stride, deformable, precision, deform),
-                                        BasicBlock(cout, cout, 1, deformable, precision, deform)))
+            stages.append(nn.Sequential(BasicBlock(cin, cout, stride, deformable, precision, deform, norm),
+                                        BasicBlock(cout, cout, 1, deformable, precision, deform, norm)))
         self.stages = nn.Sequential(*stages)
         self.fc = nn.Linear(8 * w, num_classes)
 

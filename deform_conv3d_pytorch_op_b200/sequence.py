@@ -270,8 +270,69 @@ class GatedScan(nn.Module):
         x, gate = self.proj(input).chunk(2, -1)
         return GatedScanFunction.step(x, gate, state, slots)
 
+    def new_states(self, rows):
+        """Zeros for a pool of ``rows`` sequences' states."""
+        return torch.zeros(rows, self.channels, device=self.proj.weight.device)
+
     def extra_repr(self):
         return "{features}, {channels}".format(**self.__dict__)
+
+
+class GroupNormAct(nn.Module):
+    """Weights of a group norm, and the activation behind it: ``forward(x, residual)``.  The channels are axis ``dim`` of x: 1 as in
+    ``nn.GroupNorm`` (stored channels last, x is read as it is), or -1, where all axes but the first and the last are positions."""
+
+    def __init__(self, groups, channels, activation=None, dim=1, eps=1e-5, device=None, dtype=None):
+        super().__init__()
+        if groups < 1 or channels % groups:
+            raise _lib.DcnError("%d groups do not divide the %d channels" % (groups, channels))
+        self.groups, self.channels, self.activation, self.dim, self.eps = groups, channels, activation, dim, eps
+        self.weight = nn.Parameter(torch.ones(channels, device=device, dtype=dtype))
+        self.bias = nn.Parameter(torch.zeros(channels, device=device, dtype=dtype))
+
+    def forward(self, x, residual=None):
+        if self.dim not in (-1, x.dim() - 1):
+            x = x.movedim(self.dim, -1)
+            residual = residual if residual is None else residual.movedim(self.dim, -1)
+            return GroupNormActFunction.apply(x, self.groups, self.weight, self.bias, residual, self.activation, self.eps).movedim(-1, self.dim)
+        return GroupNormActFunction.apply(x, self.groups, self.weight, self.bias, residual, self.activation, self.eps)
+
+    def extra_repr(self):
+        return "{groups}, {channels}, activation={activation}, dim={dim}, eps={eps}".format(**self.__dict__)
+
+
+class DecayAttention(nn.Module):
+    """Projection of features to queries, keys and values, decayed attention over time, and a group norm with SiLU over each head's
+    outputs: [batch, steps, features] -> [batch, steps, heads * dv].  The first head's states last about ``memory`` steps, the last
+    one's sixteen times as long."""
+
+    def __init__(self, features, heads, dk, dv=None, kv_heads=None, memory=8.0, device=None, dtype=None):
+        super().__init__()
+        dv, kv_heads = dk if dv is None else dv, heads if kv_heads is None else kv_heads
+        self.features, self.heads, self.kv_heads, self.dk, self.dv = features, heads, kv_heads, dk, dv
+        self.proj = nn.Linear(features, heads * dk + kv_heads * (dk + dv), device=device, dtype=dtype)
+        self.norm = GroupNormAct(heads, heads * dv, "silu", dim=-1, device=device, dtype=dtype)
+        last = memory * 16.0 ** (torch.arange(heads, dtype=torch.float64) / max(heads - 1, 1))
+        self.register_buffer("log_decay", torch.log1p(-1.0 / last.clamp(min=1.001)).float().to(device))
+
+    def _parts(self, input):
+        h, kv, dk, dv = self.heads, self.kv_heads, self.dk, self.dv
+        q, k, v = self.proj(input).split((h * dk, kv * dk, kv * dv), -1)
+        return q.unflatten(-1, (h, dk)), k.unflatten(-1, (kv, dk)), v.unflatten(-1, (kv, dv)), self.log_decay
+
+    def forward(self, input, state=None, lengths=None):
+        out, last = DecayAttentionFunction.apply(*self._parts(input), state, lengths)
+        return self.norm(out.flatten(0, 1).flatten(1)).unflatten(0, out.shape[:2]), last
+
+    def step(self, input, state, slots=None):
+        return self.norm(DecayAttentionFunction.step(*self._parts(input), state, slots).flatten(1))
+
+    def new_states(self, rows):
+        """Zeros for a pool of ``rows`` sequences' states."""
+        return torch.zeros(rows, self.heads, self.dk, self.dv, device=self.proj.weight.device)
+
+    def extra_repr(self):
+        return "{features}, heads={heads}, kv_heads={kv_heads}, dk={dk}, dv={dv}".format(**self.__dict__)
 
 
 class ResidualNorm(nn.Module):
