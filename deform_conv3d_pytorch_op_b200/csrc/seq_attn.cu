@@ -141,9 +141,13 @@ __device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], cons
 template <typename T>
 __device__ __forceinline__ void mma(float (&d)[4], const FragA<T>& a, const FragB<T>& b) {
     if constexpr (std::is_same<T, float>::value) {
-        mma8(d, a.low, b.v);
-        mma8(d, a.v, b.low);
-        mma8(d, a.v, b.v);
+        // (the tensor cores' own sums are cut off, not rounded: of eight products at a time, that is lost in them)
+        float t[4] = {};
+        mma8(t, a.low, b.v);
+        mma8(t, a.v, b.low);
+        mma8(t, a.v, b.v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) d[e] += t[e];
     } else {
         mma16<T>(d, a.v, b.v);
     }
@@ -212,9 +216,9 @@ __device__ __forceinline__ void load_bt(FragB<T> (&f)[2], uint32_t base, int k0,
         f[0].v[0] = r[0], f[0].v[1] = r[1], f[1].v[0] = r[2], f[1].v[1] = r[3];
     }
 }
-// A[m][k] = tile[k0 + k][m0 + m] * weight of row k0 + k.  16-bit: rounded, and (low) what the rounding left
+// A[m][k] = tile[k0 + k][m0 + m] * weight of row k0 + k.  16-bit: rounded, what the rounding left (low), and what that one's left (last)
 template <typename T>
-__device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, uint32_t base, int k0, int m0, int cols, int lane, uint32_t table,
+__device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, FragA<T>& last, uint32_t base, int k0, int m0, int cols, int lane, uint32_t table,
                                         int last_power, int rows) {
     const int g = lane >> 2, t = lane & 3;
     if constexpr (std::is_same<T, float>::value) {
@@ -239,7 +243,9 @@ __device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, uint32_t bas
         for (int i = 0; i < 4; ++i) {            // 0: (g, k 2t), 1: (g + 8, k 2t), 2: (g, k 2t + 8), 3: (g + 8, k 2t + 8)
             const float x = half_of<T>(r[i], 0) * w[(i >> 1) * 2], y = half_of<T>(r[i], 1) * w[(i >> 1) * 2 + 1];
             f.v[i] = word_of<T>(x, y);
-            low.v[i] = word_of<T>(x - half_of<T>(f.v[i], 0), y - half_of<T>(f.v[i], 1));
+            const float p = x - half_of<T>(f.v[i], 0), q = y - half_of<T>(f.v[i], 1);
+            low.v[i] = word_of<T>(p, q);
+            last.v[i] = word_of<T>(p - half_of<T>(low.v[i], 0), q - half_of<T>(low.v[i], 1));
         }
     }
 }
@@ -350,6 +356,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
     if (threadIdx.x <= kChunk) powers[threadIdx.x] = power_of(log_decay, threadIdx.x);
     const int extra = reverse ? 0 : 1;           // powers of g on the state before a chunk, at its first step
     const int wa = job.a.width, wc = job.c.width;
+    const bool exact = job.end != nullptr;       // the state is a result
     const int k_end = (wa + L::kK - 1) / L::kK * L::kK, n_end = min(kN, (wc - col0 + 15) / 16 * 2);        // of a's width, of c's columns
     const char* const from_a = static_cast<const char*>(job.a.p) + (b * job.a.s.batch + h / job.a.share * job.a.s.head) * (int64_t)sizeof(T);
     const char* const from_b = static_cast<const char*>(job.b.p) + (b * job.b.s.batch + h / job.b.share * job.b.s.head) * (int64_t)sizeof(T);
@@ -542,8 +549,8 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
                 if ((m * 4 + warp) * 16 >= wa) continue;
-                FragA<T> fa, low;
-                load_at<T>(fa, low, bt, k, (m * 4 + warp) * 16, KA, lane, table, last_power, rows);
+                FragA<T> fa, low, lowest;
+                load_at<T>(fa, low, lowest, bt, k, (m * 4 + warp) * 16, KA, lane, table, last_power, rows);
 #pragma unroll
                 for (int n = 0; n < kN; n += 2) {
                     if (n >= n_end) continue;
@@ -552,6 +559,10 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
                     if constexpr (!std::is_same<T, float>::value) {
                         mma<T>(x[m][n], low, fb[n / 2][0]);
                         mma<T>(x[m][n + 1], low, fb[n / 2][1]);
+                        if (std::is_same<T, __nv_bfloat16>::value && exact) {
+                            mma<T>(x[m][n], lowest, fb[n / 2][0]);
+                            mma<T>(x[m][n + 1], lowest, fb[n / 2][1]);
+                        }
                     }
                 }
             }

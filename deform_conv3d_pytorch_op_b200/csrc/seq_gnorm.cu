@@ -30,6 +30,7 @@ struct GnormArgs {
     void *dweight, *dbias;
     int64_t samples, positions, split_positions;
     int channels, groups, per_group, vectors, act, wide_weights, splits;
+    int tiny;                                    // a group has one or two elements
     float eps, inv;                              // 1 / elements of a group
 };
 
@@ -270,6 +271,15 @@ __device__ __forceinline__ float typical(const GnormArgs& a, const T* x, int64_t
     p.get(x), q.get(x + positions / 2 * a.channels), r.get(x + (positions - 1) * a.channels);
     return fmaxf(fminf(p.at(0), q.at(0)), fminf(fmaxf(p.at(0), q.at(0)), r.at(0)));
 }
+// The one or two elements of a tiny group
+template <typename T>
+__device__ __forceinline__ float2 two_of(const GnormArgs& a, const void* from, int64_t base, int g) {
+    const T* const x = static_cast<const T*>(from) + base + g * a.per_group;
+    Pack<T, 1> p, q;
+    p.get(x), q.zero();
+    if (a.inv < 1.0f) q.get(x + (a.per_group == 2 ? 1 : a.channels));
+    return make_float2(p.at(0), q.at(0));
+}
 // A group's mean and 1 / sqrt(var + eps) from such sums
 __device__ __forceinline__ float2 finish(const GnormArgs& a, float about, float2 s) {
     const float d = s.x * a.inv;
@@ -405,7 +415,12 @@ __global__ void __launch_bounds__(512) gnorm_held_kernel(const GnormArgs a) {
         join_channels(a, grid.rows, entries, nullptr, false, stats, [](int) { return 1.0f; });
         __syncthreads();
         for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
-            const float2 f = finish(a, about[g], make_float2(stats[2 * g], stats[2 * g + 1]));
+            float2 f = finish(a, about[g], make_float2(stats[2 * g], stats[2 * g + 1]));
+            if (a.tiny) {
+                const float2 v = two_of<T>(a, a.x, base, g);
+                const float mean = __fmul_rn(__fadd_rn(v.x, v.y), a.inv), p = __fsub_rn(v.x, mean), q = a.inv < 1.0f ? __fsub_rn(v.y, mean) : 0.0f;
+                f = make_float2(mean, rsqrtf(__fadd_rn(__fmul_rn(__fadd_rn(__fmul_rn(p, p), __fmul_rn(q, q)), a.inv), a.eps)));
+            }
             stats[2 * g] = f.x, stats[2 * g + 1] = f.y;
         }
         __syncthreads();
@@ -627,10 +642,12 @@ struct Sums {
     }
 };
 
-template <typename T, int V>
+// kTiny: where groups may have one or two elements
+template <typename T, int V, bool kTiny>
 struct Gradient {
     Channels<T, V> ch;
     Pairs<V> s1, s2;                             // negative
+    float rr[kTiny ? V : 1], w[kTiny ? V : 1];   // (of tiny ones, whose s1 and s2 are the means themselves)
     __device__ __forceinline__ void get(const GnormArgs& a, int c0, const float* stats, const float* sums) {
         ch.get(a, c0, stats);
         GroupOf group(a, c0);
@@ -640,7 +657,12 @@ struct Gradient {
             const int g = group.next();
             const float r = stats[2 * g + 1];
             p[e] = -r * (sums[2 * g] * a.inv), q[e] = -r * r * (sums[2 * g + 1] * a.inv);
+            if constexpr (kTiny)
+                if (a.tiny) p[e] = sums[2 * g], q[e] = sums[2 * g + 1], rr[e] = r;
         }
+        if constexpr (kTiny)
+            if (a.tiny) weights_at<T, V>(a.weight, c0, a.wide_weights, 1.0f, w);
+
         s1.map([&](float, int e) { return p[e]; });
         s2.map([&](float, int e) { return q[e]; });
     }
@@ -649,10 +671,38 @@ struct Gradient {
         const Pairs<V> dz = v.gradient(a, ch, d);
 #pragma unroll
         for (int i = 0; i < Pairs<V>::kN; ++i) dx.v[i] = fma(dz.v[i], ch.rw.v[i], fma(d.v[i], s2.v[i], s1.v[i]));
+        // Of two elements, the three terms cancel down to eps / (var + eps) of them, of one to nothing: every factor as it stands in the sums
+        if constexpr (kTiny)
+            if (a.tiny) dx.map([&](float, int e) {
+                const float dh = __fmul_rn(dz.at(e), w[e]), h = __fmul_rn(d.at(e), rr[e]);
+                return __fmul_rn(rr[e], __fsub_rn(__fsub_rn(dh, s1.at(e)), __fmul_rn(h, s2.at(e))));
+            });
         if (a.dx != nullptr) dx.template pack<T>().put(static_cast<T*>(a.dx) + at);
         if (a.dresidual != nullptr) dz.template pack<T>().put(static_cast<T*>(a.dresidual) + at);
     }
 };
+
+// mean(dz w) and mean(dz w h) of a tiny group
+template <typename T>
+__device__ __forceinline__ void tiny_sums(const GnormArgs& a, int64_t base, int g, const float* stats, float* sums) {
+    const float2 x = two_of<T>(a, a.x, base, g), dy = two_of<T>(a, a.dy, base, g);
+    const float2 res = a.residual != nullptr ? two_of<T>(a, a.residual, base, g) : make_float2(0.0f, 0.0f);
+    float dh[2] = {}, h[2] = {};
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        if (e == 1 && a.inv == 1.0f) break;
+        const int c = g * a.per_group + (a.per_group == 2 ? e : 0);
+        const float w = weight_at<T>(a.weight, c, a.wide_weights, 1.0f), d = (e == 0 ? x.x : x.y) - stats[2 * g];
+        Pairs<1> z, y;
+        const float zy[4] = {fmaf(d, stats[2 * g + 1] * w, weight_at<T>(a.bias, c, a.wide_weights, 0.0f)) + (e == 0 ? res.x : res.y), 0.0f,
+                             e == 0 ? dy.x : dy.y, 0.0f};
+        const float zs[2] = {zy[0], zy[1]}, ys[2] = {zy[2], zy[3]};
+        z.v[0] = lanes(zs), y.v[0] = lanes(ys);
+        dh[e] = __fmul_rn(activate_gradient(z, y, a.act).at(0), w), h[e] = __fmul_rn(d, stats[2 * g + 1]);
+    }
+    sums[2 * g] = __fmul_rn(__fadd_rn(dh[0], dh[1]), a.inv);
+    sums[2 * g + 1] = __fmul_rn(__fadd_rn(__fmul_rn(dh[0], h[0]), __fmul_rn(dh[1], h[1])), a.inv);
+}
 
 template <typename T, int V>
 __global__ void __launch_bounds__(512) gnorm_held_backward_kernel(const GnormArgs a) {
@@ -690,12 +740,16 @@ __global__ void __launch_bounds__(512) gnorm_held_backward_kernel(const GnormArg
         }
         join_channels(a, grid.rows, entries, total, true, sums, [&](int c) { return weight_at<T>(a.weight, c, a.wide_weights, 1.0f); });
         __syncthreads();
+        if (a.tiny) {
+            for (int g = threadIdx.x; g < a.groups; g += blockDim.x) tiny_sums<T>(a, base, g, stats, sums);
+            __syncthreads();
+        }
         k = 0;
         if (a.dx != nullptr || a.dresidual != nullptr)
             for (int b = 0; b < grid.blocks; ++b) {
                 const int col = grid.col + b * blockDim.x;
                 if (grid.row < 0 || col >= a.vectors) continue;
-                Gradient<T, V> gr;
+                Gradient<T, V, true> gr;
                 gr.get(a, col * V, stats, sums);
                 for (int64_t p = grid.row; p < a.positions; p += grid.rows, ++k) {
                     Loads<T, V> v;
@@ -809,7 +863,7 @@ __global__ void __launch_bounds__(kThreads, 2) gnorm_apply_backward_kernel(const
             stream_begin(col < a.vectors ? n : 0, issue);
         }
         if (grid.row < 0 || col >= a.vectors) continue;
-        Gradient<T, V> gr;
+        Gradient<T, V, false> gr;
         gr.get(a, col * V, stats, sums);
         int64_t to = at + col * V;
         stream(n, issue, [&](int slot, auto&& ahead) {
@@ -913,6 +967,7 @@ GnormArgs gnorm_args(const dcn_gnorm* p, const Plan& r) {
     a.act = p->act, a.wide_weights = p->weight_dtype == DCN_SEQ_F32;
     a.eps = p->eps;
     a.inv = (float)(1.0 / ((double)p->positions * a.per_group));
+    a.tiny = p->positions * a.per_group <= 2;
     return a;
 }
 

@@ -147,3 +147,30 @@ def test_refusals():
     got = torch.autograd.grad(y, leaf, torch.ones_like(y).requires_grad_(), create_graph=True)[0]
     with pytest.raises(RuntimeError, match="once_differentiable"):
         got.sum().backward()
+
+
+@pytest.mark.parametrize("shape,groups", [((40, 24), 24), ((40, 24), 12), ((9, 2, 10), 10), ((5, 1, 6, 4), 4)])
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_groups_of_one_and_two_elements(t, shape, groups):
+    """One element has no gradient; of two, what is left is eps / (var + eps) of terms that cancel: as exact as the same steps in float32"""
+    import deform_conv3d_pytorch_op_b200 as dcn
+    g = torch.Generator(device="cuda").manual_seed(9)
+    c = shape[-1]
+    x, dy = (torch.randn(*shape, generator=g, device="cuda").to(t) for _ in range(2))
+    w, b = (torch.randn(c, generator=g, device="cuda") for _ in range(2))
+    if len(shape) == 4:                              # [5, 1, 6, 4] as one position of 24 channels
+        x, dy, w, b, groups, c = x.reshape(5, 24), dy.reshape(5, 24), torch.ones(24, device="cuda"), torch.zeros(24, device="cuda"), 24, 24
+    leaf = x.clone().requires_grad_()
+    y = dcn.GroupNormActFunction.apply(leaf, groups, w, b)
+    dx = torch.autograd.grad(y, leaf, dy)[0]
+    split = (x.numel() // c // x.size(0), groups, c // groups)
+    v = x.float().reshape(x.size(0), *split)
+    d = v - v.mean((1, 3), keepdim=True)
+    r = torch.rsqrt(d.square().mean((1, 3), keepdim=True) + 1e-5)
+    h = d * r
+    dh = (dy.float() * w).reshape(v.shape)
+    want = (r * (dh - dh.mean((1, 3), keepdim=True) - h * (dh * h).mean((1, 3), keepdim=True))).reshape(x.shape)
+    if split[0] * split[2] == 1:
+        assert float(dx.abs().max()) == 0 and torch.equal(y.float(), b.to(t).float().expand_as(y))
+    else:
+        ref.close(dx, want.double(), "dx")
