@@ -55,9 +55,29 @@ struct AttnArgs {
     const int64_t* lengths;
     float* parts;                                // [job][batch * heads][part][a.width][c.width]
     int64_t steps, part_steps;
+    int64_t whole;                               // units (job, head, tile) whose time axis is not split
     int batch, heads, jobs, tiles, n_parts;      // tiles: of 64 columns, the most that a job has
     int tile_of[3];
     float scale;
+};
+
+// Which unit and which part of its time axis a CTA has.  kEnds: of those parts alone that another one follows
+struct Place {
+    int tile, which, unit, part;
+    int64_t part_steps;
+    template <bool kEnds>
+    static __device__ __forceinline__ Place of(const AttnArgs& a) {
+        Place p;
+        const int64_t split = (int64_t)blockIdx.x - (kEnds ? 0 : a.whole);
+        const int parts = kEnds ? a.n_parts - 1 : a.n_parts;
+        int64_t u = blockIdx.x;
+        p.part = 0, p.part_steps = a.steps;
+        if (split >= 0) u = a.whole + split / parts, p.part = (int)(split % parts), p.part_steps = a.part_steps;
+        p.tile = (int)(u % a.tiles);
+        u /= a.tiles;
+        p.which = (int)(u % a.jobs), p.unit = (int)(u / a.jobs);
+        return p;
+    }
 };
 
 __device__ __forceinline__ double log_decay_of(const float* log_decay, int h) {
@@ -336,20 +356,17 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
     const uint32_t table = shared_address(powers);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
-    int u = blockIdx.x;
-    const int tile = u % args.tiles;
-    u /= args.tiles;
-    const int which = u % args.jobs;
-    const int unit = u / args.jobs, h = unit % args.heads, b = unit / args.heads;
+    const Place place = Place::of<kEnds>(args);
+    const int tile = place.tile, which = place.which, unit = place.unit, h = unit % args.heads, b = unit / args.heads;
     const Job& job = args.job[which];
     if (tile >= args.tile_of[which]) return;
-    const int col0 = tile * kCols, part = blockIdx.y;
+    const int col0 = tile * kCols, part = place.part;
     pdl_wait();
 
     const int64_t steps = args.steps;
     int64_t length = steps;
     if (args.lengths != nullptr) length = min(max(gload_i64(args.lengths + b), (int64_t)0), steps);
-    const int64_t begin = (int64_t)part * args.part_steps, stop = min(begin + args.part_steps, steps);
+    const int64_t begin = (int64_t)part * place.part_steps, stop = min(begin + place.part_steps, steps);
     const int64_t finish = min(stop, length);    // of the steps there are
     const bool reverse = job.reverse != 0;
     const double log_decay = log_decay_of(args.log_decay, h);
@@ -387,7 +404,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
                 }
             }
     if constexpr (!kEnds) {
-        const float whole = power_of(log_decay, args.part_steps);
+        const float whole = power_of(log_decay, place.part_steps);
         for (int s = 0; s < part; ++s) {
             const float* const sums = args.parts + (parts_of + s) * wa * wc;
             // (a part that the sequence ends in is the last one that anything reads)
@@ -573,7 +590,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
     }
 
     // (the first part ends a sequence of no steps)
-    const bool ends_here = kEnds || (length > begin && length <= begin + args.part_steps) || (length == 0 && part == 0);
+    const bool ends_here = kEnds || (length > begin && length <= begin + place.part_steps) || (length == 0 && part == 0);
     float* const to = kEnds ? args.parts + (parts_of + part) * wa * wc : job.end != nullptr ? job.end + (int64_t)unit * wa * wc : nullptr;
     if (ends_here && to != nullptr) {
         const float by = kEnds ? 1.0f : job.end_scale;
@@ -691,47 +708,60 @@ int check_attn(const dcn_attn* p) {
     if (p->batch < 0 || p->steps < 0 || p->heads < 1 || p->kv_heads < 1 || p->heads % p->kv_heads != 0 || p->dk < 1 || p->dv < 1)
         return DCN_ERR_SHAPE;
     if (!std::isfinite(p->scale) || p->scale == 0.0f || !std::isfinite(1.0f / p->scale)) return DCN_ERR_SHAPE;
-    if (p->dk > kMostWidth || p->dv > kMostWidth || p->heads > 65535 || p->steps >= 1ll << 31) return DCN_ERR_LIMIT;
+    if (p->dk > kMostWidth || p->dv > kMostWidth || p->heads > 65535 || p->steps >= 1ll << 30) return DCN_ERR_LIMIT;
     if (p->batch >= (1ll << 27) / p->heads) return DCN_ERR_LIMIT;
     return DCN_OK;
 }
 
 int wide_of(const dcn_attn* p, bool backward) { return (int)(backward ? std::max(p->dk, p->dv) : p->dk) > 64 ? 128 : 64; }
 
-// How many parts the time axis is split into.  Time goes in chunks of a CTA; a GPU holds `held` of them at once.  More parts fill the
-// GPU, and cost a pass over b and c for their sums (half of a chunk's time) and the folding (a quarter of a chunk's for each part
-// before), and each CTA what it costs to begin and to end.  (5x331x6x(40, 72) float32, 30 heads: three parts instead of one.)
-int parts_for(const dcn_attn* p, bool backward, bool tensor) {
+// How the work is shared out.  Time goes in chunks of a CTA; a GPU holds `held` CTAs at once.  As many units (job, head, 64 columns)
+// as fill it a whole number of times have their time axis to themselves; that of the others is split.  More parts fill the GPU, and cost
+// a pass over b and c for their sums (half of a chunk's time) and the folding (a quarter of a chunk's for each part before), and each CTA
+// what it costs to begin and to end.  (5x331x6x(40, 72) float32, 30 heads: three parts instead of one.  2x16384x16x128 bf16, where
+// the backward pass has 192 units: 798 us with its gradients, 834 us when all units were whole.)
+struct Split {
+    int64_t whole;
+    int parts;
+};
+Split split_of(const dcn_attn* p, bool backward, bool tensor, int jobs) {
     const int64_t ct = (backward ? std::max(p->dk, p->dv) : p->dv) > 64 ? 2 : 1, chunk = tensor ? tcgen::kSteps : kChunk;
-    const int64_t units = p->batch * p->heads * ct * (backward ? 3 : 1), chunks = (p->steps + chunk - 1) / chunk;
+    const int64_t units = p->batch * p->heads * ct * jobs, chunks = (p->steps + chunk - 1) / chunk;
     const int64_t held = (int64_t)sm_count() * (tensor ? 1 : wide_of(p, backward) == 128 || p->dtype == DCN_SEQ_F32 ? 2 : 3);
-    int best = 1;
-    double least = 1e300;
-    for (int n = 1; n <= kMostParts && n <= chunks; ++n) {
+    const double fixed = tensor ? 2 : 0.7;
+    const int64_t full = units / held * held, rest = units - full;
+    Split best = {units, 1};
+    double least = (double)((rest + held - 1) / held) * (chunks + fixed);
+    for (int n = 2; n <= kMostParts && n <= chunks; ++n) {
         const int64_t each = (chunks + n - 1) / n;
         if ((chunks + each - 1) / each != n) continue;
-        const double waves = (double)((units * n + held - 1) / held), sums = n > 1 ? (double)((units * (n - 1) + held - 1) / held) : 0;
-        const double fixed = tensor ? 2 : 0.7, time = waves * (each + fixed + 0.25 * (n - 1)) + sums * (0.5 * each + fixed) + (n > 1 ? 0.5 * fixed : 0);
-        if (time < least * 0.97) least = time, best = n;
+        const double waves = (double)((rest * n + held - 1) / held), sums = (double)((rest * (n - 1) + held - 1) / held);
+        const double time = waves * (each + fixed + 0.25 * (n - 1)) + sums * (0.5 * each + fixed) + 0.5 * fixed;
+        if (time < least * 0.97) least = time, best = {full, n};
     }
     return best;
 }
 
+unsigned ctas_of(const AttnArgs& a, bool ends) {
+    const int64_t rest = (int64_t)a.batch * a.heads * a.jobs * a.tiles - a.whole;
+    return (unsigned)(ends ? rest * (a.n_parts - 1) : a.whole + rest * a.n_parts);
+}
+
 template <typename T, int KA, bool kEnds>
-int launch_attn(const AttnArgs& a, int parts, cudaStream_t st) {
+int launch_attn(const AttnArgs& a, cudaStream_t st) {
     constexpr int kBytes = Shape<T, KA>::kBytes;
     if (cudaFuncSetAttribute(attn_kernel<T, KA, kEnds>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess)
         return DCN_ERR_CUDA;
-    const dim3 grid((unsigned)((int64_t)a.batch * a.heads * a.jobs * a.tiles), (unsigned)parts);
+    const dim3 grid(ctas_of(a, kEnds));
     return launch_dependent(attn_kernel<T, KA, kEnds>, grid, dim3(kThreads), kBytes, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
 template <typename T, int KA, bool kEnds>
-int launch_attn_tc(const AttnArgs& a, const tcgen::Maps& maps, int parts, cudaStream_t st) {
+int launch_attn_tc(const AttnArgs& a, const tcgen::Maps& maps, cudaStream_t st) {
     constexpr int kBytes = tcgen::Room<T, KA>::kBytes;
     const auto kernel = tcgen::attn_tc_kernel<T, KA, kEnds>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess) return DCN_ERR_CUDA;
-    const dim3 grid((unsigned)((int64_t)a.batch * a.heads * a.jobs * a.tiles), (unsigned)parts);
+    const dim3 grid(ctas_of(a, kEnds));
     return launch_dependent(kernel, grid, dim3(tcgen::kThreads), kBytes, st, a, maps) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
@@ -739,11 +769,11 @@ template <typename T, int KA>
 int run_parts(const AttnArgs& a, const tcgen::Maps* maps, cudaStream_t st) {
     if constexpr (!std::is_same<T, float>::value)
         if (maps != nullptr) {
-            const int rc = a.n_parts > 1 ? launch_attn_tc<T, KA, true>(a, *maps, a.n_parts - 1, st) : DCN_OK;
-            return rc != DCN_OK ? rc : launch_attn_tc<T, KA, false>(a, *maps, a.n_parts, st);
+            const int rc = a.n_parts > 1 ? launch_attn_tc<T, KA, true>(a, *maps, st) : DCN_OK;
+            return rc != DCN_OK ? rc : launch_attn_tc<T, KA, false>(a, *maps, st);
         }
-    const int rc = a.n_parts > 1 ? launch_attn<T, KA, true>(a, a.n_parts - 1, st) : DCN_OK;
-    return rc != DCN_OK ? rc : launch_attn<T, KA, false>(a, a.n_parts, st);
+    const int rc = a.n_parts > 1 ? launch_attn<T, KA, true>(a, st) : DCN_OK;
+    return rc != DCN_OK ? rc : launch_attn<T, KA, false>(a, st);
 }
 
 template <typename T>
@@ -826,16 +856,21 @@ bool make_maps(const dcn_attn* p, const Operands& o, tcgen::Maps& maps) {
     return true;
 }
 
-AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* lengths, bool backward, bool tensor) {
+AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* lengths) {
     AttnArgs a = {};
     a.log_decay = log_decay, a.lengths = lengths;
     a.steps = p->steps;
     a.batch = (int)p->batch, a.heads = (int)p->heads;
-    a.n_parts = parts_for(p, backward, tensor);
-    const int64_t chunk = tensor ? tcgen::kSteps : kChunk, chunks = (p->steps + chunk - 1) / chunk;
-    a.part_steps = std::max<int64_t>(1, (chunks + a.n_parts - 1) / a.n_parts) * chunk;
     a.scale = p->scale;
     return a;
+}
+
+// (once the jobs are there)
+void share_out(AttnArgs& a, const dcn_attn* p, bool backward, bool tensor) {
+    const Split split = split_of(p, backward, tensor, a.jobs);
+    const int64_t chunk = tensor ? tcgen::kSteps : kChunk, chunks = (p->steps + chunk - 1) / chunk;
+    a.n_parts = split.parts, a.whole = split.whole;
+    a.part_steps = std::max<int64_t>(1, (chunks + a.n_parts - 1) / a.n_parts) * chunk;
 }
 
 void add(AttnArgs& a, const Job& j, int elem) {
@@ -849,7 +884,9 @@ void add(AttnArgs& a, const Job& j, int elem) {
 size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 size_t state_elems(const dcn_attn* p) { return (size_t)p->batch * p->heads * p->dk * p->dv; }
 size_t parts_bytes(const dcn_attn* p, bool backward) {
-    const int n = std::max(parts_for(p, backward, false), parts_for(p, backward, true));         // (whichever a call's pointers allow)
+    int n = 1;                                   // (whichever kernel a call's pointers allow, however many gradients it wants)
+    for (int tensor = 0; tensor < 2; ++tensor)
+        for (int jobs = 1; jobs <= (backward ? 3 : 1); ++jobs) n = std::max(n, split_of(p, backward, tensor != 0, jobs).parts);
     if (n <= 1) return 0;
     if (!backward) return rounded((size_t)n * state_elems(p) * 4);
     const size_t dk = p->dk, dv = p->dv, most = std::max(dk, dv) * dv;         // the jobs' states are dv x dk, dv x dk and dk x dv
@@ -902,9 +939,10 @@ extern "C" int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k,
     const Operands o = operands(p, q, k, v, nullptr);
     tcgen::Maps maps = {};
     const bool tensor = takes_tensor(p, o, {out, last, workspace}) && make_maps(p, o, maps);
-    AttnArgs a = attn_args(p, log_decay, lengths, false, tensor);
+    AttnArgs a = attn_args(p, log_decay, lengths);
     a.parts = static_cast<float*>(workspace);
     add(a, {o.q, o.k, o.v, out, state, last, (int)p->dv, 1, 0, 0, 1.0f, 1.0f}, elem_bytes(p->dtype));
+    share_out(a, p, false, tensor);
     return run_attn_any(p, a, false, tensor ? &maps : nullptr, (cudaStream_t)stream);
 }
 
@@ -923,7 +961,7 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
     const Operands o = operands(p, q, k, v, dout);
     tcgen::Maps maps = {};
     const bool tensor = takes_tensor(p, o, {dq, dk, dv, dstate, workspace}) && make_maps(p, o, maps);
-    AttnArgs a = attn_args(p, log_decay, lengths, true, tensor);
+    AttnArgs a = attn_args(p, log_decay, lengths);
     a.parts = static_cast<float*>(workspace);
     const bool shared = p->heads != p->kv_heads;
     char* const wide_k = static_cast<char*>(workspace) + parts_bytes(p, true);
@@ -937,6 +975,7 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
         add(a, {o.k, o.q, o.d, shared ? wide_v : dv, dlast, dstate, across, 1, 1, shared, 1.0f / s, s}, elem);
     }
     if (a.jobs == 0) return DCN_OK;
+    share_out(a, p, true, tensor);
     int rc = run_attn_any(p, a, true, tensor ? &maps : nullptr, st);
     if (rc != DCN_OK || !shared || p->steps == 0) return rc;
     const int share = (int)(p->heads / p->kv_heads);

@@ -129,14 +129,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     Control& ctl = *reinterpret_cast<Control*>(smem + R::kControl);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    int u = blockIdx.x;
-    const int tile = u % args.tiles;
-    u /= args.tiles;
-    const int which = u % args.jobs;
-    const int unit = u / args.jobs, h = unit % args.heads, b = unit / args.heads;
+    const Place place = Place::of<kEnds>(args);
+    const int tile = place.tile, which = place.which, unit = place.unit, h = unit % args.heads, b = unit / args.heads;
     const Job& job = args.job[which];
     if (tile >= args.tile_of[which]) return;
-    const int col0 = tile * kDv, part = blockIdx.y;
+    const int col0 = tile * kDv, part = place.part;
 
     if (warp == 3) {
         tc::tmem_alloc(&ctl.tmem, 512);
@@ -165,12 +162,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             if (n > 0) ctl.diagonal[job.reverse ? 32 + n : 32 - n] = 0.0f;
         }
     }
-    const int64_t steps = args.steps;
-    int64_t length = steps;
-    if (args.lengths != nullptr) length = min(max(gload_i64(args.lengths + b), (int64_t)0), steps);
-    const int64_t begin = (int64_t)part * args.part_steps, stop = min(begin + args.part_steps, steps);
-    const int64_t finish = min(stop, length);
-    const int chunks = finish > begin ? (int)((finish - begin + kSteps - 1) / kSteps) : 0;
+    const int steps = (int)args.steps, part_steps = (int)place.part_steps;       // (below 2^30)
+    int length = steps;
+    if (args.lengths != nullptr) length = (int)min(max(gload_i64(args.lengths + b), (int64_t)0), (int64_t)steps);
+    const int begin = part * part_steps, finish = min(min(begin + part_steps, steps), length);
+    const int chunks = finish > begin ? (finish - begin + kSteps - 1) / kSteps : 0;
+    const bool ends_here = kEnds || (length > begin && length <= begin + part_steps) || (length == 0 && part == 0);
     const bool reverse = job.reverse != 0;
     const int extra = reverse ? 0 : 1, wa = job.a.width, wc = job.c.width;
     tc::tc_fence_before();
@@ -181,12 +178,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     // Tiles that C' is the sum of: all where the state is a result and the chunk so near its end that two would be seen in it (those
     // before it count e^-1.5 and less), else two
     const auto parts_of_chunk = [&](int n) {
-        const float after = (float)(length - begin - (int64_t)(n + 1) * kSteps);
+        const float after = (float)(length - begin - (n + 1) * kSteps);
         return job.end != nullptr && after * -log_decay < 1.5f ? R::kParts : 2;
     };
 
     // Behind a sequence's end, but inside the tensor, rows hold what they may: b's and c's of the last chunk are made zeros
-    const int ragged = !reverse && length < steps && chunks > 0 && length < begin + (int64_t)chunks * kSteps ? chunks - 1 : -1;
+    const int ragged = !reverse && length < steps && chunks > 0 && length < begin + chunks * kSteps ? chunks - 1 : -1;
 
     if (warp == 0) {
         // ---- loads
@@ -197,8 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 uint64_t* const bar = &ctl.full[ring.i];
                 if (n >= R::kStages && !wait(&ctl.empty[ring.i], ring.ph ^ 1)) break;
                 const uint32_t to = base + ring.i * R::kStage;
-                const int64_t first = begin + (int64_t)n * kSteps;
-                const int t = (int)(reverse ? length - kSteps - first : first);
+                const int first = begin + n * kSteps, t = reverse ? length - kSteps - first : first;
                 tc::mbar_arrive_expect_tx(bar, kEnds ? R::kA : 2 * R::kA);
 #pragma unroll
                 for (int k = 0; k < KA / 64; ++k) {
@@ -274,8 +270,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 __syncwarp();
                 tc::tc_fence_after();
                 const float w1 = weight * ctl.up[n & 3];
-                const bool in = i < (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps);
-                const int64_t t = reverse ? length - kSteps - begin - (int64_t)n * kSteps + r : begin + (int64_t)n * kSteps + r;
+                const bool in = i < finish - begin - n * kSteps;
+                const int t = reverse ? length - kSteps - begin - n * kSteps + r : begin + n * kSteps + r;
                 char* to = first_row + t * row_bytes;
 #pragma unroll 1
                 for (int cb = 0; cb < 4; ++cb) {
@@ -315,9 +311,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
             }
             // zeros behind the length
-            const int64_t from = max(begin, length);
-            const int cols = min(kDv, wc - col0) / 8;
-            for (int64_t k = threadIdx.x - 256; k < (stop - from) * cols; k += 128) {
+            const int from = max(begin, length), cols = min(kDv, wc - col0) / 8;
+            for (int64_t k = threadIdx.x - 256; k < (int64_t)(min(begin + part_steps, steps) - from) * cols; k += 128) {
                 const int64_t at = (((int64_t)b * steps + from + k / cols) * args.heads + h) * wc + col0 + k % cols * 8;
                 if (job.wide) {
                     float4* const d = reinterpret_cast<float4*>(static_cast<float*>(job.out) + at);
@@ -330,12 +325,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     } else if (warp >= 12 && warp < 16) {
         // ---- the weighted c, half a chunk at a time
         const int tid = threadIdx.x - 384, c = tid & 7, r0 = tid >> 3;           // 16 bytes of rows r0, r0 + 16, ...
-        const uint32_t place = tc::swz_offset(r0, c);
+        const uint32_t spot = tc::swz_offset(r0, c);
         bool ok = true;
         tc::Ring ring;
         for (int n = 0; n < chunks && ok; ++n, ring.next(R::kStages)) {
             ok = wait(&ctl.full_c[ring.i], ring.ph);
-            const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps), top = rows - extra, parts = parts_of_chunk(n);
+            const int rows = min(kSteps, finish - begin - n * kSteps), top = rows - extra, parts = parts_of_chunk(n);
             if (ok && n == ragged && wait(&ctl.full[ring.i], ring.ph)) {
                 const uint32_t tile = base + ring.i * R::kStage + R::kA;        // b's halves, and c's behind them
                 for (int k = tid; k < (KA / 64 + 1) * (kSteps - rows) * 8; k += 128)
@@ -347,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             for (int half = 0; half < 2 && ok; ++half) {
                 ok = n == 0 || wait(&ctl.c_empty[half], (n - 1) & 1);
                 if (!ok) break;
-                const uint32_t from = base + ring.i * R::kStage + 2 * R::kA + place + half * 8192, to = base + R::kWeighted + place + half * 8192;
+                const uint32_t from = base + ring.i * R::kStage + 2 * R::kA + spot + half * 8192, to = base + R::kWeighted + spot + half * 8192;
 #pragma unroll 1
                 for (int p = 0; p < 4; ++p) {
                     const int row = r0 + 16 * p + 64 * half, j = reverse ? kSteps - 1 - row : row;
@@ -391,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         }
         if constexpr (!kEnds) {
             if (part > 0 && begin < length && i < wa) {
-                const float whole = (float)exp((double)args.part_steps * (double)log_decay);
+                const float whole = (float)exp((double)part_steps * (double)log_decay);
                 for (int s = 0; s < part; ++s) {
                     const float* const sums = args.parts + (parts_of + s) * wa * wc + (int64_t)i * wc + col0;
 #pragma unroll
@@ -437,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         bool ok = true;
         if constexpr (!kEnds) put_copy(0);
         for (int n = 0; n < chunks; ++n) {
-            const int rows = (int)min((int64_t)kSteps, finish - begin - (int64_t)n * kSteps);
+            const int rows = min(kSteps, finish - begin - n * kSteps);
             const Lanes whole = all_lanes(table(power + 4 * rows));
             ok = wait(&ctl.u_full, n & 1);
             if (!ok) break;
@@ -468,7 +463,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
             }
         }
-        const bool ends_here = kEnds || (length > begin && length <= begin + args.part_steps) || (length == 0 && part == 0);
         float* const to = kEnds ? args.parts + (parts_of + part) * wa * wc : job.end != nullptr ? job.end + (int64_t)unit * wa * wc : nullptr;
         if (ok && ends_here && to != nullptr && mine && i < wa) {
             const float by = kEnds ? 1.0f : job.end_scale;

@@ -140,7 +140,7 @@ int dcn_distill_backward(const dcn_logits* p, const void* logits, int32_t k, con
 typedef struct dcn_attn {
     int32_t dtype;                              /* q, k, v, out and their gradients */
     int64_t batch, steps, heads, kv_heads;      /* kv_heads divides heads: head h has the key and value h / (heads / kv_heads) */
-    int64_t dk, dv;                             /* 1 to 128 each */
+    int64_t dk, dv;                             /* 1 to 128 each; steps < 2^30 */
     int64_t q_batch, q_step, q_head;            /* strides */
     int64_t k_batch, k_step, k_head;
     int64_t v_batch, v_step, v_head;
