@@ -269,27 +269,27 @@ __device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, FragA<T>& la
         }
     }
 }
-// the scores of 16 steps as the left operand of the product over k0, k0 + 1, ...
-template <typename T, int N>
-__device__ __forceinline__ void scores_as_a(FragA<T>& f, const float (&s)[N][4], int step) {
-    if constexpr (std::is_same<T, float>::value) {
-        split(s[step][0], f.v[0], f.low[0]), split(s[step][2], f.v[1], f.low[1]);
-        split(s[step][1], f.v[2], f.low[2]), split(s[step][3], f.v[3], f.low[3]);
-    } else {
-        f.v[0] = word_of<T>(s[2 * step][0], s[2 * step][1]), f.v[1] = word_of<T>(s[2 * step][2], s[2 * step][3]);
-        f.v[2] = word_of<T>(s[2 * step + 1][0], s[2 * step + 1][1]), f.v[3] = word_of<T>(s[2 * step + 1][2], s[2 * step + 1][3]);
-    }
+// The warps of a group meet
+template <int kCount>
+__device__ __forceinline__ void group_sync(int barrier) {
+    asm volatile("bar.sync %0, %1;" ::"r"(barrier), "n"(kCount) : "memory");
+}
+// two scores side by side, as load_a finds them
+template <typename T>
+__device__ __forceinline__ void put_pair(uint32_t at, float p, float q) {
+    if constexpr (std::is_same<T, float>::value) asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(p), "f"(q) : "memory");
+    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(word_of<T>(p, q)) : "memory");
 }
 
 // ---- tiles ----------------------------------------------------------------------------------------------------------------
 // Rows first, first + 1, ... of a sequence (back in time from `length` where reverse) into a tile of kCols_ columns; zeros beyond the
 // length and the operand's width.
-template <typename T, int kCols_>
+template <typename T, int kCols_, int kT>
 __device__ __forceinline__ void load_tile(uint32_t base, const Operand& o, const char* from, int64_t first, int64_t length, int col0,
                                           bool reverse) {
     constexpr int kElem = sizeof(T), kVec = 16 / kElem, kPerRow = kCols_ / kVec;
     const int width = o.width - col0;            // (may be above kCols_)
-    for (int i = threadIdx.x; i < kChunk * kPerRow; i += kThreads) {
+    for (int i = threadIdx.x; i < kChunk * kPerRow; i += kT) {
         const int row = i / kPerRow, col = (i % kPerRow) * kVec;
         const int64_t pos = first + row;
         const bool in = pos < length && col < width;
@@ -321,40 +321,49 @@ __device__ __forceinline__ void load_tile(uint32_t base, const Operand& o, const
     }
 }
 
-template <typename T, int KA>
+template <typename T, int KA, bool kEnds>
 struct Shape {
-    static constexpr int kStages = sizeof(T) == 2 ? 2 : 1;
+    static constexpr bool kFloat = sizeof(T) == 4;
+    static constexpr int kAcross = kEnds ? 2 : kFloat && KA == 128 ? 4 : kFloat || KA == 128 ? 2 : 1;      // warps that share 16 steps (rows of the state), each some of c's columns
+    static constexpr int kThreads = 128 * kAcross, kWarps = 4 * kAcross;
+    static constexpr int kStages = kFloat && !kEnds && KA == 64 ? 1 : 2;
     static constexpr int kTileA = kChunk * Tile<T>::row_elems(KA) * (int)sizeof(T);
     static constexpr int kTileC = kChunk * Tile<T>::row_elems(kCols) * (int)sizeof(T);
-    static constexpr int kState = KA * Tile<T>::row_elems(kCols) * (int)sizeof(T);
-    static constexpr int kStage = 2 * kTileA + kTileC;
+    static constexpr int kState = kEnds ? 0 : KA * Tile<T>::row_elems(kCols) * (int)sizeof(T);
+    static constexpr int kB = kEnds ? 0 : kTileA, kC = kB + kTileA, kStage = kC + kTileC;                // b's and c's places
     static constexpr int kTable = kStages * kStage + kState;             // g^n, 0 to 64
-    static constexpr int kBytes = kTable + (kChunk + 1) * 4 + 32;
+    static constexpr int kBytes = kTable + (kChunk + 1) * 4 + kWarps * 4;
+    static constexpr int kHeld = kEnds ? (kFloat && KA == 128 ? 2 : 3) : kFloat && KA == 128 ? 1 : kFloat || KA == 128 ? 2 : 3;           // CTAs that an SM has room for
 };
 
 // The maximum of a CTA's states, for the power of two that keeps a float16 copy of them in range
+template <int kWarps>
 __device__ __forceinline__ float cta_max(float v, float* slots) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
     __syncthreads();
-    return fmaxf(fmaxf(slots[0], slots[1]), fmaxf(slots[2], slots[3]));
+    v = slots[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) v = fmaxf(v, slots[w]);
+    return v;
 }
 
 // kEnds: the sums of each part's b_j c_j^T alone
 template <typename T, int KA, bool kEnds>
-__global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
-    using S = Shape<T, KA>;
+__global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kEnds>::kHeld) attn_kernel(const AttnArgs args) {
+    using S = Shape<T, KA, kEnds>;
     using L = Tile<T>;
     constexpr int kM = KA / 64;                  // 16-row tiles of the state that a warp has
-    constexpr int kN = kCols / 8;
+    constexpr int kAcross = S::kAcross, kN = kCols / 8 / kAcross;       // 8-column tiles of c, in pairs
     constexpr int kSteps = kChunk / L::kK;
     extern __shared__ __align__(128) char smem[];
     const uint32_t tiles = shared_address(smem), copy = tiles + S::kStages * S::kStage;
     float* const powers = reinterpret_cast<float*>(smem + S::kTable);
     float* const slots = powers + kChunk + 1;
     const uint32_t table = shared_address(powers);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int warp = (threadIdx.x >> 5) & 3, side = threadIdx.x >> 7, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    auto col_of = [side](int n) { return ((n >> 1) * kAcross + side) * 16 + (n & 1) * 8; };              // where a warp's n-th tile lies
 
     const Place place = Place::of<kEnds>(args);
     const int tile = place.tile, which = place.which, unit = place.unit, h = unit % args.heads, b = unit / args.heads;
@@ -374,15 +383,15 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
     const int extra = reverse ? 0 : 1;           // powers of g on the state before a chunk, at its first step
     const int wa = job.a.width, wc = job.c.width;
     const bool exact = job.end != nullptr;       // the state is a result
-    const int k_end = (wa + L::kK - 1) / L::kK * L::kK, n_end = min(kN, (wc - col0 + 15) / 16 * 2);        // of a's width, of c's columns
+    const int k_end = (wa + L::kK - 1) / L::kK * L::kK, c_end = wc - col0;        // of a's width, of c's columns
     const char* const from_a = static_cast<const char*>(job.a.p) + (b * job.a.s.batch + h / job.a.share * job.a.s.head) * (int64_t)sizeof(T);
     const char* const from_b = static_cast<const char*>(job.b.p) + (b * job.b.s.batch + h / job.b.share * job.b.s.head) * (int64_t)sizeof(T);
     const char* const from_c = static_cast<const char*>(job.c.p) + (b * job.c.s.batch + h / job.c.share * job.c.s.head) * (int64_t)sizeof(T);
     auto fetch = [&](int stage, int64_t first) {
         const uint32_t base = tiles + stage * S::kStage;
-        if constexpr (!kEnds) load_tile<T, KA>(base, job.a, from_a, first, length, 0, reverse);
-        load_tile<T, KA>(base + S::kTileA, job.b, from_b, first, length, 0, reverse);
-        load_tile<T, kCols>(base + 2 * S::kTileA, job.c, from_c, first, length, col0, reverse);
+        if constexpr (!kEnds) load_tile<T, KA, S::kThreads>(base, job.a, from_a, first, length, 0, reverse);
+        load_tile<T, KA, S::kThreads>(base + S::kB, job.b, from_b, first, length, 0, reverse);
+        load_tile<T, kCols, S::kThreads>(base + S::kC, job.c, from_c, first, length, col0, reverse);
         copies_issued();
     };
     if (S::kStages == 2 && begin < finish) fetch(0, begin);
@@ -398,7 +407,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
             for (int e = 0; e < 4; ++e) {
                 x[m][n][e] = 0.0f;
                 if constexpr (!kEnds) {
-                    const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                    const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + col_of(n) + 2 * t + (e & 1);
                     if (job.init != nullptr && i < wa && j < wc)
                         x[m][n][e] = job.init_scale * gload(job.init + (int64_t)unit * wa * wc + (int64_t)i * job.init_i + (int64_t)j * job.init_j);
                 }
@@ -414,7 +423,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
                 for (int n = 0; n < kN; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                        const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + col_of(n) + 2 * t + (e & 1);
                         if (i < wa && j < wc && begin < length) x[m][n][e] = fmaf(x[m][n][e], whole, gload(sums + (int64_t)i * wc + j));
                     }
         }
@@ -430,7 +439,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
                 for (int n = 0; n < kN; ++n)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[m][n][e]));
-            most = cta_max(most, slots);
+            most = cta_max<S::kWarps>(most, slots);
             const int over = max((int)(__float_as_uint(most) >> 23) - 127 - 14, 0);
             down = __uint_as_float((uint32_t)(127 - min(over, 126)) << 23);
             up = __uint_as_float((uint32_t)(127 + min(over, 126)) << 23);
@@ -440,14 +449,9 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t at = L::at(copy, (m * 4 + warp) * 16 + g + half * 8, n * 8 + 2 * t, kCols);
-                    const float p = x[m][n][2 * half], q = x[m][n][2 * half + 1];
-                    if constexpr (std::is_same<T, float>::value)
-                        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(at), "f"(p), "f"(q) : "memory");
-                    else
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(word_of<T>(p * down, q * down)) : "memory");
-                }
+                for (int half = 0; half < 2; ++half)
+                    put_pair<T>(L::at(copy, (m * 4 + warp) * 16 + g + half * 8, col_of(n) + 2 * t, kCols), x[m][n][2 * half] * down,
+                                x[m][n][2 * half + 1] * down);
     };
     if constexpr (!kEnds) put_copy();
 
@@ -458,59 +462,63 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
         copies_arrived<0>();
         __syncthreads();                         // this chunk's tiles and the copy of the state are there
         if (S::kStages == 2 && first + kChunk < finish) fetch(stage ^ 1, first + kChunk);
-        const uint32_t at = tiles + (S::kStages == 2 ? stage : 0) * S::kStage, bt = at + S::kTileA, ct = at + 2 * S::kTileA;
+        const uint32_t at = tiles + (S::kStages == 2 ? stage : 0) * S::kStage, bt = at + S::kB, ct = at + S::kC;
         if constexpr (!kEnds) {
             // which 16 steps a warp has goes round, so that the long rows of the triangle do not always meet the same scheduler
             const int m0 = ((warp + blockIdx.x + (int)(first / kChunk)) & 3) * 16;
             if (m0 < rows) {
-                float o[kN][4] = {};
+                // a . X and a . b^T, each warp some pairs of columns of either
+                float o[kN][4] = {}, s[kN][4] = {};
 #pragma unroll 2
                 for (int k = 0; k < k_end; k += L::kK) {
                     FragA<T> fa;
                     load_a<T>(fa, at, m0, k, KA, lane);
 #pragma unroll
                     for (int n = 0; n < kN; n += 2) {
-                        if (n >= n_end) continue;
-                        FragB<T> fb[2];
-                        load_bt<T>(fb, copy, k, n * 8, kCols, lane);
-                        mma<T>(o[n], fa, fb[0]);
-                        mma<T>(o[n + 1], fa, fb[1]);
+                        if (col_of(n) < c_end) {
+                            FragB<T> fb[2];
+                            load_bt<T>(fb, copy, k, col_of(n), kCols, lane);
+                            mma<T>(o[n], fa, fb[0]);
+                            mma<T>(o[n + 1], fa, fb[1]);
+                        }
+                        if (col_of(n) <= m0) {
+                            FragB<T> fb[2];
+                            load_b<T>(fb, bt, col_of(n), k, KA, lane);
+                            mma<T>(s[n], fa, fb[0]);
+                            mma<T>(s[n + 1], fa, fb[1]);
+                        }
                     }
                 }
                 const float w0 = power(table, m0 + g + extra) * up, w1 = power(table, m0 + g + 8 + extra) * up;
 #pragma unroll
                 for (int n = 0; n < kN; ++n) o[n][0] *= w0, o[n][1] *= w0, o[n][2] *= w1, o[n][3] *= w1;
-                float s[kN][4] = {};
-#pragma unroll 2
-                for (int k = 0; k < k_end; k += L::kK) {
-                    FragA<T> fa;
-                    load_a<T>(fa, at, m0, k, KA, lane);
-#pragma unroll
-                    for (int n = 0; n < kN; n += 2) {
-                        if (n * 8 > m0) continue;
-                        FragB<T> fb[2];
-                        load_b<T>(fb, bt, n * 8, k, KA, lane);
-                        mma<T>(s[n], fa, fb[0]);
-                        mma<T>(s[n + 1], fa, fb[1]);
-                    }
-                }
+                // the scores take the place of these 16 steps of a, which these warps alone have read
+                group_sync<32 * kAcross>(1 + warp);
 #pragma unroll
                 for (int n = 0; n < kN; ++n)
+                    if (col_of(n & ~1) <= m0) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int d = m0 + g + (e >> 1) * 8 - (n * 8 + 2 * t + (e & 1));
-                        s[n][e] = d >= 0 ? s[n][e] * power(table, max(d, 0)) : 0.0f;
+                        for (int half = 0; half < 2; ++half) {
+                            float p[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int d = m0 + g + half * 8 - (col_of(n) + 2 * t + e);
+                                p[e] = d >= 0 ? s[n][2 * half + e] * power(table, max(d, 0)) : 0.0f;
+                            }
+                            put_pair<T>(L::at(at, m0 + g + half * 8, col_of(n) + 2 * t, KA), p[0], p[1]);
+                        }
                     }
+                group_sync<32 * kAcross>(1 + warp);
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     if (k * L::kK > m0 + 15 || k * L::kK >= rows) continue;
                     FragA<T> fa;
-                    scores_as_a<T>(fa, s, k);
+                    load_a<T>(fa, at, m0, k * L::kK, KA, lane);
 #pragma unroll
                     for (int n = 0; n < kN; n += 2) {
-                        if (n >= n_end) continue;
+                        if (col_of(n) >= c_end) continue;
                         FragB<T> fb[2];
-                        load_bt<T>(fb, ct, k * L::kK, n * 8, kCols, lane);
+                        load_bt<T>(fb, ct, k * L::kK, col_of(n), kCols, lane);
                         mma<T>(o[n], fa, fb[0]);
                         mma<T>(o[n + 1], fa, fb[1]);
                     }
@@ -523,7 +531,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
                     const int64_t to = (((int64_t)b * steps + step) * args.heads + h) * wc + col0;
 #pragma unroll
                     for (int n = 0; n < kN; ++n) {
-                        const int c = n * 8 + 2 * t;
+                        const int c = col_of(n) + 2 * t;
                         const float p = o[n][2 * half] * args.scale, q = o[n][2 * half + 1] * args.scale;
                         const bool both = c + 1 < wc - col0, pairs = job.pairs != 0;
                         if (c >= wc - col0) continue;
@@ -562,7 +570,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
             FragB<T> fb[kN / 2][2];
 #pragma unroll
             for (int n = 0; n < kN; n += 2)
-                if (n < n_end) load_bt<T>(fb[n / 2], ct, k, n * 8, kCols, lane);
+                if (col_of(n) < c_end) load_bt<T>(fb[n / 2], ct, k, col_of(n), kCols, lane);
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
                 if ((m * 4 + warp) * 16 >= wa) continue;
@@ -570,7 +578,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
                 load_at<T>(fa, low, lowest, bt, k, (m * 4 + warp) * 16, KA, lane, table, last_power, rows);
 #pragma unroll
                 for (int n = 0; n < kN; n += 2) {
-                    if (n >= n_end) continue;
+                    if (col_of(n) >= c_end) continue;
                     mma<T>(x[m][n], fa, fb[n / 2][0]);
                     mma<T>(x[m][n + 1], fa, fb[n / 2][1]);
                     if constexpr (!std::is_same<T, float>::value) {
@@ -600,7 +608,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
             for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + n * 8 + 2 * t + (e & 1);
+                    const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + col_of(n) + 2 * t + (e & 1);
                     if (i < wa && j < wc) to[(int64_t)i * wc + j] = by * x[m][n][e];
                 }
     }
@@ -609,7 +617,7 @@ __global__ void __launch_bounds__(kThreads) attn_kernel(const AttnArgs args) {
         const int64_t from = max(begin, length);
         const int n = min(kCols, wc - col0);
         const int64_t count = (stop - from) * n;
-        for (int64_t i = threadIdx.x; i < count; i += kThreads) {
+        for (int64_t i = threadIdx.x; i < count; i += S::kThreads) {
             const int64_t step = from + i / n, to_ = (((int64_t)b * steps + step) * args.heads + h) * wc + col0 + i % n;
             if (std::is_same<T, float>::value || job.wide) static_cast<float*>(job.out)[to_] = 0.0f;
             else static_cast<T*>(job.out)[to_] = from_float<T>(0.0f);
@@ -720,6 +728,10 @@ int wide_of(const dcn_attn* p, bool backward) { return (int)(backward ? std::max
 // a pass over b and c for their sums (half of a chunk's time) and the folding (a quarter of a chunk's for each part before), and each CTA
 // what it costs to begin and to end.  (5x331x6x(40, 72) float32, 30 heads: three parts instead of one.  2x16384x16x128 bf16, where
 // the backward pass has 192 units: 798 us with its gradients, 834 us when all units were whole.)
+int held_of(bool wide_type, int width) {
+    if (wide_type) return width == 128 ? Shape<float, 128, false>::kHeld : Shape<float, 64, false>::kHeld;
+    return width == 128 ? Shape<__half, 128, false>::kHeld : Shape<__half, 64, false>::kHeld;
+}
 struct Split {
     int64_t whole;
     int parts;
@@ -727,7 +739,7 @@ struct Split {
 Split split_of(const dcn_attn* p, bool backward, bool tensor, int jobs) {
     const int64_t ct = (backward ? std::max(p->dk, p->dv) : p->dv) > 64 ? 2 : 1, chunk = tensor ? tcgen::kSteps : kChunk;
     const int64_t units = p->batch * p->heads * ct * jobs, chunks = (p->steps + chunk - 1) / chunk;
-    const int64_t held = (int64_t)sm_count() * (tensor ? 1 : wide_of(p, backward) == 128 || p->dtype == DCN_SEQ_F32 ? 2 : 3);
+    const int64_t held = (int64_t)sm_count() * (tensor ? 1 : held_of(p->dtype == DCN_SEQ_F32, wide_of(p, backward)));
     const double fixed = tensor ? 2 : 0.7;
     const int64_t full = units / held * held, rest = units - full;
     Split best = {units, 1};
@@ -749,11 +761,12 @@ unsigned ctas_of(const AttnArgs& a, bool ends) {
 
 template <typename T, int KA, bool kEnds>
 int launch_attn(const AttnArgs& a, cudaStream_t st) {
-    constexpr int kBytes = Shape<T, KA>::kBytes;
+    using S = Shape<T, KA, kEnds>;
+    constexpr int kBytes = S::kBytes;
     if (cudaFuncSetAttribute(attn_kernel<T, KA, kEnds>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess)
         return DCN_ERR_CUDA;
     const dim3 grid(ctas_of(a, kEnds));
-    return launch_dependent(attn_kernel<T, KA, kEnds>, grid, dim3(kThreads), kBytes, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
+    return launch_dependent(attn_kernel<T, KA, kEnds>, grid, dim3(S::kThreads), kBytes, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
 template <typename T, int KA, bool kEnds>
