@@ -39,9 +39,10 @@ struct Operand {
 
 struct Job {
     Operand a, b, c;
-    void* out;                                   // [batch, steps, heads, c.width], dense; float32 where wide
+    void* out;                                   // [batch, steps, heads, room], dense; float32 where wide
     const float* init;                           // [batch, heads, ...]: element (i, j) at i * init_i + j * init_j; NULL: zeros
     float* end;                                  // [batch, heads, a.width, c.width] dense, or NULL
+    int room;                                    // elements of a row of out and of the parts: c's width, or the next multiple of 8
     int init_i, init_j;
     int reverse, wide;
     float init_scale, end_scale;
@@ -53,7 +54,7 @@ struct AttnArgs {
     Job job[3];
     const float* log_decay;
     const int64_t* lengths;
-    float* parts;                                // [job][batch * heads][part][a.width][c.width]
+    float* parts;                                // [job][batch * heads][part][a.width][room]
     int64_t steps, part_steps;
     int64_t whole;                               // units (job, head, tile) whose time axis is not split
     int batch, heads, jobs, tiles, n_parts;      // tiles: of 64 columns, the most that a job has
@@ -625,16 +626,108 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
     }
 }
 
-// Sum of the gradients of the heads that share a key or a value
+// Narrow loads that stay in L1: their neighbours find the rest of a sector there (without, each fetched it from L2 again, and joining
+// 502 K rows of 71 took 131 us)
+__device__ __forceinline__ uint32_t load_word(const void* p) {
+    uint32_t v;
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
 template <typename T>
-__global__ void __launch_bounds__(256) shared_kernel(const float* from, T* to, int64_t count, int share, int width) {
+__device__ __forceinline__ float load_element(const T* p) {
+    if constexpr (sizeof(T) == 4) {
+        return __uint_as_float(load_word(p));
+    } else {
+        uint16_t v;
+        asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));
+        return to_float(*reinterpret_cast<const T*>(&v));
+    }
+}
+
+// Rows that a bulk copy does not take (widths that 8 does not divide, odd strides, inputs that are broadcast) as rows that it takes: the
+// width rounded up to 8, heads and steps dense.  A thread moves 16 bytes, read as aligned words of 4; what lies behind a row's end is
+// not written, nor ever read.
+struct PackArgs {
+    struct One {
+        const char* from;
+        char* to;
+        int64_t batch, step, head;               // bytes
+        int width, vecs, heads;
+    } of[4];
+    const int64_t* lengths;
+    int64_t rows, steps;                         // rows: batch * steps
+    int span;                                    // 16 bytes that a CTA has at a time, about
+};
+
+__global__ void __launch_bounds__(256) pack_kernel(const PackArgs args) {
+    const PackArgs::One o = args.of[blockIdx.y];
     pdl_wait();
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
-        const int64_t row = i / width;
-        const float* p = from + row * share * width + i % width;
-        float sum = 0.0f;
-        for (int s = 0; s < share; ++s) sum += gload(p + (int64_t)s * width);
-        to[i] = from_float<T>(sum);
+    const int row_vecs = o.heads * o.vecs, block_rows = max(1, args.span / row_vecs);
+    for (int64_t row0 = (int64_t)blockIdx.x * block_rows; row0 < args.rows; row0 += (int64_t)gridDim.x * block_rows) {
+        const int64_t b0 = row0 / args.steps, t0 = row0 - b0 * args.steps;
+        const int count = (int)min((int64_t)block_rows, args.rows - row0) * row_vecs;
+#pragma unroll 4
+        for (int i = threadIdx.x; i < count; i += 256) {
+            const int row = i / row_vecs, in_row = i - row * row_vecs, h = in_row / o.vecs, v = in_row - h * o.vecs;
+            const uint32_t from0 = (uint32_t)t0 + row, more = from0 / (uint32_t)args.steps;
+            const int64_t b = b0 + more, t = from0 - more * (uint32_t)args.steps;
+            const bool live = args.lengths == nullptr || t < gload_i64(args.lengths + b);
+            const char* const from = o.from + b * o.batch + t * o.step + h * o.head + v * 16;
+            const int bytes = live ? min(16, (o.width - v * 8) * 2) : 0, skew = (int)(reinterpret_cast<uintptr_t>(from) & 2);
+            uint32_t w[5];
+#pragma unroll
+            for (int k = 0; k < 5; ++k) {
+                w[k] = bytes > 0 && 4 * k - skew < bytes ? load_word(from - skew + 4 * k) : 0;
+            }
+            Raw<16> out;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) out.u[k] = __funnelshift_r(w[k], w[k + 1], skew * 8);
+            if (live) store(o.to + ((row0 + row) * row_vecs + in_row) * 16, out);
+        }
+    }
+}
+
+// Gradients of keys and values that heads share, as sums over these (From: float); or results with rows of a multiple of 8 (From: T) as
+// the dense ones that they are.  A thread writes 16 bytes, whichever rows they are of.
+template <typename T, typename From>
+__global__ void __launch_bounds__(256) join_kernel(const From* from, T* to, int64_t count, int share, int width, int room) {
+    constexpr int kVec = 16 / (int)sizeof(T), kSpan = 256 * kVec;
+    pdl_wait();
+    const int64_t skew = (int64_t)(reinterpret_cast<uintptr_t>(to) % 16 / sizeof(T));
+    for (int64_t start = (int64_t)blockIdx.x * kSpan - skew; start < count; start += (int64_t)gridDim.x * kSpan) {
+        const int64_t row0 = max(start, (int64_t)0) / width;
+        const int in = (int)(start - row0 * width) + (int)threadIdx.x * kVec;    // (may begin in front of the first row)
+        const int64_t first = start + (int64_t)threadIdx.x * kVec;
+        const int row = max(in, 0) / width;
+        int col = in - row * width;
+        const From* p = from + (row0 + row) * share * room;
+        float sum[kVec] = {};
+        int at[kVec];
+        bool there[kVec], all = true;
+#pragma unroll
+        for (int e = 0, before = 0; e < kVec; ++e) {
+            there[e] = first + e >= 0 && first + e < count;
+            at[e] = there[e] ? before + col : 0;
+            all = all && there[e];
+            if (++col == width) col = 0, before += share * room;
+        }
+        const bool any = there[0] || there[kVec - 1];
+        for (int s = 0; s < (std::is_same<From, float>::value ? share : 1); ++s, p += room) {
+            float f[kVec];
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) f[e] = any ? load_element(p + at[e]) : 0.0f;
+#pragma unroll
+            for (int e = 0; e < kVec; ++e) sum[e] += f[e];
+        }
+        if (all) {
+            Pack<T, kVec> out;
+            out.set(sum);
+            out.put(to + first);
+        } else {
+#pragma unroll
+            for (int e = 0; e < kVec; ++e)
+                if (there[e]) to[first + e] = from_float<T>(sum[e]);
+        }
     }
 }
 
@@ -740,14 +833,16 @@ Split split_of(const dcn_attn* p, bool backward, bool tensor, int jobs) {
     const int64_t ct = (backward ? std::max(p->dk, p->dv) : p->dv) > 64 ? 2 : 1, chunk = tensor ? tcgen::kSteps : kChunk;
     const int64_t units = p->batch * p->heads * ct * jobs, chunks = (p->steps + chunk - 1) / chunk;
     const int64_t held = (int64_t)sm_count() * (tensor ? 1 : held_of(p->dtype == DCN_SEQ_F32, wide_of(p, backward)));
+    const int64_t sums_held = (int64_t)sm_count() * (tensor ? 1 : wide_of(p, backward) == 128 ? Shape<float, 128, true>::kHeld : Shape<float, 64, true>::kHeld);
     const double fixed = tensor ? 2 : 0.7;
+    if (!tensor && p->dtype != DCN_SEQ_F32) return {units, 1};           // (short ones)
     const int64_t full = units / held * held, rest = units - full;
     Split best = {units, 1};
     double least = (double)((rest + held - 1) / held) * (chunks + fixed);
     for (int n = 2; n <= kMostParts && n <= chunks; ++n) {
         const int64_t each = (chunks + n - 1) / n;
         if ((chunks + each - 1) / each != n) continue;
-        const double waves = (double)((rest * n + held - 1) / held), sums = (double)((rest * (n - 1) + held - 1) / held);
+        const double waves = (double)((rest * n + held - 1) / held), sums = (double)((rest * (n - 1) + sums_held - 1) / sums_held);
         const double time = waves * (each + fixed + 0.25 * (n - 1)) + sums * (0.5 * each + fixed) + 0.5 * fixed;
         if (time < least * 0.97) least = time, best = {full, n};
     }
@@ -785,8 +880,12 @@ int run_parts(const AttnArgs& a, const tcgen::Maps* maps, cudaStream_t st) {
             const int rc = a.n_parts > 1 ? launch_attn_tc<T, KA, true>(a, *maps, st) : DCN_OK;
             return rc != DCN_OK ? rc : launch_attn_tc<T, KA, false>(a, *maps, st);
         }
-    const int rc = a.n_parts > 1 ? launch_attn<T, KA, true>(a, st) : DCN_OK;
-    return rc != DCN_OK ? rc : launch_attn<T, KA, false>(a, st);
+    if constexpr (std::is_same<T, float>::value)
+        if (a.n_parts > 1) {
+            const int rc = launch_attn<T, KA, true>(a, st);
+            if (rc != DCN_OK) return rc;
+        }
+    return launch_attn<T, KA, false>(a, st);
 }
 
 template <typename T>
@@ -813,6 +912,8 @@ Operand operand(const dcn_attn* p, int map, const void* at, int64_t batch, int64
 
 struct Operands {
     Operand q, k, v, d;
+    Operand* begin() { return &q; }
+    Operand* end() { return &d + 1; }
 };
 Operands operands(const dcn_attn* p, const void* q, const void* k, const void* v, const void* dout) {
     const int share = (int)(p->heads / p->kv_heads);
@@ -822,18 +923,66 @@ Operands operands(const dcn_attn* p, const void* q, const void* k, const void* v
             operand(p, 3, dout, p->dout_batch, p->dout_step, p->heads > 1 ? p->dout_head : 0, p->dv, 1)};
 }
 
-// The tensor cores' kernel takes 16-bit rows of whole 16 bytes that do not lie on top of one another
-bool takes_tensor(const dcn_attn* p, const Operands& o, std::initializer_list<const void*> results) {
-    if (p->dtype == DCN_SEQ_F32 || p->dk % 8 != 0 || p->dv % 8 != 0 || p->steps == 0) return false;
-    for (const Operand* x : {&o.q, &o.k, &o.v, &o.d}) {
-        if (x->bytes != 16) return false;
-        if (x->p == nullptr) continue;
-        const int64_t heads = p->heads / x->share;
-        if ((p->batch > 1 && x->s.batch <= 0) || (p->steps > 1 && x->s.step <= 0) || (heads > 1 && x->s.head <= 0)) return false;
-        if (x->s.batch >= 1ll << 38 || x->s.step >= 1ll << 38 || x->s.head >= 1ll << 38) return false;
+size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
+int up8(int64_t width) { return (int)((width + 7) / 8 * 8); }
+
+// What a call does with its operands and its workspace, by its sizes, type and strides alone
+struct Plan {
+    bool tensor;                                 // the tensor cores' kernel, if the pointers allow it
+    bool pack[4];                                // operands that are laid out anew for it (q, k, v, dout)
+    bool shared;                                 // gradients of k and v are sums over heads
+    int room_k, room_v;                          // elements of a row of results dk and dv wide, as that kernel writes them
+    size_t packed[4], dq, dk, dv, bytes;         // places in the workspace (parts are at its beginning): packed operands, results
+};
+
+int64_t parts_floats(const dcn_attn* p, bool backward, bool tensor);
+
+Plan plan_of(const dcn_attn* p, bool backward) {
+    Plan w = {};
+    // Sequences of one chunk: a CTA of the other kernel begins and ends sooner, and two or three share an SM (1024 heads of 64 steps and
+    // 128 x 128 bf16: 129 us, 178 us on the tensor cores; of 128 steps: 200 and 184)
+    w.tensor = p->dtype != DCN_SEQ_F32 && p->steps > kChunk;
+    w.shared = backward && p->heads != p->kv_heads;
+    w.room_k = w.tensor ? up8(p->dk) : (int)p->dk, w.room_v = w.tensor ? up8(p->dv) : (int)p->dv;
+    size_t at = rounded((size_t)parts_floats(p, backward, false) * 4);
+    if (w.tensor) at = std::max(at, rounded((size_t)parts_floats(p, backward, true) * 4));
+    auto place = [&](size_t n) {
+        const size_t here = at;
+        at += rounded(n);
+        return here;
+    };
+    const size_t rows = (size_t)p->batch * p->steps;
+    if (w.tensor) {
+        const Operands all = operands(p, nullptr, nullptr, nullptr, nullptr);
+        const Operand* const of[4] = {&all.q, &all.k, &all.v, &all.d};
+        for (int i = 0; i < (backward ? 4 : 3); ++i) {
+            const Operand& o = *of[i];
+            const int64_t heads = p->heads / o.share, most = 1ll << 38;
+            w.pack[i] = o.bytes != 16 || (p->batch > 1 && o.s.batch <= 0) || (p->steps > 1 && o.s.step <= 0) || (heads > 1 && o.s.head <= 0) ||
+                        o.s.batch >= most || o.s.step >= most || o.s.head >= most;
+            if (w.pack[i]) w.packed[i] = place(rows * heads * up8(o.width) * 2);
+        }
     }
-    for (const void* r : results)
-        if (!aligned(r, 16)) return false;
+    // (results that are joined or that have rows of another length)
+    if (backward && w.room_k != p->dk) w.dq = place(rows * p->heads * w.room_k * 2);
+    if (backward && (w.shared || w.room_k != p->dk)) w.dk = place(rows * p->heads * w.room_k * (w.shared ? 4 : 2));
+    if (w.shared || w.room_v != p->dv) w.dv = place(rows * p->heads * w.room_v * (w.shared ? 4 : 2));
+    w.bytes = at;
+    return w;
+}
+
+// Whether the pointers allow what is planned for the tensor cores
+bool allowed(const Plan& w, const Operands& o, const dcn_attn* p, std::initializer_list<const void*> results_k, std::initializer_list<const void*> results_v,
+             const void* state, const void* workspace) {
+    if (!w.tensor || !aligned(state, 16) || !aligned(workspace, 16)) return false;
+    const Operand* const of[4] = {&o.q, &o.k, &o.v, &o.d};
+    for (int i = 0; i < 4; ++i)
+        if (!w.pack[i] && !aligned(of[i]->p, 16)) return false;
+    // (results with rows of another length, and those that heads share, go through the workspace)
+    for (const void* r : results_k)
+        if (w.room_k == p->dk && !aligned(r, 16)) return false;
+    for (const void* r : results_v)
+        if (w.room_v == p->dv && !aligned(r, 16)) return false;
     return true;
 }
 
@@ -851,9 +1000,24 @@ EncodeTiled encode_tiled() {
     return found;
 }
 
-bool make_maps(const dcn_attn* p, const Operands& o, tcgen::Maps& maps) {
+// Lays out anew what the plan says, and makes the maps
+bool prepare(const dcn_attn* p, const Plan& w, Operands& o, const int64_t* lengths, void* workspace, tcgen::Maps& maps, cudaStream_t st) {
     const EncodeTiled encode = encode_tiled();
     if (encode == nullptr) return false;
+    PackArgs args = {};
+    args.lengths = lengths, args.rows = p->batch * p->steps, args.steps = p->steps;
+    int64_t most = 0;
+    unsigned packs = 0;
+    int i = 0;
+    for (Operand& x : o) {
+        if (w.pack[i++] && x.p != nullptr) {
+            const int heads = (int)(p->heads / x.share), room = up8(x.width);
+            char* const to = static_cast<char*>(workspace) + w.packed[i - 1];
+            args.of[packs++] = {static_cast<const char*>(x.p), to, x.s.batch * 2, x.s.step * 2, x.s.head * 2, x.width, room / 8, heads};
+            most = std::max(most, args.rows * heads * (room / 8));
+            x.p = to, x.s = {p->steps * heads * room, (int64_t)heads * room, room}, x.bytes = 16;
+        }
+    }
     for (const Operand* x : {&o.q, &o.k, &o.v, &o.d}) {
         if (x->p == nullptr) continue;
         const cuuint64_t heads = (cuuint64_t)(p->heads / x->share), row = ((cuuint64_t)x->width * 2 + 15) / 16 * 16;
@@ -866,7 +1030,9 @@ bool make_maps(const dcn_attn* p, const Operands& o, tcgen::Maps& maps) {
                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return false;
     }
-    return true;
+    args.span = most > 1024 * 1024 ? 1024 : 256;
+    const unsigned ctas = (unsigned)std::min<int64_t>(most / args.span + 1, 148 * 8);
+    return packs == 0 || launch_dependent(pack_kernel, dim3(ctas, packs), dim3(256), 0, st, args) == cudaSuccess;
 }
 
 AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* lengths) {
@@ -890,20 +1056,34 @@ void add(AttnArgs& a, const Job& j, int elem) {
     a.tile_of[a.jobs] = (j.c.width + kCols - 1) / kCols;
     a.tiles = std::max(a.tiles, a.tile_of[a.jobs]);
     a.job[a.jobs] = j;
-    a.job[a.jobs].sectors = j.c.width % 16 == 0 && aligned(j.out, 32);
-    a.job[a.jobs++].pairs = j.c.width % 2 == 0 && aligned(j.out, 2 * (j.wide ? 4 : elem));
+    a.job[a.jobs].sectors = j.room % 16 == 0 && aligned(j.out, 32);
+    a.job[a.jobs++].pairs = j.room % 2 == 0 && aligned(j.out, 2 * (j.wide ? 4 : elem));
 }
 
-size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
-size_t state_elems(const dcn_attn* p) { return (size_t)p->batch * p->heads * p->dk * p->dv; }
-size_t parts_bytes(const dcn_attn* p, bool backward) {
-    int n = 1;                                   // (whichever kernel a call's pointers allow, however many gradients it wants)
-    for (int tensor = 0; tensor < 2; ++tensor)
-        for (int jobs = 1; jobs <= (backward ? 3 : 1); ++jobs) n = std::max(n, split_of(p, backward, tensor != 0, jobs).parts);
+// Floats that the parts' sums take, however many gradients a call wants
+int64_t parts_floats(const dcn_attn* p, bool backward, bool tensor) {
+    int n = 1;
+    for (int jobs = 1; jobs <= (backward ? 3 : 1); ++jobs) n = std::max(n, split_of(p, backward, tensor, jobs).parts);
     if (n <= 1) return 0;
-    if (!backward) return rounded((size_t)n * state_elems(p) * 4);
-    const size_t dk = p->dk, dv = p->dv, most = std::max(dk, dv) * dv;         // the jobs' states are dv x dk, dv x dk and dk x dv
-    return rounded(3 * (size_t)n * p->batch * p->heads * std::max(most, dk * dv) * 4);
+    const int64_t dk = tensor ? up8(p->dk) : p->dk, dv = tensor ? up8(p->dv) : p->dv;
+    // (the states are dk x dv, and in the backward pass dv x dk, dv x dk and dk x dv)
+    return (backward ? 3 : 1) * n * p->batch * p->heads * dk * dv;
+}
+
+// Results in the workspace to where they belong
+template <typename From>
+int join(const dcn_attn* p, const void* from, void* to, int64_t heads, int share, int64_t width, int room, cudaStream_t st) {
+    const int64_t count = p->batch * p->steps * heads * width, span = 256 * (16 / elem_bytes(p->dtype));
+    const dim3 grid((unsigned)std::min<int64_t>(count / span + 2, 148 * 16));      // (one more where the first 16 bytes are not whole)
+    auto go = [&](auto* type) {
+        using T = std::remove_pointer_t<decltype(type)>;
+        using F = std::conditional_t<std::is_same<From, float>::value, float, T>;
+        return launch_dependent(join_kernel<T, F>, grid, dim3(256), 0, st, static_cast<const F*>(from), static_cast<T*>(to), count, share, (int)width, room);
+    };
+    const cudaError_t e = p->dtype == DCN_SEQ_F32    ? go((float*)nullptr)
+                          : p->dtype == DCN_SEQ_BF16 ? go((__nv_bfloat16*)nullptr)
+                                                     : go((__half*)nullptr);
+    return e == cudaSuccess ? DCN_OK : DCN_ERR_CUDA;
 }
 
 bool attn_aligned(const dcn_attn* p, std::initializer_list<const void*> elems, std::initializer_list<const void*> floats) {
@@ -933,9 +1113,7 @@ using dcn::launch_dependent;
 
 extern "C" size_t dcn_attn_workspace_bytes(const dcn_attn* p, int32_t backward) {
     if (check_attn(p) != DCN_OK || p->batch == 0) return 0;
-    size_t n = parts_bytes(p, backward != 0);
-    if (backward && p->heads != p->kv_heads) n += rounded((size_t)p->batch * p->steps * p->heads * p->dk * 4) + rounded((size_t)p->batch * p->steps * p->heads * p->dv * 4);
-    return n;
+    return plan_of(p, backward != 0).bytes;
 }
 
 extern "C" int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay,
@@ -947,16 +1125,21 @@ extern "C" int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k,
     if (log_decay == nullptr || last == nullptr || (p->steps > 0 && (q == nullptr || k == nullptr || v == nullptr || out == nullptr)))
         return DCN_ERR_NULL;
     if (!attn_aligned(p, {q, k, v, out}, {log_decay, state, last}) || !aligned(lengths, 8)) return DCN_ERR_ALIGN;
-    const size_t need = dcn_attn_workspace_bytes(p, 0);
-    if (need > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
-    const Operands o = operands(p, q, k, v, nullptr);
+    const Plan w = plan_of(p, false);
+    if (w.bytes > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < w.bytes)) return DCN_ERR_WORKSPACE;
+    const cudaStream_t st = (cudaStream_t)stream;
+    Operands o = operands(p, q, k, v, nullptr);
     tcgen::Maps maps = {};
-    const bool tensor = takes_tensor(p, o, {out, last, workspace}) && make_maps(p, o, maps);
+    const bool tensor = allowed(w, o, p, {}, {out}, last, workspace);
+    if (tensor && !prepare(p, w, o, lengths, workspace, maps, st)) return DCN_ERR_CUDA;
+    const int room = tensor ? w.room_v : (int)p->dv;
+    void* const to = room != p->dv ? static_cast<char*>(workspace) + w.dv : out;
     AttnArgs a = attn_args(p, log_decay, lengths);
     a.parts = static_cast<float*>(workspace);
-    add(a, {o.q, o.k, o.v, out, state, last, (int)p->dv, 1, 0, 0, 1.0f, 1.0f}, elem_bytes(p->dtype));
+    add(a, {o.q, o.k, o.v, to, state, last, room, (int)p->dv, 1, 0, 0, 1.0f, 1.0f}, elem_bytes(p->dtype));
     share_out(a, p, false, tensor);
-    return run_attn_any(p, a, false, tensor ? &maps : nullptr, (cudaStream_t)stream);
+    const int rc = run_attn_any(p, a, false, tensor ? &maps : nullptr, st);
+    return rc != DCN_OK || to == out ? rc : join<void>(p, to, out, p->heads, 1, p->dv, room, st);
 }
 
 extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay,
@@ -967,43 +1150,41 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
     if (p->batch == 0) return DCN_OK;
     if (log_decay == nullptr || (p->steps > 0 && (q == nullptr || k == nullptr || v == nullptr))) return DCN_ERR_NULL;
     if (!attn_aligned(p, {q, k, v, dout, dq, dk, dv}, {log_decay, state, dlast, dstate}) || !aligned(lengths, 8)) return DCN_ERR_ALIGN;
-    const size_t need = dcn_attn_workspace_bytes(p, 1);
-    if (need > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < need)) return DCN_ERR_WORKSPACE;
+    const Plan w = plan_of(p, true);
+    if (w.bytes > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < w.bytes)) return DCN_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;
     if (dout == nullptr && p->steps > 0) return DCN_ERR_NULL;
-    const Operands o = operands(p, q, k, v, dout);
+    Operands o = operands(p, q, k, v, dout);
     tcgen::Maps maps = {};
-    const bool tensor = takes_tensor(p, o, {dq, dk, dv, dstate, workspace}) && make_maps(p, o, maps);
+    const bool tensor = w.shared ? allowed(w, o, p, {dq}, {}, dstate, workspace) : allowed(w, o, p, {dq, dk}, {dv}, dstate, workspace);
+    if (tensor && !prepare(p, w, o, lengths, workspace, maps, st)) return DCN_ERR_CUDA;
     AttnArgs a = attn_args(p, log_decay, lengths);
     a.parts = static_cast<float*>(workspace);
-    const bool shared = p->heads != p->kv_heads;
-    char* const wide_k = static_cast<char*>(workspace) + parts_bytes(p, true);
-    char* const wide_v = wide_k + rounded((size_t)p->batch * p->steps * p->heads * p->dk * 4);
-    const int across = (int)p->dv, elem = elem_bytes(p->dtype);
+    const int room_k = tensor ? w.room_k : (int)p->dk, room_v = tensor ? w.room_v : (int)p->dv;
+    const bool other_k = room_k != p->dk, other_v = room_v != p->dv;             // rows of another length than the results'
+    char* const at = static_cast<char*>(workspace);
+    void* const to_q = other_k ? at + w.dq : dq;
+    void* const to_k = w.shared || other_k ? at + w.dk : dk;
+    void* const to_v = w.shared || other_v ? at + w.dv : dv;
+    const int across = (int)p->dv, elem = elem_bytes(p->dtype), shared = w.shared;
     const float s = p->scale;
-    if (dq != nullptr) add(a, {o.d, o.v, o.k, dq, state, nullptr, 1, across, 0, 0, 1.0f, 1.0f}, elem);
-    if (dk != nullptr) add(a, {o.v, o.d, o.q, shared ? wide_k : dk, dlast, nullptr, 1, across, 1, shared, 1.0f / s, 1.0f}, elem);
+    if (dq != nullptr) add(a, {o.d, o.v, o.k, to_q, state, nullptr, room_k, 1, across, 0, 0, 1.0f, 1.0f}, elem);
+    if (dk != nullptr) add(a, {o.v, o.d, o.q, to_k, dlast, nullptr, room_k, 1, across, 1, shared, 1.0f / s, 1.0f}, elem);
     if (dv != nullptr || dstate != nullptr) {
         if (dv == nullptr && p->steps > 0) return DCN_ERR_NULL;
-        add(a, {o.k, o.q, o.d, shared ? wide_v : dv, dlast, dstate, across, 1, 1, shared, 1.0f / s, s}, elem);
+        add(a, {o.k, o.q, o.d, to_v, dlast, dstate, room_v, across, 1, 1, shared, 1.0f / s, s}, elem);
     }
     if (a.jobs == 0) return DCN_OK;
     share_out(a, p, true, tensor);
     int rc = run_attn_any(p, a, true, tensor ? &maps : nullptr, st);
-    if (rc != DCN_OK || !shared || p->steps == 0) return rc;
+    if (rc != DCN_OK || p->steps == 0) return rc;
     const int share = (int)(p->heads / p->kv_heads);
-    auto sum = [&](const char* from, void* to, int64_t width) {
-        const int64_t count = p->batch * p->steps * p->kv_heads * width;
-        const dim3 grid((unsigned)std::min<int64_t>((count + 255) / 256, 148 * 16));
-        cudaError_t e;
-        const float* f = reinterpret_cast<const float*>(from);
-        if (p->dtype == DCN_SEQ_F32) e = launch_dependent(shared_kernel<float>, grid, dim3(256), 0, st, f, static_cast<float*>(to), count, share, (int)width);
-        else if (p->dtype == DCN_SEQ_BF16) e = launch_dependent(shared_kernel<__nv_bfloat16>, grid, dim3(256), 0, st, f, static_cast<__nv_bfloat16*>(to), count, share, (int)width);
-        else e = launch_dependent(shared_kernel<__half>, grid, dim3(256), 0, st, f, static_cast<__half*>(to), count, share, (int)width);
-        return e == cudaSuccess ? DCN_OK : DCN_ERR_CUDA;
+    auto sum = [&](const void* from, void* to, int64_t width, int room) {
+        return w.shared ? join<float>(p, from, to, p->kv_heads, share, width, room, st) : join<void>(p, from, to, p->heads, 1, width, room, st);
     };
-    if (dk != nullptr) rc = sum(wide_k, dk, p->dk);
-    if (rc == DCN_OK && dv != nullptr) rc = sum(wide_v, dv, p->dv);
+    if (dq != nullptr && to_q != dq) rc = join<void>(p, to_q, dq, p->heads, 1, p->dk, room_k, st);
+    if (rc == DCN_OK && dk != nullptr && to_k != dk) rc = sum(to_k, dk, p->dk, room_k);
+    if (rc == DCN_OK && dv != nullptr && to_v != dv) rc = sum(to_v, dv, p->dv, room_v);
     return rc;
 }
 

@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     const int chunks = finish > begin ? (finish - begin + kSteps - 1) / kSteps : 0;
     const bool ends_here = kEnds || (length > begin && length <= begin + part_steps) || (length == 0 && part == 0);
     const bool reverse = job.reverse != 0;
-    const int extra = reverse ? 0 : 1, wa = job.a.width, wc = job.c.width;
+    const int extra = reverse ? 0 : 1, wa = job.a.width, wc = job.c.width, room = job.room;
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
@@ -263,8 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             const int w = warp & 3, r = w * 32 + lane, i = reverse ? kSteps - 1 - r : r;     // the row, and its position
             const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16);
             const float scale = args.scale, weight = table(power + 4 * (i + extra)) * scale;
-            const int64_t row_bytes = (int64_t)args.heads * wc * (wide ? 4 : 2);
-            char* const first_row = out + (((int64_t)b * steps * args.heads + h) * wc + col0) * (wide ? 4 : 2);
+            const int64_t row_bytes = (int64_t)args.heads * room * (wide ? 4 : 2);
+            char* const first_row = out + (((int64_t)b * steps * args.heads + h) * room + col0) * (wide ? 4 : 2);
             for (int n = 0; n < chunks; ++n) {
                 if (!wait(&ctl.out_full[n & 1], (n >> 1) & 1)) break;
                 __syncwarp();
@@ -286,8 +286,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     float o[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) o[k] = fmaf(__uint_as_float(p[k]), w1, __uint_as_float(q[k]) * scale);
-                    if (in && col0 + cb * 16 < wc) {             // (widths are multiples of 8)
-                        const bool both = col0 + cb * 16 + 8 < wc;
+                    if (in && col0 + cb * 16 < room) {           // (a multiple of 8)
+                        const bool both = col0 + cb * 16 + 8 < room;
                         if (wide) {
 #pragma unroll
                             for (int k = 0; k < 16; k += 4)
@@ -311,9 +311,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
             }
             // zeros behind the length
-            const int from = max(begin, length), cols = min(kDv, wc - col0) / 8;
+            const int from = max(begin, length), cols = min(kDv, room - col0) / 8;
             for (int64_t k = threadIdx.x - 256; k < (int64_t)(min(begin + part_steps, steps) - from) * cols; k += 128) {
-                const int64_t at = (((int64_t)b * steps + from + k / cols) * args.heads + h) * wc + col0 + k % cols * 8;
+                const int64_t at = (((int64_t)b * steps + from + k / cols) * args.heads + h) * room + col0 + k % cols * 8;
                 if (job.wide) {
                     float4* const d = reinterpret_cast<float4*>(static_cast<float*>(job.out) + at);
                     d[0] = d[1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -388,10 +388,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             if (part > 0 && begin < length && i < wa) {
                 const float whole = (float)exp((double)part_steps * (double)log_decay);
                 for (int s = 0; s < part; ++s) {
-                    const float* const sums = args.parts + (parts_of + s) * wa * wc + (int64_t)i * wc + col0;
+                    const float* const sums = args.parts + (parts_of + s) * wa * room + (int64_t)i * room + col0;
 #pragma unroll
                     for (int k = 0; k < kDv; k += 4)
-                        if (col0 + k < wc) {
+                        if (col0 + k < room) {
                             Pack<float, 4> p;
                             p.get(sums + k);
 #pragma unroll
@@ -463,13 +463,21 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
             }
         }
-        float* const to = kEnds ? args.parts + (parts_of + part) * wa * wc : job.end != nullptr ? job.end + (int64_t)unit * wa * wc : nullptr;
-        if (ok && ends_here && to != nullptr && mine && i < wa) {
+        const int row = kEnds ? room : wc;
+        float* const to = (kEnds ? args.parts + (parts_of + part) * wa * row : job.end != nullptr ? job.end + (int64_t)unit * wa * row : nullptr) + (int64_t)i * row + col0;
+        if (ok && ends_here && (kEnds || job.end != nullptr) && mine && i < wa) {
             const float by = kEnds ? 1.0f : job.end_scale;
 #pragma unroll
-            for (int k = 0; k < kDv; k += 4)
-                if (col0 + k < wc)
-                    *reinterpret_cast<float4*>(to + (int64_t)i * wc + col0 + k) = make_float4(by * x[k], by * x[k + 1], by * x[k + 2], by * x[k + 3]);
+            for (int k = 0; k < kDv; ++k) x[k] *= by;
+            if (row % 4 == 0) {
+#pragma unroll
+                for (int k = 0; k < kDv; k += 4)
+                    if (col0 + k < row) *reinterpret_cast<float4*>(to + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < kDv; ++k)
+                    if (col0 + k < row) to[k] = x[k];
+            }
         }
     } else if (warp == 1) {
         // ---- scores
