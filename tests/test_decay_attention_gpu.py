@@ -106,6 +106,30 @@ def test_padded_batches(t):
         assert bool(torch.isfinite(x).all()) and bool((x[behind] == 0).all()), name
 
 
+@pytest.mark.parametrize("heads,kv,dk,dv", [(4, 4, 107, 71), (4, 2, 33, 64), (3, 1, 64, 33), (2, 2, 12, 20)])
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+def test_rows_that_are_laid_out_anew(t, heads, kv, dk, dv):
+    """Odd widths, strides and places in memory, operands that are broadcast: with padding that is not read, whatever memory holds"""
+    import deform_conv3d_pytorch_op_b200 as dcn
+    q, k, v, decay, state = make(t, 5, 300, heads, kv, dk, dv, seed=dv, offset=1)
+    lengths = torch.tensor([300, 0, 129, 1, 128], device="cuda")
+    check(t, q, k, v, decay, state, lengths)
+    check(t, q, k[:1].expand(5, -1, -1, -1), v[:, :, :1].expand(-1, -1, kv, -1), decay, state, lengths)
+    want = dcn.DecayAttentionFunction.apply(q, k, v, decay, state, lengths)
+    behind = torch.arange(300, device="cuda")[None, :] >= lengths[:, None]
+    bad = [torch.where(behind[..., None, None], float("nan"), x).requires_grad_() for x in (q, k, v)]
+    trash = torch.full((1 << 24,), float("nan"), device="cuda")       # what the allocator gives next
+    del trash
+    out, last = dcn.DecayAttentionFunction.apply(*bad, decay, state, lengths)
+    assert torch.equal(out, want[0]) and torch.equal(last, want[1])
+    for x in torch.autograd.grad((out, last), bad, (torch.ones_like(out), torch.ones_like(last))):
+        assert bool(torch.isfinite(x).all()) and bool((x[behind] == 0).all())
+    # any order of axes, and steps that lie on one another's
+    turned = [x.permute(0, 3, 2, 1).contiguous().permute(0, 3, 2, 1) for x in (q, k, v)]
+    again = dcn.DecayAttentionFunction.apply(*turned, decay, state, lengths)
+    assert torch.equal(again[0], want[0]) and torch.equal(again[1], want[1])
+
+
 def test_no_state_and_single_gradients():
     import deform_conv3d_pytorch_op_b200 as dcn
     q, k, v, decay, state = make(torch.float32, 2, 90, 2, 2, 16, 24, seed=3)
