@@ -315,6 +315,13 @@ class DecayAttention(nn.Module):
         last = memory * 16.0 ** (torch.arange(heads, dtype=torch.float64) / max(heads - 1, 1))
         self.register_buffer("log_decay", torch.log1p(-1.0 / last.clamp(min=1.001)).float().to(device))
 
+    def _apply(self, fn, recurse=True):
+        decay = self.log_decay
+        super()._apply(fn, recurse)
+        if self.log_decay.dtype != torch.float32:            # decays stay float32 in modules of 16 bits
+            self.log_decay = decay.to(self.log_decay.device)
+        return self
+
     def _parts(self, input):
         h, kv, dk, dv = self.heads, self.kv_heads, self.dk, self.dv
         q, k, v = self.proj(input).split((h * dk, kv * dk, kv * dv), -1)
