@@ -31,6 +31,7 @@ struct GnormArgs {
     int64_t samples, positions, split_positions;
     int channels, groups, per_group, vectors, act, wide_weights, splits;
     int tiny;                                    // a group has one or two elements
+    int lanes;                                   // of a group, where samples are single positions (a power of two)
     float eps, inv;                              // 1 / elements of a group
 };
 
@@ -805,6 +806,180 @@ __global__ void __launch_bounds__(kThreads, 2) gnorm_sums_backward_kernel(const 
                   a.partial + (int64_t)blockIdx.x * 2 * a.groups, [&](int c) { return weight_at<T>(a.weight, c, a.wide_weights, 1.0f); });
 }
 
+// ---- single positions -----------------------------------------------------------------------------------------------------
+// Samples of one position (the heads' outputs of an attention, feature vectors) whose groups are up to 32 vectors: a few lanes of a warp
+// have a group, a vector each, and walk over samples, so that weights and their gradients' sums stay in registers; sums of a group are
+// shuffles.  No barrier, one read: bound by DRAM, and by the arithmetic of the activation.
+struct Place {
+    int lane, group, row, rows, blocks;          // blocks: of a sample's groups; rows: samples of a CTA
+    int64_t first, step;                         // samples
+    bool in;
+    __device__ __forceinline__ explicit Place(const GnormArgs& a) {
+        const int most = kThreads / a.lanes, slot = threadIdx.x / a.lanes, beside = min(a.groups, most);
+        lane = threadIdx.x % a.lanes;
+        rows = most / beside, blocks = (a.groups + most - 1) / most;
+        row = slot / beside, group = blockIdx.x % blocks * most + slot % beside;
+        first = (int64_t)(blockIdx.x / blocks) * rows, step = (int64_t)(gridDim.x / blocks) * rows;
+        in = row < rows && group < a.groups;
+    }
+};
+__device__ __forceinline__ float over_lanes(float v, int lanes) {
+    for (int o = lanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <int V>
+__device__ __forceinline__ float over_pairs(const Pairs<V>& p) {
+    Lanes s = p.v[0];
+#pragma unroll
+    for (int i = 1; i < Pairs<V>::kN; ++i) s = s + p.v[i];
+    return s.at(0) + s.at(1);
+}
+// d less its group's mean
+template <int V>
+__device__ __forceinline__ float centre(Pairs<V>& d, bool in, const GnormArgs& a) {
+    if (V == 1) d.map([](float f, int e) { return e == 0 ? f : 0.0f; });
+    if (!in) d.fill(0.0f);
+    const float mean = over_lanes(over_pairs(d), a.lanes) * a.inv;
+    const Lanes less = all_lanes(-mean);
+#pragma unroll
+    for (int i = 0; i < Pairs<V>::kN; ++i) d.v[i] = d.v[i] + less;
+    if (V == 1) d.map([](float f, int e) { return e == 0 ? f : 0.0f; });
+    if (!in) d.fill(0.0f);
+    return mean;
+}
+template <int V>
+__device__ __forceinline__ Pairs<V> add_residual(Pairs<V> z, const Pairs<V>& res) {
+#pragma unroll
+    for (int i = 0; i < Pairs<V>::kN; ++i) z.v[i] = z.v[i] + res.v[i];
+    return z;
+}
+template <typename T, int V>
+__device__ __forceinline__ void weights_of(const GnormArgs& a, int c, bool in, Pairs<V>& w, Pairs<V>& b) {
+    float f[V] = {}, g[V] = {};
+    if (in) weights_at<T, V>(a.weight, c, a.wide_weights, 1.0f, f), weights_at<T, V>(a.bias, c, a.wide_weights, 0.0f, g);
+    w.map([&](float, int e) { return f[e]; });
+    b.map([&](float, int e) { return g[e]; });
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) gnorm_rows_kernel(const GnormArgs a) {
+    pdl_wait();
+    const Place place(a);
+    const bool in = place.in && place.lane * V < a.per_group, residual = a.residual != nullptr;
+    const int c = place.group * a.per_group + place.lane * V;
+    Pairs<V> w, b;
+    weights_of<T, V>(a, c, in, w, b);
+    Pack<T, V> x, res, next, next_res;
+    next.zero(), next_res.zero();
+    auto fetch = [&](int64_t sample) {
+        if (!in || sample >= a.samples) return;
+        next.get(static_cast<const T*>(a.x) + sample * a.channels + c);
+        if (residual) next_res.get(static_cast<const T*>(a.residual) + sample * a.channels + c);
+    };
+    fetch(place.first + place.row);
+    for (int64_t start = place.first; start < a.samples; start += place.step) {
+        const int64_t sample = start + place.row;
+        const bool here = in && sample < a.samples;
+        x = next, res = next_res;
+        fetch(sample + place.step);
+        Pairs<V> d, z, more;
+        d.from(x);
+        // about the group's first element, so that a mean far from zero costs nothing
+        const float about = __shfl_sync(0xffffffffu, d.at(0), 0, a.lanes);
+        const Lanes less = all_lanes(-about);
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) d.v[i] = d.v[i] + less;
+        const float mean = about + centre(d, in, a);
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) z.v[i] = d.v[i] * d.v[i];
+        const float r = rsqrtf(fmaf(over_lanes(over_pairs(z), a.lanes), a.inv, a.eps));
+        if (!here) continue;
+        if (a.stats != nullptr && place.lane == 0) {
+            float* const to = a.stats + (sample * a.groups + place.group) * 2;
+            to[0] = mean, to[1] = r;
+        }
+        const Lanes by = all_lanes(r);
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) z.v[i] = fma(d.v[i], w.v[i] * by, b.v[i]);
+        if (residual) more.from(res), z = add_residual(z, more);
+        activate(z, a.act);
+        z.template pack<T>().put(static_cast<T*>(a.y) + sample * a.channels + c);
+    }
+}
+
+template <typename T, int V>
+__global__ void __launch_bounds__(kThreads) gnorm_rows_backward_kernel(const GnormArgs a) {
+    __shared__ float2 room[kThreads * V];
+    pdl_wait();
+    const Place place(a);
+    const bool in = place.in && place.lane * V < a.per_group, residual = a.residual != nullptr;
+    const int c = place.group * a.per_group + place.lane * V;
+    Pairs<V> w, b, s, q;
+    weights_of<T, V>(a, c, in, w, b);
+    s.fill(0.0f), q.fill(0.0f);
+    Loads<T, V> v, next;
+    next.x.zero(), next.dy.zero(), next.res.zero();
+    float mean = 0.0f, r = 0.0f, next_mean = 0.0f, next_r = 0.0f;
+    auto fetch = [&](int64_t sample) {
+        if (!in || sample >= a.samples) return;
+        next.get(a, sample * a.channels + c);
+        const float* const from = a.stats + (sample * a.groups + place.group) * 2;
+        next_mean = gload(from), next_r = gload(from + 1);
+    };
+    fetch(place.first + place.row);
+    for (int64_t start = place.first; start < a.samples; start += place.step) {
+        const int64_t sample = start + place.row;
+        const bool here = in && sample < a.samples;
+        v = next, mean = next_mean, r = next_r;
+        fetch(sample + place.step);
+        const Lanes by = all_lanes(r), less = all_lanes(-mean);
+        Pairs<V> d, z, dz, more, t, u;
+        d.from(v.x), dz.from(v.dy);
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) d.v[i] = d.v[i] + less;
+        centre(d, in, a);                        // (the mean has been rounded: in a group of nearly equal elements that would be seen)
+        if (a.act != DCN_ACT_NONE) {
+#pragma unroll
+            for (int i = 0; i < Pairs<V>::kN; ++i) z.v[i] = fma(d.v[i], w.v[i] * by, b.v[i]);
+            if (residual) more.from(v.res), z = add_residual(z, more);
+        }
+        dz = activate_gradient(z, dz, a.act);
+        if (!here) dz.fill(0.0f), d.fill(0.0f);
+        if (V == 1) dz.map([](float f, int e) { return e == 0 ? f : 0.0f; });
+#pragma unroll
+        for (int i = 0; i < Pairs<V>::kN; ++i) {
+            d.v[i] = d.v[i] * by;                // h
+            t.v[i] = dz.v[i] * w.v[i], u.v[i] = t.v[i] * d.v[i];
+            s.v[i] = s.v[i] + dz.v[i], q.v[i] = fma(dz.v[i], d.v[i], q.v[i]);
+        }
+        const Lanes s1 = all_lanes(-over_lanes(over_pairs(t), a.lanes) * a.inv), s2 = all_lanes(-over_lanes(over_pairs(u), a.lanes) * a.inv);
+        if (!here) continue;
+        if (a.dresidual != nullptr) dz.template pack<T>().put(static_cast<T*>(a.dresidual) + sample * a.channels + c);
+        if (a.dx != nullptr) {
+#pragma unroll
+            for (int i = 0; i < Pairs<V>::kN; ++i) t.v[i] = by * (t.v[i] + fma(d.v[i], s2, s1));
+            t.template pack<T>().put(static_cast<T*>(a.dx) + sample * a.channels + c);
+        }
+    }
+    if (a.dweight == nullptr && a.dbias == nullptr) return;
+    // the CTA's rows in order
+#pragma unroll
+    for (int e = 0; e < V; ++e) room[threadIdx.x * V + e] = make_float2(s.at(e), q.at(e));
+    __syncthreads();
+    if (place.row != 0 || !in) return;
+    float2* const to = reinterpret_cast<float2*>(a.channel_sums) + (int64_t)(blockIdx.x / place.blocks) * a.channels + c;
+    const int beside = min(a.groups, kThreads / a.lanes) * a.lanes;
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+        float2 sum = make_float2(0.0f, 0.0f);
+        for (int k = 0; k < place.rows; ++k) {
+            const float2 f = room[(threadIdx.x + k * beside) * V + e];
+            sum.x += f.x, sum.y += f.y;
+        }
+        to[e] = sum;
+    }
+}
+
 // dw and db of 32 channels: sums of n partial ones [n][channels][2], in a fixed order
 template <typename T>
 __device__ __forceinline__ void weight_gradients(const GnormArgs& a, int block, int64_t n, float* room) {
@@ -897,10 +1072,11 @@ int check_gnorm(const dcn_gnorm* p) {
 
 // How a call runs, by its sizes alone
 struct Plan {
-    int v;                                       // elements of a vector, if the pointers allow it
+    int v;                                       // elements of a vector
     int threads, rows, blocks, splits;
     int64_t split_positions, ctas;
-    bool held;
+    bool held, single;                           // single: samples of one position, some lanes to a group
+    int lanes;
     size_t smem, ring;                           // ring: of one tensor
 };
 
@@ -910,7 +1086,20 @@ Plan plan_of(const dcn_gnorm* p, int v, bool backward, bool residual) {
     r.v = v;
     const int vectors = c / v;
     const int64_t all = (int64_t)vectors * p->positions;
-    const int kinds = backward ? (residual ? 3 : 2) : 1;
+    const int kinds = backward ? (residual ? 3 : 2) : 1, per = c / (int)p->groups;
+    if (p->positions == 1 && per > 2) {
+        while (r.v > 1 && per % r.v != 0) r.v /= 2;
+        if (per / r.v <= 32) {
+            r.single = true, r.threads = kThreads, r.splits = 1;
+            for (r.lanes = 1; r.lanes * r.v < per; r.lanes *= 2) {}
+            const int most = kThreads / r.lanes, blocks = ((int)p->groups + most - 1) / most, rows = most / std::min((int)p->groups, most);
+            // (backward, a CTA's sums for the weights are read once more: half as many)
+            const int64_t fit = std::max<int64_t>(1, (int64_t)sm_count() * (backward ? 4 : 8) / blocks);
+            r.ctas = std::min(fit, (p->samples + rows - 1) / rows) * blocks, r.blocks = blocks;
+            return r;
+        }
+        r.v = v;
+    }
     auto lay = [&](int threads) {
         r.threads = threads;
         r.rows = vectors <= threads ? threads / vectors : 1;
@@ -968,6 +1157,7 @@ GnormArgs gnorm_args(const dcn_gnorm* p, const Plan& r) {
     a.eps = p->eps;
     a.inv = (float)(1.0 / ((double)p->positions * a.per_group));
     a.tiny = p->positions * a.per_group <= 2;
+    a.lanes = r.lanes;
     return a;
 }
 
@@ -980,6 +1170,8 @@ int launch_gnorm(K kernel, int64_t ctas, const Plan& r, size_t smem, const Gnorm
 
 template <typename T, int V>
 int forward_as(const GnormArgs& a, const Plan& r, cudaStream_t st) {
+    if (r.single)
+        return launch_dependent(gnorm_rows_kernel<T, V>, dim3((unsigned)r.ctas), dim3(kThreads), 0, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
     if (r.held) return launch_gnorm(gnorm_held_kernel<T, V>, r.ctas, r, r.smem, a, st);
     const int rc = launch_gnorm(gnorm_sums_kernel<T, V>, r.ctas, r, r.smem, a, st);
     return rc != DCN_OK ? rc : launch_gnorm(gnorm_apply_kernel<T, V>, r.ctas, r, (a.residual != nullptr ? 2 : 1) * r.ring + (2 * a.groups + 2 * r.threads) * 4, a, st);
@@ -990,13 +1182,16 @@ int backward_as(const GnormArgs& a, const Plan& r, cudaStream_t st) {
     const bool weights = a.dweight != nullptr || a.dbias != nullptr, data = a.dx != nullptr || a.dresidual != nullptr;
     const int blocks = weights ? (a.channels + 31) / 32 : 0;
     const size_t room = (a.residual != nullptr ? 3 : 2) * r.ring + 2 * r.threads * 4;
-    const int rc = r.held ? launch_gnorm(gnorm_held_backward_kernel<T, V>, r.ctas, r, r.smem, a, st)
-                          : launch_gnorm(gnorm_sums_backward_kernel<T, V>, r.ctas, r, r.smem, a, st);
-    if (rc != DCN_OK || (!weights && r.held)) return rc;
-    if (!r.held && data)
+    const bool once = r.held || r.single;
+    int rc;
+    if (r.single) rc = launch_dependent(gnorm_rows_backward_kernel<T, V>, dim3((unsigned)r.ctas), dim3(kThreads), 0, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
+    else rc = r.held ? launch_gnorm(gnorm_held_backward_kernel<T, V>, r.ctas, r, r.smem, a, st)
+                     : launch_gnorm(gnorm_sums_backward_kernel<T, V>, r.ctas, r, r.smem, a, st);
+    if (rc != DCN_OK || (!weights && once)) return rc;
+    if (!once && data)
         return launch_gnorm(gnorm_apply_backward_kernel<T, V>, blocks + r.ctas, r, 4 * a.groups * 4 + room, a, st);
     if (!weights) return DCN_OK;
-    return launch_dependent(gnorm_weights_kernel<T>, dim3(blocks), dim3(512), 2 * 512 * 4, st, a, r.held ? r.ctas : a.samples * a.splits) !=
+    return launch_dependent(gnorm_weights_kernel<T>, dim3(blocks), dim3(512), 2 * 512 * 4, st, a, r.single ? r.ctas / r.blocks : r.held ? r.ctas : a.samples * a.splits) !=
                    cudaSuccess
                ? DCN_ERR_CUDA
                : DCN_OK;
@@ -1026,7 +1221,7 @@ size_t gnorm_bytes(const dcn_gnorm* p, bool backward) {
         for (int residual = 0; residual < (backward ? 2 : 1); ++residual) {
             const Plan r = plan_of(p, v, backward, residual != 0);
             size_t n = 0;
-            if (!r.held) n = up256((size_t)r.ctas * 2 * p->groups * 4);
+            if (!r.held && !r.single) n = up256((size_t)r.ctas * 2 * p->groups * 4);
             if (backward) n += up256((size_t)r.ctas * 2 * p->channels * 4);
             most = std::max(most, n);
         }
@@ -1067,7 +1262,7 @@ extern "C" int dcn_gnorm_forward(const dcn_gnorm* p, const void* x, const void* 
     GnormArgs a = gnorm_args(p, r);
     a.x = x, a.weight = weight, a.bias = bias, a.residual = residual, a.y = y, a.stats = stats;
     a.partial = static_cast<float*>(workspace);
-    return by_type(p->dtype, vec.n, [&](auto* t, auto v) {
+    return by_type(p->dtype, r.v, [&](auto* t, auto v) {
         return forward_as<std::remove_pointer_t<decltype(t)>, decltype(v)::value>(a, r, (cudaStream_t)stream);
     });
 }
@@ -1097,7 +1292,7 @@ extern "C" int dcn_gnorm_backward(const dcn_gnorm* p, const void* x, const void*
     a.dx = dx, a.dresidual = dresidual, a.dweight = dweight, a.dbias = dbias;
     a.channel_sums = static_cast<float*>(workspace);
     a.partial = reinterpret_cast<float*>(static_cast<char*>(workspace) + up256((size_t)r.ctas * 2 * p->channels * 4));
-    return by_type(p->dtype, vec.n, [&](auto* t, auto v) {
+    return by_type(p->dtype, r.v, [&](auto* t, auto v) {
         return backward_as<std::remove_pointer_t<decltype(t)>, decltype(v)::value>(a, r, st);
     });
 }

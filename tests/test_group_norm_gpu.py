@@ -69,6 +69,36 @@ def test_forms(t, weights, residual, act):
         check(ref.TYPES[t], shape, 8, act, residual, weights, bias=residual or act is None)
 
 
+@pytest.mark.parametrize("shape,groups", [
+    ((1, 128), 32), ((3000, 128), 32), ((7, 12), 4), ((1500, 60), 20), ((300, 96), 8), ((40, 2048), 16), ((9, 8192), 512),
+    ((5, 8190), 2730), ((2001, 256), 1), ((6, 640), 2), ((3, 1050), 30), ((5000, 30), 6), ((1, 7), 1), ((2, 1040), 4)])
+@pytest.mark.parametrize("t,weights,act,residual", [("f32", "f32", "silu", True), ("bf16", "bf16", "silu", False), ("bf16", "f32", None, True),
+                                                    ("f16", "f16", "relu", False), ("f32", None, None, False)])
+def test_single_positions(t, shape, groups, weights, act, residual):
+    check(ref.TYPES[t], shape, groups, act, residual, weights, seed=shape[0])
+
+
+@pytest.mark.parametrize("t", list(ref.TYPES.values()), ids=list(ref.TYPES))
+def test_single_positions_each_by_itself(t):
+    """A sample's result owes nothing to the others: NaN, infinities and an outlier stay in their groups; odd places in memory"""
+    import deform_conv3d_pytorch_op_b200 as dcn
+    g = torch.Generator(device="cuda").manual_seed(3)
+    flat = torch.randn(601 * 48 + 1, generator=g, device="cuda").to(t)
+    x, w = flat[1:].view(601, 48), torch.randn(48, generator=g, device="cuda")
+    want = dcn.GroupNormActFunction.apply(x, 4, w, None, None, "silu")
+    # (the order of a group's sums is that of the vectors, which the place in memory decides: bits are compared at one place)
+    for y in (want, dcn.GroupNormActFunction.apply(x.clone(), 4, w, None, None, "silu")):
+        ref.close(y, more.group_norm_act(x.double(), 4, w.double(), None, None, "silu"))
+    bad = flat.clone()[1:].view(601, 48)
+    bad[5, 3], bad[600, 47], bad[77, 12] = float("nan"), float("inf"), 6e4
+    got = dcn.GroupNormActFunction.apply(bad, 4, w, None, None, "silu").view(601, 4, 12)
+    ref.close(got[77], more.group_norm_act(bad[77:78].double(), 4, w.double(), None, None, "silu").view(4, 12), "outlier")
+    assert bool(torch.isnan(got[5, 0]).all()) and bool(torch.isnan(got[600, 3]).all())
+    same = torch.ones(601, 4, dtype=torch.bool, device="cuda")
+    same[5, 0] = same[600, 3] = same[77, 1] = False
+    assert torch.equal(got[same], want.view(601, 4, 12)[same])
+
+
 @pytest.mark.parametrize("mean", [100.0, -3000.0])
 @pytest.mark.parametrize("shape", [(2, 50, 32), (2, 9000, 32)])
 def test_means_far_from_zero(shape, mean):
