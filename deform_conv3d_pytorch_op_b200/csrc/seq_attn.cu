@@ -6,11 +6,16 @@
 //     dq: (dout, v, k) with the states S^T;   back in time, with R_t = g R_{t+1} + scale q_t dout_t^T the gradient of S_t,
 //     dk: (v, dout, q) with R^T;   dv: (k, q, dout) with R;   R starts as dlast with one power of g less: g^i X and g^(64-j).
 //
-// A CTA of four warps walks one sequence's chunks for one head and 64 columns of c, the state in the accumulators of its warps (a
-// quarter of a's columns each).  A warp has 16 steps of the chunk: their scores become the operand of the product with c in
-// registers; the state meets a as a rounded copy in shared memory.  The next chunk's tiles are on their way (cp.async) meanwhile.
-// Where there are fewer heads than the GPU holds CTAs, the time axis is split: a first launch sums each part's k_t v_t^T, and
-// a CTA of the second folds what lies before its own part.
+// Two kernels run it.  16-bit sequences of more than a chunk go to the tensor cores (seq_attn_tc.cuh), laid out anew first where their rows
+// are not what a bulk copy takes (pack_kernel; results in join_kernel).  This file's own has float32, in which every operand is a sum of two
+// of TF32, and short sequences of any type: a CTA walks one sequence's chunks for one head and 64 columns of c, the state in the accumulators
+// of its warps.  Four groups of warps have 16 steps each; the warps of a group share columns, of the scores, of c and of the state, and meet
+// twice a chunk: the scores take the place of a's rows, which nobody else reads.  The state meets a as a rounded copy in shared memory.  What
+// bounds it is the latency of products and of the loads of their operands, so that warps count: 43x507x12x(80, 32) float32 674 us with one
+// group member, 374 us with four; 8x3000x2x(128, 96) float32 with gradients 1967 and 1021.  That is some 20 TFLOP/s of float32 products.
+//
+// Where there are fewer heads than the GPU holds CTAs, the time axis is split: a first launch sums each part's k_t v_t^T, and a CTA of the
+// second folds what lies before its own part.
 #include <algorithm>
 #include <cmath>
 
@@ -325,7 +330,10 @@ __device__ __forceinline__ void load_tile(uint32_t base, const Operand& o, const
 template <typename T, int KA, bool kEnds>
 struct Shape {
     static constexpr bool kFloat = sizeof(T) == 4;
-    static constexpr int kAcross = kEnds ? 2 : kFloat && KA == 128 ? 4 : kFloat || KA == 128 ? 2 : 1;      // warps that share 16 steps (rows of the state), each some of c's columns
+    // Warps of a group.  (Float32, 128 columns: 1114 us with two, 1016 with four for 8x3000x2x(128, 96) with gradients; 64 columns: two 660,
+    // one 838, four 747 for 16x1000x8x(64, 64).  16-bit, 64 columns: 341 with one, 374 with two for 7x11440x6x(54, 47), 128 columns:
+    // 1219 with one, 979 with two, 1189 with four for 16x2614x12x(107, 71), both before such sequences went to the tensor cores.)
+    static constexpr int kAcross = kEnds ? 2 : kFloat && KA == 128 ? 4 : kFloat || KA == 128 ? 2 : 1;
     static constexpr int kThreads = 128 * kAcross, kWarps = 4 * kAcross;
     static constexpr int kStages = kFloat && !kEnds && KA == 64 ? 1 : 2;
     static constexpr int kTileA = kChunk * Tile<T>::row_elems(KA) * (int)sizeof(T);
@@ -732,7 +740,8 @@ __global__ void __launch_bounds__(256) join_kernel(const From* from, T* to, int6
 }
 
 // ---- a single step --------------------------------------------------------------------------------------------------------
-// A CTA advances a head's state of one sequence, kW columns of dv a thread, rows of dk over the rest; it is read and written once.
+// A CTA advances a head's state of one sequence, kW columns of dv a thread, rows of dk over the rest; it is read and written once, which is
+// what bounds it: 256 sequences of 16 heads of 128 x 128, 537 MB in 102 us, 0.82 of a copy's rate.
 struct StepArgs {
     const void *q, *k, *v;
     Strides qs, ks, vs;
@@ -820,7 +829,7 @@ int wide_of(const dcn_attn* p, bool backward) { return (int)(backward ? std::max
 // as fill it a whole number of times have their time axis to themselves; that of the others is split.  More parts fill the GPU, and cost
 // a pass over b and c for their sums (half of a chunk's time) and the folding (a quarter of a chunk's for each part before), and each CTA
 // what it costs to begin and to end.  (5x331x6x(40, 72) float32, 30 heads: three parts instead of one.  2x16384x16x128 bf16, where
-// the backward pass has 192 units: 798 us with its gradients, 834 us when all units were whole.)
+// the backward pass has 192 units: 764 us with its gradients, 834 us when all units were whole.)
 int held_of(bool wide_type, int width) {
     if (wide_type) return width == 128 ? Shape<float, 128, false>::kHeld : Shape<float, 64, false>::kHeld;
     return width == 128 ? Shape<__half, 128, false>::kHeld : Shape<__half, 64, false>::kHeld;
@@ -1004,6 +1013,9 @@ EncodeTiled encode_tiled() {
 bool prepare(const dcn_attn* p, const Plan& w, Operands& o, const int64_t* lengths, void* workspace, tcgen::Maps& maps, cudaStream_t st) {
     const EncodeTiled encode = encode_tiled();
     if (encode == nullptr) return false;
+    // (the driver's function wants a context, which a thread that has launched nothing yet does not have: an engine's first backward pass)
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || cudaSetDevice(device) != cudaSuccess) return false;
     PackArgs args = {};
     args.lengths = lengths, args.rows = p->batch * p->steps, args.steps = p->steps;
     int64_t most = 0;

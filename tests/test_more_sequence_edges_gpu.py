@@ -1,5 +1,8 @@
 """Decayed attention, group norm and token sampling in autograd, traces, transforms, threads and modules of 16 bits."""
+import subprocess
+import sys
 import threading
+from pathlib import Path
 
 import pytest
 import torch
@@ -131,6 +134,36 @@ def test_several_host_threads():
     for t in threads:
         t.join(120)
     assert not bad
+
+
+FIRST = """
+import threading, torch
+import deform_conv3d_pytorch_op_b200 as dcn
+torch.manual_seed(0)
+q, k, v = (torch.randn(1, 300, 1, w, device="cuda").bfloat16().requires_grad_() for w in (21, 21, 115))
+decay = torch.full((1,), -0.1, device="cuda")
+
+def run():
+    out, last = dcn.DecayAttentionFunction.apply(q, k, v, decay)
+    return [out, last] + list(torch.autograd.grad((out, last), (q, k, v), (torch.ones_like(out), torch.ones_like(last))))
+
+torch.cuda.synchronize()
+got = []
+threads = [threading.Thread(target=lambda: got.append(run())) for _ in range(2)]
+for t in threads:
+    t.start()
+    t.join()
+torch.cuda.synchronize()
+want = run()
+assert len(got) == 2 and all(torch.equal(a, b) for g in got for a, b in zip(g, want))
+print("same")
+"""
+
+
+def test_first_calls_of_threads():
+    """The first thing that a thread does, and the first backward pass of a process, which autograd's own thread runs"""
+    done = subprocess.run([sys.executable, "-c", FIRST], capture_output=True, text=True, timeout=300, cwd=Path(__file__).parent.parent)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr
 
 
 @pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
