@@ -28,7 +28,7 @@ namespace dcn {
 namespace seq {
 namespace {
 
-constexpr int kChunk = 64, kCols = 64, kThreads = 128, kMostWidth = 128, kMostParts = 32;
+constexpr int kChunk = 64, kCols = 64, kMostWidth = 128, kMostParts = 32;
 
 struct Strides {
     int64_t batch, step, head;
@@ -754,24 +754,24 @@ struct StepArgs {
     float scale;
 };
 
-template <typename T, int kW>
-__global__ void __launch_bounds__(kThreads) attn_step_kernel(const StepArgs a) {
-    __shared__ float key[kMostWidth], query[kMostWidth], sums[kThreads * kW];
+template <typename T, int kW, int kT>
+__global__ void __launch_bounds__(kT) attn_step_kernel(const StepArgs a) {
+    __shared__ float key[kMostWidth], query[kMostWidth], sums[kT * kW];
     pdl_wait();
     const int h = blockIdx.x % a.heads;
     const int64_t r = blockIdx.x / a.heads;
     const int64_t slot = a.slots != nullptr ? gload_i64(a.slots + r) : r;
     T* const out = static_cast<T*>(a.out) + (r * a.heads + h) * a.dv;
     if (slot < 0 || slot >= a.pool) {
-        for (int j = threadIdx.x; j < a.dv; j += kThreads) out[j] = from_float<T>(0.0f);
+        for (int j = threadIdx.x; j < a.dv; j += kT) out[j] = from_float<T>(0.0f);
         return;
     }
-    const int groups = (a.dv + kW - 1) / kW, sets = kThreads / groups, set = threadIdx.x / groups, j = threadIdx.x % groups * kW;
+    const int groups = (a.dv + kW - 1) / kW, sets = kT / groups, set = threadIdx.x / groups, j = threadIdx.x % groups * kW;
     const T* const q = static_cast<const T*>(a.q) + r * a.qs.batch + h * a.qs.head;
     const T* const k = static_cast<const T*>(a.k) + r * a.ks.batch + h / a.share * a.ks.head;
     const T* const v = static_cast<const T*>(a.v) + r * a.vs.batch + h / a.share * a.vs.head;
     const float decay = power_of(log_decay_of(a.log_decay, h), 1);
-    for (int i = threadIdx.x; i < a.dk; i += kThreads) {
+    for (int i = threadIdx.x; i < a.dk; i += kT) {
         Pack<T, 1> p;
         p.get(k + i), key[i] = p.at(0);
         p.get(q + i), query[i] = p.at(0) * a.scale;
@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(kThreads) attn_step_kernel(const StepArgs a) {
         for (int e = 0; e < kW; ++e) sums[(set * groups + threadIdx.x % groups) * kW + e] = sum[e];
     }
     __syncthreads();
-    for (int c = threadIdx.x; c < a.dv; c += kThreads) {
+    for (int c = threadIdx.x; c < a.dv; c += kT) {
         float s = 0.0f;
         for (int p = 0; p < sets; ++p) s += sums[p * groups * kW + c];
         out[c] = from_float<T>(s);
@@ -1216,8 +1216,12 @@ extern "C" int dcn_attn_step(const dcn_attn* p, const void* q, const void* k, co
     const bool wide = p->dv % 4 == 0 && aligned(pool_state, 16);
     auto go = [&](auto* type) {
         using T = std::remove_pointer_t<decltype(type)>;
-        return wide ? launch_dependent(attn_step_kernel<T, 4>, grid, dim3(kThreads), 0, st, a)
-                    : launch_dependent(attn_step_kernel<T, 1>, grid, dim3(kThreads), 0, st, a);
+        // More threads to a head where they have one column each (200x8x(107, 71) bf16: 45.8 us with 128, 30.8 with 512) or where there are too
+        // few heads to fill the GPU (8x8x(128, 128): 8.6 and 4.5; 64x8x(128, 128), where there are enough: 10.3 and 11.1)
+        const bool few = grid.x < 2u * (unsigned)dcn::sm_count();
+        return !wide ? launch_dependent(attn_step_kernel<T, 1, 512>, grid, dim3(512), 0, st, a)
+               : few ? launch_dependent(attn_step_kernel<T, 4, 512>, grid, dim3(512), 0, st, a)
+                     : launch_dependent(attn_step_kernel<T, 4, 128>, grid, dim3(128), 0, st, a);
     };
     const cudaError_t e = p->dtype == DCN_SEQ_F32    ? go((float*)nullptr)
                           : p->dtype == DCN_SEQ_BF16 ? go((__nv_bfloat16*)nullptr)
