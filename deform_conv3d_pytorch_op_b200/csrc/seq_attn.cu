@@ -1165,7 +1165,8 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
     const Plan w = plan_of(p, true);
     if (w.bytes > 0 && (workspace == nullptr || !aligned(workspace, 4) || workspace_bytes < w.bytes)) return DCN_ERR_WORKSPACE;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (dout == nullptr && p->steps > 0) return DCN_ERR_NULL;
+    if (p->steps > 0 && (dout == nullptr || (dstate != nullptr && dv == nullptr))) return DCN_ERR_NULL;
+    if (dq == nullptr && dk == nullptr && dv == nullptr && dstate == nullptr) return DCN_OK;
     Operands o = operands(p, q, k, v, dout);
     tcgen::Maps maps = {};
     const bool tensor = w.shared ? allowed(w, o, p, {dq}, {}, dstate, workspace) : allowed(w, o, p, {dq, dk}, {dv}, dstate, workspace);
@@ -1182,11 +1183,7 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
     const float s = p->scale;
     if (dq != nullptr) add(a, {o.d, o.v, o.k, to_q, state, nullptr, room_k, 1, across, 0, 0, 1.0f, 1.0f}, elem);
     if (dk != nullptr) add(a, {o.v, o.d, o.q, to_k, dlast, nullptr, room_k, 1, across, 1, shared, 1.0f / s, 1.0f}, elem);
-    if (dv != nullptr || dstate != nullptr) {
-        if (dv == nullptr && p->steps > 0) return DCN_ERR_NULL;
-        add(a, {o.k, o.q, o.d, to_v, dlast, dstate, room_v, across, 1, 1, shared, 1.0f / s, s}, elem);
-    }
-    if (a.jobs == 0) return DCN_OK;
+    if (dv != nullptr || dstate != nullptr) add(a, {o.k, o.q, o.d, to_v, dlast, dstate, room_v, across, 1, 1, shared, 1.0f / s, s}, elem);
     share_out(a, p, true, tensor);
     int rc = run_attn_any(p, a, true, tensor ? &maps : nullptr, st);
     if (rc != DCN_OK || p->steps == 0) return rc;
