@@ -711,15 +711,14 @@ __global__ void __launch_bounds__(256) join_kernel(const From* from, T* to, int6
         const From* p = from + (row0 + row) * share * room;
         float sum[kVec] = {};
         int at[kVec];
-        bool there[kVec], all = true;
+        bool there[kVec], all = true, any = false;
 #pragma unroll
         for (int e = 0, before = 0; e < kVec; ++e) {
             there[e] = first + e >= 0 && first + e < count;
             at[e] = there[e] ? before + col : 0;
-            all = all && there[e];
+            all = all && there[e], any = any || there[e];
             if (++col == width) col = 0, before += share * room;
         }
-        const bool any = there[0] || there[kVec - 1];
         for (int s = 0; s < (std::is_same<From, float>::value ? share : 1); ++s, p += room) {
             float f[kVec];
 #pragma unroll

@@ -7,7 +7,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from tests.test_decay_attention_gpu import make
+from tests.test_decay_attention_gpu import EXTRA, STATE, make
 
 pytestmark = pytest.mark.gpu
 dcn = pytest.importorskip("deform_conv3d_pytorch_op_b200")
@@ -134,6 +134,88 @@ def test_several_host_threads():
     for t in threads:
         t.join(120)
     assert not bad
+
+
+def _between_guards(elements, dtype, offset):
+    """A buffer of bytes, and the part of it that starts `offset` elements behind 256 bytes"""
+    size = torch.empty(0, dtype=dtype).element_size()
+    raw = torch.full((512 + (elements + offset) * size + 16,), 0x5A, dtype=torch.uint8, device="cuda")
+    begin = 256 + offset * size
+    return raw, begin, begin + elements * size
+
+
+def _untouched(raw, begin, end):
+    return bool((raw[:begin] == 0x5A).all()) and bool((raw[end:] == 0x5A).all())
+
+
+@pytest.mark.parametrize("steps,heads,kv,dk,dv", [(1, 1, 1, 1, 1), (1, 2, 1, 3, 1), (3, 2, 1, 5, 7), (60, 4, 2, 16, 24), (100, 2, 2, 16, 24),
+                                                  (100, 4, 2, 33, 9), (300, 1, 1, 21, 115)])
+@pytest.mark.parametrize("offset", [0, 1, 3])
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_results_that_start_anywhere(t, offset, steps, heads, kv, dk, dv):
+    """The C calls with results in the middle of 16 bytes, between guards: right, and nothing written beside"""
+    import ctypes
+    from deform_conv3d_pytorch_op_b200 import _lib
+    from tests import more_sequence_reference as more
+    from tests import sequence_reference as ref
+    L, b = _lib.lib(), 2
+    q, k, v, decay, state = make(t, b, steps, heads, kv, dk, dv, seed=steps + dk)
+    do = randn(gen(9), b, steps, heads, dv).to(t)
+    leaves = [x.double().requires_grad_() for x in (q, k, v, state)]
+    want, end = more.decay_attention(*leaves[:3], decay.double(), leaves[3])
+    expected = torch.autograd.grad((want, end), leaves, (do.double(), torch.ones_like(end)))
+    p = _lib.dcn_attn(dtype=0 if t == torch.float32 else 1, batch=b, steps=steps, heads=heads, kv_heads=kv, dk=dk, dv=dv, scale=dk ** -0.5)
+    for n, x in (("q", q), ("k", k), ("v", v), ("dout", do)):
+        for i, a in enumerate(("batch", "step", "head")):
+            setattr(p, "%s_%s" % (n, a), x.stride(i))
+    ws = [torch.empty(max(L.dcn_attn_workspace_bytes(ctypes.byref(p), i), 16), dtype=torch.uint8, device="cuda") for i in range(2)]
+    sizes = [("out", want, t), ("last", end, torch.float32), ("dq", expected[0], t), ("dk", expected[1], t), ("dv", expected[2], t),
+             ("dstate", expected[3], torch.float32)]
+    bufs = {n: _between_guards(x.numel(), d, offset) for n, x, d in sizes}
+    at = {n: raw.data_ptr() + begin for n, (raw, begin, _) in bufs.items()}
+    stream = torch.cuda.current_stream().cuda_stream
+    ones = torch.ones_like(state)
+    assert L.dcn_attn_forward(ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), state.data_ptr(), 0, at["out"],
+                              at["last"], ws[0].data_ptr(), ws[0].numel(), stream) == 0
+    assert L.dcn_attn_backward(ctypes.byref(p), q.data_ptr(), k.data_ptr(), v.data_ptr(), decay.data_ptr(), state.data_ptr(), 0,
+                               do.data_ptr(), ones.data_ptr(), at["dq"], at["dk"], at["dv"], at["dstate"], ws[1].data_ptr(),
+                               ws[1].numel(), stream) == 0
+    torch.cuda.synchronize()
+    for n, x, d in sizes:
+        raw, begin, stop = bufs[n]
+        assert _untouched(raw, begin, stop), n
+        got = raw[begin:stop].clone().view(d).view(x.shape)
+        ref.close(got, x, n, chain=ref.CHAIN + (EXTRA[t] if d == t else STATE[t]))
+
+
+@pytest.mark.parametrize("shape,groups", [((1, 1, 3), 1), ((4, 1, 20), 4), ((3, 40, 24), 3), ((2, 3000, 40), 5)])
+@pytest.mark.parametrize("offset", [0, 1, 2])
+@pytest.mark.parametrize("t", [torch.float32, torch.float16], ids=["f32", "f16"])
+def test_norms_that_start_anywhere(t, offset, shape, groups):
+    import ctypes
+    from deform_conv3d_pytorch_op_b200 import _lib
+    from tests import more_sequence_reference as more
+    from tests import sequence_reference as ref
+    L, g, c = _lib.lib(), gen(sum(shape)), shape[-1]
+    x, dy, w = randn(g, *shape).to(t), randn(g, *shape).to(t), randn(g, c)
+    wx, ww = x.double().requires_grad_(), w.double().requires_grad_()
+    want = more.group_norm_act(wx, groups, ww, None, None, "silu")
+    dx, dw = torch.autograd.grad(want, (wx, ww), dy.double())
+    p = _lib.dcn_gnorm(dtype=0 if t == torch.float32 else 2, weight_dtype=0, act=2, samples=shape[0], positions=shape[1], channels=c, groups=groups, eps=1e-5)
+    ws = [torch.empty(max(L.dcn_gnorm_workspace_bytes(ctypes.byref(p), i), 16), dtype=torch.uint8, device="cuda") for i in range(2)]
+    sizes = [("y", want, t), ("stats", torch.empty(shape[0] * groups * 2), torch.float32), ("dx", dx, t), ("dw", dw, torch.float32)]
+    bufs = {n: _between_guards(v.numel(), d, offset) for n, v, d in sizes}
+    at = {n: raw.data_ptr() + begin for n, (raw, begin, _) in bufs.items()}
+    stream = torch.cuda.current_stream().cuda_stream
+    assert L.dcn_gnorm_forward(ctypes.byref(p), x.data_ptr(), w.data_ptr(), 0, 0, at["y"], at["stats"], ws[0].data_ptr(), ws[0].numel(), stream) == 0
+    assert L.dcn_gnorm_backward(ctypes.byref(p), x.data_ptr(), w.data_ptr(), 0, 0, at["stats"], dy.data_ptr(), at["dx"], at["dw"], 0, 0,
+                                ws[1].data_ptr(), ws[1].numel(), stream) == 0
+    torch.cuda.synchronize()
+    for n, v, d in sizes:
+        raw, begin, stop = bufs[n]
+        assert _untouched(raw, begin, stop), n
+        if n != "stats":
+            ref.close(raw[begin:stop].clone().view(d).view(v.shape), v, n, scale=(x.numel() / c) ** 0.5 if n == "dw" else 1.0)
 
 
 FIRST = """
