@@ -309,6 +309,9 @@ class DecayAttention(nn.Module):
     def __init__(self, features, heads, dk, dv=None, kv_heads=None, memory=8.0, device=None, dtype=None):
         super().__init__()
         dv, kv_heads = dk if dv is None else dv, heads if kv_heads is None else kv_heads
+        if not (1 <= dk <= 128 and 1 <= dv <= 128) or heads < 1 or kv_heads < 1 or heads % kv_heads:
+            raise _lib.DcnError("%d heads of %d and %d elements and %d of keys: 1 to 128 elements, and heads that the keys' divide"
+                                % (heads, dk, dv, kv_heads))
         self.features, self.heads, self.kv_heads, self.dk, self.dv = features, heads, kv_heads, dk, dv
         self.proj = nn.Linear(features, heads * dk + kv_heads * (dk + dv), device=device, dtype=dtype)
         self.norm = GroupNormAct(heads, heads * dv, "silu", dim=-1, device=device, dtype=dtype)

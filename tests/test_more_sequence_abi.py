@@ -119,3 +119,11 @@ def test_modules_hold_their_parameters_and_refuse_the_cpu():
             f()
     with pytest.raises(dcn.DcnError, match="activation"):
         dcn.GroupNormActFunction.apply(torch.zeros(4, 20), 4, None, None, None, "gelu")
+
+
+def test_attention_modules_that_are_refused():
+    for kw in (dict(heads=2, dk=129), dict(heads=2, dk=8, dv=0), dict(heads=4, dk=8, kv_heads=3), dict(heads=0, dk=8)):
+        with pytest.raises(dcn.DcnError, match="heads"):
+            dcn.DecayAttention(16, **kw)
+    block = dcn.DecayAttention(16, 4, 8, 12, kv_heads=2)
+    assert block.proj.out_features == 4 * 8 + 2 * (8 + 12) and tuple(block.new_states(3).shape) == (3, 4, 8, 12)
