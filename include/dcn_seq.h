@@ -148,7 +148,8 @@ typedef struct dcn_attn {
     float scale;                                /* finite, not 0 */
 } dcn_attn;
 
-/* Scratch bytes of dcn_attn_forward (backward = 0) and dcn_attn_backward (backward = 1) on the current device; may be 0. */
+/* Scratch bytes of dcn_attn_forward (backward = 0) and dcn_attn_backward (backward = 1) on the current device; may be 0.  Scratch and
+ * tensors that start on 16 bytes let 16-bit calls of more than 64 steps take their faster kernel. */
 size_t dcn_attn_workspace_bytes(const dcn_attn* p, int32_t backward);
 
 /* out [batch, steps, heads, dv] (dense) and last [batch, heads, dk, dv] (float32): the state after the last step.  log_decay float32
