@@ -39,6 +39,7 @@ struct GnormArgs {
     int channels, groups, per_group, vectors, act, wide_weights, splits;
     int tiny;                                    // a group has one or two elements
     int lanes;                                   // of a group, where samples are single positions (a power of two)
+    int beside;                                  // channels that a block of weight_gradients has
     float eps, inv;                              // 1 / elements of a group
 };
 
@@ -987,12 +988,12 @@ __global__ void __launch_bounds__(kThreads) gnorm_rows_backward_kernel(const Gno
     }
 }
 
-// dw and db of 32 channels: sums of n partial ones [n][channels][2], in a fixed order
+// dw and db of a.beside channels (a power of two up to 32): sums of n partial ones [n][channels][2], in a fixed order
 template <typename T>
 __device__ __forceinline__ void weight_gradients(const GnormArgs& a, int block, int64_t n, float* room) {
-    const int rows = blockDim.x / 32, lane = threadIdx.x % 32, row = threadIdx.x / 32, c = block * 32 + lane;
+    const int rows = blockDim.x / a.beside, col = threadIdx.x % a.beside, row = threadIdx.x / a.beside, c = block * a.beside + col;
     Lanes sum = all_lanes(0.0f);
-    if (c < a.channels && row < rows) {
+    if (c < a.channels) {
 #pragma unroll 8
         for (int64_t i = row; i < n; i += rows) {
             Pack<float, 2> p;
@@ -1001,11 +1002,14 @@ __device__ __forceinline__ void weight_gradients(const GnormArgs& a, int block, 
             sum = sum + lanes(f);
         }
     }
-    room[2 * threadIdx.x] = sum.at(0), room[2 * threadIdx.x + 1] = sum.at(1);
+    float s = sum.at(0), q = sum.at(1);
+    for (int o = a.beside; o < 32; o *= 2) s += __shfl_xor_sync(0xffffffffu, s, o), q += __shfl_xor_sync(0xffffffffu, q, o);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    if (lane < a.beside) room[2 * (warp * a.beside + lane)] = s, room[2 * (warp * a.beside + lane) + 1] = q;
     __syncthreads();
     if (row != 0 || c >= a.channels) return;
-    float s = 0.0f, q = 0.0f;
-    for (int k = 0; k < rows; ++k) s += room[2 * (k * 32 + lane)], q += room[2 * (k * 32 + lane) + 1];
+    s = q = 0.0f;
+    for (int k = 0; k < (int)blockDim.x / 32; ++k) s += room[2 * (k * a.beside + col)], q += room[2 * (k * a.beside + col) + 1];
     auto put = [&](void* p, float v) {
         if (p == nullptr) return;
         if (a.wide_weights) static_cast<float*>(p)[c] = v;
@@ -1021,7 +1025,7 @@ __global__ void __launch_bounds__(kThreads, 2) gnorm_apply_backward_kernel(const
     float* const stats = reinterpret_cast<float*>(smem + (a.residual != nullptr ? 3 : 2) * ring.kKind);
     float* const sums = stats + 2 * a.groups;
     const Grid grid(a.vectors);
-    const int first = a.dweight != nullptr || a.dbias != nullptr ? (a.channels + 31) / 32 : 0;      // blocks for these
+    const int first = a.dweight != nullptr || a.dbias != nullptr ? (a.channels + a.beside - 1) / a.beside : 0;      // blocks for these
     pdl_wait();
     if ((int)blockIdx.x < first) {
         weight_gradients<T>(a, blockIdx.x, a.samples * a.splits, stats);
@@ -1165,6 +1169,10 @@ GnormArgs gnorm_args(const dcn_gnorm* p, const Plan& r) {
     a.inv = (float)(1.0 / ((double)p->positions * a.per_group));
     a.tiny = p->positions * a.per_group <= 2;
     a.lanes = r.lanes;
+    // Few channels: more threads to each.  (8x50176x64: the second pass 34 us with two blocks of 32 before it, 26 with eight of 8; but
+    // 6x1183x256: 6.8 with eight of 32, 9.3 with 32 of 8.  Alone, 592 sums of 128 channels: 11.6 us with 32, 5.4 with 8.)
+    a.beside = 8;
+    while (a.beside < 32 && a.channels > (r.held || r.single ? 64 : 8) * a.beside) a.beside *= 2;
     return a;
 }
 
@@ -1187,7 +1195,7 @@ int forward_as(const GnormArgs& a, const Plan& r, cudaStream_t st) {
 template <typename T, int V>
 int backward_as(const GnormArgs& a, const Plan& r, cudaStream_t st) {
     const bool weights = a.dweight != nullptr || a.dbias != nullptr, data = a.dx != nullptr || a.dresidual != nullptr;
-    const int blocks = weights ? (a.channels + 31) / 32 : 0;
+    const int blocks = weights ? (a.channels + a.beside - 1) / a.beside : 0;
     const size_t room = (a.residual != nullptr ? 3 : 2) * r.ring + 2 * r.threads * 4;
     const bool once = r.held || r.single;
     int rc;
