@@ -14,7 +14,7 @@
 //
 // Rows of a tile are steps in the order of time.  Back in time, position i of a chunk is row 127 - i, and triangle and weights are mirrored.
 //
-// 2x16384x16x128 bf16 with its gradients takes 750 us (its bytes alone 168, its products, some 450 GFLOP, 270).  A chunk takes about 2.5 us:
+// 2x16384x16x128 bf16 with its gradients takes 750 us (850 over seconds of it; its bytes alone 168, its products, some 450 GFLOP, 270).  A chunk takes about 2.5 us:
 // products some 1.2 us at the measured rate, the rest is the chain scores - P - O2 with its two ways through tensor memory, which one CTA an SM (shared
 // memory) overlaps with the next chunk's scores only, and shared memory's bandwidth, of which operands, C' and X take about half.  What
 // moved it most: code of the roles in short loops instead of unrolled (1356 to 1168 us: together they did not stay in the instruction

@@ -11,11 +11,11 @@
 // (`held`): CTAs walk over samples.  Larger ones take two passes, the second of which finds in L2 what the first has left there; it runs from
 // the end backwards.  Both passes have the next eight vectors of a thread on their way to its own places in shared memory (`Ring`), and
 // arithmetic in packed pairs, since loads in registers and single instructions bounded them (8x50176x64 bf16 with gradients: 103 us before,
-// 86 after; 1816 with a first version).
+// 86 after, 78 with the weights' sums spread out; 1816 with a first version).
 //
-// Kernels' times: 8x50176x64 by 32 bf16, 51 MB a tensor: 15.6 + 15.0 us forward (floor 16.0), 24.2 + 34.0 backward (23.9): DRAM, and in the
-// second backward pass issue slots.  6x1183x256 by 32 float32: 4.9 + 5.9 + 6.3 + 6.8 us, latency of few loads a thread.  Single positions,
-// 18498x128 by 32 float32: 7.0 and 8.7 us (2.9 and 4.4) and 11.6 for the weights' sums; 30000x512 by 8 bf16 with SiLU 22.5 (9.5).
+// Kernels' times: 8x50176x64 by 32 bf16, 51 MB a tensor: 15.7 + 15.1 us forward (floor 16.0), 24.0 + 25.9 backward (23.9): DRAM and issue
+// slots, either at some 60 %.  6x1183x256 by 32 float32: 4.8 + 6.1 + 6.3 + 7.0 us, latency of few loads a thread.  Single positions,
+// 18498x128 by 32 float32: 6.9 and 8.7 us (2.9 and 4.4) and 5.4 for the weights' sums; 30000x512 by 8 bf16 with SiLU 22.5 (9.5).
 #include <algorithm>
 
 #include "seq_common.cuh"
