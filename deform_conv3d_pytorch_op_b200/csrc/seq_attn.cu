@@ -53,13 +53,13 @@ struct Job {
     float init_scale, end_scale;
     int pairs;                                   // out's rows start on two elements
     int sectors;                                 // ... and on 32 bytes, which all columns fill
+    float* parts;                                // [batch * heads][part][a.width][room], this job's own
 };
 
 struct AttnArgs {
     Job job[3];
     const float* log_decay;
     const int64_t* lengths;
-    float* parts;                                // [job][batch * heads][part][a.width][room]
     int64_t steps, part_steps;
     int64_t whole;                               // units (job, head, tile) whose time axis is not split
     int batch, heads, jobs, tiles, n_parts;      // tiles: of 64 columns, the most that a job has
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
 
     // the state before this part
     float x[kM][kN][4];
-    const int64_t parts_of = ((int64_t)which * args.batch * args.heads + unit) * args.n_parts;
+    const int64_t parts_of = (int64_t)unit * args.n_parts;
 #pragma unroll
     for (int m = 0; m < kM; ++m)
 #pragma unroll
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
     if constexpr (!kEnds) {
         const float whole = power_of(log_decay, place.part_steps);
         for (int s = 0; s < part; ++s) {
-            const float* const sums = args.parts + (parts_of + s) * wa * wc;
+            const float* const sums = job.parts + (parts_of + s) * wa * wc;
             // (a part that the sequence ends in is the last one that anything reads)
 #pragma unroll
             for (int m = 0; m < kM; ++m)
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
 
     // (the first part ends a sequence of no steps)
     const bool ends_here = kEnds || (length > begin && length <= begin + place.part_steps) || (length == 0 && part == 0);
-    float* const to = kEnds ? args.parts + (parts_of + part) * wa * wc : job.end != nullptr ? job.end + (int64_t)unit * wa * wc : nullptr;
+    float* const to = kEnds ? job.parts + (parts_of + part) * wa * wc : job.end != nullptr ? job.end + (int64_t)unit * wa * wc : nullptr;
     if (ends_here && to != nullptr) {
         const float by = kEnds ? 1.0f : job.end_scale;
 #pragma unroll
@@ -1055,12 +1055,18 @@ AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* len
     return a;
 }
 
-// (once the jobs are there)
-void share_out(AttnArgs& a, const dcn_attn* p, bool backward, bool tensor) {
+// (once the jobs are there.)  Each job's parts begin behind those of the job before it: a part has as many elements as that job's states,
+// which with rows of a multiple of 8 are not as many in every job (dv x dk and dk x dv)
+void share_out(AttnArgs& a, const dcn_attn* p, bool backward, bool tensor, void* workspace) {
     const Split split = split_of(p, backward, tensor, a.jobs);
     const int64_t chunk = tensor ? tcgen::kSteps : kChunk, chunks = (p->steps + chunk - 1) / chunk;
     a.n_parts = split.parts, a.whole = split.whole;
     a.part_steps = std::max<int64_t>(1, (chunks + a.n_parts - 1) / a.n_parts) * chunk;
+    float* at = static_cast<float*>(workspace);
+    for (int j = 0; j < a.jobs && a.n_parts > 1; ++j) {
+        a.job[j].parts = at;
+        at += p->batch * p->heads * a.n_parts * a.job[j].a.width * a.job[j].room;
+    }
 }
 
 void add(AttnArgs& a, const Job& j, int elem) {
@@ -1076,9 +1082,9 @@ int64_t parts_floats(const dcn_attn* p, bool backward, bool tensor) {
     int n = 1;
     for (int jobs = 1; jobs <= (backward ? 3 : 1); ++jobs) n = std::max(n, split_of(p, backward, tensor, jobs).parts);
     if (n <= 1) return 0;
-    const int64_t dk = tensor ? up8(p->dk) : p->dk, dv = tensor ? up8(p->dv) : p->dv;
+    const int64_t row_k = tensor ? up8(p->dk) : p->dk, row_v = tensor ? up8(p->dv) : p->dv;
     // (the states are dk x dv, and in the backward pass dv x dk, dv x dk and dk x dv)
-    return (backward ? 3 : 1) * n * p->batch * p->heads * dk * dv;
+    return n * p->batch * p->heads * (p->dk * row_v + (backward ? 2 * p->dv * row_k : 0));
 }
 
 // Results in the workspace to where they belong
@@ -1146,9 +1152,8 @@ extern "C" int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k,
     const int room = tensor ? w.room_v : (int)p->dv;
     void* const to = room != p->dv ? static_cast<char*>(workspace) + w.dv : out;
     AttnArgs a = attn_args(p, log_decay, lengths);
-    a.parts = static_cast<float*>(workspace);
     add(a, {o.q, o.k, o.v, to, state, last, room, (int)p->dv, 1, 0, 0, 1.0f, 1.0f}, elem_bytes(p->dtype));
-    share_out(a, p, false, tensor);
+    share_out(a, p, false, tensor, workspace);
     const int rc = run_attn_any(p, a, false, tensor ? &maps : nullptr, st);
     return rc != DCN_OK || to == out ? rc : join<void>(p, to, out, p->heads, 1, p->dv, room, st);
 }
@@ -1171,7 +1176,6 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
     const bool tensor = w.shared ? allowed(w, o, p, {dq}, {}, dstate, workspace) : allowed(w, o, p, {dq, dk}, {dv}, dstate, workspace);
     if (tensor && !prepare(p, w, o, lengths, workspace, maps, st)) return DCN_ERR_CUDA;
     AttnArgs a = attn_args(p, log_decay, lengths);
-    a.parts = static_cast<float*>(workspace);
     const int room_k = tensor ? w.room_k : (int)p->dk, room_v = tensor ? w.room_v : (int)p->dv;
     const bool other_k = room_k != p->dk, other_v = room_v != p->dv;             // rows of another length than the results'
     char* const at = static_cast<char*>(workspace);
@@ -1183,7 +1187,7 @@ extern "C" int dcn_attn_backward(const dcn_attn* p, const void* q, const void* k
     if (dq != nullptr) add(a, {o.d, o.v, o.k, to_q, state, nullptr, room_k, 1, across, 0, 0, 1.0f, 1.0f}, elem);
     if (dk != nullptr) add(a, {o.v, o.d, o.q, to_k, dlast, nullptr, room_k, 1, across, 1, shared, 1.0f / s, 1.0f}, elem);
     if (dv != nullptr || dstate != nullptr) add(a, {o.k, o.q, o.d, to_v, dlast, dstate, room_v, across, 1, 1, shared, 1.0f / s, s}, elem);
-    share_out(a, p, true, tensor);
+    share_out(a, p, true, tensor, workspace);
     int rc = run_attn_any(p, a, true, tensor ? &maps : nullptr, st);
     if (rc != DCN_OK || p->steps == 0) return rc;
     const int share = (int)(p->heads / p->kv_heads);

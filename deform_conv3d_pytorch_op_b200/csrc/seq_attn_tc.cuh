@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = ctl.tmem, power = tc::smem_u32(ctl.power);
-    const int64_t parts_of = ((int64_t)which * args.batch * args.heads + unit) * args.n_parts;
+    const int64_t parts_of = (int64_t)unit * args.n_parts;
     // Tiles that C' is the sum of: all where the state is a result and the chunk so near its end that two would be seen in it (those
     // before it count e^-1.5 and less), else two
     const auto parts_of_chunk = [&](int n) {
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             if (part > 0 && begin < length && i < wa) {
                 const float whole = (float)exp((double)part_steps * (double)log_decay);
                 for (int s = 0; s < part; ++s) {
-                    const float* const sums = args.parts + (parts_of + s) * wa * room + (int64_t)i * room + col0;
+                    const float* const sums = job.parts + (parts_of + s) * wa * room + (int64_t)i * room + col0;
 #pragma unroll
                     for (int k = 0; k < kDv; k += 4)
                         if (col0 + k < room) {
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             }
         }
         const int row = kEnds ? room : wc;
-        float* const to = (kEnds ? args.parts + (parts_of + part) * wa * row : job.end != nullptr ? job.end + (int64_t)unit * wa * row : nullptr) + (int64_t)i * row + col0;
+        float* const to = (kEnds ? job.parts + (parts_of + part) * wa * row : job.end != nullptr ? job.end + (int64_t)unit * wa * row : nullptr) + (int64_t)i * row + col0;
         if (ok && ends_here && (kEnds || job.end != nullptr) && mine && i < wa) {
             const float by = kEnds ? 1.0f : job.end_scale;
 #pragma unroll

@@ -92,3 +92,13 @@ def sample(logits, uniform, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         tokens.append(i)
         logprobs.append(math.log(int(w[r, i])) - math.log(int(mass[-1])))
     return torch.tensor(tokens, device=logits.device), torch.tensor(logprobs, device=logits.device, dtype=torch.float64)
+
+
+def decay_attention_blocks(q, k, v, log_decay, state=None, lengths=None, scale=None, block=512):
+    """decay_attention for long sequences: block by block, each from the state that the one before has left."""
+    lengths = torch.full((q.size(0),), q.size(1), device=q.device) if lengths is None else lengths.clamp(0, q.size(1))
+    out = []
+    for t in range(0, q.size(1), block):
+        o, state = decay_attention(q[:, t:t + block], k[:, t:t + block], v[:, t:t + block], log_decay, state, lengths - t, scale)
+        out.append(o)
+    return torch.cat(out, 1), state
