@@ -29,6 +29,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 2048, kMostCluster
 constexpr float kUnit = 1099511627776.0f;        // 2^40
 constexpr float kBinsPerArgument = 73.0f;        // 2048 / 28: exp(-28) < 2^-40
 constexpr int64_t kMostVocab = 1 << 20;
+static_assert(kMostVocab <= (int64_t)kBins * kShort && kShort <= kThreads, "a bucket of indices has a thread for each");
 
 struct SampleArgs {
     const void* logits;
@@ -864,9 +865,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
         own = s.shared_a[team.turn ^ 1][rank];
         if (target < before || target >= before + own) return;
         // The token among this CTA's: by buckets of indices, then inside of one
-        const int base = max(rank * kWarps * each * Row<T>::kV - row.skew, 0), span = kWarps * each * Row<T>::kV;
-        int shift = 0;
-        while (span >> shift >= kBins) ++shift;
+        const int base = max(rank * kWarps * each * Row<T>::kV - row.skew, 0), span = min(kWarps * each * Row<T>::kV, a.vocab - base);
+        int shift = 0;                           // (up to 9: indices lie below 2^20, whatever a warp's whole vectors add up to)
+        while ((span - 1) >> shift >= kBins) ++shift;
         clear(s);
 #pragma unroll
         for (int j = 0; j < Listed::kEach; ++j)
@@ -890,8 +891,8 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
 #pragma unroll
         for (int j = 0; j < Listed::kEach; ++j)
             if (index[j] != 0x7fffffff && mine.weight[j] != 0 && (index[j] - base) >> shift == bucket) {
-                const uint32_t at = atomicAdd(&s.narrowed, 1u);          // (a bucket has at most 2^20 / 2048 indices)
-                s.narrow[at] = (unsigned long long)(index[j] - base) << 41 | mine.weight[j];
+                const uint32_t at = atomicAdd(&s.narrowed, 1u);          // (a bucket has 2^20 / 2048 indices at most, which fit)
+                if (at < kShort) s.narrow[at] = (unsigned long long)(index[j] - base) << 41 | mine.weight[j];
             }
         __syncthreads();
         constexpr unsigned long long kWeight = (1ull << 41) - 1;

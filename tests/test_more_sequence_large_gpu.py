@@ -68,3 +68,23 @@ def test_tokens():
     want, score = more.sample(logits[-3:], uniform[-3:], 0.9, 50, 0.9, 0.0)
     assert torch.equal(token[-3:], want)
     ref.close(logprob[-3:], score)
+
+
+@pytest.mark.parametrize("vocab,skew", [(1 << 20, 0), (1 << 20, 3), ((1 << 20) - 100, 5), ((1 << 20) - 127, 1), ((1 << 20) - 4000, 0)])
+def test_neighbouring_tokens_of_the_largest_vocabularies(vocab, skew):
+    """So many rows that a CTA has one, and a thousand likely tokens side by side, where a CTA looks for the token among neighbours"""
+    n, likely = 160, 1000
+    g = torch.Generator(device="cuda").manual_seed(vocab + skew)
+    logits = torch.full((n * (vocab + 8) + skew,), -60.0, device="cuda", dtype=torch.bfloat16)[skew:].view(n, vocab + 8)[:, :vocab]
+    begins = torch.randint(0, vocab - likely, (n,), generator=g, device="cuda")
+    begins[:4] = torch.tensor([0, vocab - likely, 1024, 512], device="cuda")
+    places = begins[:, None] + torch.arange(likely, device="cuda")
+    close = (torch.randn(n, likely, generator=g, device="cuda") * 0.3).bfloat16()
+    logits.scatter_(1, places, close)
+    uniform = torch.rand(n, generator=g, device="cuda")
+    for settings in ((1.0, 0, 0.99, 0.0), (1.0, 900, 1.0, 0.0), (0.9, 700, 0.95, 0.0), (1.0, 0, 0.7, 0.0)):
+        token, logprob = dcn.TokenSampleFunction.apply(logits, uniform, *settings)
+        # (the others' weights are below 2^-40 of the largest: 0)
+        want, score = more.sample(close, uniform, *settings)
+        assert torch.equal(token, begins + want), settings
+        ref.close(logprob, score)
