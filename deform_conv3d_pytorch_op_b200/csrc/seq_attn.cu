@@ -837,9 +837,9 @@ struct Split {
     int64_t whole;
     int parts;
 };
-Split split_of(const dcn_attn* p, bool backward, bool tensor, int jobs) {
-    const int64_t ct = (backward ? std::max(p->dk, p->dv) : p->dv) > 64 ? 2 : 1, chunk = tensor ? tcgen::kSteps : kChunk;
-    const int64_t units = p->batch * p->heads * ct * jobs, chunks = (p->steps + chunk - 1) / chunk;
+Split split_of(const dcn_attn* p, bool backward, bool tensor, int jobs, int tiles) {
+    const int64_t chunk = tensor ? tcgen::kSteps : kChunk;
+    const int64_t units = p->batch * p->heads * tiles * jobs, chunks = (p->steps + chunk - 1) / chunk;
     const int64_t held = (int64_t)sm_count() * (tensor ? 1 : held_of(p->dtype == DCN_SEQ_F32, wide_of(p, backward)));
     const int64_t sums_held = (int64_t)sm_count() * (tensor ? 1 : wide_of(p, backward) == 128 ? Shape<float, 128, true>::kHeld : Shape<float, 64, true>::kHeld);
     const double fixed = tensor ? 2 : 0.7;
@@ -1058,7 +1058,7 @@ AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* len
 // (once the jobs are there.)  Each job's parts begin behind those of the job before it: a part has as many elements as that job's states,
 // which with rows of a multiple of 8 are not as many in every job (dv x dk and dk x dv)
 void share_out(AttnArgs& a, const dcn_attn* p, bool backward, bool tensor, void* workspace) {
-    const Split split = split_of(p, backward, tensor, a.jobs);
+    const Split split = split_of(p, backward, tensor, a.jobs, a.tiles);
     const int64_t chunk = tensor ? tcgen::kSteps : kChunk, chunks = (p->steps + chunk - 1) / chunk;
     a.n_parts = split.parts, a.whole = split.whole;
     a.part_steps = std::max<int64_t>(1, (chunks + a.n_parts - 1) / a.n_parts) * chunk;
@@ -1077,10 +1077,11 @@ void add(AttnArgs& a, const Job& j, int elem) {
     a.job[a.jobs++].pairs = j.room % 2 == 0 && aligned(j.out, 2 * (j.wide ? 4 : elem));
 }
 
-// Floats that the parts' sums take, however many gradients a call wants
+// Floats that the parts' sums take, whichever gradients a call wants: their number, and the columns of the widest, decide the split
 int64_t parts_floats(const dcn_attn* p, bool backward, bool tensor) {
     int n = 1;
-    for (int jobs = 1; jobs <= (backward ? 3 : 1); ++jobs) n = std::max(n, split_of(p, backward, tensor, jobs).parts);
+    for (int jobs = 1; jobs <= (backward ? 3 : 1); ++jobs)
+        for (int tiles = 1; tiles <= 2; ++tiles) n = std::max(n, split_of(p, backward, tensor, jobs, tiles).parts);
     if (n <= 1) return 0;
     const int64_t row_k = tensor ? up8(p->dk) : p->dk, row_v = tensor ? up8(p->dv) : p->dv;
     // (the states are dk x dv, and in the backward pass dv x dk, dv x dk and dk x dv)

@@ -52,3 +52,22 @@ def test_parts_of_each_gradient(t, batch, steps, heads, dk, dv):
 def test_parts_of_each_gradient_in_float32(dk, dv):
     q, k, v, decay, state = make(torch.float32, 1, 2050, 4, 2, dk, dv, seed=dk)
     check(torch.float32, (q, k, v, state), decay, torch.tensor([2000], device="cuda"))
+
+
+@pytest.mark.parametrize("t,batch,steps,heads,dk,dv", [
+    (torch.float32, 16, 331, 5, 40, 72), (torch.float32, 16, 777, 6, 128, 64), (torch.float32, 30, 400, 5, 33, 65),
+    (torch.bfloat16, 6, 2100, 16, 64, 128), (torch.bfloat16, 6, 2100, 16, 128, 64), (torch.float16, 10, 1500, 10, 121, 50),
+    (torch.bfloat16, 25, 1200, 6, 24, 104)])
+def test_some_gradients_alone(t, batch, steps, heads, dk, dv):
+    """Gradients whose own columns are 64 or fewer where the other width is more: as many heads as fill the GPU only with the wider one"""
+    q, k, v, decay, state = make(t, batch, steps, heads, heads, dk, dv, seed=steps)
+    g = torch.Generator(device="cuda").manual_seed(2)
+    dout = torch.randn(batch, steps, heads, dv, generator=g, device="cuda").to(t)
+    dlast = torch.randn(state.shape, generator=g, device="cuda")
+    wide = [x.detach().double().requires_grad_() for x in (q, k, v, state)]
+    want, end = more.decay_attention_blocks(*wide[:3], decay.double(), wide[3])
+    expected = dict(zip(NAMES, torch.autograd.grad((want, end), wide, (dout.double(), dlast.double()))))
+    for asked in (("q",), ("k",), ("q", "k"), ("v",), ("state",), ("v", "state"), ("k", "v"), NAMES):
+        got = results((q, k, v, state), decay, None, dout, dlast, asked)[2:]
+        for name, a in zip(asked, got):
+            ref.close(a, expected[name], (asked, name), chain=ref.CHAIN + (STATE if name == "state" else EXTRA)[t])
