@@ -47,19 +47,20 @@ struct Job {
     void* out;                                   // [batch, steps, heads, room], dense; float32 where wide
     const float* init;                           // [batch, heads, ...]: element (i, j) at i * init_i + j * init_j; NULL: zeros
     float* end;                                  // [batch, heads, a.width, c.width] dense, or NULL
-    int room;                                    // elements of a row of out and of the parts: c's width, or the next multiple of 8
+    int room;                                    // elements of a row of out: c's width, or the next multiple of 8
     int init_i, init_j;
     int reverse, wide;
     float init_scale, end_scale;
     int pairs;                                   // out's rows start on two elements
     int sectors;                                 // ... and on 32 bytes, which all columns fill
-    float* parts;                                // [batch * heads][part][a.width][room], this job's own
 };
 
 struct AttnArgs {
     Job job[3];
     const float* log_decay;
     const int64_t* lengths;
+    float* parts;                                // [unit less `whole`][part][part_floats]: sums [a.width][part_cols] of a unit's 64 columns
+    int part_floats, part_cols;
     int64_t steps, part_steps;
     int64_t whole;                               // units (job, head, tile) whose time axis is not split
     int batch, heads, jobs, tiles, n_parts;      // tiles: of 64 columns, the most that a job has
@@ -70,20 +71,21 @@ struct AttnArgs {
 // Which unit and which part of its time axis a CTA has.  kEnds: of those parts alone that another one follows
 struct Place {
     int tile, which, unit, part;
-    int64_t part_steps;
+    int64_t part_steps, split;                   // split: the unit among those that are split
     template <bool kEnds>
     static __device__ __forceinline__ Place of(const AttnArgs& a) {
         Place p;
-        const int64_t split = (int64_t)blockIdx.x - (kEnds ? 0 : a.whole);
+        const int64_t at = (int64_t)blockIdx.x - (kEnds ? 0 : a.whole);
         const int parts = kEnds ? a.n_parts - 1 : a.n_parts;
         int64_t u = blockIdx.x;
-        p.part = 0, p.part_steps = a.steps;
-        if (split >= 0) u = a.whole + split / parts, p.part = (int)(split % parts), p.part_steps = a.part_steps;
+        p.part = 0, p.part_steps = a.steps, p.split = 0;
+        if (at >= 0) p.split = at / parts, u = a.whole + p.split, p.part = (int)(at % parts), p.part_steps = a.part_steps;
         p.tile = (int)(u % a.tiles);
         u /= a.tiles;
         p.which = (int)(u % a.jobs), p.unit = (int)(u / a.jobs);
         return p;
     }
+    __device__ __forceinline__ float* sums(const AttnArgs& a, int s) const { return a.parts + (split * a.n_parts + s) * a.part_floats; }
 };
 
 __device__ __forceinline__ double log_decay_of(const float* log_decay, int h) {
@@ -407,7 +409,6 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
 
     // the state before this part
     float x[kM][kN][4];
-    const int64_t parts_of = (int64_t)unit * args.n_parts;
 #pragma unroll
     for (int m = 0; m < kM; ++m)
 #pragma unroll
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
     if constexpr (!kEnds) {
         const float whole = power_of(log_decay, place.part_steps);
         for (int s = 0; s < part; ++s) {
-            const float* const sums = job.parts + (parts_of + s) * wa * wc;
+            const float* const sums = place.sums(args, s);
             // (a part that the sequence ends in is the last one that anything reads)
 #pragma unroll
             for (int m = 0; m < kM; ++m)
@@ -433,7 +434,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + col_of(n) + 2 * t + (e & 1);
-                        if (i < wa && j < wc && begin < length) x[m][n][e] = fmaf(x[m][n][e], whole, gload(sums + (int64_t)i * wc + j));
+                        if (i < wa && j < wc && begin < length) x[m][n][e] = fmaf(x[m][n][e], whole, gload(sums + i * args.part_cols + j - col0));
                     }
         }
     }
@@ -608,7 +609,8 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
 
     // (the first part ends a sequence of no steps)
     const bool ends_here = kEnds || (length > begin && length <= begin + place.part_steps) || (length == 0 && part == 0);
-    float* const to = kEnds ? job.parts + (parts_of + part) * wa * wc : job.end != nullptr ? job.end + (int64_t)unit * wa * wc : nullptr;
+    float* const to = kEnds ? place.sums(args, part) - col0 : job.end != nullptr ? job.end + (int64_t)unit * wa * wc : nullptr;
+    const int row = kEnds ? args.part_cols : wc;
     if (ends_here && to != nullptr) {
         const float by = kEnds ? 1.0f : job.end_scale;
 #pragma unroll
@@ -618,7 +620,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const int i = (m * 4 + warp) * 16 + g + (e >> 1) * 8, j = col0 + col_of(n) + 2 * t + (e & 1);
-                    if (i < wa && j < wc) to[(int64_t)i * wc + j] = by * x[m][n][e];
+                    if (i < wa && j < wc) to[(int64_t)i * row + j] = by * x[m][n][e];
                 }
     }
     if constexpr (!kEnds) {
@@ -1055,18 +1057,24 @@ AttnArgs attn_args(const dcn_attn* p, const float* log_decay, const int64_t* len
     return a;
 }
 
-// (once the jobs are there.)  Each job's parts begin behind those of the job before it: a part has as many elements as that job's states,
-// which with rows of a multiple of 8 are not as many in every job (dv x dk and dk x dv)
+// Parts' sums are kept of the units that are split alone, of 64 columns each: the most that any job has.  (Of every unit, a batch of
+// thousands of heads would need gigabytes for the few that do not fill the GPU.)
+struct PartSize {
+    int rows, cols;
+};
+PartSize part_of(const dcn_attn* p, bool backward, bool tensor) {
+    const int row_k = (int)(tensor ? up8(p->dk) : p->dk), row_v = (int)(tensor ? up8(p->dv) : p->dv);
+    return {(int)(backward ? std::max(p->dk, p->dv) : p->dk), std::min(kCols, backward ? std::max(row_k, row_v) : row_v)};
+}
+
+// (once the jobs are there)
 void share_out(AttnArgs& a, const dcn_attn* p, bool backward, bool tensor, void* workspace) {
     const Split split = split_of(p, backward, tensor, a.jobs, a.tiles);
     const int64_t chunk = tensor ? tcgen::kSteps : kChunk, chunks = (p->steps + chunk - 1) / chunk;
+    const PartSize size = part_of(p, backward, tensor);
     a.n_parts = split.parts, a.whole = split.whole;
     a.part_steps = std::max<int64_t>(1, (chunks + a.n_parts - 1) / a.n_parts) * chunk;
-    float* at = static_cast<float*>(workspace);
-    for (int j = 0; j < a.jobs && a.n_parts > 1; ++j) {
-        a.job[j].parts = at;
-        at += p->batch * p->heads * a.n_parts * a.job[j].a.width * a.job[j].room;
-    }
+    a.parts = static_cast<float*>(workspace), a.part_cols = size.cols, a.part_floats = size.rows * size.cols;
 }
 
 void add(AttnArgs& a, const Job& j, int elem) {
@@ -1079,13 +1087,14 @@ void add(AttnArgs& a, const Job& j, int elem) {
 
 // Floats that the parts' sums take, whichever gradients a call wants: their number, and the columns of the widest, decide the split
 int64_t parts_floats(const dcn_attn* p, bool backward, bool tensor) {
-    int n = 1;
+    int64_t most = 0;
     for (int jobs = 1; jobs <= (backward ? 3 : 1); ++jobs)
-        for (int tiles = 1; tiles <= 2; ++tiles) n = std::max(n, split_of(p, backward, tensor, jobs, tiles).parts);
-    if (n <= 1) return 0;
-    const int64_t row_k = tensor ? up8(p->dk) : p->dk, row_v = tensor ? up8(p->dv) : p->dv;
-    // (the states are dk x dv, and in the backward pass dv x dk, dv x dk and dk x dv)
-    return n * p->batch * p->heads * (p->dk * row_v + (backward ? 2 * p->dv * row_k : 0));
+        for (int tiles = 1; tiles <= 2; ++tiles) {
+            const Split split = split_of(p, backward, tensor, jobs, tiles);
+            if (split.parts > 1) most = std::max(most, (p->batch * p->heads * jobs * tiles - split.whole) * split.parts);
+        }
+    const PartSize size = part_of(p, backward, tensor);
+    return most * size.rows * size.cols;
 }
 
 // Results in the workspace to where they belong

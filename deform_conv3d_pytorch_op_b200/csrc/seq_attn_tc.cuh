@@ -180,7 +180,6 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
     __syncthreads();
     tc::tc_fence_after();
     const uint32_t tmem = ctl.tmem, power = tc::smem_u32(ctl.power);
-    const int64_t parts_of = (int64_t)unit * args.n_parts;
     // Tiles that C' is the sum of: all where the state is a result and the chunk so near its end that two would be seen in it (those
     // before it count e^-1.5 and less), else two
     const auto parts_of_chunk = [&](int n) {
@@ -394,10 +393,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             if (part > 0 && begin < length && i < wa) {
                 const float whole = (float)exp((double)part_steps * (double)log_decay);
                 for (int s = 0; s < part; ++s) {
-                    const float* const sums = job.parts + (parts_of + s) * wa * room + (int64_t)i * room + col0;
+                    const float* const sums = place.sums(args, s) + i * args.part_cols;
 #pragma unroll
                     for (int k = 0; k < kDv; k += 4)
-                        if (col0 + k < room) {
+                        if (col0 + k < room) {           // (the parts' rows are multiples of 8, and reach as far as any job's)
                             Pack<float, 4> p;
                             p.get(sums + k);
 #pragma unroll
@@ -469,8 +468,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
             }
         }
-        const int row = kEnds ? room : wc;
-        float* const to = (kEnds ? job.parts + (parts_of + part) * wa * row : job.end != nullptr ? job.end + (int64_t)unit * wa * row : nullptr) + (int64_t)i * row + col0;
+        const int row = kEnds ? args.part_cols : wc, cols = kEnds ? room : wc;
+        float* const to = (kEnds ? place.sums(args, part) : job.end != nullptr ? job.end + (int64_t)unit * wa * wc + col0 : nullptr) + (int64_t)i * row;
         if (ok && ends_here && (kEnds || job.end != nullptr) && mine && i < wa) {
             const float by = kEnds ? 1.0f : job.end_scale;
 #pragma unroll
@@ -478,11 +477,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             if (row % 4 == 0) {
 #pragma unroll
                 for (int k = 0; k < kDv; k += 4)
-                    if (col0 + k < row) *reinterpret_cast<float4*>(to + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+                    if (col0 + k < cols) *reinterpret_cast<float4*>(to + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
             } else {
 #pragma unroll
                 for (int k = 0; k < kDv; ++k)
-                    if (col0 + k < row) to[k] = x[k];
+                    if (col0 + k < cols) to[k] = x[k];
             }
         }
     } else if (warp == 1) {

@@ -127,3 +127,17 @@ def test_attention_modules_that_are_refused():
             dcn.DecayAttention(16, **kw)
     block = dcn.DecayAttention(16, 4, 8, 12, kv_heads=2)
     assert block.proj.out_features == 4 * 8 + 2 * (8 + 12) and tuple(block.new_states(3).shape) == (3, 4, 8, 12)
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_attention_keeps_the_parts_of_split_heads_alone(L, dtype):
+    """Heads that do not fill the GPU a whole number of times are split in time, into 32 parts at most: the parts' sums of those few, 64
+    columns each, are all that a call without other scratch needs, however many heads there are"""
+    for heads in (1, 5, 150, 2962, 5930, 65535):
+        for dk, dv in ((128, 128), (64, 128), (128, 8), (16, 24)):
+            strides = {n + a: w for n, d in (("q", dk), ("k", dk), ("v", dv), ("dout", dv))
+                       for a, w in (("_batch", 16384 * heads * d), ("_step", heads * d), ("_head", d))}
+            p = _attn(dtype=dtype, batch=1, steps=16384, heads=heads, kv_heads=heads, dk=dk, dv=dv, **strides)
+            most = 2 * 160 * 32 * max(dk, dv) * 64 * 4         # (two CTAs an SM or fewer, on a GPU of up to 160)
+            for backward in (0, 1):
+                assert L.dcn_attn_workspace_bytes(ctypes.byref(p), backward) <= most, (heads, dk, dv, backward)
