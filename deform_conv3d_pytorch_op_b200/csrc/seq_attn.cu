@@ -103,6 +103,25 @@ __device__ __forceinline__ float power(uint32_t table, int n) {
     return f;
 }
 
+// Float16 has 11 bits of what lies between 2^-14 and 2^16 alone, and the scores, states and weighted rows that it takes part in do not stay there
+// (128 products of numbers above 22, gradients of a loss that is not scaled).  So what is rounded to it is brought near its upper end first, by
+// a power of two that the largest of a row of scores, of a head's state or of a block's rows gives, and back in float32.  From 2^14 on,
+// elements down to 2^-29 of that largest one keep their 11 bits.  (Bfloat16 has float32's range.)
+template <typename T>
+constexpr bool kNarrow = std::is_same<T, __half>::value;
+// n, where 2^n brings a largest magnitude (0 and above, not NaN) into [2^14, 2^15), as far as 2^n and 2^-n are normal numbers
+__device__ __forceinline__ int shift_of(float most) { return most > 0.0f ? min(max(14 + 127 - (int)(__float_as_uint(most) >> 23), -113), 100) : 0; }
+__device__ __forceinline__ float two_to(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
+// The larger magnitude of finite numbers, as bits above 2^23 (0: none yet); infinities and NaN, which become negative, are left out: columns
+// that do not meet them are not to be lost beside them
+__device__ __forceinline__ uint32_t larger_finite(uint32_t most, float v) {
+    return (uint32_t)__viaddmax_s32((int)(__float_as_uint(v) & 0x7fffffffu), 0x00800000, (int)most);
+}
+__device__ __forceinline__ float magnitude(uint32_t most) { return most > 0x00800000u ? __uint_as_float(most - 0x00800000u) : 0.0f; }
+// the same of pairs of float16 numbers, whose shift is up alone: they are in range
+__device__ __forceinline__ uint32_t larger_pairs(uint32_t most, uint32_t pair) { return __viaddmax_s16x2(pair & 0x7fff7fffu, 0x04000400u, most); }
+__device__ __forceinline__ int shift_up(uint32_t most) { return most > 0x400u ? max(shift_of(half_of<__half>(most - 0x400u, 0)), 0) : 0; }
+
 #include "seq_attn_tc.cuh"
 
 // ---- products: D[16 x 8] += A[16 x k] B[k x 8], k = 16 for 16-bit types and 8 for float32 -----------------------------------------
@@ -244,10 +263,18 @@ __device__ __forceinline__ void load_bt(FragB<T> (&f)[2], uint32_t base, int k0,
         f[0].v[0] = r[0], f[0].v[1] = r[1], f[1].v[0] = r[2], f[1].v[1] = r[3];
     }
 }
-// A[m][k] = tile[k0 + k][m0 + m] * weight of row k0 + k.  16-bit: rounded, what the rounding left (low), and what that one's left (last)
+// The largest magnitudes of what load_at reads in rows m0 + g and m0 + g + 8 of A, as shift_up takes them: float16
+__device__ __forceinline__ void largest_at(uint32_t (&most)[2], uint32_t base, int k0, int m0, int cols, int lane) {
+    uint32_t r[4];
+    ldsm4t(r, Tile<__half>::at(base, k0 + (lane >> 4) * 8 + (lane & 7), m0 + ((lane >> 3) & 1) * 8, cols));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most[i & 1] = larger_pairs(most[i & 1], r[i]);
+}
+// A[m][k] = tile[k0 + k][m0 + m] * weight of row k0 + k.  16-bit: rounded, what the rounding left (low), and what that one's left (last);
+// float16: times `by` of rows g and g + 8
 template <typename T>
 __device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, FragA<T>& last, uint32_t base, int k0, int m0, int cols, int lane, uint32_t table,
-                                        int last_power, int rows) {
+                                        int last_power, int rows, const float (&by)[2]) {
     const int g = lane >> 2, t = lane & 3;
     if constexpr (std::is_same<T, float>::value) {
 #pragma unroll
@@ -269,7 +296,8 @@ __device__ __forceinline__ void load_at(FragA<T>& f, FragA<T>& low, FragA<T>& la
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {            // 0: (g, k 2t), 1: (g + 8, k 2t), 2: (g, k 2t + 8), 3: (g + 8, k 2t + 8)
-            const float x = half_of<T>(r[i], 0) * w[(i >> 1) * 2], y = half_of<T>(r[i], 1) * w[(i >> 1) * 2 + 1];
+            float x = half_of<T>(r[i], 0) * w[(i >> 1) * 2], y = half_of<T>(r[i], 1) * w[(i >> 1) * 2 + 1];
+            if constexpr (kNarrow<T>) x *= by[i & 1], y *= by[i & 1];
             f.v[i] = word_of<T>(x, y);
             const float p = x - half_of<T>(f.v[i], 0), q = y - half_of<T>(f.v[i], 1);
             low.v[i] = word_of<T>(p, q);
@@ -343,20 +371,20 @@ struct Shape {
     static constexpr int kState = kEnds ? 0 : KA * Tile<T>::row_elems(kCols) * (int)sizeof(T);
     static constexpr int kB = kEnds ? 0 : kTileA, kC = kB + kTileA, kStage = kC + kTileC;                // b's and c's places
     static constexpr int kTable = kStages * kStage + kState;             // g^n, 0 to 64
-    static constexpr int kBytes = kTable + (kChunk + 1) * 4 + kWarps * 4;
+    static constexpr int kLargest = kTable + (kChunk + 1) * 4 + kWarps * 4;                  // of rows of scores, float16
+    static constexpr int kBytes = kLargest + (kNarrow<T> && !kEnds ? kAcross * kChunk * 4 : 0);
     static constexpr int kHeld = kEnds ? (kFloat && KA == 128 ? 2 : 3) : kFloat && KA == 128 ? 1 : kFloat || KA == 128 ? 2 : 3;           // CTAs that an SM has room for
 };
 
-// The maximum of a CTA's states, for the power of two that keeps a float16 copy of them in range
+// The maximum of a CTA's states, for the power of two of their float16 copy
 template <int kWarps>
-__device__ __forceinline__ float cta_max(float v, float* slots) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+__device__ __forceinline__ uint32_t cta_max(uint32_t v, uint32_t* slots) {
+    v = __reduce_max_sync(0xffffffffu, v);
     if ((threadIdx.x & 31) == 0) slots[threadIdx.x >> 5] = v;
     __syncthreads();
     v = slots[0];
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) v = fmaxf(v, slots[w]);
+    for (int w = 1; w < kWarps; ++w) v = max(v, slots[w]);
     return v;
 }
 
@@ -371,7 +399,8 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
     extern __shared__ __align__(128) char smem[];
     const uint32_t tiles = shared_address(smem), copy = tiles + S::kStages * S::kStage;
     float* const powers = reinterpret_cast<float*>(smem + S::kTable);
-    float* const slots = powers + kChunk + 1;
+    uint32_t* const slots = reinterpret_cast<uint32_t*>(powers + kChunk + 1);
+    float* const largest = reinterpret_cast<float*>(smem + S::kLargest);         // [side][row]
     const uint32_t table = shared_address(powers);
     const int warp = (threadIdx.x >> 5) & 3, side = threadIdx.x >> 7, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     auto col_of = [side](int n) { return ((n >> 1) * kAcross + side) * 16 + (n & 1) * 8; };              // where a warp's n-th tile lies
@@ -439,20 +468,18 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
         }
     }
 
-    float down = 1.0f, up = 1.0f;                // float16: the copy is the state times `down`
+    float by = 1.0f, back = 1.0f;                // float16: the copy is the state times `by`
     auto put_copy = [&]() {
-        if constexpr (std::is_same<T, __half>::value) {
-            float most = 0.0f;
+        if constexpr (kNarrow<T>) {
+            uint32_t most = 0;
 #pragma unroll
             for (int m = 0; m < kM; ++m)
 #pragma unroll
                 for (int n = 0; n < kN; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[m][n][e]));
-            most = cta_max<S::kWarps>(most, slots);
-            const int over = max((int)(__float_as_uint(most) >> 23) - 127 - 14, 0);
-            down = __uint_as_float((uint32_t)(127 - min(over, 126)) << 23);
-            up = __uint_as_float((uint32_t)(127 + min(over, 126)) << 23);
+                    for (int e = 0; e < 4; ++e) most = larger_finite(most, x[m][n][e]);
+            const int shift = shift_of(magnitude(cta_max<S::kWarps>(most, slots)));
+            by = two_to(shift), back = two_to(-shift);
         }
 #pragma unroll
         for (int m = 0; m < kM; ++m)
@@ -460,8 +487,8 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
             for (int n = 0; n < kN; ++n)
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
-                    put_pair<T>(L::at(copy, (m * 4 + warp) * 16 + g + half * 8, col_of(n) + 2 * t, kCols), x[m][n][2 * half] * down,
-                                x[m][n][2 * half + 1] * down);
+                    put_pair<T>(L::at(copy, (m * 4 + warp) * 16 + g + half * 8, col_of(n) + 2 * t, kCols), x[m][n][2 * half] * by,
+                                x[m][n][2 * half + 1] * by);
     };
     if constexpr (!kEnds) put_copy();
 
@@ -499,26 +526,54 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
                         }
                     }
                 }
-                const float w0 = power(table, m0 + g + extra) * up, w1 = power(table, m0 + g + 8 + extra) * up;
+                const float w0 = power(table, m0 + g + extra) * back, w1 = power(table, m0 + g + 8 + extra) * back;
 #pragma unroll
                 for (int n = 0; n < kN; ++n) o[n][0] *= w0, o[n][1] *= w0, o[n][2] *= w1, o[n][3] *= w1;
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int d = m0 + g + (e >> 1) * 8 - (col_of(n) + 2 * t + (e & 1));
+                        s[n][e] = d >= 0 ? s[n][e] * power(table, max(d, 0)) : 0.0f;
+                    }
+                float score_by[2] = {1.0f, 1.0f}, score_back[2] = {1.0f, 1.0f};
+                if constexpr (kNarrow<T>) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float most = 0.0f;
+#pragma unroll
+                        for (int n = 0; n < kN; ++n) most = fmaxf(fmaxf(most, fabsf(s[n][2 * half])), fabsf(s[n][2 * half + 1]));
+                        most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1)), most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                        score_by[half] = most;
+                        if (kAcross > 1 && t == 0) largest[side * kChunk + m0 + g + half * 8] = most;
+                    }
+                }
                 // the scores take the place of these 16 steps of a, which these warps alone have read
                 group_sync<32 * kAcross>(1 + warp);
+                if constexpr (kNarrow<T>) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        for (int k = 0; kAcross > 1 && k < kAcross; ++k) score_by[half] = fmaxf(score_by[half], largest[k * kChunk + m0 + g + half * 8]);
+                        const int shift = shift_of(score_by[half]);
+                        score_by[half] = two_to(shift), score_back[half] = two_to(-shift);
+                    }
+                }
 #pragma unroll
                 for (int n = 0; n < kN; ++n)
                     if (col_of(n & ~1) <= m0) {
 #pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            float p[2];
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int d = m0 + g + half * 8 - (col_of(n) + 2 * t + e);
-                                p[e] = d >= 0 ? s[n][2 * half + e] * power(table, max(d, 0)) : 0.0f;
-                            }
-                            put_pair<T>(L::at(at, m0 + g + half * 8, col_of(n) + 2 * t, KA), p[0], p[1]);
-                        }
+                        for (int half = 0; half < 2; ++half)
+                            put_pair<T>(L::at(at, m0 + g + half * 8, col_of(n) + 2 * t, KA), s[n][2 * half] * score_by[half], s[n][2 * half + 1] * score_by[half]);
                     }
                 group_sync<32 * kAcross>(1 + warp);
+                // (float16: apart from the state's part, whose power of two is another)
+                if constexpr (kNarrow<T>) {
+#pragma unroll
+                    for (int n = 0; n < kN; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+                }
+                float (&product)[kN][4] = kNarrow<T> ? s : o;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
                     if (k * L::kK > m0 + 15 || k * L::kK >= rows) continue;
@@ -529,9 +584,15 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
                         if (col_of(n) >= c_end) continue;
                         FragB<T> fb[2];
                         load_bt<T>(fb, ct, k * L::kK, col_of(n), kCols, lane);
-                        mma<T>(o[n], fa, fb[0]);
-                        mma<T>(o[n + 1], fa, fb[1]);
+                        mma<T>(product[n], fa, fb[0]);
+                        mma<T>(product[n + 1], fa, fb[1]);
                     }
+                }
+                if constexpr (kNarrow<T>) {
+#pragma unroll
+                    for (int n = 0; n < kN; ++n)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[n][e] = fmaf(s[n][e], score_back[e >> 1], o[n][e]);
                 }
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
@@ -569,34 +630,72 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
         // the state behind this chunk
         const float whole = power(table, rows);
         const int last_power = rows - extra;
-#pragma unroll
-        for (int m = 0; m < kM; ++m)
-#pragma unroll
-            for (int n = 0; n < kN; ++n)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) x[m][n][e] *= whole;
-#pragma unroll 1
-        for (int k = 0; k < rows; k += L::kK) {
-            FragB<T> fb[kN / 2][2];
-#pragma unroll
-            for (int n = 0; n < kN; n += 2)
-                if (col_of(n) < c_end) load_bt<T>(fb[n / 2], ct, k, col_of(n), kCols, lane);
+        if constexpr (kNarrow<T>) {
+            // (the sum of a chunk by itself: its power of two would take a large state out of float32)
 #pragma unroll
             for (int m = 0; m < kM; ++m) {
-                if ((m * 4 + warp) * 16 >= wa) continue;
-                FragA<T> fa, low, lowest;
-                load_at<T>(fa, low, lowest, bt, k, (m * 4 + warp) * 16, KA, lane, table, last_power, rows);
+                const int i0 = (m * 4 + warp) * 16;
+                if (i0 >= wa) continue;
+                uint32_t most[2] = {};
+                for (int k = 0; k < rows; k += L::kK) largest_at(most, bt, k, i0, KA, lane);
+                float row_by[2], row_back[2], sum[kN][4] = {};
 #pragma unroll
-                for (int n = 0; n < kN; n += 2) {
-                    if (col_of(n) >= c_end) continue;
-                    mma<T>(x[m][n], fa, fb[n / 2][0]);
-                    mma<T>(x[m][n + 1], fa, fb[n / 2][1]);
-                    if constexpr (!std::is_same<T, float>::value) {
-                        mma<T>(x[m][n], low, fb[n / 2][0]);
-                        mma<T>(x[m][n + 1], low, fb[n / 2][1]);
-                        if (std::is_same<T, __nv_bfloat16>::value && exact) {
-                            mma<T>(x[m][n], lowest, fb[n / 2][0]);
-                            mma<T>(x[m][n + 1], lowest, fb[n / 2][1]);
+                for (int half = 0; half < 2; ++half) {
+                    most[half] = __vmaxu2(most[half], __shfl_xor_sync(0xffffffffu, most[half], 1));
+                    most[half] = __vmaxu2(most[half], __shfl_xor_sync(0xffffffffu, most[half], 2));
+                    const int shift = shift_up(max(most[half] & 0xffffu, most[half] >> 16));
+                    row_by[half] = two_to(shift), row_back[half] = two_to(-shift);
+                }
+#pragma unroll 1
+                for (int k = 0; k < rows; k += L::kK) {
+                    FragA<T> fa, low, lowest;
+                    load_at<T>(fa, low, lowest, bt, k, i0, KA, lane, table, last_power, rows, row_by);
+#pragma unroll
+                    for (int n = 0; n < kN; n += 2) {
+                        if (col_of(n) >= c_end) continue;
+                        FragB<T> fb[2];
+                        load_bt<T>(fb, ct, k, col_of(n), kCols, lane);
+                        mma<T>(sum[n], fa, fb[0]);
+                        mma<T>(sum[n + 1], fa, fb[1]);
+                        mma<T>(sum[n], low, fb[0]);
+                        mma<T>(sum[n + 1], low, fb[1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[m][n][e] = fmaf(x[m][n][e], whole, sum[n][e] * row_back[e >> 1]);
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < kM; ++m)
+#pragma unroll
+                for (int n = 0; n < kN; ++n)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[m][n][e] *= whole;
+#pragma unroll 1
+            for (int k = 0; k < rows; k += L::kK) {
+                FragB<T> fb[kN / 2][2];
+#pragma unroll
+                for (int n = 0; n < kN; n += 2)
+                    if (col_of(n) < c_end) load_bt<T>(fb[n / 2], ct, k, col_of(n), kCols, lane);
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+                    if ((m * 4 + warp) * 16 >= wa) continue;
+                    FragA<T> fa, low, lowest;
+                    load_at<T>(fa, low, lowest, bt, k, (m * 4 + warp) * 16, KA, lane, table, last_power, rows, {1.0f, 1.0f});
+#pragma unroll
+                    for (int n = 0; n < kN; n += 2) {
+                        if (col_of(n) >= c_end) continue;
+                        mma<T>(x[m][n], fa, fb[n / 2][0]);
+                        mma<T>(x[m][n + 1], fa, fb[n / 2][1]);
+                        if constexpr (!std::is_same<T, float>::value) {
+                            mma<T>(x[m][n], low, fb[n / 2][0]);
+                            mma<T>(x[m][n + 1], low, fb[n / 2][1]);
+                            if (exact) {
+                                mma<T>(x[m][n], lowest, fb[n / 2][0]);
+                                mma<T>(x[m][n + 1], lowest, fb[n / 2][1]);
+                            }
                         }
                     }
                 }

@@ -5,14 +5,20 @@
 //     O1     = A X,  O2 = P C         128 x 64                     out = scale (g^(i+1) O1 + O2)
 //     U      = B^T C', C'_j = g^(127-j) c_j                        X'  = g^128 X + U
 // C' is a sum of 16-bit tiles, so many that what the state is made of is exact to 2^-17 (two of bfloat16) where it only meets A, and to
-// float32's own 2^-24 (three) where it is a result; two of float16 are exact to 2^-22.  X is in the registers of four warps in float32, and
-// meets A as a rounded copy in shared memory.
+// float32's own 2^-24 (three) where it is a result, in its last 1.5 decays; two of float16, brought up by a power of two that c's largest
+// element gives, are exact to 2^-22, or 2^-40 of that element where this is more.  X is in the registers of four warps in float32, and meets A
+// as a copy in shared memory that is rounded to the type, as P is: the products take both operands in one type, tensor memory (P) and shared
+// memory (X) are full, and a second 16-bit part of either would double O1 or O2.  It makes a 16-bit result's error 1.4 times that of its own
+// rounding (2.3e-3 and 1.7e-3 of bfloat16's norm).
 //
 // A CTA has one job's head (or a part of its time axis) and 64 columns of c: two chunks' tiles (three of up to 64 columns), C' and X fill
 // shared memory.  One warp loads (TMA), three issue products (scores; O1 and O2; U), each as soon as its own operands are there, four
 // make P, four the output, four C' (half a chunk ahead of its product), four keep the state: 20 warps.
 //
 // Rows of a tile are steps in the order of time.  Back in time, position i of a chunk is row 127 - i, and triangle and weights are mirrored.
+//
+// Float16 pays for its powers of two, of c's and X's largest elements in each chunk, with 970 us where 780 were without them, 326 and 268
+// forward (2x16384x16x128).  C''s own warps look for c's: two other roles that did it a chunk ahead took 1100, since a tile comes when C' waits for it.
 //
 // 2x16384x16x128 bf16 with its gradients takes 750 us (850 over seconds of it; its bytes alone 168, its products, some 450 GFLOP, 270).  A chunk takes about 2.5 us:
 // products some 1.2 us at the measured rate, the rest is the chain scores - P - O2 with its two ways through tensor memory, which one CTA an SM (shared
@@ -38,7 +44,11 @@ struct Control {
     uint64_t full[3], full_c[3], empty[3], zeroed, scores_full, scores_empty, p_full, p_empty, out_full[2], out_empty[2], c_full[2], c_empty[2], u_full, u_empty,
         x_full, x_empty;
     uint32_t tmem;
-    float up[4], most[4];
+    float up[4];                                 // the state's copy, back to its size
+    uint32_t most[2][4];
+    uint32_t c_most[2][4];
+    float c_back[2];                             // C', back to its size
+    int8_t score_shift[4][kSteps];               // rows of P are times 2^this; kept until the output has left its chunk, which P is two ahead of at most
     float power[kSteps + 1];                     // g^n
     float diagonal[64];                          // [32 + row - column]: weights of 32 x 32 scores on the diagonal, 0 behind it
     alignas(16) float across[32];                // [column]: those of a row in front of such a block, from its last column but one on
@@ -62,6 +72,9 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity) {
         }
     }
 }
+
+// The larger magnitude
+__device__ __forceinline__ float larger(float most, Lanes y) { return fmaxf(fmaxf(most, fabsf(y.at(0))), fabsf(y.at(1))); }
 
 // From a table in shared memory that does not change any more, by its shared address (through a generic one the 32 loads of a block
 // of scores took 600 cycles)
@@ -124,6 +137,8 @@ __device__ __forceinline__ void load_box(uint32_t to, const CUtensorMap& map, in
                  "l"(reinterpret_cast<uint64_t>(&map)), "r"(col), "r"(head), "r"(t), "r"(batch), "r"(tc::smem_u32(bar))
                  : "memory");
 }
+
+static_assert(sizeof(Control) <= 2048, "the control block's place in shared memory");
 
 // kEnds: the sums of each part's b_j c_j^T alone
 template <typename T, int KA, bool kEnds>
@@ -218,42 +233,60 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
             const int w = warp & 3;
             const uint32_t rows_at = tmem + ((uint32_t)(w * 32) << 16), diagonal = tc::smem_u32(ctl.diagonal + 32 + lane);
             const float near = table(power + 4 * (reverse ? 32 - lane : lane + 1));
+            int shift = 0;                       // float16: of this row, as the chunk before left it
             for (int n = 0; n < chunks; ++n) {
                 if (!wait(&ctl.scores_full, n & 1) || (n > 0 && !wait(&ctl.p_empty, (n - 1) & 1))) break;
                 __syncwarp();
                 tc::tc_fence_after();
                 // (short code in loops: the roles' instructions together would not stay in the caches that feed the schedulers)
+                // Float16: a row is right when its largest weight lies in [2^-8, 2^15), so that those down to 2^-6 of it have their 11 bits and
+                // smaller ones are off by 2^-17 of it; if not, it is brought to 2^6 and the warp's rows are made once more.  Rows at a place in
+                // their chunk differ little from chunk to chunk, so that this is rare.
+                for (bool again = false;; again = true) {
+                    const float by = kNarrow<T> ? two_to(shift) : 1.0f;
+                    float most = 0.0f;
 #pragma unroll 1
-                for (int cb = 0; cb < 4; ++cb) {
-                    const int back = reverse ? cb - w : w - cb;  // blocks of 32 steps back
-                    if (back < 0 && n > 0) continue;             // (zeros already)
-                    uint32_t v[32];
-                    if (back >= 0) {
-                        tc::tmem_ld32(rows_at + kTmScores + cb * 32, v);
-                        tc::tmem_ld_wait();
-                    }
-                    if (back > 0) {
-                        const Lanes f = all_lanes(near * table(power + 128 * (back - 1)));
-#pragma unroll
-                        for (int k = 0; k < 16; k += 2) {
-                            Raw<16> c;
-                            load_shared(c, ctl.across + 2 * k);
-                            const float c0[2] = {__uint_as_float(c.u[0]), __uint_as_float(c.u[1])}, c1[2] = {__uint_as_float(c.u[2]), __uint_as_float(c.u[3])};
-                            const float x0[2] = {__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])};
-                            const float x1[2] = {__uint_as_float(v[2 * k + 2]), __uint_as_float(v[2 * k + 3])};
-                            const Lanes y0 = lanes(x0) * (f * lanes(c0)), y1 = lanes(x1) * (f * lanes(c1));
-                            v[k] = word_of<T>(y0.at(0), y0.at(1)), v[k + 1] = word_of<T>(y1.at(0), y1.at(1));
+                    for (int cb = 0; cb < 4; ++cb) {
+                        const int back = reverse ? cb - w : w - cb;      // blocks of 32 steps back
+                        if (back < 0 && n > 0) continue;                 // (zeros already)
+                        uint32_t v[32];
+                        if (back >= 0) {
+                            tc::tmem_ld32(rows_at + kTmScores + cb * 32, v);
+                            tc::tmem_ld_wait();
                         }
-                    } else if (back == 0) {
+                        if (back > 0) {
+                            const Lanes f = all_lanes(near * table(power + 128 * (back - 1)) * by);
 #pragma unroll
-                        for (int k = 0; k < 16; ++k)
-                            v[k] = word_of<T>(__uint_as_float(v[2 * k]) * table(diagonal - 8 * k), __uint_as_float(v[2 * k + 1]) * table(diagonal - 8 * k - 4));
-                    } else {
+                            for (int k = 0; k < 16; k += 2) {
+                                Raw<16> c;
+                                load_shared(c, ctl.across + 2 * k);
+                                const float c0[2] = {__uint_as_float(c.u[0]), __uint_as_float(c.u[1])}, c1[2] = {__uint_as_float(c.u[2]), __uint_as_float(c.u[3])};
+                                const float x0[2] = {__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])};
+                                const float x1[2] = {__uint_as_float(v[2 * k + 2]), __uint_as_float(v[2 * k + 3])};
+                                const Lanes y0 = lanes(x0) * (f * lanes(c0)), y1 = lanes(x1) * (f * lanes(c1));
+                                if constexpr (kNarrow<T>) most = larger(larger(most, y0), y1);
+                                v[k] = word_of<T>(y0.at(0), y0.at(1)), v[k + 1] = word_of<T>(y1.at(0), y1.at(1));
+                            }
+                        } else if (back == 0) {
 #pragma unroll
-                        for (int k = 0; k < 16; ++k) v[k] = 0;
+                            for (int k = 0; k < 16; ++k) {
+                                const float x[2] = {__uint_as_float(v[2 * k]), __uint_as_float(v[2 * k + 1])}, c[2] = {table(diagonal - 8 * k), table(diagonal - 8 * k - 4)};
+                                Lanes y = lanes(x) * lanes(c);
+                                if constexpr (kNarrow<T>) y = y * all_lanes(by), most = larger(most, y);
+                                v[k] = word_of<T>(y.at(0), y.at(1));
+                            }
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k) v[k] = 0;
+                        }
+                        tmem_st16(rows_at + kTmP + cb * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
                     }
-                    tmem_st16(rows_at + kTmP + cb * 16, *reinterpret_cast<uint32_t(*)[16]>(v));
+                    if constexpr (!kNarrow<T>) break;
+                    const bool fits = most == 0.0f || most == CUDART_INF_F || (most >= 0.00390625f && most < 32768.0f);
+                    if (again || __all_sync(0xffffffffu, fits)) break;
+                    if (!fits) shift = min(max(shift + 6 + 127 - (int)(__float_as_uint(most) >> 23), -60), 60);
                 }
+                if constexpr (kNarrow<T>) ctl.score_shift[n & 3][w * 32 + lane] = (int8_t)shift;
                 tmem_st_wait();
                 tc::tc_fence_before();
                 tc::mbar_arrive_warp(&ctl.scores_empty);
@@ -274,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 if (!wait(&ctl.out_full[n & 1], (n >> 1) & 1)) break;
                 __syncwarp();
                 tc::tc_fence_after();
-                const float w1 = weight * ctl.up[n & 3];
+                const float w1 = weight * ctl.up[n & 3], w2 = kNarrow<T> ? scale * two_to(-ctl.score_shift[n & 3][r]) : scale;
                 const bool in = i < finish - begin - n * kSteps;
                 const int t = reverse ? length - kSteps - begin - n * kSteps + r : begin + n * kSteps + r;
                 char* to = first_row + t * row_bytes;
@@ -290,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     }
                     float o[16];
 #pragma unroll
-                    for (int k = 0; k < 16; ++k) o[k] = fmaf(__uint_as_float(p[k]), w1, __uint_as_float(q[k]) * scale);
+                    for (int k = 0; k < 16; ++k) o[k] = fmaf(__uint_as_float(p[k]), w1, __uint_as_float(q[k]) * w2);
                     if (in && col0 + cb * 16 < room) {           // (a multiple of 8)
                         const bool both = col0 + cb * 16 + 8 < room;
                         if (wide) {
@@ -333,25 +366,47 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         const uint32_t spot = tc::swz_offset(r0, c);
         bool ok = true;
         tc::Ring ring;
-        for (int n = 0; n < chunks && ok; ++n, ring.next(R::kStages)) {
-            ok = wait(&ctl.full_c[ring.i], ring.ph);
+        // (a warp that gives up goes on to the others' barriers: these have no limit)
+        for (int n = 0; n < chunks; ++n, ring.next(R::kStages)) {
+            ok = ok && wait(&ctl.full_c[ring.i], ring.ph);
             const int rows = min(kSteps, finish - begin - n * kSteps), top = rows - extra, parts = parts_of_chunk(n);
-            if (ok && n == ragged && wait(&ctl.full[ring.i], ring.ph)) {
+            if (n == ragged) {
+                ok = ok && wait(&ctl.full[ring.i], ring.ph);
                 const uint32_t tile = base + ring.i * R::kStage + R::kA;        // b's halves, and c's behind them
-                for (int k = tid; k < (KA / 64 + 1) * (kSteps - rows) * 8; k += 128)
+                for (int k = tid; ok && k < (KA / 64 + 1) * (kSteps - rows) * 8; k += 128)
                     tc::st_shared_v4(tile + k / ((kSteps - rows) * 8) * R::kHalf + tc::swz_offset(rows + k / 8 % (kSteps - rows), k % 8), 0, 0, 0, 0);
                 tc::fence_proxy_async_smem();
-                tc::mbar_arrive_warp(&ctl.zeroed);
+                if (ok) tc::mbar_arrive_warp(&ctl.zeroed);
                 asm volatile("bar.sync 2, 128;" ::: "memory");
+            }
+            float by = 1.0f, back = 1.0f;
+            if constexpr (kNarrow<T>) {
+                // the tile's largest
+                uint32_t m[4] = {};              // (chains of their own)
+#pragma unroll
+                for (int p = 0; p < 8; ++p) {
+                    const uint4 v = tc::lds128(base + ring.i * R::kStage + 2 * R::kA + spot + p * 2048);
+                    m[0] = larger_pairs(m[0], v.x), m[1] = larger_pairs(m[1], v.y), m[2] = larger_pairs(m[2], v.z), m[3] = larger_pairs(m[3], v.w);
+                }
+                uint32_t most = __vmaxu2(__vmaxu2(m[0], m[1]), __vmaxu2(m[2], m[3]));
+                most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+                if ((tid & 31) == 0) ctl.c_most[n & 1][warp & 3] = most;
+                asm volatile("bar.sync 2, 128;" ::: "memory");
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = max(most, ctl.c_most[n & 1][k]);
+                const int shift = shift_up(most);
+                by = two_to(shift), back = two_to(-shift);
             }
             for (int half = 0; half < 2 && ok; ++half) {
                 ok = n == 0 || wait(&ctl.c_empty[half], (n - 1) & 1);
                 if (!ok) break;
+                // (behind the wait: the state has taken the chunk before the last)
+                if (kNarrow<T> && half == 0 && tid == 0) ctl.c_back[n & 1] = back;
                 const uint32_t from = base + ring.i * R::kStage + 2 * R::kA + spot + half * 8192, to = base + R::kWeighted + spot + half * 8192;
 #pragma unroll 1
                 for (int p = 0; p < 4; ++p) {
                     const int row = r0 + 16 * p + 64 * half, j = reverse ? kSteps - 1 - row : row;
-                    const Lanes f = all_lanes(j < rows ? table(power + 4 * max(top - j, 0)) : 0.0f);
+                    const Lanes f = all_lanes(j < rows ? table(power + 4 * max(top - j, 0)) * by : 0.0f);
                     const uint4 v = tc::lds128(from + p * 2048);
                     const uint32_t in[4] = {v.x, v.y, v.z, v.w};
                     uint32_t out[R::kParts][4];
@@ -405,64 +460,65 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
             }
         }
-        auto put_copy = [&](int n) {             // the state before chunk n
-            float down = 1.0f;
-            if constexpr (std::is_same<T, __half>::value) {
-                float most = 0.0f;
+        bool ok = true;
+        auto put_copy = [&](int n) {             // the state before chunk n (a warp that gives up goes on to the others' barriers)
+            float by = 1.0f;
+            if constexpr (kNarrow<T>) {
+                uint32_t m[4] = {};              // (chains of their own)
 #pragma unroll
-                for (int k = 0; k < kDv; ++k) most = fmaxf(most, mine ? fabsf(x[k]) : 0.0f);
+                for (int k = 0; k < kDv; ++k) m[k & 3] = larger_finite(m[k & 3], x[k]);
+                uint32_t most = __reduce_max_sync(0xffffffffu, mine ? max(max(m[0], m[1]), max(m[2], m[3])) : 0);
+                if (lane == 0) ctl.most[n & 1][w] = most;
+                asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                if (lane == 0) ctl.most[w] = most;
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                most = fmaxf(fmaxf(ctl.most[0], ctl.most[1]), fmaxf(ctl.most[2], ctl.most[3]));
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                const int over = min(max((int)(__float_as_uint(most) >> 23) - 127 - 14, 0), 126);
-                down = __uint_as_float((uint32_t)(127 - over) << 23);
-                if (tid == 0) ctl.up[n & 3] = __uint_as_float((uint32_t)(127 + over) << 23);
+                for (int k = 0; k < 4; ++k) most = max(most, ctl.most[n & 1][k]);
+                const int shift = shift_of(magnitude(most));
+                by = two_to(shift);
+                if (tid == 0) ctl.up[n & 3] = two_to(-shift);
             } else {
                 if (tid == 0) ctl.up[n & 3] = 1.0f;
             }
+            if (!ok) return;
             if (mine) {
 #pragma unroll
                 for (int c = 0; c < 8; ++c) {
                     const float* const v = x + 8 * c;
-                    tc::st_shared_v4(base + R::kState + tc::swz_offset(i, c), word_of<T>(v[0] * down, v[1] * down), word_of<T>(v[2] * down, v[3] * down),
-                                     word_of<T>(v[4] * down, v[5] * down), word_of<T>(v[6] * down, v[7] * down));
+                    tc::st_shared_v4(base + R::kState + tc::swz_offset(i, c), word_of<T>(v[0] * by, v[1] * by), word_of<T>(v[2] * by, v[3] * by),
+                                     word_of<T>(v[4] * by, v[5] * by), word_of<T>(v[6] * by, v[7] * by));
                 }
             }
             tc::fence_proxy_async_smem();
             tc::mbar_arrive_warp(&ctl.x_full);
         };
-        bool ok = true;
         if constexpr (!kEnds) put_copy(0);
         for (int n = 0; n < chunks; ++n) {
             const int rows = min(kSteps, finish - begin - n * kSteps);
             const Lanes whole = all_lanes(table(power + 4 * rows));
-            ok = wait(&ctl.u_full, n & 1);
-            if (!ok) break;
-            __syncwarp();
-            tc::tc_fence_after();
+            ok = ok && wait(&ctl.u_full, n & 1);
+            if (ok) {
+                __syncwarp();
+                tc::tc_fence_after();
+                const Lanes back = all_lanes(kNarrow<T> ? ctl.c_back[n & 1] : 1.0f);
 #pragma unroll
-            for (int cb = 0; cb < 4; ++cb) {
-                uint32_t v[16];
-                tc::tmem_ld16(rows_at + cb * 16, v);
-                tc::tmem_ld_wait();
-                if (cb == 3) {
-                    tc::tc_fence_before();
-                    tc::mbar_arrive_warp(&ctl.u_empty);
-                }
+                for (int cb = 0; cb < 4; ++cb) {
+                    uint32_t v[16];
+                    tc::tmem_ld16(rows_at + cb * 16, v);
+                    tc::tmem_ld_wait();
+                    if (cb == 3) {
+                        tc::tc_fence_before();
+                        tc::mbar_arrive_warp(&ctl.u_empty);
+                    }
 #pragma unroll
-                for (int k = 0; k < 16; k += 2) {
-                    const float a[2] = {x[cb * 16 + k], x[cb * 16 + k + 1]}, e[2] = {__uint_as_float(v[k]), __uint_as_float(v[k + 1])};
-                    const Lanes r = fma(lanes(a), whole, lanes(e));
-                    x[cb * 16 + k] = r.at(0), x[cb * 16 + k + 1] = r.at(1);
+                    for (int k = 0; k < 16; k += 2) {
+                        const float a[2] = {x[cb * 16 + k], x[cb * 16 + k + 1]}, e[2] = {__uint_as_float(v[k]), __uint_as_float(v[k + 1])};
+                        const Lanes r = fma(lanes(a), whole, kNarrow<T> ? lanes(e) * back : lanes(e));
+                        x[cb * 16 + k] = r.at(0), x[cb * 16 + k + 1] = r.at(1);
+                    }
                 }
             }
             if constexpr (!kEnds) {
                 if (n + 1 < chunks) {
-                    ok = wait(&ctl.x_empty, n & 1);     // A has met the copy before
-                    if (!ok) break;
+                    ok = ok && wait(&ctl.x_empty, n & 1);       // A has met the copy before
                     __syncwarp();
                     put_copy(n + 1);
                 }

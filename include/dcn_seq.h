@@ -155,7 +155,9 @@ size_t dcn_attn_workspace_bytes(const dcn_attn* p, int32_t backward);
 /* out [batch, steps, heads, dv] (dense) and last [batch, heads, dk, dv] (float32): the state after the last step.  log_decay float32
  * [heads], taken as 0 where it is above; `state` [batch, heads, dk, dv] float32, or NULL for zeros.  `lengths` [batch] int64, or
  * NULL: sequence b has lengths[b] steps (taken into [0, steps]); behind them out is zero, and q, k and v are not read.
- * In 16-bit types the state that meets q, and the weights that meet v within a block of up to 128 steps, are rounded to the type; `last` is not. */
+ * In 16-bit types the state that meets q, and the weights that meet v within a block of up to 128 steps, are rounded to the type (float16: relative
+ * to the state's and to a step's largest, so that neither leaves its range); `last` is not, but v enters it in parts, which in bfloat16 hold 2^-24 of it
+ * (2^-17 more than 1.5 decays before the end) and in float16 2^-22, or 2^-40 of a block's largest v. */
 int dcn_attn_forward(const dcn_attn* p, const void* q, const void* k, const void* v, const float* log_decay, const float* state,
                      const int64_t* lengths, void* out, float* last, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -1,0 +1,98 @@
+"""Decayed attention in float16 where numbers lie far from one: scores and gradients' products above its largest number, states, values
+and gradients below its normal ones.  What is rounded is rounded relative to its row, its head's state or its block, by powers of two."""
+import pytest
+import torch
+
+from tests import more_sequence_reference as more
+from tests import sequence_reference as ref
+from tests.test_decay_attention_gpu import EXTRA, STATE, make
+
+pytestmark = pytest.mark.gpu
+dcn = pytest.importorskip("deform_conv3d_pytorch_op_b200")
+
+F16 = torch.float16
+NAMES = ("out", "last", "dq", "dk", "dv", "dstate")
+# steps, offset of the operands in memory: the small kernel (one block of steps, part of one, several: operands off 16 bytes), tensor cores
+WAYS = [(40, 0), (64, 0), (300, 1), (200, 0), (700, 0)]
+
+
+def run(steps, offset, dk, dv, q=1.0, k=1.0, v=1.0, state=1.0, dout=1.0, dlast=1.0, only=NAMES, lengths=None, kv=2):
+    """All results with operands of these sizes.  Bounds: those of the operator's other tests, which count roundings relative to what is
+    rounded, and so hold at any size that the types have."""
+    a = make(F16, 2, steps, 2, kv, dk, dv, seed=steps + dk, offset=offset)
+    g = torch.Generator(device="cuda").manual_seed(3)
+    args = [x * s for x, s in zip((a[0], a[1], a[2], a[4]), (q, k, v, state))]
+    if offset:
+        args[:3] = [torch.cat([x.flatten()[:1], x.flatten()])[1:].view(x.shape) for x in args[:3]]
+        assert all(x.data_ptr() % 16 == 2 for x in args[:3])
+    leaves = [x.detach().requires_grad_() for x in args]
+    if offset:
+        assert all(x.data_ptr() % 16 == 2 for x in leaves[:3])
+    wide = [x.detach().double().requires_grad_() for x in args]
+    do = torch.randn(2, steps, 2, dv, generator=g, device="cuda").mul_(dout).to(F16)
+    dl = torch.randn(2, 2, dk, dv, generator=g, device="cuda") * dlast
+    out, last = dcn.DecayAttentionFunction.apply(*leaves[:3], a[3], leaves[3], lengths)
+    want, end = more.decay_attention(*wide[:3], a[3].double(), wide[3], lengths)
+    got = [out, last] + list(torch.autograd.grad((out, last), leaves, (do, dl)))
+    expected = [want, end] + list(torch.autograd.grad((want, end), wide, (do.double(), dl.double())))
+    for name, x, y in zip(NAMES, got, expected):
+        if name in only:
+            ref.close(x, y, name, chain=ref.CHAIN + (STATE if name in ("last", "dstate") else EXTRA)[F16])
+    return expected
+
+
+@pytest.mark.parametrize("steps,offset", WAYS)
+@pytest.mark.parametrize("dk,dv", [(128, 64), (64, 64), (128, 128)])
+def test_scores_above_the_largest_number(steps, offset, dk, dv):
+    # q . k of some 64^2 * sqrt(dk) and more, where scale q . k v is some thousand times v
+    e = run(steps, offset, dk, dv, q=64.0, k=64.0, v=0.1, state=10.0, dout=0.01, only=("out", "last"))
+    assert 1000 < float(e[0].detach().abs().max()) < 65504
+
+
+@pytest.mark.parametrize("steps,offset", WAYS)
+@pytest.mark.parametrize("kv", [1, 2])
+def test_gradients_of_a_scaled_loss(steps, offset, kv):
+    # dout . v of 200 * 30 * sqrt(128) = 68000 in a third of all pairs, up to 300000.  Their sums stay in range: dk is 68000 / 8 * 0.05 times
+    # the root of the steps that a state lasts, 125 (and of two heads): 6700, and five times that in the largest of 10^5 elements
+    e = run(steps, offset, 64, 128, q=0.05, k=0.02, v=30.0, dout=200.0, dlast=10.0, kv=kv, state=0.1)
+    assert all(float(x.abs().max()) < 65504 for x in e[2:5])
+
+
+def test_scores_of_equal_rows():
+    """q = k = 32 in 128 columns: the score is 131072, and out 11585 v"""
+    for steps in (1, 20, 70):
+        q = torch.full((1, steps, 1, 128), 32.0, device="cuda", dtype=F16)
+        v = torch.randn(1, steps, 1, 64, device="cuda").to(F16)
+        out, _ = dcn.DecayAttentionFunction.apply(q, q, v, torch.full((1,), -20.0, device="cuda"))
+        ref.close(out, 131072 / 128 ** 0.5 * v.double(), chain=ref.CHAIN + EXTRA[F16] + 2 * 2.0 ** -28)
+
+
+@pytest.mark.parametrize("steps,offset", WAYS)
+@pytest.mark.parametrize("size", [0.02, 1e-3, 1e-4, 4e-6])
+def test_states_of_small_values(steps, offset, size):
+    """last and dstate are float32: as exact for small values, keys, queries and gradients as for large ones"""
+    run(steps, offset, 48, 72, v=size, state=size, dout=size, dlast=size, only=("last", "dstate"))
+    run(steps, offset, 48, 72, q=size, k=size, state=size, dlast=size, only=("last", "dstate"))
+    run(steps, offset, 48, 72, v=size, dout=size, only=("last", "dstate"), lengths=torch.tensor([steps, steps // 2 + 1], device="cuda"))
+
+
+@pytest.mark.parametrize("steps,offset", WAYS)
+def test_results_of_small_products(steps, offset):
+    """Scores, and products dout . v, below the type's normal numbers, that large operands bring back"""
+    run(steps, offset, 64, 64, q=3e-3, k=3e-3, v=300.0, state=1e-3, only=("out",))
+    run(steps, offset, 64, 64, q=100.0, k=100.0, v=1e-3, dout=1e-4, dlast=1e-4, state=1e-3, only=("dq", "dk"))
+    # and states
+    run(steps, offset, 64, 64, q=200.0, k=1e-3, v=1e-3, state=1e-5, only=("out",))
+
+
+@pytest.mark.parametrize("steps,offset", WAYS)
+def test_columns_beside_infinite_ones(steps, offset):
+    """An infinite column of the state leaves the others as they are"""
+    q, k, v, decay, state = make(F16, 1, steps, 1, 1, 32, 40, seed=steps)
+    bad = state.clone()
+    bad[..., 7] = float("inf")
+    want, end = dcn.DecayAttentionFunction.apply(q, k, v, decay, state)
+    out, last = dcn.DecayAttentionFunction.apply(q, k, v, decay, bad)
+    others = [c for c in range(40) if c != 7]
+    assert torch.equal(out[..., others], want[..., others]) and torch.equal(last[..., others], end[..., others])
+    assert not bool(torch.isfinite(last[..., 7]).any())
