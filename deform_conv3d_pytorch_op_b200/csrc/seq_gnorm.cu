@@ -27,6 +27,7 @@ namespace {
 constexpr int64_t kMostChannels = 8192;
 constexpr int kThreads = 256;                    // of a CTA of the two passes, at most
 constexpr int kHeldBytes = 96 * 1024;            // of a sample's tensors, so that two CTAs share an SM
+constexpr int kMostShared = 227 * 1024;          // what a CTA may ask for
 
 struct GnormArgs {
     const void *x, *weight, *bias, *residual, *dy;
@@ -329,6 +330,10 @@ struct Channels {
 
 // A thread's vectors of the next positions, on their way to its own places in shared memory while it works: no barrier, no registers.
 constexpr int kDepth = 8;
+// (the most that any call asks for: three tensors' rings of 16 bytes a thread beside a channel's sums and two numbers of each group, or beside
+// four numbers of each group and two of each thread)
+static_assert(3 * kDepth * kThreads * 16 + (8 + 2 * 4) * kMostChannels + 8 <= kMostShared && 3 * kDepth * kThreads * 16 + 4 * 4 * kMostChannels + 8 * kThreads <= kMostShared,
+              "a group a channel, and as many channels as there may be");
 template <typename T, int V>
 struct Ring {
     static constexpr int kBytes = sizeof(T) * V, kKind = kDepth * kThreads * kBytes;         // kKind: of a tensor
@@ -1179,7 +1184,7 @@ GnormArgs gnorm_args(const dcn_gnorm* p, const Plan& r) {
 template <typename K>
 int launch_gnorm(K kernel, int64_t ctas, const Plan& r, size_t smem, const GnormArgs& a, cudaStream_t st) {
     // (one amount per kernel, so that calls of several host threads do not take it from one another)
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) return DCN_ERR_CUDA;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostShared) != cudaSuccess) return DCN_ERR_CUDA;
     return launch_dependent(kernel, dim3((unsigned)ctas), dim3(r.threads), smem, st, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
 
