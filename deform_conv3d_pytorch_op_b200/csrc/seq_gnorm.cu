@@ -290,6 +290,13 @@ __device__ __forceinline__ float2 two_of(const GnormArgs& a, const void* from, i
     if (a.inv < 1.0f) q.get(x + (a.per_group == 2 ? 1 : a.channels));
     return make_float2(p.at(0), q.at(0));
 }
+// Mean and 1 / sqrt(var + eps) of a tiny group, in the definition's own order of steps
+template <typename T>
+__device__ __forceinline__ float2 tiny_stats(const GnormArgs& a, int64_t base, int g) {
+    const float2 v = two_of<T>(a, a.x, base, g);
+    const float mean = __fmul_rn(__fadd_rn(v.x, v.y), a.inv), p = __fsub_rn(v.x, mean), q = a.inv < 1.0f ? __fsub_rn(v.y, mean) : 0.0f;
+    return make_float2(mean, rsqrtf(__fadd_rn(__fmul_rn(__fadd_rn(__fmul_rn(p, p), __fmul_rn(q, q)), a.inv), a.eps)));
+}
 // A group's mean and 1 / sqrt(var + eps) from such sums
 __device__ __forceinline__ float2 finish(const GnormArgs& a, float about, float2 s) {
     const float d = s.x * a.inv;
@@ -429,12 +436,7 @@ __global__ void __launch_bounds__(512) gnorm_held_kernel(const GnormArgs a) {
         join_channels(a, grid.rows, entries, nullptr, false, stats, [](int) { return 1.0f; });
         __syncthreads();
         for (int g = threadIdx.x; g < a.groups; g += blockDim.x) {
-            float2 f = finish(a, about[g], make_float2(stats[2 * g], stats[2 * g + 1]));
-            if (a.tiny) {
-                const float2 v = two_of<T>(a, a.x, base, g);
-                const float mean = __fmul_rn(__fadd_rn(v.x, v.y), a.inv), p = __fsub_rn(v.x, mean), q = a.inv < 1.0f ? __fsub_rn(v.y, mean) : 0.0f;
-                f = make_float2(mean, rsqrtf(__fadd_rn(__fmul_rn(__fadd_rn(__fmul_rn(p, p), __fmul_rn(q, q)), a.inv), a.eps)));
-            }
+            const float2 f = a.tiny ? tiny_stats<T>(a, base, g) : finish(a, about[g], make_float2(stats[2 * g], stats[2 * g + 1]));
             stats[2 * g] = f.x, stats[2 * g + 1] = f.y;
         }
         __syncthreads();
@@ -571,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 3) gnorm_apply_kernel(const GnormArg
         const float c = (float)((min(from + a.split_positions, a.positions) - from) * a.per_group), d = m - m0;
         sx = c * d, sy = fmaf(c * d, d, q);
     }, [&](int g, float sx, float sy, float m0) {
-        const float2 f = finish(a, m0, make_float2(sx, sy));
+        const float2 f = a.tiny ? tiny_stats<T>(a, sample * a.positions * a.channels, g) : finish(a, m0, make_float2(sx, sy));
         stats[2 * g] = f.x, stats[2 * g + 1] = f.y;
     });
     if (a.stats != nullptr && split == 0)
@@ -656,7 +658,7 @@ struct Sums {
     }
 };
 
-// kTiny: where groups may have one or two elements
+// kTiny: where groups may have one or two elements (a.tiny says whether they do)
 template <typename T, int V, bool kTiny>
 struct Gradient {
     Channels<T, V> ch;
@@ -1023,7 +1025,8 @@ __device__ __forceinline__ void weight_gradients(const GnormArgs& a, int block, 
     put(a.dweight, q), put(a.dbias, s);
 }
 
-template <typename T, int V>
+// kTiny: groups of one or two elements, of so many channels that no CTA holds a sample
+template <typename T, int V, bool kTiny>
 __global__ void __launch_bounds__(kThreads, 2) gnorm_apply_backward_kernel(const GnormArgs a) {
     extern __shared__ __align__(16) char smem[];
     const Ring<T, V> ring(smem);
@@ -1046,7 +1049,10 @@ __global__ void __launch_bounds__(kThreads, 2) gnorm_apply_backward_kernel(const
     stream_begin(grid.col < a.vectors ? n : 0, issue);
     for (int i = threadIdx.x; i < 2 * a.groups; i += blockDim.x) stats[i] = gload(a.stats + sample * 2 * a.groups + i);
     gather_splits(a, sample, sums + 2 * a.groups, [&](int, float p, float q, float, float& x, float& y) { x = p, y = q; },
-                  [&](int g, float x, float y, float) { sums[2 * g] = x, sums[2 * g + 1] = y; });
+                  [&](int g, float x, float y, float) {
+                      sums[2 * g] = x, sums[2 * g + 1] = y;
+                      if constexpr (kTiny) tiny_sums<T>(a, sample * a.positions * a.channels, g, stats, sums);
+                  });
     for (int b = 0; b < grid.blocks; ++b) {
         const int col = grid.col + b * blockDim.x;
         if (b > 0) {
@@ -1054,7 +1060,7 @@ __global__ void __launch_bounds__(kThreads, 2) gnorm_apply_backward_kernel(const
             stream_begin(col < a.vectors ? n : 0, issue);
         }
         if (grid.row < 0 || col >= a.vectors) continue;
-        Gradient<T, V, false> gr;
+        Gradient<T, V, kTiny> gr;
         gr.get(a, col * V, stats, sums);
         int64_t to = at + col * V;
         stream(n, issue, [&](int slot, auto&& ahead) {
@@ -1209,7 +1215,8 @@ int backward_as(const GnormArgs& a, const Plan& r, cudaStream_t st) {
                      : launch_gnorm(gnorm_sums_backward_kernel<T, V>, r.ctas, r, r.smem, a, st);
     if (rc != DCN_OK || (!weights && once)) return rc;
     if (!once && data)
-        return launch_gnorm(gnorm_apply_backward_kernel<T, V>, blocks + r.ctas, r, 4 * a.groups * 4 + room, a, st);
+        return launch_gnorm(a.tiny ? gnorm_apply_backward_kernel<T, V, true> : gnorm_apply_backward_kernel<T, V, false>, blocks + r.ctas, r,
+                            4 * a.groups * 4 + room, a, st);
     if (!weights) return DCN_OK;
     return launch_dependent(gnorm_weights_kernel<T>, dim3(blocks), dim3(512), 2 * 512 * 4, st, a, r.single ? r.ctas / r.blocks : r.held ? r.ctas : a.samples * a.splits) !=
                    cudaSuccess
