@@ -286,6 +286,8 @@ class GroupNormAct(nn.Module):
         super().__init__()
         if groups < 1 or channels % groups:
             raise _lib.DcnError("%d groups do not divide the %d channels" % (groups, channels))
+        if not 1 <= channels <= 8192:
+            raise _lib.DcnError("%d channels: 1 to 8192 are supported" % channels)
         self.groups, self.channels, self.activation, self.dim, self.eps = groups, channels, activation, dim, eps
         self.weight = nn.Parameter(torch.ones(channels, device=device, dtype=dtype))
         self.bias = nn.Parameter(torch.zeros(channels, device=device, dtype=dtype))
@@ -303,7 +305,7 @@ class GroupNormAct(nn.Module):
 
 class DecayAttention(nn.Module):
     """Projection of features to queries, keys and values, decayed attention over time, and a group norm with SiLU over each head's
-    outputs: [batch, steps, features] -> [batch, steps, heads * dv].  The first head's states last about ``memory`` steps, the last
+    outputs: [batch, steps, features] -> [batch, steps, heads * dv] (up to 8192).  The first head's states last about ``memory`` steps, the last
     one's sixteen times as long."""
 
     def __init__(self, features, heads, dk, dv=None, kv_heads=None, memory=8.0, device=None, dtype=None):
@@ -312,6 +314,8 @@ class DecayAttention(nn.Module):
         if not (1 <= dk <= 128 and 1 <= dv <= 128) or heads < 1 or kv_heads < 1 or heads % kv_heads:
             raise _lib.DcnError("%d heads of %d and %d elements and %d of keys: 1 to 128 elements, and heads that the keys' divide"
                                 % (heads, dk, dv, kv_heads))
+        if heads * dv > 8192:
+            raise _lib.DcnError("%d heads of %d elements: their norm takes up to 8192 channels" % (heads, dv))
         self.features, self.heads, self.kv_heads, self.dk, self.dv = features, heads, kv_heads, dk, dv
         self.proj = nn.Linear(features, heads * dk + kv_heads * (dk + dv), device=device, dtype=dtype)
         self.norm = GroupNormAct(heads, heads * dv, "silu", dim=-1, device=device, dtype=dtype)

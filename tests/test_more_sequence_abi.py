@@ -141,3 +141,14 @@ def test_attention_keeps_the_parts_of_split_heads_alone(L, dtype):
             most = 2 * 160 * 32 * max(dk, dv) * 64 * 4         # (two CTAs an SM or fewer, on a GPU of up to 160)
             for backward in (0, 1):
                 assert L.dcn_attn_workspace_bytes(ctypes.byref(p), backward) <= most, (heads, dk, dv, backward)
+
+
+def test_modules_of_more_channels_than_their_norm_takes_are_refused():
+    for make in (lambda: dcn.DecayAttention(16, 128, 128), lambda: dcn.DecayAttention(16, 65, 8, 127), lambda: dcn.GroupNormAct(2, 8194),
+                 lambda: dcn.GroupNormAct(1, 0)):
+        with pytest.raises(dcn.DcnError, match="8192"):
+            make()
+    with pytest.raises(dcn.DcnError, match="8192"):
+        from deform_conv3d_pytorch_op_b200.video_sequence import SequenceHead
+        SequenceHead(features=8, width=8320, mixer="attention", heads=65, num_classes=3, blocks=1, device="meta")
+    assert dcn.DecayAttention(16, 64, 1, 128).norm.channels == 8192 and dcn.GroupNormAct(8192, 8192).weight.numel() == 8192
