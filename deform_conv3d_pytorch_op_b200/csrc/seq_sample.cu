@@ -16,6 +16,7 @@
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "seq_common.cuh"
 
@@ -964,25 +965,50 @@ int check_sample(const dcn_sample* p) {
     return DCN_OK;
 }
 
+// Clusters of this size that the current device has room for at once: asked once for each type, size and device
+template <typename T>
+int clusters_at_once(int size, const cudaLaunchConfig_t& cfg) {
+    static std::atomic<int> known[64][4];        // (by device and log2 of the size; one more than the number, 0: not asked yet)
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess || device < 0 || device >= 64) return 0;
+    std::atomic<int>& here = known[device][size == 8 ? 3 : size == 4 ? 2 : 1];
+    int n = here.load(std::memory_order_relaxed);
+    if (n == 0) {
+        int found = 0;
+        if (cudaOccupancyMaxActiveClusters(&found, sample_kernel<T>, &cfg) != cudaSuccess) return 0;
+        here.store(n = found + 1, std::memory_order_relaxed);
+    }
+    return n - 1;
+}
+
 template <typename T>
 int run_sample(const SampleArgs& a, int64_t rows, cudaStream_t st) {
-    int cluster = 1;
-    // As many CTAs to a row as an SM's two places for all rows allow, an eighth of them left free: clusters that no part of the GPU has room
-    // for any more would wait for the others to end (37 x 50257 f16, 0.95 of the mass: 82 us in clusters of eight, 76 us in clusters of four)
-    while (cluster < kMostCluster && rows * cluster * 2 * 8 <= 2 * dcn::sm_count() * 7 && a.vocab / (cluster * 2) >= 4096) cluster *= 2;
     constexpr size_t kBytes = sizeof(Shared);
     if (cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kBytes) != cudaSuccess) return DCN_ERR_CUDA;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * cluster));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = kBytes;
     cfg.stream = st;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = cluster, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
+    // As many CTAs to a row as leave room for all rows at once: 16-bit kernels fill an SM's registers with one CTA, float32's with two, and the
+    // parts of the GPU hold whole clusters only (bf16, 50257 tokens, 50 best: 32 rows 12.6 us in clusters of four, 25.8 of eight; 16384 tokens,
+    // 0.95 of the mass: 64 rows 26 us of two, 44 of four).  Where a CTA still has 12288 tokens, up to 7/4 as many CTAs as SMs: rows take
+    // unequal times, and the last ones begin when the first end (131072 tokens, 0.95 of the mass: 48 rows 116 us of four, 140 of two; 16 rows
+    // 55 us of eight, 84 of four; but of 50 best, 20 and 14).
+    int cluster = 1;
+    for (int size = 2; size <= kMostCluster && a.vocab / size >= 4096; size *= 2) {
+        attr[0].val.clusterDim.x = size;
+        cfg.gridDim = dim3((unsigned)(rows * size)), cfg.numAttrs = 1;
+        if (rows > clusters_at_once<T>(size, cfg) && !(a.vocab / size >= 12288 && rows * size * 4 <= 7 * dcn::sm_count())) break;
+        cluster = size;
+    }
+    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    attr[0].val.clusterDim.x = cluster;
     cfg.numAttrs = dcn::pdl_enabled() ? 2 : 1;
     return cudaLaunchKernelEx(&cfg, sample_kernel<T>, a) != cudaSuccess ? DCN_ERR_CUDA : DCN_OK;
 }
