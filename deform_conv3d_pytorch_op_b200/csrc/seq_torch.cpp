@@ -416,6 +416,17 @@ dcn_attn attn_of(const Numbers& n, const Tensor& q, const Tensor& k, const Tenso
     return p;
 }
 
+// An operand of a 16-bit sequence of more than 64 steps that begins off 16 bytes with strides that are on them (part of a wider row, say), copied:
+// the kernel that takes it as it is walks a long sequence on one CTA a head (2x16384x16x128 bf16 with gradients 7118 us, 745 on 16 bytes).
+// Other strides are laid out anew by the operator itself.
+Tensor on_16_bytes(const Tensor& operand) {
+    const Tensor t = dense_last(operand);
+    if (!t.defined() || t.element_size() != 2 || t.size(1) <= 64 || t.numel() == 0 || reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0) return t;
+    for (int64_t d = 0; d < 3; ++d)
+        if (t.size(d) > 1 && (t.stride(d) <= 0 || t.stride(d) % 8 != 0)) return t;
+    return t.clone(at::MemoryFormat::Contiguous);
+}
+
 Tensor workspace(size_t bytes, const Tensor& x) {
     return bytes > 0 ? at::empty({(int64_t)bytes}, x.options().dtype(at::kByte)) : Tensor();
 }
@@ -429,7 +440,7 @@ variable_list attn_forward(const Numbers& n, const variable_list& in, bool keep,
     shaped(in[4], "state", {batch, heads, dk, dv});
     shaped(in[5], "lengths", {batch});
     const Tensor lengths = whole_numbers(in[5], "lengths"), decay = in[3].contiguous();
-    const Tensor q = dense_last(in[0]), k = dense_last(in[1]), v = dense_last(in[2]);
+    const Tensor q = on_16_bytes(in[0]), k = on_16_bytes(in[1]), v = on_16_bytes(in[2]);
     const Tensor state = in[4].defined() ? in[4].contiguous() : in[4];
     const dcn_attn p = attn_of(n, q, k, v, Tensor());
     const c10::cuda::CUDAGuard guard(q.device());
@@ -445,13 +456,13 @@ variable_list attn_forward(const Numbers& n, const variable_list& in, bool keep,
 }
 
 variable_list attn_backward(const Numbers& n, const variable_list& kept, const variable_list& grads, const std::vector<bool>& want) {
-    const Tensor q = dense_last(kept[0]), k = dense_last(kept[1]), v = dense_last(kept[2]), decay = kept[3].contiguous();
+    const Tensor q = on_16_bytes(kept[0]), k = on_16_bytes(kept[1]), v = on_16_bytes(kept[2]), decay = kept[3].contiguous();
     const Tensor state = kept[4].defined() ? kept[4].contiguous() : kept[4];
     Tensor dout = grads[0];
     const c10::cuda::CUDAGuard guard(q.device());
     // (a gradient of the last state alone)
     if (!dout.defined()) dout = at::zeros({q.size(0), q.size(1), q.size(2), v.size(3)}, q.options());
-    dout = dense_last(dout);
+    dout = on_16_bytes(dout);
     const Tensor dlast = grads[1].defined() ? grads[1].contiguous() : grads[1];
     const dcn_attn p = attn_of(n, q, k, v, dout);
     const Tensor dq = maybe(want[0], q), dk = maybe(want[1], k), dv = maybe(want[2] || want[4], v);

@@ -149,7 +149,9 @@ typedef struct dcn_attn {
 } dcn_attn;
 
 /* Scratch bytes of dcn_attn_forward (backward = 0) and dcn_attn_backward (backward = 1) on the current device; may be 0.  Scratch and
- * tensors that start on 16 bytes let 16-bit calls of more than 64 steps take their faster kernel. */
+ * tensors that start on 16 bytes let 16-bit calls of more than 64 steps take their faster kernel.  (With rows that lie on 16 bytes, but not their
+ * first one, or a result or the scratch off them, a head's steps are walked by one CTA for 64 columns: 2x16384x16x128 bf16 with gradients
+ * takes 7118 us in place of 745.) */
 size_t dcn_attn_workspace_bytes(const dcn_attn* p, int32_t backward);
 
 /* out [batch, steps, heads, dv] (dense) and last [batch, heads, dk, dv] (float32): the state after the last step.  log_decay float32

@@ -1,5 +1,7 @@
 """Decayed attention in float16 where numbers lie far from one: scores and gradients' products above its largest number, states, values
 and gradients below its normal ones.  What is rounded is rounded relative to its row, its head's state or its block, by powers of two."""
+import ctypes
+
 import pytest
 import torch
 
@@ -9,31 +11,52 @@ from tests.test_decay_attention_gpu import EXTRA, STATE, make
 
 pytestmark = pytest.mark.gpu
 dcn = pytest.importorskip("deform_conv3d_pytorch_op_b200")
+from deform_conv3d_pytorch_op_b200 import _lib  # noqa: E402
 
 F16 = torch.float16
 NAMES = ("out", "last", "dq", "dk", "dv", "dstate")
-# steps, offset of the operands in memory: the small kernel (one block of steps, part of one, several: operands off 16 bytes), tensor cores
+# steps, offset of the results in memory: the small kernel (part of a block of steps, one, several: results off 16 bytes), tensor cores
 WAYS = [(40, 0), (64, 0), (300, 1), (200, 0), (700, 0)]
+
+
+def off_16_bytes(args, decay, lengths, do, dl):
+    """All results by the C calls, each 2 (4) bytes behind 16: so the kernel without tensor memory runs through several blocks"""
+    q, k, v, state = args
+    p = _lib.dcn_attn(dtype=2, batch=q.size(0), steps=q.size(1), heads=q.size(2), kv_heads=k.size(2), dk=q.size(3), dv=v.size(3), scale=q.size(3) ** -0.5)
+    for n, x in (("q", q), ("k", k), ("v", v), ("dout", do)):
+        for i, a in enumerate(("batch", "step", "head")):
+            setattr(p, "%s_%s" % (n, a), x.stride(i))
+    L, at = _lib.lib(), ctypes.byref(p)
+    ws = [torch.empty(max(L.dcn_attn_workspace_bytes(at, i), 16), dtype=torch.uint8, device="cuda") for i in range(2)]
+    dense = [do, state, q, k, v, state]                     # the results' shapes
+    got = [torch.empty(x.numel() + 8, dtype=x.dtype, device="cuda")[1:1 + x.numel()].view(x.shape) for x in dense]
+    lengths = 0 if lengths is None else lengths.data_ptr()
+    stream = torch.cuda.current_stream().cuda_stream
+    ins = [x.data_ptr() for x in (q, k, v, decay, state)] + [lengths]
+    outs = [x.data_ptr() for x in got]
+    assert all(x % 16 for x in outs)
+    assert L.dcn_attn_forward(at, *ins, *outs[:2], ws[0].data_ptr(), ws[0].numel(), stream) == 0
+    assert L.dcn_attn_backward(at, *ins, do.data_ptr(), dl.data_ptr(), *outs[2:], ws[1].data_ptr(), ws[1].numel(), stream) == 0
+    torch.cuda.synchronize()
+    return got
 
 
 def run(steps, offset, dk, dv, q=1.0, k=1.0, v=1.0, state=1.0, dout=1.0, dlast=1.0, only=NAMES, lengths=None, kv=2):
     """All results with operands of these sizes.  Bounds: those of the operator's other tests, which count roundings relative to what is
     rounded, and so hold at any size that the types have."""
-    a = make(F16, 2, steps, 2, kv, dk, dv, seed=steps + dk, offset=offset)
+    a = make(F16, 2, steps, 2, kv, dk, dv, seed=steps + dk)
     g = torch.Generator(device="cuda").manual_seed(3)
     args = [x * s for x, s in zip((a[0], a[1], a[2], a[4]), (q, k, v, state))]
-    if offset:
-        args[:3] = [torch.cat([x.flatten()[:1], x.flatten()])[1:].view(x.shape) for x in args[:3]]
-        assert all(x.data_ptr() % 16 == 2 for x in args[:3])
-    leaves = [x.detach().requires_grad_() for x in args]
-    if offset:
-        assert all(x.data_ptr() % 16 == 2 for x in leaves[:3])
     wide = [x.detach().double().requires_grad_() for x in args]
     do = torch.randn(2, steps, 2, dv, generator=g, device="cuda").mul_(dout).to(F16)
     dl = torch.randn(2, 2, dk, dv, generator=g, device="cuda") * dlast
-    out, last = dcn.DecayAttentionFunction.apply(*leaves[:3], a[3], leaves[3], lengths)
     want, end = more.decay_attention(*wide[:3], a[3].double(), wide[3], lengths)
-    got = [out, last] + list(torch.autograd.grad((out, last), leaves, (do, dl)))
+    if offset:
+        got = off_16_bytes(args, a[3], lengths, do, dl)
+    else:
+        leaves = [x.detach().requires_grad_() for x in args]
+        out, last = dcn.DecayAttentionFunction.apply(*leaves[:3], a[3], leaves[3], lengths)
+        got = [out, last] + list(torch.autograd.grad((out, last), leaves, (do, dl)))
     expected = [want, end] + list(torch.autograd.grad((want, end), wide, (do.double(), dl.double())))
     for name, x, y in zip(NAMES, got, expected):
         if name in only:
@@ -96,3 +119,17 @@ def test_columns_beside_infinite_ones(steps, offset):
     others = [c for c in range(40) if c != 7]
     assert torch.equal(out[..., others], want[..., others]) and torch.equal(last[..., others], end[..., others])
     assert not bool(torch.isfinite(last[..., 7]).any())
+
+
+@pytest.mark.parametrize("t", list(ref.TYPES.values()), ids=list(ref.TYPES))
+def test_parts_of_wider_rows(t):
+    """Operands that begin off 16 bytes with strides that are on them: the values of dense ones, bit for bit"""
+    row = torch.randn(2, 300, 2, 136, device="cuda").to(t)
+    q, k, v = (row[..., i:i + 40] for i in (1, 42, 91))
+    decay, state = torch.tensor([-0.01, -0.2], device="cuda"), torch.randn(2, 2, 40, 40, device="cuda")
+    leaves, dense = ([x.detach().requires_grad_() for x in y] for y in ((q, k, v), (x.contiguous() for x in (q, k, v))))
+    wide = torch.randn(2, 300, 2, 48, device="cuda").to(t)
+    do = wide[..., 3:43]
+    got, want = ((lambda o: [o[0], o[1]] + list(torch.autograd.grad(o, x, (g, torch.ones_like(state)))))(
+        dcn.DecayAttentionFunction.apply(*x, decay, state)) for x, g in ((leaves, do), (dense, do.contiguous())))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
