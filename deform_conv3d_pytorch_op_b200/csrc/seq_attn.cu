@@ -109,18 +109,19 @@ __device__ __forceinline__ float power(uint32_t table, int n) {
 // elements down to 2^-29 of that largest one keep their 11 bits.  (Bfloat16 has float32's range.)
 template <typename T>
 constexpr bool kNarrow = std::is_same<T, __half>::value;
-// n, where 2^n brings a largest magnitude (0 and above, not NaN) into [2^14, 2^15), as far as 2^n and 2^-n are normal numbers
-__device__ __forceinline__ int shift_of(float most) { return most > 0.0f ? min(max(14 + 127 - (int)(__float_as_uint(most) >> 23), -113), 100) : 0; }
-__device__ __forceinline__ float two_to(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
-// The larger magnitude of finite numbers, as bits above 2^23 (0: none yet); infinities and NaN, which become negative, are left out: columns
-// that do not meet them are not to be lost beside them
-__device__ __forceinline__ uint32_t larger_finite(uint32_t most, float v) {
-    return (uint32_t)__viaddmax_s32((int)(__float_as_uint(v) & 0x7fffffffu), 0x00800000, (int)most);
+// n, where 2^n brings a largest magnitude (0 and above, not NaN) into [2^14, 2^15), as far as 2^n and 2^-n are normal numbers; 0 for none and for
+// infinity, beside which the others stay as they are
+__device__ __forceinline__ int shift_of(float most) {
+    return most > 0.0f && most < CUDART_INF_F ? min(max(14 + 127 - (int)(__float_as_uint(most) >> 23), -113), 100) : 0;
 }
-__device__ __forceinline__ float magnitude(uint32_t most) { return most > 0x00800000u ? __uint_as_float(most - 0x00800000u) : 0.0f; }
-// the same of pairs of float16 numbers, whose shift is up alone: they are in range
-__device__ __forceinline__ uint32_t larger_pairs(uint32_t most, uint32_t pair) { return __viaddmax_s16x2(pair & 0x7fff7fffu, 0x04000400u, most); }
-__device__ __forceinline__ int shift_up(uint32_t most) { return most > 0x400u ? max(shift_of(half_of<__half>(most - 0x400u, 0)), 0) : 0; }
+__device__ __forceinline__ float two_to(int n) { return __uint_as_float((uint32_t)(127 + n) << 23); }
+// The larger magnitudes of pairs of float16 numbers, whose shift is up alone: they are in range.  (NaN is left out.)
+__device__ __forceinline__ uint32_t larger_pairs(uint32_t most, uint32_t pair) {
+    uint32_t m;
+    asm("{\n .reg .b32 a;\n abs.f16x2 a, %2;\n max.f16x2 %0, %1, a;\n}" : "=r"(m) : "r"(most), "r"(pair));
+    return m;
+}
+__device__ __forceinline__ int shift_up(uint32_t most) { return max(shift_of(half_of<__half>(most, 0)), 0); }
 
 #include "seq_attn_tc.cuh"
 
@@ -471,14 +472,14 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
     float by = 1.0f, back = 1.0f;                // float16: the copy is the state times `by`
     auto put_copy = [&]() {
         if constexpr (kNarrow<T>) {
-            uint32_t most = 0;
+            float most = 0.0f;
 #pragma unroll
             for (int m = 0; m < kM; ++m)
 #pragma unroll
                 for (int n = 0; n < kN; ++n)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) most = larger_finite(most, x[m][n][e]);
-            const int shift = shift_of(magnitude(cta_max<S::kWarps>(most, slots)));
+                    for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(x[m][n][e]));
+            const int shift = shift_of(__uint_as_float(cta_max<S::kWarps>(__float_as_uint(most), slots)));
             by = two_to(shift), back = two_to(-shift);
         }
 #pragma unroll
@@ -641,8 +642,8 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
                 float row_by[2], row_back[2], sum[kN][4] = {};
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    most[half] = __vmaxu2(most[half], __shfl_xor_sync(0xffffffffu, most[half], 1));
-                    most[half] = __vmaxu2(most[half], __shfl_xor_sync(0xffffffffu, most[half], 2));
+                    most[half] = larger_pairs(most[half], __shfl_xor_sync(0xffffffffu, most[half], 1));
+                    most[half] = larger_pairs(most[half], __shfl_xor_sync(0xffffffffu, most[half], 2));
                     const int shift = shift_up(max(most[half] & 0xffffu, most[half] >> 16));
                     row_by[half] = two_to(shift), row_back[half] = two_to(-shift);
                 }

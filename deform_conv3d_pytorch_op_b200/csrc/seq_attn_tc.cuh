@@ -17,8 +17,9 @@
 //
 // Rows of a tile are steps in the order of time.  Back in time, position i of a chunk is row 127 - i, and triangle and weights are mirrored.
 //
-// Float16 pays for its powers of two, of c's and X's largest elements in each chunk, with 970 us where 780 were without them, 326 and 268
-// forward (2x16384x16x128).  C''s own warps look for c's: two other roles that did it a chunk ahead took 1100, since a tile comes when C' waits for it.
+// Float16 pays for its powers of two, of c's and X's largest elements in each chunk, with 905 us where 780 were without them, 308 and 268
+// forward (2x16384x16x128): a tile of c comes when C' waits for it, and the state's copy is in the chain from chunk to chunk.  (C''s own warps look
+// for c's largest: two other roles that did it a chunk ahead took 1100.  Leaving infinities out of the maxima cost 60.)
 //
 // 2x16384x16x128 bf16 with its gradients takes 750 us (850 over seconds of it; its bytes alone 168, its products, some 450 GFLOP, 270).  A chunk takes about 2.5 us:
 // products some 1.2 us at the measured rate, the rest is the chain scores - P - O2 with its two ways through tensor memory, which one CTA an SM (shared
@@ -388,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     const uint4 v = tc::lds128(base + ring.i * R::kStage + 2 * R::kA + spot + p * 2048);
                     m[0] = larger_pairs(m[0], v.x), m[1] = larger_pairs(m[1], v.y), m[2] = larger_pairs(m[2], v.z), m[3] = larger_pairs(m[3], v.w);
                 }
-                uint32_t most = __vmaxu2(__vmaxu2(m[0], m[1]), __vmaxu2(m[2], m[3]));
+                uint32_t most = larger_pairs(larger_pairs(m[0], m[1]), larger_pairs(m[2], m[3]));
                 most = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
                 if ((tid & 31) == 0) ctl.c_most[n & 1][warp & 3] = most;
                 asm volatile("bar.sync 2, 128;" ::: "memory");
@@ -464,15 +465,15 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         auto put_copy = [&](int n) {             // the state before chunk n (a warp that gives up goes on to the others' barriers)
             float by = 1.0f;
             if constexpr (kNarrow<T>) {
-                uint32_t m[4] = {};              // (chains of their own)
+                float m[4] = {};                 // (chains of their own)
 #pragma unroll
-                for (int k = 0; k < kDv; ++k) m[k & 3] = larger_finite(m[k & 3], x[k]);
-                uint32_t most = __reduce_max_sync(0xffffffffu, mine ? max(max(m[0], m[1]), max(m[2], m[3])) : 0);
+                for (int k = 0; k < kDv; k += 2) m[k / 2 & 3] = fmaxf(fmaxf(m[k / 2 & 3], fabsf(x[k])), fabsf(x[k + 1]));
+                uint32_t most = __reduce_max_sync(0xffffffffu, mine ? __float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))) : 0);
                 if (lane == 0) ctl.most[n & 1][w] = most;
                 asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
                 for (int k = 0; k < 4; ++k) most = max(most, ctl.most[n & 1][k]);
-                const int shift = shift_of(magnitude(most));
+                const int shift = shift_of(__uint_as_float(most));
                 by = two_to(shift);
                 if (tid == 0) ctl.up[n & 3] = two_to(-shift);
             } else {
