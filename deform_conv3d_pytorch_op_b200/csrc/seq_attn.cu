@@ -96,6 +96,19 @@ __device__ __forceinline__ double log_decay_of(const float* log_decay, int h) {
 __device__ __forceinline__ float power_of(double log_decay, int64_t n) {
     return n == 0 && log_decay == log_decay ? 1.0f : (float)exp((double)n * log_decay);
 }
+// The decay of a whole block as the factors of one block after another, each rounded so that their product stays the power that it stands
+// for.  (One and the same rounding adds up: states of 40000 steps were off by 10^-5.)
+struct Carried {
+    double decay, inverse, off;
+    __device__ __forceinline__ void begin(double log_decay, int steps) {
+        decay = exp(steps * log_decay), inverse = decay > 1e-20 ? 1.0 / decay : 0.0, off = 0.0;          // (of less nothing is left after two)
+    }
+    __device__ __forceinline__ float next() {
+        const float f = (float)(decay - decay * off);
+        off += ((double)f - decay) * inverse;
+        return f;
+    }
+};
 // from a table of them in shared memory
 __device__ __forceinline__ float power(uint32_t table, int n) {
     float f;
@@ -371,7 +384,7 @@ struct Shape {
     static constexpr int kTileC = kChunk * Tile<T>::row_elems(kCols) * (int)sizeof(T);
     static constexpr int kState = kEnds ? 0 : KA * Tile<T>::row_elems(kCols) * (int)sizeof(T);
     static constexpr int kB = kEnds ? 0 : kTileA, kC = kB + kTileA, kStage = kC + kTileC;                // b's and c's places
-    static constexpr int kTable = kStages * kStage + kState;             // g^n, 0 to 64
+    static constexpr int kTable = kStages * kStage + kState + (int)sizeof(Carried);          // g^n, 0 to 64, behind what gives the last one
     static constexpr int kLargest = kTable + (kChunk + 1) * 4 + kWarps * 4;                  // of rows of scores, float16
     static constexpr int kBytes = kLargest + (kNarrow<T> && !kEnds ? kAcross * kChunk * 4 : 0);
     static constexpr int kHeld = kEnds ? (kFloat && KA == 128 ? 2 : 3) : kFloat && KA == 128 ? 1 : kFloat || KA == 128 ? 2 : 3;           // CTAs that an SM has room for
@@ -400,6 +413,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
     extern __shared__ __align__(128) char smem[];
     const uint32_t tiles = shared_address(smem), copy = tiles + S::kStages * S::kStage;
     float* const powers = reinterpret_cast<float*>(smem + S::kTable);
+    Carried& carried = reinterpret_cast<Carried*>(powers)[-1];
     uint32_t* const slots = reinterpret_cast<uint32_t*>(powers + kChunk + 1);
     float* const largest = reinterpret_cast<float*>(smem + S::kLargest);         // [side][row]
     const uint32_t table = shared_address(powers);
@@ -420,7 +434,8 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
     const int64_t finish = min(stop, length);    // of the steps there are
     const bool reverse = job.reverse != 0;
     const double log_decay = log_decay_of(args.log_decay, h);
-    if (threadIdx.x <= kChunk) powers[threadIdx.x] = power_of(log_decay, threadIdx.x);
+    if (threadIdx.x < kChunk) powers[threadIdx.x] = power_of(log_decay, threadIdx.x);
+    else if (threadIdx.x == kChunk) carried.begin(log_decay, kChunk), powers[kChunk] = carried.next();
     const int extra = reverse ? 0 : 1;           // powers of g on the state before a chunk, at its first step
     const int wa = job.a.width, wc = job.c.width;
     const bool exact = job.end != nullptr;       // the state is a result
@@ -703,6 +718,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
             }
         }
         __syncthreads();                         // every warp is done with the tiles and the copy
+        if (threadIdx.x == 0) powers[kChunk] = carried.next();           // (read behind the next barrier)
         if constexpr (!kEnds) put_copy();
         stage ^= 1;
     }
@@ -871,7 +887,9 @@ __global__ void __launch_bounds__(kT) attn_step_kernel(const StepArgs a) {
     const T* const q = static_cast<const T*>(a.q) + r * a.qs.batch + h * a.qs.head;
     const T* const k = static_cast<const T*>(a.k) + r * a.ks.batch + h / a.share * a.ks.head;
     const T* const v = static_cast<const T*>(a.v) + r * a.vs.batch + h / a.share * a.vs.head;
-    const float decay = power_of(log_decay_of(a.log_decay, h), 1);
+    // (and what its rounding leaves, which would add up over a stream's steps)
+    const double whole = exp(log_decay_of(a.log_decay, h));
+    const float decay = (float)whole, rest = (float)(whole - (double)decay);
     for (int i = threadIdx.x; i < a.dk; i += kT) {
         Pack<T, 1> p;
         p.get(k + i), key[i] = p.at(0);
@@ -895,7 +913,7 @@ __global__ void __launch_bounds__(kT) attn_step_kernel(const StepArgs a) {
             s.get(state + (int64_t)i * a.dv + j);
 #pragma unroll
             for (int e = 0; e < kW; ++e) {
-                f[e] = fmaf(s.at(e), decay, key[i] * value[e]);
+                f[e] = fmaf(s.at(e), decay, fmaf(s.at(e), rest, key[i] * value[e]));
                 sum[e] = fmaf(f[e], query[i], sum[e]);
             }
             s.set(f);

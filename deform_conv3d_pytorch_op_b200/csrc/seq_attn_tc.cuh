@@ -44,7 +44,9 @@ struct Room {
 struct Control {
     uint64_t full[3], full_c[3], empty[3], zeroed, scores_full, scores_empty, p_full, p_empty, out_full[2], out_empty[2], c_full[2], c_empty[2], u_full, u_empty,
         x_full, x_empty;
+    Carried carried;
     uint32_t tmem;
+    float whole[8];                              // g^128 of a chunk's turn, by the warp that loads, which is four ahead of the state at most
     float up[4];                                 // the state's copy, back to its size
     uint32_t most[2][4];
     uint32_t c_most[2][4];
@@ -178,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         const int n = threadIdx.x;
         const float w = n == 0 ? (log_decay != log_decay ? log_decay : 1.0f) : (float)exp((double)n * (double)log_decay);
         ctl.power[n] = w;
+        if (n == kSteps) ctl.carried.begin(log_decay, kSteps), ctl.whole[0] = ctl.carried.next();
         if (n < 32) {
             ctl.across[job.reverse ? n : 31 - n] = w;
             ctl.diagonal[job.reverse ? 32 - n : 32 + n] = w;
@@ -224,6 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 }
                 tc::mbar_arrive_expect_tx(&ctl.full_c[ring.i], R::kHalf);
                 load_box(to + 2 * R::kA, maps.of[job.c.map], col0, h / job.c.share, t, b, &ctl.full_c[ring.i]);
+                ctl.whole[(n + 1) & 7] = ctl.carried.next();     // (there with the next chunk's tiles)
             }
             for (int k = max(n - R::kStages, 0); k < n; ++k)     // (nothing is under way at the end)
                 wait(&ctl.full[k % R::kStages], k / R::kStages & 1), wait(&ctl.full_c[k % R::kStages], k / R::kStages & 1);
@@ -494,11 +498,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
         if constexpr (!kEnds) put_copy(0);
         for (int n = 0; n < chunks; ++n) {
             const int rows = min(kSteps, finish - begin - n * kSteps);
-            const Lanes whole = all_lanes(table(power + 4 * rows));
             ok = ok && wait(&ctl.u_full, n & 1);
             if (ok) {
                 __syncwarp();
                 tc::tc_fence_after();
+                const Lanes whole = all_lanes(rows == kSteps ? ctl.whole[n & 7] : table(power + 4 * rows));
                 const Lanes back = all_lanes(kNarrow<T> ? ctl.c_back[n & 1] : 1.0f);
 #pragma unroll
                 for (int cb = 0; cb < 4; ++cb) {

@@ -133,3 +133,37 @@ def test_parts_of_wider_rows(t):
     got, want = ((lambda o: [o[0], o[1]] + list(torch.autograd.grad(o, x, (g, torch.ones_like(state)))))(
         dcn.DecayAttentionFunction.apply(*x, decay, state)) for x, g in ((leaves, do), (dense, do.contiguous())))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("heads", [6, 300])
+@pytest.mark.parametrize("t", list(ref.TYPES.values()), ids=list(ref.TYPES))
+def test_states_that_last(t, heads):
+    """What is left of a first state and of a last one's gradient after 40000 steps, block by block: the decay of a block is rounded to
+    float32, but its roundings do not add up from block to block"""
+    steps, w = 40003, 16
+    g = torch.Generator(device="cuda").manual_seed(5)
+    decay = -torch.logspace(-6, -3.7, heads, device="cuda")
+    q, k, v = (torch.zeros(1, steps, heads, w, device="cuda", dtype=t).requires_grad_() for _ in range(3))
+    state = torch.randn(1, heads, w, w, generator=g, device="cuda").requires_grad_()
+    dl = torch.randn(1, heads, w, w, generator=g, device="cuda")
+    left = torch.exp(decay.double() * steps).view(1, heads, 1, 1)
+    out, last = dcn.DecayAttentionFunction.apply(q, k, v, decay, state)
+    (dstate,) = torch.autograd.grad(last, state, dl)
+    assert float(out.detach().abs().max()) == 0
+    # each head by itself: 626 blocks' (313 on tensor cores) products, each rounded to half a step: 2^-25 sqrt(626) and less
+    for h in range(heads):
+        ref.close(last[:, h], (left * state.double())[:, h], ("last", h))
+        ref.close(dstate[:, h], (left * dl.double())[:, h], ("dstate", h))
+
+
+def test_states_that_last_step_by_step():
+    """The same of 4000 single steps: half a step of float32 each, not the decay's rounding 4000 times"""
+    heads, steps = 200, 4000
+    decay = -torch.logspace(-5, -3, heads, device="cuda")
+    zero = torch.zeros(1, heads, 4, device="cuda")
+    pool = torch.randn(1, heads, 4, 4, generator=torch.Generator(device="cuda").manual_seed(6), device="cuda")
+    want = torch.exp(decay.double() * steps).view(1, heads, 1, 1) * pool.double()
+    for _ in range(steps):
+        dcn.DecayAttentionFunction.step(zero, zero, zero, decay, pool)
+    for h in range(heads):
+        ref.close(pool[:, h], want[:, h], h)
