@@ -134,7 +134,8 @@ __device__ __forceinline__ uint32_t larger_pairs(uint32_t most, uint32_t pair) {
     asm("{\n .reg .b32 a;\n abs.f16x2 a, %2;\n max.f16x2 %0, %1, a;\n}" : "=r"(m) : "r"(most), "r"(pair));
     return m;
 }
-__device__ __forceinline__ int shift_up(uint32_t most) { return max(shift_of(half_of<__half>(most, 0)), 0); }
+// (weight: the largest that they meet)
+__device__ __forceinline__ int shift_up(uint32_t most, float weight) { return max(shift_of(half_of<__half>(most, 0) * weight), 0); }
 
 #include "seq_attn_tc.cuh"
 
@@ -659,7 +660,7 @@ __global__ void __launch_bounds__(Shape<T, KA, kEnds>::kThreads, Shape<T, KA, kE
                 for (int half = 0; half < 2; ++half) {
                     most[half] = larger_pairs(most[half], __shfl_xor_sync(0xffffffffu, most[half], 1));
                     most[half] = larger_pairs(most[half], __shfl_xor_sync(0xffffffffu, most[half], 2));
-                    const int shift = shift_up(max(most[half] & 0xffffu, most[half] >> 16));
+                    const int shift = shift_up(max(most[half] & 0xffffu, most[half] >> 16), power(table, 1 - extra));
                     row_by[half] = two_to(shift), row_back[half] = two_to(-shift);
                 }
 #pragma unroll 1

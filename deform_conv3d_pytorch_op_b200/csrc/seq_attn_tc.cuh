@@ -399,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                 asm volatile("bar.sync 2, 128;" ::: "memory");
 #pragma unroll
                 for (int k = 0; k < 4; ++k) most = max(most, ctl.c_most[n & 1][k]);
-                const int shift = shift_up(most);
+                const int shift = shift_up(most, table(power + 4 * (1 - extra)));
                 by = two_to(shift), back = two_to(-shift);
             }
             for (int half = 0; half < 2 && ok; ++half) {

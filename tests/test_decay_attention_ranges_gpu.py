@@ -167,3 +167,23 @@ def test_states_that_last_step_by_step():
         dcn.DecayAttentionFunction.step(zero, zero, zero, decay, pool)
     for h in range(heads):
         ref.close(pool[:, h], want[:, h], h)
+
+
+@pytest.mark.parametrize("steps,offset", WAYS + [(1, 0)])
+def test_strong_decays(steps, offset):
+    """Back in time even the first step's weight is the decay itself: what little of it reaches the first state is exact"""
+    a = make(F16, 2, steps, 4, 4, 40, 64, seed=steps)
+    decay = torch.tensor([-4.0, -12.0, -25.0, -60.0], device="cuda")
+    do = torch.randn(2, steps, 4, 64, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(F16)
+    args = (a[0], a[1], a[2], a[4])
+    wide = [x.detach().double().requires_grad_() for x in args]
+    want, end = more.decay_attention(*wide[:3], decay.double(), wide[3])
+    expected = torch.autograd.grad(want, wide[3], do.double())[0]
+    if offset:
+        got = off_16_bytes(args, decay, None, do, torch.zeros_like(a[4]))[5]
+    else:
+        leaf = a[4].detach().requires_grad_()
+        out, _ = dcn.DecayAttentionFunction.apply(*args[:3], decay, leaf)
+        got = torch.autograd.grad(out, leaf, do)[0]
+    for h in range(4):
+        ref.close(got[:, h], expected[:, h], h, chain=ref.CHAIN + STATE[F16])
