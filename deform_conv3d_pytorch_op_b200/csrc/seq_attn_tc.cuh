@@ -17,7 +17,7 @@
 //
 // Rows of a tile are steps in the order of time.  Back in time, position i of a chunk is row 127 - i, and triangle and weights are mirrored.
 //
-// Float16 pays for its powers of two, of c's and X's largest elements in each chunk, with 905 us where 780 were without them, 308 and 268
+// Float16 pays for its powers of two, of c's and X's largest elements in each chunk, with 920 us where 780 were without them, 310 and 268
 // forward (2x16384x16x128): a tile of c comes when C' waits for it, and the state's copy is in the chain from chunk to chunk.  (C''s own warps look
 // for c's largest: two other roles that did it a chunk ahead took 1100.  Leaving infinities out of the maxima cost 60.)
 //

@@ -11,7 +11,7 @@
 // "Kept" is, for top-k and for top-p alike, what has less than a limit before it in falling order, equal logits by their index.
 //
 // Latency bounds it: a cluster's phases stand one behind the other, each with barriers, and reading takes a small part (64 x 131072 bf16, 50
-// best and 0.9 of the mass: 65 to 75 us, floor 2.6; 37 x 50257 f16, 0.95: 66, floor 0.6; 16 x 400 float32: 5.9 from call to call).  Lists of
+// best and 0.9 of the mass: 55 to 89 us by the logits, floor 2.6; 37 x 50257 f16, 0.95: 55 to 72, floor 0.6; 16 x 400 float32: 5.9 from call to call).  Lists of
 // the bins in question alone took the first from 187 to 89 us, limits found by bins rather than by sorting all that is kept before that.
 #include <cooperative_groups.h>
 
