@@ -888,9 +888,9 @@ __global__ void __launch_bounds__(kT) attn_step_kernel(const StepArgs a) {
     const T* const q = static_cast<const T*>(a.q) + r * a.qs.batch + h * a.qs.head;
     const T* const k = static_cast<const T*>(a.k) + r * a.ks.batch + h / a.share * a.ks.head;
     const T* const v = static_cast<const T*>(a.v) + r * a.vs.batch + h / a.share * a.vs.head;
-    // (and what its rounding leaves, which would add up over a stream's steps)
+    // (and what its rounding leaves, which would add up over a stream's steps.  Rounded down, so that this is above zero: infinity stays infinity)
     const double whole = exp(log_decay_of(a.log_decay, h));
-    const float decay = (float)whole, rest = (float)(whole - (double)decay);
+    const float decay = __double2float_rd(whole), rest = fmaxf((float)(whole - (double)decay), decay * 1e-12f);
     for (int i = threadIdx.x; i < a.dk; i += kT) {
         Pack<T, 1> p;
         p.get(k + i), key[i] = p.at(0);

@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_tc_kernel(const AttnArgs arg
                     if constexpr (!kNarrow<T>) break;
                     const bool fits = most == 0.0f || most == CUDART_INF_F || (most >= 0.00390625f && most < 32768.0f);
                     if (again || __all_sync(0xffffffffu, fits)) break;
+                    tmem_st_wait();              // (before the same places are written again)
                     if (!fits) shift = min(max(shift + 6 + 127 - (int)(__float_as_uint(most) >> 23), -60), 60);
                 }
                 if constexpr (kNarrow<T>) ctl.score_shift[n & 3][w * 32 + lane] = (int8_t)shift;

@@ -975,7 +975,10 @@ int clusters_at_once(int size, const cudaLaunchConfig_t& cfg) {
     int n = here.load(std::memory_order_relaxed);
     if (n == 0) {
         int found = 0;
-        if (cudaOccupancyMaxActiveClusters(&found, sample_kernel<T>, &cfg) != cudaSuccess) return 0;
+        if (cudaOccupancyMaxActiveClusters(&found, sample_kernel<T>, &cfg) != cudaSuccess) {
+            cudaGetLastError();                  // (it is no call's: a CTA to a row will do)
+            return 0;
+        }
         here.store(n = found + 1, std::memory_order_relaxed);
     }
     return n - 1;

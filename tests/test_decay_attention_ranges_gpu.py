@@ -187,3 +187,16 @@ def test_strong_decays(steps, offset):
         got = torch.autograd.grad(out, leaf, do)[0]
     for h in range(4):
         ref.close(got[:, h], expected[:, h], h, chain=ref.CHAIN + STATE[F16])
+
+
+def test_infinite_states_step_by_step():
+    pool = torch.randn(3, 2, 8, 8, device="cuda")
+    pool[1, 0, 3, 4], pool[2, 1, 0, 0], pool[0, 0, 7, 7] = float("inf"), float("-inf"), 3.4e38
+    q, k, v = (torch.randn(3, 2, 8, device="cuda") for _ in range(3))
+    for log_decay in (0.0, -0.3, -1e-4):
+        want = torch.exp(torch.tensor(log_decay).double()) * pool.double() + k.double()[..., None] * v.double()[..., None, :]
+        dcn.DecayAttentionFunction.step(q, k, v, torch.full((2,), log_decay, device="cuda"), pool)
+        ref.close(pool, want, log_decay)
+    zero, large = torch.zeros(1, 1, 4, device="cuda"), torch.full((1, 1, 4, 4), 3e35, device="cuda")
+    dcn.DecayAttentionFunction.step(zero, zero, zero, torch.full((1,), -float("inf"), device="cuda"), large)
+    assert float(large.abs().max()) == 0                    # none of the past at all
