@@ -197,7 +197,7 @@ class DecayAttentionFunction:
         ``scale``: 1 / sqrt(dk) if None.  Gradients: q, k, v, state.
 
         In 16-bit types a step's weight on each of the steps of its block (of 64 or 128), and the state that it meets from before, are rounded
-        to the type (the states themselves are float32); NaN or infinity at a step may reach steps of its block before it."""
+        to the type (the states themselves are float32).  In all types NaN or infinity at a step may reach steps of its block before it."""
         args = (q, k, v, log_decay, state, lengths, scale)
         out = _lib.native().decay_attention(*args)
         return _DecayAttentionFunction.apply(*args) if out is NotImplemented else out
