@@ -266,3 +266,26 @@ def test_modules_of_16_bits(t):
     head = SequenceHead(12, 24, 9, mixer="attention", heads=3, device="cuda").to(t)
     logits, _ = head(torch.randn(2, 30, 12, device="cuda", dtype=t))
     assert bool(torch.isfinite(logits).all())
+
+
+CAPTURED = """
+import torch
+import deform_conv3d_pytorch_op_b200 as dcn
+g = torch.Generator(device="cuda").manual_seed(0)
+logits = torch.randn(20, 50257, generator=g, device="cuda").bfloat16()
+uniform = torch.rand(20, generator=g, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    token, score = dcn.TokenSampleFunction.apply(logits, uniform, 0.9, 40, 0.9)
+graph.replay()
+torch.cuda.synchronize()
+want, other = dcn.TokenSampleFunction.apply(logits, uniform, 0.9, 40, 0.9)
+assert torch.equal(token, want) and torch.equal(score, other)
+print("same")
+"""
+
+
+def test_first_draw_of_a_process_is_captured():
+    """How many clusters the GPU holds is asked while a graph records"""
+    done = subprocess.run([sys.executable, "-c", CAPTURED], capture_output=True, text=True, timeout=300, cwd=Path(__file__).parent.parent)
+    assert done.returncode == 0 and "same" in done.stdout, done.stderr
